@@ -30,6 +30,7 @@ vp, u64, i32, f32p = (ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int,
                       ctypes.POINTER(ctypes.c_float))
 u64p = ctypes.POINTER(ctypes.c_uint64)
 sz = ctypes.c_size_t
+i64 = ctypes.c_int64
 
 # symbol -> (restype, argtypes); declared in include/grm_hip_router.h
 SIGNATURES = {
@@ -116,6 +117,14 @@ SIGNATURES = {
     "grm_hip_device_free": (i32, [vp]),
     "grm_hip_copy_to_host": (i32, [vp, vp, u64]),
     "grm_hip_copy_to_device": (i32, [vp, vp, u64]),
+    # the 8-bit key/value cache
+    "grm_hip_kv_work_bytes": (i32, [vp, vp]),
+    "grm_hip_kv_plan": (i32, [vp, vp]),
+    "grm_hip_kv_append": (i32, [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
+    "grm_hip_kv_attend_bytes": (i32, [vp, vp, vp]),
+    "grm_hip_kv_attend": (i32, [vp, vp, vp, i32, i64, i64, vp, i64, i64, vp, ctypes.c_float,
+                                vp, u64, vp]),
+    "grm_hip_kv_read": (i32, [vp, vp, i32, i32, vp, vp, u64, i32, vp, vp, vp]),
     "grm_hip_synth_int8_rows": (i32, [u64, u64, u64, i32, vp, i32, vp, vp]),
 }
 

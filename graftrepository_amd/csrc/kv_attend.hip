@@ -1,0 +1,232 @@
+// kv_attend.hip -- causal grouped-query attention over the 8-bit key/value
+// cache.
+//
+//   s_j = scale * (q . kc_j) * ks(j),  o = sum_j p_j vs(j) vc_j / sum_j p_j
+//
+// with p_j = exp(s_j - max s), kc and vc the int8 codes and ks, vs the
+// scales of the block that holds token j.  One pass over the cache with a
+// running maximum and sum; all sums and statistics in fp32.
+
+#include "kv_common.hpp"
+
+namespace grm {
+namespace kv {
+
+struct AttendArgs {
+  const int8_t* k_codes;
+  const int8_t* v_codes;
+  const float* k_scales;
+  const float* v_scales;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t* ctx_lens;
+  const int32_t* cu_new;
+  const int32_t* table;
+  const char* work;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  uint64_t blocks;
+  float scale;
+  int32_t requests, width, tokens, window;
+  int32_t heads, kv_heads, group, head_dim, block_log2;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Any head_dim, any number of heads: one block per (token, query head), a
+// tile of 64 keys to each of its waves in turn; a lane takes one key for
+// the scores and columns lane, lane + 64.. for the values.  Every key byte
+// is read once for each query head, so this serves what the matrix-core
+// kernels do not take.
+template <class T>
+__global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
+  const int row = blockIdx.x, h = blockIdx.y, g = h / a.group;
+  const int lane = __lane_id(), wave = threadIdx.x / kWave;
+  const int hd = a.head_dim, bs = 1 << a.block_log2;
+  __shared__ float s_q[256];
+  __shared__ float s_p[4][kTile];
+  __shared__ float s_o[4][256];
+  __shared__ float s_m[4], s_l[4];
+  if (row >= a.cu_new[a.requests]) return;
+  int lo = 0, len = a.requests;  // the last request whose first row is not past this one
+  while (len > 1) {
+    const int half = len >> 1;
+    if (a.cu_new[lo + half] <= row) lo += half;
+    len -= half;
+  }
+  const int r = lo;
+  const int pos = clamp_len(a.ctx_lens[r]) + row - a.cu_new[r];
+  const int first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+  const typename T::store* q = static_cast<const typename T::store*>(a.q) +
+                               row * a.q_token_stride + h * a.q_head_stride;
+  for (int d = threadIdx.x; d < hd; d += 256) s_q[d] = T::get(q[d]);
+  __syncthreads();
+
+  float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  bool odd = false;  // a score that is not a number
+  for (int t0 = first / kTile * kTile + wave * kTile; t0 <= pos; t0 += 4 * kTile) {
+    const int key = t0 + lane;
+    const int j = key >> a.block_log2, p = key & (bs - 1);
+    int block = -1;
+    if (key >= first && key <= pos && j < a.width) {
+      block = a.table[static_cast<size_t>(r) * a.width + j];
+      if (static_cast<uint64_t>(static_cast<int64_t>(block)) >= a.blocks) block = -1;
+    }
+    float s = -INFINITY, vs = 0.0f;
+    if (block >= 0) {
+      const size_t cell = static_cast<size_t>(block) * a.kv_heads + g;
+      const u32x4* k = reinterpret_cast<const u32x4*>(a.k_codes + (cell * bs + p) * hd);
+      float dot = 0.0f;
+      for (int c = 0; c < hd / 16; ++c) {
+        const u32x4 w = k[c];
+#pragma unroll
+        for (int b = 0; b < 16; ++b) {
+          dot = fmaf(s_q[16 * c + b], static_cast<float>(code_at(w[b / 4], b % 4)), dot);
+        }
+      }
+      s = dot * a.k_scales[cell] * a.scale;
+      vs = a.v_scales[cell];
+    }
+    odd |= s != s;
+    float top = s;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float m2 = fmaxf(m, top);
+    if (m2 == -INFINITY) continue;  // no key of this tile is seen
+    const float keep = __builtin_amdgcn_exp2f((m - m2) * kLog2e);
+    const float pr = block >= 0 ? __builtin_amdgcn_exp2f((s - m2) * kLog2e) : 0.0f;
+    m = m2;
+    float sum = pr;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    l = l * keep + sum;
+    s_p[wave][lane] = block >= 0 ? pr * vs : 0.0f;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] *= keep;
+    for (int b0 = 0; b0 < kTile; b0 += 16) {
+      // the 16 tokens lie in one block; the window may hide the first
+      const uint64_t seen = (__ballot(block >= 0) >> b0) & 0xffffull;
+      if (seen == 0) continue;
+      const int any = __shfl(block, b0 + __ffsll(static_cast<long long>(seen)) - 1);
+      const size_t cell = static_cast<size_t>(any) * a.kv_heads + g;
+      const int8_t* v = a.v_codes + cell * bs * hd + ((t0 + b0) & (bs - 1));
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int d = c * kWave + lane;
+        if (d < hd) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(v + static_cast<size_t>(d) * bs);
+#pragma unroll
+          for (int b = 0; b < 16; ++b) {
+            o[c] = fmaf(s_p[wave][b0 + b], static_cast<float>(code_at(w[b / 4], b % 4)), o[c]);
+          }
+        }
+      }
+    }
+  }
+  if (__any(odd)) l = NAN;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) s_o[wave][c * kWave + lane] = o[c];
+  if (lane == 0) {
+    s_m[wave] = m;
+    s_l[wave] = l;
+  }
+  __syncthreads();
+  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  float total = 0.0f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = s_m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((s_m[w] - top) * kLog2e);
+    total += s_l[w] != s_l[w] ? NAN : f[w] * s_l[w];
+  }
+  typename T::store* out = static_cast<typename T::store*>(a.out) + row * a.out_token_stride +
+                           h * a.out_head_stride;
+  for (int d = threadIdx.x; d < hd; d += 256) {
+    const float v = f[0] * s_o[0][d] + f[1] * s_o[1][d] + f[2] * s_o[2][d] + f[3] * s_o[3][d];
+    out[d] = T::put(total == 0.0f ? 0.0f : v / total);
+  }
+  if (a.lse && threadIdx.x == 0) {
+    a.lse[static_cast<size_t>(row) * a.heads + h] =
+        total == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(total) * kLn2;
+  }
+}
+
+}  // namespace kv
+}  // namespace grm
+
+using namespace grm::kv;
+
+extern "C" int grm_hip_kv_attend_bytes(const grm_kv_cache_desc* cache,
+                                       const grm_kv_batch_desc* batch, uint64_t* out_bytes) {
+  if (!out_bytes) return grm::fail(-1, "null output pointer");
+  GRM_CHECK_RC(check_cache(cache));
+  GRM_CHECK_RC(check_batch(batch, false));
+  *out_bytes = 0;
+  grm::clear_error();
+  return 0;
+}
+
+extern "C" int grm_hip_kv_attend(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b,
+                                 const void* q, int dtype, int64_t q_token_stride,
+                                 int64_t q_head_stride, void* out, int64_t out_token_stride,
+                                 int64_t out_head_stride, float* lse, float softmax_scale,
+                                 void* scratch, uint64_t scratch_bytes, void* stream) {
+  GRM_CHECK_RC(check_pair(c, b));
+  if (dtype != grm::kF32 && dtype != grm::kBF16 && dtype != grm::kF16) {
+    return grm::fail(-1, "queries are F32, BF16 or F16");
+  }
+  if (b->requests == 0 || b->tokens == 0) {
+    grm::clear_error();
+    return 0;
+  }
+  if (!q || !out) return grm::fail(-1, "null queries or output");
+  const int64_t unit = dtype == grm::kF32 ? 4 : 8;
+  if (!aligned16(q) || !aligned16(out) || q_token_stride % unit || q_head_stride % unit ||
+      out_token_stride % unit || out_head_stride % unit) {
+    return grm::fail(-1, "queries and output: 16-byte aligned rows");
+  }
+  if (!(softmax_scale == softmax_scale) || softmax_scale - softmax_scale != 0.0f) {
+    return grm::fail(-1, "softmax_scale must be finite");
+  }
+  (void)scratch;
+  (void)scratch_bytes;
+  Layout l;
+  GRM_CHECK_RC(layout_of(b, &l));
+  if (b->work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_kv_work_bytes");
+  AttendArgs a{};
+  a.k_codes = static_cast<const int8_t*>(c->k_codes);
+  a.v_codes = static_cast<const int8_t*>(c->v_codes);
+  a.k_scales = c->k_scales;
+  a.v_scales = c->v_scales;
+  a.q = q;
+  a.out = out;
+  a.lse = lse;
+  a.ctx_lens = b->ctx_lens;
+  a.cu_new = b->cu_new;
+  a.table = b->block_table;
+  a.work = static_cast<const char*>(b->work);
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.out_token_stride = out_token_stride;
+  a.out_head_stride = out_head_stride;
+  a.blocks = c->blocks;
+  a.scale = softmax_scale;
+  a.requests = b->requests;
+  a.width = b->table_width;
+  a.tokens = b->tokens;
+  a.window = b->window;
+  a.heads = b->heads;
+  a.kv_heads = b->kv_heads;
+  a.group = l.group;
+  a.head_dim = c->head_dim;
+  a.block_log2 = c->block_tokens == 16 ? 4 : c->block_tokens == 32 ? 5 : c->block_tokens == 64 ? 6 : 7;
+  const dim3 grid(static_cast<unsigned>(b->tokens), static_cast<unsigned>(b->heads));
+  const auto s = static_cast<hipStream_t>(stream);
+  if (dtype == grm::kF32) attend_any_kernel<F32><<<grid, 256, 0, s>>>(a);
+  else if (dtype == grm::kBF16) attend_any_kernel<BF16><<<grid, 256, 0, s>>>(a);
+  else attend_any_kernel<F16><<<grid, 256, 0, s>>>(a);
+  GRM_HIP_CHECK(hipGetLastError());
+  grm::clear_error();
+  return 0;
+}

@@ -1,0 +1,335 @@
+"""A paged key/value cache held in 8 bits, and attention over it.
+
+Routed grafts end up in the model's cache (the reference mounts them by
+surgery on a dense fp16 cache, core/graft_arena.py:2408-2622, and leaves the
+attention to its external engine).  ``KvCache`` holds keys and values as int8
+codes with one fp32 scale per (block of tokens, kv head); ``KvBatch`` is one
+step's ragged batch over it::
+
+    batch = KvBatch(ctx_lens, new_lens, block_table, 64, tokens=T, max_new=n,
+                    heads=32, kv_heads=8, free_list=free, free_head=head)
+    batch.plan()                          # once per step
+    cache.append(batch, k, v)             # per layer
+    out = cache.attend(batch, q)          # per layer
+    k, v = cache.read(table, starts, cu_rows, rows)   # dense, to harvest
+
+Arrays are device memory: torch tensors, or ``payload.DeviceArray`` (there
+bf16 is uint16 bit patterns, as everywhere in this package).  Shapes, laws
+and layouts are those of ``include/grm_hip_router.h``.  Calls are ordered on
+``stream`` (a HIP stream handle; by default torch's current stream for torch
+tensors, else the default stream) and return before the work has run; they
+can be captured into a HIP graph.  Bad arguments raise ``ValueError`` here or
+``RuntimeError`` (code -1) from the library, with nothing launched.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import sys
+
+import numpy as np
+
+from . import _lib
+from .payload import DeviceArray
+
+i32, u64, vp = ctypes.c_int32, ctypes.c_uint64, ctypes.c_void_p
+
+
+class _CacheDesc(ctypes.Structure):
+    _fields_ = [("k_codes", vp), ("v_codes", vp), ("k_scales", vp), ("v_scales", vp),
+                ("blocks", u64), ("block_tokens", i32), ("kv_heads", i32), ("head_dim", i32),
+                ("reserved", i32)]
+
+
+class _BatchDesc(ctypes.Structure):
+    _fields_ = [("ctx_lens", vp), ("new_lens", vp), ("block_table", vp), ("free_list", vp),
+                ("free_head", vp), ("free_head_out", vp), ("cu_new", vp), ("slot_map", vp),
+                ("positions", vp), ("work", vp), ("work_bytes", u64), ("requests", i32),
+                ("table_width", i32), ("tokens", i32), ("max_new", i32), ("block_tokens", i32),
+                ("heads", i32), ("kv_heads", i32), ("window", i32), ("free_count", u64)]
+
+
+_NUMPY = {"f32": np.float32, "bf16": np.uint16, "f16": np.float16, "i8": np.int8,
+          "i32": np.int32, "i64": np.int64, "u8": np.uint8}
+_NAMES = {np.dtype(v): k for k, v in _NUMPY.items()}
+_TORCH: dict[str, object] = {}
+
+
+def _torch_names() -> dict[str, object]:
+    if not _TORCH:
+        t = sys.modules["torch"]
+        pairs = {"f32": t.float32, "bf16": t.bfloat16, "f16": t.float16, "i8": t.int8,
+                 "i32": t.int32, "i64": t.int64, "u8": t.uint8}
+        _NAMES.update({v: k for k, v in pairs.items()})
+        _TORCH.update(pairs)
+    return _TORCH
+
+
+def _is_torch(a) -> bool:
+    t = sys.modules.get("torch")
+    return t is not None and isinstance(a, t.Tensor)
+
+
+def _name_of(dtype) -> str:
+    """'bf16' and the like of a name, a numpy or a torch type."""
+    if isinstance(dtype, str) and dtype in _NUMPY:
+        return dtype
+    if "torch" in sys.modules:
+        _torch_names()
+    try:
+        return _NAMES[dtype] if dtype in _NAMES else _NAMES[np.dtype(dtype)]
+    except (KeyError, TypeError):
+        raise ValueError(f"unsupported type {dtype!r}") from None
+
+
+def _type(a, what: str) -> str:
+    if _is_torch(a):
+        _torch_names()
+        if not a.is_cuda:
+            raise ValueError(f"{what} must be on the GPU")
+    elif not isinstance(a, DeviceArray):
+        raise ValueError(f"{what} must be a torch tensor on the GPU or a DeviceArray")
+    name = _NAMES.get(a.dtype)
+    if name is None:
+        raise ValueError(f"{what}: unsupported type {a.dtype}")
+    return name
+
+
+def _dense(a, what: str, dtype: str, shape) -> int:
+    """Address of a contiguous array of this type and shape (None: any)."""
+    if _type(a, what) != dtype:
+        raise ValueError(f"{what} must be {dtype}, got {a.dtype}")
+    got = tuple(a.shape)
+    if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
+        raise ValueError(f"{what} must have shape {shape}, got {got}")
+    if _is_torch(a) and not a.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return a.data_ptr()
+
+
+def _strides(a) -> tuple[int, ...]:
+    if _is_torch(a):
+        return a.stride()
+    out, step = [], 1
+    for d in reversed(a.shape):
+        out.append(step)
+        step *= d
+    return tuple(reversed(out))
+
+
+def _rows(a, what: str, shape) -> tuple[int, str, int, int]:
+    """(address, type, row stride, head stride) of [rows, heads, dim] values
+    whose last axis is contiguous."""
+    name = _type(a, what)
+    if name not in ("f32", "bf16", "f16"):
+        raise ValueError(f"{what} must be f32, bf16 or f16, got {a.dtype}")
+    if tuple(a.shape) != shape:
+        raise ValueError(f"{what} must have shape {shape}, got {tuple(a.shape)}")
+    st = _strides(a)
+    if st[2] != 1 and shape[2] > 1 and a.data_ptr():
+        raise ValueError(f"{what}: the last axis must be contiguous")
+    return a.data_ptr(), name, st[0], st[1]
+
+
+def _empty(like, shape, dtype: str):
+    if _is_torch(like):
+        return sys.modules["torch"].empty(shape, dtype=_torch_names()[dtype], device=like.device)
+    return DeviceArray(shape, _NUMPY[dtype])
+
+
+def _stream(a, stream) -> int:
+    if stream is not None:
+        return int(getattr(stream, "cuda_stream", stream))
+    if _is_torch(a):
+        return sys.modules["torch"].cuda.current_stream(a.device).cuda_stream
+    return 0
+
+
+class KvBatch:
+    """One step's ragged batch: request r holds ``ctx_lens[r]`` tokens and
+    brings ``new_lens[r]``; its tokens are rows ``cu_new[r]`` onward.
+
+    ``block_table`` int32 [requests, width]: physical block of each of a
+    request's blocks.  With ``free_list`` (int32) and ``free_head`` (int32
+    [1], entries used so far), ``plan`` takes the blocks that are missing
+    from the list, enters them in the table and leaves the new head in
+    ``free_head_out``; ``advance`` makes that the next plan's head.  Without a
+    list the table is taken as it is.
+
+    ``tokens`` is the number of rows of the step's arrays (at least the sum
+    of ``new_lens``) and ``max_new`` a bound on its entries: both fix grids
+    and buffers, so a batch object serves every step within them, with
+    ``ctx_lens``, ``new_lens`` and the table updated in place.  ``window``
+    limits a token to its last ``window`` tokens; layers with another window
+    take a second batch over the same arrays.
+    """
+
+    def __init__(self, ctx_lens, new_lens, block_table, block_tokens: int, *, tokens: int,
+                 max_new: int, heads: int, kv_heads: int, window: int = 0, free_list=None,
+                 free_head=None):
+        self._lib = _lib.load()
+        n = int(ctx_lens.shape[0])
+        d = self._desc = _BatchDesc()
+        d.ctx_lens = _dense(ctx_lens, "ctx_lens", "i32", (n,))
+        d.new_lens = _dense(new_lens, "new_lens", "i32", (n,))
+        d.block_table = _dense(block_table, "block_table", "i32", (n, None))
+        d.requests, d.table_width = n, int(block_table.shape[1])
+        d.tokens, d.max_new, d.window = int(tokens), int(max_new), int(window)
+        d.block_tokens, d.heads, d.kv_heads = int(block_tokens), int(heads), int(kv_heads)
+        need = u64()
+        _lib.check(self._lib.grm_hip_kv_work_bytes(ctypes.byref(d), ctypes.byref(need)),
+                   "kv work size")
+        self.ctx_lens, self.new_lens, self.block_table = ctx_lens, new_lens, block_table
+        self.cu_new = _empty(ctx_lens, (n + 1,), "i32")
+        self.slot_map = _empty(ctx_lens, (d.tokens,), "i64")
+        self.positions = _empty(ctx_lens, (d.tokens,), "i32")
+        self._work = _empty(ctx_lens, (need.value,), "u8")
+        d.cu_new, d.slot_map = self.cu_new.data_ptr(), self.slot_map.data_ptr()
+        d.positions, d.work = self.positions.data_ptr(), self._work.data_ptr()
+        d.work_bytes = need.value
+        self.free_list = self.free_head = self.free_head_out = None
+        if free_list is not None:
+            if free_head is None:
+                raise ValueError("a free list needs free_head")
+            d.free_list = _dense(free_list, "free_list", "i32", (None,))
+            d.free_count = int(free_list.shape[0])
+            d.free_head = _dense(free_head, "free_head", "i32", (1,))
+            self.free_list, self.free_head = free_list, free_head
+            self.free_head_out = _empty(ctx_lens, (1,), "i32")
+            d.free_head_out = self.free_head_out.data_ptr()
+        self._ref = ctypes.byref(d)
+        self._scratch: dict[int, int] = {}
+        self._held = None
+
+    def plan(self, stream=None) -> "KvBatch":
+        """Fill ``cu_new``, ``slot_map``, ``positions``, the table's new
+        entries and the schedule from the lengths as they are now."""
+        rc = self._lib.grm_hip_kv_plan(self._ref, _stream(self.ctx_lens, stream))
+        if rc:
+            _lib.check(rc, "kv plan")
+        return self
+
+    def advance(self) -> None:
+        """The next plan goes on in the free list where the last one ended."""
+        if self.free_list is None:
+            raise ValueError("the batch has no free list")
+        d = self._desc
+        self.free_head, self.free_head_out = self.free_head_out, self.free_head
+        d.free_head, d.free_head_out = d.free_head_out, d.free_head
+
+
+class KvCache:
+    """The cache of one layer, over the caller's arrays: int8 ``k_codes``
+    [blocks, kv_heads, block_tokens, head_dim] and ``v_codes`` [blocks,
+    kv_heads, head_dim, block_tokens] (transposed in its block), fp32
+    ``k_scales`` and ``v_scales`` [blocks, kv_heads].  ``KvCache.empty``
+    allocates them."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        self._lib = _lib.load()
+        if len(k_codes.shape) != 4:
+            raise ValueError("k_codes must be [blocks, kv_heads, block_tokens, head_dim]")
+        blocks, kv, bs, hd = (int(s) for s in k_codes.shape)
+        d = self._desc = _CacheDesc()
+        d.k_codes = _dense(k_codes, "k_codes", "i8", (blocks, kv, bs, hd))
+        d.v_codes = _dense(v_codes, "v_codes", "i8", (blocks, kv, hd, bs))
+        d.k_scales = _dense(k_scales, "k_scales", "f32", (blocks, kv))
+        d.v_scales = _dense(v_scales, "v_scales", "f32", (blocks, kv))
+        d.blocks, d.block_tokens, d.kv_heads, d.head_dim = blocks, bs, kv, hd
+        if bs not in (16, 32, 64, 128):
+            raise ValueError("block_tokens must be 16, 32, 64 or 128")
+        if hd % 16 or not 0 < hd <= 256:
+            raise ValueError("head_dim must be a multiple of 16, at most 256")
+        self.k_codes, self.v_codes = k_codes, v_codes
+        self.k_scales, self.v_scales = k_scales, v_scales
+        self.blocks, self.block_tokens, self.kv_heads, self.head_dim = blocks, bs, kv, hd
+        self._ref = ctypes.byref(d)
+
+    @classmethod
+    def empty(cls, blocks: int, block_tokens: int, kv_heads: int, head_dim: int) -> "KvCache":
+        """A cache in memory of its own (DeviceArrays), contents undefined:
+        every block is written before it is read."""
+        k = DeviceArray((blocks, kv_heads, block_tokens, head_dim), np.int8)
+        v = DeviceArray((blocks, kv_heads, head_dim, block_tokens), np.int8)
+        ks = DeviceArray((blocks, kv_heads), np.float32)
+        return cls(k, v, ks, DeviceArray((blocks, kv_heads), np.float32))
+
+    def append(self, batch: KvBatch, k, v, stream=None) -> None:
+        """Quantise the step's ``k`` and ``v`` [tokens, kv_heads, head_dim]
+        (f32, bf16 or f16; any row and head strides) into their blocks."""
+        shape = (batch._desc.tokens, self.kv_heads, self.head_dim)
+        kp, name, kt, kh = _rows(k, "k", shape)
+        vptr, vname, vt, vh = _rows(v, "v", shape)
+        if vname != name:
+            raise ValueError("k and v must have one type")
+        rc = self._lib.grm_hip_kv_append(self._ref, batch._ref, kp, vptr, _lib.DTYPE_CODES[name],
+                                         kt, kh, vt, vh, _stream(k, stream))
+        if rc:
+            _lib.check(rc, "kv append")
+
+    def attend(self, batch: KvBatch, q, softmax_scale: float | None = None, *, out=None,
+               lse=None, return_lse: bool = False, stream=None):
+        """Causal attention of the step's queries ``q`` [tokens, heads,
+        head_dim] over the cache, which holds the step's own tokens.  Returns
+        ``out`` (q's type; also taken as an argument), with ``return_lse``
+        also the fp32 [tokens, heads] log-sum-exp of the scores."""
+        d = batch._desc
+        shape = (d.tokens, d.heads, self.head_dim)
+        qp, name, qt, qh = _rows(q, "q", shape)
+        if out is None:
+            out = _empty(q, shape, name)
+        op, oname, ot, oh = _rows(out, "out", shape)
+        if oname != name:
+            raise ValueError("out must have q's type")
+        if lse is None and return_lse:
+            lse = _empty(q, shape[:2], "f32")
+        lp = _dense(lse, "lse", "f32", shape[:2]) if lse is not None else None
+        need = batch._scratch.get(self.head_dim)
+        if need is None:
+            got = u64()
+            _lib.check(self._lib.grm_hip_kv_attend_bytes(self._ref, batch._ref,
+                                                         ctypes.byref(got)), "kv scratch size")
+            need = batch._scratch[self.head_dim] = got.value
+        scratch = None
+        if need:
+            if _is_torch(q):
+                # from torch's pool, on the call's stream: the caller may use
+                # one batch on several streams
+                scratch = _empty(q, (need,), "u8")
+            else:
+                if batch._held is None or batch._held.nbytes < need:
+                    batch._held = DeviceArray((need,), np.uint8)
+                scratch = batch._held
+        if softmax_scale is None:
+            softmax_scale = 1.0 / math.sqrt(self.head_dim)
+        rc = self._lib.grm_hip_kv_attend(
+            self._ref, batch._ref, qp, _lib.DTYPE_CODES[name], qt, qh, op, ot, oh, lp,
+            softmax_scale, scratch.data_ptr() if scratch is not None else None, need,
+            _stream(q, stream))
+        if rc:
+            _lib.check(rc, "kv attend")
+        return (out, lse) if return_lse else out
+
+    def read(self, block_table, starts, cu_rows, rows: int, *, dtype="f16", stream=None):
+        """Dense (k, v) [rows, kv_heads, head_dim] of positions ``starts[r]``
+        onward of every request, ``cu_rows[r + 1] - cu_rows[r]`` of them;
+        ``rows`` is ``cu_rows[-1]``.  A deposit harvests a turn with it."""
+        name = _name_of(dtype)
+        if name not in ("f32", "bf16", "f16"):
+            raise ValueError("values are read as f32, bf16 or f16")
+        n = int(starts.shape[0])
+        table = _dense(block_table, "block_table", "i32", (n, None))
+        sp = _dense(starts, "starts", "i32", (n,))
+        cp = _dense(cu_rows, "cu_rows", "i32", (n + 1,))
+        shape = (int(rows), self.kv_heads, self.head_dim)
+        k, v = _empty(starts, shape, name), _empty(starts, shape, name)
+        rc = self._lib.grm_hip_kv_read(
+            self._ref, table, int(block_table.shape[1]), n, sp, cp, shape[0],
+            _lib.DTYPE_CODES[name], k.data_ptr(), v.data_ptr(), _stream(starts, stream))
+        if rc:
+            _lib.check(rc, "kv read")
+        return k, v
+
+
+__all__ = ["KvBatch", "KvCache"]

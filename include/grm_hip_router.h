@@ -480,6 +480,123 @@ int grm_hip_device_free(void* ptr);
 int grm_hip_copy_to_host(void* host, const void* device, uint64_t bytes);
 int grm_hip_copy_to_device(void* device, const void* host, uint64_t bytes);
 
+/* ---- 8-bit key/value cache ------------------------------------------------
+ * A paged cache the routed grafts are mounted into and the model attends
+ * over.  The reference mounts grafts into a dense fp16 cache by surgery
+ * (core/graft_arena.py:2408-2622) and leaves attention to its external
+ * engine; these entry points have no counterpart.
+ *
+ * Keys and values are int8 codes with one fp32 scale per (block of
+ * block_tokens tokens, kv head); a code stands for code * scale.  Arrays are
+ * the caller's device memory, contiguous:
+ *   k_codes [blocks][kv_heads][block_tokens][head_dim] int8
+ *   v_codes [blocks][kv_heads][head_dim][block_tokens] int8 (transposed in
+ *           its block: one load reads neighbouring tokens of one column)
+ *   k_scales, v_scales [blocks][kv_heads] fp32
+ * block_tokens is 16, 32, 64 or 128; head_dim a multiple of 16, at most 256.
+ * Code arrays are 16-byte aligned.
+ *
+ * A step is a ragged batch: request r holds ctx_lens[r] tokens and brings
+ * new_lens[r]; its new token i has position ctx_lens[r] + i and row
+ * cu_new[r] + i of every per-token array.  Its position p lies in block
+ * block_table[r][p / block_tokens].
+ *
+ * Unlike the rest of the library these calls are ordered on the caller's
+ * stream (a hipStream_t; NULL is the default stream): they launch and
+ * return, allocate nothing, read no device memory on the host and can be
+ * captured into a HIP graph.  Argument errors are found on the host and
+ * return -1 with nothing launched.  Every array must stay valid, and be
+ * used on that stream or ordered with it, until the work has run. */
+typedef struct grm_kv_cache_desc {
+  void* k_codes;
+  void* v_codes;
+  float* k_scales;
+  float* v_scales;
+  uint64_t blocks;
+  int32_t block_tokens;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t reserved; /* 0 */
+} grm_kv_cache_desc;
+
+typedef struct grm_kv_batch_desc {
+  const int32_t* ctx_lens; /* [requests] tokens held before the step */
+  const int32_t* new_lens; /* [requests] tokens the step brings (0 is fine) */
+  int32_t* block_table;    /* [requests][table_width]; -1: no block */
+  const int32_t* free_list;   /* [free_count] block ids */
+  const int32_t* free_head;   /* [1] entries of the list used so far; NULL:
+                                 no list, the table is taken as it is */
+  int32_t* free_head_out;     /* [1] the same after the step; not free_head */
+  int32_t* cu_new;         /* out [requests + 1] exclusive sums of new_lens */
+  int64_t* slot_map;       /* out [tokens] block * block_tokens + place, -1
+                              where there is none; may be NULL */
+  int32_t* positions;      /* out [tokens], -1 past the last; may be NULL */
+  void* work;              /* out: the step's schedule, 16-byte aligned */
+  uint64_t work_bytes;     /* at least grm_hip_kv_work_bytes */
+  int32_t requests;
+  int32_t table_width;
+  int32_t tokens;          /* rows of the per-token arrays, >= sum(new_lens) */
+  int32_t max_new;         /* no new_lens entry is larger */
+  int32_t block_tokens;
+  int32_t heads;           /* query heads, a multiple of kv_heads */
+  int32_t kv_heads;
+  int32_t window;          /* a token sees its last `window` tokens, itself
+                              included; 0: all of them */
+  uint64_t free_count;
+} grm_kv_batch_desc;
+
+/* Bytes of the schedule of a batch of this shape (host fields only). */
+int grm_hip_kv_work_bytes(const grm_kv_batch_desc* batch, uint64_t* out_bytes);
+
+/* Once per step: cu_new, slot_map, positions and the schedule that append
+ * and attend follow.  With a free list, the blocks a request lacks come from
+ * it in request order, from entry *free_head on, and are entered in
+ * block_table; past the list's end they are -1 (their tokens have slot -1,
+ * are not written by append and not seen by attend).  A request's tokens
+ * past table_width blocks have no slot either. */
+int grm_hip_kv_plan(const grm_kv_batch_desc* batch, void* stream);
+
+/* Quantise a step's keys and values into their blocks.  k, v [tokens]
+ * [kv_heads][head_dim] of dtype (F32, BF16, F16); strides in elements.  Per
+ * (block, head): a = max |new value| * fp32(1 / 127); s = max(a, scale before) if the
+ * block held tokens of the request, else a; held codes follow as
+ * rint(code * (before / s)); new codes are rint(x / s) in [-127, 127], 0
+ * where s is 0 (fp32 arithmetic, ties to even).  A value that is not finite
+ * makes s NaN, and so every row that attends to the block. */
+int grm_hip_kv_append(const grm_kv_cache_desc* cache, const grm_kv_batch_desc* batch,
+                      const void* k, const void* v, int dtype, int64_t k_token_stride,
+                      int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                      void* stream);
+
+/* Bytes of scratch one attend call needs (may be 0). */
+int grm_hip_kv_attend_bytes(const grm_kv_cache_desc* cache, const grm_kv_batch_desc* batch,
+                            uint64_t* out_bytes);
+
+/* Causal grouped-query attention of the step's tokens over the cache
+ * (which holds the step's own keys and values: append first).  q, out
+ * [tokens][heads][head_dim] of dtype (F32, BF16, F16); strides in elements,
+ * multiples of 16 bytes; head h reads kv head h / (heads / kv_heads).
+ *   s_j = softmax_scale * q . k_j,  o = sum_j softmax(s)_j v_j
+ * over the positions j a token sees (its own and earlier, within the window,
+ * in a block that is there).  lse (may be NULL) [tokens][heads] fp32
+ * receives log sum_j exp(s_j).  A token that sees nothing gets o = 0 and
+ * lse = -inf.  Rows past cu_new[requests] are not written.  Two runs on the
+ * same inputs give the same bits. */
+int grm_hip_kv_attend(const grm_kv_cache_desc* cache, const grm_kv_batch_desc* batch,
+                      const void* q, int dtype, int64_t q_token_stride, int64_t q_head_stride,
+                      void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                      float softmax_scale, void* scratch, uint64_t scratch_bytes, void* stream);
+
+/* The cache's values of positions [starts[r], starts[r] + cu_rows[r + 1] -
+ * cu_rows[r]) of each request, dense: k_out, v_out (either may be NULL)
+ * [rows][kv_heads][head_dim] of dtype, contiguous, 16-byte aligned; code *
+ * scale in fp32, rounded once.  Positions without a block read as 0.  rows
+ * is cu_rows[requests], known to the caller. */
+int grm_hip_kv_read(const grm_kv_cache_desc* cache, const int32_t* block_table,
+                    int table_width, int requests, const int32_t* starts,
+                    const int32_t* cu_rows, uint64_t rows, int dtype, void* k_out, void* v_out,
+                    void* stream);
+
 /* ---- Synthetic workload keys (host only) --------------------------------
  * Rows [row0, row0 + rows) of the synthetic INT8 key stream: each row's dim
  * values are normal quantiles (normal_table[65536], the caller's table of
