@@ -7,32 +7,11 @@
 // scales of the block that holds token j.  One pass over the cache with a
 // running maximum and sum; all sums and statistics in fp32.
 
-#include "kv_common.hpp"
+#include "kv_attend.hpp"
+#include "kv_narrow.hpp"
 
 namespace grm {
 namespace kv {
-
-struct AttendArgs {
-  const int8_t* k_codes;
-  const int8_t* v_codes;
-  const float* k_scales;
-  const float* v_scales;
-  const void* q;
-  void* out;
-  float* lse;
-  const int32_t* ctx_lens;
-  const int32_t* cu_new;
-  const int32_t* table;
-  const char* work;
-  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-  uint64_t blocks;
-  float scale;
-  int32_t requests, width, tokens, window;
-  int32_t heads, kv_heads, group, head_dim, block_log2;
-};
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // Any head_dim, any number of heads: one block per (token, query head), a
 // tile of 64 keys to each of its waves in turn; a lane takes one key for
@@ -56,6 +35,7 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
     len -= half;
   }
   const int r = lo;
+  if (static_cast<int64_t>(a.cu_new[r + 1] - a.cu_new[r]) * a.group <= a.skip_cols) return;
   const int pos = clamp_len(a.ctx_lens[r]) + row - a.cu_new[r];
   const int first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
   const typename T::store* q = static_cast<const typename T::store*>(a.q) +
@@ -152,6 +132,54 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
   }
 }
 
+// ------------------------------------------------------------- dispatch
+
+struct Shape {
+  bool narrow;        // the narrow kernel takes the requests it can
+  int blocks;         // its blocks per kv head, four runs each
+  int joins;          // blocks of its join per (kv head, column)
+  bool join_by_unit;
+  uint64_t part_floats, bytes;
+};
+
+static int shape_of(const grm_kv_cache_desc* c, const Layout& l, Shape* out) {
+  int cus = 0;
+  GRM_CHECK_RC(device_cus(&cus));
+  Shape s{};
+  const int hd = c->head_dim;
+  s.narrow = (hd == 64 || hd == 128 || hd == 256) && l.cap_units > 0;
+  // two blocks to a CU, one where a wave holds 256 columns
+  s.blocks = std::max(1, (hd == 256 ? 1 : 2) * cus / c->kv_heads);
+  s.join_by_unit = l.cap_units < static_cast<uint64_t>(4 * s.blocks - 1);
+  s.joins = s.join_by_unit ? static_cast<int>(l.cap_units) : 4 * s.blocks - 1;
+  if (s.narrow) {
+    s.bytes = static_cast<uint64_t>(c->kv_heads) * s.blocks * 8 * kNarrowCols * (hd + 2) * 4;
+  }
+  *out = s;
+  return 0;
+}
+
+template <class T, int D>
+static void launch_narrow(const AttendArgs& a, const Shape& s, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.blocks));
+  attend_narrow_kernel<T, D><<<grid, 256, 0, stream>>>(a);
+  const dim3 joins(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.joins),
+                   static_cast<unsigned>(a.cols));
+  join_narrow_kernel<T, D><<<joins, 256, 0, stream>>>(a, 4 * s.blocks, s.join_by_unit);
+}
+
+template <class T>
+static void launch(const AttendArgs& a, const Shape& s, bool all_narrow, hipStream_t stream) {
+  if (s.narrow) {
+    if (a.head_dim == 64) launch_narrow<T, 64>(a, s, stream);
+    else if (a.head_dim == 128) launch_narrow<T, 128>(a, s, stream);
+    else launch_narrow<T, 256>(a, s, stream);
+    if (all_narrow) return;
+  }
+  const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads));
+  attend_any_kernel<T><<<grid, 256, 0, stream>>>(a);
+}
+
 }  // namespace kv
 }  // namespace grm
 
@@ -162,7 +190,11 @@ extern "C" int grm_hip_kv_attend_bytes(const grm_kv_cache_desc* cache,
   if (!out_bytes) return grm::fail(-1, "null output pointer");
   GRM_CHECK_RC(check_cache(cache));
   GRM_CHECK_RC(check_batch(batch, false));
-  *out_bytes = 0;
+  Layout l;
+  GRM_CHECK_RC(layout_of(batch, &l));
+  Shape s;
+  GRM_CHECK_RC(shape_of(cache, l, &s));
+  *out_bytes = s.bytes;
   grm::clear_error();
   return 0;
 }
@@ -189,11 +221,15 @@ extern "C" int grm_hip_kv_attend(const grm_kv_cache_desc* c, const grm_kv_batch_
   if (!(softmax_scale == softmax_scale) || softmax_scale - softmax_scale != 0.0f) {
     return grm::fail(-1, "softmax_scale must be finite");
   }
-  (void)scratch;
-  (void)scratch_bytes;
   Layout l;
   GRM_CHECK_RC(layout_of(b, &l));
   if (b->work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_kv_work_bytes");
+  Shape sh;
+  GRM_CHECK_RC(shape_of(c, l, &sh));
+  if (scratch_bytes < sh.bytes || (sh.bytes && !scratch)) {
+    return grm::fail(-1, "scratch is smaller than grm_hip_kv_attend_bytes");
+  }
+  if (sh.bytes && !aligned16(scratch)) return grm::fail(-1, "scratch must be 16-byte aligned");
   AttendArgs a{};
   a.k_codes = static_cast<const int8_t*>(c->k_codes);
   a.v_codes = static_cast<const int8_t*>(c->v_codes);
@@ -221,11 +257,19 @@ extern "C" int grm_hip_kv_attend(const grm_kv_cache_desc* c, const grm_kv_batch_
   a.group = l.group;
   a.head_dim = c->head_dim;
   a.block_log2 = c->block_tokens == 16 ? 4 : c->block_tokens == 32 ? 5 : c->block_tokens == 64 ? 6 : 7;
-  const dim3 grid(static_cast<unsigned>(b->tokens), static_cast<unsigned>(b->heads));
+  a.parts = static_cast<float*>(scratch);
+  a.at_units = l.at_units;
+  a.at_tiles = l.at_tiles;
+  a.at_items = l.at_items;
+  a.at_joins = l.at_joins;
+  a.skip_cols = sh.narrow ? kNarrowCols : 0;
+  const bool all_narrow = static_cast<int64_t>(b->max_new) * l.group <= kNarrowCols;
+  a.cols = static_cast<int32_t>(
+      std::min<int64_t>(kNarrowCols, static_cast<int64_t>(std::max(1, b->max_new)) * l.group));
   const auto s = static_cast<hipStream_t>(stream);
-  if (dtype == grm::kF32) attend_any_kernel<F32><<<grid, 256, 0, s>>>(a);
-  else if (dtype == grm::kBF16) attend_any_kernel<BF16><<<grid, 256, 0, s>>>(a);
-  else attend_any_kernel<F16><<<grid, 256, 0, s>>>(a);
+  if (dtype == grm::kF32) launch<F32>(a, sh, all_narrow, s);
+  else if (dtype == grm::kBF16) launch<BF16>(a, sh, all_narrow, s);
+  else launch<F16>(a, sh, all_narrow, s);
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();
   return 0;

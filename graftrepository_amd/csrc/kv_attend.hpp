@@ -1,0 +1,151 @@
+// kv_attend.hpp -- what the attention kernels of the 8-bit key/value cache
+// share: their arguments, int8 codes to fp16, queries to fp16 terms, and the
+// last step of a row.
+#pragma once
+
+#include "kv_common.hpp"
+
+namespace grm {
+namespace kv {
+
+struct AttendArgs {
+  const int8_t* k_codes;
+  const int8_t* v_codes;
+  const float* k_scales;
+  const float* v_scales;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t* ctx_lens;
+  const int32_t* cu_new;
+  const int32_t* table;
+  const char* work;
+  float* parts;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  uint64_t blocks, at_units, at_tiles, at_items, at_joins;
+  float scale;
+  int32_t requests, width, tokens, window;
+  int32_t heads, kv_heads, group, head_dim, block_log2;
+  int32_t cols;       // columns a narrow unit may have
+  int32_t skip_cols;  // attend_any leaves out requests of at most this many columns
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Key tiles to a wavefront of the narrow kernel.
+__host__ __device__ inline int narrow_share(int tiles, int runs) {
+  const int even = (tiles + runs - 1) / runs;
+  return even > 1 ? even : 1;
+}
+
+// A run has at most two partial results: of its first unit and of its last.
+__device__ inline size_t narrow_part(int g, int runs, int run, int which) {
+  return (static_cast<size_t>(g) * runs + run) * 2 + which;
+}
+
+// Sixteen codes to fp16, exactly: a byte under the exponent of 1024 is
+// 1024 + u, and u = code + 128.
+__device__ inline void codes_to_f16(u32x4 w, f16x8 (&out)[2]) {
+  const f16x2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t u = w[k] ^ 0x80808080u;
+    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    const f16x2 a = __builtin_bit_cast(f16x2, lo) + off;
+    const f16x2 b = __builtin_bit_cast(f16x2, hi) + off;
+    const int at = 4 * (k & 1);
+    out[k >> 1][at] = a[0];
+    out[k >> 1][at + 1] = a[1];
+    out[k >> 1][at + 2] = b[0];
+    out[k >> 1][at + 3] = b[1];
+  }
+}
+
+template <class T>
+__device__ inline void load8(const typename T::store* p, float (&x)[8]) {
+  if constexpr (T::code == kF32) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+    const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = a[e];
+      x[4 + e] = b[e];
+    }
+  } else {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = T::get(static_cast<uint16_t>((w[e / 2] >> (16 * (e & 1))) & 0xffffu));
+    }
+  }
+}
+
+// Query values to fp16 terms, in units of a power of two that brings the
+// column's largest (`top`) into [1/2, 1): bf16's range is wider than fp16's,
+// and what falls below 2^-24 of the largest is below fp32's own rounding of
+// the sum.  fp16 queries are taken as they are.  Returns `scale` times the
+// unit.
+template <class T, int N, int TERMS>
+__device__ inline float split_query(const float (&x)[N][8], float top, float scale,
+                                    f16x8 (&q)[TERMS][N]) {
+  int unit = 0;
+  if constexpr (T::code != kF16) {
+    if (top > 0.0f && top <= 3.4028235e38f) unit = __builtin_amdgcn_frexp_expf(top);
+  }
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = T::code == kF16 ? x[s][e] : __builtin_amdgcn_ldexpf(x[s][e], -unit);
+      q[0][s][e] = static_cast<_Float16>(v);
+      if constexpr (TERMS == 2) {
+        q[1][s][e] = static_cast<_Float16>(v - static_cast<float>(q[0][s][e]));
+      }
+    }
+  }
+  return __builtin_amdgcn_ldexpf(scale, unit);
+}
+
+// The power of two at or above a positive finite number.
+__device__ inline float power_above(float v) {
+  // frexp: v = f 2^e with f in [1/2, 1), so 2^e > v; kept where its
+  // reciprocal is a number too
+  const int e = __builtin_amdgcn_frexp_expf(v);
+  return __builtin_amdgcn_ldexpf(1.0f, e > 127 ? 127 : e < -120 ? -120 : e);
+}
+
+// Four values of a finished row: o / l rounded once, and the row's log-sum-exp
+// by the thread of its first column.  m in log2 units, l and o biased by 2^7.
+template <class T>
+__device__ inline void finish4(const AttendArgs& a, int row, int h, int d, f32x4 o, float m,
+                               float l) {
+  const bool empty = m == -INFINITY && l == 0.0f;
+  const float inv = 1.0f / l;
+  typename T::store* out = static_cast<typename T::store*>(a.out) +
+                           static_cast<int64_t>(row) * a.out_token_stride +
+                           static_cast<int64_t>(h) * a.out_head_stride + d;
+  if constexpr (T::code == kF32) {
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = empty ? 0.0f : o[e] * inv;
+    *reinterpret_cast<f32x4*>(out) = v;
+  } else {
+    u32x2 v;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv);
+      const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv);
+      v[e] = lo | (hi << 16);
+    }
+    *reinterpret_cast<u32x2*>(out) = v;
+  }
+  if (a.lse && d == 0) {
+    a.lse[static_cast<size_t>(row) * a.heads + h] =
+        empty ? -INFINITY : (m - 7.0f + __builtin_amdgcn_logf(l)) * kLn2;
+  }
+}
+
+}  // namespace kv
+}  // namespace grm

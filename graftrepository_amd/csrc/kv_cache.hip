@@ -101,7 +101,6 @@ int layout_of(const grm_kv_batch_desc* b, Layout* out) {
   // no more than n.
   l.cap_append = std::min(rows, rows / b->block_tokens + 2 * busy);
   l.cap_units = l.group <= kNarrowCols ? busy : 0;
-  l.narrow_blocks = std::max(1, 2 * cus / b->kv_heads);
   l.wide_blocks = std::max(1, 2 * cus / b->kv_heads);
   const bool wide = static_cast<int64_t>(b->max_new) * l.group > kNarrowCols;
   l.wide_tokens = wide && l.group <= kWideCols ? kWideCols / l.group : 0;
@@ -156,7 +155,7 @@ struct PlanArgs {
   char* work;
   int32_t requests, width, tokens, window;
   int32_t free_count, group, wide_tokens, kv_heads;
-  int32_t narrow_blocks, wide_blocks, block_log2;
+  int32_t wide_blocks, block_log2;
   int32_t cap_append, cap_units, cap_items, cap_joins, cap_parts;
   uint64_t at_append, at_units, at_tiles, at_scan, at_items, at_joins;
 };
@@ -344,6 +343,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
         n.row = done[0] + v[0];
         n.tokens = max(0, min(l.fresh, a.tokens - n.row));
         n.tile_lo = lo;
+        n.ctx = l.ctx;
         units[at] = n;
         tiles[at] = done[3] + v[3];
       }
@@ -366,8 +366,6 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     head->appends = min(done[2], a.cap_append);
     head->units = done_units;
     head->narrow_tiles = done[3];
-    // at least a tile for each of a block's four waves
-    head->narrow_share = max(4, (done[3] + a.narrow_blocks - 1) / a.narrow_blocks);
     head->items = 0;
     head->joins = 0;
   }
@@ -454,7 +452,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
         it.request = r;
         it.row = ctx_row + t0;
         it.tokens = max(0, min(n, a.tokens - it.row));
-        it.first = ctx_row;
+        it.pos = clamp_len(a.ctx_lens[r]) + t0;
         it.tile_lo = min(hi, lo + i * each);
         it.tile_hi = min(hi, lo + (i + 1) * each);
         it.part = cut > 1 ? part + i : -1;
@@ -645,7 +643,6 @@ extern "C" int grm_hip_kv_plan(const grm_kv_batch_desc* b, void* stream) {
   a.group = l.group;
   a.wide_tokens = l.wide_tokens;
   a.kv_heads = b->kv_heads;
-  a.narrow_blocks = l.narrow_blocks;
   a.wide_blocks = l.wide_blocks;
   a.block_log2 = log2_of(b->block_tokens);
   a.cap_append = static_cast<int32_t>(l.cap_append);

@@ -23,10 +23,9 @@ struct SchedHead {
   int32_t appends;       // (request, block) pairs that take new tokens
   int32_t units;         // narrow units: a request whose columns fit kNarrowCols
   int32_t narrow_tiles;  // their key tiles in all
-  int32_t narrow_share;  // tiles to a block of the narrow kernel
   int32_t items;         // wide items
   int32_t joins;         // wide units cut into several items
-  int32_t pad[10];
+  int32_t pad[11];
 };
 static_assert(sizeof(SchedHead) == 64, "the lists behind it stay aligned");
 
@@ -39,14 +38,14 @@ struct AppendItem {
 // One narrow unit: all of a request's new tokens, for every kv head.
 struct NarrowUnit {
   int32_t request, row, tokens, tile_lo;
+  int32_t ctx, pad[3];
 };
 
 // One wide item: query rows [row, row + tokens) of a request against key
-// tiles [tile_lo, tile_hi); first = the request's row 0 (its position is
-// ctx_lens).  part: where the partial result goes, -1 where the item is the
-// whole unit.
+// tiles [tile_lo, tile_hi); the first of them has position `pos`.  part:
+// where the partial result goes, -1 where the item is the whole unit.
 struct WideItem {
-  int32_t request, row, tokens, first;
+  int32_t request, row, tokens, pos;
   int32_t tile_lo, tile_hi, part, pad;
 };
 
@@ -59,7 +58,6 @@ struct WideJoin {
 struct Layout {
   int group;          // query heads to a kv head
   int wide_tokens;    // tokens to a wide unit (0: no wide units)
-  int narrow_blocks;  // blocks per kv head of the narrow kernel
   int wide_blocks;    // wide blocks that run at once, per kv head
   uint64_t cap_append, cap_units, cap_items, cap_joins, cap_parts;
   uint64_t at_append, at_units, at_tiles, at_scan, at_items, at_joins, bytes;
