@@ -136,36 +136,44 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
 
 struct Shape {
   bool narrow;        // the narrow kernel takes the requests it can
-  int blocks;         // its blocks per kv head, four runs each
-  int joins;          // blocks of its join per (kv head, column)
-  bool join_by_unit;
-  uint64_t part_floats, bytes;
+  int cus;
+  uint64_t units;     // at most so many narrow units
+  int runs[2];
+  uint64_t at_runs[2];
+  uint64_t bytes;     // of scratch
 };
 
 static int shape_of(const grm_kv_cache_desc* c, const Layout& l, Shape* out) {
-  int cus = 0;
-  GRM_CHECK_RC(device_cus(&cus));
   Shape s{};
+  GRM_CHECK_RC(device_cus(&s.cus));
   const int hd = c->head_dim;
   s.narrow = (hd == 64 || hd == 128 || hd == 256) && l.cap_units > 0;
-  // two blocks to a CU, one where a wave holds 256 columns
-  s.blocks = std::max(1, (hd == 256 ? 1 : 2) * cus / c->kv_heads);
-  s.join_by_unit = l.cap_units < static_cast<uint64_t>(4 * s.blocks - 1);
-  s.joins = s.join_by_unit ? static_cast<int>(l.cap_units) : 4 * s.blocks - 1;
+  s.units = l.cap_units;
+  for (int k = 0; k < 2; ++k) {
+    s.runs[k] = l.runs[k];
+    s.at_runs[k] = l.at_runs[k];
+  }
   if (s.narrow) {
-    s.bytes = static_cast<uint64_t>(c->kv_heads) * s.blocks * 8 * kNarrowCols * (hd + 2) * 4;
+    s.bytes = static_cast<uint64_t>(c->kv_heads) * l.runs[hd == 256 ? 0 : 1] * 2 * kNarrowCols *
+              (hd + 2) * 4;
   }
   *out = s;
   return 0;
 }
 
 template <class T, int D>
-static void launch_narrow(const AttendArgs& a, const Shape& s, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.blocks));
-  attend_narrow_kernel<T, D><<<grid, 256, 0, stream>>>(a);
-  const dim3 joins(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.joins),
+static void launch_narrow(AttendArgs a, const Shape& s, hipStream_t stream) {
+  const int k = narrow_blocks_per_cu(T::code, D) - 1;
+  const int runs = s.runs[k];
+  a.at_runs = s.at_runs[k];
+  const dim3 grid(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(runs / 4));
+  if (a.block_log2 == 7) attend_narrow_kernel<T, D, 2><<<grid, 256, 0, stream>>>(a);
+  else attend_narrow_kernel<T, D, 1><<<grid, 256, 0, stream>>>(a);
+  const bool by_unit = s.units < static_cast<uint64_t>(runs - 1);
+  const dim3 joins(static_cast<unsigned>(a.kv_heads),
+                   by_unit ? static_cast<unsigned>(s.units) : static_cast<unsigned>(runs - 1),
                    static_cast<unsigned>(a.cols));
-  join_narrow_kernel<T, D><<<joins, 256, 0, stream>>>(a, 4 * s.blocks, s.join_by_unit);
+  join_narrow_kernel<T, D><<<joins, 256, 0, stream>>>(a, runs, by_unit);
 }
 
 template <class T>

@@ -22,7 +22,7 @@ struct AttendArgs {
   const char* work;
   float* parts;
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-  uint64_t blocks, at_units, at_tiles, at_items, at_joins;
+  uint64_t blocks, at_units, at_tiles, at_runs, at_items, at_joins;
   float scale;
   int32_t requests, width, tokens, window;
   int32_t heads, kv_heads, group, head_dim, block_log2;
@@ -33,10 +33,9 @@ struct AttendArgs {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Key tiles to a wavefront of the narrow kernel.
-__host__ __device__ inline int narrow_share(int tiles, int runs) {
-  const int even = (tiles + runs - 1) / runs;
-  return even > 1 ? even : 1;
+// Blocks of the narrow kernel to a CU: what its registers allow.
+__host__ __device__ constexpr int narrow_blocks_per_cu(int dtype, int head_dim) {
+  return head_dim == 256 || (dtype == kF32 && head_dim == 128) ? 1 : 2;
 }
 
 // A run has at most two partial results: of its first unit and of its last.

@@ -102,6 +102,7 @@ int layout_of(const grm_kv_batch_desc* b, Layout* out) {
   l.cap_append = std::min(rows, rows / b->block_tokens + 2 * busy);
   l.cap_units = l.group <= kNarrowCols ? busy : 0;
   l.wide_blocks = std::max(1, 2 * cus / b->kv_heads);
+  for (int k = 0; k < 2; ++k) l.runs[k] = narrow_runs(cus, b->kv_heads, k + 1);
   const bool wide = static_cast<int64_t>(b->max_new) * l.group > kNarrowCols;
   l.wide_tokens = wide && l.group <= kWideCols ? kWideCols / l.group : 0;
   if (l.wide_tokens) {
@@ -121,6 +122,9 @@ int layout_of(const grm_kv_batch_desc* b, Layout* out) {
   l.at_append = place(l.cap_append * sizeof(AppendItem));
   l.at_units = place(l.cap_units * sizeof(NarrowUnit));
   l.at_tiles = place((l.cap_units + 1) * 4);
+  for (int k = 0; k < 2; ++k) {
+    l.at_runs[k] = place(l.cap_units ? l.runs[k] * sizeof(NarrowRun) : 0);
+  }
   l.at_scan = place(l.wide_tokens ? (reqs + 1) * 4 : 0);
   l.at_items = place(l.cap_items * sizeof(WideItem));
   l.at_joins = place(l.cap_joins * sizeof(WideJoin));
@@ -157,7 +161,8 @@ struct PlanArgs {
   int32_t free_count, group, wide_tokens, kv_heads;
   int32_t wide_blocks, block_log2;
   int32_t cap_append, cap_units, cap_items, cap_joins, cap_parts;
-  uint64_t at_append, at_units, at_tiles, at_scan, at_items, at_joins;
+  int32_t runs[2];
+  uint64_t at_append, at_units, at_tiles, at_runs[2], at_scan, at_items, at_joins;
 };
 
 // Exclusive sums over the block of N values per thread; totals to `sum`.
@@ -223,12 +228,14 @@ __device__ inline int upper(const int* pre, int n, int x) {
   return lo;
 }
 
-// Key tiles [lo, hi) that query tokens [t0, t0 + n) of a request see.
-__device__ inline void tiles_of(const PlanArgs& a, int ctx, int t0, int n, int* lo, int* hi) {
+// Key tiles [lo, hi) of `tile` tokens that query tokens [t0, t0 + n) of a
+// request see.
+__device__ inline void tiles_of(const PlanArgs& a, int tile, int ctx, int t0, int n, int* lo,
+                                int* hi) {
   const int last = ctx + t0 + n;  // keys before this are seen by the last token
   const int first = a.window > 0 ? max(0, ctx + t0 + 1 - a.window) : 0;
-  *lo = first / kTile;
-  *hi = (last + kTile - 1) / kTile;
+  *lo = first / tile;
+  *hi = (last + tile - 1) / tile;
 }
 
 __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
@@ -312,8 +319,10 @@ __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
   }
 }
 
+constexpr int kScanInts = 5 * 16 + 16;
+
 __device__ void plan_schedule(const PlanArgs& a, int* lds) {
-  int* scratch = lds;  // [5 * 16] and, after it, the candidates' counts
+  int* scratch = lds;  // [5 * 16] and, after it, the candidates' counts: kScanInts
   SchedHead* head = reinterpret_cast<SchedHead*>(a.work);
   NarrowUnit* units = reinterpret_cast<NarrowUnit*>(a.work + a.at_units);
   int* tiles = reinterpret_cast<int*>(a.work + a.at_tiles);
@@ -326,7 +335,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     const bool narrow =
         l.fresh > 0 && static_cast<int64_t>(l.fresh) * a.group <= kNarrowCols && a.cap_units > 0;
     int lo = 0, hi = 0;
-    if (narrow) tiles_of(a, l.ctx, 0, l.fresh, &lo, &hi);
+    if (narrow) tiles_of(a, narrow_tile(1 << a.block_log2), l.ctx, 0, l.fresh, &lo, &hi);
     const int wide = a.wide_tokens && l.fresh > 0 && !narrow
                          ? (l.fresh + a.wide_tokens - 1) / a.wide_tokens : 0;
     int v[5] = {l.fresh, l.need, l.touched, hi - lo, wide}, sum[5];
@@ -369,8 +378,47 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     head->items = 0;
     head->joins = 0;
   }
+  __syncthreads();  // the lists are read back by other threads of this block
+
+  // Where the narrow kernel's wavefronts begin; without units every run is
+  // empty.
+  if (a.cap_units > 0) {
+    int* cached = lds + kScanInts;
+    const bool fits = done_units < kPlanChunk;
+    if (fits) {
+      for (int u = threadIdx.x; u <= done_units; u += kPlanThreads) cached[u] = tiles[u];
+      __syncthreads();
+    }
+    const int* from = fits ? cached : tiles;
+    for (int k = 0; k < 2; ++k) {
+      NarrowRun* runs = reinterpret_cast<NarrowRun*>(a.work + a.at_runs[k]);
+      for (int r = threadIdx.x; r < a.runs[k]; r += kPlanThreads) {
+        NarrowRun n;
+        n.begin = run_begin(done[3], a.runs[k], r);
+        n.stop = run_begin(done[3], a.runs[k], r + 1);
+        n.block_begin = run_begin(done[3], a.runs[k], r / 4 * 4);
+        n.block_stop = run_begin(done[3], a.runs[k], r / 4 * 4 + 4);
+        NarrowUnit u{};
+        n.at = n.first = n.end = 0;
+        if (n.begin < n.stop) {
+          n.at = upper(from, done_units, n.begin);
+          n.first = from[n.at];
+          n.end = from[n.at + 1];
+          u = units[n.at];
+        }
+        n.request = u.request;
+        n.row = u.row;
+        n.tokens = u.tokens;
+        n.tile_lo = u.tile_lo;
+        n.ctx = u.ctx;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n.pad[e] = 0;
+        runs[r] = n;
+      }
+    }
+  }
   if (wide_units == 0) return;
-  __syncthreads();  // wide_at is read back by other threads of this block
+  __syncthreads();
 
   // Longest share C of a wide item.  More blocks than units: units are cut.
   // Candidates are the even share over k = 1..4; the estimate of each is
@@ -386,7 +434,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     *t0 = (u - wide_at[*r]) * a.wide_tokens;
     const int ctx = clamp_len(a.ctx_lens[*r]);
     *n = min(a.wide_tokens, clamp_len(a.new_lens[*r]) - *t0);
-    tiles_of(a, ctx, *t0, *n, lo, hi);
+    tiles_of(a, kTile, ctx, *t0, *n, lo, hi);
   };
   int mine = 0, longest = 0;
   for (int u = threadIdx.x; u < wide_units; u += kPlanThreads) {
@@ -653,6 +701,10 @@ extern "C" int grm_hip_kv_plan(const grm_kv_batch_desc* b, void* stream) {
   a.at_append = l.at_append;
   a.at_units = l.at_units;
   a.at_tiles = l.at_tiles;
+  for (int k = 0; k < 2; ++k) {
+    a.runs[k] = l.runs[k];
+    a.at_runs[k] = l.at_runs[k];
+  }
   a.at_scan = l.at_scan;
   a.at_items = l.at_items;
   a.at_joins = l.at_joins;

@@ -11,7 +11,7 @@
 namespace grm {
 namespace kv {
 
-constexpr int kTile = 64;         // key tokens to an attention tile
+constexpr int kTile = 64;         // key tokens to a tile of the wide kernel
 constexpr int kNarrowCols = 16;   // (token, head) columns of a narrow unit
 constexpr int kWideCols = 128;    // and of a wide one
 // A length read from the device is cut to this: two of them and a block fit
@@ -41,6 +41,43 @@ struct NarrowUnit {
   int32_t ctx, pad[3];
 };
 
+// Where a wavefront of the narrow kernel begins: its run [begin, stop) of all
+// narrow tiles in order, its block's [block_begin, block_stop), and the unit
+// of the first tile (index, its tiles [first, end), the unit itself).
+struct NarrowRun {
+  int32_t begin, stop, block_begin, block_stop;
+  int32_t at, first, end, request;
+  int32_t row, tokens, tile_lo, ctx;
+  int32_t pad[4];
+};
+static_assert(sizeof(NarrowRun) == 64, "one line");
+
+// Key tokens to a tile of the narrow kernel: both halves of a 128-token
+// block's value lines, else the least that fills its loads.
+__host__ __device__ constexpr int narrow_tile(int block_tokens) {
+  return block_tokens == 128 ? 128 : 64;
+}
+
+// Runs of the narrow kernel to a kv head, with `per_cu` blocks of four to a CU.
+inline int narrow_runs(int cus, int kv_heads, int per_cu) {
+  return 4 * std::max(1, per_cu * cus / kv_heads);
+}
+
+// First tile of run r of `runs`, `tiles` in all; equal to within one.
+__host__ __device__ inline int run_begin(int tiles, int runs, int r) {
+  const int used = runs < tiles ? runs : tiles;
+  if (r >= used) return tiles;
+  return static_cast<int>(static_cast<uint64_t>(tiles) * static_cast<uint32_t>(r) /
+                          static_cast<uint32_t>(used));
+}
+
+// The run that tile t lies in.
+__device__ inline int run_of(int tiles, int runs, int t) {
+  const int used = runs < tiles ? runs : tiles;
+  return static_cast<int>((static_cast<uint64_t>(t + 1) * static_cast<uint32_t>(used) - 1) /
+                          static_cast<uint32_t>(tiles));
+}
+
 // One wide item: query rows [row, row + tokens) of a request against key
 // tiles [tile_lo, tile_hi); the first of them has position `pos`.  part:
 // where the partial result goes, -1 where the item is the whole unit.
@@ -60,7 +97,8 @@ struct Layout {
   int wide_tokens;    // tokens to a wide unit (0: no wide units)
   int wide_blocks;    // wide blocks that run at once, per kv head
   uint64_t cap_append, cap_units, cap_items, cap_joins, cap_parts;
-  uint64_t at_append, at_units, at_tiles, at_scan, at_items, at_joins, bytes;
+  int runs[2];        // of the narrow kernel, with one and two blocks to a CU
+  uint64_t at_append, at_units, at_tiles, at_runs[2], at_scan, at_items, at_joins, bytes;
 };
 
 int device_cus(int* out);

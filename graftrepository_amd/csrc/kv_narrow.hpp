@@ -4,27 +4,30 @@
 // The work is one pass over the request's codes, so it is cut by bytes: the
 // key tiles (64 tokens) of all requests, in order, are dealt to the
 // wavefronts of a kv head in equal runs, whatever request they belong to.  A
-// wavefront streams its run without a pause: while one tile is computed the
-// next one's codes are in flight (each register is loaded again as soon as
-// it is used up) and the block ids of the one after, across request
-// boundaries too.  Of a run at most the first and the last request are
-// shared with a neighbour; their partial results (maximum, sum, unnormalised
-// output) go to scratch, and the join kernel adds them in order.  Where the
-// four runs of a block lie in one request, the block adds them itself.
+// wavefront streams its run across request boundaries: the codes of the next
+// half tile are in flight while one is computed (each register is loaded
+// again as soon as it is used up), and the block ids and scales of the next
+// tile.  Of a run at most the first and the last request are shared with a
+// neighbour; their partial results (maximum, sum, unnormalised output) go to
+// scratch, and the join kernel adds them in order.  Where the four runs of a
+// block lie in one request, the block adds them itself.  The plan leaves a
+// record of where each run begins, so a wave is two loads from its codes.
 //
 // Inside a tile both products run on the matrix cores in fp16, where an int8
 // code is exact (16x16x32; rows: 16 keys or 16 value columns, columns: the
 // queries):
 //   S^T = K Q^T: lane (i, G) = (lane % 16, lane / 16) loads 16 bytes of one
-//     key: code row 16 (i / 4) + 4 t + i % 4 of the tile for row tile t, so
-//     that results 4 t + j of the lane belong to keys 16 G + 4 t + j: each
-//     lane ends up with 16 neighbouring keys of column i;
+//     key: of half h of the tile, code row 16 (i / 4) + 4 t + i % 4 for row
+//     tile t, so that results 4 t + j of the lane belong to the half's keys
+//     16 G + 4 t + j: each lane ends up with 16 neighbouring keys of column i;
 //   O^T = V^T P^T: those 16 are the lane's part of the B operand as they
 //     are, and the A operand is 16 neighbouring tokens of one value column,
 //     one 16-byte load of the transposed value codes.
-// Nothing crosses lanes until the end, and nothing goes through LDS.  The 16
+// Nothing crosses lanes and nothing goes through LDS until the end.  The 16
 // keys lie in one block of the cache, so a lane has one key scale and one
-// value scale per tile.
+// value scale.  With 128-token blocks a tile is two such halves, and the two
+// halves of a value column, one 128-byte line, are read together (tiles of 64
+// tokens fetched 1.4 times the bytes there).
 //
 // Probabilities enter the second product as fp16(2^7 p vs / v), with v a
 // power of two no less than any value scale the column has met: they stay
@@ -32,22 +35,33 @@
 // running maximum follows only when a score passes it by more than 8
 // (log2 units); until then nothing is rescaled.
 //
-// For fp32 and fp16 outputs the probabilities are two fp16 terms: the second
-// is what the first leaves, scaled and summed apart (one term alone is off by
-// 2.4e-4 of a flat row, more than the rounding to fp16).  For fp16 it is
-// scaled by 2^11, which keeps it below 2^15.  For fp32 the scale is 2^19 and
-// the maximum follows at once, so both terms stay below 2^15 and reach 2^-51
-// of the largest; fp32 queries are two terms too.
+// For fp16 and fp32 outputs the probabilities are two fp16 terms, the second
+// what the first leaves (one term alone is off by 2.4e-4 of a flat row, more
+// than the rounding to fp16).  For fp16 both are summed in one place; the
+// second is exact to 2^-25, 2^-32 of the largest probability.  For fp32 the
+// second is scaled by 2^19 and summed apart, and the maximum follows at once,
+// so that both stay below 2^15 and reach 2^-51 of the largest; fp32 queries
+// are two terms too.
 #pragma once
 
 #include "kv_attend.hpp"
 
+#include <type_traits>
+
 namespace grm {
 namespace kv {
 
+// What the plan wrote, as memory that no kernel running beside this one
+// changes: scalar loads where the address is uniform.
+typedef const __attribute__((address_space(4))) SchedHead* ConstHead;
+typedef const __attribute__((address_space(4))) NarrowUnit* ConstUnit;
+typedef const __attribute__((address_space(4))) NarrowRun* ConstRun;
+typedef const __attribute__((address_space(4))) int32_t* ConstInt;
+
 // The last unit whose first tile is not past t (wave-uniform; first tiles
 // ascend).  64 entries a step.
-__device__ inline int find_unit(const int32_t* first, int n, int t) {
+template <class P>
+__device__ inline int find_unit(P first, int n, int t) {
   const int lane = __lane_id();
   int lo = 0;
   while (true) {
@@ -61,19 +75,29 @@ __device__ inline int find_unit(const int32_t* first, int n, int t) {
   }
 }
 
+// The kernel's arguments, read again where they are used: kept in scalar
+// registers through the loop, those of a unit's begin and end would push out
+// the loop's own.
+__device__ __forceinline__ const AttendArgs& late_args() {
+  typedef const __attribute__((address_space(4))) AttendArgs* ConstArgs;
+  uintptr_t p = reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return *(const AttendArgs*)(ConstArgs)p;
+}
+
 constexpr float kWeightBias = 7.0f;
 
 // Everything one wave carries for one unit.
 template <class T, int D>
 struct NarrowState {
   static constexpr int kTerms = T::code == kF32 ? 2 : 1;        // of a query
-  static constexpr bool kRest = T::code != kBF16;               // of a probability
-  static constexpr float kRestScale = T::code == kF32 ? 524288.0f : 2048.0f;
+  static constexpr bool kRest = T::code != kBF16;               // of a probability: two
+  static constexpr bool kApart = T::code == kF32;               // and summed apart
+  static constexpr float kRestScale = kApart ? 524288.0f : 1.0f;
   static constexpr float kRescale = T::code == kF32 ? 0.0f : 8.0f;
-  f16x8 q[kTerms][D / 32];
   float col_scale;  // softmax scale, log2 e and the query's own power of two
   f32x4 o[D / 16];
-  f32x4 rest[kRest ? D / 16 : 1];
+  f32x4 rest[kApart ? D / 16 : 1];
   float m, l;       // running maximum and this lane's sum of 2^(s - m + 7)
   float v_ref, v_inv;
 };
@@ -85,7 +109,7 @@ struct UnitView {
 
 template <class T, int D>
 __device__ inline void narrow_query(const AttendArgs& a, const UnitView& u, int g,
-                                    NarrowState<T, D>& st) {
+                                    NarrowState<T, D>& st, f16x8* s_q) {
   const int lane = __lane_id(), i = lane & 15, G = lane >> 4;
   const bool mine = i < u.tokens * a.group;
   const int t = mine ? i / a.group : 0, h = mine ? i % a.group : 0;
@@ -105,95 +129,129 @@ __device__ inline void narrow_query(const AttendArgs& a, const UnitView& u, int 
   }
   top = fmaxf(top, __shfl_xor(top, 16));
   top = fmaxf(top, __shfl_xor(top, 32));
-  st.col_scale = split_query<T, D / 32>(x, top, a.scale * kLog2e, st.q);
+  f16x8 f[NarrowState<T, D>::kTerms][D / 32];
+  st.col_scale = split_query<T, D / 32>(x, top, a.scale * kLog2e, f);
+#pragma unroll
+  for (int e = 0; e < NarrowState<T, D>::kTerms; ++e) {
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) s_q[(e * (D / 32) + s) * kWave + lane] = f[e][s];
+  }
 }
 
-template <class T, int D>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void attend_narrow_kernel(AttendArgs a) {
+template <class T, int D, int H>
+__global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_narrow_kernel(AttendArgs a) {
   typedef NarrowState<T, D> State;
-  constexpr int kPieces = D / 64;   // 64-byte pieces of a key
+  constexpr int kPieces = D / 64;  // 64-byte pieces of a key
   constexpr int kValueTiles = D / 16;
+  constexpr int kHeld = (T::code == kF32 && D == 256 ? 4 : kValueTiles) / H;
+  constexpr int kNarrowTile = 64 * H;
   const int g = blockIdx.x;
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int i = lane & 15, G = lane >> 4;
-  const SchedHead* head = reinterpret_cast<const SchedHead*>(a.work);
-  const NarrowUnit* units = reinterpret_cast<const NarrowUnit*>(a.work + a.at_units);
-  const int32_t* first = reinterpret_cast<const int32_t*>(a.work + a.at_tiles);
-  const int total = __builtin_amdgcn_readfirstlane(head->narrow_tiles);
-  const int n_units = __builtin_amdgcn_readfirstlane(head->units);
-  const int share = narrow_share(total, 4 * gridDim.y);
-  const int run = 4 * blockIdx.y + wave;
-  const int block_begin = 4 * blockIdx.y * share;
-  if (block_begin >= total) return;
-  const int block_end = min(total, block_begin + 4 * share);
-  const int begin = min(total, run * share), end = min(total, begin + share);
+  const int i = lane & 15, G = lane >> 4, Gk = (lane & 15) >> 2;
+  const auto* units = reinterpret_cast<ConstUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_units);
+  const auto* first = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) + a.at_tiles);
+  const auto* table = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.table));
+  const int run = 4 * blockIdx.y + wave, runs = 4 * gridDim.y;
+  const auto* mine_at =
+      reinterpret_cast<ConstRun>(reinterpret_cast<uintptr_t>(a.work) + a.at_runs) + run;
+  const int begin = mine_at->begin, end = mine_at->stop;
+  const int block_begin = mine_at->block_begin, block_end = mine_at->block_stop;
+  if (block_begin >= block_end) return;
   const int bs = 1 << a.block_log2;
-  const size_t cell_bytes = static_cast<size_t>(bs) * D;
+  const uint32_t cell_bytes = static_cast<uint32_t>(bs * D);
+  // a lane's column's token, and its part of a load's address
+  const int col_token = i / a.group;
+  const int8_t* k_lane = a.k_codes + (((16 * Gk) & (bs - 1)) + (i & 3)) * D + 16 * G;
+  const int8_t* v_lane = a.v_codes + static_cast<size_t>(i) * bs + ((16 * G) & (bs - 1));
 
   auto unit_at = [&](int at) {
-    const NarrowUnit u = units[at];
     UnitView v;
     v.at = at;
-    v.first = __builtin_amdgcn_readfirstlane(first[at]);
-    v.end = __builtin_amdgcn_readfirstlane(first[at + 1]);
-    v.request = __builtin_amdgcn_readfirstlane(u.request);
-    v.row = __builtin_amdgcn_readfirstlane(u.row);
-    v.tokens = __builtin_amdgcn_readfirstlane(u.tokens);
-    v.tile_lo = __builtin_amdgcn_readfirstlane(u.tile_lo);
-    v.ctx = __builtin_amdgcn_readfirstlane(u.ctx);
+    v.first = first[at];
+    v.end = first[at + 1];
+    v.request = units[at].request;
+    v.row = units[at].row;
+    v.tokens = units[at].tokens;
+    v.tile_lo = units[at].tile_lo;
+    v.ctx = units[at].ctx;
     return v;
   };
 
-  u32x4 kr[4][kPieces], vr[kValueTiles];
-  float ks = 0.0f, vs = 0.0f;
-  // Block of the 16 keys from `key` on; -1 where no column sees any of them.
-  auto block_of = [&](const UnitView& u, int key) {
+  // Half a tile: where a lane's keys and values are.  `Asked` holds the
+  // table's entries for its four groups of 16 keys on their way.
+  struct Asked {
+    int id[4], seen;
+  };
+  struct Half {
+    bool all, here;  // every group has a block that some column sees; this lane's has
+    const int8_t* k;
+    const int8_t* v;
+    uint32_t cell;
+  };
+  auto ask_half = [&](const UnitView& u, int key0) {
     const int last_pos = u.ctx + u.tokens - 1;
     const int first_seen = a.window > 0 ? max(0, u.ctx + 1 - a.window) : 0;
-    const int j = key >> a.block_log2;
-    int b = -1;
-    if (key <= last_pos && key + 15 >= first_seen && j < a.width) {
-      b = a.table[static_cast<size_t>(u.request) * a.width + j];
-    }
-    return static_cast<uint64_t>(static_cast<int64_t>(b)) < a.blocks ? b : -1;
-  };
-  auto load_k = [&](int tile, int kb) {
-    const int key = tile * kTile + 16 * (i >> 2);
-    const int8_t* k = a.k_codes +
-                      (static_cast<size_t>(kb < 0 ? 0 : kb) * a.kv_heads + g) * cell_bytes +
-                      ((key & (bs - 1)) + (i & 3)) * D + 16 * G;
+    const size_t row = static_cast<size_t>(u.request) * a.width;
+    Asked r;
+    r.seen = 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int k = 0; k < 4; ++k) {
+      const int key = key0 + 16 * k, at = key >> a.block_log2;
+      if (key <= last_pos && key + 15 >= first_seen && at < a.width) r.seen |= 1 << k;
+      r.id[k] = table[row + max(0, min(at, a.width - 1))];
+    }
+    return r;
+  };
+  auto take = [&](const Asked& r, int h) {
+    Half t;
+    int id[4], ok = 0;
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p) {
-        kr[r][p] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4*>(k + 4 * r * D + 64 * p));
-      }
+    for (int k = 0; k < 4; ++k) {
+      const bool there = (r.seen >> k & 1) && static_cast<uint32_t>(r.id[k]) < a.blocks;
+      id[k] = there ? r.id[k] : 0;  // no block: any one, what it gives is not used
+      ok |= there ? 1 << k : 0;
+    }
+    auto cell_of = [&](int k) {
+      const int lo = k & 1 ? id[1] : id[0], hi = k & 1 ? id[3] : id[2];
+      return static_cast<uint32_t>(k & 2 ? hi : lo) * a.kv_heads + g;
+    };
+    t.all = ok == 15;
+    t.here = ok >> G & 1;
+    t.cell = cell_of(G);
+    const int place = 64 * h & (bs - 1);  // the second half of a 128-token block
+    t.k = k_lane + place * D + static_cast<uint64_t>(cell_of(Gk)) * cell_bytes;
+    t.v = v_lane + place + static_cast<uint64_t>(t.cell) * cell_bytes;
+    return t;
+  };
+
+  // Keys: four row tiles held, eight to a tile.  Values: half of the tile's
+  // columns held, both halves of the tokens.
+  u32x4 kr[4][kPieces], vr[kHeld][H];
+  auto load_keys = [&](const Half& t, int r) {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      kr[r][p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(t.k + 4 * r * D + 64 * p));
     }
   };
-  auto load_v = [&](int tile, int vb) {
-    const int key = tile * kTile + 16 * G;
-    const int8_t* v = a.v_codes +
-                      (static_cast<size_t>(vb < 0 ? 0 : vb) * a.kv_heads + g) * cell_bytes +
-                      static_cast<size_t>(i) * bs + (key & (bs - 1));
+  auto load_values = [&](const Half (&t)[H], int d) {
 #pragma unroll
-    for (int d = 0; d < kValueTiles; ++d) {
-      vr[d] = __builtin_nontemporal_load(
-          reinterpret_cast<const u32x4*>(v + static_cast<size_t>(16 * d) * bs));
+    for (int h = 0; h < H; ++h) {
+      vr[d % kHeld][h] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x4*>(t[h].v + static_cast<size_t>(16 * d) * bs));
     }
   };
-  auto load_scales = [&](int vb) {
-    const size_t cell = static_cast<size_t>(vb < 0 ? 0 : vb) * a.kv_heads + g;
-    ks = vb < 0 ? 0.0f : a.k_scales[cell];
-    vs = vb < 0 ? 0.0f : a.v_scales[cell];
-  };
+
+  // The unit's queries, as the lane's part of the B operands: in LDS, so that
+  // they take registers during the first product only.
+  __shared__ f16x8 s_queries[4][State::kTerms * (D / 32)][kWave];
+  f16x8* s_q = &s_queries[wave][0][0];
 
   State st;
   auto reset = [&]() {
 #pragma unroll
     for (int d = 0; d < kValueTiles; ++d) {
       st.o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (State::kRest) st.rest[d] = st.o[d];
+      if constexpr (State::kApart) st.rest[d] = st.o[d];
     }
     st.m = -INFINITY;
     st.l = 0.0f;
@@ -206,101 +264,143 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void attend_narrow_kernel(Att
   UnitView now{};
   bool spans = false;
   if (begin < end) {
-    now = unit_at(find_unit(first, n_units, begin));
+    now = {mine_at->at,  mine_at->first,  mine_at->end,     mine_at->request,
+           mine_at->row, mine_at->tokens, mine_at->tile_lo, mine_at->ctx};
     spans = now.first <= block_begin && now.end >= block_end;
-    UnitView next = now;  // the unit of tile x + 1
-    int vb = -1, kb1 = -1, vb1 = -1;
+    UnitView ahead = now;  // the unit of the tile whose blocks were asked for last
+    Half cur[H], nxt[H];
+    float ks[H], vs[H];
     {
-      const int tile = now.tile_lo + begin - now.first;
-      const int kb = block_of(now, tile * kTile + 16 * (i >> 2));
-      vb = block_of(now, tile * kTile + 16 * G);
-      load_k(tile, kb);
-      load_scales(vb);
-      load_v(tile, vb);
-      if (begin + 1 < end) {
-        if (begin + 1 >= next.end) next = unit_at(next.at + 1);
-        const int tile1 = next.tile_lo + begin + 1 - next.first;
-        kb1 = block_of(next, tile1 * kTile + 16 * (i >> 2));
-        vb1 = block_of(next, tile1 * kTile + 16 * G);
-      }
-    }
-    narrow_query<T, D>(a, now, g, st);
-    for (int x = begin; x < end; ++x) {
-      const int tile = now.tile_lo + x - now.first;
-      const bool more = x + 1 < end;
-      const int tile1 = next.tile_lo + x + 1 - next.first;
-      // the block ids of the tile after the next one
-      UnitView after = next;
-      int kb2 = -1, vb2 = -1;
-      if (x + 2 < end) {
-        if (x + 2 >= after.end) after = unit_at(after.at + 1);
-        const int tile2 = after.tile_lo + x + 2 - after.first;
-        kb2 = block_of(after, tile2 * kTile + 16 * (i >> 2));
-        vb2 = block_of(after, tile2 * kTile + 16 * G);
-      }
-      const int cols = now.tokens * a.group;
-      const int pos = now.ctx + (i < cols ? i / a.group : 0);
-      const int seen = a.window > 0 ? max(0, pos + 1 - a.window) : 0;  // first key it sees
-      const int all_from = a.window > 0 ? max(0, now.ctx + now.tokens - a.window) : 0;
-
-      // scores of keys 16 G + 4 r + j
-      f32x4 s[4];
+      const int key = (now.tile_lo + begin - now.first) * kNarrowTile;
+      Asked asked[H];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int h = 0; h < H; ++h) asked[h] = ask_half(now, key + 64 * h);
+#pragma unroll
+      for (int h = 0; h < H; ++h) cur[h] = take(asked[h], h);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_keys(cur[0], r);
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        ks[h] = a.k_scales[cur[h].cell];
+        vs[h] = a.v_scales[cur[h].cell];
+      }
+#pragma unroll
+      for (int d = 0; d < kHeld; ++d) load_values(cur, d);
+    }
+    narrow_query<T, D>(late_args(), now, g, st, s_q);
+
+    // Tile x of the run; MORE: another one follows.
+    auto step = [&](int x, auto more_follow) {
+      constexpr bool kMore = decltype(more_follow)::value;
+      const int key0 = (now.tile_lo + x - now.first) * kNarrowTile;
+      Asked asked[H];
+      if constexpr (kMore) {
+        if (x + 1 >= ahead.end) ahead = unit_at(ahead.at + 1);
+        const int key = (ahead.tile_lo + x + 1 - ahead.first) * kNarrowTile;
+#pragma unroll
+        for (int h = 0; h < H; ++h) asked[h] = ask_half(ahead, key + 64 * h);
+      }
+      // products of the halves' keys 16 G + 4 r + j
+      f32x4 s[H][4];
+      f16x8 q[State::kTerms][D / 32];
+#pragma unroll
+      for (int e = 0; e < State::kTerms; ++e) {
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) q[e][k] = s_q[(e * (D / 32) + k) * kWave + lane];
+      }
+      auto multiply = [&](int h, int r) {
+        s[h][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
           f16x8 c[2];
           codes_to_f16(kr[r][p], c);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int k = 0; k < 2; ++k) {
 #pragma unroll
             for (int e = 0; e < State::kTerms; ++e) {
-              s[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h], st.q[e][2 * p + h], s[r], 0, 0, 0);
+              s[h][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[k], q[e][2 * p + k], s[h][r], 0, 0, 0);
             }
           }
         }
-      }
-      const float kscale = ks * st.col_scale, vscale = vs;
-      if (more) {
-        load_k(tile1, kb1);
-        load_scales(vb1);
-      }
-      const int key = tile * kTile + 16 * G;
-      const bool whole = tile * kTile >= all_from && tile * kTile + kTile - 1 <= now.ctx &&
-                         __all(vb >= 0);
-      float top = -INFINITY, v_top = 0.0f;
-      if (whole) {
+      };
+      if constexpr (H == 2) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[r][j] *= kscale;
-            top = fmaxf(top, s[r][j]);
-          }
+          multiply(0, r);
+          load_keys(cur[H - 1], r);
         }
-        v_top = vscale;
+      }
+      float kscale[H], vscale[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        kscale[h] = cur[h].here ? ks[h] * st.col_scale : 0.0f;
+        vscale[h] = cur[h].here ? vs[h] : 0.0f;
+      }
+      if constexpr (kMore) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          nxt[h] = take(asked[h], h);
+          ks[h] = a.k_scales[nxt[h].cell];
+          vs[h] = a.v_scales[nxt[h].cell];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        multiply(H - 1, r);
+        if constexpr (kMore) load_keys(nxt[0], r);
+      }
+
+      const int all_from = a.window > 0 ? max(0, now.ctx + now.tokens - a.window) : 0;
+      const bool whole =
+          key0 >= all_from && key0 + kNarrowTile - 1 <= now.ctx && cur[0].all && cur[H - 1].all;
+      // Scaling by what is not negative keeps the order, so the whole tile's
+      // maximum is taken before it.  A partly seen tile is scaled first, and
+      // what a column does not see is -inf.
+      float top[H], v_top[H], mul[H];
+      if (whole && __all(!(kscale[0] < 0.0f || kscale[H - 1] < 0.0f))) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          top[h] = s[h][0][0];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top[h] = fmaxf(top[h], s[h][r][j]);
+          }
+          top[h] *= kscale[h];
+          v_top[h] = vscale[h];
+          mul[h] = kscale[h];
+        }
       } else {
-        const bool some = vb >= 0 && key <= pos && key + 15 >= seen;
+        const int pos = now.ctx + min(col_token, now.tokens - 1);
+        const int seen = a.window > 0 ? max(0, pos + 1 - a.window) : 0;  // first key it sees
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int h = 0; h < H; ++h) {
+          const int key = key0 + 64 * h + 16 * G;
+          const bool some = cur[h].here && key <= pos && key + 15 >= seen;
+          top[h] = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int k = key + 4 * r + j;
-            s[r][j] = some && k <= pos && k >= seen ? s[r][j] * kscale : -INFINITY;
-            top = fmaxf(top, s[r][j]);
+          for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int k = key + 4 * r + j;
+              s[h][r][j] = some && k <= pos && k >= seen ? s[h][r][j] * kscale[h] : -INFINITY;
+              top[h] = fmaxf(top[h], s[h][r][j]);
+            }
           }
+          v_top[h] = some ? vscale[h] : 0.0f;
+          mul[h] = 1.0f;
         }
-        v_top = some ? vscale : 0.0f;
       }
       // a scale that is not finite makes the products what they should be,
       // but is no reference for others
-      v_top = v_top <= 3.0e38f ? v_top : 0.0f;
-      if (__any(top > st.m + State::kRescale || v_top > st.v_ref)) {
-        float m2 = fmaxf(st.m, top);
+      const float t_top = fmaxf(top[0], top[H - 1]);
+      const float t_v = fmaxf(v_top[0] <= 3.0e38f ? v_top[0] : 0.0f,
+                              v_top[H - 1] <= 3.0e38f ? v_top[H - 1] : 0.0f);
+      if (__any(t_top > st.m + State::kRescale || t_v > st.v_ref)) {
+        float m2 = fmaxf(st.m, t_top);
         m2 = fmaxf(m2, __shfl_xor(m2, 16));
         m2 = fmaxf(m2, __shfl_xor(m2, 32));
-        float v2 = fmaxf(st.v_ref, v_top);
+        float v2 = fmaxf(st.v_ref, t_v);
         v2 = fmaxf(v2, __shfl_xor(v2, 16));
         v2 = fmaxf(v2, __shfl_xor(v2, 32));
         const float ref = v2 > st.v_ref ? power_above(v2) : st.v_ref;
@@ -310,59 +410,84 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void attend_narrow_kernel(Att
 #pragma unroll
         for (int d = 0; d < kValueTiles; ++d) {
           st.o[d] *= keep_o;
-          if constexpr (State::kRest) st.rest[d] *= keep_o;
+          if constexpr (State::kApart) st.rest[d] *= keep_o;
         }
         st.m = m2;
         st.v_ref = ref;
         st.v_inv = ref > 0.0f ? 1.0f / ref : 0.0f;
       }
-      const float shift = (st.m == -INFINITY ? 0.0f : st.m) - kWeightBias;
-      const float v_factor = vscale * st.v_inv;
-      f16x8 w[2], w_rest[2];
+      const float shift = kWeightBias - (st.m == -INFINITY ? 0.0f : st.m);
+      float v_factor[H];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < H; ++h) v_factor[h] = vscale[h] * st.v_inv;
+      f16x8 w[H][2], w_rest[H][2];
+      // probabilities and their weights; `some_hidden`: 0 times a scale that
+      // is no number has to be 0
+      auto weights = [&](auto some_hidden) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float sc = s[2 * h + (e >> 2)][e & 3];
-          const float p = __builtin_amdgcn_exp2f(sc - shift);
-          st.l += p;
-          const float v = whole || sc != -INFINITY ? p * v_factor : 0.0f;
-          w[h][e] = static_cast<_Float16>(v);
-          if constexpr (State::kRest) {
-            w_rest[h][e] =
-                static_cast<_Float16>((v - static_cast<float>(w[h][e])) * State::kRestScale);
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float sc = s[h][2 * k + (e >> 2)][e & 3];
+              p[e] = __builtin_amdgcn_exp2f(fmaf(sc, mul[h], shift));
+              float v = p[e] * v_factor[h];
+              if constexpr (decltype(some_hidden)::value) v = sc == -INFINITY ? 0.0f : v;
+              w[h][k][e] = static_cast<_Float16>(v);
+              if constexpr (State::kRest) {
+                w_rest[h][k][e] =
+                    static_cast<_Float16>((v - static_cast<float>(w[h][k][e])) * State::kRestScale);
+              }
+            }
+            st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
           }
         }
+      };
+      if (!whole && __any(!(fabsf(v_factor[0]) <= 3.0e38f && fabsf(v_factor[H - 1]) <= 3.0e38f))) {
+        weights(std::true_type{});
+      } else {
+        weights(std::false_type{});
       }
+
 #pragma unroll
       for (int d = 0; d < kValueTiles; ++d) {
-        f16x8 c[2];
-        codes_to_f16(vr[d], c);
+        f16x8 c[H][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h], w[h], st.o[d], 0, 0, 0);
-          if constexpr (State::kRest) {
-            st.rest[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h], w_rest[h], st.rest[d], 0, 0, 0);
+        for (int h = 0; h < H; ++h) codes_to_f16(vr[d % kHeld][h], c[h]);
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][k], w[h][k], st.o[d], 0, 0, 0);
+            if constexpr (State::kRest) {
+              f32x4& o = State::kApart ? st.rest[d] : st.o[d];
+              o = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][k], w_rest[h][k], o, 0, 0, 0);
+            }
           }
         }
+        if (d + kHeld < kValueTiles) load_values(cur, d + kHeld);
+        else if constexpr (kMore) load_values(nxt, d + kHeld - kValueTiles);
       }
-      if (more) load_v(tile1, vb1);
 
-      if (!spans && (x + 1 == now.end || !more)) {
+      if (!spans && (!kMore || x + 1 == now.end)) {
         // the unit, or this run's share of it, is done
+        const AttendArgs& b = late_args();
+        const int cols = now.tokens * b.group;
         float l = st.l + __shfl_xor(st.l, 16);
         l += __shfl_xor(l, 32);
         const bool alone = now.first >= begin && now.end <= end;
-        float* part = a.parts + narrow_part(g, 4 * gridDim.y, run, now.first <= begin ? 0 : 1) *
+        float* part = b.parts + narrow_part(g, runs, run, now.first <= begin ? 0 : 1) *
                                     (kNarrowCols * (D + 2));
         if (i < cols) {
-          const int row = now.row + i / a.group, h = g * a.group + i % a.group;
+          const int row = now.row + col_token, h = g * b.group + i - col_token * b.group;
 #pragma unroll
           for (int d = 0; d < kValueTiles; ++d) {
             f32x4 o = st.o[d];
-            if constexpr (State::kRest) o += st.rest[d] * (1.0f / State::kRestScale);
+            if constexpr (State::kApart) o += st.rest[d] * (1.0f / State::kRestScale);
             o *= st.v_ref;
-            if (alone) finish4<T>(a, row, h, 16 * d + 4 * G, o, st.m, l);
+            if (alone) finish4<T>(b, row, h, 16 * d + 4 * G, o, st.m, l);
             else *reinterpret_cast<f32x4*>(part + i * D + 16 * d + 4 * G) = o;
           }
           if (!alone && G == 0) {
@@ -370,17 +495,20 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void attend_narrow_kernel(Att
             part[kNarrowCols * (D + 1) + i] = l;
           }
         }
-        if (more) {
+        if constexpr (kMore) {
+          now = unit_at(now.at + 1);
           reset();
-          narrow_query<T, D>(a, next, g, st);
+          narrow_query<T, D>(b, now, g, st, s_q);
         }
       }
-      now = next;
-      next = after;
-      vb = vb1;
-      kb1 = kb2;
-      vb1 = vb2;
-    }
+      if constexpr (kMore) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) cur[h] = nxt[h];
+      }
+    };
+    int x = begin;
+    for (; x + 1 < end; ++x) step(x, std::true_type{});
+    step(x, std::false_type{});
   }
 
   // The block's first tile decides for all four waves alike; a wave without
@@ -411,13 +539,13 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void attend_narrow_kernel(Att
 #pragma unroll
     for (int d = 0; d < kValueTiles; ++d) {
       f32x4 o = st.o[d];
-      if constexpr (State::kRest) o += st.rest[d] * (1.0f / State::kRestScale);
+      if constexpr (State::kApart) o += st.rest[d] * (1.0f / State::kRestScale);
       *reinterpret_cast<f32x4*>(&s_o[wave][i][16 * d + 4 * G]) = o * mine;
     }
   }
   __syncthreads();
   const bool alone = u.first == block_begin && u.end == block_end;
-  float* part = a.parts + narrow_part(g, 4 * gridDim.y, 4 * blockIdx.y, 0) * (kNarrowCols * (D + 2));
+  float* part = a.parts + narrow_part(g, runs, 4 * blockIdx.y, 0) * (kNarrowCols * (D + 2));
   for (int e = threadIdx.x; e < cols * (D / 4); e += 256) {
     const int c = e / (D / 4), d = e % (D / 4) * 4;
     f32x4 o = *reinterpret_cast<const f32x4*>(&s_o[0][c][d]);
@@ -455,28 +583,30 @@ __global__ __launch_bounds__(256) void join_narrow_kernel(AttendArgs a, int runs
   const NarrowUnit* units = reinterpret_cast<const NarrowUnit*>(a.work + a.at_units);
   const int32_t* first = reinterpret_cast<const int32_t*>(a.work + a.at_tiles);
   const int total = head->narrow_tiles, n_units = head->units;
-  const int share = narrow_share(total, runs);
   int at = blockIdx.y;
   if (by_unit) {
     if (at >= n_units) return;
   } else {
-    const int t = (blockIdx.y + 1) * share;
+    const int t = run_begin(total, runs, blockIdx.y + 1);
     if (t >= total) return;
     at = find_unit(first, n_units, t);
-    if (first[at] >= t || first[at] < t - share) return;  // not cut here, or cut before
+    // not cut here, or cut before
+    if (first[at] >= t || first[at] < run_begin(total, runs, blockIdx.y)) return;
   }
   const int from = first[at], to = first[at + 1];
   const NarrowUnit u = units[at];
   if (to <= from || c >= u.tokens * a.group) return;
-  const int r0 = from / share, r1 = (to - 1) / share;
+  const int r0 = run_of(total, runs, from), r1 = run_of(total, runs, to - 1);
   if (r0 == r1) return;
+  const NarrowRun* run = reinterpret_cast<const NarrowRun*>(a.work + a.at_runs);
   // One block held all of it: finished there.
-  if (r0 / 4 * 4 * share == from && min(total, (r0 / 4 + 1) * 4 * share) == to) return;
+  if (run[r0].block_begin == from && run[r0].block_stop == to) return;
   // Parts in order: a whole block's, or a run's.
   auto part_of = [&](int r) -> const float* {
-    const int b0 = r / 4 * 4 * share, b1 = min(total, (r / 4 + 1) * 4 * share);
-    if (from <= b0 && to >= b1) return r % 4 ? nullptr : a.parts + narrow_part(g, runs, r, 0) * (kNarrowCols * (D + 2));
-    return a.parts + narrow_part(g, runs, r, from > r * share ? 1 : 0) * (kNarrowCols * (D + 2));
+    const NarrowRun& n = run[r];
+    const bool whole = from <= n.block_begin && to >= n.block_stop;
+    if (whole && r % 4) return nullptr;
+    return a.parts + narrow_part(g, runs, r, from > n.begin ? 1 : 0) * (kNarrowCols * (D + 2));
   };
   __shared__ float s_top[4];
   __shared__ float s_l[kGroups];

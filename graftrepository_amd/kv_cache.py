@@ -201,6 +201,7 @@ class KvBatch:
         self._ref = ctypes.byref(d)
         self._scratch: dict[int, int] = {}
         self._held = None
+        self._planned = False
 
     def plan(self, stream=None) -> "KvBatch":
         """Fill ``cu_new``, ``slot_map``, ``positions``, the table's new
@@ -208,7 +209,12 @@ class KvBatch:
         rc = self._lib.grm_hip_kv_plan(self._ref, _stream(self.ctx_lens, stream))
         if rc:
             _lib.check(rc, "kv plan")
+        self._planned = True
         return self
+
+    def _need_plan(self):
+        if not self._planned:
+            raise ValueError("the batch has no plan yet: call plan() first")
 
     def advance(self) -> None:
         """The next plan goes on in the free list where the last one ended."""
@@ -258,6 +264,7 @@ class KvCache:
     def append(self, batch: KvBatch, k, v, stream=None) -> None:
         """Quantise the step's ``k`` and ``v`` [tokens, kv_heads, head_dim]
         (f32, bf16 or f16; any row and head strides) into their blocks."""
+        batch._need_plan()
         shape = (batch._desc.tokens, self.kv_heads, self.head_dim)
         kp, name, kt, kh = _rows(k, "k", shape)
         vptr, vname, vt, vh = _rows(v, "v", shape)
@@ -274,6 +281,7 @@ class KvCache:
         head_dim] over the cache, which holds the step's own tokens.  Returns
         ``out`` (q's type; also taken as an argument), with ``return_lse``
         also the fp32 [tokens, heads] log-sum-exp of the scores."""
+        batch._need_plan()
         d = batch._desc
         shape = (d.tokens, d.heads, self.head_dim)
         qp, name, qt, qh = _rows(q, "q", shape)
