@@ -9,6 +9,7 @@
 
 #include "kv_attend.hpp"
 #include "kv_narrow.hpp"
+#include "kv_wide.hpp"
 
 namespace grm {
 namespace kv {
@@ -35,7 +36,6 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
     len -= half;
   }
   const int r = lo;
-  if (static_cast<int64_t>(a.cu_new[r + 1] - a.cu_new[r]) * a.group <= a.skip_cols) return;
   const int pos = clamp_len(a.ctx_lens[r]) + row - a.cu_new[r];
   const int first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
   const typename T::store* q = static_cast<const typename T::store*>(a.q) +
@@ -135,28 +135,38 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
 // ------------------------------------------------------------- dispatch
 
 struct Shape {
-  bool narrow;        // the narrow kernel takes the requests it can
+  bool cores;         // the matrix-core kernels take the batch
+  uint64_t wide_bytes;  // of scratch that the wide kernel's parts take
+  int cap_parts, cap_items, cap_joins;
   int cus;
   uint64_t units;     // at most so many narrow units
   int runs[2];
   uint64_t at_runs[2];
-  uint64_t bytes;     // of scratch
+  uint64_t narrow_bytes, bytes;  // of scratch: the narrow parts, all
 };
 
 static int shape_of(const grm_kv_cache_desc* c, const Layout& l, Shape* out) {
   Shape s{};
   GRM_CHECK_RC(device_cus(&s.cus));
   const int hd = c->head_dim;
-  s.narrow = (hd == 64 || hd == 128 || hd == 256) && l.cap_units > 0;
+  s.cores = (hd == 64 || hd == 128 || hd == 256) && l.group <= kWideCols;
+  s.cap_parts = static_cast<int>(l.cap_parts);
+  s.cap_items = static_cast<int>(l.cap_items);
+  s.cap_joins = static_cast<int>(l.cap_joins);
   s.units = l.cap_units;
   for (int k = 0; k < 2; ++k) {
     s.runs[k] = l.runs[k];
     s.at_runs[k] = l.at_runs[k];
   }
-  if (s.narrow) {
+  if (s.cores && l.cap_units > 0) {
     s.bytes = static_cast<uint64_t>(c->kv_heads) * l.runs[hd == 256 ? 0 : 1] * 2 * kNarrowCols *
               (hd + 2) * 4;
   }
+  if (s.cores) {
+    s.wide_bytes = static_cast<uint64_t>(c->kv_heads) * l.cap_parts * wide_part_floats(hd) * 4;
+  }
+  s.narrow_bytes = (s.bytes + 255) / 256 * 256;
+  s.bytes = s.narrow_bytes + s.wide_bytes;
   *out = s;
   return 0;
 }
@@ -176,16 +186,34 @@ static void launch_narrow(AttendArgs a, const Shape& s, hipStream_t stream) {
   join_narrow_kernel<T, D><<<joins, 256, 0, stream>>>(a, runs, by_unit);
 }
 
+template <class T, int D>
+static void launch_wide(AttendArgs a, const Shape& s, hipStream_t stream) {
+  a.parts += s.narrow_bytes / 4;
+  const dim3 grid(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.cap_items));
+  attend_wide_kernel<T, D><<<grid, 256, 0, stream>>>(a);
+  const dim3 joins(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.cap_joins),
+                   kWideCols / 16);
+  join_wide_kernel<T, D><<<joins, 256, 0, stream>>>(a);
+}
+
+template <class T, int D>
+static void launch_cores(const AttendArgs& a, const Shape& s, hipStream_t stream) {
+  if (s.cap_items) launch_wide<T, D>(a, s, stream);
+  if (s.units) launch_narrow<T, D>(a, s, stream);
+}
+
 template <class T>
-static void launch(const AttendArgs& a, const Shape& s, bool all_narrow, hipStream_t stream) {
-  if (s.narrow) {
-    if (a.head_dim == 64) launch_narrow<T, 64>(a, s, stream);
-    else if (a.head_dim == 128) launch_narrow<T, 128>(a, s, stream);
-    else launch_narrow<T, 256>(a, s, stream);
-    if (all_narrow) return;
+static void launch(const AttendArgs& a, const Shape& s, hipStream_t stream) {
+  if (!s.cores) {
+    const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads));
+    attend_any_kernel<T><<<grid, 256, 0, stream>>>(a);
+  } else if (a.head_dim == 64) {
+    launch_cores<T, 64>(a, s, stream);
+  } else if (a.head_dim == 128) {
+    launch_cores<T, 128>(a, s, stream);
+  } else {
+    launch_cores<T, 256>(a, s, stream);
   }
-  const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads));
-  attend_any_kernel<T><<<grid, 256, 0, stream>>>(a);
 }
 
 }  // namespace kv
@@ -270,14 +298,13 @@ extern "C" int grm_hip_kv_attend(const grm_kv_cache_desc* c, const grm_kv_batch_
   a.at_tiles = l.at_tiles;
   a.at_items = l.at_items;
   a.at_joins = l.at_joins;
-  a.skip_cols = sh.narrow ? kNarrowCols : 0;
-  const bool all_narrow = static_cast<int64_t>(b->max_new) * l.group <= kNarrowCols;
+  a.cap_parts = sh.cap_parts;
   a.cols = static_cast<int32_t>(
       std::min<int64_t>(kNarrowCols, static_cast<int64_t>(std::max(1, b->max_new)) * l.group));
   const auto s = static_cast<hipStream_t>(stream);
-  if (dtype == grm::kF32) launch<F32>(a, sh, all_narrow, s);
-  else if (dtype == grm::kBF16) launch<BF16>(a, sh, all_narrow, s);
-  else launch<F16>(a, sh, all_narrow, s);
+  if (dtype == grm::kF32) launch<F32>(a, sh, s);
+  else if (dtype == grm::kBF16) launch<BF16>(a, sh, s);
+  else launch<F16>(a, sh, s);
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();
   return 0;

@@ -27,7 +27,7 @@ struct AttendArgs {
   int32_t requests, width, tokens, window;
   int32_t heads, kv_heads, group, head_dim, block_log2;
   int32_t cols;       // columns a narrow unit may have
-  int32_t skip_cols;  // attend_any leaves out requests of at most this many columns
+  int32_t cap_parts;  // wide partial results to a kv head
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -115,8 +115,11 @@ __device__ inline float power_above(float v) {
   return __builtin_amdgcn_ldexpf(1.0f, e > 127 ? 127 : e < -120 ? -120 : e);
 }
 
+// Log2 of what probabilities are scaled by on their way into fp16.
+__host__ __device__ constexpr float weight_bias(int dtype) { return dtype == kF32 ? 7.0f : 14.0f; }
+
 // Four values of a finished row: o / l rounded once, and the row's log-sum-exp
-// by the thread of its first column.  m in log2 units, l and o biased by 2^7.
+// by the thread of its first column.  m in log2 units, l and o biased.
 template <class T>
 __device__ inline void finish4(const AttendArgs& a, int row, int h, int d, f32x4 o, float m,
                                float l) {
@@ -142,7 +145,7 @@ __device__ inline void finish4(const AttendArgs& a, int row, int h, int d, f32x4
   }
   if (a.lse && d == 0) {
     a.lse[static_cast<size_t>(row) * a.heads + h] =
-        empty ? -INFINITY : (m - 7.0f + __builtin_amdgcn_logf(l)) * kLn2;
+        empty ? -INFINITY : (m - weight_bias(T::code) + __builtin_amdgcn_logf(l)) * kLn2;
   }
 }
 

@@ -29,19 +29,20 @@
 // halves of a value column, one 128-byte line, are read together (tiles of 64
 // tokens fetched 1.4 times the bytes there).
 //
-// Probabilities enter the second product as fp16(2^7 p vs / v), with v a
-// power of two no less than any value scale the column has met: they stay
-// below 2^15, and 2^-21 of the largest is still a normal number.  The
-// running maximum follows only when a score passes it by more than 8
-// (log2 units); until then nothing is rescaled.
+// Probabilities enter the second product as fp16(2^14 p vs / v), with v a
+// power of two no less than any value scale the column has met and at most
+// twice the largest.  The running maximum follows only when a score passes it
+// by more than 1 (log2 units), so weights stay below 2^15; 2^-28 of the
+// largest probability is still a normal number, and what is lost below that
+// is 2^-39 of it.  (An allowance of 8 would rescale less often, but lose
+// 2^-32.)
 //
 // For fp16 and fp32 outputs the probabilities are two fp16 terms, the second
 // what the first leaves (one term alone is off by 2.4e-4 of a flat row, more
-// than the rounding to fp16).  For fp16 both are summed in one place; the
-// second is exact to 2^-25, 2^-32 of the largest probability.  For fp32 the
-// second is scaled by 2^19 and summed apart, and the maximum follows at once,
-// so that both stay below 2^15 and reach 2^-51 of the largest; fp32 queries
-// are two terms too.
+// than the rounding to fp16).  For fp16 both are summed in one place.  For
+// fp32 the first is scaled by 2^7, the second by 2^19 more and summed apart,
+// and the maximum follows at once, so that both stay below 2^15 and reach
+// 2^-51 of the largest; fp32 queries are two terms too.
 #pragma once
 
 #include "kv_attend.hpp"
@@ -85,7 +86,6 @@ __device__ __forceinline__ const AttendArgs& late_args() {
   return *(const AttendArgs*)(ConstArgs)p;
 }
 
-constexpr float kWeightBias = 7.0f;
 
 // Everything one wave carries for one unit.
 template <class T, int D>
@@ -94,11 +94,11 @@ struct NarrowState {
   static constexpr bool kRest = T::code != kBF16;               // of a probability: two
   static constexpr bool kApart = T::code == kF32;               // and summed apart
   static constexpr float kRestScale = kApart ? 524288.0f : 1.0f;
-  static constexpr float kRescale = T::code == kF32 ? 0.0f : 8.0f;
+  static constexpr float kRescale = kApart ? 0.0f : 1.0f;
   float col_scale;  // softmax scale, log2 e and the query's own power of two
   f32x4 o[D / 16];
   f32x4 rest[kApart ? D / 16 : 1];
-  float m, l;       // running maximum and this lane's sum of 2^(s - m + 7)
+  float m, l;       // running maximum and this lane's sum of 2^(s - m + bias)
   float v_ref, v_inv;
 };
 
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
         st.v_ref = ref;
         st.v_inv = ref > 0.0f ? 1.0f / ref : 0.0f;
       }
-      const float shift = kWeightBias - (st.m == -INFINITY ? 0.0f : st.m);
+      const float shift = weight_bias(T::code) - (st.m == -INFINITY ? 0.0f : st.m);
       float v_factor[H];
 #pragma unroll
       for (int h = 0; h < H; ++h) v_factor[h] = vscale[h] * st.v_inv;
