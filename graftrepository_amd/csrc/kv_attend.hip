@@ -141,7 +141,7 @@ struct Shape {
   int cus;
   uint64_t units;     // at most so many narrow units
   int runs[2];
-  uint64_t at_runs[2];
+  uint64_t at_run_units[2];
   uint64_t narrow_bytes, bytes;  // of scratch: the narrow parts, all
 };
 
@@ -156,7 +156,7 @@ static int shape_of(const grm_kv_cache_desc* c, const Layout& l, Shape* out) {
   s.units = l.cap_units;
   for (int k = 0; k < 2; ++k) {
     s.runs[k] = l.runs[k];
-    s.at_runs[k] = l.at_runs[k];
+    s.at_run_units[k] = l.at_run_units[k];
   }
   if (s.cores && l.cap_units > 0) {
     s.bytes = static_cast<uint64_t>(c->kv_heads) * l.runs[hd == 256 ? 0 : 1] * 2 * kNarrowCols *
@@ -175,7 +175,7 @@ template <class T, int D>
 static void launch_narrow(AttendArgs a, const Shape& s, hipStream_t stream) {
   const int k = narrow_blocks_per_cu(T::code, D) - 1;
   const int runs = s.runs[k];
-  a.at_runs = s.at_runs[k];
+  a.at_run_units = s.at_run_units[k];
   const dim3 grid(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(runs / 4));
   if (a.block_log2 == 7) attend_narrow_kernel<T, D, 2><<<grid, 256, 0, stream>>>(a);
   else attend_narrow_kernel<T, D, 1><<<grid, 256, 0, stream>>>(a);

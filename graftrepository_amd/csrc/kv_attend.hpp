@@ -22,7 +22,7 @@ struct AttendArgs {
   const char* work;
   float* parts;
   int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-  uint64_t blocks, at_units, at_tiles, at_runs, at_items, at_joins;
+  uint64_t blocks, at_units, at_tiles, at_run_units, at_items, at_joins;
   float scale;
   int32_t requests, width, tokens, window;
   int32_t heads, kv_heads, group, head_dim, block_log2;

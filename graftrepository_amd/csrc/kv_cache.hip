@@ -9,6 +9,7 @@
 #include "kv_common.hpp"
 
 #include <mutex>
+#include <type_traits>
 
 namespace grm {
 namespace kv {
@@ -106,12 +107,12 @@ int layout_of(const grm_kv_batch_desc* b, Layout* out) {
   const bool wide = static_cast<int64_t>(b->max_new) * l.group > kNarrowCols;
   l.wide_tokens = wide && l.group <= kWideCols ? kWideCols / l.group : 0;
   if (l.wide_tokens) {
-    const uint64_t units = rows / l.wide_tokens + busy;
+    l.cap_wide = rows / l.wide_tokens + busy;
     // Only units longer than the share C = all / (4 x blocks) are cut, into
     // at most 2 x length / C parts.
     l.cap_parts = 8 * static_cast<uint64_t>(l.wide_blocks) + 8;
     l.cap_joins = l.cap_parts / 2;
-    l.cap_items = units + l.cap_parts;
+    l.cap_items = l.cap_wide + l.cap_parts;
   }
   auto place = [&l](uint64_t bytes) {
     const uint64_t at = l.bytes;
@@ -123,9 +124,10 @@ int layout_of(const grm_kv_batch_desc* b, Layout* out) {
   l.at_units = place(l.cap_units * sizeof(NarrowUnit));
   l.at_tiles = place((l.cap_units + 1) * 4);
   for (int k = 0; k < 2; ++k) {
-    l.at_runs[k] = place(l.cap_units ? l.runs[k] * sizeof(NarrowRun) : 0);
+    l.at_run_units[k] = place(l.cap_units ? l.runs[k] * 4 : 0);
   }
   l.at_scan = place(l.wide_tokens ? (reqs + 1) * 4 : 0);
+  l.at_wide = place(l.cap_wide * sizeof(WideUnit));
   l.at_items = place(l.cap_items * sizeof(WideItem));
   l.at_joins = place(l.cap_joins * sizeof(WideJoin));
   *out = l;
@@ -160,9 +162,9 @@ struct PlanArgs {
   int32_t requests, width, tokens, window;
   int32_t free_count, group, wide_tokens, kv_heads;
   int32_t wide_blocks, block_log2;
-  int32_t cap_append, cap_units, cap_items, cap_joins, cap_parts;
+  int32_t cap_append, cap_units, cap_wide, cap_items, cap_joins, cap_parts;
   int32_t runs[2];
-  uint64_t at_append, at_units, at_tiles, at_runs[2], at_scan, at_items, at_joins;
+  uint64_t at_append, at_units, at_tiles, at_run_units[2], at_scan, at_wide, at_items, at_joins;
 };
 
 // Exclusive sums over the block of N values per thread; totals to `sum`.
@@ -196,6 +198,12 @@ __device__ void block_scan(int (&v)[N], int (&sum)[N], int* scratch) {
     sum[k] = all;
   }
   __syncthreads();
+}
+
+__device__ inline int wave_sum(int v) {
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
 }
 
 struct Lens {
@@ -319,54 +327,90 @@ __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
   }
 }
 
-constexpr int kScanInts = 5 * 16 + 16;
+constexpr int kScanInts = 6 * 16 + 32;  // scan sums, and the candidates' counts
+constexpr int kPlanInts = 4 * kPlanChunk + 256;
 
 __device__ void plan_schedule(const PlanArgs& a, int* lds) {
-  int* scratch = lds;  // [5 * 16] and, after it, the candidates' counts: kScanInts
+  int* scratch = lds;                                     // [kScanInts]
+  int* tiles_lds = lds + kScanInts;                       // [kPlanChunk]
+  int* wide_lds = tiles_lds + kPlanChunk;                 // the rest
+  constexpr int kWideInts = kPlanInts - kScanInts - kPlanChunk;
   SchedHead* head = reinterpret_cast<SchedHead*>(a.work);
   NarrowUnit* units = reinterpret_cast<NarrowUnit*>(a.work + a.at_units);
   int* tiles = reinterpret_cast<int*>(a.work + a.at_tiles);
   int* wide_at = reinterpret_cast<int*>(a.work + a.at_scan);
-  int done[5] = {0, 0, 0, 0, 0};  // new, need, touched, narrow tiles, wide units
-  int done_units = 0;
-  for (int base = 0; base < a.requests; base += kPlanThreads) {
-    const int r = base + static_cast<int>(threadIdx.x);
-    const Lens l = lens_of(a, r);
-    const bool narrow =
-        l.fresh > 0 && static_cast<int64_t>(l.fresh) * a.group <= kNarrowCols && a.cap_units > 0;
-    int lo = 0, hi = 0;
-    if (narrow) tiles_of(a, narrow_tile(1 << a.block_log2), l.ctx, 0, l.fresh, &lo, &hi);
-    const int wide = a.wide_tokens && l.fresh > 0 && !narrow
-                         ? (l.fresh + a.wide_tokens - 1) / a.wide_tokens : 0;
-    int v[5] = {l.fresh, l.need, l.touched, hi - lo, wide}, sum[5];
-    block_scan(v, sum, scratch);
-    int u[1] = {narrow ? 1 : 0}, usum[1];
-    block_scan(u, usum, scratch);
-    if (r < a.requests) {
-      a.cu_new[r] = done[0] + v[0];
-      if (a.wide_tokens) wide_at[r] = done[4] + v[4];
-      const int at = done_units + u[0];
-      if (narrow && static_cast<unsigned>(at) < static_cast<unsigned>(a.cap_units)) {
-        NarrowUnit n;
-        n.request = r;
-        n.row = done[0] + v[0];
-        n.tokens = max(0, min(l.fresh, a.tokens - n.row));
-        n.tile_lo = lo;
-        n.ctx = l.ctx;
-        units[at] = n;
-        tiles[at] = done[3] + v[3];
+  const bool wide_fits = a.requests < kWideInts;
+  // new tokens, blocks needed, touched blocks, narrow tiles, wide units,
+  // narrow units
+  int done[6] = {0, 0, 0, 0, 0, 0};
+  for (int base = 0; base < a.requests; base += kPlanChunk) {
+    const int r0 = base + static_cast<int>(threadIdx.x) * kPerThread;
+    Lens l[kPerThread];
+    int lo[kPerThread], hi[kPerThread], wide[kPerThread];
+    bool narrow[kPerThread];
+    int v[6] = {0, 0, 0, 0, 0, 0}, sum[6];
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+      l[j] = lens_of(a, r0 + j);
+      narrow[j] = l[j].fresh > 0 && a.cap_units > 0 &&
+                  static_cast<int64_t>(l[j].fresh) * a.group <= kNarrowCols;
+      lo[j] = hi[j] = 0;
+      if (narrow[j]) {
+        tiles_of(a, narrow_tile(1 << a.block_log2), l[j].ctx, 0, l[j].fresh, &lo[j], &hi[j]);
       }
+      wide[j] = a.wide_tokens && l[j].fresh > 0 && !narrow[j]
+                    ? (l[j].fresh + a.wide_tokens - 1) / a.wide_tokens : 0;
+      v[0] += l[j].fresh;
+      v[1] += l[j].need;
+      v[2] += l[j].touched;
+      v[3] += hi[j] - lo[j];
+      v[4] += wide[j];
+      v[5] += narrow[j];
+    }
+    block_scan(v, sum, scratch);
+#pragma unroll
+    for (int k = 0; k < 6; ++k) v[k] += done[k];
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+      const int r = r0 + j;
+      if (r < a.requests) {
+        a.cu_new[r] = v[0];
+        if (a.wide_tokens) {
+          wide_at[r] = v[4];
+          if (wide_fits) wide_lds[r] = v[4];
+        }
+        if (narrow[j] && static_cast<unsigned>(v[5]) < static_cast<unsigned>(a.cap_units)) {
+          NarrowUnit n;
+          n.request = r;
+          n.row = v[0];
+          n.tokens = max(0, min(l[j].fresh, a.tokens - n.row));
+          n.tile_lo = lo[j];
+          n.ctx = l[j].ctx;
+          n.pad[0] = n.pad[1] = n.pad[2] = 0;
+          units[v[5]] = n;
+          tiles[v[5]] = v[3];
+          if (v[5] < kPlanChunk) tiles_lds[v[5]] = v[3];
+        }
+      }
+      v[0] += l[j].fresh;
+      v[3] += hi[j] - lo[j];
+      v[4] += wide[j];
+      v[5] += narrow[j];
     }
 #pragma unroll
-    for (int k = 0; k < 5; ++k) done[k] += sum[k];
-    done_units += usum[0];
+    for (int k = 0; k < 6; ++k) done[k] += sum[k];
   }
-  done_units = min(done_units, a.cap_units);
+  const int done_units = max(0, min(done[5], a.cap_units));
   const int wide_units = done[4];
+  const bool tiles_fit = done_units < kPlanChunk;
   if (threadIdx.x == 0) {
     a.cu_new[a.requests] = done[0];
     tiles[done_units] = done[3];
-    if (a.wide_tokens) wide_at[a.requests] = wide_units;
+    if (tiles_fit) tiles_lds[done_units] = done[3];
+    if (a.wide_tokens) {
+      wide_at[a.requests] = wide_units;
+      if (wide_fits) wide_lds[a.requests] = wide_units;
+    }
     if (a.free_head) {
       const int at = max(0, *a.free_head);
       const int left = max(0, a.free_count - at);
@@ -380,71 +424,52 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   }
   __syncthreads();  // the lists are read back by other threads of this block
 
-  // Where the narrow kernel's wavefronts begin; without units every run is
-  // empty.
+  // The unit that each run of the narrow kernel begins in; 0 where it is empty.
   if (a.cap_units > 0) {
-    int* cached = lds + kScanInts;
-    const bool fits = done_units < kPlanChunk;
-    if (fits) {
-      for (int u = threadIdx.x; u <= done_units; u += kPlanThreads) cached[u] = tiles[u];
-      __syncthreads();
-    }
-    const int* from = fits ? cached : tiles;
+    const int* from = tiles_fit ? tiles_lds : tiles;
     for (int k = 0; k < 2; ++k) {
-      NarrowRun* runs = reinterpret_cast<NarrowRun*>(a.work + a.at_runs[k]);
+      const Deal deal(done[3], a.runs[k]);
+      int* run_units = reinterpret_cast<int*>(a.work + a.at_run_units[k]);
       for (int r = threadIdx.x; r < a.runs[k]; r += kPlanThreads) {
-        NarrowRun n;
-        n.begin = run_begin(done[3], a.runs[k], r);
-        n.stop = run_begin(done[3], a.runs[k], r + 1);
-        n.block_begin = run_begin(done[3], a.runs[k], r / 4 * 4);
-        n.block_stop = run_begin(done[3], a.runs[k], r / 4 * 4 + 4);
-        NarrowUnit u{};
-        n.at = n.first = n.end = 0;
-        if (n.begin < n.stop) {
-          n.at = upper(from, done_units, n.begin);
-          n.first = from[n.at];
-          n.end = from[n.at + 1];
-          u = units[n.at];
-        }
-        n.request = u.request;
-        n.row = u.row;
-        n.tokens = u.tokens;
-        n.tile_lo = u.tile_lo;
-        n.ctx = u.ctx;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) n.pad[e] = 0;
-        runs[r] = n;
+        const int begin = deal.begin(r);
+        run_units[r] = begin < deal.begin(r + 1) ? upper(from, done_units, begin) : 0;
       }
     }
   }
   if (wide_units == 0) return;
-  __syncthreads();
 
   // Longest share C of a wide item.  More blocks than units: units are cut.
   // Candidates are the even share over k = 1..4; the estimate of each is
   // (rounds of blocks) x (mean item + 2 tiles for its prologue), no less
   // than its longest item.
   constexpr int kCands = 4;
-  int* count = lds + 5 * 16;  // [kCands], then total and longest
+  int* count = lds + 6 * 16;  // [kCands], then total and longest
   int* total_at = count + kCands;
   if (threadIdx.x < kCands + 2) count[threadIdx.x] = 0;
   __syncthreads();
-  auto unit_tiles = [&](int u, int* r, int* t0, int* n, int* lo, int* hi) {
-    *r = upper(wide_at, a.requests, u);
-    *t0 = (u - wide_at[*r]) * a.wide_tokens;
-    const int ctx = clamp_len(a.ctx_lens[*r]);
-    *n = min(a.wide_tokens, clamp_len(a.new_lens[*r]) - *t0);
-    tiles_of(a, kTile, ctx, *t0, *n, lo, hi);
-  };
+  // Each unit's request is searched for once, in LDS where the sums fit.
+  const int* wide_from = wide_fits ? wide_lds : wide_at;
+  WideUnit* wide = reinterpret_cast<WideUnit*>(a.work + a.at_wide);
+  const int stored = min(wide_units, a.cap_wide);
   int mine = 0, longest = 0;
-  for (int u = threadIdx.x; u < wide_units; u += kPlanThreads) {
-    int r, t0, n, lo, hi;
-    unit_tiles(u, &r, &t0, &n, &lo, &hi);
-    mine += hi - lo;
-    longest = max(longest, hi - lo);
+  for (int u = threadIdx.x; u < stored; u += kPlanThreads) {
+    WideUnit w;
+    w.request = upper(wide_from, a.requests, u);
+    w.t0 = (u - wide_from[w.request]) * a.wide_tokens;
+    const int ctx = clamp_len(a.ctx_lens[w.request]);
+    const int n = min(a.wide_tokens, clamp_len(a.new_lens[w.request]) - w.t0);
+    tiles_of(a, kTile, ctx, w.t0, n, &w.lo, &w.hi);
+    wide[u] = w;
+    mine += w.hi - w.lo;
+    longest = max(longest, w.hi - w.lo);
   }
-  atomicAdd(&total_at[0], mine);
-  atomicMax(&total_at[1], longest);
+  mine = wave_sum(mine);
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) longest = max(longest, __shfl_xor(longest, d));
+  if (__lane_id() == 0) {
+    atomicAdd(&total_at[0], mine);
+    atomicMax(&total_at[1], longest);
+  }
   __syncthreads();
   const int total = total_at[0];
   longest = total_at[1];
@@ -455,14 +480,16 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     cand[k] = max(8, (even + k) / (k + 1));
     items_of[k] = 0;
   }
-  for (int u = threadIdx.x; u < wide_units; u += kPlanThreads) {
-    int r, t0, n, lo, hi;
-    unit_tiles(u, &r, &t0, &n, &lo, &hi);
+  for (int u = threadIdx.x; u < stored; u += kPlanThreads) {
+    const int tiles_here = wide[u].hi - wide[u].lo;
 #pragma unroll
-    for (int k = 0; k < kCands; ++k) items_of[k] += (hi - lo + cand[k] - 1) / cand[k];
+    for (int k = 0; k < kCands; ++k) items_of[k] += (tiles_here + cand[k] - 1) / cand[k];
   }
 #pragma unroll
-  for (int k = 0; k < kCands; ++k) atomicAdd(&count[k], items_of[k]);
+  for (int k = 0; k < kCands; ++k) {
+    const int n = wave_sum(items_of[k]);
+    if (__lane_id() == 0) atomicAdd(&count[k], n);
+  }
   __syncthreads();
   int share = cand[0];
   float best = INFINITY;
@@ -481,11 +508,18 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   WideItem* items = reinterpret_cast<WideItem*>(a.work + a.at_items);
   WideJoin* joins = reinterpret_cast<WideJoin*>(a.work + a.at_joins);
   int done_items = 0, done_joins = 0, done_parts = 0;
-  for (int base = 0; base < wide_units; base += kPlanThreads) {
+  for (int base = 0; base < stored; base += kPlanThreads) {
     // The last units of a causal request are its longest: they go first.
-    const int u = wide_units - 1 - (base + static_cast<int>(threadIdx.x));
+    const int u = stored - 1 - (base + static_cast<int>(threadIdx.x));
     int r = 0, t0 = 0, n = 0, lo = 0, hi = 0;
-    if (u >= 0) unit_tiles(u, &r, &t0, &n, &lo, &hi);
+    if (u >= 0) {
+      const WideUnit w = wide[u];
+      r = w.request;
+      t0 = w.t0;
+      n = min(a.wide_tokens, clamp_len(a.new_lens[r]) - t0);
+      lo = w.lo;
+      hi = w.hi;
+    }
     int cut = u >= 0 ? max(1, (hi - lo + share - 1) / share) : 0;
     int v[3] = {cut, cut > 1 ? 1 : 0, cut > 1 ? cut : 0}, sum[3];
     block_scan(v, sum, scratch);
@@ -527,7 +561,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
-  __shared__ int lds[4 * kPlanChunk + 1 + 3 * 16];
+  __shared__ int lds[kPlanInts];
   if (blockIdx.x == 0) plan_schedule(a, lds);
   else plan_slots(a, static_cast<int>(blockIdx.x - 1) * kPlanTokens, lds);
 }
@@ -553,60 +587,307 @@ __device__ inline float wave_max(float v) {
   return v;
 }
 
-// One block per (touched block, kv head, keys or values).
-template <class T>
-__global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
-  const SchedHead* head = reinterpret_cast<const SchedHead*>(a.work);
-  const int item = blockIdx.x, g = blockIdx.y, kv = blockIdx.z;
-  if (item >= head->appends) return;
-  const AppendItem it = reinterpret_cast<const AppendItem*>(a.work + a.at_append)[item];
-  if (it.block < 0 || static_cast<uint64_t>(it.block) >= a.blocks) return;
-  const int bs = 1 << a.block_log2, hd = a.head_dim;
-  const typename T::store* x = static_cast<const typename T::store*>(a.x[kv]) +
-                               static_cast<int64_t>(it.row) * a.token_stride[kv] +
-                               static_cast<int64_t>(g) * a.head_stride[kv];
-  const size_t cell = static_cast<size_t>(it.block) * a.kv_heads + g;
-  int8_t* codes = a.codes[kv] + cell * bs * hd;
-  float* scale_at = a.scales[kv] + cell;
-  const int n = it.count * hd;
+// The step of a (block, head) whose new values reach `top` in magnitude.
+__device__ inline float step_of(float top, float before, bool odd) {
+  const float scale = fmaxf(before, top * (1.0f / 127.0f));
+  return odd || !(before <= 3.4028235e38f) ? NAN : scale;
+}
 
+// rint(v / step) in [-127, 127], the quotient rounded to fp32 first.  QUICK:
+// the correctly rounded quotient from the correctly rounded reciprocal, by
+// Markstein's theorem (q' = q + (v - q s) / s in two fused steps, exact where
+// nothing under- or overflows); elsewhere the division itself.  A step of 0 or
+// NaN gives 0.
+constexpr float kQuickFrom = 0x1p-90f, kQuickTo = 0x1p100f;
+
+template <bool QUICK>
+__device__ inline int quantise(float v, float scale, float inv) {
+  float q;
+  if constexpr (QUICK) {
+    const float q0 = v * inv;
+    q = fmaf(fmaf(-q0, scale, v), inv, q0);
+  } else {
+    q = scale > 0.0f ? v / scale : 0.0f;
+  }
+  return static_cast<int>(fminf(fmaxf(rintf(q), -127.0f), 127.0f));
+}
+
+__device__ inline int follow(int code, float ratio) {
+  return static_cast<int>(rintf(static_cast<float>(code) * ratio));
+}
+
+// Four codes of a word after a change of step.
+__device__ inline uint32_t follow4(uint32_t w, float ratio) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    r |= (static_cast<uint32_t>(follow(code_at(w, b), ratio)) & 0xffu) << (8 * b);
+  }
+  return r;
+}
+
+// Bytes [lo, hi) of a word, as a mask (any lo and hi).
+__device__ inline uint32_t bytes_in(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 4);
+  if (lo >= hi) return 0u;
+  return (hi == 4 ? 0xffffffffu : (1u << (8 * hi)) - 1u) & ~((1u << (8 * lo)) - 1u);
+}
+
+// What one block of an append works on.
+template <class T>
+struct AppendWork {
+  AppendItem it;
+  const typename T::store* x;  // the item's first row, this head
+  int64_t token_stride;
+  int8_t* codes;
+  float* scale;
+};
+
+template <class T>
+__device__ inline bool append_work(const AppendArgs& a, AppendWork<T>* w) {
+  const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
+  const int item = blockIdx.x, g = blockIdx.y, kv = blockIdx.z;
+  const auto* list =
+      reinterpret_cast<ConstAppend>(reinterpret_cast<uintptr_t>(a.work) + a.at_append);
+  // the list has a place for every block of the grid
+  w->it = {list[item].block, list[item].row, list[item].place, list[item].count};
+  if (item >= head->appends) return false;
+  if (w->it.block < 0 || static_cast<uint64_t>(w->it.block) >= a.blocks) return false;
+  w->token_stride = a.token_stride[kv];
+  w->x = static_cast<const typename T::store*>(a.x[kv]) +
+         static_cast<int64_t>(w->it.row) * a.token_stride[kv] +
+         static_cast<int64_t>(g) * a.head_stride[kv];
+  const size_t cell = static_cast<size_t>(w->it.block) * a.kv_heads + g;
+  w->codes = a.codes[kv] + (cell * a.head_dim << a.block_log2);
+  w->scale = a.scales[kv] + cell;
+  return true;
+}
+
+// The new step from the threads' largest values.
+__device__ inline float block_step(float top, bool odd, float before) {
+  __shared__ float s_top[kAppendThreads / kWave];
+  __shared__ int s_odd[kAppendThreads / kWave];
+  top = wave_max(top);
+  const bool wave_odd = __any(odd);
+  if (__lane_id() == 0) {
+    s_top[threadIdx.x / kWave] = top;
+    s_odd[threadIdx.x / kWave] = wave_odd;
+  }
+  __syncthreads();
+  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  return step_of(top, before, s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]);
+}
+
+// Value by value: any strides; also the faster way for a token or two (4.4
+// against 7.4 us for 64 requests of one token).
+template <class T>
+__device__ inline void append_values(const AppendArgs& a, const AppendWork<T>& w) {
+  const int kv = blockIdx.z, bs = 1 << a.block_log2, hd = a.head_dim;
+  const int n = w.it.count * hd, place = w.it.place;
+  const float before = place > 0 ? *w.scale : 0.0f;
   float top = 0.0f;
   bool odd = false;  // something not finite
   for (int i = threadIdx.x; i < n; i += kAppendThreads) {
-    const float v = fabsf(T::get(x[static_cast<int64_t>(i / hd) * a.token_stride[kv] + i % hd]));
+    const float v = fabsf(T::get(w.x[static_cast<int64_t>(i / hd) * w.token_stride + i % hd]));
     odd |= !(v <= 3.4028235e38f);
     top = fmaxf(top, v);
   }
-  __shared__ float s_top[kAppendThreads / kWave];
-  __shared__ int s_odd;
-  if (threadIdx.x == 0) s_odd = 0;
-  __syncthreads();
-  top = wave_max(top);
-  if (__lane_id() == 0) s_top[threadIdx.x / kWave] = top;
-  if (odd) s_odd = 1;
-  const float before = it.place > 0 ? *scale_at : 0.0f;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  float scale = fmaxf(before, top * (1.0f / 127.0f));
-  if (s_odd || !(before <= 3.4028235e38f)) scale = NAN;
-
+  const float scale = block_step(top, odd, before);
   // V is transposed in its block: element (place p, column d) at d * bs + p.
   const int step_p = kv ? 1 : hd, step_d = kv ? bs : 1;
-  if (it.place > 0 && !(scale == before)) {
+  if (place > 0 && !(scale == before)) {  // the held codes follow
     const float ratio = scale > 0.0f ? before / scale : 0.0f;
-    for (int i = threadIdx.x; i < it.place * hd; i += kAppendThreads) {
-      const int p = kv ? i % it.place : i / hd, d = kv ? i / it.place : i % hd;
-      int8_t* c = codes + p * step_p + d * step_d;
-      *c = static_cast<int8_t>(rintf(static_cast<float>(*c) * ratio));
+    if (kv == 0) {
+      uint32_t* held = reinterpret_cast<uint32_t*>(w.codes);
+      for (int i = threadIdx.x; i < place * hd / 4; i += kAppendThreads) {
+        held[i] = follow4(held[i], ratio);
+      }
+    } else {
+      const int words = (place + 3) / 4;
+      for (int i = threadIdx.x; i < words * hd; i += kAppendThreads) {
+        const int p = i % words * 4;
+        uint32_t* at = reinterpret_cast<uint32_t*>(w.codes + i / words * bs + p);
+        const uint32_t held = bytes_in(0, place - p);
+        *at = (follow4(*at, ratio) & held) | (*at & ~held);
+      }
+      __syncthreads();  // a word may hold new places too
     }
   }
   for (int i = threadIdx.x; i < n; i += kAppendThreads) {
     const int t = i / hd, d = i % hd;
-    const float v = T::get(x[static_cast<int64_t>(t) * a.token_stride[kv] + d]);
-    const float q = scale > 0.0f ? fminf(fmaxf(rintf(v / scale), -127.0f), 127.0f) : 0.0f;
-    codes[(it.place + t) * step_p + d * step_d] = static_cast<int8_t>(q);
+    const float v = T::get(w.x[static_cast<int64_t>(t) * w.token_stride + d]);
+    w.codes[(place + t) * step_p + d * step_d] = static_cast<int8_t>(quantise<false>(v, scale, 0.0f));
   }
-  if (threadIdx.x == 0) *scale_at = scale;
+  if (threadIdx.x == 0) *w.scale = scale;
+}
+
+// One block per (touched block, kv head, keys or values).  A thread takes 4
+// neighbouring places x 8 columns (up to UNITS such), loads them once in
+// 16-byte pieces and keeps them while the block's largest is found.  Keys go
+// out as 8 bytes a place.  Values are transposed in their block: 4 places of
+// a column are one word, gathered in LDS, and leave as 16 bytes; where a
+// group of 16 places holds tokens that were there, its old codes are merged.
+// Bound by bytes: a new value is read once and its code written once.
+template <class T, int UNITS>
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
+  constexpr int kWords = 8 * sizeof(typename T::store) / 16;  // 16-byte pieces of 8 values
+  AppendWork<T> work;
+  if (!append_work(a, &work)) return;
+  if (work.it.count <= 2) {
+    append_values(a, work);
+    return;
+  }
+  const AppendItem it = work.it;
+  const int kv = blockIdx.z, bs = 1 << a.block_log2, hd = a.head_dim;
+  const typename T::store* x = work.x;
+  int8_t* codes = work.codes;
+  const int end = it.place + it.count;       // places [it.place, end) are new
+  const int p0 = it.place & ~3;              // units begin at whole words
+  const int vecs = hd / 8, units = ((end - p0 + 3) / 4) * vecs;
+
+  u32x4 raw[UNITS][4][kWords];
+  float top = 0.0f;
+  bool odd = false;  // something not finite
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k) {
+    const int u = k * kAppendThreads + static_cast<int>(threadIdx.x);
+    if (u < units) {
+      const int p = p0 + u / vecs * 4, d = u % vecs * 8;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (p + t >= it.place && p + t < end) {
+          const u32x4* from = reinterpret_cast<const u32x4*>(
+              x + static_cast<int64_t>(p + t - it.place) * work.token_stride + d);
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) raw[k][t][w] = from[w];
+        } else {
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) raw[k][t][w] = u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+    }
+  }
+  auto value = [&](int k, int t, int e) {
+    if constexpr (T::code == kF32) {
+      return __uint_as_float(raw[k][t][e / 4][e % 4]);
+    } else {
+      return T::get(static_cast<uint16_t>((raw[k][t][0][e / 2] >> (16 * (e & 1))) & 0xffffu));
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k) {
+    if (k * kAppendThreads + static_cast<int>(threadIdx.x) < units) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = fabsf(value(k, t, e));
+          odd |= !(v <= 3.4028235e38f);
+          top = fmaxf(top, v);
+        }
+      }
+    }
+  }
+  __shared__ __align__(16) uint32_t s_v[UNITS * kAppendThreads * 8];  // [column][places / 4]
+  const float before = it.place > 0 ? *work.scale : 0.0f;
+  const float scale = block_step(top, odd, before);
+  const bool moved = it.place > 0 && !(scale == before);
+  const float ratio = scale > 0.0f ? before / scale : 0.0f;
+
+  const int words = bs / 4;  // of a value column
+  const float inv = 1.0f / scale;
+  auto write_codes = [&](auto quick) {
+    constexpr bool kQuick = decltype(quick)::value;
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+      const int u = k * kAppendThreads + static_cast<int>(threadIdx.x);
+      if (u < units) {
+        const int p = p0 + u / vecs * 4, d = u % vecs * 8;
+        uint32_t q[4][2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            q[t][w] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              q[t][w] |= (static_cast<uint32_t>(quantise<kQuick>(value(k, t, 4 * w + e), scale, inv)) & 0xffu)
+                         << (8 * e);
+            }
+          }
+          if (kv == 0 && p + t >= it.place && p + t < end) {
+            *reinterpret_cast<u32x2*>(codes + (p + t) * hd + d) = u32x2{q[t][0], q[t][1]};
+          }
+        }
+        if (kv == 1) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            uint32_t w = 0u;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w |= (q[t][e / 4] >> (8 * (e % 4)) & 0xffu) << (8 * t);
+            s_v[(d + e) * words + (p >> 2)] = w;
+          }
+        }
+      }
+    }
+  };
+  if (scale >= kQuickFrom && scale <= kQuickTo) write_codes(std::true_type{});
+  else write_codes(std::false_type{});
+  if (kv == 0) {
+    if (moved) {  // the held codes follow
+      uint32_t* held = reinterpret_cast<uint32_t*>(codes);
+      for (int i = threadIdx.x; i < it.place * hd / 4; i += kAppendThreads) {
+        held[i] = follow4(held[i], ratio);
+      }
+    }
+  } else {
+    __syncthreads();
+    const int first_group = moved ? 0 : it.place >> 4, groups = (end + 15) >> 4;
+    for (int i = threadIdx.x; i < (groups - first_group) * hd; i += kAppendThreads) {
+      const int d = i % hd, grp = first_group + i / hd;
+      u32x4* at = reinterpret_cast<u32x4*>(codes + d * bs + 16 * grp);
+      u32x4 v;
+      if (16 * grp >= it.place && 16 * grp + 16 <= end) {
+        v = *reinterpret_cast<const u32x4*>(&s_v[d * words + 4 * grp]);
+      } else if (!moved) {
+        // what is there stays: only the new bytes are written
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int p = 16 * grp + 4 * w;
+          const uint32_t fresh = s_v[d * words + 4 * grp + w];
+          if (p >= it.place && p + 4 <= end) {
+            reinterpret_cast<uint32_t*>(at)[w] = fresh;
+          } else {
+            for (int b = max(0, it.place - p); b < min(4, end - p); ++b) {
+              reinterpret_cast<int8_t*>(at)[4 * w + b] = static_cast<int8_t>(code_at(fresh, b));
+            }
+          }
+        }
+        continue;
+      } else {
+        v = *at;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int p = 16 * grp + 4 * w;  // the word's first place
+          const uint32_t fresh = bytes_in(it.place - p, end - p), held = bytes_in(0, it.place - p);
+          uint32_t x2 = v[w];
+          if (held) x2 = (follow4(x2, ratio) & held) | (x2 & ~held);
+          if (fresh) x2 = (s_v[d * words + 4 * grp + w] & fresh) | (x2 & ~fresh);
+          v[w] = x2;
+        }
+      }
+      *at = v;
+    }
+  }
+  if (threadIdx.x == 0) *work.scale = scale;
+}
+
+// Inputs whose rows are not 16-byte aligned.
+template <class T>
+__global__ __launch_bounds__(kAppendThreads) void append_any_kernel(AppendArgs a) {
+  AppendWork<T> work;
+  if (append_work(a, &work)) append_values(a, work);
 }
 
 // ------------------------------------------------------------------- read
@@ -622,28 +903,168 @@ struct ReadArgs {
   uint64_t rows, blocks;
 };
 
+// A run of rows inside one group of 16 places: `rows` from output row `row`
+// on, the first at place `place` (of the group) of `cell` (-1: no block).
+struct ReadJob {
+  int32_t row, rows, block, place;
+  float scale[2];
+};
+
+constexpr int kReadRows = 64, kReadBatch = 8;
+
+// Values of codes w, as many as fill 16 bytes of T.
+template <class T>
+__device__ inline void put(typename T::store* out, u32x2 w, float scale) {
+  if constexpr (T::code == kF32) {
+    f32x4 v;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) v[b] = static_cast<float>(code_at(w[0], b)) * scale;
+    __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(out));
+  } else {
+    u32x4 v;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t word = w[b / 2];
+      const uint32_t lo = T::put(static_cast<float>(code_at(word, 2 * (b & 1))) * scale);
+      const uint32_t hi = T::put(static_cast<float>(code_at(word, 2 * (b & 1) + 1)) * scale);
+      v[b] = lo | (hi << 16);
+    }
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out));
+  }
+}
+
+template <class T>
+__device__ inline u32x2 codes_for(const int8_t* p) {
+  if constexpr (T::code == kF32) return u32x2{*reinterpret_cast<const uint32_t*>(p), 0u};
+  else return *reinterpret_cast<const u32x2*>(p);
+}
+
+// One block per 64 output rows and kv head: the rows that begin a group of 16
+// places become jobs (a request's rows follow each other, so there are 4 or
+// 5 of them unless requests are tiny).  A thread writes 16 bytes, its wave 1 KiB.
+// A value column's 16 places are one 16-byte load; they turn through LDS.
 template <class T>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
-  const uint64_t row = blockIdx.x;
-  const int kv = blockIdx.y;
-  if (!a.out[kv]) return;
-  const int bs = 1 << a.block_log2, hd = a.head_dim;
-  const int r = upper(a.cu, a.requests, static_cast<int>(row));
-  const int pos = a.starts[r] + static_cast<int>(row) - a.cu[r];
-  const int j = pos >> a.block_log2, p = pos & (bs - 1);
-  const int block = pos >= 0 && j < a.width ? a.table[static_cast<size_t>(r) * a.width + j] : -1;
-  const bool there = block >= 0 && static_cast<uint64_t>(block) < a.blocks;
-  typename T::store* out = static_cast<typename T::store*>(a.out[kv]) + row * a.kv_heads * hd;
-  for (int i = threadIdx.x; i < a.kv_heads * hd; i += 256) {
-    const int g = i / hd, d = i % hd;
-    float v = 0.0f;
-    if (there) {
-      const size_t cell = static_cast<size_t>(block) * a.kv_heads + g;
-      v = static_cast<float>(a.codes[kv][cell * bs * hd + (kv ? d * bs + p : p * hd + d)]) *
-          a.scales[kv][cell];
+  const int bs = 1 << a.block_log2, hd = a.head_dim, g = blockIdx.y;
+  const uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * kReadRows;
+  __shared__ ReadJob s_job[kReadRows];
+  __shared__ int s_jobs;
+  __shared__ __align__(16) int8_t s_v[kReadBatch * 16 * 256];
+  __shared__ int s_cu[kWave];
+  if (threadIdx.x < kWave) {
+    const int row = static_cast<int>(row0) + static_cast<int>(threadIdx.x);
+    const int r0 = find_unit(a.cu, a.requests, static_cast<int>(row0));
+    const int next = r0 + 1 + static_cast<int>(threadIdx.x);
+    s_cu[threadIdx.x] = next < a.requests ? a.cu[next] : 0x7fffffff;
+    __builtin_amdgcn_wave_barrier();
+    bool begins = false;
+    ReadJob job{row, 0, -1, 0, {0.0f, 0.0f}};
+    if (static_cast<uint64_t>(row) < a.rows) {
+      // the requests of the block's rows follow each other: 64 sums are looked
+      // at in LDS, and all of them only where more end here
+      int r = r0 + (s_cu[0] <= row ? 1 + upper(s_cu, kWave, row) : 0);
+      if (r >= r0 + kWave) r = r0 + kWave + upper(a.cu + r0 + kWave, a.requests - r0 - kWave, row);
+      const int from = a.cu[r], to = min(a.cu[r + 1], static_cast<int>(a.rows));
+      const int pos = a.starts[r] + row - from, j = pos >> a.block_log2;
+      begins = row == from || (pos & 15) == 0;
+      job.place = pos & (bs - 1);
+      job.rows = min(16 - (pos & 15), to - row);
+      if (pos >= 0 && j < a.width) {
+        const int block = a.table[static_cast<size_t>(r) * a.width + j];
+        if (static_cast<uint64_t>(static_cast<int64_t>(block)) < a.blocks) {
+          job.block = block;
+          const size_t cell = static_cast<size_t>(block) * a.kv_heads + g;
+          job.scale[0] = a.scales[0][cell];
+          job.scale[1] = a.scales[1][cell];
+        }
+      }
     }
-    out[i] = T::put(v);
+    const uint64_t all = __ballot(begins);
+    if (begins) s_job[__popcll(all & ((1ull << threadIdx.x) - 1ull))] = job;
+    if (threadIdx.x == 0) s_jobs = __popcll(all);
   }
+  __syncthreads();
+  constexpr int kPer = 16 / sizeof(typename T::store);  // values a thread writes
+  const int jobs = s_jobs, chunks = hd / kPer;
+  auto out_at = [&](int kv, int row, int d) {
+    return static_cast<typename T::store*>(a.out[kv]) +
+           (static_cast<size_t>(row) * a.kv_heads + g) * hd + d;
+  };
+  for (int first = 0; first < jobs; first += kReadBatch) {
+    const int n = min(kReadBatch, jobs - first);
+    if (a.out[1]) {
+      for (int i0 = threadIdx.x; i0 < n * hd; i0 += 4 * 256) {
+        u32x4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * 256, d = i % hd, k = i / hd;
+          w[u] = u32x4{0u, 0u, 0u, 0u};
+          if (k < n && s_job[first + k].block >= 0) {
+            const ReadJob& job = s_job[first + k];
+            const size_t cell = static_cast<size_t>(job.block) * a.kv_heads + g;
+            w[u] = *reinterpret_cast<const u32x4*>(a.codes[1] + cell * bs * hd +
+                                                   static_cast<size_t>(d) * bs + (job.place & ~15));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * 256, d = i % hd, k = i / hd;
+          if (k < n) {
+#pragma unroll
+            for (int b = 0; b < 16; ++b) {
+              s_v[(k * 16 + b) * hd + d] = static_cast<int8_t>(code_at(w[u][b / 4], b % 4));
+            }
+          }
+        }
+      }
+    }
+    if (a.out[0]) {
+      // four pieces at a time, so that their loads do not wait for each other
+      for (int i0 = threadIdx.x; i0 < n * 16 * chunks; i0 += 4 * 256) {
+        u32x2 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * 256;
+          const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
+          w[u] = u32x2{0u, 0u};
+          if (k < n && b < s_job[first + k].rows && s_job[first + k].block >= 0) {
+            const ReadJob& job = s_job[first + k];
+            const size_t cell = static_cast<size_t>(job.block) * a.kv_heads + g;
+            w[u] = codes_for<T>(a.codes[0] + (cell * bs + job.place + b) * hd + d);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * 256;
+          const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
+          if (k < n && b < s_job[first + k].rows) {
+            put<T>(out_at(0, s_job[first + k].row + b, d), w[u], s_job[first + k].scale[0]);
+          }
+        }
+      }
+    }
+    if (a.out[1]) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n * 16 * chunks; i += 256) {
+        const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
+        const ReadJob& job = s_job[first + k];
+        if (b >= job.rows) continue;
+        put<T>(out_at(1, job.row + b, d),
+               codes_for<T>(&s_v[(k * 16 + (job.place & 15) + b) * hd + d]), job.scale[1]);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+template <class T>
+static void launch_append(const AppendArgs& a, unsigned items, bool aligned, hipStream_t s) {
+  const dim3 grid(items, static_cast<unsigned>(a.kv_heads), 2);
+  const int values = a.head_dim << a.block_log2;  // of a block
+  if (!aligned) append_any_kernel<T><<<grid, kAppendThreads, 0, s>>>(a);
+  else if (values <= 32 * kAppendThreads) append_kernel<T, 1><<<grid, kAppendThreads, 0, s>>>(a);
+  else if (values <= 64 * kAppendThreads) append_kernel<T, 2><<<grid, kAppendThreads, 0, s>>>(a);
+  else append_kernel<T, 4><<<grid, kAppendThreads, 0, s>>>(a);
 }
 
 static int log2_of(int n) { return n == 16 ? 4 : n == 32 ? 5 : n == 64 ? 6 : 7; }
@@ -695,6 +1116,7 @@ extern "C" int grm_hip_kv_plan(const grm_kv_batch_desc* b, void* stream) {
   a.block_log2 = log2_of(b->block_tokens);
   a.cap_append = static_cast<int32_t>(l.cap_append);
   a.cap_units = static_cast<int32_t>(l.cap_units);
+  a.cap_wide = static_cast<int32_t>(l.cap_wide);
   a.cap_items = static_cast<int32_t>(l.cap_items);
   a.cap_joins = static_cast<int32_t>(l.cap_joins);
   a.cap_parts = static_cast<int32_t>(l.cap_parts);
@@ -703,9 +1125,10 @@ extern "C" int grm_hip_kv_plan(const grm_kv_batch_desc* b, void* stream) {
   a.at_tiles = l.at_tiles;
   for (int k = 0; k < 2; ++k) {
     a.runs[k] = l.runs[k];
-    a.at_runs[k] = l.at_runs[k];
+    a.at_run_units[k] = l.at_run_units[k];
   }
   a.at_scan = l.at_scan;
+  a.at_wide = l.at_wide;
   a.at_items = l.at_items;
   a.at_joins = l.at_joins;
   const unsigned blocks = 1u + static_cast<unsigned>((b->tokens + kPlanTokens - 1) / kPlanTokens);
@@ -749,11 +1172,15 @@ extern "C" int grm_hip_kv_append(const grm_kv_cache_desc* c, const grm_kv_batch_
   a.block_log2 = log2_of(c->block_tokens);
   a.rows = b->tokens;
   a.blocks = c->blocks;
-  const dim3 grid(static_cast<unsigned>(l.cap_append), static_cast<unsigned>(c->kv_heads), 2);
+  const int64_t unit = dtype == grm::kF32 ? 4 : 8;
+  const bool aligned = aligned16(k) && aligned16(v) && k_token_stride % unit == 0 &&
+                       k_head_stride % unit == 0 && v_token_stride % unit == 0 &&
+                       v_head_stride % unit == 0;
+  const auto items = static_cast<unsigned>(l.cap_append);
   const auto s = static_cast<hipStream_t>(stream);
-  if (dtype == grm::kF32) append_kernel<F32><<<grid, kAppendThreads, 0, s>>>(a);
-  else if (dtype == grm::kBF16) append_kernel<BF16><<<grid, kAppendThreads, 0, s>>>(a);
-  else append_kernel<F16><<<grid, kAppendThreads, 0, s>>>(a);
+  if (dtype == grm::kF32) launch_append<F32>(a, items, aligned, s);
+  else if (dtype == grm::kBF16) launch_append<BF16>(a, items, aligned, s);
+  else launch_append<F16>(a, items, aligned, s);
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();
   return 0;
@@ -795,7 +1222,8 @@ extern "C" int grm_hip_kv_read(const grm_kv_cache_desc* c, const int32_t* block_
   a.block_log2 = log2_of(c->block_tokens);
   a.rows = rows;
   a.blocks = c->blocks;
-  const dim3 grid(static_cast<unsigned>(rows), 2);
+  const dim3 grid(static_cast<unsigned>((rows + kReadRows - 1) / kReadRows),
+                  static_cast<unsigned>(c->kv_heads));
   const auto s = static_cast<hipStream_t>(stream);
   if (dtype == grm::kF32) read_kernel<F32><<<grid, 256, 0, s>>>(a);
   else if (dtype == grm::kBF16) read_kernel<BF16><<<grid, 256, 0, s>>>(a);

@@ -41,17 +41,6 @@ struct NarrowUnit {
   int32_t ctx, pad[3];
 };
 
-// Where a wavefront of the narrow kernel begins: its run [begin, stop) of all
-// narrow tiles in order, its block's [block_begin, block_stop), and the unit
-// of the first tile (index, its tiles [first, end), the unit itself).
-struct NarrowRun {
-  int32_t begin, stop, block_begin, block_stop;
-  int32_t at, first, end, request;
-  int32_t row, tokens, tile_lo, ctx;
-  int32_t pad[4];
-};
-static_assert(sizeof(NarrowRun) == 64, "one line");
-
 // Key tokens to a tile of the narrow kernel: both halves of a 128-token
 // block's value lines, else the least that fills its loads.
 __host__ __device__ constexpr int narrow_tile(int block_tokens) {
@@ -63,20 +52,29 @@ inline int narrow_runs(int cus, int kv_heads, int per_cu) {
   return 4 * std::max(1, per_cu * cus / kv_heads);
 }
 
-// First tile of run r of `runs`, `tiles` in all; equal to within one.
-__host__ __device__ inline int run_begin(int tiles, int runs, int r) {
-  const int used = runs < tiles ? runs : tiles;
-  if (r >= used) return tiles;
-  return static_cast<int>(static_cast<uint64_t>(tiles) * static_cast<uint32_t>(r) /
-                          static_cast<uint32_t>(used));
-}
+// Tiles dealt to runs, equal to within one: the first `rem` of the `used`
+// runs have `each` + 1 tiles.
+struct Deal {
+  int tiles, used, each, rem;
+  __host__ __device__ Deal(int tiles_, int runs)
+      : tiles(tiles_), used(runs < tiles_ ? runs : tiles_),
+        each(used ? tiles_ / used : 0), rem(used ? tiles_ % used : 0) {}
+  // First tile of run r.
+  __host__ __device__ int begin(int r) const {
+    return r >= used ? tiles : r * each + (r < rem ? r : rem);
+  }
+  // The run that tile t lies in.
+  __host__ __device__ int run(int t) const {
+    const int more = rem * (each + 1);
+    return t < more ? t / (each + 1) : rem + (t - more) / each;
+  }
+};
 
-// The run that tile t lies in.
-__device__ inline int run_of(int tiles, int runs, int t) {
-  const int used = runs < tiles ? runs : tiles;
-  return static_cast<int>((static_cast<uint64_t>(t + 1) * static_cast<uint32_t>(used) - 1) /
-                          static_cast<uint32_t>(tiles));
-}
+// A wide unit while the plan cuts it: tokens from t0 on of a request, key
+// tiles [lo, hi).
+struct WideUnit {
+  int32_t request, t0, lo, hi;
+};
 
 // One wide item: query rows [row, row + tokens) of a request against key
 // tiles [tile_lo, tile_hi); the first of them has position `pos`.  part:
@@ -91,14 +89,22 @@ struct WideJoin {
   int32_t row, tokens, part, parts;
 };
 
+// What the plan wrote, as memory that no kernel running beside this one
+// changes: scalar loads where the address is uniform.
+typedef const __attribute__((address_space(4))) SchedHead* ConstHead;
+typedef const __attribute__((address_space(4))) AppendItem* ConstAppend;
+typedef const __attribute__((address_space(4))) NarrowUnit* ConstUnit;
+typedef const __attribute__((address_space(4))) WideItem* ConstItem;
+typedef const __attribute__((address_space(4))) int32_t* ConstInt;
+
 // Sizes and places of the schedule, from host-known fields alone.
 struct Layout {
   int group;          // query heads to a kv head
   int wide_tokens;    // tokens to a wide unit (0: no wide units)
   int wide_blocks;    // wide blocks that run at once, per kv head
-  uint64_t cap_append, cap_units, cap_items, cap_joins, cap_parts;
+  uint64_t cap_append, cap_units, cap_wide, cap_items, cap_joins, cap_parts;
   int runs[2];        // of the narrow kernel, with one and two blocks to a CU
-  uint64_t at_append, at_units, at_tiles, at_runs[2], at_scan, at_items, at_joins, bytes;
+  uint64_t at_append, at_units, at_tiles, at_run_units[2], at_scan, at_wide, at_items, at_joins, bytes;
 };
 
 int device_cus(int* out);
@@ -152,6 +158,23 @@ __device__ inline int clamp_len(int v) { return v < 0 ? 0 : (v > kMaxLen ? kMaxL
 
 __device__ inline int code_at(uint32_t word, int byte) {
   return static_cast<int>(static_cast<int8_t>((word >> (8 * byte)) & 0xffu));
+}
+
+// The last unit whose first tile is not past t (wave-uniform; first tiles
+// ascend).  64 entries a step.
+template <class P>
+__device__ inline int find_unit(P first, int n, int t) {
+  const int lane = __lane_id();
+  int lo = 0;
+  while (true) {
+    const int step = (n + kWave - 1) / kWave;
+    const int at = lane * step;
+    const bool le = at < n && first[lo + at] <= t;
+    const int k = __popcll(__ballot(le)) - 1;
+    lo += k * step;
+    if (step == 1) return lo;
+    n = min(step, n - k * step);
+  }
 }
 
 }  // namespace kv

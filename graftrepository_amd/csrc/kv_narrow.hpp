@@ -52,30 +52,6 @@
 namespace grm {
 namespace kv {
 
-// What the plan wrote, as memory that no kernel running beside this one
-// changes: scalar loads where the address is uniform.
-typedef const __attribute__((address_space(4))) SchedHead* ConstHead;
-typedef const __attribute__((address_space(4))) NarrowUnit* ConstUnit;
-typedef const __attribute__((address_space(4))) NarrowRun* ConstRun;
-typedef const __attribute__((address_space(4))) int32_t* ConstInt;
-
-// The last unit whose first tile is not past t (wave-uniform; first tiles
-// ascend).  64 entries a step.
-template <class P>
-__device__ inline int find_unit(P first, int n, int t) {
-  const int lane = __lane_id();
-  int lo = 0;
-  while (true) {
-    const int step = (n + kWave - 1) / kWave;
-    const int at = lane * step;
-    const bool le = at < n && first[lo + at] <= t;
-    const int k = __popcll(__ballot(le)) - 1;
-    lo += k * step;
-    if (step == 1) return lo;
-    n = min(step, n - k * step);
-  }
-}
-
 // The kernel's arguments, read again where they are used: kept in scalar
 // registers through the loop, those of a unit's begin and end would push out
 // the loop's own.
@@ -152,10 +128,13 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   const auto* first = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) + a.at_tiles);
   const auto* table = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.table));
   const int run = 4 * blockIdx.y + wave, runs = 4 * gridDim.y;
-  const auto* mine_at =
-      reinterpret_cast<ConstRun>(reinterpret_cast<uintptr_t>(a.work) + a.at_runs) + run;
-  const int begin = mine_at->begin, end = mine_at->stop;
-  const int block_begin = mine_at->block_begin, block_end = mine_at->block_stop;
+  const int start_unit = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) +
+                                                    a.at_run_units)[run];
+  const Deal deal(reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work))->narrow_tiles,
+                  runs);
+  const int begin = deal.begin(run), end = deal.begin(run + 1);
+  const int block_begin = deal.begin(4 * blockIdx.y);
+  const int block_end = deal.begin(4 * blockIdx.y + 4);
   if (block_begin >= block_end) return;
   const int bs = 1 << a.block_log2;
   const uint32_t cell_bytes = static_cast<uint32_t>(bs * D);
@@ -264,8 +243,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   UnitView now{};
   bool spans = false;
   if (begin < end) {
-    now = {mine_at->at,  mine_at->first,  mine_at->end,     mine_at->request,
-           mine_at->row, mine_at->tokens, mine_at->tile_lo, mine_at->ctx};
+    now = unit_at(start_unit);
     spans = now.first <= block_begin && now.end >= block_end;
     UnitView ahead = now;  // the unit of the tile whose blocks were asked for last
     Half cur[H], nxt[H];
@@ -583,30 +561,30 @@ __global__ __launch_bounds__(256) void join_narrow_kernel(AttendArgs a, int runs
   const NarrowUnit* units = reinterpret_cast<const NarrowUnit*>(a.work + a.at_units);
   const int32_t* first = reinterpret_cast<const int32_t*>(a.work + a.at_tiles);
   const int total = head->narrow_tiles, n_units = head->units;
+  const Deal deal(total, runs);
   int at = blockIdx.y;
   if (by_unit) {
     if (at >= n_units) return;
   } else {
-    const int t = run_begin(total, runs, blockIdx.y + 1);
+    const int t = deal.begin(blockIdx.y + 1);
     if (t >= total) return;
     at = find_unit(first, n_units, t);
     // not cut here, or cut before
-    if (first[at] >= t || first[at] < run_begin(total, runs, blockIdx.y)) return;
+    if (first[at] >= t || first[at] < deal.begin(blockIdx.y)) return;
   }
   const int from = first[at], to = first[at + 1];
   const NarrowUnit u = units[at];
   if (to <= from || c >= u.tokens * a.group) return;
-  const int r0 = run_of(total, runs, from), r1 = run_of(total, runs, to - 1);
+  const int r0 = deal.run(from), r1 = deal.run(to - 1);
   if (r0 == r1) return;
-  const NarrowRun* run = reinterpret_cast<const NarrowRun*>(a.work + a.at_runs);
   // One block held all of it: finished there.
-  if (run[r0].block_begin == from && run[r0].block_stop == to) return;
+  if (deal.begin(r0 / 4 * 4) == from && deal.begin(r0 / 4 * 4 + 4) == to) return;
   // Parts in order: a whole block's, or a run's.
   auto part_of = [&](int r) -> const float* {
-    const NarrowRun& n = run[r];
-    const bool whole = from <= n.block_begin && to >= n.block_stop;
+    const bool whole = from <= deal.begin(r / 4 * 4) && to >= deal.begin(r / 4 * 4 + 4);
     if (whole && r % 4) return nullptr;
-    return a.parts + narrow_part(g, runs, r, from > n.begin ? 1 : 0) * (kNarrowCols * (D + 2));
+    return a.parts +
+           narrow_part(g, runs, r, from > deal.begin(r) ? 1 : 0) * (kNarrowCols * (D + 2));
   };
   __shared__ float s_top[4];
   __shared__ float s_l[kGroups];

@@ -30,7 +30,7 @@
 namespace grm {
 namespace kv {
 
-typedef const __attribute__((address_space(4))) WideItem* ConstItem;
+
 
 // Blocks to a CU: registers (accumulators of 32 columns, twice for fp32) and
 // the two LDS buffers.

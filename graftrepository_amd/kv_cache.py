@@ -54,6 +54,7 @@ _NUMPY = {"f32": np.float32, "bf16": np.uint16, "f16": np.float16, "i8": np.int8
           "i32": np.int32, "i64": np.int64, "u8": np.uint8}
 _NAMES = {np.dtype(v): k for k, v in _NUMPY.items()}
 _TORCH: dict[str, object] = {}
+_FLOATS: dict[object, str] = {}   # torch's floating types, once torch is there
 
 
 def _torch_names() -> dict[str, object]:
@@ -62,6 +63,7 @@ def _torch_names() -> dict[str, object]:
         pairs = {"f32": t.float32, "bf16": t.bfloat16, "f16": t.float16, "i8": t.int8,
                  "i32": t.int32, "i64": t.int64, "u8": t.uint8}
         _NAMES.update({v: k for k, v in pairs.items()})
+        _FLOATS.update({pairs[k]: k for k in ("f32", "bf16", "f16")})
         _TORCH.update(pairs)
     return _TORCH
 
@@ -121,6 +123,10 @@ def _strides(a) -> tuple[int, ...]:
 def _rows(a, what: str, shape) -> tuple[int, str, int, int]:
     """(address, type, row stride, head stride) of [rows, heads, dim] values
     whose last axis is contiguous."""
+    if _FLOATS and _FLOATS.get(getattr(a, "dtype", None)) and a.is_cuda and a.shape == shape:
+        st = a.stride()
+        if st[2] == 1:  # the usual call, on its short way
+            return a.data_ptr(), _FLOATS[a.dtype], st[0], st[1]
     name = _type(a, what)
     if name not in ("f32", "bf16", "f16"):
         raise ValueError(f"{what} must be f32, bf16 or f16, got {a.dtype}")
@@ -138,12 +144,20 @@ def _empty(like, shape, dtype: str):
     return DeviceArray(shape, _NUMPY[dtype])
 
 
+_raw_stream = None  # torch's current stream of a device as a handle
+
+
 def _stream(a, stream) -> int:
+    global _raw_stream
     if stream is not None:
         return int(getattr(stream, "cuda_stream", stream))
-    if _is_torch(a):
-        return sys.modules["torch"].cuda.current_stream(a.device).cuda_stream
-    return 0
+    if not _is_torch(a):
+        return 0
+    if _raw_stream is None:
+        t = sys.modules["torch"]
+        _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: t.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(a.get_device())
 
 
 class KvBatch:
@@ -200,7 +214,7 @@ class KvBatch:
             d.free_head_out = self.free_head_out.data_ptr()
         self._ref = ctypes.byref(d)
         self._scratch: dict[int, int] = {}
-        self._held = None
+        self._held: dict[int, object] = {}
         self._planned = False
 
     def plan(self, stream=None) -> "KvBatch":
@@ -211,6 +225,14 @@ class KvBatch:
             _lib.check(rc, "kv plan")
         self._planned = True
         return self
+
+    def _scratch_on(self, like, need: int, stream: int) -> int:
+        """Scratch of a call, one per stream: calls on one stream follow each
+        other and may share it."""
+        held = self._held.get(stream)
+        if held is None or held.nbytes < need:
+            held = self._held[stream] = _empty(like, (need,), "u8")
+        return held.data_ptr()
 
     def _need_plan(self):
         if not self._planned:
@@ -287,34 +309,28 @@ class KvCache:
         qp, name, qt, qh = _rows(q, "q", shape)
         if out is None:
             out = _empty(q, shape, name)
-        op, oname, ot, oh = _rows(out, "out", shape)
-        if oname != name:
-            raise ValueError("out must have q's type")
+            op, ot, oh = out.data_ptr(), shape[1] * shape[2], shape[2]
+        else:
+            op, oname, ot, oh = _rows(out, "out", shape)
+            if oname != name:
+                raise ValueError("out must have q's type")
         if lse is None and return_lse:
             lse = _empty(q, shape[:2], "f32")
-        lp = _dense(lse, "lse", "f32", shape[:2]) if lse is not None else None
+            lp = lse.data_ptr()
+        else:
+            lp = _dense(lse, "lse", "f32", shape[:2]) if lse is not None else None
         need = batch._scratch.get(self.head_dim)
         if need is None:
             got = u64()
             _lib.check(self._lib.grm_hip_kv_attend_bytes(self._ref, batch._ref,
                                                          ctypes.byref(got)), "kv scratch size")
             need = batch._scratch[self.head_dim] = got.value
-        scratch = None
-        if need:
-            if _is_torch(q):
-                # from torch's pool, on the call's stream: the caller may use
-                # one batch on several streams
-                scratch = _empty(q, (need,), "u8")
-            else:
-                if batch._held is None or batch._held.nbytes < need:
-                    batch._held = DeviceArray((need,), np.uint8)
-                scratch = batch._held
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(self.head_dim)
+        on = _stream(q, stream)
         rc = self._lib.grm_hip_kv_attend(
             self._ref, batch._ref, qp, _lib.DTYPE_CODES[name], qt, qh, op, ot, oh, lp,
-            softmax_scale, scratch.data_ptr() if scratch is not None else None, need,
-            _stream(q, stream))
+            softmax_scale, batch._scratch_on(q, need, on) if need else None, need, on)
         if rc:
             _lib.check(rc, "kv attend")
         return (out, lse) if return_lse else out
