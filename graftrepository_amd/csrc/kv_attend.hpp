@@ -62,6 +62,14 @@ __device__ inline void codes_to_f16(u32x4 w, f16x8 (&out)[2]) {
   }
 }
 
+// A product as fp32 holds it.  Left open, the compiler rounds it to fp16 from
+// its exact value in one place and from fp32 in another, and where the two
+// differ the rest that is taken of one is a unit off the other.
+__device__ inline float as_rounded(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
 template <class T>
 __device__ inline void load8(const typename T::store* p, float (&x)[8]) {
   if constexpr (T::code == kF32) {

@@ -413,6 +413,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
               p[e] = __builtin_amdgcn_exp2f(fmaf(sc, mul[h], shift));
               float v = p[e] * v_factor[h];
               if constexpr (decltype(some_hidden)::value) v = sc == -INFINITY ? 0.0f : v;
+              if constexpr (State::kRest) v = as_rounded(v);
               w[h][k][e] = static_cast<_Float16>(v);
               if constexpr (State::kRest) {
                 w_rest[h][k][e] =

@@ -25,17 +25,24 @@
 // with 8 kv heads an XCD's L2 serves one of them.
 #pragma once
 
+#include <type_traits>
+
 #include "kv_narrow.hpp"
 
 namespace grm {
 namespace kv {
 
 
+// Columns of a wavefront.  32 read a tile half as often from LDS as 16; 16
+// need half the registers, and are taken where 32 would fill more than a
+// half of a SIMD's, with one wavefront that nothing covers (attend of 1021
+// tokens on 14011, head_dim 256 in fp16: OLD us with 32, NEW with 16).
+__host__ __device__ constexpr int wide_wave_cols(int dtype, int head_dim) {
+  return head_dim == 256 || (dtype == kF32 && head_dim == 128) ? 16 : 32;
+}
 
-// Blocks to a CU: registers (accumulators of 32 columns, twice for fp32) and
-// the two LDS buffers.
-__host__ __device__ constexpr int wide_blocks_per_cu(int dtype, int head_dim) {
-  return head_dim == 256 || (dtype == kF32 && head_dim == 128) ? 1 : 2;
+__host__ __device__ constexpr int wide_threads(int dtype, int head_dim) {
+  return kWideCols / wide_wave_cols(dtype, head_dim) * kWave;
 }
 
 // Floats of one partial result: 128 columns, and their maxima and sums.
@@ -43,22 +50,60 @@ __host__ __device__ constexpr int wide_part_floats(int head_dim) {
   return kWideCols * (head_dim + 2);
 }
 
+// Scales of 16 tokens, 0 where they have no block or none of the item's
+// columns sees them.
+struct __align__(16) GroupScale {
+  float k, v;
+  int there, pad;
+};
+
+// A value joined over the lanes of a column.
+template <int W, class F>
+__device__ inline float across(float v, F join) {
+#pragma unroll
+  for (int by = W; by < kWave; by *= 2) v = join(v, __shfl_xor(v, by));
+  return v;
+}
+
+__device__ inline f32x16 wide_mul(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x4 wide_mul(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// The order of a product's reads from LDS and matrix instructions (MULS for
+// each of READS reads): reads run kAhead before what needs them.
+template <int READS, int MULS>
+__device__ inline void feed() {
+  constexpr int kAhead = 6, kMul = 0x8, kRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMul, MULS, 0);
+    if (i + kAhead < READS) __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+  }
+}
+
 template <class T, int D>
-__global__ __launch_bounds__(256, wide_blocks_per_cu(T::code, D)) void attend_wide_kernel(
-    AttendArgs a) {
+__global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kernel(AttendArgs a) {
   typedef NarrowState<T, D> State;  // its constants: terms and allowances
-  constexpr int kSteps = D / 16;    // of the first product
-  constexpr int kTilesD = D / 32;   // value row tiles
-  constexpr int kChunks = D / 64;   // 16-byte chunks of keys, and of values, to a thread
+  constexpr int W = wide_wave_cols(T::code, D);
+  constexpr int kWaves = kWideCols / W, kLanes = kWave / W;  // lanes of a column
+  constexpr int kStepD = 8 * kLanes, kSteps = D / kStepD;    // of the first product
+  constexpr int kTilesD = D / W;                             // value row tiles
+  constexpr int kLoads = 16 * D * 4 / (kWaves * kWave * 16);  // 16 bytes of keys to a lane
+  constexpr int kPer = W / 2, kHalves = 32 / W;  // scores, accumulators of 32 keys to a lane
+  constexpr int kAcc = W * W / kWave;
+  typedef typename std::conditional<W == 32, f32x16, f32x4>::type Acc;
   const int g = blockIdx.x;
   const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
   if (static_cast<int>(blockIdx.y) >= head->items) return;
   const auto* item = reinterpret_cast<ConstItem>(reinterpret_cast<uintptr_t>(a.work) + a.at_items) +
                      blockIdx.y;
   if (item->tokens <= 0) return;
-  const auto* table = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.table));
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int c = lane & 31, h = lane >> 5;
+  const int c = lane % W, h = lane / W;
   const int tile_lo = item->tile_lo, tile_hi = item->tile_hi;
   const int first_pos = item->pos, last_pos = first_pos + item->tokens - 1;
   const int cols = item->tokens * a.group;
@@ -66,176 +111,194 @@ __global__ __launch_bounds__(256, wide_blocks_per_cu(T::code, D)) void attend_wi
   const int bs = 1 << a.block_log2;
   const uint32_t cell_bytes = static_cast<uint32_t>(bs * D);
 
-  __shared__ f16x8 s_k[2][2 * kSteps * kWave];       // [row tile][step][lane]
-  __shared__ f16x8 s_v[2][kTilesD * 4 * kWave];      // [d tile][row tile][half][lane]
-  __shared__ float s_scale[2][2][4];                 // [keys, values][group of 16]
+  // a lane's eight values of the instruction's operand
+  __shared__ f16x8 s_k[2][2 * kHalves * kSteps * kWave];  // [row tile][step][lane]
+  __shared__ f16x8 s_v[2][kTilesD * 2 * kPer / 8 * kWave];  // [d tile][32 keys][lane]
+  __shared__ GroupScale s_scale[2][4];                      // of a group of 16 tokens
 
-  // ---- codes of a tile to registers
-  u32x4 k_reg[kChunks], v_reg[kChunks];
-  float scale_reg = 0.0f;
-  int seen_reg = 0;  // groups whose block is there, as bits
-  auto load_codes = [&](int tile) {
-    const int first_seen = a.window > 0 ? max(0, first_pos + 1 - a.window) : 0;
-    int id[4], seen = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int key = tile * kTile + 16 * k, at = key >> a.block_log2;
-      const int raw = table[table_row + max(0, min(at, a.width - 1))];
-      const bool there = key <= last_pos && key + 15 >= first_seen && at < a.width &&
-                         static_cast<uint32_t>(raw) < a.blocks;
-      id[k] = there ? raw : 0;
-      seen |= there ? 1 << k : 0;
-    }
-    seen_reg = seen;
-    auto cell_of = [&](int k) {
-      const int lo = k & 1 ? id[1] : id[0], hi = k & 1 ? id[3] : id[2];
-      return static_cast<uint32_t>(k & 2 ? hi : lo) * a.kv_heads + g;
-    };
-    // Keys: lane = 8 tokens x 8 chunks of a wave's group.
-#pragma unroll
-    for (int q = 0; q < kChunks; ++q) {
-      const int n = q * 256 + static_cast<int>(threadIdx.x);
-      const int t8 = n & 7, chunk = (n >> 3) % kSteps, grp = (n >> 3) / kSteps;
-      const int key = 32 * (grp >> 2) + 16 * (t8 >> 2) + 4 * (grp & 3) + (t8 & 3);
-      const int8_t* p = a.k_codes + static_cast<uint64_t>(cell_of(key >> 4)) * cell_bytes +
-                        ((tile * kTile + key) & (bs - 1)) * D + 16 * chunk;
-      k_reg[q] = *reinterpret_cast<const u32x4*>(p);
-    }
-    // Values: a wave's 16 tokens, a value column per lane.
-#pragma unroll
-    for (int q = 0; q < kChunks; ++q) {
-      const int8_t* p = a.v_codes + static_cast<uint64_t>(cell_of(wave)) * cell_bytes +
-                        static_cast<size_t>(q * kWave + lane) * bs +
-                        ((tile * kTile + 16 * wave) & (bs - 1));
-      v_reg[q] = *reinterpret_cast<const u32x4*>(p);
-    }
-    if (threadIdx.x < 8) {
-      const int k = threadIdx.x & 3;
-      const uint32_t cell = cell_of(k);
-      scale_reg = seen >> k & 1 ? (threadIdx.x < 4 ? a.k_scales[cell] : a.v_scales[cell]) : 0.0f;
-    }
+  // ---- codes of a tile to registers: a wavefront (or two) loads 16 of its
+  // tokens, which lie in one block, so that addresses are a scalar base and a
+  // lane's fixed offset.  The block's id is loaded a tile ahead.
+  const int grp = wave * 4 / kWaves, part_of = wave % (kWaves / 4);
+  u32x4 k_reg[kLoads], v_reg[kLoads];
+  float k_scale_reg, v_scale_reg;
+  int raw_id, there_reg;
+  const int first_seen = a.window > 0 ? max(0, first_pos + 1 - a.window) : 0;
+  // Keys: 8 tokens by 8 chunks of 16 values to a load (of 32 columns and
+  // head_dim 64, 16 tokens by 4); with two wavefronts the second has the
+  // tokens of the other row tile.
+  constexpr int kChunks = D / 16;
+  const int token = W == 32 ? (lane & 7) + (lane >> 3) / kChunks * 8
+                            : (lane & 3) + 2 * (lane & 4) + 4 * part_of;
+  const uint32_t k_at = static_cast<uint32_t>(token * D + (lane >> 3) % kChunks * 16);
+  const uint32_t v_at = static_cast<uint32_t>((part_of * (D / 2) + lane) * bs);
+  auto load_id = [&](int tile) {
+    const int at = (tile * kTile + 16 * grp) >> a.block_log2;
+    raw_id = a.table[table_row + max(0, min(at, a.width - 1))];
   };
+  auto load_codes = [&](int tile) {
+    const int key = tile * kTile + 16 * grp;
+    const int raw = __builtin_amdgcn_readfirstlane(raw_id);
+    const bool there = key <= last_pos && key + 15 >= first_seen &&
+                       (key >> a.block_log2) < a.width && static_cast<uint32_t>(raw) < a.blocks;
+    const uint32_t cell = static_cast<uint32_t>(there ? raw : 0) * a.kv_heads + g;
+    const uint64_t base = static_cast<uint64_t>(cell) * cell_bytes;
+    const int place = key & (bs - 1);
+    const int8_t* k_base = a.k_codes + base + place * D;
+    const int8_t* v_base = a.v_codes + base + place;
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+      const int chunk = 8 * q % kChunks, token8 = 8 * q / kChunks;
+      k_reg[q] = *reinterpret_cast<const u32x4*>(k_base + chunk * 16 + token8 * 8 * D + k_at);
+    }
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+      v_reg[q] = *reinterpret_cast<const u32x4*>(v_base + q * kWave * bs + v_at);
+    }
+    k_scale_reg = a.k_scales[cell];
+    v_scale_reg = a.v_scales[cell];
+    there_reg = there ? 1 : 0;
+  };
+  // Eight lanes write rows of eight different bank groups: with 32 columns
+  // their rows have one bit 2, which rows of odd eights therefore turn over.
+  const int k_slot = W == 32
+                         ? 8 * (lane >> 2 & 1) + 4 * ((wave ^ lane >> 2) & 1) + (lane & 3)
+                         : 8 * (grp & 1) + (lane & 7);
+  const int k_read = W == 32 ? 32 * h + (c ^ (c >> 3 & 1) << 2) : lane;
   auto store_codes = [&](int b) {
 #pragma unroll
-    for (int q = 0; q < kChunks; ++q) {
-      const int n = q * 256 + static_cast<int>(threadIdx.x);
-      const int t8 = n & 7, chunk = (n >> 3) % kSteps, grp = (n >> 3) / kSteps;
+    for (int q = 0; q < kLoads; ++q) {
+      const int at = 8 * q + (lane >> 3), chunk = at % kChunks, token8 = at / kChunks;
       f16x8 f[2];
       codes_to_f16(k_reg[q], f);
-      f16x8* to = &s_k[b][((grp >> 2) * kSteps + chunk) * kWave + 8 * (grp & 3) + t8];
+      const int row_tile = W == 32 ? grp >> 1 : 2 * (grp >> 1) + part_of;
+      const int step = chunk * 16 / kStepD, half = chunk * 16 % kStepD / 8;
+      f16x8* to = &s_k[b][(row_tile * kSteps + step) * kWave + half * W +
+                          (W == 32 ? 16 * token8 : 0) + k_slot];
       to[0] = f[0];
-      to[32] = f[1];
+      to[W] = f[1];
     }
 #pragma unroll
-    for (int q = 0; q < kChunks; ++q) {
-      const int d = q * kWave + lane;
+    for (int q = 0; q < kLoads; ++q) {
+      const int d = part_of * (D / 2) + q * kWave + lane;
       f16x8 f[2];
       codes_to_f16(v_reg[q], f);
-      f16x8* to = &s_v[b][(((d >> 5) * 2 + (wave >> 1)) * 2) * kWave + (d & 31) + 32 * (wave & 1)];
+      f16x8* to =
+          W == 32 ? &s_v[b][((d / 32 * 2 + (grp >> 1)) * 2) * kWave + d % 32 + 32 * (grp & 1)]
+                  : &s_v[b][(d / 16 * 2 + (grp >> 1)) * kWave + d % 16 + 32 * (grp & 1)];
       to[0] = f[0];
-      to[kWave] = f[1];
+      to[W == 32 ? kWave : 16] = f[1];
     }
-    if (threadIdx.x < 8) s_scale[b][threadIdx.x >> 2][threadIdx.x & 3] = scale_reg;
+    if (part_of == 0 && lane == 0) {
+      s_scale[b][grp] = {there_reg ? k_scale_reg : 0.0f, there_reg ? v_scale_reg : 0.0f,
+                         there_reg, 0};
+    }
   };
 
   // ---- the wave's columns
-  const int col = 32 * wave + c;
+  const int col = W * wave + c;
   const bool mine = col < cols;
-  const int token = mine ? col / a.group : item->tokens - 1;
-  const int q_head = g * a.group + (mine ? col - token * a.group : 0);
-  const int pos = first_pos + token;
+  const int row = mine ? col / a.group : item->tokens - 1;
+  const int q_head = g * a.group + (mine ? col - row * a.group : 0);
+  const int pos = first_pos + row;
   const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
   // the wave's first and last token: what all and what any of its columns see
-  const int wave_first = first_pos + min(32 * wave, cols - 1) / a.group;
-  const int wave_last = first_pos + min(32 * wave + 31, cols - 1) / a.group;
+  const int wave_first = first_pos + min(W * wave, cols - 1) / a.group;
+  const int wave_last = first_pos + min(W * wave + W - 1, cols - 1) / a.group;
   const int all_from = a.window > 0 ? max(0, wave_last + 1 - a.window) : 0;
   const int any_from = a.window > 0 ? max(0, wave_first + 1 - a.window) : 0;
-  const bool busy = 32 * wave < cols;
+  const bool busy = W * wave < cols;
 
-  if (tile_lo < tile_hi) load_codes(tile_lo);
+  const int tile_last = tile_hi - 1;
+  if (tile_lo < tile_hi) {
+    load_id(tile_lo);
+    load_codes(tile_lo);
+    load_id(min(tile_lo + 1, tile_last));
+  }
   f16x8 q[State::kTerms][kSteps];
   float col_scale;
   {
     const typename T::store* from = static_cast<const typename T::store*>(a.q) +
-                                    static_cast<int64_t>(min(item->row + token, a.tokens - 1)) *
+                                    static_cast<int64_t>(min(item->row + row, a.tokens - 1)) *
                                         a.q_token_stride +
                                     static_cast<int64_t>(q_head) * a.q_head_stride + 8 * h;
     float x[kSteps][8];
     float top = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      load8<T>(from + 16 * s, x[s]);
+      load8<T>(from + kStepD * s, x[s]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x[s][e] = mine ? x[s][e] : 0.0f;
         top = fmaxf(top, fabsf(x[s][e]));
       }
     }
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = across<W>(top, [](float x, float y) { return fmaxf(x, y); });
     col_scale = split_query<T, kSteps>(x, top, a.scale * kLog2e, q);
   }
 
-  f32x16 o[kTilesD], rest[State::kApart ? kTilesD : 1];
+  Acc o[kTilesD], rest[State::kApart ? kTilesD : 1];
 #pragma unroll
   for (int d = 0; d < kTilesD; ++d) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
+    for (int e = 0; e < kAcc; ++e) {
       o[d][e] = 0.0f;
       if constexpr (State::kApart) rest[d][e] = 0.0f;
     }
   }
   float m = -INFINITY, l = 0.0f, v_ref = 0.0f, v_inv = 0.0f;
 
-  int seen = 0;
   if (tile_lo < tile_hi) {
     store_codes(0);
-    seen = seen_reg;
-    if (tile_lo + 1 < tile_hi) load_codes(tile_lo + 1);
+    load_codes(min(tile_lo + 1, tile_last));
+    load_id(min(tile_lo + 2, tile_last));
   }
   for (int tile = tile_lo; tile < tile_hi; ++tile) {
     const int b = (tile - tile_lo) & 1;
     __syncthreads();  // the tile is in LDS; the other buffer is read
-    const int seen_now = seen;
-    if (tile + 1 < tile_hi) {
-      store_codes(b ^ 1);
-      seen = seen_reg;
-      if (tile + 2 < tile_hi) load_codes(tile + 2);
-    }
-    const int key0 = tile * kTile;
-    if (!busy || key0 > wave_last || key0 + kTile - 1 < any_from || seen_now == 0) continue;
-
-    f32x16 s[2];
+    Acc s[2][kHalves];  // of 32 keys each
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < 2 * kHalves; ++r) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[r][e] = 0.0f;
+      for (int e = 0; e < kAcc; ++e) s[r / kHalves][r % kHalves][e] = 0.0f;
     }
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const f16x8 f = s_k[b][(r * kSteps + k) * kWave + lane];
+      for (int r = 0; r < 2 * kHalves; ++r) {
+        const f16x8 f = s_k[b][(r * kSteps + k) * kWave + k_read];
+        Acc& to = s[r / kHalves][r % kHalves];
 #pragma unroll
-        for (int e = 0; e < State::kTerms; ++e) {
-          s[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, q[e][k], s[r], 0, 0, 0);
-        }
+        for (int e = 0; e < State::kTerms; ++e) to = wide_mul(f, q[e][k], to);
       }
     }
+    feed<2 * kHalves * kSteps, State::kTerms>();
+    auto score = [&](int r, int e) { return s[r][e / kAcc][e % kAcc]; };
+    store_codes(b ^ 1);  // past the last tile: what nobody reads
+    load_codes(min(tile + 2, tile_last));
+    load_id(min(tile + 3, tile_last));
+    const GroupScale of[2] = {s_scale[b][h * kPer / 16], s_scale[b][2 + h * kPer / 16]};
+    const int seen_0 = s_scale[b][0].there, seen_1 = s_scale[b][1].there;
+    const int seen_2 = s_scale[b][2].there, seen_3 = s_scale[b][3].there;
+    const int seen_now =
+        __builtin_amdgcn_readfirstlane(seen_0 | seen_1 << 1 | seen_2 << 2 | seen_3 << 3);
+    const int key0 = tile * kTile;
+    if (!busy || key0 > wave_last || key0 + kTile - 1 < any_from || seen_now == 0) continue;
 
-    // scales of keys 16 h .. 16 h + 15 of the row tiles
+    // a lane's keys: kPer neighbours of either 32, which share their scales
     float kscale[2], vscale[2], top[2], v_top[2], mul[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      kscale[r] = s_scale[b][0][2 * r + h] * col_scale;
-      vscale[r] = s_scale[b][1][2 * r + h];
+      kscale[r] = of[r].k * col_scale;
+      vscale[r] = of[r].v;
     }
     const bool whole = key0 >= all_from && key0 + kTile - 1 <= wave_first && seen_now == 15;
     if (whole && __all(!(kscale[0] < 0.0f || kscale[1] < 0.0f))) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        top[r] = s[r][0];
+        top[r] = score(r, 0);
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top[r] = fmaxf(top[r], s[r][e]);
+        for (int e = 1; e < kPer; ++e) top[r] = fmaxf(top[r], score(r, e));
         top[r] *= kscale[r];
         v_top[r] = vscale[r];
         mul[r] = kscale[r];
@@ -243,14 +306,15 @@ __global__ __launch_bounds__(256, wide_blocks_per_cu(T::code, D)) void attend_wi
     } else {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int key = key0 + 32 * r + 16 * h;
-        const bool some = (seen_now >> (2 * r + h) & 1) && key <= pos && key + 15 >= seen_from;
+        const int key = key0 + 32 * r + kPer * h;
+        const bool some = of[r].there && key <= pos && key + kPer - 1 >= seen_from;
         top[r] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < kPer; ++e) {
           const int k = key + e;
-          s[r][e] = some && k <= pos && k >= seen_from ? s[r][e] * kscale[r] : -INFINITY;
-          top[r] = fmaxf(top[r], s[r][e]);
+          const float sc = some && k <= pos && k >= seen_from ? score(r, e) * kscale[r] : -INFINITY;
+          s[r][e / kAcc][e % kAcc] = sc;
+          top[r] = fmaxf(top[r], sc);
         }
         v_top[r] = some ? vscale[r] : 0.0f;
         mul[r] = 1.0f;
@@ -260,10 +324,9 @@ __global__ __launch_bounds__(256, wide_blocks_per_cu(T::code, D)) void attend_wi
     const float t_v =
         fmaxf(v_top[0] <= 3.0e38f ? v_top[0] : 0.0f, v_top[1] <= 3.0e38f ? v_top[1] : 0.0f);
     if (__any(t_top > m + State::kRescale || t_v > v_ref)) {
-      float m2 = fmaxf(m, t_top);
-      m2 = fmaxf(m2, __shfl_xor(m2, 32));
-      float v2 = fmaxf(v_ref, t_v);
-      v2 = fmaxf(v2, __shfl_xor(v2, 32));
+      const auto larger = [](float x, float y) { return fmaxf(x, y); };
+      const float m2 = across<W>(fmaxf(m, t_top), larger);
+      const float v2 = across<W>(fmaxf(v_ref, t_v), larger);
       const float ref = v2 > v_ref ? power_above(v2) : v_ref;
       const float keep = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m2);
       const float keep_o = ref > 0.0f ? keep * (v_ref / ref) : 1.0f;
@@ -279,19 +342,20 @@ __global__ __launch_bounds__(256, wide_blocks_per_cu(T::code, D)) void attend_wi
     }
     const float shift = weight_bias(T::code) - (m == -INFINITY ? 0.0f : m);
     const float v_factor[2] = {vscale[0] * v_inv, vscale[1] * v_inv};
-    f16x8 w[2][2], w_rest[2][2];
+    f16x8 w[2][kPer / 8], w_rest[2][kPer / 8];
     auto weights = [&](auto some_hidden) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < kPer / 8; ++k) {
           float p[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float sc = s[r][8 * k + e];
+            const float sc = score(r, 8 * k + e);
             p[e] = __builtin_amdgcn_exp2f(fmaf(sc, mul[r], shift));
             float v = p[e] * v_factor[r];
             if constexpr (decltype(some_hidden)::value) v = sc == -INFINITY ? 0.0f : v;
+            if constexpr (State::kRest) v = as_rounded(v);
             w[r][k][e] = static_cast<_Float16>(v);
             if constexpr (State::kRest) {
               w_rest[r][k][e] =
@@ -311,29 +375,30 @@ __global__ __launch_bounds__(256, wide_blocks_per_cu(T::code, D)) void attend_wi
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < kPer / 8; ++k) {
 #pragma unroll
         for (int d = 0; d < kTilesD; ++d) {
-          const f16x8 f = s_v[b][((d * 2 + r) * 2 + k) * kWave + lane];
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, w[r][k], o[d], 0, 0, 0);
+          const f16x8 f = s_v[b][((d * 2 + r) * (kPer / 8) + k) * kWave + lane];
+          o[d] = wide_mul(f, w[r][k], o[d]);
           if constexpr (State::kRest) {
-            f32x16& to = State::kApart ? rest[d] : o[d];
-            to = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, w_rest[r][k], to, 0, 0, 0);
+            Acc& to = State::kApart ? rest[d] : o[d];
+            to = wide_mul(f, w_rest[r][k], to);
           }
         }
       }
     }
+    feed<2 * kPer / 8 * kTilesD, State::kRest ? 2 : 1>();
   }
 
   if (!busy) return;
-  l += __shfl_xor(l, 32);
+  l = across<W>(l, [](float x, float y) { return x + y; });
   if (!mine) return;
   const int part = item->part;
   float* to = a.parts + (static_cast<size_t>(g) * a.cap_parts + max(0, part)) * wide_part_floats(D);
 #pragma unroll
   for (int d = 0; d < kTilesD; ++d) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kAcc / 4; ++k) {
       f32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -341,8 +406,8 @@ __global__ __launch_bounds__(256, wide_blocks_per_cu(T::code, D)) void attend_wi
         if constexpr (State::kApart) v[e] += rest[d][4 * k + e] * (1.0f / State::kRestScale);
         v[e] *= v_ref;
       }
-      const int at = 32 * d + 8 * k + 4 * h;
-      if (part < 0) finish4<T>(a, item->row + token, q_head, at, v, m, l);
+      const int at = W * d + 4 * kLanes * k + 4 * h;
+      if (part < 0) finish4<T>(a, item->row + row, q_head, at, v, m, l);
       else *reinterpret_cast<f32x4*>(to + col * D + at) = v;
     }
   }

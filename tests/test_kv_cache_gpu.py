@@ -361,6 +361,16 @@ def test_attend_extreme_scores_and_scales(hip_lib, dtype, hd):
     attend_case(s, 8, 0, dtype, q=q)
 
 
+@pytest.mark.parametrize("heads,kv,ctx,new", [(16, 4, [0] * 60, [30] * 60),
+                                              (16, 16, [i % 25 for i in range(200)], [2] * 200)])
+def test_attend_f32_weights_keep_their_second_term(hip_lib, heads, kv, ctx, new):
+    """Scores near 0 and few keys: what is left of the bound is the weights'
+    own 21 bits, so that one weight that lost a unit of its first 11 shows.
+    One in 2^13 is where that could happen."""
+    s = Setup(ctx, new, kv, 64, 16, seed=5)
+    attend_case(s, heads, 0, "f32", q=s.rng.standard_normal((s.tokens, heads, 64)) * 2.0 ** -9)
+
+
 def test_attend_on_another_stream_and_in_a_graph(hip_lib):
     s = Setup([300, 10, 2000], [1, 30, 1], 2, 128, 32)
     cache, batch = s.cache(), s.batch(8)
