@@ -189,10 +189,12 @@ static void launch_narrow(AttendArgs a, const Shape& s, hipStream_t stream) {
 template <class T, int D>
 static void launch_wide(AttendArgs a, const Shape& s, hipStream_t stream) {
   a.parts += s.narrow_bytes / 4;
-  const dim3 grid(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.cap_items));
+  constexpr int kItems = wide_items(T::code, D);
+  const dim3 grid(static_cast<unsigned>(a.kv_heads),
+                  static_cast<unsigned>((s.cap_items + kItems - 1) / kItems));
   attend_wide_kernel<T, D><<<grid, wide_threads(T::code, D), 0, stream>>>(a);
   const dim3 joins(static_cast<unsigned>(a.kv_heads), static_cast<unsigned>(s.cap_joins),
-                   kWideCols / 16);
+                   kWideCols / join_wide_cols<D>());
   join_wide_kernel<T, D><<<joins, 256, 0, stream>>>(a);
 }
 

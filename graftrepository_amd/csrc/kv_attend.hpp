@@ -43,23 +43,29 @@ __device__ inline size_t narrow_part(int g, int runs, int run, int which) {
   return (static_cast<size_t>(g) * runs + run) * 2 + which;
 }
 
-// Sixteen codes to fp16, exactly: a byte under the exponent of 1024 is
+// Eight codes to fp16, exactly: a byte under the exponent of 1024 is
 // 1024 + u, and u = code + 128.
-__device__ inline void codes_to_f16(u32x4 w, f16x8 (&out)[2]) {
+__device__ inline f16x8 codes_to_f16(uint32_t first, uint32_t second) {
   const f16x2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+  f16x8 out;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t u = w[k] ^ 0x80808080u;
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t u = (k ? second : first) ^ 0x80808080u;
     const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
     const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
     const f16x2 a = __builtin_bit_cast(f16x2, lo) + off;
     const f16x2 b = __builtin_bit_cast(f16x2, hi) + off;
-    const int at = 4 * (k & 1);
-    out[k >> 1][at] = a[0];
-    out[k >> 1][at + 1] = a[1];
-    out[k >> 1][at + 2] = b[0];
-    out[k >> 1][at + 3] = b[1];
+    out[4 * k] = a[0];
+    out[4 * k + 1] = a[1];
+    out[4 * k + 2] = b[0];
+    out[4 * k + 3] = b[1];
   }
+  return out;
+}
+
+__device__ inline void codes_to_f16(u32x4 w, f16x8 (&out)[2]) {
+  out[0] = codes_to_f16(w[0], w[1]);
+  out[1] = codes_to_f16(w[2], w[3]);
 }
 
 // A product as fp32 holds it.  Left open, the compiler rounds it to fp16 from
@@ -124,7 +130,7 @@ __device__ inline float power_above(float v) {
 }
 
 // Log2 of what probabilities are scaled by on their way into fp16.
-__host__ __device__ constexpr float weight_bias(int dtype) { return dtype == kF32 ? 7.0f : 14.0f; }
+__host__ __device__ constexpr float weight_bias(int dtype) { return dtype == kF32 ? 7.0f : 13.0f; }
 
 // Four values of a finished row: o / l rounded once, and the row's log-sum-exp
 // by the thread of its first column.  m in log2 units, l and o biased.

@@ -70,7 +70,7 @@ struct NarrowState {
   static constexpr bool kRest = T::code != kBF16;               // of a probability: two
   static constexpr bool kApart = T::code == kF32;               // and summed apart
   static constexpr float kRestScale = kApart ? 524288.0f : 1.0f;
-  static constexpr float kRescale = kApart ? 0.0f : 1.0f;
+  static constexpr float kRescale = kApart ? 0.0f : 2.0f;
   float col_scale;  // softmax scale, log2 e and the query's own power of two
   f32x4 o[D / 16];
   f32x4 rest[kApart ? D / 16 : 1];

@@ -51,11 +51,13 @@ __host__ __device__ constexpr int wide_part_floats(int head_dim) {
 }
 
 // Scales of 16 tokens, 0 where they have no block or none of the item's
-// columns sees them.
+// columns sees them, and the value scale's logarithm (0 for no number).
 struct __align__(16) GroupScale {
-  float k, v;
-  int there, pad;
+  float k, v, v_log;
+  int there;
 };
+
+constexpr float kLargest = 3.0e38f;  // below are numbers
 
 // A value joined over the lanes of a column.
 template <int W, class F>
@@ -72,49 +74,63 @@ __device__ inline f32x4 wide_mul(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// The order of a product's reads from LDS and matrix instructions (MULS for
-// each of READS reads): reads run kAhead before what needs them.
-template <int READS, int MULS>
-__device__ inline void feed() {
-  constexpr int kAhead = 6, kMul = 0x8, kRead = 0x100;
-  __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+// A product's reads from LDS and what is done with each, in this order: reads
+// run kAhead before their use, and what `use` does beside the matrix
+// instruction stays beside it.
+template <int READS, class Read, class Use>
+__device__ inline void in_step(Read read, Use use) {
+  constexpr int kAhead = 6;
+  f16x8 f[READS];
+#pragma unroll
+  for (int i = 0; i < kAhead && i < READS; ++i) f[i] = read(i);
 #pragma unroll
   for (int i = 0; i < READS; ++i) {
-    __builtin_amdgcn_sched_group_barrier(kMul, MULS, 0);
-    if (i + kAhead < READS) __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+    if (i + kAhead < READS) f[i + kAhead] = read(i + kAhead);
+    use(i, f);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kernel(AttendArgs a) {
+struct WideShape {
   typedef NarrowState<T, D> State;  // its constants: terms and allowances
-  constexpr int W = wide_wave_cols(T::code, D);
-  constexpr int kWaves = kWideCols / W, kLanes = kWave / W;  // lanes of a column
-  constexpr int kStepD = 8 * kLanes, kSteps = D / kStepD;    // of the first product
-  constexpr int kTilesD = D / W;                             // value row tiles
-  constexpr int kLoads = 16 * D * 4 / (kWaves * kWave * 16);  // 16 bytes of keys to a lane
-  constexpr int kPer = W / 2, kHalves = 32 / W;  // scores, accumulators of 32 keys to a lane
-  constexpr int kAcc = W * W / kWave;
+  static constexpr int W = wide_wave_cols(T::code, D);
+  static constexpr int kWaves = kWideCols / W, kLanes = kWave / W;  // lanes of a column
+  static constexpr int kStepD = 8 * kLanes, kSteps = D / kStepD;    // of the first product
+  static constexpr int kTilesD = D / W;                             // value row tiles
+  static constexpr int kLoads = 16 * D * 4 / (kWaves * kWave * 16);  // 16 bytes of keys to a lane
+  static constexpr int kPer = W / 2, kHalves = 32 / W;  // scores, accumulators of 32 keys to a lane
+  static constexpr int kAcc = W * W / kWave;
   typedef typename std::conditional<W == 32, f32x16, f32x4>::type Acc;
+
+  // a lane's eight values of an instruction's operand
+  f16x8 k[2][2 * kHalves * kSteps * kWave];       // [row tile][step][lane]
+  f16x8 v[2][kTilesD * 2 * kPer / 8 * kWave];     // [d tile][32 keys][lane]
+  GroupScale scale[2][4];                         // of a group of 16 tokens
+};
+
+// One item's tiles up to tile_hi, which may be the next item's.
+template <class T, int D>
+__device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_hi,
+                                 WideShape<T, D>& lds) {
+  typedef WideShape<T, D> S;
+  typedef typename S::State State;
+  typedef typename S::Acc Acc;
+  constexpr int W = S::W, kWaves = S::kWaves, kLanes = S::kLanes, kStepD = S::kStepD;
+  constexpr int kSteps = S::kSteps, kTilesD = S::kTilesD, kLoads = S::kLoads;
+  constexpr int kPer = S::kPer, kHalves = S::kHalves, kAcc = S::kAcc;
+  auto& s_k = lds.k;
+  auto& s_v = lds.v;
+  auto& s_scale = lds.scale;
   const int g = blockIdx.x;
-  const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
-  if (static_cast<int>(blockIdx.y) >= head->items) return;
-  const auto* item = reinterpret_cast<ConstItem>(reinterpret_cast<uintptr_t>(a.work) + a.at_items) +
-                     blockIdx.y;
-  if (item->tokens <= 0) return;
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % W, h = lane / W;
-  const int tile_lo = item->tile_lo, tile_hi = item->tile_hi;
+  const int tile_lo = item->tile_lo;
   const int first_pos = item->pos, last_pos = first_pos + item->tokens - 1;
   const int cols = item->tokens * a.group;
   const size_t table_row = static_cast<size_t>(item->request) * a.width;
   const int bs = 1 << a.block_log2;
   const uint32_t cell_bytes = static_cast<uint32_t>(bs * D);
-
-  // a lane's eight values of the instruction's operand
-  __shared__ f16x8 s_k[2][2 * kHalves * kSteps * kWave];  // [row tile][step][lane]
-  __shared__ f16x8 s_v[2][kTilesD * 2 * kPer / 8 * kWave];  // [d tile][32 keys][lane]
-  __shared__ GroupScale s_scale[2][4];                      // of a group of 16 tokens
 
   // ---- codes of a tile to registers: a wavefront (or two) loads 16 of its
   // tokens, which lie in one block, so that addresses are a scalar base and a
@@ -136,28 +152,32 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
     const int at = (tile * kTile + 16 * grp) >> a.block_log2;
     raw_id = a.table[table_row + max(0, min(at, a.width - 1))];
   };
-  auto load_codes = [&](int tile) {
+  int32_t v_cell = 0, v_place = 0;
+  auto load_keys = [&](int tile) {
     const int key = tile * kTile + 16 * grp;
     const int raw = __builtin_amdgcn_readfirstlane(raw_id);
     const bool there = key <= last_pos && key + 15 >= first_seen &&
                        (key >> a.block_log2) < a.width && static_cast<uint32_t>(raw) < a.blocks;
     const uint32_t cell = static_cast<uint32_t>(there ? raw : 0) * a.kv_heads + g;
-    const uint64_t base = static_cast<uint64_t>(cell) * cell_bytes;
     const int place = key & (bs - 1);
-    const int8_t* k_base = a.k_codes + base + place * D;
-    const int8_t* v_base = a.v_codes + base + place;
+    const int8_t* k_base = a.k_codes + static_cast<uint64_t>(cell) * cell_bytes + place * D;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
       const int chunk = 8 * q % kChunks, token8 = 8 * q / kChunks;
       k_reg[q] = *reinterpret_cast<const u32x4*>(k_base + chunk * 16 + token8 * 8 * D + k_at);
     }
+    k_scale_reg = a.k_scales[cell];
+    v_scale_reg = a.v_scales[cell];
+    there_reg = there ? 1 : 0;
+    v_cell = cell;
+    v_place = place;
+  };
+  auto load_values = [&]() {  // of the tile whose keys were loaded last
+    const int8_t* v_base = a.v_codes + static_cast<uint64_t>(static_cast<uint32_t>(v_cell)) * cell_bytes + v_place;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
       v_reg[q] = *reinterpret_cast<const u32x4*>(v_base + q * kWave * bs + v_at);
     }
-    k_scale_reg = a.k_scales[cell];
-    v_scale_reg = a.v_scales[cell];
-    there_reg = there ? 1 : 0;
   };
   // Eight lanes write rows of eight different bank groups: with 32 columns
   // their rows have one bit 2, which rows of odd eights therefore turn over.
@@ -165,33 +185,31 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
                          ? 8 * (lane >> 2 & 1) + 4 * ((wave ^ lane >> 2) & 1) + (lane & 3)
                          : 8 * (grp & 1) + (lane & 7);
   const int k_read = W == 32 ? 32 * h + (c ^ (c >> 3 & 1) << 2) : lane;
-  auto store_codes = [&](int b) {
-#pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
+  // Half a register's codes at a time, so that the products' instructions have
+  // something beside each: kPieces of a tile's keys and the one's before values.
+  constexpr int kPieces = 4 * kLoads;
+  auto store_piece = [&](int piece, int b) {
+    const int q = piece / 2 % kLoads, half = piece % 2;
+    if (piece < 2 * kLoads) {
       const int at = 8 * q + (lane >> 3), chunk = at % kChunks, token8 = at / kChunks;
-      f16x8 f[2];
-      codes_to_f16(k_reg[q], f);
       const int row_tile = W == 32 ? grp >> 1 : 2 * (grp >> 1) + part_of;
-      const int step = chunk * 16 / kStepD, half = chunk * 16 % kStepD / 8;
-      f16x8* to = &s_k[b][(row_tile * kSteps + step) * kWave + half * W +
-                          (W == 32 ? 16 * token8 : 0) + k_slot];
-      to[0] = f[0];
-      to[W] = f[1];
-    }
-#pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
+      const int step = chunk * 16 / kStepD, first = chunk * 16 % kStepD / 8;
+      s_k[b ^ 1][(row_tile * kSteps + step) * kWave + (first + half) * W +
+                 (W == 32 ? 16 * token8 : 0) + k_slot] =
+          codes_to_f16(k_reg[q][2 * half], k_reg[q][2 * half + 1]);
+    } else {
       const int d = part_of * (D / 2) + q * kWave + lane;
-      f16x8 f[2];
-      codes_to_f16(v_reg[q], f);
-      f16x8* to =
-          W == 32 ? &s_v[b][((d / 32 * 2 + (grp >> 1)) * 2) * kWave + d % 32 + 32 * (grp & 1)]
-                  : &s_v[b][(d / 16 * 2 + (grp >> 1)) * kWave + d % 16 + 32 * (grp & 1)];
-      to[0] = f[0];
-      to[W == 32 ? kWave : 16] = f[1];
+      const int at =
+          W == 32 ? ((d / 32 * 2 + (grp >> 1)) * 2 + half) * kWave + d % 32 + 32 * (grp & 1)
+                  : (d / 16 * 2 + (grp >> 1)) * kWave + d % 16 + 32 * (grp & 1) + 16 * half;
+      s_v[b][at] = codes_to_f16(v_reg[q][2 * half], v_reg[q][2 * half + 1]);
     }
+  };
+  auto store_scales = [&](int b) {
     if (part_of == 0 && lane == 0) {
-      s_scale[b][grp] = {there_reg ? k_scale_reg : 0.0f, there_reg ? v_scale_reg : 0.0f,
-                         there_reg, 0};
+      const float v = there_reg ? v_scale_reg : 0.0f;
+      s_scale[b][grp] = {there_reg ? k_scale_reg : 0.0f, v,
+                         v <= kLargest ? __builtin_amdgcn_logf(v) : 0.0f, there_reg};
     }
   };
 
@@ -206,13 +224,13 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
   const int wave_first = first_pos + min(W * wave, cols - 1) / a.group;
   const int wave_last = first_pos + min(W * wave + W - 1, cols - 1) / a.group;
   const int all_from = a.window > 0 ? max(0, wave_last + 1 - a.window) : 0;
-  const int any_from = a.window > 0 ? max(0, wave_first + 1 - a.window) : 0;
   const bool busy = W * wave < cols;
 
   const int tile_last = tile_hi - 1;
   if (tile_lo < tile_hi) {
     load_id(tile_lo);
-    load_codes(tile_lo);
+    load_keys(tile_lo);
+    load_values();
     load_id(min(tile_lo + 1, tile_last));
   }
   f16x8 q[State::kTerms][kSteps];
@@ -246,12 +264,65 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
       if constexpr (State::kApart) rest[d][e] = 0.0f;
     }
   }
-  float m = -INFINITY, l = 0.0f, v_ref = 0.0f, v_inv = 0.0f;
+  float m = -INFINITY, l = 0.0f, v_ref = 0.0f, ref_log = 0.0f, poison = 0.0f;
+  // The sums of the tiles so far take a change of the references with them
+  // when the next tile's scores are there: then their products are done.
+  bool moves = false;
+  float keep_o = 1.0f;
+  auto rescale = [&]() {
+    if (moves) {
+#pragma unroll
+      for (int d = 0; d < kTilesD; ++d) {
+        o[d] *= keep_o;
+        if constexpr (State::kApart) rest[d] *= keep_o;
+      }
+    }
+  };
 
+  auto next_codes = [&](int tile) {
+    load_values();
+    load_keys(min(tile + 2, tile_last));
+    load_id(min(tile + 3, tile_last));
+  };
   if (tile_lo < tile_hi) {
-    store_codes(0);
-    load_codes(min(tile_lo + 1, tile_last));
+    // the values go where the first product, with weights of 0, reads them
+#pragma unroll
+    for (int piece = 0; piece < kPieces; ++piece) store_piece(piece, 1);
+    store_scales(0);
+    load_keys(min(tile_lo + 1, tile_last));
     load_id(min(tile_lo + 2, tile_last));
+  }
+  f16x8 w[2][kPer / 8] = {}, w_rest[2][kPer / 8] = {};
+  // Weights of a tile times its values.
+  constexpr int kValueReads = 2 * kPer / 8 * kTilesD;
+  constexpr int kLag = State::kApart ? 0 : 2;
+  auto multiply = [&](int b, auto beside) {
+    in_step<kValueReads>([&](int i) { return s_v[b][(i % kTilesD * 2 * (kPer / 8) + i / kTilesD) * kWave + lane]; },
+        [&](int i, const f16x8(&f)[kValueReads]) {
+          const int d = i % kTilesD, rk = i / kTilesD;
+          o[d] = wide_mul(f[i], w[rk / (kPer / 8)][rk % (kPer / 8)], o[d]);
+          if constexpr (State::kRest) {
+            // a step of its own sums later, which need not wait for the first's
+            for (int n = max(0, i - kLag); n <= (i == kValueReads - 1 ? i : i - kLag); ++n) {
+              Acc& to = State::kApart ? rest[n % kTilesD] : o[n % kTilesD];
+              to = wide_mul(f[n], w_rest[n / kTilesD / (kPer / 8)][n / kTilesD % (kPer / 8)], to);
+            }
+          }
+          beside(i);
+        });
+  };
+
+  if (!busy) {  // loads its share of the codes
+    for (int tile = tile_lo; tile < tile_hi; ++tile) {
+      const int b = (tile - tile_lo) & 1;
+      __syncthreads();
+#pragma unroll
+      for (int piece = 0; piece < kPieces; ++piece) store_piece(piece, b);
+      store_scales(b ^ 1);
+      next_codes(tile);
+    }
+    __syncthreads();
+    return;
   }
   for (int tile = tile_lo; tile < tile_hi; ++tile) {
     const int b = (tile - tile_lo) & 1;
@@ -262,35 +333,37 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
 #pragma unroll
       for (int e = 0; e < kAcc; ++e) s[r / kHalves][r % kHalves][e] = 0.0f;
     }
+    constexpr int kKeyReads = 2 * kHalves * kSteps;
+    in_step<kKeyReads>(
+        [&](int i) {
+          return s_k[b][(i % (2 * kHalves) * kSteps + i / (2 * kHalves)) * kWave + k_read];
+        },
+        [&](int i, const f16x8(&f)[kKeyReads]) {
+          Acc& to = s[i % (2 * kHalves) / kHalves][i % kHalves];
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
+          for (int e = 0; e < State::kTerms; ++e) to = wide_mul(f[i], q[e][i / (2 * kHalves)], to);
 #pragma unroll
-      for (int r = 0; r < 2 * kHalves; ++r) {
-        const f16x8 f = s_k[b][(r * kSteps + k) * kWave + k_read];
-        Acc& to = s[r / kHalves][r % kHalves];
-#pragma unroll
-        for (int e = 0; e < State::kTerms; ++e) to = wide_mul(f, q[e][k], to);
-      }
-    }
-    feed<2 * kHalves * kSteps, State::kTerms>();
+          for (int piece = i * kPieces / kKeyReads; piece < (i + 1) * kPieces / kKeyReads;
+               ++piece) {
+            store_piece(piece, b);  // past the last tile: what nobody reads
+          }
+        });
+    store_scales(b ^ 1);
+    next_codes(tile);
     auto score = [&](int r, int e) { return s[r][e / kAcc][e % kAcc]; };
-    store_codes(b ^ 1);  // past the last tile: what nobody reads
-    load_codes(min(tile + 2, tile_last));
-    load_id(min(tile + 3, tile_last));
     const GroupScale of[2] = {s_scale[b][h * kPer / 16], s_scale[b][2 + h * kPer / 16]};
     const int seen_0 = s_scale[b][0].there, seen_1 = s_scale[b][1].there;
     const int seen_2 = s_scale[b][2].there, seen_3 = s_scale[b][3].there;
     const int seen_now =
         __builtin_amdgcn_readfirstlane(seen_0 | seen_1 << 1 | seen_2 << 2 | seen_3 << 3);
     const int key0 = tile * kTile;
-    if (!busy || key0 > wave_last || key0 + kTile - 1 < any_from || seen_now == 0) continue;
-
     // a lane's keys: kPer neighbours of either 32, which share their scales
-    float kscale[2], vscale[2], top[2], v_top[2], mul[2];
+    float kscale[2], v_log[2], top[2], v_top[2], mul[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       kscale[r] = of[r].k * col_scale;
-      vscale[r] = of[r].v;
+      v_log[r] = of[r].v_log;
+      v_top[r] = of[r].v;
     }
     const bool whole = key0 >= all_from && key0 + kTile - 1 <= wave_first && seen_now == 15;
     if (whole && __all(!(kscale[0] < 0.0f || kscale[1] < 0.0f))) {
@@ -300,7 +373,6 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
 #pragma unroll
         for (int e = 1; e < kPer; ++e) top[r] = fmaxf(top[r], score(r, e));
         top[r] *= kscale[r];
-        v_top[r] = vscale[r];
         mul[r] = kscale[r];
       }
     } else {
@@ -316,82 +388,79 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
           s[r][e / kAcc][e % kAcc] = sc;
           top[r] = fmaxf(top[r], sc);
         }
-        v_top[r] = some ? vscale[r] : 0.0f;
+        if (!some) {
+          v_top[r] = 0.0f;
+          v_log[r] = -INFINITY;
+        }
         mul[r] = 1.0f;
       }
     }
     const float t_top = fmaxf(top[0], top[1]);
     const float t_v =
-        fmaxf(v_top[0] <= 3.0e38f ? v_top[0] : 0.0f, v_top[1] <= 3.0e38f ? v_top[1] : 0.0f);
-    if (__any(t_top > m + State::kRescale || t_v > v_ref)) {
+        fmaxf(v_top[0] <= kLargest ? v_top[0] : 0.0f, v_top[1] <= kLargest ? v_top[1] : 0.0f);
+    rescale();
+    moves = __any(t_top > m + State::kRescale || t_v > v_ref);
+    if (moves) {
       const auto larger = [](float x, float y) { return fmaxf(x, y); };
       const float m2 = across<W>(fmaxf(m, t_top), larger);
       const float v2 = across<W>(fmaxf(v_ref, t_v), larger);
       const float ref = v2 > v_ref ? power_above(v2) : v_ref;
       const float keep = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m2);
-      const float keep_o = ref > 0.0f ? keep * (v_ref / ref) : 1.0f;
+      keep_o = ref > 0.0f ? keep * (v_ref / ref) : 1.0f;
       l *= keep;
-#pragma unroll
-      for (int d = 0; d < kTilesD; ++d) {
-        o[d] *= keep_o;
-        if constexpr (State::kApart) rest[d] *= keep_o;
-      }
       m = m2;
       v_ref = ref;
-      v_inv = ref > 0.0f ? 1.0f / ref : 0.0f;
+      ref_log = ref > 0.0f ? __builtin_amdgcn_logf(ref) : 0.0f;
     }
     const float shift = weight_bias(T::code) - (m == -INFINITY ? 0.0f : m);
-    const float v_factor[2] = {vscale[0] * v_inv, vscale[1] * v_inv};
-    f16x8 w[2][kPer / 8], w_rest[2][kPer / 8];
-    auto weights = [&](auto some_hidden) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-#pragma unroll
-        for (int k = 0; k < kPer / 8; ++k) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float sc = score(r, 8 * k + e);
-            p[e] = __builtin_amdgcn_exp2f(fmaf(sc, mul[r], shift));
-            float v = p[e] * v_factor[r];
-            if constexpr (decltype(some_hidden)::value) v = sc == -INFINITY ? 0.0f : v;
-            if constexpr (State::kRest) v = as_rounded(v);
-            w[r][k][e] = static_cast<_Float16>(v);
-            if constexpr (State::kRest) {
-              w_rest[r][k][e] =
-                  static_cast<_Float16>((v - static_cast<float>(w[r][k][e])) * State::kRestScale);
-            }
-          }
-          l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        }
-      }
-    };
-    if (!whole && __any(!(fabsf(v_factor[0]) <= 3.0e38f && fabsf(v_factor[1]) <= 3.0e38f))) {
-      weights(std::true_type{});
-    } else {
-      weights(std::false_type{});
-    }
-
+    // The value scale, as a part of the largest, goes into the exponent and out
+    // of the sum again.  One below 2^-60 takes no part in a product of fp32;
+    // one that is no number makes its columns so at the end.
+    float at[2], out_of[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      poison += v_top[r] <= kLargest ? 0.0f : NAN;
+      const float part = __builtin_amdgcn_fmed3f(v_log[r] - ref_log, -60.0f, 0.0f);
+      at[r] = shift + part;
+      out_of[r] = __builtin_amdgcn_exp2f(-part);
+    }
+    // The last tile's product runs beside this tile's weights.
+    f16x8 w2[2][kPer / 8], w2_rest[2][kPer / 8];
+    float sum[2] = {0.0f, 0.0f};
+    multiply(b ^ 1, [&](int i) {
 #pragma unroll
-      for (int k = 0; k < kPer / 8; ++k) {
+      for (int j = i * kPer / kValueReads; j < (i + 1) * kPer / kValueReads; ++j) {
+        const int r = 2 * j / kPer;  // two weights at a time
 #pragma unroll
-        for (int d = 0; d < kTilesD; ++d) {
-          const f16x8 f = s_v[b][((d * 2 + r) * (kPer / 8) + k) * kWave + lane];
-          o[d] = wide_mul(f, w[r][k], o[d]);
+        for (int e = 2 * j % kPer; e < 2 * j % kPer + 2; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(score(r, e), mul[r], at[r]));
+          const _Float16 first = static_cast<_Float16>(p);
+          w2[r][e / 8][e % 8] = first;
           if constexpr (State::kRest) {
-            Acc& to = State::kApart ? rest[d] : o[d];
-            to = wide_mul(f, w_rest[r][k], to);
+            w2_rest[r][e / 8][e % 8] =
+                static_cast<_Float16>((p - static_cast<float>(first)) * State::kRestScale);
           }
+          sum[r] += p;
         }
       }
+    });
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l = fmaf(sum[r], out_of[r], l);
+#pragma unroll
+      for (int k = 0; k < kPer / 8; ++k) {
+        w[r][k] = w2[r][k];
+        if constexpr (State::kRest) w_rest[r][k] = w2_rest[r][k];
+      }
     }
-    feed<2 * kPer / 8 * kTilesD, State::kRest ? 2 : 1>();
   }
+  __syncthreads();
+  rescale();
+  if (tile_lo < tile_hi) multiply((tile_last - tile_lo) & 1, [](int) {});
 
-  if (!busy) return;
-  l = across<W>(l, [](float x, float y) { return x + y; });
+  const auto sum_of = [](float x, float y) { return x + y; };
+  l = across<W>(l, sum_of);
+  poison = across<W>(poison, sum_of);
   if (!mine) return;
   const int part = item->part;
   float* to = a.parts + (static_cast<size_t>(g) * a.cap_parts + max(0, part)) * wide_part_floats(D);
@@ -404,7 +473,7 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
       for (int e = 0; e < 4; ++e) {
         v[e] = o[d][4 * k + e];
         if constexpr (State::kApart) v[e] += rest[d][4 * k + e] * (1.0f / State::kRestScale);
-        v[e] *= v_ref;
+        v[e] = fmaf(v[e], v_ref, poison);
       }
       const int at = W * d + 4 * kLanes * k + 4 * h;
       if (part < 0) finish4<T>(a, item->row + row, q_head, at, v, m, l);
@@ -414,39 +483,92 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
   if (part >= 0 && h == 0) {
     to[kWideCols * D + col] = m;
     to[kWideCols * (D + 1) + col] = l;
+    if (tile_hi != item->tile_hi) {  // the next item's part has nothing left
+      to[wide_part_floats(D) + kWideCols * D + col] = -INFINITY;
+      to[wide_part_floats(D) + kWideCols * (D + 1) + col] = 0.0f;
+    }
   }
 }
 
-// Joins the parts of cut units: a block per kv head, unit and 16 columns.
+// Items to a block.  The plan cuts for two blocks to a CU; where one fits, it
+// takes two items, as one where they are neighbours of one unit.
+__host__ __device__ constexpr int wide_items(int dtype, int head_dim) {
+  return 32 / wide_wave_cols(dtype, head_dim);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kernel(AttendArgs a) {
+  constexpr int kItems = wide_items(T::code, D);
+  __shared__ WideShape<T, D> lds;
+  const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
+  const int items = head->items, first = static_cast<int>(blockIdx.y) * kItems;
+  for (int n = first; n < min(items, first + kItems); ++n) {
+    const auto* item =
+        reinterpret_cast<ConstItem>(reinterpret_cast<uintptr_t>(a.work) + a.at_items) + n;
+    int tile_hi = item->tile_hi;
+    const bool two = kItems == 2 && n == first && n + 1 < items && item->part >= 0 &&
+                     item[1].part == item->part + 1 && item[1].row == item->row;
+    if (two) tile_hi = item[1].tile_hi;
+    if (n > first) __syncthreads();  // the item before has read its tiles
+    if (item->tokens > 0) wide_item<T, D>(a, item, tile_hi, lds);
+    if (two) break;
+  }
+}
+
+// Joins the parts of cut units: four values of a column to a thread.
+template <int D>
+__host__ __device__ constexpr int join_wide_cols() {
+  return 256 / (D / 4);
+}
+
 template <class T, int D>
 __global__ __launch_bounds__(256) void join_wide_kernel(AttendArgs a) {
-  constexpr int kVecs = D / 4, kGroups = 256 / kVecs;
+  constexpr int kVecs = D / 4;
   const int g = blockIdx.x;
-  const SchedHead* head = reinterpret_cast<const SchedHead*>(a.work);
+  const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
   if (static_cast<int>(blockIdx.y) >= head->joins) return;
   const WideJoin j = reinterpret_cast<const WideJoin*>(a.work + a.at_joins)[blockIdx.y];
-  const int cols = j.tokens * a.group, d = threadIdx.x % kVecs * 4;
+  const int c = blockIdx.z * join_wide_cols<D>() + threadIdx.x / kVecs;
+  const int d = threadIdx.x % kVecs * 4;
+  if (c >= j.tokens * a.group) return;
   const float* from =
       a.parts + (static_cast<size_t>(g) * a.cap_parts + j.part) * wide_part_floats(D);
-  const int stop = min(cols, static_cast<int>(blockIdx.z + 1) * 16);
-  for (int c = blockIdx.z * 16 + threadIdx.x / kVecs; c < stop; c += kGroups) {
-    float m = -INFINITY;
-    for (int p = 0; p < j.parts; ++p) {
-      m = fmaxf(m, from[static_cast<size_t>(p) * wide_part_floats(D) + kWideCols * D + c]);
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int kBatch = 4;  // parts whose loads go out together
+  for (int p0 = 0; p0 < j.parts; p0 += kBatch) {
+    float pm[kBatch], pl[kBatch];
+    f32x4 po[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float* q = from + static_cast<size_t>(min(p0 + u, j.parts - 1)) * wide_part_floats(D);
+      pm[u] = q[kWideCols * D + c];
+      pl[u] = p0 + u < j.parts ? q[kWideCols * (D + 1) + c] : 0.0f;
     }
-    f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-#pragma unroll 4
-    for (int p = 0; p < j.parts; ++p) {
-      const float* q = from + static_cast<size_t>(p) * wide_part_floats(D);
-      const float pm = q[kWideCols * D + c], pl = q[kWideCols * (D + 1) + c];
-      const f32x4 po = *reinterpret_cast<const f32x4*>(q + c * D + d);
-      const float f = pm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pm - m);
-      o += po * f;
-      l += pl * f;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      // no keys, or the part before has them: then nothing was written
+      po[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (pl[u] != 0.0f) {
+        const float* q = from + static_cast<size_t>(p0 + u) * wide_part_floats(D);
+        po[u] = *reinterpret_cast<const f32x4*>(q + c * D + d);
+      }
     }
-    finish4<T>(a, j.row + c / a.group, g * a.group + c % a.group, d, o, m, l);
+    float m2 = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) m2 = p0 + u < j.parts ? fmaxf(m2, pm[u]) : m2;
+    const float keep = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m2);
+    o *= keep;
+    l *= keep;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float f = pm[u] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pm[u] - m2);
+      o += po[u] * f;
+      l += pl[u] * f;
+    }
+    m = m2;
   }
+  finish4<T>(a, j.row + c / a.group, g * a.group + c % a.group, d, o, m, l);
 }
 
 }  // namespace kv
