@@ -438,20 +438,29 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   }
   if (wide_units == 0) return;
 
-  // Longest share C of a wide item.  More blocks than units: units are cut.
-  // Candidates are the even share over k = 1..4; the estimate of each is
-  // (rounds of blocks) x (mean item + 2 tiles for its prologue), no less
-  // than its longest item.
-  constexpr int kCands = 4;
-  int* count = lds + 6 * 16;  // [kCands], then total and longest
-  int* total_at = count + kCands;
-  if (threadIdx.x < kCands + 2) count[threadIdx.x] = 0;
+  // Longest share C of a wide item, from kCands parts of the even share.
+  // Blocks take items longest first, so that a candidate's time is estimated
+  // as its mean load and, where the last round is not full, its shortest
+  // item; no less than its longest.  Four tiles are added to each item for its
+  // start and end.
+  constexpr int kCands = 8;
+  const float kOf[kCands] = {1.25f, 1.125f, 1.0f, 0.625f, 0.5f, 0.4f, 1.0f / 3.0f, 0.25f};
+  int* count = lds + 6 * 16;  // of each candidate: items, longest, shortest; then all tiles and the longest unit
+  int* longest_of = count + kCands;
+  int* shortest_of = longest_of + kCands;
+  auto* total_at = reinterpret_cast<unsigned long long*>(shortest_of + kCands);
+  int* longest_at = shortest_of + kCands + 2;
+  if (threadIdx.x < 3 * kCands + 3) {
+    const int k = static_cast<int>(threadIdx.x) - 2 * kCands;
+    count[threadIdx.x] = k >= 0 && k < kCands ? kMaxLen : 0;
+  }
   __syncthreads();
   // Each unit's request is searched for once, in LDS where the sums fit.
   const int* wide_from = wide_fits ? wide_lds : wide_at;
   WideUnit* wide = reinterpret_cast<WideUnit*>(a.work + a.at_wide);
   const int stored = min(wide_units, a.cap_wide);
-  int mine = 0, longest = 0;
+  unsigned long long mine = 0;  // long prompts of many: past 32 bits
+  int longest = 0;
   for (int u = threadIdx.x; u < stored; u += kPlanThreads) {
     WideUnit w;
     w.request = upper(wide_from, a.requests, u);
@@ -463,45 +472,77 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     mine += w.hi - w.lo;
     longest = max(longest, w.hi - w.lo);
   }
-  mine = wave_sum(mine);
 #pragma unroll
-  for (int d = kWave / 2; d > 0; d >>= 1) longest = max(longest, __shfl_xor(longest, d));
+  for (int d = kWave / 2; d > 0; d >>= 1) {
+    mine += __shfl_xor(mine, d);
+    longest = max(longest, __shfl_xor(longest, d));
+  }
   if (__lane_id() == 0) {
-    atomicAdd(&total_at[0], mine);
-    atomicMax(&total_at[1], longest);
+    atomicAdd(total_at, mine);
+    atomicMax(longest_at, longest);
   }
   __syncthreads();
-  const int total = total_at[0];
-  longest = total_at[1];
-  const int even = max(1, (total + a.wide_blocks - 1) / a.wide_blocks);
-  int cand[kCands], items_of[kCands];
+  longest = *longest_at;
+  const unsigned long long total = *total_at;
+  const int even = static_cast<int>(
+      min(max(1ull, (total + a.wide_blocks - 1) / a.wide_blocks),
+          static_cast<unsigned long long>(kMaxLen)));
+  int share = longest;
+  if (even < longest) {  // else none is cut
+    int cand[kCands], items_of[kCands], high[kCands], low[kCands];
+    float part[kCands];
 #pragma unroll
-  for (int k = 0; k < kCands; ++k) {
-    cand[k] = max(8, (even + k) / (k + 1));
-    items_of[k] = 0;
-  }
-  for (int u = threadIdx.x; u < stored; u += kPlanThreads) {
-    const int tiles_here = wide[u].hi - wide[u].lo;
+    for (int k = 0; k < kCands; ++k) {
+      cand[k] = max(8, static_cast<int>(ceilf(static_cast<float>(even) * kOf[k])));
+      part[k] = 1.0f / static_cast<float>(cand[k]);
+      items_of[k] = high[k] = 0;
+      low[k] = kMaxLen;
+    }
+    for (int u = threadIdx.x; u < stored; u += kPlanThreads) {
+      const int tiles_here = wide[u].hi - wide[u].lo;
 #pragma unroll
-    for (int k = 0; k < kCands; ++k) items_of[k] += (tiles_here + cand[k] - 1) / cand[k];
-  }
+      for (int k = 0; k < kCands; ++k) {
+        // in fp32: an estimate
+        const float cut_f = fmaxf(1.0f, ceilf(static_cast<float>(tiles_here) * part[k]));
+        const int cut = static_cast<int>(cut_f);
+        const int each = static_cast<int>(
+            ceilf(static_cast<float>(tiles_here) * __builtin_amdgcn_rcpf(cut_f)));
+        items_of[k] += cut;
+        high[k] = max(high[k], each);
+        low[k] = min(low[k], each);
+      }
+    }
 #pragma unroll
-  for (int k = 0; k < kCands; ++k) {
-    const int n = wave_sum(items_of[k]);
-    if (__lane_id() == 0) atomicAdd(&count[k], n);
-  }
-  __syncthreads();
-  int share = cand[0];
-  float best = INFINITY;
+    for (int k = 0; k < kCands; ++k) {
+      items_of[k] = wave_sum(items_of[k]);
 #pragma unroll
-  for (int k = 0; k < kCands; ++k) {
-    const int items = max(1, count[k]);
-    const float rounds = static_cast<float>((items + a.wide_blocks - 1) / a.wide_blocks);
-    const float mean = static_cast<float>(total) / static_cast<float>(items) + 2.0f;
-    const float est = fmaxf(rounds * mean, static_cast<float>(min(longest, cand[k])) + 2.0f);
-    if (est < best) {
-      best = est;
-      share = cand[k];
+      for (int d = kWave / 2; d > 0; d >>= 1) {
+        high[k] = max(high[k], __shfl_xor(high[k], d));
+        low[k] = min(low[k], __shfl_xor(low[k], d));
+      }
+      if (__lane_id() == 0) {
+        atomicAdd(&count[k], items_of[k]);
+        atomicMax(&longest_of[k], high[k]);
+        atomicMin(&shortest_of[k], low[k]);
+      }
+    }
+    __syncthreads();
+    share = cand[0];
+    float best = INFINITY;
+#pragma unroll
+    for (int k = 0; k < kCands; ++k) {
+      constexpr float kEnds = 4.0f;
+      const float blocks = static_cast<float>(a.wide_blocks);
+      const float items = static_cast<float>(max(1, count[k]));
+      const float rounds = items / blocks;
+      const float open = ceilf(rounds) - rounds;  // of the last round
+      const float est = fmaxf((static_cast<float>(total) + kEnds * items) / blocks +
+                                  open * (static_cast<float>(shortest_of[k]) + kEnds),
+                              static_cast<float>(longest_of[k]) + kEnds);
+      if (est < best) {
+        best = est;
+        share = cand[k];
+      }
     }
   }
 
@@ -561,7 +602,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
-  __shared__ int lds[kPlanInts];
+  __shared__ __align__(16) int lds[kPlanInts];
   if (blockIdx.x == 0) plan_schedule(a, lds);
   else plan_slots(a, static_cast<int>(blockIdx.x - 1) * kPlanTokens, lds);
 }

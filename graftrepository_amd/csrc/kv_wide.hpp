@@ -79,7 +79,7 @@ __device__ inline f32x4 wide_mul(f16x8 a, f16x8 b, f32x4 c) {
 // instruction stays beside it.
 template <int READS, class Read, class Use>
 __device__ inline void in_step(Read read, Use use) {
-  constexpr int kAhead = 6;
+  constexpr int kAhead = 4;
   f16x8 f[READS];
 #pragma unroll
   for (int i = 0; i < kAhead && i < READS; ++i) f[i] = read(i);
@@ -327,6 +327,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
   for (int tile = tile_lo; tile < tile_hi; ++tile) {
     const int b = (tile - tile_lo) & 1;
     __syncthreads();  // the tile is in LDS; the other buffer is read
+    const GroupScale of[2] = {s_scale[b][h * kPer / 16], s_scale[b][2 + h * kPer / 16]};
     Acc s[2][kHalves];  // of 32 keys each
 #pragma unroll
     for (int r = 0; r < 2 * kHalves; ++r) {
@@ -351,11 +352,6 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
     store_scales(b ^ 1);
     next_codes(tile);
     auto score = [&](int r, int e) { return s[r][e / kAcc][e % kAcc]; };
-    const GroupScale of[2] = {s_scale[b][h * kPer / 16], s_scale[b][2 + h * kPer / 16]};
-    const int seen_0 = s_scale[b][0].there, seen_1 = s_scale[b][1].there;
-    const int seen_2 = s_scale[b][2].there, seen_3 = s_scale[b][3].there;
-    const int seen_now =
-        __builtin_amdgcn_readfirstlane(seen_0 | seen_1 << 1 | seen_2 << 2 | seen_3 << 3);
     const int key0 = tile * kTile;
     // a lane's keys: kPer neighbours of either 32, which share their scales
     float kscale[2], v_log[2], top[2], v_top[2], mul[2];
@@ -365,8 +361,8 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       v_log[r] = of[r].v_log;
       v_top[r] = of[r].v;
     }
-    const bool whole = key0 >= all_from && key0 + kTile - 1 <= wave_first && seen_now == 15;
-    if (whole && __all(!(kscale[0] < 0.0f || kscale[1] < 0.0f))) {
+    const bool whole = key0 >= all_from && key0 + kTile - 1 <= wave_first;
+    if (whole && __all(of[0].there && of[1].there && !(kscale[0] < 0.0f || kscale[1] < 0.0f))) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         top[r] = score(r, 0);
