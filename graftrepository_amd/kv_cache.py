@@ -138,10 +138,18 @@ def _rows(a, what: str, shape) -> tuple[int, str, int, int]:
     return a.data_ptr(), name, st[0], st[1]
 
 
-def _empty(like, shape, dtype: str):
-    if _is_torch(like):
-        return sys.modules["torch"].empty(shape, dtype=_torch_names()[dtype], device=like.device)
-    return DeviceArray(shape, _NUMPY[dtype])
+def _empty(like, shape, dtype: str, stream=None):
+    """Memory beside ``like``.  Torch's belongs to the stream that the call
+    uses, since that is where its last use is when it is freed."""
+    if not _is_torch(like):
+        return DeviceArray(shape, _NUMPY[dtype])
+    t = sys.modules["torch"]
+    if stream is None:
+        return t.empty(shape, dtype=_torch_names()[dtype], device=like.device)
+    on = _stream(like, stream)
+    s = t.cuda.ExternalStream(on, like.device) if on else t.cuda.default_stream(like.device)
+    with t.cuda.stream(s):
+        return t.empty(shape, dtype=_torch_names()[dtype], device=like.device)
 
 
 _raw_stream = None  # torch's current stream of a device as a handle
@@ -177,6 +185,11 @@ class KvBatch:
     ``ctx_lens``, ``new_lens`` and the table updated in place.  ``window``
     limits a token to its last ``window`` tokens; layers with another window
     take a second batch over the same arrays.
+
+    Calls with one batch follow each other: on one stream, or ordered by the
+    caller.  Work that runs at the same time on several streams, replays of
+    captured graphs included, takes a batch each, and a graph's batch stays
+    as long as the graph.
     """
 
     def __init__(self, ctx_lens, new_lens, block_table, block_tokens: int, *, tokens: int,
@@ -226,12 +239,12 @@ class KvBatch:
         self._planned = True
         return self
 
-    def _scratch_on(self, like, need: int, stream: int) -> int:
+    def _scratch_on(self, like, need: int, on: int, stream) -> int:
         """Scratch of a call, one per stream: calls on one stream follow each
         other and may share it."""
-        held = self._held.get(stream)
+        held = self._held.get(on)
         if held is None or held.nbytes < need:
-            held = self._held[stream] = _empty(like, (need,), "u8")
+            held = self._held[on] = _empty(like, (need,), "u8", stream)
         return held.data_ptr()
 
     def _need_plan(self):
@@ -308,14 +321,14 @@ class KvCache:
         shape = (d.tokens, d.heads, self.head_dim)
         qp, name, qt, qh = _rows(q, "q", shape)
         if out is None:
-            out = _empty(q, shape, name)
+            out = _empty(q, shape, name, stream)
             op, ot, oh = out.data_ptr(), shape[1] * shape[2], shape[2]
         else:
             op, oname, ot, oh = _rows(out, "out", shape)
             if oname != name:
                 raise ValueError("out must have q's type")
         if lse is None and return_lse:
-            lse = _empty(q, shape[:2], "f32")
+            lse = _empty(q, shape[:2], "f32", stream)
             lp = lse.data_ptr()
         else:
             lp = _dense(lse, "lse", "f32", shape[:2]) if lse is not None else None
@@ -330,7 +343,7 @@ class KvCache:
         on = _stream(q, stream)
         rc = self._lib.grm_hip_kv_attend(
             self._ref, batch._ref, qp, _lib.DTYPE_CODES[name], qt, qh, op, ot, oh, lp,
-            softmax_scale, batch._scratch_on(q, need, on) if need else None, need, on)
+            softmax_scale, batch._scratch_on(q, need, on, stream) if need else None, need, on)
         if rc:
             _lib.check(rc, "kv attend")
         return (out, lse) if return_lse else out
@@ -347,7 +360,7 @@ class KvCache:
         sp = _dense(starts, "starts", "i32", (n,))
         cp = _dense(cu_rows, "cu_rows", "i32", (n + 1,))
         shape = (int(rows), self.kv_heads, self.head_dim)
-        k, v = _empty(starts, shape, name), _empty(starts, shape, name)
+        k, v = _empty(starts, shape, name, stream), _empty(starts, shape, name, stream)
         rc = self._lib.grm_hip_kv_read(
             self._ref, table, int(block_table.shape[1]), n, sp, cp, shape[0],
             _lib.DTYPE_CODES[name], k.data_ptr(), v.data_ptr(), _stream(starts, stream))

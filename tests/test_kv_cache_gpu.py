@@ -452,3 +452,20 @@ def test_a_cache_past_four_gib(hip_lib):
     want = torch.einsum("hqk,khd->qhd", s.softmax(-1), v.double())
     # fp32 sums of at most 640 terms and 128-term scores below 2^4
     assert (out - want).abs().max() < 640 * 2 ** -24 * 8 + 128 * 2 ** -24 * 16 * 2 * 4
+
+
+def test_results_on_a_stream_that_is_named(hip_lib):
+    """Memory that a call makes belongs to the stream it was given."""
+    s = Setup([300, 10, 900], [1, 30, 1], 2, 128, 32)
+    cache, batch = s.cache(), s.batch(8)
+    q = dev(s.rng.standard_normal((s.tokens, 8, 128)).astype(np.float32), torch.bfloat16)
+    starts, cu = dev(np.array(s.ctx, np.int32)), dev(np.array([0, 1, 31, 32], np.int32))
+    want = (*cache.attend(batch, q, return_lse=True), *cache.read(batch.block_table, starts, cu, 32))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for on in (side, side.cuda_stream, torch.cuda.current_stream(), 0):
+        for _ in range(3):
+            got = (*cache.attend(batch, q, return_lse=True, stream=on),
+                   *cache.read(batch.block_table, starts, cu, 32, stream=on))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
