@@ -580,10 +580,14 @@ __global__ __launch_bounds__(256) void join_narrow_kernel(AttendArgs a, int runs
   if (r0 == r1) return;
   // One block held all of it: finished there.
   if (deal.begin(r0 / 4 * 4) == from && deal.begin(r0 / 4 * 4 + 4) == to) return;
-  // Parts in order: a whole block's, or a run's.
-  auto part_of = [&](int r) -> const float* {
-    const bool whole = from <= deal.begin(r / 4 * 4) && to >= deal.begin(r / 4 * 4 + 4);
-    if (whole && r % 4) return nullptr;
+  // Parts in order: runs up to the first block of runs that the unit holds
+  // whole, a part to each such block, and runs behind them.
+  const int b0 = from <= deal.begin(r0 / 4 * 4) ? r0 / 4 * 4 : r0 / 4 * 4 + 4;
+  const int b1 = to >= deal.begin(r1 / 4 * 4 + 4) ? r1 / 4 * 4 + 4 : r1 / 4 * 4;
+  const int lead = b0 < b1 ? b0 - r0 : r1 + 1 - r0, whole = b0 < b1 ? (b1 - b0) / 4 : 0;
+  const int parts = lead + whole + (b0 < b1 ? max(0, r1 + 1 - b1) : 0);
+  auto part_of = [&](int p) -> const float* {
+    const int r = p < lead ? r0 + p : p < lead + whole ? b0 + 4 * (p - lead) : b1 + p - lead - whole;
     return a.parts +
            narrow_part(g, runs, r, from > deal.begin(r) ? 1 : 0) * (kNarrowCols * (D + 2));
   };
@@ -591,10 +595,7 @@ __global__ __launch_bounds__(256) void join_narrow_kernel(AttendArgs a, int runs
   __shared__ float s_l[kGroups];
   __shared__ f32x4 s_o[kGroups][kVecs];
   float m = -INFINITY;
-  for (int r = r0 + static_cast<int>(threadIdx.x); r <= r1; r += 256) {
-    const float* p = part_of(r);
-    if (p) m = fmaxf(m, p[kNarrowCols * D + c]);
-  }
+  for (int r = threadIdx.x; r < parts; r += 256) m = fmaxf(m, part_of(r)[kNarrowCols * D + c]);
 #pragma unroll
   for (int d = kWave / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
   if (__lane_id() == 0) s_top[threadIdx.x / kWave] = m;
@@ -604,9 +605,8 @@ __global__ __launch_bounds__(256) void join_narrow_kernel(AttendArgs a, int runs
   f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float l = 0.0f;
 #pragma unroll 4
-  for (int r = r0 + group; r <= r1; r += kGroups) {
+  for (int r = group; r < parts; r += kGroups) {
     const float* p = part_of(r);
-    if (!p) continue;
     const float pm = p[kNarrowCols * D + c], pl = p[kNarrowCols * (D + 1) + c];
     const f32x4 po = *reinterpret_cast<const f32x4*>(p + c * D + 4 * d);
     const float f = pm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pm - m);
