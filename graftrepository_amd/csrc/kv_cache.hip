@@ -948,7 +948,6 @@ struct ReadArgs {
 // on, the first at place `place` (of the group) of `cell` (-1: no block).
 struct ReadJob {
   int32_t row, rows, block, place;
-  float scale[2];
 };
 
 constexpr int kReadRows = 64, kReadBatch = 8;
@@ -991,38 +990,45 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   __shared__ ReadJob s_job[kReadRows];
   __shared__ int s_jobs;
   __shared__ __align__(16) int8_t s_v[kReadBatch * 16 * 256];
-  __shared__ int s_cu[kWave];
+  __shared__ float s_scale[2][kReadBatch];
+  __shared__ int s_cu[kWave], s_start[kWave];
   if (threadIdx.x < kWave) {
-    const int row = static_cast<int>(row0) + static_cast<int>(threadIdx.x);
-    const int r0 = find_unit(a.cu, a.requests, static_cast<int>(row0));
-    const int next = r0 + 1 + static_cast<int>(threadIdx.x);
-    s_cu[threadIdx.x] = next < a.requests ? a.cu[next] : 0x7fffffff;
+    const int lane = threadIdx.x, row = static_cast<int>(row0) + lane;
+    // The requests of the block's rows follow each other: 64 are looked at in
+    // LDS, and all of them only where more end here.
+    const int r0 = a.requests <= kWave ? 0 : find_unit(a.cu, a.requests, static_cast<int>(row0));
+    s_cu[lane] = r0 + 1 + lane <= a.requests ? a.cu[r0 + 1 + lane] : 0x7fffffff;
+    s_start[lane] = a.starts[min(r0 + lane, a.requests - 1)];
+    const int cu0 = a.cu[r0];
     __builtin_amdgcn_wave_barrier();
     bool begins = false;
-    ReadJob job{row, 0, -1, 0, {0.0f, 0.0f}};
+    ReadJob job{row, 0, -1, 0};
     if (static_cast<uint64_t>(row) < a.rows) {
-      // the requests of the block's rows follow each other: 64 sums are looked
-      // at in LDS, and all of them only where more end here
-      int r = r0 + (s_cu[0] <= row ? 1 + upper(s_cu, kWave, row) : 0);
-      if (r >= r0 + kWave) r = r0 + kWave + upper(a.cu + r0 + kWave, a.requests - r0 - kWave, row);
-      const int from = a.cu[r], to = min(a.cu[r + 1], static_cast<int>(a.rows));
-      const int pos = a.starts[r] + row - from, j = pos >> a.block_log2;
+      const int ended = s_cu[0] <= row ? 1 + upper(s_cu, kWave, row) : 0;
+      int r = min(r0 + ended, a.requests - 1), from, to, start;
+      if (r < r0 + kWave) {
+        from = r > r0 ? s_cu[r - r0 - 1] : cu0;
+        to = s_cu[r - r0];
+        start = s_start[r - r0];
+      } else {
+        r = r0 + kWave + upper(a.cu + r0 + kWave, a.requests - r0 - kWave, row);
+        from = a.cu[r];
+        to = a.cu[r + 1];
+        start = a.starts[r];
+      }
+      to = min(to, static_cast<int>(a.rows));
+      const int pos = start + row - from, j = pos >> a.block_log2;
       begins = row == from || (pos & 15) == 0;
       job.place = pos & (bs - 1);
       job.rows = min(16 - (pos & 15), to - row);
       if (pos >= 0 && j < a.width) {
         const int block = a.table[static_cast<size_t>(r) * a.width + j];
-        if (static_cast<uint64_t>(static_cast<int64_t>(block)) < a.blocks) {
-          job.block = block;
-          const size_t cell = static_cast<size_t>(block) * a.kv_heads + g;
-          job.scale[0] = a.scales[0][cell];
-          job.scale[1] = a.scales[1][cell];
-        }
+        if (static_cast<uint64_t>(static_cast<int64_t>(block)) < a.blocks) job.block = block;
       }
     }
     const uint64_t all = __ballot(begins);
-    if (begins) s_job[__popcll(all & ((1ull << threadIdx.x) - 1ull))] = job;
-    if (threadIdx.x == 0) s_jobs = __popcll(all);
+    if (begins) s_job[__popcll(all & ((1ull << lane) - 1ull))] = job;
+    if (lane == 0) s_jobs = __popcll(all);
   }
   __syncthreads();
   constexpr int kPer = 16 / sizeof(typename T::store);  // values a thread writes
@@ -1033,68 +1039,79 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   };
   for (int first = 0; first < jobs; first += kReadBatch) {
     const int n = min(kReadBatch, jobs - first);
-    if (a.out[1]) {
-      for (int i0 = threadIdx.x; i0 < n * hd; i0 += 4 * 256) {
-        u32x4 w[4];
+    // Four pieces at a time, so that their loads do not wait for each other.
+    const int keys = a.out[0] ? n * 16 * chunks : 0, columns = a.out[1] ? n * hd : 0;
+    u32x2 kw[4];
+    auto load_keys = [&](int i0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * 256, d = i % hd, k = i / hd;
-          w[u] = u32x4{0u, 0u, 0u, 0u};
-          if (k < n && s_job[first + k].block >= 0) {
-            const ReadJob& job = s_job[first + k];
-            const size_t cell = static_cast<size_t>(job.block) * a.kv_heads + g;
-            w[u] = *reinterpret_cast<const u32x4*>(a.codes[1] + cell * bs * hd +
-                                                   static_cast<size_t>(d) * bs + (job.place & ~15));
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * 256, d = i % hd, k = i / hd;
-          if (k < n) {
-#pragma unroll
-            for (int b = 0; b < 16; ++b) {
-              s_v[(k * 16 + b) * hd + d] = static_cast<int8_t>(code_at(w[u][b / 4], b % 4));
-            }
-          }
-        }
-      }
-    }
-    if (a.out[0]) {
-      // four pieces at a time, so that their loads do not wait for each other
-      for (int i0 = threadIdx.x; i0 < n * 16 * chunks; i0 += 4 * 256) {
-        u32x2 w[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * 256;
-          const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
-          w[u] = u32x2{0u, 0u};
-          if (k < n && b < s_job[first + k].rows && s_job[first + k].block >= 0) {
-            const ReadJob& job = s_job[first + k];
-            const size_t cell = static_cast<size_t>(job.block) * a.kv_heads + g;
-            w[u] = codes_for<T>(a.codes[0] + (cell * bs + job.place + b) * hd + d);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * 256;
-          const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
-          if (k < n && b < s_job[first + k].rows) {
-            put<T>(out_at(0, s_job[first + k].row + b, d), w[u], s_job[first + k].scale[0]);
-          }
-        }
-      }
-    }
-    if (a.out[1]) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n * 16 * chunks; i += 256) {
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * 256;
         const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
-        const ReadJob& job = s_job[first + k];
-        if (b >= job.rows) continue;
-        put<T>(out_at(1, job.row + b, d),
-               codes_for<T>(&s_v[(k * 16 + (job.place & 15) + b) * hd + d]), job.scale[1]);
+        kw[u] = u32x2{0u, 0u};
+        if (i < keys && b < s_job[first + k].rows && s_job[first + k].block >= 0) {
+          const ReadJob& job = s_job[first + k];
+          const size_t cell = static_cast<size_t>(job.block) * a.kv_heads + g;
+          kw[u] = codes_for<T>(a.codes[0] + (cell * bs + job.place + b) * hd + d);
+        }
       }
-      __syncthreads();
+    };
+    float scale = 0.0f;
+    if (threadIdx.x < 2 * kReadBatch) {
+      const int k = threadIdx.x % kReadBatch;
+      if (k < n && s_job[first + k].block >= 0) {
+        scale = a.scales[threadIdx.x / kReadBatch]
+                        [static_cast<size_t>(s_job[first + k].block) * a.kv_heads + g];
+      }
     }
+    load_keys(threadIdx.x);
+    for (int i0 = threadIdx.x; i0 < columns; i0 += 4 * 256) {
+      u32x4 w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * 256, d = i % hd, k = i / hd;
+        w[u] = u32x4{0u, 0u, 0u, 0u};
+        if (i < columns && s_job[first + k].block >= 0) {
+          const ReadJob& job = s_job[first + k];
+          const size_t cell = static_cast<size_t>(job.block) * a.kv_heads + g;
+          w[u] = *reinterpret_cast<const u32x4*>(a.codes[1] + cell * bs * hd +
+                                                 static_cast<size_t>(d) * bs + (job.place & ~15));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * 256, d = i % hd, k = i / hd;
+        if (i < columns) {
+#pragma unroll
+          for (int b = 0; b < 16; ++b) {
+            s_v[(k * 16 + b) * hd + d] = static_cast<int8_t>(code_at(w[u][b / 4], b % 4));
+          }
+        }
+      }
+    }
+    if (threadIdx.x < 2 * kReadBatch) {
+      s_scale[threadIdx.x / kReadBatch][threadIdx.x % kReadBatch] = scale;
+    }
+    __syncthreads();
+    for (int i0 = threadIdx.x; i0 < keys; i0 += 4 * 256) {
+      if (i0 >= 4 * 256) load_keys(i0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * 256;
+        const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
+        if (i < keys && b < s_job[first + k].rows) {
+          put<T>(out_at(0, s_job[first + k].row + b, d), kw[u], s_scale[0][k]);
+        }
+      }
+    }
+    const int values = a.out[1] ? n * 16 * chunks : 0;
+    for (int i = threadIdx.x; i < values; i += 256) {
+      const int d = i % chunks * kPer, b = i / chunks % 16, k = i / chunks / 16;
+      const ReadJob& job = s_job[first + k];
+      if (b >= job.rows) continue;
+      put<T>(out_at(1, job.row + b, d),
+             codes_for<T>(&s_v[(k * 16 + (job.place & 15) + b) * hd + d]), s_scale[1][k]);
+    }
+    __syncthreads();
   }
 }
 

@@ -100,6 +100,9 @@ def _type(a, what: str) -> str:
 
 def _dense(a, what: str, dtype: str, shape) -> int:
     """Address of a contiguous array of this type and shape (None: any)."""
+    if _TORCH and getattr(a, "dtype", None) is _TORCH[dtype] and a.is_cuda and \
+            a.shape == shape and a.is_contiguous():
+        return a.data_ptr()  # the usual call, on its short way
     if _type(a, what) != dtype:
         raise ValueError(f"{what} must be {dtype}, got {a.dtype}")
     got = tuple(a.shape)
@@ -356,7 +359,7 @@ class KvCache:
         if name not in ("f32", "bf16", "f16"):
             raise ValueError("values are read as f32, bf16 or f16")
         n = int(starts.shape[0])
-        table = _dense(block_table, "block_table", "i32", (n, None))
+        table = _dense(block_table, "block_table", "i32", (n, block_table.shape[1]))
         sp = _dense(starts, "starts", "i32", (n,))
         cp = _dense(cu_rows, "cu_rows", "i32", (n + 1,))
         shape = (int(rows), self.kv_heads, self.head_dim)
