@@ -550,32 +550,33 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   }
 }
 
-// Joins the parts of units that several runs share: one block per kv head,
-// column, and unit (or, where there are more units than runs, per boundary
-// between two runs; the first boundary inside a unit does it).  The threads
-// take four output columns each, and the parts in 1024 / D groups.
+// Joins the parts of units that several runs share: one block per kv head and
+// unit (or, where there are more units than runs, per boundary between two
+// runs; the first boundary inside a unit does it) takes every `step`-th of the
+// unit's columns.  The threads take four output columns each, and the parts in
+// 1024 / D groups.
 template <class T, int D>
-__global__ __launch_bounds__(256) void join_narrow_kernel(AttendArgs a, int runs, int by_unit) {
+__device__ inline void join_narrow(const AttendArgs& a, int runs, bool by_unit, int at,
+                                   int first_col, int step) {
   constexpr int kVecs = D / 4, kGroups = 256 / kVecs;
-  const int g = blockIdx.x, c = blockIdx.z;
+  const int g = blockIdx.y;
   const SchedHead* head = reinterpret_cast<const SchedHead*>(a.work);
   const NarrowUnit* units = reinterpret_cast<const NarrowUnit*>(a.work + a.at_units);
   const int32_t* first = reinterpret_cast<const int32_t*>(a.work + a.at_tiles);
   const int total = head->narrow_tiles, n_units = head->units;
   const Deal deal(total, runs);
-  int at = blockIdx.y;
   if (by_unit) {
     if (at >= n_units) return;
   } else {
-    const int t = deal.begin(blockIdx.y + 1);
+    const int t = deal.begin(at + 1), before = deal.begin(at);
     if (t >= total) return;
     at = find_unit(first, n_units, t);
     // not cut here, or cut before
-    if (first[at] >= t || first[at] < deal.begin(blockIdx.y)) return;
+    if (first[at] >= t || first[at] < before) return;
   }
   const int from = first[at], to = first[at + 1];
   const NarrowUnit u = units[at];
-  if (to <= from || c >= u.tokens * a.group) return;
+  if (to <= from) return;
   const int r0 = deal.run(from), r1 = deal.run(to - 1);
   if (r0 == r1) return;
   // One block held all of it: finished there.
@@ -594,35 +595,38 @@ __global__ __launch_bounds__(256) void join_narrow_kernel(AttendArgs a, int runs
   __shared__ float s_top[4];
   __shared__ float s_l[kGroups];
   __shared__ f32x4 s_o[kGroups][kVecs];
-  float m = -INFINITY;
-  for (int r = threadIdx.x; r < parts; r += 256) m = fmaxf(m, part_of(r)[kNarrowCols * D + c]);
+  for (int c = first_col; c < u.tokens * a.group; c += step) {
+    float m = -INFINITY;
+    for (int r = threadIdx.x; r < parts; r += 256) m = fmaxf(m, part_of(r)[kNarrowCols * D + c]);
 #pragma unroll
-  for (int d = kWave / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  if (__lane_id() == 0) s_top[threadIdx.x / kWave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  const int group = threadIdx.x / kVecs, d = threadIdx.x % kVecs;
-  f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float l = 0.0f;
+    for (int d = kWave / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (__lane_id() == 0) s_top[threadIdx.x / kWave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    const int group = threadIdx.x / kVecs, d = threadIdx.x % kVecs;
+    f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
 #pragma unroll 4
-  for (int r = group; r < parts; r += kGroups) {
-    const float* p = part_of(r);
-    const float pm = p[kNarrowCols * D + c], pl = p[kNarrowCols * (D + 1) + c];
-    const f32x4 po = *reinterpret_cast<const f32x4*>(p + c * D + 4 * d);
-    const float f = pm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pm - m);
-    o += po * f;
-    l += pl * f;
-  }
-  s_o[group][d] = o;
-  if (d == 0) s_l[group] = l;
-  __syncthreads();
-  if (group == 0) {
-#pragma unroll
-    for (int k = 1; k < kGroups; ++k) {
-      o += s_o[k][d];
-      l += s_l[k];
+    for (int r = group; r < parts; r += kGroups) {
+      const float* p = part_of(r);
+      const float pm = p[kNarrowCols * D + c], pl = p[kNarrowCols * (D + 1) + c];
+      const f32x4 po = *reinterpret_cast<const f32x4*>(p + c * D + 4 * d);
+      const float f = pm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pm - m);
+      o += po * f;
+      l += pl * f;
     }
-    finish4<T>(a, u.row + c / a.group, g * a.group + c % a.group, 4 * d, o, m, l);
+    s_o[group][d] = o;
+    if (d == 0) s_l[group] = l;
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int k = 1; k < kGroups; ++k) {
+        o += s_o[k][d];
+        l += s_l[k];
+      }
+      finish4<T>(a, u.row + c / a.group, g * a.group + c % a.group, 4 * d, o, m, l);
+    }
+    __syncthreads();  // what LDS holds has been read
   }
 }
 

@@ -87,7 +87,7 @@ __device__ inline void in_step(Read read, Use use) {
   for (int i = 0; i < READS; ++i) {
     if (i + kAhead < READS) f[i + kAhead] = read(i + kAhead);
     use(i, f);
-    __builtin_amdgcn_sched_barrier(0);
+    if (i % 2) __builtin_amdgcn_sched_barrier(0);  // two at a time
   }
 }
 
@@ -518,17 +518,14 @@ __host__ __device__ constexpr int join_wide_cols() {
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(256) void join_wide_kernel(AttendArgs a) {
+__device__ inline void join_wide(const AttendArgs& a, const float* parts, int unit, int piece) {
   constexpr int kVecs = D / 4;
-  const int g = blockIdx.x;
-  const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
-  if (static_cast<int>(blockIdx.y) >= head->joins) return;
-  const WideJoin j = reinterpret_cast<const WideJoin*>(a.work + a.at_joins)[blockIdx.y];
-  const int c = blockIdx.z * join_wide_cols<D>() + threadIdx.x / kVecs;
+  const int g = blockIdx.y;
+  const WideJoin j = reinterpret_cast<const WideJoin*>(a.work + a.at_joins)[unit];
+  const int c = piece * join_wide_cols<D>() + threadIdx.x / kVecs;
   const int d = threadIdx.x % kVecs * 4;
   if (c >= j.tokens * a.group) return;
-  const float* from =
-      a.parts + (static_cast<size_t>(g) * a.cap_parts + j.part) * wide_part_floats(D);
+  const float* from = parts + (static_cast<size_t>(g) * a.cap_parts + j.part) * wide_part_floats(D);
   float m = -INFINITY, l = 0.0f;
   f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kBatch = 4;  // parts whose loads go out together
@@ -565,6 +562,29 @@ __global__ __launch_bounds__(256) void join_wide_kernel(AttendArgs a) {
     m = m2;
   }
   finish4<T>(a, j.row + c / a.group, g * a.group + c % a.group, d, o, m, l);
+}
+
+// What joins the parts of both kernels, in one launch (one for each took 4.5 us
+// more, also where there was nothing to join): `narrow` blocks of narrow units
+// to a kv head, then blocks that go through what the plan cut of wide ones.
+struct JoinShape {
+  const float* wide_parts;
+  int narrow, runs, by_unit, cols;
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, JoinShape s) {
+  const int at = blockIdx.x;
+  if (at < s.narrow) {
+    join_narrow<T, D>(a, s.runs, s.by_unit, at / s.cols, at % s.cols, s.cols);
+    return;
+  }
+  constexpr int kPieces = kWideCols / join_wide_cols<D>();
+  const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
+  const int all = head->joins * kPieces, blocks = gridDim.x - s.narrow;
+  for (int k = at - s.narrow; k < all; k += blocks) {
+    join_wide<T, D>(a, s.wide_parts, k / kPieces, k % kPieces);
+  }
 }
 
 }  // namespace kv
