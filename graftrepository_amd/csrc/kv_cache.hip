@@ -489,45 +489,40 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
           static_cast<unsigned long long>(kMaxLen)));
   int share = longest;
   if (even < longest) {  // else none is cut
-    int cand[kCands], items_of[kCands], high[kCands], low[kCands];
-    float part[kCands];
-#pragma unroll
-    for (int k = 0; k < kCands; ++k) {
-      cand[k] = max(8, static_cast<int>(ceilf(static_cast<float>(even) * kOf[k])));
-      part[k] = 1.0f / static_cast<float>(cand[k]);
-      items_of[k] = high[k] = 0;
-      low[k] = kMaxLen;
-    }
-    for (int u = threadIdx.x; u < stored; u += kPlanThreads) {
-      const int tiles_here = wide[u].hi - wide[u].lo;
-#pragma unroll
-      for (int k = 0; k < kCands; ++k) {
+    auto candidate = [&](float of) {
+      return max(8, static_cast<int>(ceilf(static_cast<float>(even) * of)));
+    };
+    // A candidate to a wavefront, or to several that share the units.
+    constexpr int kShare = kPlanThreads / kWave / kCands;
+    static_assert(kShare >= 1, "a wavefront to each candidate");
+    const int wave = static_cast<int>(threadIdx.x) / kWave, mine_k = wave % kCands;
+    if (wave < kShare * kCands) {
+      const float part = 1.0f / static_cast<float>(candidate(kOf[mine_k]));
+      int items = 0, high = 0, low = kMaxLen;
+      for (int u = wave / kCands * kWave + __lane_id(); u < stored; u += kShare * kWave) {
+        const int tiles_here = wide[u].hi - wide[u].lo;
         // in fp32: an estimate
-        const float cut_f = fmaxf(1.0f, ceilf(static_cast<float>(tiles_here) * part[k]));
-        const int cut = static_cast<int>(cut_f);
-        const int each = static_cast<int>(
-            ceilf(static_cast<float>(tiles_here) * __builtin_amdgcn_rcpf(cut_f)));
-        items_of[k] += cut;
-        high[k] = max(high[k], each);
-        low[k] = min(low[k], each);
+        const float cut = fmaxf(1.0f, ceilf(static_cast<float>(tiles_here) * part));
+        const int each =
+            static_cast<int>(ceilf(static_cast<float>(tiles_here) * __builtin_amdgcn_rcpf(cut)));
+        items += static_cast<int>(cut);
+        high = max(high, each);
+        low = min(low, each);
       }
-    }
-#pragma unroll
-    for (int k = 0; k < kCands; ++k) {
-      items_of[k] = wave_sum(items_of[k]);
 #pragma unroll
       for (int d = kWave / 2; d > 0; d >>= 1) {
-        high[k] = max(high[k], __shfl_xor(high[k], d));
-        low[k] = min(low[k], __shfl_xor(low[k], d));
+        items += __shfl_xor(items, d);
+        high = max(high, __shfl_xor(high, d));
+        low = min(low, __shfl_xor(low, d));
       }
       if (__lane_id() == 0) {
-        atomicAdd(&count[k], items_of[k]);
-        atomicMax(&longest_of[k], high[k]);
-        atomicMin(&shortest_of[k], low[k]);
+        atomicAdd(&count[mine_k], items);
+        atomicMax(&longest_of[mine_k], high);
+        atomicMin(&shortest_of[mine_k], low);
       }
     }
     __syncthreads();
-    share = cand[0];
+    share = candidate(kOf[0]);
     float best = INFINITY;
 #pragma unroll
     for (int k = 0; k < kCands; ++k) {
@@ -541,7 +536,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
                               static_cast<float>(longest_of[k]) + kEnds);
       if (est < best) {
         best = est;
-        share = cand[k];
+        share = candidate(kOf[k]);
       }
     }
   }
