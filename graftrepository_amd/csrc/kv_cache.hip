@@ -330,6 +330,10 @@ __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
 constexpr int kScanInts = 6 * 16 + 32;  // scan sums, and the candidates' counts
 constexpr int kPlanInts = 4 * kPlanChunk + 256;
 
+// The schedule, by one block, beside the blocks that write slots and positions:
+// one scan over the requests for all sums, four requests to a thread, then the
+// units.  Latency: 256 requests of one token take 10 us, 4001 of 1 to 300
+// tokens 27.5, 24 prompts whose units are cut 17.
 __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   int* scratch = lds;                                     // [kScanInts]
   int* tiles_lds = lds + kScanInts;                       // [kPlanChunk]
@@ -764,7 +768,9 @@ __device__ inline void append_values(const AppendArgs& a, const AppendWork<T>& w
 // out as 8 bytes a place.  Values are transposed in their block: 4 places of
 // a column are one word, gathered in LDS, and leave as 16 bytes; where a
 // group of 16 places holds tokens that were there, its old codes are merged.
-// Bound by bytes: a new value is read once and its code written once.
+// A new value is read once and its code written once: 15235 fp16 tokens of 4
+// heads x 256, keys and values, take 28 us (94 MB, 3.3 TB/s; 34.7 us with the
+// divisions themselves, so the vector unit still has its part in it).
 template <class T, int UNITS>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
   constexpr int kWords = 8 * sizeof(typename T::store) / 16;  // 16-byte pieces of 8 values
@@ -978,6 +984,9 @@ __device__ inline u32x2 codes_for(const int8_t* p) {
 // places become jobs (a request's rows follow each other, so there are 4 or
 // 5 of them unless requests are tiny).  A thread writes 16 bytes, its wave 1 KiB.
 // A value column's 16 places are one 16-byte load; they turn through LDS.
+// Bound by bytes: 15521 rows of 4 heads x 256 to fp32, keys and values, take
+// 34 us (159 MB, 4.7 TB/s; a large copy reaches 4.8).  Few rows are latency:
+// 2078 rows of 8 heads x 128 take 11 us, a chain of four loads that miss.
 template <class T>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const int bs = 1 << a.block_log2, hd = a.head_dim, g = blockIdx.y;

@@ -2,19 +2,30 @@
 // chunks of prompts).
 //
 // An item is up to 128 (token, head) columns of one kv head against a range
-// of key tiles (64 tokens).  It is bound by the matrix cores and the vector
-// unit beside them, so the codes are turned into fp16 once per block and tile:
-// a block's four wavefronts load the next tile's codes to registers, write
-// them to LDS as fp16 (exact) in the order in which the matrix instructions
-// take them (16 bytes per lane, no bank conflicts), and each multiplies the
-// tile with its own 32 columns (32x32x16).  Two LDS buffers, one barrier per
-// tile; two blocks share a CU where registers allow, so that one's vector
-// work runs beside the other's matrix work.
+// of key tiles (64 tokens).  A block turns each tile's codes into fp16 once:
+// its wavefronts load the next tiles' codes to registers and write them to LDS
+// as fp16 (exact) in the order in which the matrix instructions take them (16
+// bytes per lane, no bank conflicts); each multiplies the tile with its own
+// columns.  Two LDS buffers, one barrier per tile.
 //
-// Layout of the products (lane = c + 32 h):
-//   S^T = K Q^T: row 8 m + 4 h' + j of a 32-key row tile is its key
-//     16 h' + 4 m + j, so that a lane's 16 results are the neighbouring keys
-//     16 h .. 16 h + 15 of column c;
+// In a wavefront, vector work stands beside matrix work: the codes are turned
+// between the instructions of the first product, and the tile's weights are
+// made between those of the last tile's second product (values are stored a
+// tile later than keys for that).  Two wavefronts share a SIMD.
+//
+// Bound by the vector unit and the matrix cores together.  Prompts of 333 to
+// 4100 tokens (32 heads on 8, head_dim 128, bf16, 167 GFLOP): 215 us of the
+// call's 224, 0.78 PFLOP/s; the vector unit is busy for 63 % of the cycles and
+// the matrix cores for 40 %.  A chunk of 1021 tokens on 14011 (16 heads on 4,
+// head_dim 256, fp16, 243 GFLOP and half as many again for the second term of
+// the weights): 330 us of 347; 42 % and 50 %.
+//
+// Layout of the products (W columns to a wavefront, lane = c + W h):
+//   S^T = K Q^T, 32 columns (32x32x16): row 8 m + 4 h' + j of a 32-key row
+//     tile is its key 16 h' + 4 m + j, so that a lane's 16 results are the
+//     neighbouring keys 16 h .. 16 h + 15 of column c; 16 columns (16x16x32):
+//     row 4 h' + j of 16-row tile r is key 8 h' + 4 r + j of 32 keys, and a
+//     lane has keys 8 h .. 8 h + 7 of each 32;
 //   O^T = V^T P^T: those are the lane's part of the B operand, 8 keys to an
 //     instruction, and the A operand's lane holds the same keys of a value
 //     column.
@@ -36,7 +47,8 @@ namespace kv {
 // Columns of a wavefront.  32 read a tile half as often from LDS as 16; 16
 // need half the registers, and are taken where 32 would fill more than a
 // half of a SIMD's, with one wavefront that nothing covers (attend of 1021
-// tokens on 14011, head_dim 256 in fp16: OLD us with 32, NEW with 16).
+// tokens on 14011, head_dim 256 in fp16: 865 us with 32, 488 with 16; at
+// head_dim 128 32 columns are faster, in bf16 227 us against 317).
 __host__ __device__ constexpr int wide_wave_cols(int dtype, int head_dim) {
   return head_dim == 256 || (dtype == kF32 && head_dim == 128) ? 16 : 32;
 }

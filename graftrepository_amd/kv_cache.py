@@ -267,8 +267,8 @@ class KvCache:
     """The cache of one layer, over the caller's arrays: int8 ``k_codes``
     [blocks, kv_heads, block_tokens, head_dim] and ``v_codes`` [blocks,
     kv_heads, head_dim, block_tokens] (transposed in its block), fp32
-    ``k_scales`` and ``v_scales`` [blocks, kv_heads].  ``KvCache.empty``
-    allocates them."""
+    ``k_scales`` and ``v_scales`` [blocks, kv_heads], 0, positive or NaN.
+    ``KvCache.empty`` allocates them."""
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales):
         self._lib = _lib.load()

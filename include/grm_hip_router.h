@@ -494,7 +494,9 @@ int grm_hip_copy_to_device(void* device, const void* host, uint64_t bytes);
  *           its block: one load reads neighbouring tokens of one column)
  *   k_scales, v_scales [blocks][kv_heads] fp32
  * block_tokens is 16, 32, 64 or 128; head_dim a multiple of 16, at most 256.
- * Code arrays are 16-byte aligned.
+ * Code arrays are 16-byte aligned.  Scales are 0, positive or NaN, as append
+ * writes them; one that is not finite makes every output that sees a token of
+ * its block so too.  Blocks that no token sees may hold anything.
  *
  * A step is a ragged batch: request r holds ctx_lens[r] tokens and brings
  * new_lens[r]; its new token i has position ctx_lens[r] + i and row
@@ -536,7 +538,9 @@ typedef struct grm_kv_batch_desc {
   int32_t requests;
   int32_t table_width;
   int32_t tokens;          /* rows of the per-token arrays, >= sum(new_lens) */
-  int32_t max_new;         /* no new_lens entry is larger */
+  int32_t max_new;         /* no new_lens entry is larger: it decides which
+                              kernels a step launches, and tokens past it may
+                              not be attended */
   int32_t block_tokens;
   int32_t heads;           /* query heads, a multiple of kv_heads */
   int32_t kv_heads;
@@ -553,7 +557,9 @@ int grm_hip_kv_work_bytes(const grm_kv_batch_desc* batch, uint64_t* out_bytes);
  * it in request order, from entry *free_head on, and are entered in
  * block_table; past the list's end they are -1 (their tokens have slot -1,
  * are not written by append and not seen by attend).  A request's tokens
- * past table_width blocks have no slot either. */
+ * past table_width blocks have no slot either.  Append and attend follow the
+ * last plan: lengths, table and rows may change only before the next one.
+ * Lengths below 0 count as 0, and past 2^30 - 256 as that. */
 int grm_hip_kv_plan(const grm_kv_batch_desc* batch, void* stream);
 
 /* Quantise a step's keys and values into their blocks.  k, v [tokens]

@@ -79,7 +79,8 @@ def values(codes, scales, blocks, transposed):
     out = np.zeros((len(blocks), bs, kv, hd), np.float32)
     for i, b in enumerate(blocks):
         if b >= 0:
-            out[i] = (view[b].astype(np.float32) * scales[b][:, None, None]).transpose(1, 0, 2)
+            with np.errstate(invalid="ignore"):    # a scale that is no number
+                out[i] = (view[b].astype(np.float32) * scales[b][:, None, None]).transpose(1, 0, 2)
     return out.reshape(len(blocks) * bs, kv, hd)
 
 
