@@ -280,7 +280,9 @@ extern "C" int grm_hip_kv_attend(const grm_kv_cache_desc* c, const grm_kv_batch_
   a.lse = lse;
   a.ctx_lens = b->ctx_lens;
   a.cu_new = b->cu_new;
-  a.table = b->block_table;
+  // A table without columns may have no memory; entry 0, which the kernels ask
+  // for all the same and do not use, is then the first sum's.
+  a.table = b->table_width ? b->block_table : b->cu_new;
   a.work = static_cast<const char*>(b->work);
   a.q_token_stride = q_token_stride;
   a.q_head_stride = q_head_stride;

@@ -469,3 +469,20 @@ def test_results_on_a_stream_that_is_named(hip_lib):
                    *cache.read(batch.block_table, starts, cu, 32, stream=on))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 48])
+def test_a_table_without_columns(hip_lib, hd):
+    """No token has a block: nothing is written, and every row sees nothing."""
+    s = Setup([0, 5, 0], [1, 0, 40], 2, hd, 16)
+    cache = s.cache()
+    b = KvBatch(dev(np.array(s.ctx, np.int32)), dev(np.array(s.new, np.int32)),
+                torch.empty((3, 0), dtype=torch.int32, device="cuda"), 16, tokens=41, max_new=40,
+                heads=4, kv_heads=2).plan()
+    assert (b.slot_map == -1).all()
+    x = dev(s.rng.standard_normal((41, 2, hd)).astype(np.float32))
+    cache.append(b, x, x)
+    np.testing.assert_array_equal(cache.k_codes.cpu().numpy(), s.kc)
+    q = dev(s.rng.standard_normal((41, 4, hd)).astype(np.float32))
+    out, lse = cache.attend(b, q, return_lse=True)
+    assert not out.any() and torch.isneginf(lse).all()
