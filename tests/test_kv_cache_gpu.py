@@ -486,3 +486,29 @@ def test_a_table_without_columns(hip_lib, hd):
     q = dev(s.rng.standard_normal((41, 4, hd)).astype(np.float32))
     out, lse = cache.attend(b, q, return_lse=True)
     assert not out.any() and torch.isneginf(lse).all()
+
+
+def test_attend_more_items_than_a_grid_dimension(hip_lib):
+    """128 query heads to a kv head: an item to a token, 66000 of them."""
+    n, heads, hd, bs, window = 66_000, 128, 64, 128, 9
+    g = torch.Generator(device="cuda").manual_seed(1)
+    blocks = -(-n // bs)
+    cache = KvCache(torch.randint(-127, 128, (blocks, 1, bs, hd), generator=g, device="cuda",
+                                  dtype=torch.int8),
+                    torch.randint(-127, 128, (blocks, 1, hd, bs), generator=g, device="cuda",
+                                  dtype=torch.int8),
+                    torch.full((blocks, 1), 0.01, device="cuda"),
+                    torch.full((blocks, 1), 0.01, device="cuda"))
+    batch = KvBatch(dev(np.array([0], np.int32)), dev(np.array([n], np.int32)),
+                    torch.arange(blocks, dtype=torch.int32, device="cuda")[None], bs, tokens=n,
+                    max_new=n, heads=heads, kv_heads=1, window=window).plan()
+    q = torch.randn(n, heads, hd, generator=g, device="cuda", dtype=torch.bfloat16)
+    out = cache.attend(batch, q)
+    for row in (0, 8, 32_767, 65_535, 65_536, 65_999):
+        at = torch.arange(max(0, row + 1 - window), row + 1, device="cuda")
+        k = cache.k_codes[at // bs, 0, at % bs].double() * cache.k_scales[0, 0].double()
+        v = cache.v_codes[at // bs, 0, :, at % bs].double() * cache.v_scales[0, 0].double()
+        p = torch.softmax(q[row].double() @ k.t() / hd ** 0.5, -1)
+        # bf16's rounding of the output, fp16's of the weights, fp32 scores
+        bound = 2.0 ** -8 * (p @ v).abs() + 2.0 ** -10 * (p @ v.abs())
+        assert ((out[row].double() - p @ v).abs() <= bound).all(), row
