@@ -140,6 +140,7 @@ struct Shape {
   int cap_parts, cap_items, cap_joins;
   int cus;
   uint64_t units;     // at most so many narrow units
+  int64_t reach;      // tokens that a request can see
   int runs[2];
   uint64_t at_run_units[2];
   uint64_t narrow_bytes, bytes;  // of scratch: the narrow parts, all
@@ -171,6 +172,14 @@ static int shape_of(const grm_kv_cache_desc* c, const Layout& l, Shape* out) {
   return 0;
 }
 
+// Measured with a block to a request and with runs and a join (us a call;
+// sessions x tokens):          1 x 40       16 x 250     1 x 1000     16 x 1000    1 x 2000
+//   bf16, 32 heads on 8 x 128  8.8, 11.5    8.5, 13.0    12.5, 11.9   13.8, 16.5   15.9, 11.7
+//   bf16, 12 on 4 x 64         8.4, 11.5    8.5, 12.0    8.6, 11.7    9.6, 11.4    10.5, 11.7
+//                              (16 x 2000: 14.6, 12.2)
+//   fp16, 16 on 4 x 256        8.7, 12.1    11.0, 16.3   21.1, 15.8 (1 x 500: 13.1, 15.0)
+constexpr int kWholeTokens = 1152;  // to a block, half of it at head_dim 256
+
 template <class T, int D>
 static void launch_cores(AttendArgs a, const Shape& s, hipStream_t stream) {
   const auto kv = static_cast<unsigned>(a.kv_heads);
@@ -180,7 +189,7 @@ static void launch_cores(AttendArgs a, const Shape& s, hipStream_t stream) {
     constexpr int kItems = wide_items(T::code, D);
     AttendArgs b = a;
     b.parts += s.narrow_bytes / 4;
-    const dim3 grid(kv, static_cast<unsigned>((s.cap_items + kItems - 1) / kItems));
+    const unsigned grid = kv * static_cast<unsigned>((s.cap_items + kItems - 1) / kItems);
     attend_wide_kernel<T, D><<<grid, wide_threads(T::code, D), 0, stream>>>(b);
     // eight blocks to a CU, or one to each that there can be
     joins = std::min(s.cap_joins * (kWideCols / join_wide_cols<D>()),
@@ -190,9 +199,14 @@ static void launch_cores(AttendArgs a, const Shape& s, hipStream_t stream) {
     const int k = narrow_blocks_per_cu(T::code, D) - 1;
     a.at_run_units = s.at_run_units[k];
     join.runs = s.runs[k];
-    const dim3 grid(kv, static_cast<unsigned>(join.runs / 4));
+    // A block to a request, without a join, where the table (or the window)
+    // bounds the requests to kWholeTokens and the blocks run all at once.
+    a.whole = s.cap_items == 0 && s.reach <= kWholeTokens * 128 / std::max(128, D) &&
+              s.units * kv <= static_cast<uint64_t>(s.cus) * (k + 1);
+    const dim3 grid(kv, static_cast<unsigned>(a.whole ? s.units : join.runs / 4));
     if (a.block_log2 == 7) attend_narrow_kernel<T, D, 2><<<grid, 256, 0, stream>>>(a);
     else attend_narrow_kernel<T, D, 1><<<grid, 256, 0, stream>>>(a);
+    if (a.whole) return;
     // Blocks to a unit or, where there are fewer, a boundary between two runs:
     // one to a column where eight to a CU are enough for that, else one to a
     // head of the group (three tokens of 7 sessions: 4.6 against 8.5 us; one
@@ -305,6 +319,9 @@ extern "C" int grm_hip_kv_attend(const grm_kv_cache_desc* c, const grm_kv_batch_
   a.at_items = l.at_items;
   a.at_joins = l.at_joins;
   a.cap_parts = sh.cap_parts;
+  const int64_t reach = static_cast<int64_t>(b->table_width) * b->block_tokens;
+  const int64_t seen = b->window ? static_cast<int64_t>(b->window) + b->max_new : reach;
+  sh.reach = std::min(reach, seen);
   a.cols = static_cast<int32_t>(
       std::min<int64_t>(kNarrowCols, static_cast<int64_t>(std::max(1, b->max_new)) * l.group));
   const auto s = static_cast<hipStream_t>(stream);

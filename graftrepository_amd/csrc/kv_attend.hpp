@@ -27,6 +27,7 @@ struct AttendArgs {
   int32_t requests, width, tokens, window;
   int32_t heads, kv_heads, group, head_dim, block_log2;
   int32_t cols;       // columns a narrow unit may have
+  int32_t whole;      // each block of the narrow kernel takes a whole unit
   int32_t cap_parts;  // wide partial results to a kv head
 };
 

@@ -10,7 +10,8 @@
 // tile.  Of a run at most the first and the last request are shared with a
 // neighbour; their partial results (maximum, sum, unnormalised output) go to
 // scratch, and the join kernel adds them in order.  Where the four runs of a
-// block lie in one request, the block adds them itself.  The plan leaves a
+// block lie in one request, the block adds them itself; where requests are
+// known to be short, each has a block, and there is no join.  The plan leaves a
 // unit that each run begins in, so a wave is three loads from its codes.
 //
 // Bound by bytes where there are many: each further byte comes at 6.5 TB/s
@@ -133,14 +134,26 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   const auto* units = reinterpret_cast<ConstUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_units);
   const auto* first = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) + a.at_tiles);
   const auto* table = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.table));
+  const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
   const int run = 4 * blockIdx.y + wave, runs = 4 * gridDim.y;
-  const int start_unit = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) +
-                                                    a.at_run_units)[run];
-  const Deal deal(reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work))->narrow_tiles,
-                  runs);
-  const int begin = deal.begin(run), end = deal.begin(run + 1);
-  const int block_begin = deal.begin(4 * blockIdx.y);
-  const int block_end = deal.begin(4 * blockIdx.y + 4);
+  int start_unit, begin, end, block_begin, block_end;
+  if (a.whole) {
+    start_unit = blockIdx.y;
+    if (start_unit >= head->units) return;
+    block_begin = first[start_unit];
+    block_end = first[start_unit + 1];
+    const int each = (block_end - block_begin + 3) / 4;
+    begin = min(block_end, block_begin + wave * each);
+    end = min(block_end, begin + each);
+  } else {
+    start_unit = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) +
+                                            a.at_run_units)[run];
+    const Deal deal(head->narrow_tiles, runs);
+    begin = deal.begin(run);
+    end = deal.begin(run + 1);
+    block_begin = deal.begin(4 * blockIdx.y);
+    block_end = deal.begin(4 * blockIdx.y + 4);
+  }
   if (block_begin >= block_end) return;
   const int bs = 1 << a.block_log2;
   const uint32_t cell_bytes = static_cast<uint32_t>(bs * D);

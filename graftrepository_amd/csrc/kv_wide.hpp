@@ -124,7 +124,7 @@ struct WideShape {
 // One item's tiles up to tile_hi, which may be the next item's.
 template <class T, int D>
 __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_hi,
-                                 WideShape<T, D>& lds) {
+                                 int g, WideShape<T, D>& lds) {
   typedef WideShape<T, D> S;
   typedef typename S::State State;
   typedef typename S::Acc Acc;
@@ -134,7 +134,6 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
   auto& s_k = lds.k;
   auto& s_v = lds.v;
   auto& s_scale = lds.scale;
-  const int g = blockIdx.x;
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % W, h = lane / W;
   const int tile_lo = item->tile_lo;
@@ -509,7 +508,9 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
   constexpr int kItems = wide_items(T::code, D);
   __shared__ WideShape<T, D> lds;
   const auto* head = reinterpret_cast<ConstHead>(reinterpret_cast<uintptr_t>(a.work));
-  const int items = head->items, first = static_cast<int>(blockIdx.y) * kItems;
+  // in one dimension, which alone has room for millions of tokens
+  const int g = static_cast<int>(blockIdx.x) % a.kv_heads;
+  const int items = head->items, first = static_cast<int>(blockIdx.x) / a.kv_heads * kItems;
   for (int n = first; n < min(items, first + kItems); ++n) {
     const auto* item =
         reinterpret_cast<ConstItem>(reinterpret_cast<uintptr_t>(a.work) + a.at_items) + n;
@@ -518,7 +519,7 @@ __global__ __launch_bounds__(wide_threads(T::code, D), 2) void attend_wide_kerne
                      item[1].part == item->part + 1 && item[1].row == item->row;
     if (two) tile_hi = item[1].tile_hi;
     if (n > first) __syncthreads();  // the item before has read its tiles
-    if (item->tokens > 0) wide_item<T, D>(a, item, tile_hi, lds);
+    if (item->tokens > 0) wide_item<T, D>(a, item, tile_hi, g, lds);
     if (two) break;
   }
 }
