@@ -512,3 +512,14 @@ def test_attend_more_items_than_a_grid_dimension(hip_lib):
         # bf16's rounding of the output, fp16's of the weights, fp32 scores
         bound = 2.0 ** -8 * (p @ v).abs() + 2.0 ** -10 * (p @ v.abs())
         assert ((out[row].double() - p @ v).abs() <= bound).all(), row
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hd,bs", [(64, 16), (128, 128), (256, 32)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_attend_steps_where_the_window_or_the_table_bounds_the_work(hip_lib, dtype, hd, bs, window):
+    """Steps of single tokens: long contexts behind a short window, and short
+    ones on either side of a tile, with a block to a request."""
+    ctx = [2900, 3, 64, 127, 1000] if window else [0, 3, 63, 64, 127, 128, 450]
+    s = Setup(ctx, [1] * len(ctx), 2, hd, bs, seed=hd, holes=[(3, 0)])
+    attend_case(s, 8, window, dtype)
