@@ -45,9 +45,9 @@
 // is 2^-38 of it.  (An allowance of 8 would rescale less often, but lose
 // 2^-32.)
 //
-// For fp16 and fp32 outputs the probabilities are two fp16 terms, the second
-// what the first leaves (one term alone is off by 2.4e-4 of a flat row, more
-// than the rounding to fp16).  For fp16 both are summed in one place.  For
+// The probabilities are two fp16 terms, the second what the first leaves: one
+// term alone is off by up to 2^-12 of each value, which shows in every output
+// whose values cancel.  For 16-bit outputs both are summed in one place.  For
 // fp32 the first is scaled by 2^7, the second by 2^19 more and summed apart,
 // and the maximum follows at once, so that both stay below 2^15 and reach
 // 2^-51 of the largest; fp32 queries are two terms too.
@@ -74,8 +74,7 @@ __device__ __forceinline__ const AttendArgs& late_args() {
 template <class T, int D>
 struct NarrowState {
   static constexpr int kTerms = T::code == kF32 ? 2 : 1;        // of a query
-  static constexpr bool kRest = T::code != kBF16;               // of a probability: two
-  static constexpr bool kApart = T::code == kF32;               // and summed apart
+  static constexpr bool kApart = T::code == kF32;  // a probability's two are summed apart
   static constexpr float kRestScale = kApart ? 524288.0f : 1.0f;
   static constexpr float kRescale = kApart ? 0.0f : 2.0f;
   float col_scale;  // softmax scale, log2 e and the query's own power of two
@@ -425,18 +424,22 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
         for (int h = 0; h < H; ++h) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float p[8];
+            float p[8], v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float sc = s[h][2 * k + (e >> 2)][e & 3];
               p[e] = __builtin_amdgcn_exp2f(fmaf(sc, mul[h], shift));
-              float v = p[e] * v_factor[h];
-              if constexpr (decltype(some_hidden)::value) v = sc == -INFINITY ? 0.0f : v;
-              if constexpr (State::kRest) v = as_rounded(v);
-              w[h][k][e] = static_cast<_Float16>(v);
-              if constexpr (State::kRest) {
-                w_rest[h][k][e] =
-                    static_cast<_Float16>((v - static_cast<float>(w[h][k][e])) * State::kRestScale);
+              v[e] = p[e] * v_factor[h];
+              if constexpr (decltype(some_hidden)::value) v[e] = sc == -INFINITY ? 0.0f : v[e];
+              v[e] = as_rounded(v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const Terms two = terms_of(v[e], v[e + 1]);
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                w[h][k][e + n] = two.first[n];
+                w_rest[h][k][e + n] = static_cast<_Float16>(two.left[n] * State::kRestScale);
               }
             }
             st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
@@ -459,10 +462,8 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][k], w[h][k], st.o[d], 0, 0, 0);
-            if constexpr (State::kRest) {
-              f32x4& o = State::kApart ? st.rest[d] : st.o[d];
-              o = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][k], w_rest[h][k], o, 0, 0, 0);
-            }
+            f32x4& o = State::kApart ? st.rest[d] : st.o[d];
+            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][k], w_rest[h][k], o, 0, 0, 0);
           }
         }
         if (d + kHeld < kValueTiles) load_values(cur, d + kHeld);

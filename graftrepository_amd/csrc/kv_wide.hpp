@@ -30,7 +30,7 @@
 //     instruction, and the A operand's lane holds the same keys of a value
 //     column.
 // The softmax is the narrow kernel's: one pass, scores and statistics in fp32,
-// weights in fp16 (two terms for fp16 and fp32 outputs).
+// weights as two fp16 terms.
 //
 // Items of one kv head follow each other at a distance of kv_heads blocks, so
 // with 8 kv heads an XCD's L2 serves one of them.
@@ -312,12 +312,10 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
         [&](int i, const f16x8(&f)[kValueReads]) {
           const int d = i % kTilesD, rk = i / kTilesD;
           o[d] = wide_mul(f[i], w[rk / (kPer / 8)][rk % (kPer / 8)], o[d]);
-          if constexpr (State::kRest) {
-            // a step of its own sums later, which need not wait for the first's
-            for (int n = max(0, i - kLag); n <= (i == kValueReads - 1 ? i : i - kLag); ++n) {
-              Acc& to = State::kApart ? rest[n % kTilesD] : o[n % kTilesD];
-              to = wide_mul(f[n], w_rest[n / kTilesD / (kPer / 8)][n / kTilesD % (kPer / 8)], to);
-            }
+          // a step of its own sums later, which need not wait for the first's
+          for (int n = max(0, i - kLag); n <= (i == kValueReads - 1 ? i : i - kLag); ++n) {
+            Acc& to = State::kApart ? rest[n % kTilesD] : o[n % kTilesD];
+            to = wide_mul(f[n], w_rest[n / kTilesD / (kPer / 8)][n / kTilesD % (kPer / 8)], to);
           }
           beside(i);
         });
@@ -435,19 +433,23 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
     f16x8 w2[2][kPer / 8], w2_rest[2][kPer / 8];
     float sum[2] = {0.0f, 0.0f};
     multiply(b ^ 1, [&](int i) {
+      // two weights at a time, spread over the reads
+      constexpr int kEvery = kValueReads > kPer ? kValueReads / kPer : 1;
+      constexpr int kCount = kPer > kValueReads ? kPer / kValueReads : 1;
+      if ((i + 1) % kEvery != 0) return;
 #pragma unroll
-      for (int j = i * kPer / kValueReads; j < (i + 1) * kPer / kValueReads; ++j) {
-        const int r = 2 * j / kPer;  // two weights at a time
+      for (int u = 0; u < kCount; ++u) {
+        const int j = ((i + 1) / kEvery - 1) * kCount + u, r = 2 * j / kPer;
+        const int e = 2 * j % kPer;
+        const float p[2] = {__builtin_amdgcn_exp2f(fmaf(score(r, e), mul[r], at[r])),
+                            __builtin_amdgcn_exp2f(fmaf(score(r, e + 1), mul[r], at[r]))};
+        const Terms two = terms_of(p[0], p[1]);
 #pragma unroll
-        for (int e = 2 * j % kPer; e < 2 * j % kPer + 2; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(score(r, e), mul[r], at[r]));
-          const _Float16 first = static_cast<_Float16>(p);
-          w2[r][e / 8][e % 8] = first;
-          if constexpr (State::kRest) {
-            w2_rest[r][e / 8][e % 8] =
-                static_cast<_Float16>((p - static_cast<float>(first)) * State::kRestScale);
-          }
-          sum[r] += p;
+        for (int k = 0; k < 2; ++k) {
+          w2[r][(e + k) / 8][(e + k) % 8] = two.first[k];
+          w2_rest[r][(e + k) / 8][(e + k) % 8] =
+              static_cast<_Float16>(two.left[k] * State::kRestScale);
+          sum[r] += p[k];
         }
       }
     });
@@ -457,7 +459,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
 #pragma unroll
       for (int k = 0; k < kPer / 8; ++k) {
         w[r][k] = w2[r][k];
-        if constexpr (State::kRest) w_rest[r][k] = w2_rest[r][k];
+        w_rest[r][k] = w2_rest[r][k];
       }
     }
   }

@@ -1,0 +1,46 @@
+"""How many bits the 8-bit cache's attention keeps where a plain form in fp32
+keeps them: weights whose products cancel, queries whose channels are of very
+unlike size, value scales far from 1."""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from oracle import kv as law  # noqa: E402
+from tests.test_kv_cache_gpu import TYPES, Setup, dev  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(s, q, heads, dtype, window=0):
+    """(out, lse) in fp64 on the host, and the queries' values as held."""
+    t = dev(q.astype(np.float32), TYPES[dtype])
+    out, lse = s.cache().attend(s.batch(heads, window), t, 1 / np.sqrt(s.hd), return_lse=True)
+    return out.double().cpu().numpy(), lse.double().cpu().numpy(), t.float().cpu().numpy()
+
+
+def within(s, got, q, heads, dtype, window=0):
+    """Against 64 bits, within the bound of fp32 weights (whole ones: 2^-20)."""
+    o, l, ob, lb = law.attend(q, s.kc, s.vc, s.ks, s.vs, s.ctx, s.new, s.table,
+                              float(np.float32(1 / np.sqrt(s.hd))), window, dtype, half_p=False)
+    off = np.abs(got[0] - o) - ob
+    assert (off <= 0).all(), (float((off / ob).max()), np.argwhere(off > 0)[:4].tolist())
+    assert (np.abs(got[1] - l) <= lb).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128, 256, 48])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_16_bit_outputs_keep_the_weights_second_term(hip_lib, dtype, hd, new):
+    """Values that cancel but for the small difference of two blocks' scales:
+    weights of 11 bits are off by 2^-12 of what cancels, several times the
+    bound, in which the output's own rounding is small."""
+    s = Setup([32], [new], 2, hd, 16, seed=hd + new)
+    a, b = s.table[0, :2]
+    s.vc[b] = -s.vc[a]
+    s.vc[s.table[0, 2:4]] = 0                      # the new tokens' own values
+    s.vs[a] = s.vs[b] * np.float32(1 + 2.0 ** -10)
+    q = np.zeros((s.tokens, 8, hd))
+    got = attend(s, q, 8, dtype)
+    within(s, got, got[2], 8, dtype)
