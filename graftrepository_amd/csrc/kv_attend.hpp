@@ -1,6 +1,6 @@
 // kv_attend.hpp -- what the attention kernels of the 8-bit key/value cache
-// share: their arguments, int8 codes to fp16, queries to fp16 terms, and the
-// last step of a row.
+// share: their arguments, codes and queries as operands of the matrix cores,
+// and the last step of a row.
 #pragma once
 
 #include "kv_common.hpp"
@@ -44,29 +44,64 @@ __device__ inline size_t narrow_part(int g, int runs, int run, int which) {
   return (static_cast<size_t>(g) * runs + run) * 2 + which;
 }
 
-// Eight codes to fp16, exactly: a byte under the exponent of 1024 is
-// 1024 + u, and u = code + 128.
-__device__ inline f16x8 codes_to_f16(uint32_t first, uint32_t second) {
-  const f16x2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
-  f16x8 out;
+// A lane's eight values of an operand, all fp16 or (BF) all bf16.
+template <bool BF>
+__device__ inline f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (BF) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+template <bool BF>
+__device__ inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (BF) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+// The upper halves of two words: two fp32 values as bf16, cut.
+__device__ inline uint32_t upper_halves(uint32_t lo, uint32_t hi) {
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+}
+
+// Eight codes, exactly.  fp16: a byte under the exponent of 1024 is 1024 + u,
+// and u = code + 128.  bf16: by fp32, of which an integer below 256 needs the
+// upper half only (12 instructions against 10).
+template <bool BF>
+__device__ inline u32x4 codes_as(uint32_t first, uint32_t second) {
+  u32x4 out;
+  if constexpr (BF) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const uint32_t u = (k ? second : first) ^ 0x80808080u;
-    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
-    const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-    const f16x2 a = __builtin_bit_cast(f16x2, lo) + off;
-    const f16x2 b = __builtin_bit_cast(f16x2, hi) + off;
-    out[4 * k] = a[0];
-    out[4 * k + 1] = a[1];
-    out[4 * k + 2] = b[0];
-    out[4 * k + 3] = b[1];
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = k < 2 ? first : second;
+      out[k] = upper_halves(__float_as_uint(static_cast<float>(code_at(w, 2 * (k & 1)))),
+                            __float_as_uint(static_cast<float>(code_at(w, 2 * (k & 1) + 1))));
+    }
+  } else {
+    const f16x2 off = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t u = (k ? second : first) ^ 0x80808080u;
+      const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+      const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+      out[2 * k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, lo) + off);
+      out[2 * k + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, hi) + off);
+    }
   }
   return out;
 }
 
-__device__ inline void codes_to_f16(u32x4 w, f16x8 (&out)[2]) {
-  out[0] = codes_to_f16(w[0], w[1]);
-  out[1] = codes_to_f16(w[2], w[3]);
+template <bool BF>
+__device__ inline void codes_as(u32x4 w, u32x4 (&out)[2]) {
+  out[0] = codes_as<BF>(w[0], w[1]);
+  out[1] = codes_as<BF>(w[2], w[3]);
 }
 
 // A product as fp32 holds it.  Left open, the compiler rounds it to fp16 from
@@ -116,26 +151,43 @@ __device__ inline void load8(const typename T::store* p, float (&x)[8]) {
   }
 }
 
-// Query values to fp16 terms, in units of a power of two that brings the
-// column's largest (`top`) into [1/2, 1): bf16's range is wider than fp16's,
-// and what falls below 2^-24 of the largest is below fp32's own rounding of
-// the sum.  fp16 queries are taken as they are.  Returns `scale` times the
-// unit.
+// Query values as terms of the first product.  fp16 is taken as it is.  bf16
+// and fp32 go as bf16 (one term, three), which holds every bit of channels of
+// any size beside each other: a key may have nothing in the largest.  They are
+// in units of a power of two that brings the column's largest (`top`) into
+// [1/2, 1), for sums that stay in range.  Returns `scale` times the unit.
+template <class T>
+__host__ __device__ constexpr bool query_bf16() { return T::code != kF16; }
+
 template <class T, int N, int TERMS>
 __device__ inline float split_query(const float (&x)[N][8], float top, float scale,
-                                    f16x8 (&q)[TERMS][N]) {
+                                    u32x4 (&q)[TERMS][N]) {
   int unit = 0;
-  if constexpr (T::code != kF16) {
+  if constexpr (query_bf16<T>()) {
     if (top > 0.0f && top <= 3.4028235e38f) unit = __builtin_amdgcn_frexp_expf(top);
   }
 #pragma unroll
   for (int s = 0; s < N; ++s) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = T::code == kF16 ? x[s][e] : __builtin_amdgcn_ldexpf(x[s][e], -unit);
-      q[0][s][e] = static_cast<_Float16>(v);
-      if constexpr (TERMS == 2) {
-        q[1][s][e] = static_cast<_Float16>(v - static_cast<float>(q[0][s][e]));
+    for (int e = 0; e < 8; e += 2) {
+      if constexpr (query_bf16<T>()) {
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[k] = __builtin_amdgcn_ldexpf(x[s][e + k], -unit);
+#pragma unroll
+        for (int n = 0; n < TERMS; ++n) {
+          // eight bits, cut; what is left is exact
+          q[n][s][e / 2] = upper_halves(__float_as_uint(v[0]), __float_as_uint(v[1]));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            v[k] -= __uint_as_float(__float_as_uint(v[k]) & 0xffff0000u);
+          }
+        }
+      } else {
+        f16x2 v;
+        v[0] = static_cast<_Float16>(x[s][e]);
+        v[1] = static_cast<_Float16>(x[s][e + 1]);
+        q[0][s][e / 2] = __builtin_bit_cast(uint32_t, v);
       }
     }
   }

@@ -21,8 +21,8 @@
 // and 5; 48 sessions of 32 to 4095 tokens at head_dim 256 (77 MB) 30 and 5.
 // Codes through LDS by direct loads measured 4.35 TB/s instead.
 //
-// Inside a tile both products run on the matrix cores in fp16, where an int8
-// code is exact (16x16x32; rows: 16 keys or 16 value columns, columns: the
+// Inside a tile both products run on the matrix cores in fp16 or bf16, where an
+// int8 code is exact (16x16x32; rows: 16 keys or 16 value columns, columns: the
 // queries):
 //   S^T = K Q^T: lane (i, G) = (lane % 16, lane / 16) loads 16 bytes of one
 //     key: of half h of the tile, code row 16 (i / 4) + 4 t + i % 4 for row
@@ -50,7 +50,7 @@
 // whose values cancel.  For 16-bit outputs both are summed in one place.  For
 // fp32 the first is scaled by 2^7, the second by 2^19 more and summed apart,
 // and the maximum follows at once, so that both stay below 2^15 and reach
-// 2^-51 of the largest; fp32 queries are two terms too.
+// 2^-51 of the largest; fp32 queries are three bf16 terms.
 #pragma once
 
 #include "kv_attend.hpp"
@@ -73,7 +73,7 @@ __device__ __forceinline__ const AttendArgs& late_args() {
 // Everything one wave carries for one unit.
 template <class T, int D>
 struct NarrowState {
-  static constexpr int kTerms = T::code == kF32 ? 2 : 1;        // of a query
+  static constexpr int kTerms = T::code == kF32 ? 3 : 1;  // of a query
   static constexpr bool kApart = T::code == kF32;  // a probability's two are summed apart
   static constexpr float kRestScale = kApart ? 524288.0f : 1.0f;
   static constexpr float kRescale = kApart ? 0.0f : 2.0f;
@@ -91,7 +91,7 @@ struct UnitView {
 
 template <class T, int D>
 __device__ inline void narrow_query(const AttendArgs& a, const UnitView& u, int g,
-                                    NarrowState<T, D>& st, f16x8* s_q) {
+                                    NarrowState<T, D>& st, u32x4* s_q) {
   const int lane = __lane_id(), i = lane & 15, G = lane >> 4;
   const bool mine = i < u.tokens * a.group;
   const int t = mine ? i / a.group : 0, h = mine ? i % a.group : 0;
@@ -111,7 +111,7 @@ __device__ inline void narrow_query(const AttendArgs& a, const UnitView& u, int 
   }
   top = fmaxf(top, __shfl_xor(top, 16));
   top = fmaxf(top, __shfl_xor(top, 32));
-  f16x8 f[NarrowState<T, D>::kTerms][D / 32];
+  u32x4 f[NarrowState<T, D>::kTerms][D / 32];
   st.col_scale = split_query<T, D / 32>(x, top, a.scale * kLog2e, f);
 #pragma unroll
   for (int e = 0; e < NarrowState<T, D>::kTerms; ++e) {
@@ -239,9 +239,14 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   };
 
   // The unit's queries, as the lane's part of the B operands: in LDS, so that
-  // they take registers during the first product only.
-  __shared__ f16x8 s_queries[4][State::kTerms * (D / 32)][kWave];
-  f16x8* s_q = &s_queries[wave][0][0];
+  // they take registers during the first product only;
+  // their memory is the outputs' when the waves are done with them.
+  union Lds {
+    u32x4 q[4][State::kTerms * (D / 32)][kWave];
+    float o[4][16][D];
+  };
+  __shared__ Lds s_lds;
+  u32x4* s_q = &s_lds.q[wave][0][0];
 
   State st;
   auto reset = [&]() {
@@ -298,26 +303,29 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
       }
       // products of the halves' keys 16 G + 4 r + j
       f32x4 s[H][4];
-      f16x8 q[State::kTerms][D / 32];
+      u32x4 q[State::kTerms][D / 32];
 #pragma unroll
       for (int e = 0; e < State::kTerms; ++e) {
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) q[e][k] = s_q[(e * (D / 32) + k) * kWave + lane];
       }
       auto multiply = [&](int h, int r) {
-        s[h][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        // the lesser terms apart: their sums are small, and so is what they round
+        f32x4 sum[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
-          f16x8 c[2];
-          codes_to_f16(kr[r][p], c);
+          u32x4 c[2];
+          codes_as<query_bf16<T>()>(kr[r][p], c);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
 #pragma unroll
             for (int e = 0; e < State::kTerms; ++e) {
-              s[h][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[k], q[e][2 * p + k], s[h][r], 0, 0, 0);
+              f32x4& to = sum[e ? 1 : 0];
+              to = mfma<query_bf16<T>()>(c[k], q[e][2 * p + k], to);
             }
           }
         }
+        s[h][r] = State::kTerms > 1 ? sum[0] + sum[1] : sum[0];
       };
       if constexpr (H == 2) {
 #pragma unroll
@@ -454,16 +462,16 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
 
 #pragma unroll
       for (int d = 0; d < kValueTiles; ++d) {
-        f16x8 c[H][2];
+        u32x4 c[H][2];
 #pragma unroll
-        for (int h = 0; h < H; ++h) codes_to_f16(vr[d % kHeld][h], c[h]);
+        for (int h = 0; h < H; ++h) codes_as<false>(vr[d % kHeld][h], c[h]);
 #pragma unroll
         for (int h = 0; h < H; ++h) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][k], w[h][k], st.o[d], 0, 0, 0);
+            st.o[d] = mfma<false>(c[h][k], __builtin_bit_cast(u32x4, w[h][k]), st.o[d]);
             f32x4& o = State::kApart ? st.rest[d] : st.o[d];
-            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][k], w_rest[h][k], o, 0, 0, 0);
+            o = mfma<false>(c[h][k], __builtin_bit_cast(u32x4, w_rest[h][k]), o);
           }
         }
         if (d + kHeld < kValueTiles) load_values(cur, d + kHeld);
@@ -513,7 +521,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   // The block's first tile decides for all four waves alike; a wave without
   // a run of its own adds nothing.
   __shared__ float s_ml[2][4][16];
-  __shared__ float s_o[4][16][D];
+  auto& s_o = s_lds.o;
   __shared__ int s_unit[2];  // wave 0 has the first run
   if (threadIdx.x == 0) {
     s_unit[0] = spans;

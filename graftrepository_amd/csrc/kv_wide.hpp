@@ -2,9 +2,9 @@
 // chunks of prompts).
 //
 // An item is up to 128 (token, head) columns of one kv head against a range
-// of key tiles (64 tokens).  A block turns each tile's codes into fp16 once:
-// its wavefronts load the next tiles' codes to registers and write them to LDS
-// as fp16 (exact) in the order in which the matrix instructions take them (16
+// of key tiles (64 tokens).  A block turns each tile's codes into fp16 or bf16
+// once: its wavefronts load the next tiles' codes to registers and write them to
+// LDS as such (exact) in the order in which the matrix instructions take them (16
 // bytes per lane, no bank conflicts); each multiplies the tile with its own
 // columns.  Two LDS buffers, one barrier per tile.
 //
@@ -79,20 +79,13 @@ __device__ inline float across(float v, F join) {
   return v;
 }
 
-__device__ inline f32x16 wide_mul(f16x8 a, f16x8 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-__device__ inline f32x4 wide_mul(f16x8 a, f16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
 // A product's reads from LDS and what is done with each, in this order: reads
 // run kAhead before their use, and what `use` does beside the matrix
 // instruction stays beside it.
 template <int READS, class Read, class Use>
 __device__ inline void in_step(Read read, Use use) {
   constexpr int kAhead = 4;
-  f16x8 f[READS];
+  u32x4 f[READS];
 #pragma unroll
   for (int i = 0; i < kAhead && i < READS; ++i) f[i] = read(i);
 #pragma unroll
@@ -116,8 +109,8 @@ struct WideShape {
   typedef typename std::conditional<W == 32, f32x16, f32x4>::type Acc;
 
   // a lane's eight values of an instruction's operand
-  f16x8 k[2][2 * kHalves * kSteps * kWave];       // [row tile][step][lane]
-  f16x8 v[2][kTilesD * 2 * kPer / 8 * kWave];     // [d tile][32 keys][lane]
+  u32x4 k[2][2 * kHalves * kSteps * kWave];       // [row tile][step][lane]
+  u32x4 v[2][kTilesD * 2 * kPer / 8 * kWave];     // [d tile][32 keys][lane]
   GroupScale scale[2][4];                         // of a group of 16 tokens
 };
 
@@ -207,13 +200,13 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       const int step = chunk * 16 / kStepD, first = chunk * 16 % kStepD / 8;
       s_k[b ^ 1][(row_tile * kSteps + step) * kWave + (first + half) * W +
                  (W == 32 ? 16 * token8 : 0) + k_slot] =
-          codes_to_f16(k_reg[q][2 * half], k_reg[q][2 * half + 1]);
+          codes_as<query_bf16<T>()>(k_reg[q][2 * half], k_reg[q][2 * half + 1]);
     } else {
       const int d = part_of * (D / 2) + q * kWave + lane;
       const int at =
           W == 32 ? ((d / 32 * 2 + (grp >> 1)) * 2 + half) * kWave + d % 32 + 32 * (grp & 1)
                   : (d / 16 * 2 + (grp >> 1)) * kWave + d % 16 + 32 * (grp & 1) + 16 * half;
-      s_v[b][at] = codes_to_f16(v_reg[q][2 * half], v_reg[q][2 * half + 1]);
+      s_v[b][at] = codes_as<false>(v_reg[q][2 * half], v_reg[q][2 * half + 1]);
     }
   };
   auto store_scales = [&](int b) {
@@ -244,7 +237,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
     load_values();
     load_id(min(tile_lo + 1, tile_last));
   }
-  f16x8 q[State::kTerms][kSteps];
+  u32x4 q[State::kTerms][kSteps];
   float col_scale;
   {
     const typename T::store* from = static_cast<const typename T::store*>(a.q) +
@@ -309,13 +302,15 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
   constexpr int kLag = State::kApart ? 0 : 2;
   auto multiply = [&](int b, auto beside) {
     in_step<kValueReads>([&](int i) { return s_v[b][(i % kTilesD * 2 * (kPer / 8) + i / kTilesD) * kWave + lane]; },
-        [&](int i, const f16x8(&f)[kValueReads]) {
+        [&](int i, const u32x4(&f)[kValueReads]) {
           const int d = i % kTilesD, rk = i / kTilesD;
-          o[d] = wide_mul(f[i], w[rk / (kPer / 8)][rk % (kPer / 8)], o[d]);
+          o[d] = mfma<false>(f[i], __builtin_bit_cast(u32x4, w[rk / (kPer / 8)][rk % (kPer / 8)]), o[d]);
           // a step of its own sums later, which need not wait for the first's
           for (int n = max(0, i - kLag); n <= (i == kValueReads - 1 ? i : i - kLag); ++n) {
             Acc& to = State::kApart ? rest[n % kTilesD] : o[n % kTilesD];
-            to = wide_mul(f[n], w_rest[n / kTilesD / (kPer / 8)][n / kTilesD % (kPer / 8)], to);
+            to = mfma<false>(f[n],
+                            __builtin_bit_cast(u32x4, w_rest[n / kTilesD / (kPer / 8)][n / kTilesD % (kPer / 8)]),
+                            to);
           }
           beside(i);
         });
@@ -338,20 +333,28 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
     __syncthreads();  // the tile is in LDS; the other buffer is read
     const GroupScale of[2] = {s_scale[b][h * kPer / 16], s_scale[b][2 + h * kPer / 16]};
     Acc s[2][kHalves];  // of 32 keys each
+    constexpr bool kLesser = State::kTerms > 1;  // a query's lesser terms are summed apart
+    Acc lesser[kLesser ? 2 * kHalves : 1];
 #pragma unroll
     for (int r = 0; r < 2 * kHalves; ++r) {
 #pragma unroll
-      for (int e = 0; e < kAcc; ++e) s[r / kHalves][r % kHalves][e] = 0.0f;
+      for (int e = 0; e < kAcc; ++e) {
+        s[r / kHalves][r % kHalves][e] = 0.0f;
+        if constexpr (kLesser) lesser[r][e] = 0.0f;
+      }
     }
     constexpr int kKeyReads = 2 * kHalves * kSteps;
     in_step<kKeyReads>(
         [&](int i) {
           return s_k[b][(i % (2 * kHalves) * kSteps + i / (2 * kHalves)) * kWave + k_read];
         },
-        [&](int i, const f16x8(&f)[kKeyReads]) {
-          Acc& to = s[i % (2 * kHalves) / kHalves][i % kHalves];
+        [&](int i, const u32x4(&f)[kKeyReads]) {
+          constexpr int kRows = 2 * kHalves;
 #pragma unroll
-          for (int e = 0; e < State::kTerms; ++e) to = wide_mul(f[i], q[e][i / (2 * kHalves)], to);
+          for (int e = 0; e < State::kTerms; ++e) {
+            Acc& to = e ? lesser[i % kRows * kLesser] : s[i % kRows / kHalves][i % kHalves];
+            to = mfma<query_bf16<T>()>(f[i], q[e][i / kRows], to);
+          }
 #pragma unroll
           for (int piece = i * kPieces / kKeyReads; piece < (i + 1) * kPieces / kKeyReads;
                ++piece) {
@@ -360,6 +363,10 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
         });
     store_scales(b ^ 1);
     next_codes(tile);
+    if constexpr (kLesser) {
+#pragma unroll
+      for (int r = 0; r < 2 * kHalves; ++r) s[r / kHalves][r % kHalves] += lesser[r];
+    }
     auto score = [&](int r, int e) { return s[r][e / kAcc][e % kAcc]; };
     const int key0 = tile * kTile;
     // a lane's keys: kPer neighbours of either 32, which share their scales

@@ -44,3 +44,19 @@ def test_16_bit_outputs_keep_the_weights_second_term(hip_lib, dtype, hd, new):
     q = np.zeros((s.tokens, 8, hd))
     got = attend(s, q, 8, dtype)
     within(s, got, got[2], 8, dtype)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128, 256, 48])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_queries_of_unlike_channels_keep_their_bits(hip_lib, dtype, hd, new):
+    """One channel far above the others, and no key has anything in it: the
+    scores are the others' alone, with all their bits."""
+    s = Setup([100], [new], 2, hd, 16, seed=hd + new)
+    s.kc[:, :, :, 5] = 0
+    q = s.rng.standard_normal((s.tokens, 8, hd)) * 2
+    q[..., 5] = 2.0 ** (15 if dtype == "f16" else 24)
+    got = attend(s, q, 8, dtype)
+    rest = got[2].copy()
+    rest[..., 5] = 0.0
+    within(s, got, rest, 8, dtype)
