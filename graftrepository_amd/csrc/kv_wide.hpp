@@ -63,10 +63,10 @@ __host__ __device__ constexpr int wide_part_floats(int head_dim) {
 }
 
 // Scales of 16 tokens, 0 where they have no block or none of the item's
-// columns sees them, and the value scale's logarithm (0 for no number).
+// columns sees them.
 struct __align__(16) GroupScale {
-  float k, v, v_log;
-  int there;
+  float k, v;
+  int there, pad;
 };
 
 constexpr float kLargest = 3.0e38f;  // below are numbers
@@ -211,9 +211,8 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
   };
   auto store_scales = [&](int b) {
     if (part_of == 0 && lane == 0) {
-      const float v = there_reg ? v_scale_reg : 0.0f;
-      s_scale[b][grp] = {there_reg ? k_scale_reg : 0.0f, v,
-                         v <= kLargest ? __builtin_amdgcn_logf(v) : 0.0f, there_reg};
+      s_scale[b][grp] = {there_reg ? k_scale_reg : 0.0f, there_reg ? v_scale_reg : 0.0f, there_reg,
+                         0};
     }
   };
 
@@ -268,7 +267,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       if constexpr (State::kApart) rest[d][e] = 0.0f;
     }
   }
-  float m = -INFINITY, l = 0.0f, v_ref = 0.0f, ref_log = 0.0f, poison = 0.0f;
+  float m = -INFINITY, l = 0.0f, v_ref = 0.0f, v_inv = 0.0f, poison = 0.0f;
   // The sums of the tiles so far take a change of the references with them
   // when the next tile's scores are there: then their products are done.
   bool moves = false;
@@ -370,11 +369,10 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
     auto score = [&](int r, int e) { return s[r][e / kAcc][e % kAcc]; };
     const int key0 = tile * kTile;
     // a lane's keys: kPer neighbours of either 32, which share their scales
-    float kscale[2], v_log[2], top[2], v_top[2], mul[2];
+    float kscale[2], top[2], v_top[2], mul[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       kscale[r] = of[r].k * col_scale;
-      v_log[r] = of[r].v_log;
       v_top[r] = of[r].v;
     }
     const bool whole = key0 >= all_from && key0 + kTile - 1 <= wave_first;
@@ -400,10 +398,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
           s[r][e / kAcc][e % kAcc] = sc;
           top[r] = fmaxf(top[r], sc);
         }
-        if (!some) {
-          v_top[r] = 0.0f;
-          v_log[r] = -INFINITY;
-        }
+        if (!some) v_top[r] = 0.0f;
         mul[r] = 1.0f;
       }
     }
@@ -422,19 +417,17 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       l *= keep;
       m = m2;
       v_ref = ref;
-      ref_log = ref > 0.0f ? __builtin_amdgcn_logf(ref) : 0.0f;
+      v_inv = ref > 0.0f ? 1.0f / ref : 0.0f;
     }
     const float shift = weight_bias(T::code) - (m == -INFINITY ? 0.0f : m);
-    // The value scale, as a part of the largest, goes into the exponent and out
-    // of the sum again.  One below 2^-60 takes no part in a product of fp32;
-    // one that is no number makes its columns so at the end.
-    float at[2], out_of[2];
+    // A value scale that is no number makes its columns so at the end.  (As a
+    // logarithm in the exponent a scale would cost a product less to a weight,
+    // but its own rounding, which grows with its distance from 1.)
+    float v_factor[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       poison += v_top[r] <= kLargest ? 0.0f : NAN;
-      const float part = __builtin_amdgcn_fmed3f(v_log[r] - ref_log, -60.0f, 0.0f);
-      at[r] = shift + part;
-      out_of[r] = __builtin_amdgcn_exp2f(-part);
+      v_factor[r] = v_top[r] <= kLargest ? v_top[r] * v_inv : 0.0f;
     }
     // The last tile's product runs beside this tile's weights.
     f16x8 w2[2][kPer / 8], w2_rest[2][kPer / 8];
@@ -448,9 +441,9 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       for (int u = 0; u < kCount; ++u) {
         const int j = ((i + 1) / kEvery - 1) * kCount + u, r = 2 * j / kPer;
         const int e = 2 * j % kPer;
-        const float p[2] = {__builtin_amdgcn_exp2f(fmaf(score(r, e), mul[r], at[r])),
-                            __builtin_amdgcn_exp2f(fmaf(score(r, e + 1), mul[r], at[r]))};
-        const Terms two = terms_of(p[0], p[1]);
+        const float p[2] = {__builtin_amdgcn_exp2f(fmaf(score(r, e), mul[r], shift)),
+                            __builtin_amdgcn_exp2f(fmaf(score(r, e + 1), mul[r], shift))};
+        const Terms two = terms_of(as_rounded(p[0] * v_factor[r]), as_rounded(p[1] * v_factor[r]));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           w2[r][(e + k) / 8][(e + k) % 8] = two.first[k];
@@ -462,7 +455,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
     });
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      l = fmaf(sum[r], out_of[r], l);
+      l += sum[r];
 #pragma unroll
       for (int k = 0; k < kPer / 8; ++k) {
         w[r][k] = w2[r][k];

@@ -60,3 +60,19 @@ def test_queries_of_unlike_channels_keep_their_bits(hip_lib, dtype, hd, new):
     rest = got[2].copy()
     rest[..., 5] = 0.0
     within(s, got, rest, 8, dtype)
+
+
+@pytest.mark.parametrize("power", [-100, -40, 40])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128, 256, 48])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_value_scales_times_a_power_of_two(hip_lib, dtype, hd, new, power):
+    """All value scales times 2^n give the outputs times 2^n, to the bit."""
+    s = Setup([200], [new], 2, hd, 32, seed=hd + new)
+    s.vs = np.where(np.isnan(s.vs), s.vs, np.float32(1.0) + np.abs(s.vs)).astype(np.float32)
+    q = s.rng.standard_normal((s.tokens, 4, hd))
+    plain = attend(s, q, 4, dtype)
+    s.vs *= np.float32(2.0) ** power
+    scaled = attend(s, q, 4, dtype)
+    np.testing.assert_array_equal(scaled[0], plain[0] * 2.0 ** power)
+    np.testing.assert_array_equal(scaled[1], plain[1])
