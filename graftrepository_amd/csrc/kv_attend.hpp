@@ -112,24 +112,48 @@ __device__ inline float as_rounded(float v) {
   return v;
 }
 
-// Two values as fp16 terms: both rounded in one instruction, and what that
+// Two values as N bf16 terms of eight bits, cut: what is left is exact, and of
+// three terms nothing is.
+template <int N>
+__device__ inline void bf16_terms(float a, float b, uint32_t (&t)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    t[n] = upper_halves(__float_as_uint(a), __float_as_uint(b));
+    a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+    b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+  }
+}
+
+// Two values as two fp16 terms: both rounded in one instruction, and what that
 // leaves of each (exact) with the conversion back in one.  Spelt out, since the
 // compiler rounds each of them a second time for the conversion back: 112
 // instructions more to a tile of the wide kernel's against 48.
-struct Terms {
-  f16x2 first;
+__device__ inline void fp16_terms(float a, float b, uint32_t (&t)[2]) {
+  f16x2 v;
+  v[0] = static_cast<_Float16>(a);
+  v[1] = static_cast<_Float16>(b);
+  t[0] = __builtin_bit_cast(uint32_t, v);
   float left[2];
-};
-__device__ inline Terms terms_of(float a, float b) {
-  Terms t;
-  t.first[0] = static_cast<_Float16>(a);
-  t.first[1] = static_cast<_Float16>(b);
-  const uint32_t w = __builtin_bit_cast(uint32_t, t.first);
   asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]"
-      : "=v"(t.left[0]) : "v"(w), "v"(a));
+      : "=v"(left[0]) : "v"(t[0]), "v"(a));
   asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-      : "=v"(t.left[1]) : "v"(w), "v"(b));
-  return t;
+      : "=v"(left[1]) : "v"(t[0]), "v"(b));
+  v[0] = static_cast<_Float16>(left[0]);
+  v[1] = static_cast<_Float16>(left[1]);
+  t[1] = __builtin_bit_cast(uint32_t, v);
+}
+
+// A weight's terms in the second product: whole for fp32 outputs, 22 bits for
+// 16-bit ones.
+template <class T>
+__host__ __device__ constexpr bool weight_bf16() { return T::code == kF32; }
+template <class T>
+__host__ __device__ constexpr int weight_terms() { return T::code == kF32 ? 3 : 2; }
+
+template <class T>
+__device__ inline void split_weights(float a, float b, uint32_t (&t)[weight_terms<T>()]) {
+  if constexpr (weight_bf16<T>()) bf16_terms(a, b, t);
+  else fp16_terms(a, b, t);
 }
 
 template <class T>
@@ -171,18 +195,11 @@ __device__ inline float split_query(const float (&x)[N][8], float top, float sca
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       if constexpr (query_bf16<T>()) {
-        float v[2];
+        uint32_t t[TERMS];
+        bf16_terms(__builtin_amdgcn_ldexpf(x[s][e], -unit),
+                   __builtin_amdgcn_ldexpf(x[s][e + 1], -unit), t);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) v[k] = __builtin_amdgcn_ldexpf(x[s][e + k], -unit);
-#pragma unroll
-        for (int n = 0; n < TERMS; ++n) {
-          // eight bits, cut; what is left is exact
-          q[n][s][e / 2] = upper_halves(__float_as_uint(v[0]), __float_as_uint(v[1]));
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            v[k] -= __uint_as_float(__float_as_uint(v[k]) & 0xffff0000u);
-          }
-        }
+        for (int n = 0; n < TERMS; ++n) q[n][s][e / 2] = t[n];
       } else {
         f16x2 v;
         v[0] = static_cast<_Float16>(x[s][e]);
@@ -203,7 +220,7 @@ __device__ inline float power_above(float v) {
 }
 
 // Log2 of what probabilities are scaled by on their way into fp16.
-__host__ __device__ constexpr float weight_bias(int dtype) { return dtype == kF32 ? 7.0f : 13.0f; }
+__host__ __device__ constexpr float weight_bias(int dtype) { return dtype == kF32 ? 0.0f : 13.0f; }
 
 // Four values of a finished row: o / l rounded once, and the row's log-sum-exp
 // by the thread of its first column.  m in log2 units, l and o biased.

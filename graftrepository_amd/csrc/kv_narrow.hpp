@@ -37,20 +37,17 @@
 // halves of a value column, one 128-byte line, are read together (tiles of 64
 // tokens fetched 1.4 times the bytes there).
 //
-// Probabilities enter the second product as fp16(2^13 p vs / v), with v a
-// power of two no less than any value scale the column has met and at most
-// twice the largest.  The running maximum follows only when a score passes it
-// by more than 2 (log2 units), so weights stay below 2^15; 2^-27 of the
-// largest probability is still a normal number, and what is lost below that
-// is 2^-38 of it.  (An allowance of 8 would rescale less often, but lose
-// 2^-32.)
-//
-// The probabilities are two fp16 terms, the second what the first leaves: one
-// term alone is off by up to 2^-12 of each value, which shows in every output
-// whose values cancel.  For 16-bit outputs both are summed in one place.  For
-// fp32 the first is scaled by 2^7, the second by 2^19 more and summed apart,
-// and the maximum follows at once, so that both stay below 2^15 and reach
-// 2^-51 of the largest; fp32 queries are three bf16 terms.
+// Probabilities enter the second product as p vs / v, with v a power of two no
+// less than any value scale the column has met and at most twice the largest.
+// For 16-bit outputs they are two fp16 terms of 2^13 times that, the second
+// what the first leaves: one term alone is off by up to 2^-12 of each value,
+// which shows in every output whose values cancel.  The running maximum follows
+// only when a score passes it by more than 2 (log2 units), so weights stay
+// below 2^15; 2^-27 of the largest probability is still a normal number, and
+// what is lost below that is 2^-38 of it.  (An allowance of 8 would rescale
+// less often, but lose 2^-32.)  For fp32 outputs they are three bf16 terms,
+// which hold all 24 bits and fp32's range; the lesser two are summed apart, so
+// that the sums that grow round no more often than fp32's own would.
 #pragma once
 
 #include "kv_attend.hpp"
@@ -74,9 +71,9 @@ __device__ __forceinline__ const AttendArgs& late_args() {
 template <class T, int D>
 struct NarrowState {
   static constexpr int kTerms = T::code == kF32 ? 3 : 1;  // of a query
-  static constexpr bool kApart = T::code == kF32;  // a probability's two are summed apart
-  static constexpr float kRestScale = kApart ? 524288.0f : 1.0f;
-  static constexpr float kRescale = kApart ? 0.0f : 2.0f;
+  static constexpr int kWeights = weight_terms<T>();      // of a probability
+  static constexpr bool kApart = T::code == kF32;  // the lesser ones are summed apart
+  static constexpr float kRescale = 2.0f;
   float col_scale;  // softmax scale, log2 e and the query's own power of two
   f32x4 o[D / 16];
   f32x4 rest[kApart ? D / 16 : 1];
@@ -424,7 +421,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
       float v_factor[H];
 #pragma unroll
       for (int h = 0; h < H; ++h) v_factor[h] = vscale[h] * st.v_inv;
-      f16x8 w[H][2], w_rest[H][2];
+      u32x4 w[State::kWeights][H][2];
       // probabilities and their weights; `some_hidden`: 0 times a scale that
       // is no number has to be 0
       auto weights = [&](auto some_hidden) {
@@ -443,12 +440,10 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
             }
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-              const Terms two = terms_of(v[e], v[e + 1]);
+              uint32_t t[State::kWeights];
+              split_weights<T>(v[e], v[e + 1], t);
 #pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                w[h][k][e + n] = two.first[n];
-                w_rest[h][k][e + n] = static_cast<_Float16>(two.left[n] * State::kRestScale);
-              }
+              for (int n = 0; n < State::kWeights; ++n) w[n][h][k][e / 2] = t[n];
             }
             st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
           }
@@ -464,14 +459,16 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
       for (int d = 0; d < kValueTiles; ++d) {
         u32x4 c[H][2];
 #pragma unroll
-        for (int h = 0; h < H; ++h) codes_as<false>(vr[d % kHeld][h], c[h]);
+        for (int h = 0; h < H; ++h) codes_as<weight_bf16<T>()>(vr[d % kHeld][h], c[h]);
 #pragma unroll
         for (int h = 0; h < H; ++h) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            st.o[d] = mfma<false>(c[h][k], __builtin_bit_cast(u32x4, w[h][k]), st.o[d]);
-            f32x4& o = State::kApart ? st.rest[d] : st.o[d];
-            o = mfma<false>(c[h][k], __builtin_bit_cast(u32x4, w_rest[h][k]), o);
+#pragma unroll
+            for (int n = 0; n < State::kWeights; ++n) {
+              f32x4& o = n && State::kApart ? st.rest[d] : st.o[d];
+              o = mfma<weight_bf16<T>()>(c[h][k], w[n][h][k], o);
+            }
           }
         }
         if (d + kHeld < kValueTiles) load_values(cur, d + kHeld);
@@ -492,7 +489,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
 #pragma unroll
           for (int d = 0; d < kValueTiles; ++d) {
             f32x4 o = st.o[d];
-            if constexpr (State::kApart) o += st.rest[d] * (1.0f / State::kRestScale);
+            if constexpr (State::kApart) o += st.rest[d];
             o *= st.v_ref;
             if (alone) finish4<T>(b, row, h, 16 * d + 4 * G, o, st.m, l);
             else *reinterpret_cast<f32x4*>(part + i * D + 16 * d + 4 * G) = o;
@@ -546,7 +543,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
 #pragma unroll
     for (int d = 0; d < kValueTiles; ++d) {
       f32x4 o = st.o[d];
-      if constexpr (State::kApart) o += st.rest[d] * (1.0f / State::kRestScale);
+      if constexpr (State::kApart) o += st.rest[d];
       *reinterpret_cast<f32x4*>(&s_o[wave][i][16 * d + 4 * G]) = o * mine;
     }
   }

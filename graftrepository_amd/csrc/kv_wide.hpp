@@ -30,7 +30,7 @@
 //     instruction, and the A operand's lane holds the same keys of a value
 //     column.
 // The softmax is the narrow kernel's: one pass, scores and statistics in fp32,
-// weights as two fp16 terms.
+// weights as two fp16 terms, or three bf16 ones.
 //
 // Items of one kv head follow each other at a distance of kv_heads blocks, so
 // with 8 kv heads an XCD's L2 serves one of them.
@@ -206,7 +206,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       const int at =
           W == 32 ? ((d / 32 * 2 + (grp >> 1)) * 2 + half) * kWave + d % 32 + 32 * (grp & 1)
                   : (d / 16 * 2 + (grp >> 1)) * kWave + d % 16 + 32 * (grp & 1) + 16 * half;
-      s_v[b][at] = codes_as<false>(v_reg[q][2 * half], v_reg[q][2 * half + 1]);
+      s_v[b][at] = codes_as<weight_bf16<T>()>(v_reg[q][2 * half], v_reg[q][2 * half + 1]);
     }
   };
   auto store_scales = [&](int b) {
@@ -295,21 +295,20 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
     load_keys(min(tile_lo + 1, tile_last));
     load_id(min(tile_lo + 2, tile_last));
   }
-  f16x8 w[2][kPer / 8] = {}, w_rest[2][kPer / 8] = {};
+  // kept as halves: as words they spill more (fp16, head_dim 128: 35 registers
+  // against 14, prompts in 307 us against 243)
+  f16x8 w[State::kWeights][2][kPer / 8] = {};
   // Weights of a tile times its values.
   constexpr int kValueReads = 2 * kPer / 8 * kTilesD;
-  constexpr int kLag = State::kApart ? 0 : 2;
   auto multiply = [&](int b, auto beside) {
     in_step<kValueReads>([&](int i) { return s_v[b][(i % kTilesD * 2 * (kPer / 8) + i / kTilesD) * kWave + lane]; },
         [&](int i, const u32x4(&f)[kValueReads]) {
           const int d = i % kTilesD, rk = i / kTilesD;
-          o[d] = mfma<false>(f[i], __builtin_bit_cast(u32x4, w[rk / (kPer / 8)][rk % (kPer / 8)]), o[d]);
-          // a step of its own sums later, which need not wait for the first's
-          for (int n = max(0, i - kLag); n <= (i == kValueReads - 1 ? i : i - kLag); ++n) {
-            Acc& to = State::kApart ? rest[n % kTilesD] : o[n % kTilesD];
-            to = mfma<false>(f[n],
-                            __builtin_bit_cast(u32x4, w_rest[n / kTilesD / (kPer / 8)][n / kTilesD % (kPer / 8)]),
-                            to);
+#pragma unroll
+          for (int n = 0; n < State::kWeights; ++n) {
+            Acc& to = n && State::kApart ? rest[d] : o[d];
+            to = mfma<weight_bf16<T>()>(
+                f[i], __builtin_bit_cast(u32x4, w[n][rk / (kPer / 8)][rk % (kPer / 8)]), to);
           }
           beside(i);
         });
@@ -430,7 +429,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       v_factor[r] = v_top[r] <= kLargest ? v_top[r] * v_inv : 0.0f;
     }
     // The last tile's product runs beside this tile's weights.
-    f16x8 w2[2][kPer / 8], w2_rest[2][kPer / 8];
+    u32x4 w2[State::kWeights][2][kPer / 8];
     float sum[2] = {0.0f, 0.0f};
     multiply(b ^ 1, [&](int i) {
       // two weights at a time, spread over the reads
@@ -443,14 +442,12 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
         const int e = 2 * j % kPer;
         const float p[2] = {__builtin_amdgcn_exp2f(fmaf(score(r, e), mul[r], shift)),
                             __builtin_amdgcn_exp2f(fmaf(score(r, e + 1), mul[r], shift))};
-        const Terms two = terms_of(as_rounded(p[0] * v_factor[r]), as_rounded(p[1] * v_factor[r]));
+        uint32_t t[State::kWeights];
+        split_weights<T>(as_rounded(p[0] * v_factor[r]), as_rounded(p[1] * v_factor[r]), t);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          w2[r][(e + k) / 8][(e + k) % 8] = two.first[k];
-          w2_rest[r][(e + k) / 8][(e + k) % 8] =
-              static_cast<_Float16>(two.left[k] * State::kRestScale);
-          sum[r] += p[k];
-        }
+        for (int n = 0; n < State::kWeights; ++n) w2[n][r][e / 8][e % 8 / 2] = t[n];
+        sum[r] += p[0];
+        sum[r] += p[1];
       }
     });
 #pragma unroll
@@ -458,8 +455,8 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       l += sum[r];
 #pragma unroll
       for (int k = 0; k < kPer / 8; ++k) {
-        w[r][k] = w2[r][k];
-        w_rest[r][k] = w2_rest[r][k];
+#pragma unroll
+        for (int n = 0; n < State::kWeights; ++n) w[n][r][k] = __builtin_bit_cast(f16x8, w2[n][r][k]);
       }
     }
   }
@@ -481,7 +478,7 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] = o[d][4 * k + e];
-        if constexpr (State::kApart) v[e] += rest[d][4 * k + e] * (1.0f / State::kRestScale);
+        if constexpr (State::kApart) v[e] += rest[d][4 * k + e];
         v[e] = fmaf(v[e], v_ref, poison);
       }
       const int at = W * d + 4 * kLanes * k + 4 * h;

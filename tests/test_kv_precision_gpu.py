@@ -62,6 +62,28 @@ def test_queries_of_unlike_channels_keep_their_bits(hip_lib, dtype, hd, new):
     within(s, got, rest, 8, dtype)
 
 
+@pytest.mark.parametrize("new", [1, 64])
+@pytest.mark.parametrize("hd", [64, 128, 256, 48])
+def test_fp32_weights_are_whole(hip_lib, hd, new):
+    """Rows that see one token: the output is its code times its scale, of 31
+    bits.  A sum of exact products is rounded once or, if the matrix core cuts
+    instead, off by a unit at most; the steps after it are by powers of two."""
+    ctx = [16 * 30 - 1] * 40
+    s = Setup(ctx, [new if r % 8 == 0 else 1 for r in range(40)], 2, hd, 16, seed=hd + new)
+    s.vs *= np.exp2(s.rng.integers(-3, 4, s.vs.shape)).astype(np.float32)
+    q = s.rng.standard_normal((s.tokens, 4, hd))
+    got, _, _ = attend(s, q, 4, "f32", window=1)
+    row = 0
+    for r, n in enumerate(s.new):
+        for i in range(n):
+            p = s.ctx[r] + i
+            b = s.table[r, p // 16]
+            want = s.vc[b, :, :, p % 16].astype(np.float64) * s.vs[b][:, None].astype(np.float64)
+            want = np.repeat(want, 2, 0)
+            assert (np.abs(got[row] - want) <= np.abs(want) * 2.0 ** -23).all()
+            row += 1
+
+
 @pytest.mark.parametrize("power", [-100, -40, 40])
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("hd", [64, 128, 256, 48])
