@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
   __shared__ float s_q[256];
   __shared__ float s_p[4][kTile];
   __shared__ float s_o[4][256];
-  __shared__ float s_m[4], s_l[4];
+  __shared__ float s_m[4], s_l[4], s_ref[4];
   if (row >= a.cu_new[a.requests]) return;
   int lo = 0, len = a.requests;  // the last request whose first row is not past this one
   while (len > 1) {
@@ -44,6 +44,7 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
   __syncthreads();
 
   float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float ref = 0.0f;  // o is in units of this power of two, above all value scales
   bool odd = false;  // a score that is not a number
   for (int t0 = first / kTile * kTile + wave * kTile; t0 <= pos; t0 += 4 * kTile) {
     const int key = t0 + lane;
@@ -69,22 +70,28 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
       vs = a.v_scales[cell];
     }
     odd |= s != s;
-    float top = s;
+    float top = s, v_top = vs <= 3.0e38f ? vs : 0.0f;
 #pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+      top = fmaxf(top, __shfl_xor(top, d));
+      v_top = fmaxf(v_top, __shfl_xor(v_top, d));
+    }
     const float m2 = fmaxf(m, top);
     if (m2 == -INFINITY) continue;  // no key of this tile is seen
     const float keep = __builtin_amdgcn_exp2f((m - m2) * kLog2e);
+    const float ref2 = v_top > ref ? power_above(v_top) : ref;
+    const float keep_o = keep * unit_change(ref, ref2);
+    ref = ref2;
     const float pr = block >= 0 ? __builtin_amdgcn_exp2f((s - m2) * kLog2e) : 0.0f;
     m = m2;
     float sum = pr;
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
     l = l * keep + sum;
-    s_p[wave][lane] = block >= 0 ? pr * vs : 0.0f;
+    s_p[wave][lane] = block >= 0 ? pr * (vs * (ref > 0.0f ? 1.0f / ref : 0.0f)) : 0.0f;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] *= keep;
+    for (int c = 0; c < 4; ++c) o[c] *= keep_o;
     for (int b0 = 0; b0 < kTile; b0 += 16) {
       // the 16 tokens lie in one block; the window may hide the first
       const uint64_t seen = (__ballot(block >= 0) >> b0) & 0xffffull;
@@ -111,20 +118,23 @@ __global__ __launch_bounds__(256) void attend_any_kernel(AttendArgs a) {
   if (lane == 0) {
     s_m[wave] = m;
     s_l[wave] = l;
+    s_ref[wave] = ref;
   }
   __syncthreads();
   const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  ref = fmaxf(fmaxf(s_ref[0], s_ref[1]), fmaxf(s_ref[2], s_ref[3]));
   float total = 0.0f, f[4];
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     f[w] = s_m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((s_m[w] - top) * kLog2e);
     total += s_l[w] != s_l[w] ? NAN : f[w] * s_l[w];
+    f[w] *= unit_change(s_ref[w], ref);
   }
   typename T::store* out = static_cast<typename T::store*>(a.out) + row * a.out_token_stride +
                            h * a.out_head_stride;
   for (int d = threadIdx.x; d < hd; d += 256) {
     const float v = f[0] * s_o[0][d] + f[1] * s_o[1][d] + f[2] * s_o[2][d] + f[3] * s_o[3][d];
-    out[d] = T::put(total == 0.0f ? 0.0f : v / total);
+    out[d] = T::put(total == 0.0f ? 0.0f : v / total * ref);
   }
   if (a.lse && threadIdx.x == 0) {
     a.lse[static_cast<size_t>(row) * a.heads + h] =
@@ -160,8 +170,8 @@ static int shape_of(const grm_kv_cache_desc* c, const Layout& l, Shape* out) {
     s.at_run_units[k] = l.at_run_units[k];
   }
   if (s.cores && l.cap_units > 0) {
-    s.bytes = static_cast<uint64_t>(c->kv_heads) * l.runs[hd == 256 ? 0 : 1] * 2 * kNarrowCols *
-              (hd + 2) * 4;
+    s.bytes = static_cast<uint64_t>(c->kv_heads) * l.runs[hd == 256 ? 0 : 1] * 2 *
+              narrow_part_floats(hd) * 4;
   }
   if (s.cores) {
     s.wide_bytes = static_cast<uint64_t>(c->kv_heads) * l.cap_parts * wide_part_floats(hd) * 4;

@@ -39,6 +39,13 @@ __host__ __device__ constexpr int narrow_blocks_per_cu(int dtype, int head_dim) 
   return head_dim == 256 || (dtype == kF32 && head_dim == 128) ? 1 : 2;
 }
 
+// Floats of one partial result of the narrow kernel: its columns' sums of
+// weights times codes, then their maxima, their sums of probabilities and the
+// powers of two that the sums are in.
+__host__ __device__ constexpr int narrow_part_floats(int head_dim) {
+  return kNarrowCols * (head_dim + 3);
+}
+
 // A run has at most two partial results: of its first unit and of its last.
 __device__ inline size_t narrow_part(int g, int runs, int run, int which) {
   return (static_cast<size_t>(g) * runs + run) * 2 + which;
@@ -222,11 +229,17 @@ __device__ inline float power_above(float v) {
 // Log2 of what probabilities are scaled by on their way into fp16.
 __host__ __device__ constexpr float weight_bias(int dtype) { return dtype == kF32 ? 0.0f : 13.0f; }
 
-// Four values of a finished row: o / l rounded once, and the row's log-sum-exp
-// by the thread of its first column.  m in log2 units, l and o biased.
+// What takes sums in units of `from` to units of `to`, a power of two no less
+// (0: nothing was summed).
+__device__ inline float unit_change(float from, float to) { return to > 0.0f ? from / to : 1.0f; }
+
+// Four values of a finished row: o / l, which is a mean, times the power of two
+// it is in, so that nothing passes fp32's range before (a sum of large values
+// would), rounded once; and the row's log-sum-exp by the thread of its first
+// column.  m in log2 units, l and o biased.
 template <class T>
 __device__ inline void finish4(const AttendArgs& a, int row, int h, int d, f32x4 o, float m,
-                               float l) {
+                               float l, float ref) {
   const bool empty = m == -INFINITY && l == 0.0f;
   const float inv = 1.0f / l;
   typename T::store* out = static_cast<typename T::store*>(a.out) +
@@ -235,14 +248,14 @@ __device__ inline void finish4(const AttendArgs& a, int row, int h, int d, f32x4
   if constexpr (T::code == kF32) {
     f32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = empty ? 0.0f : o[e] * inv;
+    for (int e = 0; e < 4; ++e) v[e] = empty ? 0.0f : o[e] * inv * ref;
     *reinterpret_cast<f32x4*>(out) = v;
   } else {
     u32x2 v;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv);
-      const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv);
+      const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv * ref);
+      const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv * ref);
       v[e] = lo | (hi << 16);
     }
     *reinterpret_cast<u32x2*>(out) = v;

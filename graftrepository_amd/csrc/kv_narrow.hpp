@@ -483,20 +483,20 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
         l += __shfl_xor(l, 32);
         const bool alone = now.first >= begin && now.end <= end;
         float* part = b.parts + narrow_part(g, runs, run, now.first <= begin ? 0 : 1) *
-                                    (kNarrowCols * (D + 2));
+                                    narrow_part_floats(D);
         if (i < cols) {
           const int row = now.row + col_token, h = g * b.group + i - col_token * b.group;
 #pragma unroll
           for (int d = 0; d < kValueTiles; ++d) {
             f32x4 o = st.o[d];
             if constexpr (State::kApart) o += st.rest[d];
-            o *= st.v_ref;
-            if (alone) finish4<T>(b, row, h, 16 * d + 4 * G, o, st.m, l);
+            if (alone) finish4<T>(b, row, h, 16 * d + 4 * G, o, st.m, l, st.v_ref);
             else *reinterpret_cast<f32x4*>(part + i * D + 16 * d + 4 * G) = o;
           }
           if (!alone && G == 0) {
             part[kNarrowCols * D + i] = st.m;
             part[kNarrowCols * (D + 1) + i] = l;
+            part[kNarrowCols * (D + 2) + i] = st.v_ref;
           }
         }
         if constexpr (kMore) {
@@ -517,7 +517,7 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
 
   // The block's first tile decides for all four waves alike; a wave without
   // a run of its own adds nothing.
-  __shared__ float s_ml[2][4][16];
+  __shared__ float s_ml[3][4][16];
   auto& s_o = s_lds.o;
   __shared__ int s_unit[2];  // wave 0 has the first run
   if (threadIdx.x == 0) {
@@ -533,12 +533,17 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   if (G == 0) {
     s_ml[0][wave][i] = st.m;
     s_ml[1][wave][i] = st.l;
+    s_ml[2][wave][i] = st.v_ref;
   }
   __syncthreads();
-  float top = s_ml[0][0][i];
+  float top = s_ml[0][0][i], ref = s_ml[2][0][i];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, s_ml[0][w][i]);
-  const float mine = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - top) * st.v_ref;
+  for (int w = 1; w < 4; ++w) {
+    top = fmaxf(top, s_ml[0][w][i]);
+    ref = fmaxf(ref, s_ml[2][w][i]);
+  }
+  const float mine = st.m == -INFINITY
+                         ? 0.0f : __builtin_amdgcn_exp2f(st.m - top) * unit_change(st.v_ref, ref);
   if (i < cols) {
 #pragma unroll
     for (int d = 0; d < kValueTiles; ++d) {
@@ -549,27 +554,31 @@ __global__ __launch_bounds__(256, narrow_blocks_per_cu(T::code, D)) void attend_
   }
   __syncthreads();
   const bool alone = u.first == block_begin && u.end == block_end;
-  float* part = a.parts + narrow_part(g, runs, 4 * blockIdx.y, 0) * (kNarrowCols * (D + 2));
+  float* part = a.parts + narrow_part(g, runs, 4 * blockIdx.y, 0) * narrow_part_floats(D);
   for (int e = threadIdx.x; e < cols * (D / 4); e += 256) {
     const int c = e / (D / 4), d = e % (D / 4) * 4;
     f32x4 o = *reinterpret_cast<const f32x4*>(&s_o[0][c][d]);
 #pragma unroll
     for (int w = 1; w < 4; ++w) o += *reinterpret_cast<const f32x4*>(&s_o[w][c][d]);
-    float m = s_ml[0][0][c], l = 0.0f;
+    float m = s_ml[0][0][c], l = 0.0f, all_ref = s_ml[2][0][c];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, s_ml[0][w][c]);
+    for (int w = 1; w < 4; ++w) {
+      m = fmaxf(m, s_ml[0][w][c]);
+      all_ref = fmaxf(all_ref, s_ml[2][w][c]);
+    }
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       l += s_ml[0][w][c] == -INFINITY ? s_ml[1][w][c]
                                       : s_ml[1][w][c] * __builtin_amdgcn_exp2f(s_ml[0][w][c] - m);
     }
     if (alone) {
-      finish4<T>(a, u.row + c / a.group, g * a.group + c % a.group, d, o, m, l);
+      finish4<T>(a, u.row + c / a.group, g * a.group + c % a.group, d, o, m, l, all_ref);
     } else {
       *reinterpret_cast<f32x4*>(part + c * D + d) = o;
       if (d == 0) {
         part[kNarrowCols * D + c] = m;
         part[kNarrowCols * (D + 1) + c] = l;
+        part[kNarrowCols * (D + 2) + c] = all_ref;
       }
     }
   }
@@ -615,19 +624,30 @@ __device__ inline void join_narrow(const AttendArgs& a, int runs, bool by_unit, 
   auto part_of = [&](int p) -> const float* {
     const int r = p < lead ? r0 + p : p < lead + whole ? b0 + 4 * (p - lead) : b1 + p - lead - whole;
     return a.parts +
-           narrow_part(g, runs, r, from > deal.begin(r) ? 1 : 0) * (kNarrowCols * (D + 2));
+           narrow_part(g, runs, r, from > deal.begin(r) ? 1 : 0) * narrow_part_floats(D);
   };
-  __shared__ float s_top[4];
+  __shared__ float s_top[2][4];
   __shared__ float s_l[kGroups];
   __shared__ f32x4 s_o[kGroups][kVecs];
   for (int c = first_col; c < u.tokens * a.group; c += step) {
-    float m = -INFINITY;
-    for (int r = threadIdx.x; r < parts; r += 256) m = fmaxf(m, part_of(r)[kNarrowCols * D + c]);
+    float m = -INFINITY, ref = 0.0f;
+    for (int r = threadIdx.x; r < parts; r += 256) {
+      const float* p = part_of(r);
+      m = fmaxf(m, p[kNarrowCols * D + c]);
+      ref = fmaxf(ref, p[kNarrowCols * (D + 2) + c]);
+    }
 #pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if (__lane_id() == 0) s_top[threadIdx.x / kWave] = m;
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+      m = fmaxf(m, __shfl_xor(m, d));
+      ref = fmaxf(ref, __shfl_xor(ref, d));
+    }
+    if (__lane_id() == 0) {
+      s_top[0][threadIdx.x / kWave] = m;
+      s_top[1][threadIdx.x / kWave] = ref;
+    }
     __syncthreads();
-    m = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+    m = fmaxf(fmaxf(s_top[0][0], s_top[0][1]), fmaxf(s_top[0][2], s_top[0][3]));
+    ref = fmaxf(fmaxf(s_top[1][0], s_top[1][1]), fmaxf(s_top[1][2], s_top[1][3]));
     const int group = threadIdx.x / kVecs, d = threadIdx.x % kVecs;
     f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
@@ -637,7 +657,7 @@ __device__ inline void join_narrow(const AttendArgs& a, int runs, bool by_unit, 
       const float pm = p[kNarrowCols * D + c], pl = p[kNarrowCols * (D + 1) + c];
       const f32x4 po = *reinterpret_cast<const f32x4*>(p + c * D + 4 * d);
       const float f = pm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pm - m);
-      o += po * f;
+      o += po * (f * unit_change(p[kNarrowCols * (D + 2) + c], ref));
       l += pl * f;
     }
     s_o[group][d] = o;
@@ -649,7 +669,7 @@ __device__ inline void join_narrow(const AttendArgs& a, int runs, bool by_unit, 
         o += s_o[k][d];
         l += s_l[k];
       }
-      finish4<T>(a, u.row + c / a.group, g * a.group + c % a.group, 4 * d, o, m, l);
+      finish4<T>(a, u.row + c / a.group, g * a.group + c % a.group, 4 * d, o, m, l, ref);
     }
     __syncthreads();  // what LDS holds has been read
   }

@@ -57,9 +57,9 @@ __host__ __device__ constexpr int wide_threads(int dtype, int head_dim) {
   return kWideCols / wide_wave_cols(dtype, head_dim) * kWave;
 }
 
-// Floats of one partial result: 128 columns, and their maxima and sums.
+// Floats of one partial result: 128 columns, as in the narrow kernel's.
 __host__ __device__ constexpr int wide_part_floats(int head_dim) {
-  return kWideCols * (head_dim + 2);
+  return kWideCols * (head_dim + 3);
 }
 
 // Scales of 16 tokens, 0 where they have no block or none of the item's
@@ -479,19 +479,21 @@ __device__ inline void wide_item(const AttendArgs& a, ConstItem item, int tile_h
       for (int e = 0; e < 4; ++e) {
         v[e] = o[d][4 * k + e];
         if constexpr (State::kApart) v[e] += rest[d][4 * k + e];
-        v[e] = fmaf(v[e], v_ref, poison);
+        v[e] += poison;
       }
       const int at = W * d + 4 * kLanes * k + 4 * h;
-      if (part < 0) finish4<T>(a, item->row + row, q_head, at, v, m, l);
+      if (part < 0) finish4<T>(a, item->row + row, q_head, at, v, m, l, v_ref);
       else *reinterpret_cast<f32x4*>(to + col * D + at) = v;
     }
   }
   if (part >= 0 && h == 0) {
     to[kWideCols * D + col] = m;
     to[kWideCols * (D + 1) + col] = l;
+    to[kWideCols * (D + 2) + col] = v_ref;
     if (tile_hi != item->tile_hi) {  // the next item's part has nothing left
       to[wide_part_floats(D) + kWideCols * D + col] = -INFINITY;
       to[wide_part_floats(D) + kWideCols * (D + 1) + col] = 0.0f;
+      to[wide_part_floats(D) + kWideCols * (D + 2) + col] = 0.0f;
     }
   }
 }
@@ -538,17 +540,18 @@ __device__ inline void join_wide(const AttendArgs& a, const float* parts, int un
   const int d = threadIdx.x % kVecs * 4;
   if (c >= j.tokens * a.group) return;
   const float* from = parts + (static_cast<size_t>(g) * a.cap_parts + j.part) * wide_part_floats(D);
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY, l = 0.0f, ref = 0.0f;
   f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kBatch = 4;  // parts whose loads go out together
   for (int p0 = 0; p0 < j.parts; p0 += kBatch) {
-    float pm[kBatch], pl[kBatch];
+    float pm[kBatch], pl[kBatch], pr[kBatch];
     f32x4 po[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const float* q = from + static_cast<size_t>(min(p0 + u, j.parts - 1)) * wide_part_floats(D);
       pm[u] = q[kWideCols * D + c];
       pl[u] = p0 + u < j.parts ? q[kWideCols * (D + 1) + c] : 0.0f;
+      pr[u] = q[kWideCols * (D + 2) + c];
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
@@ -559,21 +562,25 @@ __device__ inline void join_wide(const AttendArgs& a, const float* parts, int un
         po[u] = *reinterpret_cast<const f32x4*>(q + c * D + d);
       }
     }
-    float m2 = m;
+    float m2 = m, ref2 = ref;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) m2 = p0 + u < j.parts ? fmaxf(m2, pm[u]) : m2;
+    for (int u = 0; u < kBatch; ++u) {
+      m2 = p0 + u < j.parts ? fmaxf(m2, pm[u]) : m2;
+      ref2 = p0 + u < j.parts ? fmaxf(ref2, pr[u]) : ref2;
+    }
     const float keep = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m2);
-    o *= keep;
+    o *= keep * unit_change(ref, ref2);
     l *= keep;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const float f = pm[u] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pm[u] - m2);
-      o += po[u] * f;
+      o += po[u] * (f * unit_change(pr[u], ref2));
       l += pl[u] * f;
     }
     m = m2;
+    ref = ref2;
   }
-  finish4<T>(a, j.row + c / a.group, g * a.group + c % a.group, d, o, m, l);
+  finish4<T>(a, j.row + c / a.group, g * a.group + c % a.group, d, o, m, l, ref);
 }
 
 // What joins the parts of both kernels, in one launch (one for each took 4.5 us

@@ -98,3 +98,17 @@ def test_value_scales_times_a_power_of_two(hip_lib, dtype, hd, new, power):
     scaled = attend(s, q, 4, dtype)
     np.testing.assert_array_equal(scaled[0], plain[0] * 2.0 ** power)
     np.testing.assert_array_equal(scaled[1], plain[1])
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128, 256, 48])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_large_values_do_not_overflow_before_they_are_means(hip_lib, dtype, hd, new):
+    """Sums of many values near fp32's largest pass it, their mean does not."""
+    s = Setup([3000, 700], [new, 1], 2, hd, 64, seed=hd + new)
+    s.vs *= np.float32(2.0) ** 119                 # values up to 2^127
+    s.vs = np.minimum(s.vs, np.float32(2.0) ** 119)
+    q = s.rng.standard_normal((s.tokens, 4, hd)) * 0.1
+    got = attend(s, q, 4, dtype)
+    assert np.isfinite(got[0]).all()
+    within(s, got, got[2], 4, dtype)
