@@ -230,7 +230,7 @@ class KvBatch:
             d.free_head_out = self.free_head_out.data_ptr()
         self._ref = ctypes.byref(d)
         self._scratch: dict[int, int] = {}
-        self._held: dict[int, object] = {}
+        self._held: dict[int, list] = {}
         self._planned = False
 
     def plan(self, stream=None) -> "KvBatch":
@@ -243,12 +243,13 @@ class KvBatch:
         return self
 
     def _scratch_on(self, like, need: int, on: int, stream) -> int:
-        """Scratch of a call, one per stream: calls on one stream follow each
-        other and may share it."""
-        held = self._held.get(on)
-        if held is None or held.nbytes < need:
-            held = self._held[on] = _empty(like, (need,), "u8", stream)
-        return held.data_ptr()
+        """Scratch of a call, the largest of its stream: calls on one stream
+        follow each other and may share it.  What a call was given stays for
+        the batch's life, since a captured graph goes on writing to it."""
+        held = self._held.setdefault(on, [])
+        if not held or held[-1].nbytes < need:
+            held.append(_empty(like, (need,), "u8", stream))
+        return held[-1].data_ptr()
 
     def _need_plan(self):
         if not self._planned:

@@ -1,0 +1,75 @@
+"""What the key/value cache's Python side keeps and checks on the host, with a
+library and arrays that only write down what they are asked (CPU only)."""
+
+import ctypes
+import gc
+import weakref
+
+import numpy as np
+import pytest
+
+import graftrepository_amd as g
+from graftrepository_amd import kv_cache as kc
+from tests.test_kv_cache import fake
+
+
+class Lib:
+    """The library's key/value entries: sizes by head_dim, calls written down."""
+
+    def __init__(self):
+        self.calls = []
+
+    def grm_hip_kv_work_bytes(self, batch, out):
+        out._obj.value = 640
+        return 0
+
+    def grm_hip_kv_attend_bytes(self, cache, batch, out):
+        out._obj.value = 1000 * cache._obj.head_dim
+        return 0
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    lib, places = Lib(), iter(range(1, 1 << 30))
+    monkeypatch.setattr(kc._lib, "load", lambda: lib)
+
+    def empty(like, shape, dtype, stream=None):
+        a = fake(shape, kc._NUMPY[dtype])
+        a.ptr = next(places) << 12
+        lib.made.append(weakref.ref(a))
+        return a
+    lib.made = []
+    monkeypatch.setattr(kc, "_empty", empty)
+    return lib
+
+
+def cache_of(hd, kv=2):
+    return g.KvCache(fake((4, kv, 16, hd), np.int8), fake((4, kv, hd, 16), np.int8),
+                     fake((4, kv), np.float32), fake((4, kv), np.float32))
+
+
+def batch_of(tokens=3, **kw):
+    kw = {**dict(tokens=tokens, max_new=1, heads=4, kv_heads=2), **kw}
+    return g.KvBatch(fake((3,), np.int32), fake((3,), np.int32), fake((3, 4), np.int32), 16, **kw)
+
+
+def test_scratch_that_was_handed_out_stays_as_long_as_its_batch(lib):
+    """A captured graph holds the address of the scratch that its call was
+    given: a later call that needs more must not free it."""
+    b = batch_of().plan()
+    given = []
+    for hd in (64, 256, 128, 64):
+        cache_of(hd).attend(b, fake((3, 4, hd), np.float32))
+        args = lib.calls[-1][1]
+        given.append((args[11], args[12]))
+    gc.collect()
+    there = {r().ptr: r().nbytes for r in lib.made if r() is not None}
+    for ptr, need in given:
+        assert there.get(ptr, 0) >= need
+    assert len({p for p, _ in given[1:]}) == 1     # and what is large enough serves again
