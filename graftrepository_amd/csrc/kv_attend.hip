@@ -252,8 +252,7 @@ using namespace grm::kv;
 extern "C" int grm_hip_kv_attend_bytes(const grm_kv_cache_desc* cache,
                                        const grm_kv_batch_desc* batch, uint64_t* out_bytes) {
   if (!out_bytes) return grm::fail(-1, "null output pointer");
-  GRM_CHECK_RC(check_cache(cache));
-  GRM_CHECK_RC(check_batch(batch, false));
+  GRM_CHECK_RC(check_pair(cache, batch, false));
   Layout l;
   GRM_CHECK_RC(layout_of(batch, &l));
   Shape s;
@@ -268,7 +267,7 @@ extern "C" int grm_hip_kv_attend(const grm_kv_cache_desc* c, const grm_kv_batch_
                                  int64_t q_head_stride, void* out, int64_t out_token_stride,
                                  int64_t out_head_stride, float* lse, float softmax_scale,
                                  void* scratch, uint64_t scratch_bytes, void* stream) {
-  GRM_CHECK_RC(check_pair(c, b));
+  GRM_CHECK_RC(check_pair(c, b, true));
   if (dtype != grm::kF32 && dtype != grm::kBF16 && dtype != grm::kF16) {
     return grm::fail(-1, "queries are F32, BF16 or F16");
   }

@@ -81,9 +81,9 @@ int check_cache(const grm_kv_cache_desc* c) {
   return 0;
 }
 
-int check_pair(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b) {
+int check_pair(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b, bool with_arrays) {
   GRM_CHECK_RC(check_cache(c));
-  GRM_CHECK_RC(check_batch(b, true));
+  GRM_CHECK_RC(check_batch(b, with_arrays));
   if (c->block_tokens != b->block_tokens || c->kv_heads != b->kv_heads) {
     return fail(-1, "cache and batch differ in block_tokens or kv_heads");
   }
@@ -1204,7 +1204,7 @@ extern "C" int grm_hip_kv_append(const grm_kv_cache_desc* c, const grm_kv_batch_
                                  const void* k, const void* v, int dtype, int64_t k_token_stride,
                                  int64_t k_head_stride, int64_t v_token_stride,
                                  int64_t v_head_stride, void* stream) {
-  GRM_CHECK_RC(check_pair(c, b));
+  GRM_CHECK_RC(check_pair(c, b, true));
   if (dtype != grm::kF32 && dtype != grm::kBF16 && dtype != grm::kF16) {
     return grm::fail(-1, "keys and values are F32, BF16 or F16");
   }

@@ -111,7 +111,7 @@ int device_cus(int* out);
 int layout_of(const grm_kv_batch_desc* b, Layout* out);
 int check_batch(const grm_kv_batch_desc* b, bool with_arrays);
 int check_cache(const grm_kv_cache_desc* c);
-int check_pair(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b);
+int check_pair(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b, bool with_arrays);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -73,3 +73,31 @@ def test_scratch_that_was_handed_out_stays_as_long_as_its_batch(lib):
     for ptr, need in given:
         assert there.get(ptr, 0) >= need
     assert len({p for p, _ in given[1:]}) == 1     # and what is large enough serves again
+
+
+def test_a_refused_attend_leaves_no_size_behind(lib):
+    """The scratch's size is kept by head_dim: one asked with a cache that does
+    not fit the batch must not be."""
+    b, sizes = batch_of().plan(), []
+
+    def attend_bytes(cache, batch, out):
+        if cache._obj.kv_heads != batch._obj.kv_heads:
+            return -1
+        out._obj.value = 4096
+        sizes.append(1)
+        return 0
+    lib.grm_hip_kv_attend_bytes = attend_bytes
+    with pytest.raises(RuntimeError):
+        cache_of(64, kv=1).attend(b, fake((3, 4, 64), np.float32))
+    cache_of(64).attend(b, fake((3, 4, 64), np.float32))
+    assert sizes == [1] and lib.calls[-1][1][12] == 4096
+
+
+@pytest.mark.parametrize("change", [dict(kv_heads=4), dict(block_tokens=32)])
+def test_scratch_of_a_cache_that_does_not_fit_is_refused(change):
+    real = g.load()
+    from tests.test_kv_cache import batch_desc, cache_desc
+    out = ctypes.c_uint64(7)
+    assert real.grm_hip_kv_attend_bytes(ctypes.byref(cache_desc(**change)),
+                                        ctypes.byref(batch_desc()), ctypes.byref(out)) == -1
+    assert b"differ" in real.grm_hip_last_error() and out.value == 7
