@@ -149,10 +149,14 @@ def _empty(like, shape, dtype: str, stream=None):
     t = sys.modules["torch"]
     if stream is None:
         return t.empty(shape, dtype=_torch_names()[dtype], device=like.device)
-    on = _stream(like, stream)
-    s = t.cuda.ExternalStream(on, like.device) if on else t.cuda.default_stream(like.device)
-    with t.cuda.stream(s):
+    with t.cuda.stream(_torch_stream(like, _stream(like, stream))):
         return t.empty(shape, dtype=_torch_names()[dtype], device=like.device)
+
+
+def _torch_stream(like, on: int):
+    """The stream of this handle, on the tensor's device."""
+    t = sys.modules["torch"]
+    return t.cuda.ExternalStream(on, like.device) if on else t.cuda.default_stream(like.device)
 
 
 _raw_stream = None  # torch's current stream of a device as a handle
@@ -218,7 +222,7 @@ class KvBatch:
         d.cu_new, d.slot_map = self.cu_new.data_ptr(), self.slot_map.data_ptr()
         d.positions, d.work = self.positions.data_ptr(), self._work.data_ptr()
         d.work_bytes = need.value
-        self.free_list = self.free_head = self.free_head_out = None
+        self.free_list = self.free_head = self.free_head_out = self._made_head = None
         if free_list is not None:
             if free_head is None:
                 raise ValueError("a free list needs free_head")
@@ -226,17 +230,18 @@ class KvBatch:
             d.free_count = int(free_list.shape[0])
             d.free_head = _dense(free_head, "free_head", "i32", (1,))
             self.free_list, self.free_head = free_list, free_head
-            self.free_head_out = _empty(ctx_lens, (1,), "i32")
+            self.free_head_out = self._made_head = _empty(ctx_lens, (1,), "i32")
             d.free_head_out = self.free_head_out.data_ptr()
         self._ref = ctypes.byref(d)
         self._scratch: dict[int, int] = {}
         self._held: dict[int, list] = {}
+        self._streams = {_stream(ctx_lens, None)}
         self._planned = False
 
     def plan(self, stream=None) -> "KvBatch":
         """Fill ``cu_new``, ``slot_map``, ``positions``, the table's new
         entries and the schedule from the lengths as they are now."""
-        rc = self._lib.grm_hip_kv_plan(self._ref, _stream(self.ctx_lens, stream))
+        rc = self._lib.grm_hip_kv_plan(self._ref, self._on(self.ctx_lens, stream))
         if rc:
             _lib.check(rc, "kv plan")
         self._planned = True
@@ -250,6 +255,21 @@ class KvBatch:
         if not held or held[-1].nbytes < need:
             held.append(_empty(like, (need,), "u8", stream))
         return held[-1].data_ptr()
+
+    def _on(self, like, stream) -> int:
+        """The stream a call runs on.  What this object made is torch's to hand
+        out again once it is dropped, but not before that stream is through
+        with it."""
+        on = _stream(like, stream)
+        if on not in self._streams:
+            self._streams.add(on)
+            if _is_torch(self._work):
+                s = _torch_stream(self._work, on)
+                for a in (self.cu_new, self.slot_map, self.positions, self._work,
+                          self._made_head):
+                    if a is not None:
+                        a.record_stream(s)
+        return on
 
     def _need_plan(self):
         if not self._planned:
@@ -310,7 +330,7 @@ class KvCache:
         if vname != name:
             raise ValueError("k and v must have one type")
         rc = self._lib.grm_hip_kv_append(self._ref, batch._ref, kp, vptr, _lib.DTYPE_CODES[name],
-                                         kt, kh, vt, vh, _stream(k, stream))
+                                         kt, kh, vt, vh, batch._on(k, stream))
         if rc:
             _lib.check(rc, "kv append")
 
@@ -344,7 +364,7 @@ class KvCache:
             need = batch._scratch[self.head_dim] = got.value
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(self.head_dim)
-        on = _stream(q, stream)
+        on = batch._on(q, stream)
         rc = self._lib.grm_hip_kv_attend(
             self._ref, batch._ref, qp, _lib.DTYPE_CODES[name], qt, qh, op, ot, oh, lp,
             softmax_scale, batch._scratch_on(q, need, on, stream) if need else None, need, on)

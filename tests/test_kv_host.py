@@ -101,3 +101,51 @@ def test_scratch_of_a_cache_that_does_not_fit_is_refused(change):
     assert real.grm_hip_kv_attend_bytes(ctypes.byref(cache_desc(**change)),
                                         ctypes.byref(batch_desc()), ctypes.byref(out)) == -1
     assert b"differ" in real.grm_hip_last_error() and out.value == 7
+
+
+def test_a_batch_is_kept_for_the_streams_that_read_it(lib, monkeypatch):
+    """The schedule and the other arrays that a batch made are recorded for every
+    stream that a call names, beside the one that they were made on."""
+    kept = []
+
+    class Tensorlike:
+        """An array that is torch's, as far as this side asks."""
+
+        def __init__(self, shape, dtype):
+            self.shape, self.dtype, self.is_cuda = tuple(shape), np.dtype(dtype), True
+            self.nbytes = int(np.prod(shape)) * self.dtype.itemsize
+
+        data_ptr = lambda self: 0x1000        # noqa: E731
+        get_device = lambda self: 0           # noqa: E731
+        is_contiguous = lambda self: True     # noqa: E731
+
+        def stride(self):
+            return tuple(np.cumprod((1, *self.shape[:0:-1]))[::-1].tolist())
+
+        def record_stream(self, s):
+            kept.append((id(self), s))
+
+    monkeypatch.setattr(kc, "_is_torch", lambda a: isinstance(a, Tensorlike))
+    monkeypatch.setattr(kc, "_torch_names", lambda: kc._TORCH)
+    monkeypatch.setattr(kc, "_empty", lambda like, shape, dtype, stream=None: Tensorlike(
+        shape, kc._NUMPY[dtype]))
+    monkeypatch.setattr(kc, "_stream", lambda a, stream: 5 if stream is None else stream)
+    monkeypatch.setattr(kc, "_torch_stream", lambda a, on: ("stream", on))
+    T = Tensorlike
+    b = g.KvBatch(T((3,), np.int32), T((3,), np.int32), T((3, 4), np.int32), 16, tokens=3,
+                  max_new=1, heads=4, kv_heads=2, free_list=T((9,), np.int32),
+                  free_head=T((1,), np.int32))
+    mine = {id(a) for a in (b.cu_new, b.slot_map, b.positions, b._work, b.free_head_out)}
+    c = g.KvCache(T((4, 2, 16, 64), np.int8), T((4, 2, 64, 16), np.int8), T((4, 2), np.float32),
+                  T((4, 2), np.float32))
+    b.plan()
+    b.plan(stream=5)
+    assert not kept                                # where they were made
+    b.plan(stream=7)
+    assert {i for i, _ in kept} == mine and {s for _, s in kept} == {("stream", 7)}
+    c.append(b, T((3, 2, 64), np.float32), T((3, 2, 64), np.float32), stream=7)
+    assert len(kept) == len(mine)                  # once is enough
+    c.append(b, T((3, 2, 64), np.float32), T((3, 2, 64), np.float32), stream=8)
+    assert kept[-1][1] == ("stream", 8)
+    c.attend(b, T((3, 4, 64), np.float32), stream=0)
+    assert {i for i, s in kept if s == ("stream", 0)} == mine
