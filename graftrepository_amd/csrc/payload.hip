@@ -169,6 +169,12 @@ extern "C" int grm_hip_device_alloc(uint64_t bytes, void** out_ptr) {
   return 0;
 }
 
+extern "C" int grm_hip_current_device(int* out_device) {
+  if (!out_device) return grm::fail(-1, "null output pointer");
+  GRM_HIP_CHECK(hipGetDevice(out_device));
+  return 0;
+}
+
 extern "C" int grm_hip_device_free(void* ptr) {
   if (ptr) GRM_HIP_CHECK(hipFree(ptr));
   return 0;

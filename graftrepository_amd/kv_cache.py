@@ -15,7 +15,9 @@ step's ragged batch over it::
 
 Arrays are device memory: torch tensors, or ``payload.DeviceArray`` (there
 bf16 is uint16 bit patterns, as everywhere in this package).  Shapes, laws
-and layouts are those of ``include/grm_hip_router.h``.  Calls are ordered on
+and layouts are those of ``include/grm_hip_router.h``.  All arrays of a batch,
+its caches and its calls are on one GPU, which need not be the current one for
+torch tensors; DeviceArrays are used with theirs current.  Calls are ordered on
 ``stream`` (a HIP stream handle; by default torch's current stream for torch
 tensors, else the default stream) and return before the work has run; they
 can be captured into a HIP graph.  Bad arguments raise ``ValueError`` here or
@@ -31,7 +33,7 @@ import sys
 import numpy as np
 
 from . import _lib
-from .payload import DeviceArray
+from .payload import DeviceArray, current_device
 
 i32, u64, vp = ctypes.c_int32, ctypes.c_uint64, ctypes.c_void_p
 
@@ -153,6 +155,41 @@ def _empty(like, shape, dtype: str, stream=None):
         return t.empty(shape, dtype=_torch_names()[dtype], device=like.device)
 
 
+def _one_device(**arrays) -> int:
+    """The device that all of these are on."""
+    on = {what: a.get_device() for what, a in arrays.items() if a is not None}
+    if len(set(on.values())) != 1:
+        raise ValueError(f"arrays are on more than one GPU: {on}")
+    return next(iter(on.values()))
+
+
+def _same_device(a, what: str, device: int) -> None:
+    if a.get_device() != device:
+        raise ValueError(f"{what} is on GPU {a.get_device()}, the batch or cache on GPU {device}")
+
+
+def _find_torch_device() -> int:
+    global _torch_device
+    t = sys.modules["torch"]
+    _torch_device = getattr(t._C, "_cuda_getDevice", None) or t.cuda.current_device
+    return _torch_device()
+
+
+_torch_device = _find_torch_device  # torch's current device
+
+
+def _call(fn, like, device: int, *args) -> int:
+    """fn(*args) with the arrays' device current, which the library launches on."""
+    if isinstance(like, DeviceArray):
+        here = current_device()
+        if here != device:
+            raise ValueError(f"the arrays are on GPU {device}, the current device is GPU {here}")
+    elif _torch_device() != device:
+        with sys.modules["torch"].cuda.device(device):
+            return fn(*args)
+    return fn(*args)
+
+
 def _torch_stream(like, on: int):
     """The stream of this handle, on the tensor's device."""
     t = sys.modules["torch"]
@@ -165,8 +202,11 @@ _raw_stream = None  # torch's current stream of a device as a handle
 def _stream(a, stream) -> int:
     global _raw_stream
     if stream is not None:
+        if not isinstance(stream, int) and getattr(stream, "device_index", a.get_device()) != a.get_device():
+            raise ValueError(f"a stream of GPU {stream.device_index} for arrays on GPU "
+                             f"{a.get_device()}")
         return int(getattr(stream, "cuda_stream", stream))
-    if not _is_torch(a):
+    if isinstance(a, DeviceArray):
         return 0
     if _raw_stream is None:
         t = sys.modules["torch"]
@@ -211,9 +251,11 @@ class KvBatch:
         d.requests, d.table_width = n, int(block_table.shape[1])
         d.tokens, d.max_new, d.window = int(tokens), int(max_new), int(window)
         d.block_tokens, d.heads, d.kv_heads = int(block_tokens), int(heads), int(kv_heads)
+        self.device = _one_device(ctx_lens=ctx_lens, new_lens=new_lens, block_table=block_table,
+                                  free_list=free_list, free_head=free_head)
         need = u64()
-        _lib.check(self._lib.grm_hip_kv_work_bytes(ctypes.byref(d), ctypes.byref(need)),
-                   "kv work size")
+        _lib.check(_call(self._lib.grm_hip_kv_work_bytes, ctx_lens, self.device, ctypes.byref(d),
+                         ctypes.byref(need)), "kv work size")
         self.ctx_lens, self.new_lens, self.block_table = ctx_lens, new_lens, block_table
         self.cu_new = _empty(ctx_lens, (n + 1,), "i32")
         self.slot_map = _empty(ctx_lens, (d.tokens,), "i64")
@@ -241,7 +283,8 @@ class KvBatch:
     def plan(self, stream=None) -> "KvBatch":
         """Fill ``cu_new``, ``slot_map``, ``positions``, the table's new
         entries and the schedule from the lengths as they are now."""
-        rc = self._lib.grm_hip_kv_plan(self._ref, self._on(self.ctx_lens, stream))
+        rc = _call(self._lib.grm_hip_kv_plan, self.ctx_lens, self.device, self._ref,
+                   self._on(self.ctx_lens, stream))
         if rc:
             _lib.check(rc, "kv plan")
         self._planned = True
@@ -271,7 +314,9 @@ class KvBatch:
                         a.record_stream(s)
         return on
 
-    def _need_plan(self):
+    def _ready_for(self, cache):
+        if cache.device != self.device:
+            raise ValueError(f"the cache is on GPU {cache.device}, the batch on GPU {self.device}")
         if not self._planned:
             raise ValueError("the batch has no plan yet: call plan() first")
 
@@ -301,6 +346,8 @@ class KvCache:
         d.v_codes = _dense(v_codes, "v_codes", "i8", (blocks, kv, hd, bs))
         d.k_scales = _dense(k_scales, "k_scales", "f32", (blocks, kv))
         d.v_scales = _dense(v_scales, "v_scales", "f32", (blocks, kv))
+        self.device = _one_device(k_codes=k_codes, v_codes=v_codes, k_scales=k_scales,
+                                  v_scales=v_scales)
         d.blocks, d.block_tokens, d.kv_heads, d.head_dim = blocks, bs, kv, hd
         if bs not in (16, 32, 64, 128):
             raise ValueError("block_tokens must be 16, 32, 64 or 128")
@@ -323,14 +370,16 @@ class KvCache:
     def append(self, batch: KvBatch, k, v, stream=None) -> None:
         """Quantise the step's ``k`` and ``v`` [tokens, kv_heads, head_dim]
         (f32, bf16 or f16; any row and head strides) into their blocks."""
-        batch._need_plan()
+        batch._ready_for(self)
         shape = (batch._desc.tokens, self.kv_heads, self.head_dim)
         kp, name, kt, kh = _rows(k, "k", shape)
         vptr, vname, vt, vh = _rows(v, "v", shape)
         if vname != name:
             raise ValueError("k and v must have one type")
-        rc = self._lib.grm_hip_kv_append(self._ref, batch._ref, kp, vptr, _lib.DTYPE_CODES[name],
-                                         kt, kh, vt, vh, batch._on(k, stream))
+        _same_device(k, "k", self.device)
+        _same_device(v, "v", self.device)
+        rc = _call(self._lib.grm_hip_kv_append, k, self.device, self._ref, batch._ref, kp, vptr,
+                   _lib.DTYPE_CODES[name], kt, kh, vt, vh, batch._on(k, stream))
         if rc:
             _lib.check(rc, "kv append")
 
@@ -340,10 +389,12 @@ class KvCache:
         head_dim] over the cache, which holds the step's own tokens.  Returns
         ``out`` (q's type; also taken as an argument), with ``return_lse``
         also the fp32 [tokens, heads] log-sum-exp of the scores."""
-        batch._need_plan()
+        batch._ready_for(self)
         d = batch._desc
         shape = (d.tokens, d.heads, self.head_dim)
         qp, name, qt, qh = _rows(q, "q", shape)
+        if q.get_device() != self.device:
+            _same_device(q, "q", self.device)
         if out is None:
             out = _empty(q, shape, name, stream)
             op, ot, oh = out.data_ptr(), shape[1] * shape[2], shape[2]
@@ -351,23 +402,27 @@ class KvCache:
             op, oname, ot, oh = _rows(out, "out", shape)
             if oname != name:
                 raise ValueError("out must have q's type")
+            _same_device(out, "out", self.device)
         if lse is None and return_lse:
             lse = _empty(q, shape[:2], "f32", stream)
             lp = lse.data_ptr()
         else:
             lp = _dense(lse, "lse", "f32", shape[:2]) if lse is not None else None
+            if lse is not None:
+                _same_device(lse, "lse", self.device)
         need = batch._scratch.get(self.head_dim)
         if need is None:
             got = u64()
-            _lib.check(self._lib.grm_hip_kv_attend_bytes(self._ref, batch._ref,
-                                                         ctypes.byref(got)), "kv scratch size")
+            _lib.check(_call(self._lib.grm_hip_kv_attend_bytes, q, self.device, self._ref,
+                             batch._ref, ctypes.byref(got)), "kv scratch size")
             need = batch._scratch[self.head_dim] = got.value
         if softmax_scale is None:
             softmax_scale = 1.0 / math.sqrt(self.head_dim)
         on = batch._on(q, stream)
-        rc = self._lib.grm_hip_kv_attend(
-            self._ref, batch._ref, qp, _lib.DTYPE_CODES[name], qt, qh, op, ot, oh, lp,
-            softmax_scale, batch._scratch_on(q, need, on, stream) if need else None, need, on)
+        rc = _call(
+            self._lib.grm_hip_kv_attend, q, self.device, self._ref, batch._ref, qp,
+            _lib.DTYPE_CODES[name], qt, qh, op, ot, oh, lp, softmax_scale,
+            batch._scratch_on(q, need, on, stream) if need else None, need, on)
         if rc:
             _lib.check(rc, "kv attend")
         return (out, lse) if return_lse else out
@@ -383,11 +438,14 @@ class KvCache:
         table = _dense(block_table, "block_table", "i32", (n, block_table.shape[1]))
         sp = _dense(starts, "starts", "i32", (n,))
         cp = _dense(cu_rows, "cu_rows", "i32", (n + 1,))
+        for a, what in ((block_table, "block_table"), (starts, "starts"), (cu_rows, "cu_rows")):
+            _same_device(a, what, self.device)
         shape = (int(rows), self.kv_heads, self.head_dim)
         k, v = _empty(starts, shape, name, stream), _empty(starts, shape, name, stream)
-        rc = self._lib.grm_hip_kv_read(
-            self._ref, table, int(block_table.shape[1]), n, sp, cp, shape[0],
-            _lib.DTYPE_CODES[name], k.data_ptr(), v.data_ptr(), _stream(starts, stream))
+        rc = _call(
+            self._lib.grm_hip_kv_read, starts, self.device, self._ref, table,
+            int(block_table.shape[1]), n, sp, cp, shape[0], _lib.DTYPE_CODES[name], k.data_ptr(),
+            v.data_ptr(), _stream(starts, stream))
         if rc:
             _lib.check(rc, "kv read")
         return k, v

@@ -35,12 +35,22 @@ class PayloadFormatError(ValueError):
     core/graft_quant.py:74-76)."""
 
 
+def current_device() -> int:
+    """The calling thread's HIP device."""
+    got = ctypes.c_int()
+    _lib.check(_lib.load().grm_hip_current_device(ctypes.byref(got)), "current device")
+    return got.value
+
+
 class DeviceArray:
     """Values in device memory owned by this object (row-major ``shape``,
     numpy ``dtype``, fp16 by default).  ``ptr`` is the device address;
     ``to_host()`` copies them back, ``from_host(a)`` makes one holding a
     copy of a host array.  ``sub(i)`` is the address of entry i along the
-    first axis, e.g. one layer of an (L, H, S, D) node payload."""
+    first axis, e.g. one layer of an (L, H, S, D) node payload.  ``device`` is
+    the HIP device it is on, the current one when it was made."""
+
+    device = 0
 
     def __init__(self, shape, dtype=np.float16):
         self.shape = tuple(int(d) for d in shape)
@@ -52,6 +62,7 @@ class DeviceArray:
         _lib.check(self._lib.grm_hip_device_alloc(max(self.nbytes, 2), ctypes.byref(p)),
                    "device alloc")
         self.ptr = int(p.value)
+        self.device = current_device()
 
     def to_host(self) -> np.ndarray:
         out = np.empty(self.shape, dtype=self.dtype)
@@ -74,6 +85,9 @@ class DeviceArray:
 
     def data_ptr(self) -> int:
         return self.ptr
+
+    def get_device(self) -> int:
+        return self.device
 
     def close(self) -> None:
         if getattr(self, "ptr", 0):

@@ -476,6 +476,8 @@ int grm_hip_payload_upload(const void* h_codes, const void* h_scales, uint64_t n
 /* Device memory for payload outputs (no counterpart; the reference's
  * equivalents are the sidecars' upload_queries / free_device_ptr). */
 int grm_hip_device_alloc(uint64_t bytes, void** out_ptr);
+/* The calling thread's HIP device, on which grm_hip_device_alloc allocates. */
+int grm_hip_current_device(int* out_device);
 int grm_hip_device_free(void* ptr);
 int grm_hip_copy_to_host(void* host, const void* device, uint64_t bytes);
 int grm_hip_copy_to_device(void* device, const void* host, uint64_t bytes);
@@ -503,8 +505,10 @@ int grm_hip_copy_to_device(void* device, const void* host, uint64_t bytes);
  * cu_new[r] + i of every per-token array.  Its position p lies in block
  * block_table[r][p / block_tokens].
  *
- * Unlike the rest of the library these calls are ordered on the caller's
- * stream (a hipStream_t; NULL is the default stream): they launch and
+ * Unlike the rest of the library these calls run on the calling thread's
+ * device, which has to be the one that the arrays and the stream are of, and
+ * are ordered on the caller's
+ * stream (a hipStream_t; NULL is the device's default stream): they launch and
  * return, allocate nothing, read no device memory on the host and can be
  * captured into a HIP graph.  Argument errors are found on the host and
  * return -1 with nothing launched.  Every array must stay valid, and be

@@ -1,8 +1,11 @@
 """What the key/value cache's Python side keeps and checks on the host, with a
 library and arrays that only write down what they are asked (CPU only)."""
 
+import contextlib
 import ctypes
 import gc
+import sys
+import types
 import weakref
 
 import numpy as np
@@ -103,49 +106,138 @@ def test_scratch_of_a_cache_that_does_not_fit_is_refused(change):
     assert b"differ" in real.grm_hip_last_error() and out.value == 7
 
 
+class Tensorlike:
+    """An array that is torch's, as far as this side asks."""
+
+    def __init__(self, shape, dtype, device=0, kept=None):
+        self.shape, self.dtype, self.is_cuda = tuple(shape), np.dtype(dtype), True
+        self.nbytes, self.on, self.kept = int(np.prod(shape)) * self.dtype.itemsize, device, kept
+
+    def data_ptr(self):
+        return 0x1000
+
+    def get_device(self):
+        return self.on
+
+    def is_contiguous(self):
+        return True
+
+    def stride(self):
+        return tuple(np.cumprod((1, *self.shape[:0:-1]))[::-1].tolist())
+
+    def record_stream(self, s):
+        self.kept.append((id(self), s))
+
+
+class Device:
+    """torch's current device, and what is called under which."""
+
+    def __init__(self, monkeypatch, lib, current):
+        self.current, self.under = current, []
+        monkeypatch.setattr(kc, "_is_torch", lambda a: isinstance(a, Tensorlike))
+        monkeypatch.setattr(kc, "_torch_names", lambda: kc._TORCH)
+        monkeypatch.setattr(kc, "_empty", lambda like, shape, dtype, stream=None: Tensorlike(
+            shape, kc._NUMPY[dtype], like.on, like.kept))
+        monkeypatch.setattr(kc, "_torch_device", lambda: self.current)
+        monkeypatch.setattr(kc, "_raw_stream", lambda device: 16 + device)
+        monkeypatch.setitem(sys.modules, "torch", types.SimpleNamespace(
+            cuda=types.SimpleNamespace(device=self.switch), Tensor=Tensorlike))
+        for name in ("work_bytes", "attend_bytes", "plan", "append", "attend", "read"):
+            name = "grm_hip_kv_" + name
+            setattr(lib, name, lambda *a, fn=getattr(lib, name), n=name: (
+                self.under.append((n, self.current, a)), fn(*a))[1])
+
+    @contextlib.contextmanager
+    def switch(self, device):
+        was, self.current = self.current, device
+        yield
+        self.current = was
+
+
+def on_gpu(device, **kw):
+    def T(shape, dtype):
+        return Tensorlike(shape, dtype, kw.get(str(shape), device), kw.get("kept"))
+    cache = g.KvCache(T((4, 2, 16, 64), np.int8), T((4, 2, 64, 16), np.int8),
+                      T((4, 2), np.float32), T((4, 2), np.float32))
+    batch = g.KvBatch(T((3,), np.int32), T((3,), np.int32), T((3, 4), np.int32), 16, tokens=3,
+                      max_new=1, heads=4, kv_heads=2, free_list=T((9,), np.int32),
+                      free_head=T((1,), np.int32))
+    return T, cache, batch
+
+
 def test_a_batch_is_kept_for_the_streams_that_read_it(lib, monkeypatch):
     """The schedule and the other arrays that a batch made are recorded for every
     stream that a call names, beside the one that they were made on."""
     kept = []
-
-    class Tensorlike:
-        """An array that is torch's, as far as this side asks."""
-
-        def __init__(self, shape, dtype):
-            self.shape, self.dtype, self.is_cuda = tuple(shape), np.dtype(dtype), True
-            self.nbytes = int(np.prod(shape)) * self.dtype.itemsize
-
-        data_ptr = lambda self: 0x1000        # noqa: E731
-        get_device = lambda self: 0           # noqa: E731
-        is_contiguous = lambda self: True     # noqa: E731
-
-        def stride(self):
-            return tuple(np.cumprod((1, *self.shape[:0:-1]))[::-1].tolist())
-
-        def record_stream(self, s):
-            kept.append((id(self), s))
-
-    monkeypatch.setattr(kc, "_is_torch", lambda a: isinstance(a, Tensorlike))
-    monkeypatch.setattr(kc, "_torch_names", lambda: kc._TORCH)
-    monkeypatch.setattr(kc, "_empty", lambda like, shape, dtype, stream=None: Tensorlike(
-        shape, kc._NUMPY[dtype]))
-    monkeypatch.setattr(kc, "_stream", lambda a, stream: 5 if stream is None else stream)
+    Device(monkeypatch, lib, current=0)
     monkeypatch.setattr(kc, "_torch_stream", lambda a, on: ("stream", on))
-    T = Tensorlike
-    b = g.KvBatch(T((3,), np.int32), T((3,), np.int32), T((3, 4), np.int32), 16, tokens=3,
-                  max_new=1, heads=4, kv_heads=2, free_list=T((9,), np.int32),
-                  free_head=T((1,), np.int32))
+    T, c, b = on_gpu(0, kept=kept)
     mine = {id(a) for a in (b.cu_new, b.slot_map, b.positions, b._work, b.free_head_out)}
-    c = g.KvCache(T((4, 2, 16, 64), np.int8), T((4, 2, 64, 16), np.int8), T((4, 2), np.float32),
-                  T((4, 2), np.float32))
     b.plan()
-    b.plan(stream=5)
+    b.plan(stream=16)
     assert not kept                                # where they were made
     b.plan(stream=7)
     assert {i for i, _ in kept} == mine and {s for _, s in kept} == {("stream", 7)}
-    c.append(b, T((3, 2, 64), np.float32), T((3, 2, 64), np.float32), stream=7)
+    x = T((3, 2, 64), np.float32)
+    c.append(b, x, x, stream=7)
     assert len(kept) == len(mine)                  # once is enough
-    c.append(b, T((3, 2, 64), np.float32), T((3, 2, 64), np.float32), stream=8)
+    c.append(b, x, x, stream=8)
     assert kept[-1][1] == ("stream", 8)
     c.attend(b, T((3, 4, 64), np.float32), stream=0)
     assert {i for i, s in kept if s == ("stream", 0)} == mine
+
+
+def test_calls_run_on_the_arrays_device(lib, monkeypatch):
+    """Whatever device is current: sizes, launches and streams are those of the
+    GPU that the arrays are on."""
+    d = Device(monkeypatch, lib, current=0)
+    T, cache, batch = on_gpu(1)
+    batch.plan()
+    cache.append(batch, T((3, 2, 64), np.float32), T((3, 2, 64), np.float32))
+    cache.attend(batch, T((3, 4, 64), np.float32), return_lse=True)
+    cache.read(T((3, 4), np.int32), T((3,), np.int32), T((4,), np.int32), 5)
+    assert len(d.under) == 6 and d.current == 0
+    for name, current, args in d.under:
+        assert current == 1, name
+        if not name.endswith("bytes"):
+            assert args[-1] == 17, name            # that device's stream
+    assert {batch.device, cache.device, batch.cu_new.get_device()} == {1}
+
+
+def test_arrays_of_several_gpus_are_refused(lib, monkeypatch):
+    d = Device(monkeypatch, lib, current=0)
+    for other in ((3, 4), (9,), (4, 2)):
+        with pytest.raises(ValueError, match="more than one GPU"):
+            on_gpu(0, **{str(other): 1})
+    T, cache, batch = on_gpu(0)
+    _, far, _ = on_gpu(1)
+    batch.plan()
+    d.under.clear()
+    f4, i4 = np.float32, np.int32
+    kv, q, there = T((3, 2, 64), f4), T((3, 4, 64), f4), lambda s, t: Tensorlike(s, t, 1)
+    for call in (lambda: cache.append(batch, there((3, 2, 64), f4), kv),
+                 lambda: cache.append(batch, kv, there((3, 2, 64), f4)),
+                 lambda: cache.attend(batch, there((3, 4, 64), f4)),
+                 lambda: cache.attend(batch, q, out=there((3, 4, 64), f4)),
+                 lambda: cache.attend(batch, q, lse=there((3, 4), f4)),
+                 lambda: far.append(batch, kv, kv), lambda: far.attend(batch, q),
+                 lambda: cache.read(T((3, 4), i4), there((3,), i4), T((4,), i4), 5),
+                 lambda: far.read(T((3, 4), i4), T((3,), i4), T((4,), i4), 5),
+                 lambda: batch.plan(stream=types.SimpleNamespace(device_index=1, cuda_stream=9))):
+        with pytest.raises(ValueError, match="GPU 1"):
+            call()
+    assert not [u for u in d.under if not u[0].endswith("bytes")]
+
+
+def test_device_arrays_of_another_gpu_than_the_current_are_refused(lib, monkeypatch):
+    b, c = batch_of(), cache_of(64)
+    monkeypatch.setattr(kc, "current_device", lambda: 1)
+    for call in (b.plan, batch_of):
+        with pytest.raises(ValueError, match="GPU 0, the current device is GPU 1"):
+            call()
+    monkeypatch.setattr(kc, "current_device", lambda: 0)
+    b.plan()
+    x = fake((3, 4, 64), np.float32)
+    x.device = 1
+    with pytest.raises(ValueError, match="GPU 1"):
+        c.attend(b, x)
