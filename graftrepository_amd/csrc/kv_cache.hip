@@ -167,9 +167,15 @@ struct PlanArgs {
   uint64_t at_append, at_units, at_tiles, at_run_units[2], at_scan, at_wide, at_items, at_joins;
 };
 
-// Exclusive sums over the block of N values per thread; totals to `sum`.
-// `scratch` holds N * 16 ints.  Two barriers.
-template <int N>
+// Sums of rows and wide units stop at the largest int: lengths of more tokens
+// than the batch has rows leave what follows past its end.  The other sums are
+// looked at only before that.
+__device__ inline int add(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
+
+// Exclusive sums over the block of N values per thread (0 or more); totals to
+// `sum`.  Bits of STOPS: those that stop.  `scratch` holds N * 16 ints.  Two
+// barriers.
+template <int N, unsigned STOPS>
 __device__ void block_scan(int (&v)[N], int (&sum)[N], int* scratch) {
   const int lane = __lane_id(), wave = threadIdx.x / kWave;
   constexpr int kWaves = kPlanThreads / kWave;
@@ -180,7 +186,7 @@ __device__ void block_scan(int (&v)[N], int (&sum)[N], int* scratch) {
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
       const int o = __shfl_up(v[k], d);
-      if (lane >= d) v[k] += o;
+      if (lane >= d) v[k] = STOPS >> k & 1 ? add(v[k], o) : v[k] + o;
     }
     if (lane == kWave - 1) scratch[k * kWaves + wave] = v[k];
   }
@@ -191,10 +197,11 @@ __device__ void block_scan(int (&v)[N], int (&sum)[N], int* scratch) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const int t = scratch[k * kWaves + w];
-      before += w < wave ? t : 0;
-      all += t;
+      const int mine = w < wave ? t : 0;
+      before = STOPS >> k & 1 ? add(before, mine) : before + mine;
+      all = STOPS >> k & 1 ? add(all, t) : all + t;
     }
-    v[k] = v[k] - own[k] + before;
+    v[k] = STOPS >> k & 1 ? add(v[k] - own[k], before) : v[k] - own[k] + before;
     sum[k] = all;
   }
   __syncthreads();
@@ -265,25 +272,25 @@ __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
       l[j] = lens_of(a, r0 + j);
-      v[0] += l[j].fresh;
+      v[0] = add(v[0], l[j].fresh);
       v[1] += l[j].need;
       v[2] += l[j].touched;
     }
-    block_scan(v, sum, scratch);
+    block_scan<3, 1u>(v, sum, scratch);
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
       const int i = threadIdx.x * kPerThread + j;
-      s_cu[i] = done_new + v[0];
+      s_cu[i] = add(done_new, v[0]);
       s_ctx[i] = l[j].ctx;
       s_need[i] = done_need + v[1];
       s_touch[i] = done_touch + v[2];
-      v[0] += l[j].fresh;
+      v[0] = add(v[0], l[j].fresh);
       v[1] += l[j].need;
       v[2] += l[j].touched;
     }
     __syncthreads();
     const int here = min(kPlanChunk, a.requests - base);
-    const int end = min(t1, done_new + sum[0]);
+    const int end = min(t1, add(done_new, sum[0]));
     for (int i = max(t0, done_new) + static_cast<int>(threadIdx.x); i < end; i += kPlanThreads) {
       // the last request whose first row is not past i: it has a token there
       const int k = upper(s_cu, here, i);
@@ -304,7 +311,7 @@ __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
       if (a.positions) a.positions[i] = pos;
       if (place == 0 || t == 0) {
         const int at = s_touch[k] + j - (ctx >> a.block_log2);
-        const int next = k + 1 < here ? s_cu[k + 1] : done_new + sum[0];
+        const int next = k + 1 < here ? s_cu[k + 1] : add(done_new, sum[0]);
         if (static_cast<unsigned>(at) < static_cast<unsigned>(a.cap_append)) {
           AppendItem it;
           it.block = block;
@@ -316,7 +323,7 @@ __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
       }
     }
     filled = max(filled, end);
-    done_new += sum[0];
+    done_new = add(done_new, sum[0]);
     done_need += sum[1];
     done_touch += sum[2];
     __syncthreads();
@@ -344,6 +351,8 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   int* tiles = reinterpret_cast<int*>(a.work + a.at_tiles);
   int* wide_at = reinterpret_cast<int*>(a.work + a.at_scan);
   const bool wide_fits = a.requests < kWideInts;
+  int* appends = lds + 6 * 16;  // touched blocks before the batch's last row
+  if (threadIdx.x == 0) *appends = a.cap_append;
   // new tokens, blocks needed, touched blocks, narrow tiles, wide units,
   // narrow units
   int done[6] = {0, 0, 0, 0, 0, 0};
@@ -364,16 +373,16 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
       }
       wide[j] = a.wide_tokens && l[j].fresh > 0 && !narrow[j]
                     ? (l[j].fresh + a.wide_tokens - 1) / a.wide_tokens : 0;
-      v[0] += l[j].fresh;
+      v[0] = add(v[0], l[j].fresh);
       v[1] += l[j].need;
       v[2] += l[j].touched;
       v[3] += hi[j] - lo[j];
-      v[4] += wide[j];
+      v[4] = add(v[4], wide[j]);
       v[5] += narrow[j];
     }
-    block_scan(v, sum, scratch);
+    block_scan<6, 0x11u>(v, sum, scratch);
 #pragma unroll
-    for (int k = 0; k < 6; ++k) v[k] += done[k];
+    for (int k = 0; k < 6; ++k) v[k] = k % 4 == 0 ? add(v[k], done[k]) : v[k] + done[k];
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
       const int r = r0 + j;
@@ -396,13 +405,22 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
           if (v[5] < kPlanChunk) tiles_lds[v[5]] = v[3];
         }
       }
-      v[0] += l[j].fresh;
+      const int left = a.tokens - v[0];
+      if (left >= 0 && l[j].fresh > left) {
+        // The request that passes the last row: blocks from the first token
+        // without one on are in no entry of the list.
+        const int bs = 1 << a.block_log2;
+        *appends = v[2] + (left ? ((l[j].ctx + left + bs - 1) >> a.block_log2) -
+                                      (l[j].ctx >> a.block_log2) : 0);
+      }
+      v[0] = add(v[0], l[j].fresh);
+      v[2] += l[j].touched;
       v[3] += hi[j] - lo[j];
-      v[4] += wide[j];
+      v[4] = add(v[4], wide[j]);
       v[5] += narrow[j];
     }
 #pragma unroll
-    for (int k = 0; k < 6; ++k) done[k] += sum[k];
+    for (int k = 0; k < 6; ++k) done[k] = k % 4 == 0 ? add(done[k], sum[k]) : done[k] + sum[k];
   }
   const int done_units = max(0, min(done[5], a.cap_units));
   const int wide_units = done[4];
@@ -418,15 +436,15 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     if (a.free_head) {
       const int at = max(0, *a.free_head);
       const int left = max(0, a.free_count - at);
-      *a.free_head_out = at + min(left, done[1]);
+      *a.free_head_out = at + min(left, max(0, done[1]));
     }
-    head->appends = min(done[2], a.cap_append);
     head->units = done_units;
     head->narrow_tiles = done[3];
     head->items = 0;
     head->joins = 0;
   }
   __syncthreads();  // the lists are read back by other threads of this block
+  if (threadIdx.x == 0) head->appends = min(done[0] > a.tokens ? *appends : done[2], a.cap_append);
 
   // The unit that each run of the narrow kernel begins in; 0 where it is empty.
   if (a.cap_units > 0) {
@@ -449,7 +467,9 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   // start and end.
   constexpr int kCands = 8;
   const float kOf[kCands] = {1.25f, 1.125f, 1.0f, 0.625f, 0.5f, 0.4f, 1.0f / 3.0f, 0.25f};
-  int* count = lds + 6 * 16;  // of each candidate: items, longest, shortest; then all tiles and the longest unit
+  // Of each candidate: items, longest, shortest; then all tiles and the longest
+  // unit.  (In the place of `appends`, which the same thread has read.)
+  int* count = lds + 6 * 16;
   int* longest_of = count + kCands;
   int* shortest_of = longest_of + kCands;
   auto* total_at = reinterpret_cast<unsigned long long*>(shortest_of + kCands);
@@ -562,7 +582,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
     }
     int cut = u >= 0 ? max(1, (hi - lo + share - 1) / share) : 0;
     int v[3] = {cut, cut > 1 ? 1 : 0, cut > 1 ? cut : 0}, sum[3];
-    block_scan(v, sum, scratch);
+    block_scan<3, 0u>(v, sum, scratch);
     if (u >= 0) {
       const int ctx_row = a.cu_new[r];
       const int part = done_parts + v[2];
@@ -693,6 +713,7 @@ __device__ inline bool append_work(const AppendArgs& a, AppendWork<T>* w) {
   // the list has a place for every block of the grid
   w->it = {list[item].block, list[item].row, list[item].place, list[item].count};
   if (item >= head->appends) return false;
+  if (w->it.count <= 0 || w->it.row < 0 || w->it.row > a.rows - w->it.count) return false;
   if (w->it.block < 0 || static_cast<uint64_t>(w->it.block) >= a.blocks) return false;
   w->token_stride = a.token_stride[kv];
   w->x = static_cast<const typename T::store*>(a.x[kv]) +

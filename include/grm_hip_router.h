@@ -563,7 +563,9 @@ int grm_hip_kv_work_bytes(const grm_kv_batch_desc* batch, uint64_t* out_bytes);
  * are not written by append and not seen by attend).  A request's tokens
  * past table_width blocks have no slot either.  Append and attend follow the
  * last plan: lengths, table and rows may change only before the next one.
- * Lengths below 0 count as 0, and past 2^30 - 256 as that. */
+ * Lengths below 0 count as 0, and past 2^30 - 256 as that.  Where they sum to
+ * more than `tokens`, those past its rows are not written, and a request that
+ * passes them is not attended whole. */
 int grm_hip_kv_plan(const grm_kv_batch_desc* batch, void* stream);
 
 /* Quantise a step's keys and values into their blocks.  k, v [tokens]
