@@ -227,7 +227,8 @@ static void launch_cores(AttendArgs a, const Shape& s, hipStream_t stream) {
     join.narrow = places * join.cols;
     joins += join.narrow;
   }
-  join_kernel<T, D><<<dim3(static_cast<unsigned>(joins), kv), 256, 0, stream>>>(a, join);
+  // no units of either kind (a step that may bring no token): nothing to do
+  if (joins) join_kernel<T, D><<<dim3(static_cast<unsigned>(joins), kv), 256, 0, stream>>>(a, join);
 }
 
 template <class T>

@@ -29,3 +29,17 @@ def test_a_batch_dropped_while_another_stream_reads_it(hip_lib):
     assert at not in [o.data_ptr() for o in others]
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("heads", [2, 32, 64, 256, 260])
+@pytest.mark.parametrize("hd", [128, 48])
+def test_a_step_that_may_bring_no_token(hip_lib, heads, hd):
+    """max_new = 0 with rows to spare: nothing to attend, whatever the group."""
+    s = Setup([40, 3], [0, 0], 2, hd, 16, extra_rows=3)
+    cache, batch = s.cache(), s.batch(heads)
+    q = torch.randn(3, heads, hd, device="cuda", dtype=torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    cache.append(batch, q[:, :2], q[:, :2])
+    cache.attend(batch, q, out=out)
+    assert (out == 7.0).all()
+    np.testing.assert_array_equal(cache.k_codes.cpu().numpy(), s.kc)
