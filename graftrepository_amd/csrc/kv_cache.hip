@@ -342,6 +342,14 @@ constexpr int kPlanInts = 4 * kPlanChunk + 256;
 // units.  Latency: 256 requests of one token take 10 us, 4001 of 1 to 300
 // tokens 27.5, 24 prompts whose units are cut 17.
 __device__ void plan_schedule(const PlanArgs& a, int* lds) {
+  if (a.requests == 0) {
+    // no schedule, which nobody reads; the lists that others go on from
+    if (threadIdx.x == 0) {
+      if (a.cu_new) a.cu_new[0] = 0;
+      if (a.free_head && a.free_head_out) *a.free_head_out = max(0, *a.free_head);
+    }
+    return;
+  }
   int* scratch = lds;                                     // [kScanInts]
   int* tiles_lds = lds + kScanInts;                       // [kPlanChunk]
   int* wide_lds = tiles_lds + kPlanChunk;                 // the rest
@@ -1169,13 +1177,9 @@ extern "C" int grm_hip_kv_work_bytes(const grm_kv_batch_desc* batch, uint64_t* o
 
 extern "C" int grm_hip_kv_plan(const grm_kv_batch_desc* b, void* stream) {
   GRM_CHECK_RC(check_batch(b, true));
-  if (b->requests == 0) {
-    grm::clear_error();
-    return 0;
-  }
   Layout l;
   GRM_CHECK_RC(layout_of(b, &l));
-  if (b->work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_kv_work_bytes");
+  if (b->requests && b->work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_kv_work_bytes");
   PlanArgs a{};
   a.ctx_lens = b->ctx_lens;
   a.new_lens = b->new_lens;

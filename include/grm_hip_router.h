@@ -563,6 +563,8 @@ int grm_hip_kv_work_bytes(const grm_kv_batch_desc* batch, uint64_t* out_bytes);
  * are not written by append and not seen by attend).  A request's tokens
  * past table_width blocks have no slot either.  Append and attend follow the
  * last plan: lengths, table and rows may change only before the next one.
+ * A batch without requests has its sums, rows and free_head_out written too
+ * (arrays that it does not have may be NULL), and no schedule.
  * Lengths below 0 count as 0, and past 2^30 - 256 as that.  Where they sum to
  * more than `tokens`, those past its rows are not written, and a request that
  * passes them is not attended whole. */

@@ -43,3 +43,25 @@ def test_a_step_that_may_bring_no_token(hip_lib, heads, hd):
     cache.attend(batch, q, out=out)
     assert (out == 7.0).all()
     np.testing.assert_array_equal(cache.k_codes.cpu().numpy(), s.kc)
+
+
+@pytest.mark.parametrize("tokens", [0, 5, 9000])
+def test_a_batch_without_requests(hip_lib, tokens):
+    """The plan writes its outputs all the same: sums, rows without a slot, and
+    the free list's head, from which the next step goes on."""
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    b = KvBatch(none, none, none.view(0, 4), 16, tokens=tokens, max_new=1, heads=2, kv_heads=2,
+                free_list=dev(np.arange(9, dtype=np.int32)),
+                free_head=dev(np.array([3], np.int32)))
+    for a in (b.cu_new, b.slot_map, b.positions, b.free_head_out):
+        a.fill_(77)
+    b.plan()
+    assert b.cu_new.tolist() == [0] and b.free_head_out.tolist() == [3]
+    assert (b.slot_map == -1).all() and (b.positions == -1).all()
+    s = Setup([0], [1], 2, 64, 16)
+    cache = s.cache()
+    x = torch.randn(tokens, 2, 64, device="cuda")
+    cache.append(b, x, x)
+    assert cache.attend(b, x, out=torch.full_like(x, 7.0)).eq(7.0).all()
+    b.advance()
+    assert b.free_head.tolist() == [3]
