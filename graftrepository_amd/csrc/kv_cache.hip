@@ -47,6 +47,8 @@ int check_batch(const grm_kv_batch_desc* b, bool with_arrays) {
     return fail(-1, "heads must be a positive multiple of kv_heads");
   }
   if (b->heads > 65535) return fail(-1, "more than 65535 heads");
+  const int64_t columns = static_cast<int64_t>(b->table_width) * b->block_tokens / kTile + 2;
+  if (columns * b->requests > 0x7fffffff) return fail(-1, "batch too large");
   if (!with_arrays || b->requests == 0) return 0;
   if (!b->ctx_lens || !b->new_lens || !b->cu_new || !b->work) {
     return fail(-1, "null array in the batch");
@@ -95,6 +97,8 @@ int layout_of(const grm_kv_batch_desc* b, Layout* out) {
   int cus = 0;
   GRM_CHECK_RC(device_cus(&cus));
   l.group = b->heads / b->kv_heads;
+  l.reach = static_cast<int32_t>(std::min<int64_t>(
+      static_cast<int64_t>(b->table_width) * b->block_tokens, 2 * static_cast<int64_t>(kMaxLen)));
   const uint64_t rows = static_cast<uint64_t>(b->tokens);
   const uint64_t reqs = static_cast<uint64_t>(b->requests);
   const uint64_t busy = std::min(rows, reqs);  // requests that bring tokens
@@ -109,8 +113,16 @@ int layout_of(const grm_kv_batch_desc* b, Layout* out) {
   if (l.wide_tokens) {
     l.cap_wide = rows / l.wide_tokens + busy;
     // Only units longer than the share C = all / (4 x blocks) are cut, into
-    // at most 2 x length / C parts.
-    l.cap_parts = 8 * static_cast<uint64_t>(l.wide_blocks) + 8;
+    // at most 2 x length / C parts; and only into parts of kLeastShare tiles.
+    // A unit's tiles are the table's or, with a window, what it spans.
+    uint64_t tiles = (static_cast<uint64_t>(l.reach) + kTile - 1) / kTile;
+    if (b->window) {
+      tiles = std::min(tiles, (static_cast<uint64_t>(b->window) + l.wide_tokens + 2 * kTile) / kTile);
+    }
+    if (tiles > kLeastShare) {
+      l.cap_parts = std::min(8 * static_cast<uint64_t>(l.wide_blocks) + 8,
+                             l.cap_wide * ((tiles + kLeastShare - 1) / kLeastShare));
+    }
     l.cap_joins = l.cap_parts / 2;
     l.cap_items = l.cap_wide + l.cap_parts;
   }
@@ -159,7 +171,7 @@ struct PlanArgs {
   int64_t* slots;
   int32_t* positions;
   char* work;
-  int32_t requests, width, tokens, window;
+  int32_t requests, width, tokens, window, reach;
   int32_t free_count, group, wide_tokens, kv_heads;
   int32_t wide_blocks, block_log2;
   int32_t cap_append, cap_units, cap_wide, cap_items, cap_joins, cap_parts;
@@ -244,13 +256,13 @@ __device__ inline int upper(const int* pre, int n, int x) {
 }
 
 // Key tiles [lo, hi) of `tile` tokens that query tokens [t0, t0 + n) of a
-// request see.
+// request see, as far as the table has blocks; one at least.
 __device__ inline void tiles_of(const PlanArgs& a, int tile, int ctx, int t0, int n, int* lo,
                                 int* hi) {
   const int last = ctx + t0 + n;  // keys before this are seen by the last token
   const int first = a.window > 0 ? max(0, ctx + t0 + 1 - a.window) : 0;
   *lo = first / tile;
-  *hi = (last + tile - 1) / tile;
+  *hi = max(*lo + 1, (min(last, a.reach) + tile - 1) / tile);
 }
 
 __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
@@ -522,7 +534,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   int share = longest;
   if (even < longest) {  // else none is cut
     auto candidate = [&](float of) {
-      return max(8, static_cast<int>(ceilf(static_cast<float>(even) * of)));
+      return max(kLeastShare, static_cast<int>(ceilf(static_cast<float>(even) * of)));
     };
     // A candidate to a wavefront, or to several that share the units.
     constexpr int kShare = kPlanThreads / kWave / kCands;
@@ -1195,6 +1207,7 @@ extern "C" int grm_hip_kv_plan(const grm_kv_batch_desc* b, void* stream) {
   a.width = b->table_width;
   a.tokens = b->tokens;
   a.window = b->window;
+  a.reach = l.reach;
   a.free_count = static_cast<int32_t>(b->free_count);
   a.group = l.group;
   a.wide_tokens = l.wide_tokens;

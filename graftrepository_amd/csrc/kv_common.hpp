@@ -14,6 +14,7 @@ namespace kv {
 constexpr int kTile = 64;         // key tokens to a tile of the wide kernel
 constexpr int kNarrowCols = 16;   // (token, head) columns of a narrow unit
 constexpr int kWideCols = 128;    // and of a wide one
+constexpr int kLeastShare = 8;    // key tiles that a wide unit is cut by, at least
 // A length read from the device is cut to this: two of them and a block fit
 // an int.
 constexpr int kMaxLen = (1 << 30) - 256;
@@ -103,6 +104,7 @@ struct Layout {
   int wide_tokens;    // tokens to a wide unit (0: no wide units)
   int wide_blocks;    // wide blocks that run at once, per kv head
   uint64_t cap_append, cap_units, cap_wide, cap_items, cap_joins, cap_parts;
+  int32_t reach;      // tokens of a request that the table has blocks for
   int runs[2];        // of the narrow kernel, with one and two blocks to a CU
   uint64_t at_append, at_units, at_tiles, at_run_units[2], at_scan, at_wide, at_items, at_joins, bytes;
 };
