@@ -20,7 +20,8 @@ its caches and its calls are on one GPU, which need not be the current one for
 torch tensors; DeviceArrays are used with theirs current.  Calls are ordered on
 ``stream`` (a HIP stream handle; by default torch's current stream for torch
 tensors, else the default stream) and return before the work has run; they
-can be captured into a HIP graph.  Bad arguments raise ``ValueError`` here or
+can be captured into a HIP graph.  There is no backward pass: values that
+require a gradient are refused where gradients are recorded.  Bad arguments raise ``ValueError`` here or
 ``RuntimeError`` (code -1) from the library, with nothing launched.
 """
 
@@ -128,6 +129,9 @@ def _strides(a) -> tuple[int, ...]:
 def _rows(a, what: str, shape) -> tuple[int, str, int, int]:
     """(address, type, row stride, head stride) of [rows, heads, dim] values
     whose last axis is contiguous."""
+    if getattr(a, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, and the cache has no backward pass: "
+                         "detach it, or call under torch.no_grad()")
     if _FLOATS and _FLOATS.get(getattr(a, "dtype", None)) and a.is_cuda and a.shape == shape:
         st = a.stride()
         if st[2] == 1:  # the usual call, on its short way

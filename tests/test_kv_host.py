@@ -241,3 +241,21 @@ def test_device_arrays_of_another_gpu_than_the_current_are_refused(lib, monkeypa
     x.device = 1
     with pytest.raises(ValueError, match="GPU 1"):
         c.attend(b, x)
+
+
+def test_values_that_require_a_gradient_are_refused(lib, monkeypatch):
+    """There is no backward pass, and a result without one must not look like one."""
+    Device(monkeypatch, lib, current=0)
+    T, cache, batch = on_gpu(0)
+    batch.plan()
+    kv, q = T((3, 2, 64), np.float32), T((3, 4, 64), np.float32)
+    kv2, q2 = T((3, 2, 64), np.float32), T((3, 4, 64), np.float32)
+    kv2.requires_grad = q2.requires_grad = True
+    sys.modules["torch"].is_grad_enabled = lambda: True
+    for call in (lambda: cache.append(batch, kv2, kv), lambda: cache.append(batch, kv, kv2),
+                 lambda: cache.attend(batch, q2), lambda: cache.attend(batch, q, out=q2)):
+        with pytest.raises(ValueError, match="no backward"):
+            call()
+    sys.modules["torch"].is_grad_enabled = lambda: False
+    cache.append(batch, kv2, kv2)
+    cache.attend(batch, q2)
