@@ -282,7 +282,8 @@ class KvBatch:
         self._scratch: dict[int, int] = {}
         self._held: dict[int, list] = {}
         self._streams = {_stream(ctx_lens, None)}
-        self._planned = False
+        self._planned = False  # once
+        self._taken = False    # since the free list last went on
 
     def plan(self, stream=None) -> "KvBatch":
         """Fill ``cu_new``, ``slot_map``, ``positions``, the table's new
@@ -291,7 +292,7 @@ class KvBatch:
                    self._on(self.ctx_lens, stream))
         if rc:
             _lib.check(rc, "kv plan")
-        self._planned = True
+        self._planned = self._taken = True
         return self
 
     def _scratch_on(self, like, need: int, on: int, stream) -> int:
@@ -328,6 +329,10 @@ class KvBatch:
         """The next plan goes on in the free list where the last one ended."""
         if self.free_list is None:
             raise ValueError("the batch has no free list")
+        if not self._taken:
+            raise ValueError("no plan since the last advance: the list would go back to where "
+                             "that began, and hand its blocks out again")
+        self._taken = False
         d = self._desc
         self.free_head, self.free_head_out = self.free_head_out, self.free_head
         d.free_head, d.free_head_out = d.free_head_out, d.free_head

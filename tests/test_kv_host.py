@@ -259,3 +259,19 @@ def test_values_that_require_a_gradient_are_refused(lib, monkeypatch):
     sys.modules["torch"].is_grad_enabled = lambda: False
     cache.append(batch, kv2, kv2)
     cache.attend(batch, q2)
+
+
+def test_the_free_list_goes_on_once_a_plan(lib):
+    """A second advance would go back to the head before, whose blocks the plan
+    has handed out; one before any plan, to memory that nobody has written."""
+    b = batch_of(free_list=fake((9,), np.int32), free_head=fake((1,), np.int32))
+    first, second = b.free_head, b.free_head_out
+    with pytest.raises(ValueError, match="no plan"):
+        b.advance()
+    assert b.free_head is first
+    b.plan().plan().advance()
+    assert b.free_head is second and b._desc.free_head == second.data_ptr()
+    with pytest.raises(ValueError, match="no plan"):
+        b.advance()
+    b.plan().advance()
+    assert b.free_head is first
