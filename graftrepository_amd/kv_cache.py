@@ -71,6 +71,14 @@ def _torch_names() -> dict[str, object]:
     return _TORCH
 
 
+def _size(n, what: str) -> int:
+    """A size for a field of 32 bits, which ctypes would cut to them."""
+    n = int(n)
+    if not -(1 << 31) <= n < 1 << 31:
+        raise ValueError(f"{what} must fit 32 bits, got {n}")
+    return n
+
+
 def _is_torch(a) -> bool:
     t = sys.modules.get("torch")
     return t is not None and isinstance(a, t.Tensor)
@@ -253,8 +261,10 @@ class KvBatch:
         d.new_lens = _dense(new_lens, "new_lens", "i32", (n,))
         d.block_table = _dense(block_table, "block_table", "i32", (n, None))
         d.requests, d.table_width = n, int(block_table.shape[1])
-        d.tokens, d.max_new, d.window = int(tokens), int(max_new), int(window)
-        d.block_tokens, d.heads, d.kv_heads = int(block_tokens), int(heads), int(kv_heads)
+        for what, size in (("tokens", tokens), ("max_new", max_new), ("window", window),
+                           ("block_tokens", block_tokens), ("heads", heads),
+                           ("kv_heads", kv_heads)):
+            setattr(d, what, _size(size, what))
         self.device = _one_device(ctx_lens=ctx_lens, new_lens=new_lens, block_table=block_table,
                                   free_list=free_list, free_head=free_head)
         need = u64()
@@ -449,6 +459,8 @@ class KvCache:
         cp = _dense(cu_rows, "cu_rows", "i32", (n + 1,))
         for a, what in ((block_table, "block_table"), (starts, "starts"), (cu_rows, "cu_rows")):
             _same_device(a, what, self.device)
+        if not 0 <= int(rows) < 1 << 31:
+            raise ValueError(f"rows must be 0 or more and fit 32 bits, got {rows}")
         shape = (int(rows), self.kv_heads, self.head_dim)
         k, v = _empty(starts, shape, name, stream), _empty(starts, shape, name, stream)
         rc = _call(

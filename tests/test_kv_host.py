@@ -275,3 +275,17 @@ def test_the_free_list_goes_on_once_a_plan(lib):
         b.advance()
     b.plan().advance()
     assert b.free_head is first
+
+
+@pytest.mark.parametrize("name", ["tokens", "max_new", "heads", "kv_heads", "window",
+                                  "block_tokens"])
+def test_sizes_that_do_not_fit_are_refused(lib, name):
+    """The descriptor's fields have 32 bits: 2^32 + 4 is not 4."""
+    sizes = dict(tokens=3, max_new=1, heads=4, kv_heads=2, window=0, block_tokens=16)
+    for off in (1 << 32, 1 << 31, -(1 << 32)):
+        bad = {**sizes, name: sizes[name] + off}
+        bs = bad.pop("block_tokens")
+        with pytest.raises(ValueError, match=name):
+            g.KvBatch(fake((3,), np.int32), fake((3,), np.int32), fake((3, 4), np.int32), bs, **bad)
+    with pytest.raises(ValueError, match="rows"):
+        cache_of(64).read(fake((3, 4), np.int32), fake((3,), np.int32), fake((4,), np.int32), -1)
