@@ -11,7 +11,6 @@ and reads its own turn back as the dense values that a deposit packs.
 from __future__ import annotations
 
 import argparse
-import ctypes
 import sys
 import time
 from pathlib import Path
@@ -21,7 +20,8 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
-from graftrepository_amd import KvBatch, KvCache, MlaNodeBank, load  # noqa: E402
+from graftrepository_amd import KvBatch, KvCache, MlaNodeBank  # noqa: E402
+from graftrepository_amd.payload import FORMAT_VERSION, unpack_node_device  # noqa: E402
 
 LAYERS, HEADS, KV_HEADS, DIM, BLOCK = 2, 8, 2, 64, 32
 WIDTH = HEADS * DIM
@@ -30,24 +30,20 @@ GROUP = 32                                   # codes to a scale in a payload
 
 def make_node(rng, tokens: int) -> dict[str, np.ndarray]:
     """A packed node: codes and scales of K and V [layers, kv_heads, tokens, dim]."""
-    node = {"shape": np.array([LAYERS, KV_HEADS, tokens, DIM])}
+    node = dict(format_version=FORMAT_VERSION, storage_bits=8, group_size=GROUP)
     for name in ("k", "v"):
         x = rng.standard_normal((LAYERS, KV_HEADS, tokens, DIM // GROUP, GROUP))
         scale = np.abs(x).max(-1, keepdims=True).astype(np.float32) / 127
         node[name + "_codes"] = np.rint(x / scale).astype(np.int8)
         node[name + "_scales"] = scale
+        node[name + "_shape"] = np.array([LAYERS, KV_HEADS, tokens, DIM])
     return node
 
 
-def unpack(node, name: str) -> torch.Tensor:
-    """fp16 [layers, kv_heads, tokens, dim] on the device."""
-    out = torch.empty(tuple(node["shape"]), dtype=torch.float16, device="cuda")
-    codes, scales, ms = node[name + "_codes"], node[name + "_scales"], ctypes.c_float()
-    rc = load().grm_hip_payload_upload(codes.ctypes.data, scales.ctypes.data, codes.size, GROUP,
-                                       out.data_ptr(), ctypes.byref(ms))
-    if rc:
-        raise RuntimeError("payload unpack failed")
-    return out
+def unpack(node) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V, fp16 [layers, kv_heads, tokens, dim] on the device."""
+    got = unpack_node_device(node)
+    return tuple(torch.as_tensor(got[name], device="cuda") for name in ("k", "v"))
 
 
 def run(sessions: int = 4, steps: int = 8, nodes: int = 16, seed: int = 0) -> dict:
@@ -63,8 +59,8 @@ def run(sessions: int = 4, steps: int = 8, nodes: int = 16, seed: int = 0) -> di
     store = [make_node(rng, int(rng.integers(20, 300))) for _ in range(nodes)]
     with MlaNodeBank(keys) as bank:
         chosen = bank.route(keys[rng.permutation(nodes)[:sessions]], 1).ids[:, 0].astype(int)
-    grafts = [(unpack(store[n], "k"), unpack(store[n], "v")) for n in chosen]
-    lengths = [int(store[n]["shape"][2]) for n in chosen]
+    grafts = [unpack(store[n]) for n in chosen]
+    lengths = [k.shape[2] for k, _ in grafts]
 
     # One pool of blocks for all sessions; a layer's cache is a pool of its own.
     total = [n + steps for n in lengths]

@@ -14,7 +14,8 @@ step's ragged batch over it::
     k, v = cache.read(table, starts, cu_rows, rows)   # dense, to harvest
 
 Arrays are device memory: torch tensors, or ``payload.DeviceArray`` (there
-bf16 is uint16 bit patterns, as everywhere in this package).  Shapes, laws
+bf16 is uint16 bit patterns, as everywhere in this package; a layer of an
+unpacked node goes to ``append`` as ``node["k"].rows(layer)``).  Shapes, laws
 and layouts are those of ``include/grm_hip_router.h``.  All arrays of a batch,
 its caches and its calls are on one GPU, which need not be the current one for
 torch tensors; DeviceArrays are used with theirs current.  Calls are ordered on
@@ -34,7 +35,7 @@ import sys
 import numpy as np
 
 from . import _lib
-from .payload import DeviceArray, current_device
+from .payload import DeviceArray, DeviceRows, current_device
 
 i32, u64, vp = ctypes.c_int32, ctypes.c_uint64, ctypes.c_void_p
 
@@ -101,7 +102,7 @@ def _type(a, what: str) -> str:
         _torch_names()
         if not a.is_cuda:
             raise ValueError(f"{what} must be on the GPU")
-    elif not isinstance(a, DeviceArray):
+    elif not isinstance(a, (DeviceArray, DeviceRows)):
         raise ValueError(f"{what} must be a torch tensor on the GPU or a DeviceArray")
     name = _NAMES.get(a.dtype)
     if name is None:
@@ -119,7 +120,7 @@ def _dense(a, what: str, dtype: str, shape) -> int:
     got = tuple(a.shape)
     if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
         raise ValueError(f"{what} must have shape {shape}, got {got}")
-    if _is_torch(a) and not a.is_contiguous():
+    if not a.is_contiguous() if _is_torch(a) else isinstance(a, DeviceRows):
         raise ValueError(f"{what} must be contiguous")
     return a.data_ptr()
 
@@ -127,6 +128,8 @@ def _dense(a, what: str, dtype: str, shape) -> int:
 def _strides(a) -> tuple[int, ...]:
     if _is_torch(a):
         return a.stride()
+    if isinstance(a, DeviceRows):
+        return a.strides
     out, step = [], 1
     for d in reversed(a.shape):
         out.append(step)
@@ -192,7 +195,7 @@ _torch_device = _find_torch_device  # torch's current device
 
 def _call(fn, like, device: int, *args) -> int:
     """fn(*args) with the arrays' device current, which the library launches on."""
-    if isinstance(like, DeviceArray):
+    if isinstance(like, (DeviceArray, DeviceRows)):
         here = current_device()
         if here != device:
             raise ValueError(f"the arrays are on GPU {device}, the current device is GPU {here}")
@@ -218,7 +221,7 @@ def _stream(a, stream) -> int:
             raise ValueError(f"a stream of GPU {stream.device_index} for arrays on GPU "
                              f"{a.get_device()}")
         return int(getattr(stream, "cuda_stream", stream))
-    if isinstance(a, DeviceArray):
+    if isinstance(a, (DeviceArray, DeviceRows)):
         return 0
     if _raw_stream is None:
         t = sys.modules["torch"]

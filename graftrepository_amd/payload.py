@@ -48,7 +48,9 @@ class DeviceArray:
     ``to_host()`` copies them back, ``from_host(a)`` makes one holding a
     copy of a host array.  ``sub(i)`` is the address of entry i along the
     first axis, e.g. one layer of an (L, H, S, D) node payload.  ``device`` is
-    the HIP device it is on, the current one when it was made."""
+    the HIP device it is on, the current one when it was made.  ``rows(i)`` is
+    such a layer in the order [S, H, D], which a cache's ``append`` takes, and
+    ``torch.as_tensor(a, device="cuda")`` the array as a tensor, both in place."""
 
     device = 0
 
@@ -83,6 +85,16 @@ class DeviceArray:
             raise IndexError(i)
         return self.ptr + i * (self.nbytes // self.shape[0])
 
+    def rows(self, i: int) -> "DeviceRows":
+        """Entry i of an (L, H, S, D) payload as [S, H, D], in place."""
+        if len(self.shape) != 4:
+            raise ValueError(f"rows of a (L, H, S, D) array, this one has shape {self.shape}")
+        return DeviceRows(self, self.sub(i))
+
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        return dict(shape=self.shape, typestr=self.dtype.str, data=(self.ptr, False), version=2)
+
     def data_ptr(self) -> int:
         return self.ptr
 
@@ -105,6 +117,22 @@ class DeviceArray:
             self.close()
         except Exception:
             pass
+
+
+class DeviceRows:
+    """A layer of a (L, H, S, D) DeviceArray as [S, H, D], over its memory,
+    which it keeps."""
+
+    def __init__(self, base: DeviceArray, ptr: int):
+        _, h, s, d = base.shape
+        self.base, self.ptr, self.dtype, self.device = base, ptr, base.dtype, base.device
+        self.shape, self.strides = (s, h, d), (d, s * d, 1)   # in elements
+
+    def data_ptr(self) -> int:
+        return self.ptr
+
+    def get_device(self) -> int:
+        return self.device
 
 
 def is_packed_payload(payload) -> bool:
@@ -195,6 +223,6 @@ def unpack_node_device(payload, names=("k", "v")) -> dict[str, DeviceArray]:
     return out
 
 
-__all__ = ["DeviceArray", "PayloadFormatError", "is_packed_payload", "upload_packed",
+__all__ = ["DeviceArray", "DeviceRows", "PayloadFormatError", "is_packed_payload", "upload_packed",
            "unpack_kv_arrays_device", "unpack_node_device", "FORMAT_VERSION",
            "SUPPORTED_BITS"]

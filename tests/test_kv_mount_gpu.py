@@ -1,0 +1,61 @@
+"""An unpacked node mounted into the 8-bit cache as the package gives it."""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from graftrepository_amd import KvBatch, KvCache  # noqa: E402
+from graftrepository_amd import kv_cache as kc  # noqa: E402
+from graftrepository_amd.payload import DeviceArray, unpack_node_device  # noqa: E402
+from oracle import kv as law  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_node_is_mounted_layer_by_layer_without_torch(hip_lib, packed):
+    layers, kv, n, hd, bs = 3, 2, 37, 64, 16
+    rng = np.random.default_rng(packed)
+    values = {name: rng.standard_normal((layers, kv, n, hd)).astype(np.float16) for name in "kv"}
+    node = dict(values)
+    if packed:
+        node = dict(format_version=1, storage_bits=8, group_size=32)
+        for name, x in values.items():
+            x = x.astype(np.float32).reshape(layers, kv, n, hd // 32, 32)
+            scale = np.abs(x).max(-1, keepdims=True) / np.float32(127)
+            codes = np.rint(x / scale).astype(np.int8)
+            node |= {name + "_codes": codes, name + "_scales": scale,
+                     name + "_shape": np.array((layers, kv, n, hd))}
+            values[name] = (codes * scale).astype(np.float16).reshape(layers, kv, n, hd)
+    got = unpack_node_device(node)
+    put = DeviceArray.from_host
+    table = np.array([[2, 0, 1]], np.int32)
+    batch = KvBatch(put(np.zeros(1, np.int32)), put(np.full(1, n, np.int32)), put(table), bs,
+                    tokens=n, max_new=n, heads=kv, kv_heads=kv).plan()
+    for layer in range(layers):
+        cache = KvCache(put(np.zeros((3, kv, bs, hd), np.int8)),
+                        put(np.zeros((3, kv, hd, bs), np.int8)),
+                        put(np.zeros((3, kv), np.float32)), put(np.zeros((3, kv), np.float32)))
+        cache.append(batch, got["k"].rows(layer), got["v"].rows(layer))
+        for name, codes, scales, shape in (("k", cache.k_codes, cache.k_scales, (3, kv, bs, hd)),
+                                           ("v", cache.v_codes, cache.v_scales, (3, kv, hd, bs))):
+            want, step = np.zeros(shape, np.int8), np.zeros((3, kv), np.float32)
+            law.append(want, step, values[name][layer].transpose(1, 0, 2).astype(np.float32), [0],
+                       [n], table, name == "v")
+            np.testing.assert_array_equal(codes.to_host(), want)
+            np.testing.assert_array_equal(scales.to_host(), step)
+    # and as a tensor, over the same memory
+    t = torch.as_tensor(got["v"], device="cuda")
+    assert t.data_ptr() == got["v"].data_ptr() and t.dtype == torch.float16
+    np.testing.assert_array_equal(t.cpu().numpy(), got["v"].to_host())
+
+
+def test_rows_are_refused_where_arrays_are_dense(hip_lib):
+    a = DeviceArray((2, 2, 16, 64), np.int8)
+    with pytest.raises(ValueError, match="contiguous"):
+        kc._dense(a.rows(0), "rows", "i8", (16, 2, 64))
+    with pytest.raises(ValueError, match="L, H, S, D"):
+        DeviceArray((3, 4)).rows(0)
+    with pytest.raises(IndexError):
+        a.rows(2)
