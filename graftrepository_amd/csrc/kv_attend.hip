@@ -184,10 +184,15 @@ static int shape_of(const grm_kv_cache_desc* c, const Layout& l, Shape* out) {
 
 // Measured with a block to a request and with runs and a join (us a call;
 // sessions x tokens):          1 x 40       16 x 250     1 x 1000     16 x 1000    1 x 2000
-//   bf16, 32 heads on 8 x 128  8.8, 11.5    8.5, 13.0    12.5, 11.9   13.8, 16.5   15.9, 11.7
-//   bf16, 12 on 4 x 64         8.4, 11.5    8.5, 12.0    8.6, 11.7    9.6, 11.4    10.5, 11.7
-//                              (16 x 2000: 14.6, 12.2)
-//   fp16, 16 on 4 x 256        8.7, 12.1    11.0, 16.3   21.1, 15.8 (1 x 500: 13.1, 15.0)
+//   bf16, 32 heads on 8 x 128  9.4, 12.0    9.5, 13.2    13.2, 12.1   14.5, 16.9   17.0, 12.2
+//   fp32, the same             9.4, 11.2    9.5, 14.5    16.9, 13.4   18.0, 19.6   26.2, 14.0
+//   bf16, 12 on 4 x 64         9.4, 11.2    9.3, 11.6    9.2, 11.5    10.2, 11.3   11.1, 11.6
+//   fp32, the same             9.3, 11.3    9.4, 11.6    11.2, 11.4   11.4, 11.4   15.9, 11.3
+//                                           1 x 500      16 x 500     1 x 1000
+//   fp16, 16 on 4 x 256        9.4, 11.6    13.1, 14.8   16.2, 17.2   20.4, 15.2
+//   fp32, 8 on 2 x 256         11.0, 13.0   16.9, 17.4   18.8, 19.8   27.4, 17.3
+// The bound is where a step of many sessions still gains; a lone one near it
+// loses 1 us in 16 bits and 3.5 in fp32.
 constexpr int kWholeTokens = 1152;  // to a block, half of it at head_dim 256
 
 template <class T, int D>
