@@ -321,6 +321,12 @@ __device__ void plan_slots(const PlanArgs& a, int t0, int* lds) {
       }
       if (a.slots) a.slots[i] = block < 0 ? -1 : static_cast<int64_t>(block) * bs + place;
       if (a.positions) a.positions[i] = pos;
+      if (i == a.tokens - 1) {
+        // The last row: blocks past it, of lengths longer than the batch has
+        // rows, are in no entry of the list.
+        reinterpret_cast<SchedHead*>(a.work)->appends =
+            min(s_touch[k] + j - (ctx >> a.block_log2) + 1, a.cap_append);
+      }
       if (place == 0 || t == 0) {
         const int at = s_touch[k] + j - (ctx >> a.block_log2);
         const int next = k + 1 < here ? s_cu[k + 1] : add(done_new, sum[0]);
@@ -371,8 +377,6 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   int* tiles = reinterpret_cast<int*>(a.work + a.at_tiles);
   int* wide_at = reinterpret_cast<int*>(a.work + a.at_scan);
   const bool wide_fits = a.requests < kWideInts;
-  int* appends = lds + 6 * 16;  // touched blocks before the batch's last row
-  if (threadIdx.x == 0) *appends = a.cap_append;
   // new tokens, blocks needed, touched blocks, narrow tiles, wide units,
   // narrow units
   int done[6] = {0, 0, 0, 0, 0, 0};
@@ -425,14 +429,6 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
           if (v[5] < kPlanChunk) tiles_lds[v[5]] = v[3];
         }
       }
-      const int left = a.tokens - v[0];
-      if (left >= 0 && l[j].fresh > left) {
-        // The request that passes the last row: blocks from the first token
-        // without one on are in no entry of the list.
-        const int bs = 1 << a.block_log2;
-        *appends = v[2] + (left ? ((l[j].ctx + left + bs - 1) >> a.block_log2) -
-                                      (l[j].ctx >> a.block_log2) : 0);
-      }
       v[0] = add(v[0], l[j].fresh);
       v[2] += l[j].touched;
       v[3] += hi[j] - lo[j];
@@ -458,13 +454,13 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
       const int left = max(0, a.free_count - at);
       *a.free_head_out = at + min(left, max(0, done[1]));
     }
+    if (done[0] < a.tokens || a.tokens == 0) head->appends = min(done[2], a.cap_append);
     head->units = done_units;
     head->narrow_tiles = done[3];
     head->items = 0;
     head->joins = 0;
   }
   __syncthreads();  // the lists are read back by other threads of this block
-  if (threadIdx.x == 0) head->appends = min(done[0] > a.tokens ? *appends : done[2], a.cap_append);
 
   // The unit that each run of the narrow kernel begins in; 0 where it is empty.
   if (a.cap_units > 0) {
@@ -488,7 +484,7 @@ __device__ void plan_schedule(const PlanArgs& a, int* lds) {
   constexpr int kCands = 8;
   const float kOf[kCands] = {1.25f, 1.125f, 1.0f, 0.625f, 0.5f, 0.4f, 1.0f / 3.0f, 0.25f};
   // Of each candidate: items, longest, shortest; then all tiles and the longest
-  // unit.  (In the place of `appends`, which the same thread has read.)
+  // unit.
   int* count = lds + 6 * 16;
   int* longest_of = count + kCands;
   int* shortest_of = longest_of + kCands;

@@ -112,3 +112,18 @@ def test_large_values_do_not_overflow_before_they_are_means(hip_lib, dtype, hd, 
     got = attend(s, q, 4, dtype)
     assert np.isfinite(got[0]).all()
     within(s, got, got[2], 4, dtype)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128, 256, 48])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_queries_that_are_not_finite(hip_lib, dtype, hd, new):
+    """They make their own row and head NaN, and no other."""
+    s = Setup([130, 20], [new, 1], 2, hd, 16, seed=hd)
+    q = s.rng.standard_normal((s.tokens, 8, hd))
+    q[0, 1, 3], q[new, 6, hd - 1], q[new // 2, 5, 0] = np.nan, np.inf, -np.inf
+    out, lse, _ = attend(s, q, 8, dtype)
+    bad = np.zeros((s.tokens, 8), bool)
+    bad[0, 1] = bad[new, 6] = bad[new // 2, 5] = True
+    np.testing.assert_array_equal(np.isnan(out).all(-1), bad)
+    np.testing.assert_array_equal(np.isnan(out).any(-1), bad)
