@@ -17,8 +17,8 @@
 // Bound by bytes where there are many: each further byte comes at 6.5 TB/s
 // (bf16, head_dim 128, blocks of 64).  Start, end and join are about 12 us of
 // a call: a step of 32 sessions of 190 to 8150 tokens (32 heads on 8, 167 MB)
-// takes 32 us here and 5 in the join; one session of 131071 tokens (268 MB) 54
-// and 5; 48 sessions of 32 to 4095 tokens at head_dim 256 (77 MB) 30 and 5.
+// takes 33 us here and 6 in the join; one session of 131071 tokens (268 MB) 54
+// and 5; 48 sessions of 32 to 4095 tokens at head_dim 256 (77 MB) 29 and 6.
 // Codes through LDS by direct loads measured 4.35 TB/s instead.
 //
 // Inside a tile both products run on the matrix cores in fp16 or bf16, where an

@@ -14,11 +14,11 @@
 // tile later than keys for that).  Two wavefronts share a SIMD.
 //
 // Bound by the vector unit and the matrix cores together.  Prompts of 333 to
-// 4100 tokens (32 heads on 8, head_dim 128, bf16, 167 GFLOP): 215 us of the
-// call's 224, 0.78 PFLOP/s; the vector unit is busy for 63 % of the cycles and
-// the matrix cores for 40 %.  A chunk of 1021 tokens on 14011 (16 heads on 4,
-// head_dim 256, fp16, 243 GFLOP and half as many again for the second term of
-// the weights): 330 us of 347; 42 % and 50 %.
+// 4100 tokens (32 heads on 8, head_dim 128, bf16, 167 GFLOP and half as many
+// again for the second term of the weights): a call of 283 us, 0.89 PFLOP/s with
+// that term; the vector unit is busy for 66 % of the cycles and the matrix cores
+// for 49 %.  A chunk of 1021 tokens on 14011 (16 heads on 4, head_dim 256, fp16,
+// 243 GFLOP and half as many again): 342 us; 41 % and 50 %.
 //
 // Layout of the products (W columns to a wavefront, lane = c + W h):
 //   S^T = K Q^T, 32 columns (32x32x16): row 8 m + 4 h' + j of a 32-key row
@@ -43,12 +43,11 @@
 namespace grm {
 namespace kv {
 
-
 // Columns of a wavefront.  32 read a tile half as often from LDS as 16; 16
 // need half the registers, and are taken where 32 would fill more than a
 // half of a SIMD's, with one wavefront that nothing covers (attend of 1021
 // tokens on 14011, head_dim 256 in fp16: 865 us with 32, 488 with 16; at
-// head_dim 128 32 columns are faster, in bf16 227 us against 317).
+// head_dim 128 32 columns are faster, four prompts in bf16 262 us against 328).
 __host__ __device__ constexpr int wide_wave_cols(int dtype, int head_dim) {
   return head_dim == 256 || (dtype == kF32 && head_dim == 128) ? 16 : 32;
 }
