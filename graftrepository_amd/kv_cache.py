@@ -158,6 +158,19 @@ def _rows(a, what: str, shape) -> tuple[int, str, int, int]:
     return a.data_ptr(), name, st[0], st[1]
 
 
+def _off(row) -> bool:
+    """Whether such rows (address, type, strides) are not 16-byte aligned."""
+    ptr, name, token, head = row
+    return bool(ptr & 15 or (token | head) & (3 if name == "f32" else 7))
+
+
+def _copied(a, stream):
+    """A torch tensor's values, contiguous, made on the stream of the call."""
+    t = sys.modules["torch"]
+    with t.cuda.stream(_torch_stream(a, _stream(a, stream))):
+        return a.clone(memory_format=t.contiguous_format)
+
+
 def _empty(like, shape, dtype: str, stream=None):
     """Memory beside ``like``.  Torch's belongs to the stream that the call
     uses, since that is where its last use is when it is freed."""
@@ -410,18 +423,28 @@ class KvCache:
         """Causal attention of the step's queries ``q`` [tokens, heads,
         head_dim] over the cache, which holds the step's own tokens.  Returns
         ``out`` (q's type; also taken as an argument), with ``return_lse``
-        also the fp32 [tokens, heads] log-sum-exp of the scores."""
+        also the fp32 [tokens, heads] log-sum-exp of the scores.  Rows of torch
+        tensors that are not 16-byte aligned are copied on the way."""
         batch._ready_for(self)
         d = batch._desc
         shape = (d.tokens, d.heads, self.head_dim)
-        qp, name, qt, qh = _rows(q, "q", shape)
+        row = _rows(q, "q", shape)
+        if _off(row) and _is_torch(q):
+            q = _copied(q, stream)
+            row = _rows(q, "q", shape)
+        qp, name, qt, qh = row
         if q.get_device() != self.device:
             _same_device(q, "q", self.device)
+        result = None   # what an output of other rows is copied from
         if out is None:
             out = _empty(q, shape, name, stream)
             op, ot, oh = out.data_ptr(), shape[1] * shape[2], shape[2]
         else:
-            op, oname, ot, oh = _rows(out, "out", shape)
+            row = _rows(out, "out", shape)
+            if _off(row) and _is_torch(out):
+                result = _copied(out, stream)   # rows that are not written stay
+                row = _rows(result, "out", shape)
+            op, oname, ot, oh = row
             if oname != name:
                 raise ValueError("out must have q's type")
             _same_device(out, "out", self.device)
@@ -447,6 +470,9 @@ class KvCache:
             batch._scratch_on(q, need, on, stream) if need else None, need, on)
         if rc:
             _lib.check(rc, "kv attend")
+        if result is not None:
+            with sys.modules["torch"].cuda.stream(_torch_stream(out, on)):
+                out.copy_(result)
         return (out, lse) if return_lse else out
 
     def read(self, block_table, starts, cu_rows, rows: int, *, dtype="f16", stream=None):

@@ -59,3 +59,26 @@ def test_rows_are_refused_where_arrays_are_dense(hip_lib):
         DeviceArray((3, 4)).rows(0)
     with pytest.raises(IndexError):
         a.rows(2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("other_stream", [False, True])
+def test_attend_takes_rows_of_any_alignment(hip_lib, dtype, other_stream):
+    """Queries and outputs inside a projection whose pieces are padded by one."""
+    from tests.test_kv_cache_gpu import Setup
+    s = Setup([100, 0], [1, 30], 2, 64, 16, extra_rows=2)
+    cache, batch = s.cache(), s.batch(4)
+    q = torch.randn(s.tokens, 4, 64, device="cuda").to(dtype)
+    want, lse = cache.attend(batch, q, return_lse=True)
+    wide = torch.full((s.tokens, 4, 2 * 64 + 3), 5.0, dtype=dtype, device="cuda")
+    wide[:, :, 1:65] = q
+    out = wide[:, :, 66:130]
+    side = torch.cuda.Stream() if other_stream else None
+    if side:
+        side.wait_stream(torch.cuda.current_stream())
+    got, lse2 = cache.attend(batch, wide[:, :, 1:65], out=out, return_lse=True, stream=side)
+    torch.cuda.synchronize()
+    n = sum(s.new)
+    assert got is out and torch.equal(out[:n], want[:n]) and torch.equal(lse[:n], lse2[:n])
+    assert (out[n:] == 5.0).all() and (wide[:, :, [0, 65, 130]] == 5.0).all()
+    assert torch.equal(wide[:, :, 1:65], q)
