@@ -12,6 +12,8 @@ surface.
   evictions and appends instead of full rebuilds
 * ``kv_cache``: the 8-bit paged key/value cache grafts are mounted into:
   block tables, quantising append, attention, dense read back
+* ``rotary``: keys and queries turned to their positions
+* ``latent``: the paged cache of models with one latent vector a token
 * ``workloads``: seeded synthetic route workloads
 """
 
@@ -19,7 +21,9 @@ from ._lib import HipRouterUnavailable, library_path, load, runtime_info
 from .node_bank import GqaNodeBank, MlaNodeBank, RouteResult
 from .bank_bridge import GqaRouteBankBridge, MlaRouteBankBridge
 from .kv_cache import KvBatch, KvCache
+from .latent import LatentCache
+from .rotary import Rotary
 
 __all__ = ["HipRouterUnavailable", "library_path", "load", "runtime_info",
            "GqaNodeBank", "MlaNodeBank", "RouteResult", "GqaRouteBankBridge",
-           "MlaRouteBankBridge", "KvBatch", "KvCache"]
+           "MlaRouteBankBridge", "KvBatch", "KvCache", "LatentCache", "Rotary"]

@@ -126,6 +126,11 @@ SIGNATURES = {
     "grm_hip_kv_attend": (i32, [vp, vp, vp, i32, i64, i64, vp, i64, i64, vp, ctypes.c_float,
                                 vp, u64, vp]),
     "grm_hip_kv_read": (i32, [vp, vp, i32, i32, vp, vp, u64, i32, vp, vp, vp]),
+    # rotary positions and the latent cache
+    "grm_hip_rotate": (i32, [vp, vp, i32, i64, i64, vp, i64, i64, vp, u64, i32, i32, i32, vp]),
+    "grm_hip_kv_append_turned": (i32, [vp, vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
+    "grm_hip_latent_append": (i32, [vp, vp, vp, vp, vp, i32, i64, i64, vp]),
+    "grm_hip_latent_read": (i32, [vp, vp, i32, i32, vp, vp, u64, i32, vp, vp]),
     "grm_hip_synth_int8_rows": (i32, [u64, u64, u64, i32, vp, i32, vp, vp]),
 }
 

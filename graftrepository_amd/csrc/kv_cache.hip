@@ -6,7 +6,7 @@
 // once, and writes a byte for each; read loads a byte per value and writes
 // two or four.
 
-#include "kv_common.hpp"
+#include "rotary.hpp"
 
 #include <mutex>
 #include <type_traits>
@@ -809,14 +809,8 @@ __device__ inline void append_values(const AppendArgs& a, const AppendWork<T>& w
 // heads x 256, keys and values, take 28 us (94 MB, 3.3 TB/s; 34.7 us with the
 // divisions themselves, so the vector unit still has its part in it).
 template <class T, int UNITS>
-__global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
+__device__ inline void append_block(const AppendArgs& a, const AppendWork<T>& work) {
   constexpr int kWords = 8 * sizeof(typename T::store) / 16;  // 16-byte pieces of 8 values
-  AppendWork<T> work;
-  if (!append_work(a, &work)) return;
-  if (work.it.count <= 2) {
-    append_values(a, work);
-    return;
-  }
   const AppendItem it = work.it;
   const int kv = blockIdx.z, bs = 1 << a.block_log2, hd = a.head_dim;
   const typename T::store* x = work.x;
@@ -962,11 +956,168 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
   if (threadIdx.x == 0) *work.scale = scale;
 }
 
+template <class T, int UNITS>
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
+  AppendWork<T> work;
+  if (!append_work(a, &work)) return;
+  if (work.it.count <= 2) append_values(a, work);
+  else append_block<T, UNITS>(a, work);
+}
+
 // Inputs whose rows are not 16-byte aligned.
 template <class T>
 __global__ __launch_bounds__(kAppendThreads) void append_any_kernel(AppendArgs a) {
   AppendWork<T> work;
   if (append_work(a, &work)) append_values(a, work);
+}
+
+// ----------------------------------------------------------- turned append
+
+// A block's keys, turned to their positions in fp32 and quantised from there:
+// a thread takes up to UNITS times eight pairs of a place (or sixteen channels
+// that are not turned), and keeps the turned values while the block's largest
+// is found.
+template <class T, int UNITS, bool ALIGNED>
+__device__ inline void append_turned(const AppendArgs& a, const Rotary& r,
+                                     const AppendWork<T>& work, int position) {
+  const AppendItem it = work.it;
+  const int hd = a.head_dim, units = hd / 16, turned = r.dim / 16, half = r.dim / 2;
+  const float before = it.place > 0 ? *work.scale : 0.0f;
+  float v[UNITS][2][8];
+  auto channels = [&](int u, int* first, int* second) {
+    if (u < turned) {
+      unit_channels(r.layout, half, u, first, second);
+    } else {
+      *first = 16 * u;
+      *second = 16 * u + 8;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k) {
+    const int i = k * kAppendThreads + static_cast<int>(threadIdx.x);
+    if (i < it.count * units) {
+      const int t = i / units;
+      int first, second;
+      channels(i - t * units, &first, &second);
+      const typename T::store* x = work.x + static_cast<int64_t>(t) * work.token_stride;
+      get8<T, ALIGNED>(x + first, v[k][0]);
+      get8<T, ALIGNED>(x + second, v[k][1]);
+    }
+  }
+  float top = 0.0f;
+  bool odd = false;  // something not finite
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k) {
+    const int i = k * kAppendThreads + static_cast<int>(threadIdx.x);
+    if (i < it.count * units) {
+      const int t = i / units, u = i - t * units;
+      if (u < turned) {
+        turn_unit(r.layout, v[k], [&](int e) { return angle(r, 8 * u + e, position + t); });
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float m = fabsf(v[k][e / 8][e % 8]);
+        odd |= !(m <= 3.4028235e38f);
+        top = fmaxf(top, m);
+      }
+    }
+  }
+  const float scale = block_step(top, odd, before);
+  if (it.place > 0 && !(scale == before)) {  // the held codes follow
+    const float ratio = scale > 0.0f ? before / scale : 0.0f;
+    uint32_t* held = reinterpret_cast<uint32_t*>(work.codes);
+    for (int i = threadIdx.x; i < it.place * hd / 4; i += kAppendThreads) {
+      held[i] = follow4(held[i], ratio);
+    }
+  }
+  const float inv = 1.0f / scale;
+  auto write_codes = [&](auto quick) {
+    constexpr bool kQuick = decltype(quick)::value;
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+      const int i = k * kAppendThreads + static_cast<int>(threadIdx.x);
+      if (i < it.count * units) {
+        const int t = i / units;
+        int at[2];
+        channels(i - t * units, &at[0], &at[1]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          u32x2 q = {0u, 0u};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            q[e / 4] |= (static_cast<uint32_t>(quantise<kQuick>(v[k][s][e], scale, inv)) & 0xffu)
+                        << (8 * (e % 4));
+          }
+          *reinterpret_cast<u32x2*>(work.codes + (it.place + t) * hd + at[s]) = q;
+        }
+      }
+    }
+  };
+  if (scale >= kQuickFrom && scale <= kQuickTo) write_codes(std::true_type{});
+  else write_codes(std::false_type{});
+  if (threadIdx.x == 0) *work.scale = scale;
+}
+
+// Any even number of turned channels: value by value, its angle made for both
+// passes.
+template <class T>
+__device__ inline void append_turned_any(const AppendArgs& a, const Rotary& r,
+                                         const AppendWork<T>& work, int position) {
+  const AppendItem it = work.it;
+  const int hd = a.head_dim, n = it.count * hd;
+  const float before = it.place > 0 ? *work.scale : 0.0f;
+  auto value = [&](int t, int d) {
+    const typename T::store* x = work.x + static_cast<int64_t>(t) * work.token_stride;
+    float v = T::get(x[d]);
+    if (d >= r.dim) return v;
+    int other;
+    const int p = pair_of(r.layout, r.dim / 2, d, &other);
+    float w = T::get(x[other]);
+    const CosSin c = angle(r, p, position + t);
+    if (d < other) turn(c, v, w);
+    else turn(c, w, v);
+    return v;
+  };
+  float top = 0.0f;
+  bool odd = false;
+  for (int i = threadIdx.x; i < n; i += kAppendThreads) {
+    const float m = fabsf(value(i / hd, i % hd));
+    odd |= !(m <= 3.4028235e38f);
+    top = fmaxf(top, m);
+  }
+  const float scale = block_step(top, odd, before);
+  if (it.place > 0 && !(scale == before)) {
+    const float ratio = scale > 0.0f ? before / scale : 0.0f;
+    uint32_t* held = reinterpret_cast<uint32_t*>(work.codes);
+    for (int i = threadIdx.x; i < it.place * hd / 4; i += kAppendThreads) {
+      held[i] = follow4(held[i], ratio);
+    }
+  }
+  for (int i = threadIdx.x; i < n; i += kAppendThreads) {
+    work.codes[it.place * hd + i] =
+        static_cast<int8_t>(quantise<false>(value(i / hd, i % hd), scale, 0.0f));
+  }
+  if (threadIdx.x == 0) *work.scale = scale;
+}
+
+// UNITS of the values' blocks; a key thread's sixteen channels are half as many.
+// 0: any dims and alignment.
+template <class T, int UNITS>
+__global__ __launch_bounds__(kAppendThreads) void append_turned_kernel(AppendArgs a, Rotary r,
+                                                                       const int32_t* positions) {
+  AppendWork<T> work;
+  if (!append_work(a, &work)) return;
+  if (blockIdx.z == 0) {
+    const int position = positions[work.it.row];
+    if constexpr (UNITS == 0) append_turned_any(a, r, work, position);
+    else if (work.it.count * a.head_dim <= 16 * kAppendThreads) append_turned<T, 1, true>(a, r, work, position);
+    else append_turned<T, 2 * UNITS, true>(a, r, work, position);
+  } else if constexpr (UNITS == 0) {
+    append_values(a, work);
+  } else {
+    if (work.it.count <= 2) append_values(a, work);
+    else append_block<T, UNITS>(a, work);
+  }
 }
 
 // ------------------------------------------------------------------- read
@@ -1166,6 +1317,22 @@ static void launch_append(const AppendArgs& a, unsigned items, bool aligned, hip
   else append_kernel<T, 4><<<grid, kAppendThreads, 0, s>>>(a);
 }
 
+template <class T>
+static void launch_append_turned(const AppendArgs& a, const Rotary& r, const int32_t* positions,
+                                 unsigned items, bool aligned, hipStream_t s) {
+  const dim3 grid(items, static_cast<unsigned>(a.kv_heads), 2);
+  const int values = a.head_dim << a.block_log2;
+  if (!aligned || !whole_units(r)) {
+    append_turned_kernel<T, 0><<<grid, kAppendThreads, 0, s>>>(a, r, positions);
+  } else if (values <= 32 * kAppendThreads) {
+    append_turned_kernel<T, 1><<<grid, kAppendThreads, 0, s>>>(a, r, positions);
+  } else if (values <= 64 * kAppendThreads) {
+    append_turned_kernel<T, 2><<<grid, kAppendThreads, 0, s>>>(a, r, positions);
+  } else {
+    append_turned_kernel<T, 4><<<grid, kAppendThreads, 0, s>>>(a, r, positions);
+  }
+}
+
 static int log2_of(int n) { return n == 16 ? 4 : n == 32 ? 5 : n == 64 ? 6 : 7; }
 
 }  // namespace kv
@@ -1234,11 +1401,14 @@ extern "C" int grm_hip_kv_plan(const grm_kv_batch_desc* b, void* stream) {
   return 0;
 }
 
-extern "C" int grm_hip_kv_append(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b,
-                                 const void* k, const void* v, int dtype, int64_t k_token_stride,
-                                 int64_t k_head_stride, int64_t v_token_stride,
-                                 int64_t v_head_stride, void* stream) {
+// Appends, with keys turned where there is a rotary.
+static int append_call(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b, bool turned,
+                       const grm_rotary_desc* rotary, const void* k, const void* v, int dtype,
+                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                       int64_t v_head_stride, void* stream) {
   GRM_CHECK_RC(check_pair(c, b, true));
+  Rotary r;
+  if (turned) GRM_CHECK_RC(rotary_of(rotary, c->head_dim, &r));
   if (dtype != grm::kF32 && dtype != grm::kBF16 && dtype != grm::kF16) {
     return grm::fail(-1, "keys and values are F32, BF16 or F16");
   }
@@ -1247,6 +1417,7 @@ extern "C" int grm_hip_kv_append(const grm_kv_cache_desc* c, const grm_kv_batch_
     return 0;
   }
   if (!k || !v) return grm::fail(-1, "null keys or values");
+  if (turned && !b->positions) return grm::fail(-1, "turned keys need the batch's positions");
   Layout l;
   GRM_CHECK_RC(layout_of(b, &l));
   if (b->work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_kv_work_bytes");
@@ -1274,12 +1445,37 @@ extern "C" int grm_hip_kv_append(const grm_kv_cache_desc* c, const grm_kv_batch_
                        v_head_stride % unit == 0;
   const auto items = static_cast<unsigned>(l.cap_append);
   const auto s = static_cast<hipStream_t>(stream);
-  if (dtype == grm::kF32) launch_append<F32>(a, items, aligned, s);
-  else if (dtype == grm::kBF16) launch_append<BF16>(a, items, aligned, s);
-  else launch_append<F16>(a, items, aligned, s);
+  if (turned) {
+    if (dtype == grm::kF32) launch_append_turned<F32>(a, r, b->positions, items, aligned, s);
+    else if (dtype == grm::kBF16) launch_append_turned<BF16>(a, r, b->positions, items, aligned, s);
+    else launch_append_turned<F16>(a, r, b->positions, items, aligned, s);
+  } else if (dtype == grm::kF32) {
+    launch_append<F32>(a, items, aligned, s);
+  } else if (dtype == grm::kBF16) {
+    launch_append<BF16>(a, items, aligned, s);
+  } else {
+    launch_append<F16>(a, items, aligned, s);
+  }
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();
   return 0;
+}
+
+extern "C" int grm_hip_kv_append(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b,
+                                 const void* k, const void* v, int dtype, int64_t k_token_stride,
+                                 int64_t k_head_stride, int64_t v_token_stride,
+                                 int64_t v_head_stride, void* stream) {
+  return append_call(c, b, false, nullptr, k, v, dtype, k_token_stride, k_head_stride,
+                     v_token_stride, v_head_stride, stream);
+}
+
+extern "C" int grm_hip_kv_append_turned(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b,
+                                        const grm_rotary_desc* rotary, const void* k,
+                                        const void* v, int dtype, int64_t k_token_stride,
+                                        int64_t k_head_stride, int64_t v_token_stride,
+                                        int64_t v_head_stride, void* stream) {
+  return append_call(c, b, true, rotary, k, v, dtype, k_token_stride, k_head_stride,
+                     v_token_stride, v_head_stride, stream);
 }
 
 extern "C" int grm_hip_kv_read(const grm_kv_cache_desc* c, const int32_t* block_table,

@@ -137,11 +137,11 @@ def _strides(a) -> tuple[int, ...]:
     return tuple(reversed(out))
 
 
-def _rows(a, what: str, shape) -> tuple[int, str, int, int]:
+def _rows(a, what: str, shape, of: str = "cache") -> tuple[int, str, int, int]:
     """(address, type, row stride, head stride) of [rows, heads, dim] values
     whose last axis is contiguous."""
     if getattr(a, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
-        raise ValueError(f"{what} requires a gradient, and the cache has no backward pass: "
+        raise ValueError(f"{what} requires a gradient, and the {of} has no backward pass: "
                          "detach it, or call under torch.no_grad()")
     if _FLOATS and _FLOATS.get(getattr(a, "dtype", None)) and a.is_cuda and a.shape == shape:
         st = a.stride()
@@ -402,9 +402,11 @@ class KvCache:
         ks = DeviceArray((blocks, kv_heads), np.float32)
         return cls(k, v, ks, DeviceArray((blocks, kv_heads), np.float32))
 
-    def append(self, batch: KvBatch, k, v, stream=None) -> None:
+    def append(self, batch: KvBatch, k, v, stream=None, *, rotary=None) -> None:
         """Quantise the step's ``k`` and ``v`` [tokens, kv_heads, head_dim]
-        (f32, bf16 or f16; any row and head strides) into their blocks."""
+        (f32, bf16 or f16; any row and head strides) into their blocks.  With a
+        ``Rotary`` the keys' first channels are turned to the batch's positions
+        on the way, without a rounding between."""
         batch._ready_for(self)
         shape = (batch._desc.tokens, self.kv_heads, self.head_dim)
         kp, name, kt, kh = _rows(k, "k", shape)
@@ -413,8 +415,13 @@ class KvCache:
             raise ValueError("k and v must have one type")
         _same_device(k, "k", self.device)
         _same_device(v, "v", self.device)
-        rc = _call(self._lib.grm_hip_kv_append, k, self.device, self._ref, batch._ref, kp, vptr,
-                   _lib.DTYPE_CODES[name], kt, kh, vt, vh, batch._on(k, stream))
+        if rotary is None:
+            rc = _call(self._lib.grm_hip_kv_append, k, self.device, self._ref, batch._ref, kp,
+                       vptr, _lib.DTYPE_CODES[name], kt, kh, vt, vh, batch._on(k, stream))
+        else:
+            rc = _call(self._lib.grm_hip_kv_append_turned, k, self.device, self._ref, batch._ref,
+                       rotary._ref, kp, vptr, _lib.DTYPE_CODES[name], kt, kh, vt, vh,
+                       batch._on(k, stream))
         if rc:
             _lib.check(rc, "kv append")
 

@@ -1,0 +1,140 @@
+"""A paged cache of latent vectors, for models whose keys and values come from
+one (the MLA dialect's).
+
+A row holds a token's latent and its turned key part, shared by all heads::
+
+    batch = KvBatch(..., heads=40, kv_heads=1)
+    batch.plan()                                       # once per step
+    cache.append(batch, latent, key_part, rotary=rotary)   # per layer
+    rows = cache.read(table, starts, cu_rows, rows)        # dense, to harvest
+
+Batches, memory, streams and errors are those of ``kv_cache``; laws and layouts
+those of ``include/grm_hip_router.h``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+from . import _lib
+from .kv_cache import (KvBatch, _call, _dense, _empty, _name_of, _one_device, _rows,
+                       _same_device, _stream, _type, i32, u64, vp)
+from .payload import DeviceArray
+
+
+class _LatentDesc(ctypes.Structure):
+    _fields_ = [("rows", vp), ("blocks", u64), ("block_tokens", i32), ("rank", i32),
+                ("rope", i32), ("dtype", i32)]
+
+
+def _flat(a, what: str, tokens: int, values: int):
+    """(address, type, row stride) of [tokens, values] rows."""
+    if len(a.shape) != 2:
+        raise ValueError(f"{what} must have shape {(tokens, values)}, got {tuple(a.shape)}")
+    if isinstance(a, DeviceArray):
+        name = _type(a, what)
+        if name not in ("f32", "bf16", "f16"):
+            raise ValueError(f"{what} must be f32, bf16 or f16, got {a.dtype}")
+        if tuple(a.shape) != (tokens, values):
+            raise ValueError(f"{what} must have shape {(tokens, values)}, got {tuple(a.shape)}")
+        return a.data_ptr(), name, values
+    if not hasattr(a, "unsqueeze"):
+        _type(a, what)
+    ptr, name, stride, _ = _rows(a.unsqueeze(1), what, (tokens, 1, values))
+    return ptr, name, stride
+
+
+class LatentCache:
+    """The latent cache of one layer, over the caller's ``rows`` [blocks,
+    block_tokens, rank + rope] (bf16 or f16), of which ``rank`` values are the
+    latent and the rest the key part.  ``LatentCache.empty`` allocates them."""
+
+    def __init__(self, rows, rank: int):
+        self._lib = _lib.load()
+        if len(rows.shape) != 3:
+            raise ValueError("rows must be [blocks, block_tokens, rank + rope]")
+        blocks, bs, values = (int(n) for n in rows.shape)
+        rank = int(rank)
+        name = _type(rows, "rows")
+        if name not in ("bf16", "f16"):
+            raise ValueError(f"rows must be bf16 or f16, got {rows.dtype}")
+        d = self._desc = _LatentDesc()
+        d.rows = _dense(rows, "rows", name, (blocks, bs, values))
+        if bs not in (16, 32, 64, 128):
+            raise ValueError("block_tokens must be 16, 32, 64 or 128")
+        if rank % 16 or not 0 < rank <= 512:
+            raise ValueError("rank must be a multiple of 16, at most 512")
+        rope = values - rank
+        if rope % 16 or not 0 <= rope <= 128:
+            raise ValueError("rope must be a multiple of 16, at most 128")
+        self.device = _one_device(rows=rows)
+        d.blocks, d.block_tokens, d.rank, d.rope = blocks, bs, rank, rope
+        d.dtype = _lib.DTYPE_CODES[name]
+        self.rows, self.dtype = rows, name
+        self.blocks, self.block_tokens, self.rank, self.rope = blocks, bs, rank, rope
+        self._ref = ctypes.byref(d)
+
+    @classmethod
+    def empty(cls, blocks: int, block_tokens: int, rank: int, rope: int,
+              dtype: str = "f16") -> "LatentCache":
+        """A cache in memory of its own (a DeviceArray), contents undefined:
+        every row is written before it is read."""
+        from .kv_cache import _NUMPY
+        if dtype not in ("bf16", "f16"):
+            raise ValueError("rows are bf16 or f16")
+        return cls(DeviceArray((blocks, block_tokens, rank + rope), _NUMPY[dtype]), rank)
+
+    def append(self, batch: KvBatch, latent, key_part=None, stream=None, *, rotary=None) -> None:
+        """The step's ``latent`` [tokens, rank] and ``key_part`` [tokens, rope]
+        (f32, bf16 or f16, of one type; any row strides) into their rows,
+        rounded once; with a ``Rotary`` the key part's first channels are turned
+        to the batch's positions on the way."""
+        batch._ready_for(self)
+        tokens = batch._desc.tokens
+        lp, name, lt = _flat(latent, "latent", tokens, self.rank)
+        kp, kt = None, 0
+        if self.rope:
+            if key_part is None:
+                raise ValueError("the cache's rows have a key part")
+            kp, kname, kt = _flat(key_part, "key_part", tokens, self.rope)
+            if kname != name:
+                raise ValueError("latent and key_part must have one type")
+            _same_device(key_part, "key_part", self.device)
+        elif key_part is not None or rotary is not None:
+            raise ValueError("the cache's rows have no key part")
+        _same_device(latent, "latent", self.device)
+        rc = _call(self._lib.grm_hip_latent_append, latent, self.device, self._ref, batch._ref,
+                   rotary._ref if rotary is not None else None, lp, kp, _lib.DTYPE_CODES[name], lt,
+                   kt, batch._on(latent, stream))
+        if rc:
+            _lib.check(rc, "latent append")
+
+    def _ranges(self, block_table, starts, cu_rows, rows):
+        n = int(starts.shape[0])
+        table = _dense(block_table, "block_table", "i32", (n, block_table.shape[1]))
+        sp = _dense(starts, "starts", "i32", (n,))
+        cp = _dense(cu_rows, "cu_rows", "i32", (n + 1,))
+        for a, what in ((block_table, "block_table"), (starts, "starts"), (cu_rows, "cu_rows")):
+            _same_device(a, what, self.device)
+        if not 0 <= int(rows) < 1 << 31:
+            raise ValueError(f"rows must be 0 or more and fit 32 bits, got {rows}")
+        return table, int(block_table.shape[1]), n, sp, cp, int(rows)
+
+    def read(self, block_table, starts, cu_rows, rows: int, *, dtype=None, stream=None):
+        """Dense rows [rows, rank + rope] of positions ``starts[r]`` onward of
+        every request, ``cu_rows[r + 1] - cu_rows[r]`` of them; ``rows`` is
+        ``cu_rows[-1]``.  In the cache's type unless told.  A deposit harvests a
+        turn with it."""
+        name = self.dtype if dtype is None else _name_of(dtype)
+        if name not in ("f32", "bf16", "f16"):
+            raise ValueError("rows are read as f32, bf16 or f16")
+        at = self._ranges(block_table, starts, cu_rows, rows)
+        out = _empty(starts, (at[5], self.rank + self.rope), name, stream)
+        rc = _call(self._lib.grm_hip_latent_read, starts, self.device, self._ref, *at,
+                   _lib.DTYPE_CODES[name], out.data_ptr(), _stream(starts, stream))
+        if rc:
+            _lib.check(rc, "latent read")
+        return out
+
+
+__all__ = ["LatentCache"]

@@ -611,6 +611,77 @@ int grm_hip_kv_read(const grm_kv_cache_desc* cache, const int32_t* block_table,
                     const int32_t* cu_rows, uint64_t rows, int dtype, void* k_out, void* v_out,
                     void* stream);
 
+/* ---- Rotary positions --------------------------------------------------------
+ * A pair (a, b) of channels at position p is turned to
+ *   (a cos t - b sin t, b cos t + a sin t) * magnitude,  t = 2 pi p turns[pair]
+ * in fp32, the angle made in fp64: no position is too far.  The pairs of
+ * `dim` channels are (i, i + dim / 2) or, with layout 1, (2 i, 2 i + 1).
+ * `inverse` undoes it (turns back and divides by magnitude).  The reference
+ * leaves rotations to its external engine; no counterpart.  The descriptor is
+ * host memory, read during the call. */
+typedef struct grm_rotary_desc {
+  double turns[128]; /* of each pair: whole turns that a position adds, at most 1 */
+  float magnitude;   /* positive */
+  int32_t dim;       /* even, at most 256 */
+  int32_t layout;    /* 0: halves, 1: neighbours */
+  int32_t inverse;
+} grm_rotary_desc;
+
+/* x [tokens][heads][head_dim] of dtype (F32, BF16, F16; strides in elements)
+ * to out of the same type: channels [start, start + dim) of every head turned
+ * to positions[token], the others copied.  out may be x with the same strides
+ * (other overlaps are not defined).  Rows whose position is below 0 belong to
+ * no token and are not written.  Streams and errors as below. */
+int grm_hip_rotate(const grm_rotary_desc* rotary, const void* x, int dtype,
+                   int64_t x_token_stride, int64_t x_head_stride, void* out,
+                   int64_t out_token_stride, int64_t out_head_stride, const int32_t* positions,
+                   uint64_t tokens, int heads, int head_dim, int start, void* stream);
+
+/* grm_hip_kv_append with the keys' first `dim` channels turned to the batch's
+ * positions (which must not be NULL) on the way: fp32 from the stored value to
+ * the code, one rounding. */
+int grm_hip_kv_append_turned(const grm_kv_cache_desc* cache, const grm_kv_batch_desc* batch,
+                             const grm_rotary_desc* rotary, const void* k, const void* v,
+                             int dtype, int64_t k_token_stride, int64_t k_head_stride,
+                             int64_t v_token_stride, int64_t v_head_stride, void* stream);
+
+/* ---- Latent cache ------------------------------------------------------------
+ * A paged cache of models whose keys and values come from one latent vector a
+ * token (the MLA dialect's): a row is [latent (rank) | turned key part (rope)],
+ * 16 bits a value, shared by all heads.  rows [blocks][block_tokens][rank +
+ * rope] of dtype (BF16, F16), 16-byte aligned; rank a multiple of 16, at most
+ * 512; rope a multiple of 16, at most 128 (0 is fine).  Batches are the 8-bit
+ * cache's, with kv_heads 1; so are streams, lifetimes and errors.  The
+ * reference keeps latents in a dense cache (core/graft_arena.py:2408-2622) and
+ * leaves attention to its engine; no counterpart.
+ *
+ * A row with a value that is not finite makes the outputs of every token that
+ * sees it NaN, and no other's.  Rows that no token sees may hold anything. */
+typedef struct grm_latent_desc {
+  void* rows;
+  uint64_t blocks;
+  int32_t block_tokens;
+  int32_t rank;
+  int32_t rope;
+  int32_t dtype;
+} grm_latent_desc;
+
+/* A step's latents [tokens][rank] and key parts [tokens][rope] (NULL where
+ * rope is 0) of dtype (F32, BF16, F16; strides in elements) to the batch's
+ * slots, rounded once; with a rotary (may be NULL; its dim a multiple of 16)
+ * the key parts' first channels are turned to the batch's positions. */
+int grm_hip_latent_append(const grm_latent_desc* cache, const grm_kv_batch_desc* batch,
+                          const grm_rotary_desc* rotary, const void* latents, const void* keys,
+                          int dtype, int64_t latent_token_stride, int64_t key_token_stride,
+                          void* stream);
+
+/* Rows of positions [starts[r], starts[r] + cu_rows[r + 1] - cu_rows[r]) of each
+ * request, dense: out [rows][rank + rope] of dtype, contiguous, 16-byte aligned.
+ * Positions without a block read as 0. */
+int grm_hip_latent_read(const grm_latent_desc* cache, const int32_t* block_table,
+                        int table_width, int requests, const int32_t* starts,
+                        const int32_t* cu_rows, uint64_t rows, int dtype, void* out, void* stream);
+
 /* ---- Synthetic workload keys (host only) --------------------------------
  * Rows [row0, row0 + rows) of the synthetic INT8 key stream: each row's dim
  * values are normal quantiles (normal_table[65536], the caller's table of
