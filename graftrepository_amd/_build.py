@@ -50,8 +50,11 @@ def sources() -> list[Path]:
 
 # Per-source flags.  The MLA screens: MFMA accumulators in VGPRs (the ring
 # screen keeps its query fragments in AGPRs and reduces the accumulators
-# with VALU instructions, which then need no AGPR-to-VGPR copies).
+# with VALU instructions, which then need no AGPR-to-VGPR copies).  So has
+# latent attention its queries; without, its scores share the AGPRs with its
+# sums, and spill.
 SOURCE_FLAGS = {
+    "latent_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mla_route.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mla_screen_probe.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }

@@ -131,6 +131,11 @@ SIGNATURES = {
     "grm_hip_kv_append_turned": (i32, [vp, vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
     "grm_hip_latent_append": (i32, [vp, vp, vp, vp, vp, i32, i64, i64, vp]),
     "grm_hip_latent_read": (i32, [vp, vp, i32, i32, vp, vp, u64, i32, vp, vp]),
+    "grm_hip_latent_work_bytes": (i32, [vp, vp]),
+    "grm_hip_latent_plan": (i32, [vp, vp, u64, vp]),
+    "grm_hip_latent_attend_bytes": (i32, [vp, vp, vp]),
+    "grm_hip_latent_attend": (i32, [vp, vp, vp, u64, vp, i64, i64, vp, i64, i64, vp,
+                                    ctypes.c_float, vp, u64, vp]),
     "grm_hip_synth_int8_rows": (i32, [u64, u64, u64, i32, vp, i32, vp, vp]),
 }
 

@@ -1,0 +1,461 @@
+// latent_attend.hip -- the latent schedule of a step, and absorbed attention over
+// the latent cache (see latent_attend.hpp).
+#include "latent_attend.hpp"
+
+namespace grm {
+namespace kv {
+
+int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
+  LatentLayout l{};
+  int cus = 0;
+  GRM_CHECK_RC(device_cus(&cus));
+  const uint64_t rows = static_cast<uint64_t>(b->tokens);
+  const uint64_t reqs = static_cast<uint64_t>(b->requests);
+  const uint64_t busy = std::min(rows, reqs);
+  const int64_t most = static_cast<int64_t>(std::max(1, b->max_new)) * b->heads;
+  l.cols = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : kLatentCols;
+  l.unit_tokens = std::max(1, l.cols / b->heads);
+  l.runs = 2 * cus;  // at most
+  l.cap_units = rows / l.unit_tokens + busy;
+  l.cap_rows = rows / kRowUnit + busy;
+  l.reach = static_cast<int32_t>(std::min<int64_t>(
+      static_cast<int64_t>(b->table_width) * b->block_tokens, 2 * static_cast<int64_t>(kMaxLen)));
+  auto place = [&l](uint64_t bytes) {
+    const uint64_t at = l.bytes;
+    l.bytes += (bytes + 63) / 64 * 64;
+    return at;
+  };
+  place(sizeof(LatentHead));
+  l.at_units = place(l.cap_units * sizeof(LatentUnit));
+  l.at_first = place((l.cap_units + 1) * 8);
+  l.at_runs = place(2 * static_cast<uint64_t>(l.runs) * 4);
+  l.at_unit_scan = place((reqs + 1) * 4);
+  l.at_row_scan = place((reqs + 1) * 4);
+  l.at_rows = place(l.cap_rows * sizeof(RowUnit));
+  *out = l;
+  return 0;
+}
+
+// ------------------------------------------------------------------- plan
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+
+struct LatentPlanArgs {
+  const int32_t* ctx_lens;
+  const int32_t* new_lens;
+  const int32_t* cu_new;
+  char* work;
+  int32_t requests, tokens, window, reach, unit_tokens, cap_units, cap_rows;
+  int32_t runs[2];
+  uint64_t at_units, at_first, at_runs, at_unit_scan, at_row_scan, at_rows;
+};
+
+// Exclusive sum over the block; the total in *sum.  Two barriers.
+template <class N>
+__device__ inline N block_sum(N v, N* sum, N* scratch) {
+  const int lane = __lane_id(), wave = threadIdx.x / kWave;
+  const N own = v;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const N o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == kWave - 1) scratch[wave] = v;
+  __syncthreads();
+  N before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    const N t = scratch[w];
+    before += w < wave ? t : 0;
+    all += t;
+  }
+  __syncthreads();
+  *sum = all;
+  return v - own + before;
+}
+
+// Largest i in [0, n) with pre[i] <= x.
+template <class N>
+__device__ inline int last_of(const N* pre, int n, N x) {
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int half = len >> 1;
+    if (pre[lo + half] <= x) lo += half;
+    len -= half;
+  }
+  return lo;
+}
+
+// One block, beside nothing: latency (a scan over the requests, one over the
+// units, a search for each run).
+__global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArgs a) {
+  __shared__ int64_t scratch[kPlanWaves];
+  constexpr int kHeld = 4096;  // requests whose sums stay in LDS
+  __shared__ int s_units[kHeld + 1];
+  __shared__ int s_rows[kHeld + 1];
+  const int tid = threadIdx.x;
+  const bool held = a.requests <= kHeld;
+  int* unit_at = held ? s_units : reinterpret_cast<int*>(a.work + a.at_unit_scan);
+  int* row_at = held ? s_rows : reinterpret_cast<int*>(a.work + a.at_row_scan);
+  auto* head = reinterpret_cast<LatentHead*>(a.work);
+  auto* units = reinterpret_cast<LatentUnit*>(a.work + a.at_units);
+  auto* firsts = reinterpret_cast<int64_t*>(a.work + a.at_first);
+  auto* row_units = reinterpret_cast<RowUnit*>(a.work + a.at_rows);
+
+  // units and row units before each request; sums past an int end at the lists'
+  // ends, which are never that long
+  int64_t units_all = 0, rows_all = 0;
+  for (int base = 0; base < a.requests; base += kPlanThreads) {
+    const int r = base + tid;
+    const int fresh = r < a.requests ? clamp_len(a.new_lens[r]) : 0;
+    int64_t sum;
+    int64_t v = block_sum<int64_t>((fresh + a.unit_tokens - 1) / a.unit_tokens, &sum, scratch);
+    if (r < a.requests) unit_at[r] = static_cast<int>(min(units_all + v, static_cast<int64_t>(0x7fffffff)));
+    units_all += sum;
+    v = block_sum<int64_t>((fresh + kRowUnit - 1) / kRowUnit, &sum, scratch);
+    if (r < a.requests) row_at[r] = static_cast<int>(min(rows_all + v, static_cast<int64_t>(0x7fffffff)));
+    rows_all += sum;
+  }
+  const int n_units = static_cast<int>(min(units_all, static_cast<int64_t>(a.cap_units)));
+  const int n_rows = static_cast<int>(min(rows_all, static_cast<int64_t>(a.cap_rows)));
+  __syncthreads();
+
+  // Unit i's first token within its request, its rows and how many: those past
+  // the batch's rows are none.
+  auto unit_of = [&](const int* at, int i, int each, auto* u) {
+    u->request = last_of(at, a.requests, i);
+    const int t0 = (i - at[u->request]) * each;
+    const int fresh = clamp_len(a.new_lens[u->request]);
+    u->pos = clamp_len(a.ctx_lens[u->request]) + t0;
+    const int64_t row = static_cast<int64_t>(a.cu_new[u->request]) + t0;
+    u->row = static_cast<int>(min(row, static_cast<int64_t>(a.tokens)));
+    u->tokens = max(0, min(min(each, fresh - t0), a.tokens - u->row));
+  };
+  int64_t tiles = 0;
+  for (int base = 0; base < n_units; base += kPlanThreads) {
+    const int i = base + tid;
+    int64_t mine = 0, sum;
+    LatentUnit u{};
+    if (i < n_units) {
+      unit_of(unit_at, i, a.unit_tokens, &u);
+      const int first = a.window > 0 ? max(0, u.pos + 1 - a.window) : 0;
+      u.tile_lo = first / kLatentTile;
+      const int hi = (min(u.pos + u.tokens, a.reach) + kLatentTile - 1) / kLatentTile;
+      mine = max(1, hi - u.tile_lo);
+    }
+    const int64_t v = block_sum<int64_t>(mine, &sum, scratch);
+    if (i < n_units) {
+      units[i] = u;
+      firsts[i] = tiles + v;
+    }
+    tiles += sum;
+  }
+  for (int i = tid; i < n_rows; i += kPlanThreads) {
+    RowUnit u;
+    unit_of(row_at, i, kRowUnit, &u);
+    row_units[i] = u;
+  }
+  if (tid == 0) {
+    firsts[n_units] = tiles;
+    head->tiles = tiles;
+    head->units = n_units;
+    head->row_units = n_rows;
+  }
+  __syncthreads();  // the lists are read back by other threads of this block
+  // The unit that each run begins in.
+  for (int k = 0; k < 2; ++k) {
+    const LongDeal deal(tiles, a.runs[k]);
+    int* to = reinterpret_cast<int*>(a.work + a.at_runs) + k * a.runs[1];
+    for (int r = tid; r < a.runs[k]; r += kPlanThreads) {
+      to[r] = r < deal.used ? last_of(firsts, n_units, deal.begin(r)) : 0;
+    }
+  }
+}
+
+// ------------------------------------------------------- any shape of row
+
+// One block to a (token, head): each of its wavefronts takes 64 rows in turn, a row
+// to a lane for the scores and eight columns to a lane for the values.  Rows are
+// read once for each head.
+template <class T>
+__global__ __launch_bounds__(256) void latent_any_kernel(LatentArgs a) {
+  const int row = blockIdx.x, h = blockIdx.y;
+  const int lane = __lane_id(), wave = threadIdx.x / kWave;
+  const int values = a.rank + a.rope, bs = 1 << a.block_log2;
+  __shared__ float s_q[640];
+  __shared__ float s_p[4][kWave];
+  __shared__ int64_t s_row[4][kWave];
+  __shared__ float s_o[4][512];
+  __shared__ float s_m[4], s_l[4];
+  if (row >= a.cu_new[a.requests]) return;
+  const int r = last_not_past(a.cu_new, a.requests, row);
+  const int pos = clamp_len(a.ctx_lens[r]) + row - a.cu_new[r];
+  const int first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+  const auto* q = static_cast<const typename T::store*>(a.q) + static_cast<int64_t>(row) * a.q_token +
+                  static_cast<int64_t>(h) * a.q_head;
+  for (int d = threadIdx.x; d < values; d += 256) s_q[d] = T::get(q[d]);
+  __syncthreads();
+  const auto* rows = reinterpret_cast<const typename T::store*>(a.rows);
+  float m = -INFINITY, l = 0.0f, o[8] = {};
+  const int reach = static_cast<int>(min(static_cast<int64_t>(pos), (static_cast<int64_t>(a.width) << a.block_log2) - 1));
+  for (int t0 = first / kWave * kWave + wave * kWave; t0 <= reach; t0 += 4 * kWave) {
+    const int key = t0 + lane;
+    int64_t at = -1;
+    if (key >= first && key <= reach) {
+      const int block = a.table[static_cast<size_t>(r) * a.width + (key >> a.block_log2)];
+      if (static_cast<uint64_t>(static_cast<int64_t>(block)) < a.blocks) {
+        at = (static_cast<int64_t>(block) << a.block_log2) + (key & (bs - 1));
+      }
+    }
+    float s = -INFINITY;
+    if (at >= 0) {
+      float dot = 0.0f;
+      for (int d = 0; d < values; d += 8) {
+        float x[8];
+        get8<T, true>(rows + at * values + d, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(s_q[d + e], x[e], dot);
+      }
+      s = dot * a.scale * kLog2e;
+      if (!(fabsf(dot) <= 3.4028235e38f)) s = NAN;
+    }
+    float top = s;
+    const bool odd = __any(s != s);
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float m2 = fmaxf(m, top);
+    if (odd) l = NAN;
+    if (m2 == -INFINITY) continue;
+    const float keep = __builtin_amdgcn_exp2f(m - m2);
+    m = m2;
+    const float p = at >= 0 && s == s ? __builtin_amdgcn_exp2f(s - m2) : 0.0f;
+    float sum = p;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    l = l * keep + sum;
+    s_p[wave][lane] = p;
+    s_row[wave][lane] = s == s ? at : -1;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= keep;
+    if (8 * lane < a.rank) {
+      for (int k = 0; k < kWave; ++k) {
+        const int64_t from = s_row[wave][k];
+        if (from < 0) continue;
+        const float w = s_p[wave][k];
+        float x[8];
+        get8<T, true>(rows + from * values + 8 * lane, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(w, x[e], o[e]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (8 * lane < a.rank) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_o[wave][8 * lane + e] = o[e];
+  }
+  if (lane == 0) {
+    s_m[wave] = m;
+    s_l[wave] = l;
+  }
+  __syncthreads();
+  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  float total = 0.0f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = s_m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w] - top);
+    total += s_l[w] != s_l[w] ? NAN : f[w] * s_l[w];
+  }
+  auto* out = static_cast<typename T::store*>(a.out) + static_cast<int64_t>(row) * a.out_token +
+              static_cast<int64_t>(h) * a.out_head;
+  for (int d = threadIdx.x; d < a.rank; d += 256) {
+    const float v = f[0] * s_o[0][d] + f[1] * s_o[1][d] + f[2] * s_o[2][d] + f[3] * s_o[3][d];
+    out[d] = T::put(total == 0.0f ? 0.0f : v / total);
+  }
+  if (a.lse && threadIdx.x == 0) {
+    a.lse[static_cast<size_t>(row) * a.heads + h] =
+        total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  }
+}
+
+// ------------------------------------------------------------- dispatch
+
+// The matrix cores' shapes: (rank, rope) of (512, 64) and (256, 32), up to 128
+// heads.
+static bool latent_cores(const grm_latent_desc* c, const grm_kv_batch_desc* b) {
+  return b->heads <= kLatentCols &&
+         ((c->rank == 512 && c->rope == 64) || (c->rank == 256 && c->rope == 32));
+}
+
+// Blocks to a CU: what the ring's LDS allows.
+static int latent_per_cu(int rank) { return rank == 512 ? 1 : 2; }
+
+template <class T, int R, int P, int W, int G>
+static void launch_cols(LatentArgs a, hipStream_t stream) {
+  constexpr int kCols = LatentShape<T, R, P, W, G>::kCols;
+  latent_attend_kernel<T, R, P, W, G><<<static_cast<unsigned>(a.runs), 256, 0, stream>>>(a);
+  // real columns of a unit: whole tokens'
+  const int cols = std::max(1, kCols / a.heads) * a.heads;
+  constexpr int kEach = 256 / (R / 4);
+  const dim3 grid(static_cast<unsigned>(a.runs - 1), static_cast<unsigned>((cols + kEach - 1) / kEach));
+  if (a.runs > 1) {
+    latent_join_kernel<T, R, kCols><<<grid, 256, 0, stream>>>(a, LatentShape<T, R, P, W, G>::kBias);
+  }
+}
+
+template <class T, int R, int P>
+static void launch_latent(const LatentArgs& a, int cols, hipStream_t stream) {
+  if (cols == 16) launch_cols<T, R, P, 16, 4>(a, stream);
+  else if (cols == 32) launch_cols<T, R, P, 32, 4>(a, stream);
+  else if (cols == 64) launch_cols<T, R, P, 32, 2>(a, stream);
+  else launch_cols<T, R, P, 32, 1>(a, stream);
+}
+
+template <class T>
+static void launch_latent_any(const LatentArgs& a, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads));
+  latent_any_kernel<T><<<grid, 256, 0, stream>>>(a);
+}
+
+}  // namespace kv
+}  // namespace grm
+
+using namespace grm::kv;
+
+extern "C" int grm_hip_latent_work_bytes(const grm_kv_batch_desc* batch, uint64_t* out_bytes) {
+  if (!out_bytes) return grm::fail(-1, "null output pointer");
+  GRM_CHECK_RC(check_batch(batch, false));
+  LatentLayout l;
+  GRM_CHECK_RC(latent_layout_of(batch, &l));
+  *out_bytes = l.bytes;
+  grm::clear_error();
+  return 0;
+}
+
+extern "C" int grm_hip_latent_plan(const grm_kv_batch_desc* b, void* work, uint64_t work_bytes,
+                                   void* stream) {
+  GRM_CHECK_RC(check_batch(b, true));
+  if (b->requests == 0) {
+    grm::clear_error();
+    return 0;
+  }
+  if (!work || !aligned16(work)) return grm::fail(-1, "latent work must be 16-byte aligned");
+  LatentLayout l;
+  GRM_CHECK_RC(latent_layout_of(b, &l));
+  if (work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_latent_work_bytes");
+  LatentPlanArgs a{};
+  a.ctx_lens = b->ctx_lens;
+  a.new_lens = b->new_lens;
+  a.cu_new = b->cu_new;
+  a.work = static_cast<char*>(work);
+  a.requests = b->requests;
+  a.tokens = b->tokens;
+  a.window = b->window;
+  a.reach = l.reach;
+  a.unit_tokens = l.unit_tokens;
+  a.cap_units = static_cast<int32_t>(l.cap_units);
+  a.cap_rows = static_cast<int32_t>(l.cap_rows);
+  a.runs[0] = l.runs / 2;
+  a.runs[1] = l.runs;
+  a.at_units = l.at_units;
+  a.at_first = l.at_first;
+  a.at_runs = l.at_runs;
+  a.at_unit_scan = l.at_unit_scan;
+  a.at_row_scan = l.at_row_scan;
+  a.at_rows = l.at_rows;
+  latent_plan_kernel<<<1, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  GRM_HIP_CHECK(hipGetLastError());
+  grm::clear_error();
+  return 0;
+}
+
+extern "C" int grm_hip_latent_attend_bytes(const grm_latent_desc* c, const grm_kv_batch_desc* b,
+                                           uint64_t* out_bytes) {
+  if (!out_bytes) return grm::fail(-1, "null output pointer");
+  GRM_CHECK_RC(check_latent_pair(c, b, false));
+  LatentLayout l;
+  GRM_CHECK_RC(latent_layout_of(b, &l));
+  *out_bytes = latent_cores(c, b) ? static_cast<uint64_t>(l.runs / 2 * latent_per_cu(c->rank)) * 2 *
+                                        latent_part_floats(l.cols, c->rank) * 4
+                                  : 0;
+  grm::clear_error();
+  return 0;
+}
+
+extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batch_desc* b,
+                                     const void* work, uint64_t work_bytes, const void* q,
+                                     int64_t q_token_stride, int64_t q_head_stride, void* out,
+                                     int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                                     float softmax_scale, void* scratch, uint64_t scratch_bytes,
+                                     void* stream) {
+  GRM_CHECK_RC(check_latent_pair(c, b, true));
+  if (!(softmax_scale - softmax_scale == 0.0f)) return grm::fail(-1, "softmax_scale must be finite");
+  if (b->requests == 0 || b->tokens == 0) {
+    grm::clear_error();
+    return 0;
+  }
+  if (!q || !out) return grm::fail(-1, "null queries or output");
+  if (!aligned16(q) || !aligned16(out) ||
+      (q_token_stride | q_head_stride | out_token_stride | out_head_stride) % 8 != 0) {
+    return grm::fail(-1, "queries and output: 16-byte aligned rows");
+  }
+  const bool cores = latent_cores(c, b);
+  const int per = latent_per_cu(c->rank);
+  if (cores && (!work || !aligned16(work))) {
+    return grm::fail(-1, "latent work must be 16-byte aligned");
+  }
+  LatentLayout l;
+  GRM_CHECK_RC(latent_layout_of(b, &l));
+  if (cores) {
+    if (work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_latent_work_bytes");
+    const uint64_t need = static_cast<uint64_t>(l.runs / 2 * per) * 2 * latent_part_floats(l.cols, c->rank) * 4;
+    if (!scratch || !aligned16(scratch) || scratch_bytes < need) {
+      return grm::fail(-1, "scratch is smaller than grm_hip_latent_attend_bytes, or not 16-byte aligned");
+    }
+  }
+  LatentArgs a{};
+  a.rows = static_cast<const char*>(c->rows);
+  a.q = q;
+  a.out = out;
+  a.lse = lse;
+  a.cu_new = b->cu_new;
+  a.ctx_lens = b->ctx_lens;
+  a.table = b->table_width ? b->block_table : b->cu_new;  // entry 0 is asked for all the same
+  a.work = static_cast<const char*>(work);
+  a.parts = static_cast<float*>(scratch);
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.out_token = out_token_stride;
+  a.out_head = out_head_stride;
+  a.blocks = c->blocks;
+  a.at_units = l.at_units;
+  a.at_first = l.at_first;
+  a.at_runs = l.at_runs + (per == 2 ? static_cast<uint64_t>(l.runs) * 4 : 0);
+  a.scale = softmax_scale;
+  a.requests = b->requests;
+  a.width = b->table_width;
+  a.tokens = b->tokens;
+  a.window = b->window;
+  a.heads = b->heads;
+  a.rank = c->rank;
+  a.rope = c->rope;
+  a.block_log2 = block_log2(c->block_tokens);
+  a.runs = l.runs / 2 * per;
+  const auto s = static_cast<hipStream_t>(stream);
+  const bool bf = c->dtype == grm::kBF16;
+  if (!cores) {
+    if (bf) launch_latent_any<BF16>(a, s);
+    else launch_latent_any<F16>(a, s);
+  } else if (c->rank == 512) {
+    if (bf) launch_latent<BF16, 512, 64>(a, l.cols, s);
+    else launch_latent<F16, 512, 64>(a, l.cols, s);
+  } else {
+    if (bf) launch_latent<BF16, 256, 32>(a, l.cols, s);
+    else launch_latent<F16, 256, 32>(a, l.cols, s);
+  }
+  GRM_HIP_CHECK(hipGetLastError());
+  grm::clear_error();
+  return 0;
+}

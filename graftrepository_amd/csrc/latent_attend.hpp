@@ -1,0 +1,718 @@
+// latent_attend.hpp -- absorbed attention over the latent cache: a token's row is
+// every head's key, and its first `rank` values every head's value.
+//
+//   s_j = scale * (q . row_j),  o = sum_j p_j row_j[:rank] / sum_j p_j,
+//   p_j = exp(s_j - max s)
+//
+// A unit is the columns (token, head) of some neighbouring tokens of a request,
+// at most 128; all of a step's (unit, tile of 32 rows) pairs are dealt to blocks
+// in equal runs (`latent_plan_kernel`).  A unit that a run's end cuts leaves parts
+// in scratch, which a second launch joins in order: results do not depend on
+// timing.
+//
+// A block's four wavefronts hold their columns' queries and sums in registers: a
+// row is read from memory once for all heads.  With few columns (16, 32, 64)
+// wavefronts take several tiles at once, G of them, and are joined through LDS at
+// the unit's end.
+//
+// Rows go to LDS by direct loads (no registers), a ring of four tiles, and are
+// read from there twice: as the first product's operand 16 bytes to a lane, and
+// transposed (ds_read_b64_tr_b16) as the second's.  Chunks of 16 bytes are stored
+// at c ^ f(row) of their 128, where f sends the eight rows that a quarter of a
+// wavefront reads to eight places, and the four that a transposed read takes to
+// four pairs of places: neither has a bank conflict.
+//
+// Layout of the products (W columns to a wavefront, lane = c + W h):
+//   S^T = K Q^T.  W = 32 (32x32x16): row 8 m + 4 h' + j is key 16 h' + 4 m + j, so
+//     that a lane's 16 results are keys 16 h .. 16 h + 15 of column c.  W = 16
+//     (16x16x32): row 4 h' + j of row tile r is key 8 h' + 4 r + j; a lane has keys
+//     8 h .. 8 h + 7.
+//   O^T = V^T P^T: those are the lane's part of the B operand; the A operand's
+//     lane has the same keys of a value column.
+//
+// Scores, statistics and sums are fp32.  Weights go to the cache's type (one
+// term: 2^-9 of each weight in bf16, 2^-12 in fp16, as the output's own
+// rounding); their sum is taken before that.  fp16 weights are scaled by 2^13, so
+// that those below 2^-27 of the largest still count.
+#pragma once
+
+#include "kv_attend.hpp"
+#include "latent_common.hpp"
+
+namespace grm {
+namespace kv {
+
+constexpr int kLatentTile = 32;     // rows to a tile
+constexpr int kLatentCols = 128;    // columns to a unit, at most
+constexpr int kLatentLeast = 4;     // tiles to a run, at least
+constexpr int kRowUnit = 128;       // tokens to a unit of attention over dense rows
+
+struct LatentHead {
+  int64_t tiles;      // of all units
+  int32_t units;
+  int32_t row_units;
+  int32_t pad[12];
+};
+static_assert(sizeof(LatentHead) == 64, "the lists behind it stay aligned");
+
+// Tokens of a request from `row` on, the first at position `pos`.
+struct LatentUnit {
+  int32_t request, row, tokens, pos;
+  int32_t tile_lo, pad[3];
+};
+struct RowUnit {
+  int32_t request, row, tokens, pos;
+};
+
+typedef const __attribute__((address_space(4))) LatentHead* ConstLatentHead;
+typedef const __attribute__((address_space(4))) LatentUnit* ConstLatentUnit;
+typedef const __attribute__((address_space(4))) RowUnit* ConstRowUnit;
+typedef const __attribute__((address_space(4))) int64_t* ConstLong;
+
+// Tiles dealt to runs, equal to within one, kLatentLeast at least.
+struct LongDeal {
+  int64_t tiles, each;
+  int used, rem;
+  __host__ __device__ LongDeal(int64_t tiles_, int runs) : tiles(tiles_) {
+    const int64_t most = (tiles + kLatentLeast - 1) / kLatentLeast;
+    used = static_cast<int>(most < runs ? most : runs);
+    each = used ? tiles / used : 0;
+    rem = used ? static_cast<int>(tiles - each * used) : 0;
+  }
+  __host__ __device__ int64_t begin(int r) const {
+    return r >= used ? tiles : r * each + (r < rem ? r : rem);
+  }
+  __host__ __device__ int run(int64_t t) const {
+    const int64_t more = rem * (each + 1);
+    return static_cast<int>(t < more ? t / (each + 1) : rem + (t - more) / each);
+  }
+};
+
+// Sizes and places of the latent schedule, from host-known fields alone.
+struct LatentLayout {
+  int cols;          // columns to a block: 16, 32, 64 or 128
+  int unit_tokens;   // tokens to a unit
+  int runs;
+  uint64_t cap_units, cap_rows;
+  int32_t reach;
+  uint64_t at_units, at_first, at_runs, at_unit_scan, at_row_scan, at_rows, bytes;
+};
+
+int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out);
+
+struct LatentArgs {
+  const char* rows;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t* cu_new;
+  const int32_t* ctx_lens;
+  const int32_t* table;
+  const char* work;
+  float* parts;
+  int64_t q_token, q_head, out_token, out_head;  // strides
+  uint64_t blocks, at_units, at_first, at_runs;
+  float scale;
+  int32_t requests, width, tokens, window, heads, rank, rope, block_log2, runs;
+};
+
+// Rows of nobody: what a tile has where there is no block.  Written by no one.
+static __device__ __align__(16) const uint32_t latent_zeros[16 * (512 + 64) / 2] = {};
+
+// s_waitcnt vmcnt(n) lgkmcnt(0): the wavefront's loads but the last n are done,
+// and its LDS reads.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Four rows of a column to a lane: of 16 lanes, lanes 4 j .. 4 j + 3 name 16
+// columns of row j.
+__device__ __forceinline__ u32x2 read_transposed(const char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)p));
+}
+
+// A product's reads from LDS and what is done with each, in this order: reads run
+// AHEAD before their use, and no further (left to itself the compiler reads all
+// of them first, and spills).
+template <int READS, int AHEAD, class Read, class Use>
+__device__ __forceinline__ void in_order(Read read, Use use) {
+  u32x4 f[READS];
+#pragma unroll
+  for (int i = 0; i < AHEAD && i < READS; ++i) f[i] = read(i);
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    if (i + AHEAD < READS) f[i + AHEAD] = read(i + AHEAD);
+    use(i, f[i]);
+    if (i % 2) __builtin_amdgcn_sched_barrier(0);  // two at a time
+  }
+}
+
+template <class T, int R, int P, int W, int G>
+struct LatentShape {
+  static constexpr int kGroups = G;              // tiles at once
+  static constexpr int kColGroups = 4 / G;       // wavefronts that share a tile
+  static constexpr int kCols = W * kColGroups;
+  static constexpr int kRowBytes = 2 * (R + P);
+  static constexpr int kTileBytes = kLatentTile * kRowBytes;
+  static constexpr int kStages = 4 / G;          // of the ring, G tiles each
+  static constexpr int kLds = 4 * kTileBytes;
+  static constexpr int kH = kWave / W;           // lanes of a column
+  static constexpr int kStep = 8 * kH;           // values to an instruction
+  static constexpr int kLatSteps = R / kStep, kKeySteps = P / kStep;
+  static constexpr int kSteps = kLatSteps + kKeySteps;
+  static constexpr int kTilesD = R / W;
+  static constexpr int kAcc = W * W / kWave;     // results of an instruction to a lane
+  static constexpr int kPer = W / 2;             // scores of a tile to a lane
+  static constexpr int kRowTiles = 32 / W;
+  // direct loads of a wavefront: its rows of a tile
+  static constexpr int kRowsEach = kLatentTile / kColGroups;
+  static constexpr int kLatRows = 1024 / (2 * R);      // rows to a load of latents
+  static constexpr int kKeyRows = 1024 / (2 * P);      // rows to a load of key parts
+  static constexpr int kLatLoads = kRowsEach / kLatRows;
+  static constexpr int kKeyLoads = kRowsEach > kKeyRows ? kRowsEach / kKeyRows : 1;
+  static constexpr int kLoads = kLatLoads + kKeyLoads;
+  static constexpr bool kBf = T::code == kBF16;
+  // Columns may pass their reference by 2^kSlack before the sums are scaled.
+  static constexpr float kSlack = kBf ? 8.0f : 2.0f;
+  static constexpr float kBias = kBf ? 0.0f : 13.0f;
+  typedef typename std::conditional<W == 32, f32x16, f32x4>::type Acc;
+
+  // two weights, rounded
+  static __device__ __forceinline__ uint32_t weights(float x, float y) {
+    if constexpr (kBf) {
+      typedef __bf16 pair __attribute__((ext_vector_type(2)));
+      return __builtin_bit_cast(uint32_t, pair{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+    } else {
+      return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
+    }
+  }
+
+  // where a row's chunks are turned to
+  static __device__ __forceinline__ int turn8(int row) {
+    return 2 * (row & 3) + ((W == 32 ? row >> 4 : row >> 3) & 1);
+  }
+  static __device__ __forceinline__ int turn4(int row) {  // key parts of 64 bytes
+    return ((row >> 1) & 1) + 2 * ((W == 32 ? row >> 4 : row >> 3) & 1);
+  }
+  static __device__ __forceinline__ int turn_key(int row) { return P == 32 ? turn4(row) : turn8(row); }
+};
+
+template <class T>
+__device__ inline void latent_finish(const LatentArgs& a, int row, int h, int d, f32x4 o, float inv,
+                                     bool empty) {
+  typename T::store* out = static_cast<typename T::store*>(a.out) +
+                           static_cast<int64_t>(row) * a.out_token +
+                           static_cast<int64_t>(h) * a.out_head + d;
+  u32x2 v;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv);
+    const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv);
+    v[e] = lo | (hi << 16);
+  }
+  *reinterpret_cast<u32x2*>(out) = v;
+}
+
+template <class T>
+__device__ inline float latent_lse(float m, float l, float bias) {
+  return m == -INFINITY && l == 0.0f ? -INFINITY : (m - bias + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Floats of a part: its columns' sums, maxima and sums of weights.
+__host__ __device__ constexpr size_t latent_part_floats(int cols, int rank) {
+  return static_cast<size_t>(cols) * (rank + 2);
+}
+
+template <class T, int R, int P, int W, int G>
+__global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(LatentArgs a) {
+  typedef LatentShape<T, R, P, W, G> S;
+  typedef typename S::Acc Acc;
+  __shared__ __align__(1024) char ring[S::kLds];
+  __shared__ float s_m[4][W], s_l[4][W];
+  __shared__ int s_odd;
+  const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c = lane % W, h = lane / W;
+  const int group = wave / S::kColGroups, col_group = wave % S::kColGroups;
+  const auto* head = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
+  const LongDeal deal(head->tiles, a.runs);
+  // Neighbouring runs on one XCD (blocks go to the eight in turn): a unit's
+  // neighbours read the same rows.
+  const int xcd = static_cast<int>(blockIdx.x % 8), nth = static_cast<int>(blockIdx.x / 8);
+  if (nth >= deal.used / 8 + (xcd < deal.used % 8)) return;
+  const int run = xcd * (deal.used / 8) + min(xcd, deal.used % 8) + nth;
+  const int64_t begin = deal.begin(run), end = deal.begin(run + 1);
+  const auto* units = reinterpret_cast<ConstLatentUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_units);
+  const auto* firsts = reinterpret_cast<ConstLong>(reinterpret_cast<uintptr_t>(a.work) + a.at_first);
+  const auto* table = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.table));
+  int u = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) + a.at_runs)[run];
+  const int bs = 1 << a.block_log2;
+
+  if (threadIdx.x == 0) s_odd = 0;
+  __syncthreads();
+
+  // ---- lane offsets into a tile
+  // first product: row of this lane's key
+  const int key_row = W == 32 ? 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3) : 8 * (c >> 2) + (c & 3);
+  const int k_at = key_row * 2 * R + 16 * (h ^ S::turn8(key_row));
+  const int p_at = kLatentTile * 2 * R + key_row * 2 * P + 16 * (h ^ S::turn_key(key_row));
+  // second product: a lane of 16 names four columns of a row
+  const int i16 = lane % 16;
+  const int v_row = W == 32 ? 16 * h + i16 / 4 : 8 * h + i16 / 4;
+  const int v_at = v_row * 2 * R + 8 * (i16 & 1) +
+                   16 * (((W == 32 ? 2 * (lane >> 4 & 1) : 0) + (i16 % 4 >> 1)) ^ S::turn8(v_row));
+
+  for (int64_t at = begin; at < end; ++u) {
+    const int64_t first = firsts[u], last = firsts[u + 1];
+    const int64_t stop = last < end ? last : end;
+    const int tile_lo = units[u].tile_lo + static_cast<int>(at - first);
+    const int tile_hi = units[u].tile_lo + static_cast<int>(stop - first);
+    const int request = units[u].request, unit_row = units[u].row, tokens = units[u].tokens;
+    const int first_pos = units[u].pos, last_pos = first_pos + tokens - 1;
+    const bool is_whole = first >= begin && last <= end;
+    const int which = first >= begin ? 1 : 0;
+    at = stop;
+    if (tokens <= 0) continue;
+    wait_loads<0>();  // the last unit's stores: loads are counted from here
+    const int cols = tokens * a.heads;
+    const int first_seen = a.window > 0 ? max(0, first_pos + 1 - a.window) : 0;
+    const int64_t table_row = static_cast<int64_t>(request) * a.width;
+
+    const int col = W * col_group + c;
+    const bool mine = col < cols;
+    const int token = mine ? col / a.heads : tokens - 1;
+    const int q_head = mine ? col - token * a.heads : 0;
+    const int pos = first_pos + token;
+    const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+    const int all_from = a.window > 0 ? max(0, last_pos + 1 - a.window) : 0;
+    const bool busy = W * col_group < cols;  // this wavefront has a column
+
+    // ---- direct loads: this wavefront's rows of the tile that its group takes
+    const int n = (tile_hi - tile_lo + G - 1) / G;
+    const int row0 = col_group * S::kRowsEach;
+    uint32_t there = 0;  // two bits to a stage: its halves have a block
+    // A half's block is looked up a stage before its loads.
+    int id[2];
+    auto look_up = [&](int stage) {
+      const int key = (tile_lo + group + G * stage) * kLatentTile;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int j = (key + 16 * k) >> a.block_log2;
+        id[k] = table[table_row + max(0, min(j, a.width - 1))];
+      }
+    };
+    auto issue = [&](int stage) {
+      const int tile = tile_lo + group + G * stage;
+      const int slot = (stage % S::kStages) * G + group;
+      const char* base[2];
+      uint32_t bits = 0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int key = tile * kLatentTile + 16 * k;
+        const bool ok = tile < tile_hi && key <= last_pos && key + 15 >= first_seen &&
+                        (key >> a.block_log2) < a.width &&
+                        static_cast<uint32_t>(id[k]) < a.blocks;
+        base[k] = ok ? a.rows + ((static_cast<uint64_t>(static_cast<uint32_t>(id[k])) << a.block_log2) +
+                                 (key & (bs - 1))) * S::kRowBytes
+                     : reinterpret_cast<const char*>(latent_zeros);
+        bits |= ok ? 1u << k : 0u;
+      }
+      there |= bits << (2 * (stage % S::kStages));
+      char* to = ring + slot * S::kTileBytes;
+      int lane = __lane_id();
+      asm volatile("" : "+v"(lane));  // offsets made here, not kept over the products
+#pragma unroll
+      for (int i = 0; i < S::kLatLoads; ++i) {
+        const int row = row0 + i * S::kLatRows;                      // of the load
+        const int r = row + lane / (64 / S::kLatRows), chunk = lane % (64 / S::kLatRows);
+        const uint32_t off = (r & 15) * S::kRowBytes + 16 * (chunk ^ S::turn8(r));
+        __builtin_amdgcn_global_load_lds(
+            reinterpret_cast<const u32x4*>(base[S::kRowsEach == 32 ? i * S::kLatRows / 16 : row / 16] + off),
+            (__attribute__((address_space(3))) void*)(to + row * 2 * R), 16, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < S::kKeyLoads; ++i) {
+        // (two wavefronts bring the same 16 rows where eight are a half load)
+        const int row = (row0 / S::kKeyRows + i) * S::kKeyRows;
+        constexpr int kChunks = 2 * P / 16;
+        const int r = row + lane / kChunks, chunk = lane % kChunks;
+        const uint32_t off = (r & 15) * S::kRowBytes + 2 * R + 16 * (chunk ^ S::turn_key(r));
+        __builtin_amdgcn_global_load_lds(
+            reinterpret_cast<const u32x4*>(base[S::kRowsEach == 32 ? i * S::kKeyRows / 16 : row / 16] + off),
+            (__attribute__((address_space(3))) void*)(to + kLatentTile * 2 * R + row * 2 * P), 16, 0, 0);
+      }
+    };
+
+    // ---- queries
+    u32x4 q[S::kSteps];
+    {
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) +
+                             static_cast<int64_t>(min(unit_row + token, a.tokens - 1)) * a.q_token +
+                             static_cast<int64_t>(q_head) * a.q_head + 8 * h;
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s) {
+        q[s] = *reinterpret_cast<const u32x4*>(from + S::kStep * s);
+      }
+    }
+    // In registers before the rows' loads begin, so that a stage waits for rows only.
+    // At rank 512 they live in AGPRs, where the matrix instructions read them, and
+    // leave the VGPRs to the sums (this file is built with the MFMA
+    // VGPR-accumulator form).
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) {
+      if constexpr (R == 512) asm volatile("" : "+a"(q[s]));
+      else asm volatile("" : "+v"(q[s]));
+    }
+    asm volatile("" ::: "memory");
+    look_up(0);
+    if constexpr (S::kStages > 1) {
+#pragma unroll
+      for (int s = 0; s < S::kStages - 1; ++s) {
+        if (s < n) {
+          issue(s);
+          look_up(s + 1);
+        }
+      }
+    }
+
+    Acc o[S::kTilesD];
+#pragma unroll
+    for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+      for (int e = 0; e < S::kAcc; ++e) o[d][e] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f, poison = 0.0f;
+    const float mul = a.scale * kLog2e;
+
+    // The stage's rows are in LDS, and all are done with the one before, whose place
+    // the next loads take.
+    auto enter = [&](int i) {
+      if constexpr (S::kStages == 1) {
+        asm volatile("" ::: "memory");
+        issue(i);
+        look_up(i + 1);
+        wait_loads<0>();
+      } else {
+        if (i + S::kStages - 2 < n) wait_loads<(S::kStages - 2) * S::kLoads>();
+        else wait_loads<0>();
+        block_barrier();
+        if (i + S::kStages - 1 < n) {
+          issue(i + S::kStages - 1);
+          look_up(i + S::kStages);
+        }
+      }
+    };
+    // A row that is not finite has no finite score with any column.  Where some
+    // column does not see all rows of the stage, such values (which a weight of 0
+    // would not keep out) are taken from the rows in LDS between the products;
+    // columns that do see them have their scores by then.
+    auto partly_seen = [&](int i) {
+      const int tile = tile_lo + G * i;
+      return tile * kLatentTile < all_from || (tile + G) * kLatentTile - 1 > first_pos;
+    };
+    auto keep_finite = [&](int i, bool odd) {
+      if constexpr (G < 4) {
+        if (odd && lane == 0) s_odd = 1;
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        block_barrier();
+        odd = *static_cast<volatile int*>(&s_odd) != 0;
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        block_barrier();
+        if (!odd) return;
+        if (threadIdx.x == 0) s_odd = 0;
+      } else if (!odd) {
+        return;
+      }
+      char* rows = ring + ((i % S::kStages) * G + group) * S::kTileBytes;
+      constexpr uint32_t kLo = S::kBf ? 0x7f80u : 0x7c00u, kHi = kLo << 16;
+#pragma nounroll
+      for (int at = 16 * (col_group * kWave + lane); at < kLatentTile * 2 * R;
+           at += 16 * kWave * S::kColGroups) {
+        u32x4 v = *reinterpret_cast<u32x4*>(rows + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((v[e] & kLo) == kLo) v[e] &= 0xffff0000u;
+          if ((v[e] & kHi) == kHi) v[e] &= 0xffffu;
+        }
+        *reinterpret_cast<u32x4*>(rows + at) = v;
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+      if constexpr (G < 4) block_barrier();
+      else asm volatile("" ::: "memory");
+    };
+    if (!busy) {  // brings its rows
+      for (int i = 0; i < n; ++i) {
+        enter(i);
+        if (partly_seen(i)) keep_finite(i, false);
+      }
+    }
+    for (int i = 0; i < n && busy; ++i) {
+      enter(i);
+      const int slot = i % S::kStages;
+      const uint32_t have = there >> (2 * slot) & 3u;
+      there &= ~(3u << (2 * slot));
+      const int tile = tile_lo + group + G * i;
+      const char* from = ring + (slot * G + group) * S::kTileBytes;
+
+      // scores
+      Acc s[S::kRowTiles];
+#pragma unroll
+      for (int r = 0; r < S::kRowTiles; ++r) {
+#pragma unroll
+        for (int e = 0; e < S::kAcc; ++e) s[r][e] = 0.0f;
+      }
+      auto key_chunk = [&](int step, int r) {
+        // a step is 16 kH bytes of a row; steps of 128 bytes on have a constant
+        // distance
+        constexpr int kIn = 8 / S::kH;  // steps to 128 bytes
+        if (step < S::kLatSteps) {
+          return *reinterpret_cast<const u32x4*>(
+              from + ((k_at ^ (16 * S::kH * (step % kIn))) + 128 * (step / kIn) + r * 4 * 2 * R));
+        }
+        const int k = step - S::kLatSteps;
+        return *reinterpret_cast<const u32x4*>(
+            from + ((p_at ^ (16 * S::kH * (k % kIn))) + 128 * (k / kIn) + r * 4 * 2 * P));
+      };
+      in_order<S::kSteps * S::kRowTiles, 4>(
+          [&](int i) { return key_chunk(i / S::kRowTiles, i % S::kRowTiles); },
+          [&](int i, u32x4 f) {
+            s[i % S::kRowTiles] = mfma<S::kBf>(f, q[i / S::kRowTiles], s[i % S::kRowTiles]);
+          });
+      float score[S::kPer];
+#pragma unroll
+      for (int e = 0; e < S::kPer; ++e) score[e] = s[e / S::kAcc][e % S::kAcc];
+      float odd_sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < S::kPer; ++e) odd_sum = fmaf(score[e], 0.0f, odd_sum);
+      const bool odd = __any(odd_sum != 0.0f);
+      if (partly_seen(i)) keep_finite(i, odd);
+      const int key0 = tile * kLatentTile + S::kPer * h;  // a lane's first
+      const bool whole = tile * kLatentTile >= all_from && tile < tile_hi &&
+                         tile * kLatentTile + kLatentTile - 1 <= first_pos && have == 3u;
+      float top = -INFINITY;
+      if (whole && !odd) {
+#pragma unroll
+        for (int e = 0; e < S::kPer; ++e) {
+          score[e] *= mul;
+          top = fmaxf(top, score[e]);
+        }
+      } else {
+        // a lane's keys lie in one half
+        const bool some = tile < tile_hi && (have >> (S::kPer * h >> 4) & 1u);
+#pragma unroll
+        for (int e = 0; e < S::kPer; ++e) {
+          const int key = key0 + e;
+          const bool see = some && key <= pos && key >= seen_from;
+          const bool fine = fabsf(score[e]) <= 3.4028235e38f;
+          poison += see && !fine ? NAN : 0.0f;
+          score[e] = see && fine ? score[e] * mul : -INFINITY;
+          top = fmaxf(top, score[e]);
+        }
+      }
+      if (__any(top > m + S::kSlack)) {
+        float m2 = fmaxf(m, top);
+#pragma unroll
+        for (int by = W; by < kWave; by *= 2) m2 = fmaxf(m2, __shfl_xor(m2, by));
+        const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
+        if (__any(m != -INFINITY)) {
+#pragma unroll
+          for (int d = 0; d < S::kTilesD; ++d) o[d] *= keep;
+        }
+        l *= keep;
+        m = m2;
+      }
+      const float shift = S::kBias - (m == -INFINITY ? 0.0f : m);
+      u32x4 w[S::kPer / 8];
+#pragma unroll
+      for (int e = 0; e < S::kPer; e += 2) {
+        const float x = __builtin_amdgcn_exp2f(score[e] + shift);
+        const float y = __builtin_amdgcn_exp2f(score[e + 1] + shift);
+        l += x;
+        l += y;
+        w[e / 8][e % 8 / 2] = S::weights(x, y);
+      }
+      // values
+      auto value_chunk = [&](int d, int k) {
+        // W = 32: two value tiles to 128 bytes, 8 keys on from 16 h + 8 k; W = 16:
+        // four tiles to 128 bytes
+        constexpr int kIn = 64 / W;
+        const char* p = from + ((v_at ^ (2 * W * (d % kIn))) + 128 * (d / kIn) + k * 8 * 2 * R);
+        const u32x2 lo = read_transposed(p), hi = read_transposed(p + 4 * 2 * R);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      };
+      in_order<S::kTilesD * (S::kPer / 8), 4>(
+          [&](int i) { return value_chunk(i / (S::kPer / 8), i % (S::kPer / 8)); },
+          [&](int i, u32x4 f) {
+            o[i / (S::kPer / 8)] = mfma<S::kBf>(f, w[i % (S::kPer / 8)], o[i / (S::kPer / 8)]);
+          });
+    }
+
+#pragma unroll
+    for (int by = W; by < kWave; by *= 2) {
+      l += __shfl_xor(l, by);
+      poison += __shfl_xor(poison, by);
+    }
+    l += poison;
+    // ---- the groups' results together
+    if constexpr (G > 1) {
+      if (h == 0) {
+        s_m[wave][c] = m;
+        s_l[wave][c] = l;
+      }
+      __syncthreads();  // also: the ring is read
+      float top = -INFINITY, total = 0.0f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) top = fmaxf(top, s_m[g * S::kColGroups + col_group][c]);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float mg = s_m[g * S::kColGroups + col_group][c], lg = s_l[g * S::kColGroups + col_group][c];
+        total += lg * (mg == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mg - top));
+      }
+      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l = total;
+      constexpr int kVecs = S::kAcc / 4;
+      constexpr int kAt = S::kLds / (4 * kWave * 16 * kVecs);          // value tiles at once
+      constexpr int kTiles = kAt / G * G < S::kTilesD ? kAt / G * G : S::kTilesD;
+      static_assert(kTiles > 0 && S::kTilesD % kTiles == 0, "whole rounds");
+      f32x4* box = reinterpret_cast<f32x4*>(ring);
+#pragma unroll
+      for (int d0 = 0; d0 < S::kTilesD; d0 += kTiles) {
+        if (d0) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) {
+#pragma unroll
+          for (int k = 0; k < kVecs; ++k) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = o[d0 + d][4 * k + e] * f;
+            box[((wave * kTiles + d) * kVecs + k) * kWave + lane] = v;
+          }
+        }
+        __syncthreads();
+        if (mine) {
+          const float inv = 1.0f / l;
+          const bool empty = m == -INFINITY && l == 0.0f;
+          float* part = a.parts + (static_cast<size_t>(run) * 2 + which) * latent_part_floats(S::kCols, R);
+          for (int d = group; d < kTiles; d += G) {
+#pragma unroll
+            for (int k = 0; k < kVecs; ++k) {
+              f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+                v += box[(((g * S::kColGroups + col_group) * kTiles + d) * kVecs + k) * kWave + lane];
+              }
+              const int x = W * (d0 + d) + 4 * S::kH * k + 4 * h;
+              if (is_whole) latent_finish<T>(a, unit_row + token, q_head, x, v, inv, empty);
+              else *reinterpret_cast<f32x4*>(part + col * R + x) = v;
+            }
+          }
+        }
+      }
+      __syncthreads();  // the ring takes the next unit's rows
+    } else if (mine) {
+      const float inv = 1.0f / l;
+      const bool empty = m == -INFINITY && l == 0.0f;
+      float* part = a.parts + (static_cast<size_t>(run) * 2 + which) * latent_part_floats(S::kCols, R);
+#pragma unroll
+      for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+        for (int k = 0; k < S::kAcc / 4; ++k) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = o[d][4 * k + e];
+          const int x = W * d + 4 * S::kH * k + 4 * h;
+          if (is_whole) latent_finish<T>(a, unit_row + token, q_head, x, v, inv, empty);
+          else *reinterpret_cast<f32x4*>(part + col * R + x) = v;
+        }
+      }
+    }
+    if constexpr (G == 1) __syncthreads();
+    if (mine && h == 0 && group == 0) {
+      if (is_whole) {
+        if (a.lse) {
+          a.lse[static_cast<size_t>(unit_row + token) * a.heads + q_head] = latent_lse<T>(m, l, S::kBias);
+        }
+      } else {
+        float* part = a.parts + (static_cast<size_t>(run) * 2 + which) * latent_part_floats(S::kCols, R);
+        part[S::kCols * R + col] = m;
+        part[S::kCols * (R + 1) + col] = l;
+      }
+    }
+  }
+}
+
+// Joins the parts of the unit that a run's end cuts first: block x is the end of
+// run x, and a block of it takes 1024 / R columns, four values to a thread.
+template <class T, int R, int COLS>
+__global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bias) {
+  constexpr int kVecs = R / 4, kEach = 256 / kVecs;
+  const auto* head = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
+  const LongDeal deal(head->tiles, a.runs);
+  const int run = static_cast<int>(blockIdx.x) + 1;
+  if (run >= deal.used) return;
+  const auto* units = reinterpret_cast<ConstLatentUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_units);
+  const auto* firsts = reinterpret_cast<ConstLong>(reinterpret_cast<uintptr_t>(a.work) + a.at_first);
+  const int u = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) + a.at_runs)[run];
+  const int64_t first = firsts[u], last = firsts[u + 1];
+  if (first >= deal.begin(run)) return;             // begins with this run
+  if (first < deal.begin(run - 1)) return;          // an end before this one cuts it too
+  const int from = run - 1, to = deal.run(last - 1);
+  const int from_which = first >= deal.begin(from) ? 1 : 0;
+  const int cols = units[u].tokens * a.heads;
+  const int c = static_cast<int>(blockIdx.y) * kEach + static_cast<int>(threadIdx.x) / kVecs;
+  const int d = static_cast<int>(threadIdx.x) % kVecs * 4;
+  if (c >= cols) return;
+  constexpr size_t kPart = latent_part_floats(COLS, R);
+  auto part = [&](int r) { return a.parts + (static_cast<size_t>(r) * 2 + (r == from ? from_which : 0)) * kPart; };
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int kBatch = 8;  // parts whose loads go out together
+  for (int r0 = from; r0 <= to; r0 += kBatch) {
+    float pm[kBatch], pl[kBatch];
+    f32x4 po[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float* p = part(min(r0 + k, to));
+      pm[k] = p[COLS * R + c];
+      pl[k] = p[COLS * (R + 1) + c];
+      po[k] = *reinterpret_cast<const f32x4*>(p + c * R + d);
+    }
+    float m2 = m;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) m2 = r0 + k <= to ? fmaxf(m2, pm[k]) : m2;
+    const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
+    o *= keep;
+    l = l == l ? l * keep : l;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (r0 + k <= to) {
+        // nothing seen: sums of 0 (or NaN, which stays)
+        const float f = pm[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[k] - m2);
+        o += po[k] * f;
+        l += pl[k] == pl[k] ? pl[k] * f : NAN;
+      }
+    }
+    m = m2;
+  }
+  const bool empty = m == -INFINITY && l == 0.0f;
+  const int token = c / a.heads, h = c - token * a.heads;
+  latent_finish<T>(a, units[u].row + token, h, d, o, 1.0f / l, empty);
+  if (a.lse && d == 0) {
+    a.lse[static_cast<size_t>(units[u].row + token) * a.heads + h] = latent_lse<T>(m, l, bias);
+  }
+}
+
+}  // namespace kv
+}  // namespace grm

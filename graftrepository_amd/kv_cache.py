@@ -259,7 +259,8 @@ class KvBatch:
     and buffers, so a batch object serves every step within them, with
     ``ctx_lens``, ``new_lens`` and the table updated in place.  ``window``
     limits a token to its last ``window`` tokens; layers with another window
-    take a second batch over the same arrays.
+    take a second batch over the same arrays.  ``latent``: the plan also makes
+    the schedule of ``LatentCache.attend`` and ``attend_rows`` (kv_heads 1).
 
     Calls with one batch follow each other: on one stream, or ordered by the
     caller.  Work that runs at the same time on several streams, replays of
@@ -269,8 +270,10 @@ class KvBatch:
 
     def __init__(self, ctx_lens, new_lens, block_table, block_tokens: int, *, tokens: int,
                  max_new: int, heads: int, kv_heads: int, window: int = 0, free_list=None,
-                 free_head=None):
+                 free_head=None, latent: bool = False):
         self._lib = _lib.load()
+        if latent and kv_heads != 1:
+            raise ValueError("a latent batch has kv_heads 1: heads share a token's row")
         n = int(ctx_lens.shape[0])
         d = self._desc = _BatchDesc()
         d.ctx_lens = _dense(ctx_lens, "ctx_lens", "i32", (n,))
@@ -305,6 +308,12 @@ class KvBatch:
             self.free_head_out = self._made_head = _empty(ctx_lens, (1,), "i32")
             d.free_head_out = self.free_head_out.data_ptr()
         self._ref = ctypes.byref(d)
+        self._latent = None
+        if latent:
+            _lib.check(_call(self._lib.grm_hip_latent_work_bytes, ctx_lens, self.device,
+                             self._ref, ctypes.byref(need)), "latent work size")
+            self._latent = _empty(ctx_lens, (need.value,), "u8")
+            self._latent_at, self._latent_bytes = self._latent.data_ptr(), need.value
         self._scratch: dict[int, int] = {}
         self._held: dict[int, list] = {}
         self._streams = {_stream(ctx_lens, None)}
@@ -314,10 +323,15 @@ class KvBatch:
     def plan(self, stream=None) -> "KvBatch":
         """Fill ``cu_new``, ``slot_map``, ``positions``, the table's new
         entries and the schedule from the lengths as they are now."""
-        rc = _call(self._lib.grm_hip_kv_plan, self.ctx_lens, self.device, self._ref,
-                   self._on(self.ctx_lens, stream))
+        on = self._on(self.ctx_lens, stream)
+        rc = _call(self._lib.grm_hip_kv_plan, self.ctx_lens, self.device, self._ref, on)
         if rc:
             _lib.check(rc, "kv plan")
+        if self._latent is not None:
+            rc = _call(self._lib.grm_hip_latent_plan, self.ctx_lens, self.device, self._ref,
+                       self._latent_at, self._latent_bytes, on)
+            if rc:
+                _lib.check(rc, "latent plan")
         self._planned = self._taken = True
         return self
 
@@ -340,7 +354,7 @@ class KvBatch:
             if _is_torch(self._work):
                 s = _torch_stream(self._work, on)
                 for a in (self.cu_new, self.slot_map, self.positions, self._work,
-                          self._made_head):
+                          self._latent, self._made_head):
                     if a is not None:
                         a.record_stream(s)
         return on

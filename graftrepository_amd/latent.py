@@ -3,10 +3,15 @@ one (the MLA dialect's).
 
 A row holds a token's latent and its turned key part, shared by all heads::
 
-    batch = KvBatch(..., heads=40, kv_heads=1)
-    batch.plan()                                       # once per step
+    batch = KvBatch(..., heads=40, kv_heads=1, latent=True)
+    batch.plan()                                           # once per step
     cache.append(batch, latent, key_part, rotary=rotary)   # per layer
+    out = cache.attend(batch, q, scale)                    # per layer, absorbed
     rows = cache.read(table, starts, cu_rows, rows)        # dense, to harvest
+
+In the absorbed form a head's query is taken to the latent's space before (its
+own part times the weights that make a head's keys), and its output, a mean of
+latents, goes through the weights that make its values after.
 
 Batches, memory, streams and errors are those of ``kv_cache``; laws and layouts
 those of ``include/grm_hip_router.h``.
@@ -15,10 +20,12 @@ those of ``include/grm_hip_router.h``.
 from __future__ import annotations
 
 import ctypes
+import sys
 
 from . import _lib
-from .kv_cache import (KvBatch, _call, _dense, _empty, _name_of, _one_device, _rows,
-                       _same_device, _stream, _type, i32, u64, vp)
+from .kv_cache import (KvBatch, _call, _copied, _dense, _empty, _is_torch, _name_of, _off,
+                       _one_device, _rows, _same_device, _stream, _torch_stream, _type, i32, u64,
+                       vp)
 from .payload import DeviceArray
 
 
@@ -42,6 +49,51 @@ def _flat(a, what: str, tokens: int, values: int):
         _type(a, what)
     ptr, name, stride, _ = _rows(a.unsqueeze(1), what, (tokens, 1, values))
     return ptr, name, stride
+
+
+def _latent_batch(batch: KvBatch) -> None:
+    if batch._latent is None:
+        raise ValueError("the batch has no latent schedule: make it with latent=True")
+
+
+def _aligned(a, what: str, shape, dtype: str, stream):
+    """(the values, their (address, row stride, head stride)), copied where a
+    torch tensor's rows are not 16-byte aligned."""
+    row = _rows(a, what, shape)
+    if row[1] != dtype:
+        raise ValueError(f"{what} must be {dtype}, got {a.dtype}")
+    if _off(row) and _is_torch(a):
+        a = _copied(a, stream)
+        row = _rows(a, what, shape)
+    return a, (row[0], row[2], row[3])
+
+
+def _output(like, out, shape, dtype: str, device: int, stream):
+    """(the output, its (address, row stride, head stride), what it is copied
+    from where its own rows are not 16-byte aligned)."""
+    if out is None:
+        out = _empty(like, shape, dtype, stream)
+        return out, (out.data_ptr(), shape[1] * shape[2], shape[2]), None
+    _same_device(out, "out", device)
+    result, row = _aligned(out, "out", shape, dtype, stream)  # rows that are not written stay
+    return out, row, None if result is out else result
+
+
+def _statistics(like, lse, wanted: bool, shape, device: int, stream):
+    if lse is None:
+        if not wanted:
+            return None, None
+        lse = _empty(like, shape, "f32", stream)
+        return lse, lse.data_ptr()
+    at = _dense(lse, "lse", "f32", shape)
+    _same_device(lse, "lse", device)
+    return lse, at
+
+
+def _written(out, result, on: int) -> None:
+    if result is not None:
+        with sys.modules["torch"].cuda.stream(_torch_stream(out, on)):
+            out.copy_(result)
 
 
 class LatentCache:
@@ -108,6 +160,38 @@ class LatentCache:
                    kt, batch._on(latent, stream))
         if rc:
             _lib.check(rc, "latent append")
+
+    def attend(self, batch: KvBatch, q, softmax_scale: float, *, out=None, lse=None,
+               return_lse: bool = False, stream=None):
+        """Absorbed causal attention of the step's queries ``q`` [tokens, heads,
+        rank + rope] (the cache's type) over the cache, which holds the step's
+        own rows.  Returns ``out`` [tokens, heads, rank] (also taken as an
+        argument), with ``return_lse`` also the fp32 [tokens, heads] log-sum-exp
+        of the scores.  Rows of torch tensors that are not 16-byte aligned are
+        copied on the way."""
+        batch._ready_for(self)
+        d = batch._desc
+        _latent_batch(batch)
+        q, row = _aligned(q, "q", (d.tokens, d.heads, self.rank + self.rope), self.dtype, stream)
+        _same_device(q, "q", self.device)
+        out, to, result = _output(q, out, (d.tokens, d.heads, self.rank), self.dtype, self.device,
+                                  stream)
+        lse, lp = _statistics(q, lse, return_lse, (d.tokens, d.heads), self.device, stream)
+        key = ("latent", self.rank)
+        need = batch._scratch.get(key)
+        if need is None:
+            got = u64()
+            _lib.check(_call(self._lib.grm_hip_latent_attend_bytes, q, self.device, self._ref,
+                             batch._ref, ctypes.byref(got)), "latent scratch size")
+            need = batch._scratch[key] = got.value
+        on = batch._on(q, stream)
+        rc = _call(self._lib.grm_hip_latent_attend, q, self.device, self._ref, batch._ref,
+                   batch._latent_at, batch._latent_bytes, *row, *to, lp, softmax_scale,
+                   batch._scratch_on(q, need, on, stream) if need else None, need, on)
+        if rc:
+            _lib.check(rc, "latent attend")
+        _written(out, result, on)
+        return (out, lse) if return_lse else out
 
     def _ranges(self, block_table, starts, cu_rows, rows):
         n = int(starts.shape[0])

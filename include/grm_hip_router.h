@@ -682,6 +682,35 @@ int grm_hip_latent_read(const grm_latent_desc* cache, const int32_t* block_table
                         int table_width, int requests, const int32_t* starts,
                         const int32_t* cu_rows, uint64_t rows, int dtype, void* out, void* stream);
 
+/* Bytes of the latent schedule of a batch of this shape (host fields only). */
+int grm_hip_latent_work_bytes(const grm_kv_batch_desc* batch, uint64_t* out_bytes);
+
+/* Once per step, after grm_hip_kv_plan: the schedule that
+ * grm_hip_latent_attend and grm_hip_rows_attend follow, into `work` (16-byte
+ * aligned device memory, beside the batch's own). */
+int grm_hip_latent_plan(const grm_kv_batch_desc* batch, void* work, uint64_t work_bytes,
+                        void* stream);
+
+/* Bytes of scratch one latent attend call needs (may be 0). */
+int grm_hip_latent_attend_bytes(const grm_latent_desc* cache, const grm_kv_batch_desc* batch,
+                                uint64_t* out_bytes);
+
+/* Absorbed attention of the step's tokens over the cache (which holds the
+ * step's own rows: append first).  q [tokens][heads][rank + rope] and out
+ * [tokens][heads][rank], both of the cache's dtype; strides in elements,
+ * multiples of 16 bytes:
+ *   s_j = softmax_scale * q . row_j,  o = sum_j softmax(s)_j row_j[0 .. rank)
+ * over the positions j a token sees, as in grm_hip_kv_attend; so are lse,
+ * tokens that see nothing, rows past the last and the order of sums.  A query
+ * is W_k^T times a head's own query beside its turned part, and W_v takes an
+ * output to the head's own. */
+int grm_hip_latent_attend(const grm_latent_desc* cache, const grm_kv_batch_desc* batch,
+                          const void* work, uint64_t work_bytes, const void* q,
+                          int64_t q_token_stride, int64_t q_head_stride, void* out,
+                          int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                          float softmax_scale, void* scratch, uint64_t scratch_bytes,
+                          void* stream);
+
 /* ---- Synthetic workload keys (host only) --------------------------------
  * Rows [row0, row0 + rows) of the synthetic INT8 key stream: each row's dim
  * values are normal quantiles (normal_table[65536], the caller's table of

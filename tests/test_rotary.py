@@ -198,3 +198,31 @@ def test_python_checks_of_a_latent_cache():
         c.read(fake((3, 4), np.int32), fake((3,), np.int32), fake((3,), np.int32), 5)
     with pytest.raises(ValueError):
         c.read(fake((3, 4), np.int32), fake((3,), np.int32), fake((4,), np.int32), 5, dtype="i8")
+
+
+def test_bad_attention_calls_are_refused():
+    lib = g.load()
+    c, out = ctypes.byref(latent_desc()), ctypes.c_uint64()
+    b = one_head()
+    rb = ctypes.byref(b)
+    assert lib.grm_hip_latent_work_bytes(rb, None) == -1
+    assert lib.grm_hip_latent_work_bytes(None, ctypes.byref(out)) == -1
+    assert lib.grm_hip_latent_attend_bytes(c, rb, None) == -1
+    assert lib.grm_hip_latent_plan(rb, None, 1 << 40, None) == -1
+    assert lib.grm_hip_latent_plan(rb, 0x1008, 1 << 40, None) == -1
+    assert lib.grm_hip_latent_plan(ctypes.byref(one_head(new_lens=None)), 0x1000, 1 << 40, None) == -1
+
+    def attend(cache=c, batch=rb, work=0x1000, q=0x1000, qt=384, qh=96, o=0x2000, ot=256, oh=64,
+               scale=1.0):
+        return lib.grm_hip_latent_attend(cache, batch, work, 1 << 40, q, qt, qh, o, ot, oh, None,
+                                         scale, None, 0, None)
+    for kw in (dict(q=None), dict(o=None), dict(q=0x1002), dict(o=0x2008), dict(qt=385), dict(qh=100),
+               dict(ot=4), dict(oh=66), dict(scale=float("nan")), dict(scale=float("inf")),
+               dict(batch=ctypes.byref(one_head(kv_heads=2))), dict(cache=None), dict(batch=None)):
+        assert attend(**kw) == -1, kw
+
+
+def test_python_checks_of_latent_batches():
+    ints = [fake((3,), np.int32), fake((3,), np.int32), fake((3, 4), np.int32)]
+    with pytest.raises(ValueError, match="kv_heads"):
+        g.KvBatch(*ints, 16, tokens=3, max_new=1, heads=4, kv_heads=2, latent=True)
