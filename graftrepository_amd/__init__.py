@@ -21,9 +21,9 @@ from ._lib import HipRouterUnavailable, library_path, load, runtime_info
 from .node_bank import GqaNodeBank, MlaNodeBank, RouteResult
 from .bank_bridge import GqaRouteBankBridge, MlaRouteBankBridge
 from .kv_cache import KvBatch, KvCache
-from .latent import LatentCache
+from .latent import LatentCache, attend_rows
 from .rotary import Rotary
 
 __all__ = ["HipRouterUnavailable", "library_path", "load", "runtime_info",
            "GqaNodeBank", "MlaNodeBank", "RouteResult", "GqaRouteBankBridge",
-           "MlaRouteBankBridge", "KvBatch", "KvCache", "LatentCache", "Rotary"]
+           "MlaRouteBankBridge", "KvBatch", "KvCache", "LatentCache", "Rotary", "attend_rows"]

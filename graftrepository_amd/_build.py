@@ -55,6 +55,7 @@ def sources() -> list[Path]:
 # sums, and spill.
 SOURCE_FLAGS = {
     "latent_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "latent_expand.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mla_route.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mla_screen_probe.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }

@@ -1,0 +1,686 @@
+// latent_expand.hip -- the expanded form of latent attention: a head's own keys and
+// values from cached latents, and causal attention over such dense rows.
+//
+//   k[row, head] = [W_k[head] c | key part],  v[row, head] = W_v[head] c
+//
+// An expansion is a matrix product whose left operand is gathered through the
+// block table; a prompt of n tokens needs 2 n (dk + dv) operations a key after it,
+// where the absorbed form needs 2 n (2 rank + rope).
+#include "latent_attend.hpp"
+
+namespace grm {
+namespace kv {
+
+// ----------------------------------------------------------------- expand
+
+struct ExpandArgs {
+  const uint16_t* rows;
+  const uint16_t* weight;  // [heads][key_dim + value_dim][rank]
+  uint16_t* k;             // [rows][heads][key_dim + rope]
+  uint16_t* v;             // [rows][heads][value_dim]
+  RowRanges of;
+  int32_t rank, rope, heads, key_dim, value_dim;
+};
+
+// 128 rows x 256 columns to a block, 64 x 128 to a wavefront, 32 of the rank a
+// stage; three stages of direct loads in LDS, two blocks to a CU, so that one's
+// stores run beside the other's products.  Chunks of 16 bytes are stored at c ^ (row >> 1
+// & 3) of their 64: eight rows' chunk c lie in eight places.  Results leave
+// through LDS, 16 bytes to a lane.
+constexpr int kExpandRows = 128, kExpandCols = 256, kExpandStep = 32, kExpandStages = 3;
+constexpr int kExpandStage = (kExpandRows + kExpandCols) * kExpandStep * 2;  // bytes
+constexpr int kExpandOut = kExpandCols * 2 + 16;                             // of a row on its way out
+
+template <class T>
+__global__ __launch_bounds__(256, 2) void latent_expand_kernel(ExpandArgs a) {
+  __shared__ __align__(1024) char lds[kExpandStages * kExpandStage];
+  __shared__ int64_t s_row[kExpandRows];
+  static_assert(kExpandRows * kExpandOut <= kExpandStages * kExpandStage, "results fit the ring");
+  const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c = lane % 32, h = lane / 32;
+  const int width = a.key_dim + a.value_dim, columns = a.heads * width;
+  // Blocks go to the XCDs in turn: with whole eighths of the columns each has its
+  // own of the weights, which stay in its L2.
+  const int wide = (columns + kExpandCols - 1) / kExpandCols;
+  const int col0 = static_cast<int>(blockIdx.x % wide) * kExpandCols;
+  const int row0 = static_cast<int>(blockIdx.x / wide) * kExpandRows;
+  const int values = a.rank + a.rope;
+  if (threadIdx.x < kExpandRows) {
+    s_row[threadIdx.x] = cache_row(a.of, row0 + static_cast<int>(threadIdx.x));
+  }
+  __syncthreads();
+  // loads of 16 rows by four chunks: two of cache rows, four of weights
+  const int r16 = lane / 4, chunk = (lane % 4) ^ (r16 >> 1 & 3);
+  const uint16_t* from[6];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t row = s_row[(2 * wave + i) * 16 + r16];
+    from[i] = (row >= 0 ? a.rows + row * values : reinterpret_cast<const uint16_t*>(latent_zeros)) + 8 * chunk;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = min(col0 + (4 * wave + i) * 16 + r16, columns - 1);
+    from[2 + i] = a.weight + static_cast<int64_t>(n) * a.rank + 8 * chunk;
+  }
+  auto issue = [&](int step) {
+    char* to = lds + (step % kExpandStages) * kExpandStage;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      char* at = i < 2 ? to + (2 * wave + i) * 1024
+                       : to + kExpandRows * kExpandStep * 2 + (4 * wave + i - 2) * 1024;
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const u32x4*>(from[i] + step * kExpandStep),
+                                       (__attribute__((address_space(3))) void*)at, 16, 0, 0);
+    }
+  };
+  const int steps = a.rank / kExpandStep;
+  issue(0);
+  if (steps > 1) issue(1);
+
+  const int wave_row = 64 * (wave & 1), wave_col = 128 * (wave >> 1);
+  f32x16 acc[2][4];  // [rows][columns]: a lane's column of 32 is a row, its results columns
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    }
+  }
+  const int at = c * 64 + 16 * (h ^ (c >> 1 & 3));
+  for (int s = 0; s < steps; ++s) {
+    if (s + 1 < steps) wait_loads<6>();
+    else wait_loads<0>();
+    block_barrier();
+    if (s + 2 < steps) issue(s + 2);
+    const char* rows = lds + (s % kExpandStages) * kExpandStage + wave_row * 64;
+    const char* cols = lds + (s % kExpandStages) * kExpandStage + kExpandRows * 64 + wave_col * 64;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      u32x4 x[2], w[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[i] = *reinterpret_cast<const u32x4*>(rows + i * 32 * 64 + (at ^ 32 * k));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const u32x4*>(cols + j * 32 * 64 + (at ^ 32 * k));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][j] = mfma<T::code == kBF16>(w[j], x[i], acc[i][j]);
+      }
+    }
+  }
+  wait_loads<0>();
+  block_barrier();  // the ring is read
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        u32x2 v;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t lo = T::put(acc[i][j][4 * q + 2 * e]), hi = T::put(acc[i][j][4 * q + 2 * e + 1]);
+          v[e] = lo | (hi << 16);
+        }
+        *reinterpret_cast<u32x2*>(lds + (wave_row + 32 * i + c) * kExpandOut +
+                                  2 * (wave_col + 32 * j + 8 * q + 4 * h)) = v;
+      }
+    }
+  }
+  __syncthreads();
+  const int rows_here = static_cast<int>(min(static_cast<uint64_t>(kExpandRows), a.of.rows - row0));
+  {
+    // a thread's eight columns stay, its row goes on by eight
+    const int n = col0 + 8 * (static_cast<int>(threadIdx.x) % 32);
+    if (n < columns) {
+      const int head = n / width, d = n - head * width;
+      const bool key = d < a.key_dim;
+      const int64_t stride = static_cast<int64_t>(a.heads) * (key ? a.key_dim + a.rope : a.value_dim);
+      uint16_t* to = key ? a.k + static_cast<int64_t>(head) * (a.key_dim + a.rope) + d
+                         : a.v + static_cast<int64_t>(head) * a.value_dim + d - a.key_dim;
+      for (int r = threadIdx.x / 32; r < rows_here; r += 8) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(lds + r * kExpandOut + 2 * (n - col0));
+        *reinterpret_cast<u32x4*>(to + (row0 + r) * stride) = x;
+      }
+    }
+  }
+  // the key parts of the heads that begin in this block's columns
+  const int first = (col0 + width - 1) / width, last = min(a.heads, (col0 + kExpandCols + width - 1) / width);
+  const int chunks = a.rope / 8, each = chunks * (last - first);
+  for (int i = threadIdx.x; i < each * rows_here; i += 256) {
+    const int r = i / each, j = i - r * each, head = first + j / chunks, d = 8 * (j % chunks);
+    const int64_t row = s_row[r];
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (row >= 0) x = *reinterpret_cast<const u32x4*>(a.rows + row * values + a.rank + d);
+    *reinterpret_cast<u32x4*>(a.k + (static_cast<int64_t>(row0 + r) * a.heads + head) * (a.key_dim + a.rope) +
+                              a.key_dim + d) = x;
+  }
+}
+
+// Ranks that are no whole stages: a row to a block, its latent in LDS.
+template <class T>
+__global__ __launch_bounds__(256) void latent_expand_any_kernel(ExpandArgs a) {
+  __shared__ float s_c[512];
+  const int row = blockIdx.x, values = a.rank + a.rope, width = a.key_dim + a.value_dim;
+  const int64_t at = cache_row(a.of, row);
+  for (int d = threadIdx.x; d < a.rank; d += 256) s_c[d] = at >= 0 ? T::get(a.rows[at * values + d]) : 0.0f;
+  __syncthreads();
+  for (int n = threadIdx.x; n < a.heads * width; n += 256) {
+    float sum = 0.0f;
+    for (int d = 0; d < a.rank; d += 8) {
+      float w[8];
+      get8<T, true>(a.weight + static_cast<int64_t>(n) * a.rank + d, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(w[e], s_c[d + e], sum);
+    }
+    const int head = n / width, d = n - head * width;
+    if (d < a.key_dim) a.k[(static_cast<int64_t>(row) * a.heads + head) * (a.key_dim + a.rope) + d] = T::put(sum);
+    else a.v[(static_cast<int64_t>(row) * a.heads + head) * a.value_dim + d - a.key_dim] = T::put(sum);
+  }
+  for (int i = threadIdx.x; i < a.heads * a.rope; i += 256) {
+    const int head = i / a.rope, d = i - head * a.rope;
+    a.k[(static_cast<int64_t>(row) * a.heads + head) * (a.key_dim + a.rope) + a.key_dim + d] =
+        at >= 0 ? a.rows[at * values + a.rank + d] : uint16_t{0};
+  }
+}
+
+// ------------------------------------------------- attention over dense rows
+
+struct RowsArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* out;
+  float* lse;
+  const int32_t* cu_new;
+  const int32_t* ctx_lens;
+  const int32_t* cu_rows;
+  const int32_t* starts;  // NULL: 0
+  const char* work;
+  int64_t q_token, q_head, k_row, k_head, v_row, v_head, out_token, out_head;
+  uint64_t at_rows;
+  float scale;
+  int32_t requests, tokens, window, heads, key_dim, value_dim, rows;
+};
+
+// A unit's rows: where its request's begin, how many there are, the first's
+// position.
+struct KeyRows {
+  int first, count, start;
+};
+__device__ inline KeyRows key_rows(const RowsArgs& a, int request) {
+  KeyRows k;
+  k.first = a.cu_rows[request];
+  const int end = min(a.cu_rows[request + 1], a.rows);
+  k.first = max(0, min(k.first, a.rows));
+  k.count = max(0, end - k.first);
+  k.start = a.starts ? max(-kMaxLen, min(a.starts[request], kMaxLen)) : 0;
+  return k;
+}
+
+// 128 tokens of a head to a block, 32 to a wavefront, against tiles of 32 rows that
+// all four read from LDS: the layout and the softmax of latent_attend.hpp, with a
+// head's own keys and values.
+template <class T, int DK, int DV>
+struct RowsShape {
+  static constexpr int kKeyBytes = (2 * DK + 127) / 128 * 128;  // of a row in LDS
+  static constexpr int kValueBytes = 2 * DV;
+  static constexpr int kStage = kLatentTile * (kKeyBytes + kValueBytes);
+  static constexpr int kStages = 3;
+  // direct loads of a wavefront
+  static constexpr int kKeyLoads = kLatentTile * kKeyBytes / 4096, kValueLoads = kLatentTile * kValueBytes / 4096;
+  static constexpr int kLoads = kKeyLoads + kValueLoads;
+  static constexpr int kSteps = DK / 16, kTilesD = DV / 32;
+  static constexpr bool kBf = T::code == kBF16;
+  static constexpr float kSlack = kBf ? 8.0f : 2.0f, kBias = kBf ? 0.0f : 13.0f;
+};
+
+template <class T, int DK, int DV>
+__global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
+  typedef RowsShape<T, DK, DV> S;
+  typedef LatentShape<T, 256, 32, 32, 1> L;  // chunks' places and weights' rounding
+  static_assert(S::kKeyLoads * 4096 == kLatentTile * S::kKeyBytes &&
+                    S::kValueLoads * 4096 == kLatentTile * S::kValueBytes,
+                "whole loads to a wavefront");
+  __shared__ __align__(1024) char ring[S::kStages * S::kStage];
+  __shared__ uint32_t s_bad[2];
+  const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c = lane % 32, h = lane / 32;
+  const auto* plan = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
+  // the last units of a request see most: they go first
+  const int head = static_cast<int>(blockIdx.x % a.heads);
+  const int unit = plan->row_units - 1 - static_cast<int>(blockIdx.x / a.heads);
+  if (unit < 0) return;
+  const auto* u = reinterpret_cast<ConstRowUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_rows) + unit;
+  const int tokens = u->tokens, first_pos = u->pos, unit_row = u->row;
+  if (tokens <= 0) return;
+  const KeyRows keys = key_rows(a, u->request);
+  const int last_pos = first_pos + tokens - 1;
+  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;  // (the first stage's barrier is after)
+
+  // columns: tokens; positions are counted from the rows' first
+  const bool mine = 32 * wave + c < tokens;
+  const int token = min(32 * wave + c, tokens - 1);
+  const int pos = first_pos + token - keys.start;
+  const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+  const int seen_to = min(pos, keys.count - 1);
+  const int wave_last = first_pos + min(32 * wave + 31, tokens - 1) - keys.start;
+  const int wave_first = first_pos + min(32 * wave, tokens - 1) - keys.start;
+  const int wave_from = a.window > 0 ? max(0, wave_first + 1 - a.window) : 0;
+  const int wave_all_from = a.window > 0 ? max(0, wave_last + 1 - a.window) : 0;
+  const bool busy = 32 * wave < tokens;
+  const int block_first = first_pos - keys.start;
+  const int all_from = a.window > 0 ? max(0, last_pos - keys.start + 1 - a.window) : 0;
+  const int block_from = a.window > 0 ? max(0, block_first + 1 - a.window) : 0;
+  const int tile_lo = block_from / kLatentTile;
+  const int tile_hi = (min(last_pos - keys.start + 1, keys.count) + kLatentTile - 1) / kLatentTile;
+  const int n = max(0, tile_hi - tile_lo);
+
+  auto issue = [&](int i) {
+    char* to = ring + (i % S::kStages) * S::kStage;
+    const int key0 = (tile_lo + i) * kLatentTile;
+    int lane = __lane_id();
+    asm volatile("" : "+v"(lane));  // offsets made here, not kept over the products
+#pragma unroll
+    for (int j = 0; j < S::kKeyLoads; ++j) {
+      constexpr int kChunks = S::kKeyBytes / 16;
+      const int load = wave * S::kKeyLoads + j, at = load * kWave + lane, r = at / kChunks;
+      const int chunk = (at - r * kChunks) ^ L::turn8(r);
+      // (a row's last places in LDS may be nobody's)
+      const int64_t key = keys.first + min(key0 + r, keys.count - 1);
+      __builtin_amdgcn_global_load_lds(
+          reinterpret_cast<const u32x4*>(a.k + key * a.k_row + head * a.k_head +
+                                         8 * (chunk < DK / 8 ? chunk : 0)),
+          (__attribute__((address_space(3))) void*)(to + load * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < S::kValueLoads; ++j) {
+      constexpr int kChunks = S::kValueBytes / 16;
+      const int load = wave * S::kValueLoads + j, at = load * kWave + lane, r = at / kChunks;
+      const int chunk = (at - r * kChunks) ^ L::turn8(r);
+      const int64_t key = keys.first + min(key0 + r, keys.count - 1);
+      __builtin_amdgcn_global_load_lds(
+          reinterpret_cast<const u32x4*>(a.v + key * a.v_row + head * a.v_head + 8 * chunk),
+          (__attribute__((address_space(3))) void*)(to + kLatentTile * S::kKeyBytes + load * 1024), 16, 0, 0);
+    }
+  };
+
+  u32x4 q[S::kSteps];
+  {
+    const uint16_t* from = a.q + static_cast<int64_t>(unit_row + token) * a.q_token + head * a.q_head + 8 * h;
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) q[s] = *reinterpret_cast<const u32x4*>(from + 16 * s);
+  }
+  // In registers before the rows' loads begin, so that a stage waits for rows only.
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) asm volatile("" : "+v"(q[s]));
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) {
+    if (i < n) issue(i);
+  }
+  const int key_row = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
+  const int k_at = key_row * S::kKeyBytes + 16 * (h ^ L::turn8(key_row));
+  const int i16 = lane % 16, v_row = 16 * h + i16 / 4;
+  const int v_at = kLatentTile * S::kKeyBytes + v_row * S::kValueBytes + 8 * (i16 & 1) +
+                   16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ L::turn8(v_row));
+  f32x16 o[S::kTilesD];
+#pragma unroll
+  for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f, poison = 0.0f;
+  const float mul = a.scale * kLog2e;
+
+  for (int i = 0; i < n; ++i) {
+    if (i + S::kStages - 2 < n) wait_loads<(S::kStages - 2) * S::kLoads>();
+    else wait_loads<0>();
+    block_barrier();
+    if (i + S::kStages - 1 < n) issue(i + S::kStages - 1);
+    const int key0 = (tile_lo + i) * kLatentTile;
+    char* stage = ring + (i % S::kStages) * S::kStage;
+    // Where some column does not see all rows, values that are no finite numbers
+    // (which a weight of 0 would not keep out) are taken from LDS, and the rows
+    // that had them noted.
+    const bool partly = key0 < all_from || key0 + kLatentTile - 1 > min(block_first, keys.count - 1);
+    uint32_t bad = 0;
+    if (threadIdx.x == 0) s_bad[(i + 1) & 1] = 0;  // all have read it before this stage
+    if (partly) {
+      constexpr uint32_t kLo = S::kBf ? 0x7f80u : 0x7c00u, kHi = kLo << 16;
+#pragma unroll
+      for (int at = 16 * static_cast<int>(threadIdx.x); at < kLatentTile * S::kValueBytes; at += 4096) {
+        u32x4* p = reinterpret_cast<u32x4*>(stage + kLatentTile * S::kKeyBytes + at);
+        u32x4 v = *p;
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((v[e] & kLo) == kLo) {
+            v[e] &= 0xffff0000u;
+            odd = true;
+          }
+          if ((v[e] & kHi) == kHi) {
+            v[e] &= 0xffffu;
+            odd = true;
+          }
+        }
+        if (odd) {
+          *p = v;
+          atomicOr(&s_bad[i & 1], 1u << (at / S::kValueBytes));
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+      block_barrier();
+      bad = *static_cast<volatile uint32_t*>(&s_bad[i & 1]);
+    }
+    if (!busy || key0 > wave_last || key0 + kLatentTile <= wave_from) continue;
+
+    f32x16 s;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+    in_order<S::kSteps, 4>(
+        [&](int k) { return *reinterpret_cast<const u32x4*>(stage + ((k_at ^ 32 * (k % 4)) + 128 * (k / 4))); },
+        [&](int k, u32x4 f) { s = mfma<S::kBf>(f, q[k], s); });
+    float score[16], top = -INFINITY, odd = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      score[e] = s[e];
+      odd = fmaf(s[e], 0.0f, odd);
+    }
+    const bool whole = key0 >= wave_all_from && key0 + kLatentTile - 1 <= min(wave_first, keys.count - 1);
+    if (whole && bad == 0 && !__any(odd != 0.0f)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        score[e] *= mul;
+        top = fmaxf(top, score[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = key0 + 16 * h + e;
+        const bool see = key <= seen_to && key >= seen_from;
+        const bool fine = fabsf(score[e]) <= 3.4028235e38f;
+        poison += see && (!fine || (bad >> (16 * h + e) & 1u)) ? NAN : 0.0f;
+        score[e] = see && fine ? score[e] * mul : -INFINITY;
+        top = fmaxf(top, score[e]);
+      }
+    }
+    if (__any(top > m + S::kSlack)) {
+      float m2 = fmaxf(m, top);
+      m2 = fmaxf(m2, __shfl_xor(m2, 32));
+      const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
+      if (__any(m != -INFINITY)) {
+#pragma unroll
+        for (int d = 0; d < S::kTilesD; ++d) o[d] *= keep;
+      }
+      l *= keep;
+      m = m2;
+    }
+    const float shift = S::kBias - (m == -INFINITY ? 0.0f : m);
+    u32x4 w[2];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      const float x = __builtin_amdgcn_exp2f(score[e] + shift);
+      const float y = __builtin_amdgcn_exp2f(score[e + 1] + shift);
+      l += x;
+      l += y;
+      w[e / 8][e % 8 / 2] = L::weights(x, y);
+    }
+    in_order<2 * S::kTilesD, 4>(
+        [&](int k) {
+          const int d = k / 2;
+          const char* p = stage + ((v_at ^ 64 * (d % 2)) + 128 * (d / 2) + (k % 2) * 8 * S::kValueBytes);
+          const u32x2 lo = read_transposed(p), hi = read_transposed(p + 4 * S::kValueBytes);
+          return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        },
+        [&](int k, u32x4 f) { o[k / 2] = mfma<S::kBf>(f, w[k % 2], o[k / 2]); });
+  }
+  l += __shfl_xor(l, 32);
+  poison += __shfl_xor(poison, 32);
+  l += poison;
+  if (!mine) return;
+  const float inv = 1.0f / l;
+  const bool empty = m == -INFINITY && l == 0.0f;
+  uint16_t* to = a.out + static_cast<int64_t>(unit_row + token) * a.out_token + head * a.out_head + 4 * h;
+#pragma unroll
+  for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      u32x2 v;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t lo = T::put(empty ? 0.0f : o[d][4 * k + 2 * e] * inv);
+        const uint32_t hi = T::put(empty ? 0.0f : o[d][4 * k + 2 * e + 1] * inv);
+        v[e] = lo | (hi << 16);
+      }
+      *reinterpret_cast<u32x2*>(to + 32 * d + 8 * k) = v;
+    }
+  }
+  if (a.lse && h == 0) {
+    a.lse[static_cast<int64_t>(unit_row + token) * a.heads + head] = latent_lse<T>(m, l, S::kBias);
+  }
+}
+
+// Any dims: one block to a (token, head); each of its wavefronts takes 64 rows in
+// turn, a row to a lane for the scores and eight columns to a lane for the values.
+template <class T>
+__global__ __launch_bounds__(256) void rows_any_kernel(RowsArgs a) {
+  const int row = blockIdx.x, head = blockIdx.y;
+  const int lane = __lane_id(), wave = threadIdx.x / kWave;
+  __shared__ float s_q[512];
+  __shared__ float s_p[4][kWave];
+  __shared__ float s_o[4][512];
+  __shared__ float s_m[4], s_l[4];
+  if (row >= a.cu_new[a.requests]) return;
+  const int r = last_not_past(a.cu_new, a.requests, row);
+  const KeyRows keys = key_rows(a, r);
+  const int pos = clamp_len(a.ctx_lens[r]) + row - a.cu_new[r] - keys.start;
+  const int first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+  const int last = min(pos, keys.count - 1);
+  const uint16_t* q = a.q + static_cast<int64_t>(row) * a.q_token + head * a.q_head;
+  for (int d = threadIdx.x; d < a.key_dim; d += 256) s_q[d] = T::get(q[d]);
+  __syncthreads();
+  const uint16_t* k = a.k + keys.first * a.k_row + head * a.k_head;
+  const uint16_t* v = a.v + keys.first * a.v_row + head * a.v_head;
+  float m = -INFINITY, l = 0.0f, o[8] = {};
+  for (int t0 = first / kWave * kWave + wave * kWave; t0 <= last; t0 += 4 * kWave) {
+    const int key = t0 + lane;
+    float s = -INFINITY;
+    if (key >= first && key <= last) {
+      float dot = 0.0f;
+      for (int d = 0; d < a.key_dim; d += 8) {
+        float x[8];
+        get8<T, true>(k + key * a.k_row + d, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(s_q[d + e], x[e], dot);
+      }
+      s = fabsf(dot) <= 3.4028235e38f ? dot * a.scale * kLog2e : NAN;
+    }
+    float top = s;
+    if (__any(s != s)) l = NAN;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float m2 = fmaxf(m, top);
+    if (m2 == -INFINITY) continue;
+    const float keep = __builtin_amdgcn_exp2f(m - m2);
+    m = m2;
+    const float p = s > -INFINITY ? __builtin_amdgcn_exp2f(s - m2) : 0.0f;
+    float sum = p;
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    l = l * keep + sum;
+    s_p[wave][lane] = p;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= keep;
+    if (8 * lane < a.value_dim) {
+      const int lo = max(0, first - t0), hi = min(kWave, last + 1 - t0);
+      for (int j = lo; j < hi; ++j) {
+        const float w = s_p[wave][j];
+        float x[8];
+        get8<T, true>(v + (t0 + j) * a.v_row + 8 * lane, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(w, x[e], o[e]);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  if (8 * lane < a.value_dim) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_o[wave][8 * lane + e] = o[e];
+  }
+  if (lane == 0) {
+    s_m[wave] = m;
+    s_l[wave] = l;
+  }
+  __syncthreads();
+  const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  float total = 0.0f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = s_m[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w] - top);
+    total += s_l[w] != s_l[w] ? NAN : f[w] * s_l[w];
+  }
+  uint16_t* out = a.out + static_cast<int64_t>(row) * a.out_token + head * a.out_head;
+  for (int d = threadIdx.x; d < a.value_dim; d += 256) {
+    const float x = f[0] * s_o[0][d] + f[1] * s_o[1][d] + f[2] * s_o[2][d] + f[3] * s_o[3][d];
+    out[d] = T::put(total == 0.0f ? 0.0f : x / total);
+  }
+  if (a.lse && threadIdx.x == 0) {
+    a.lse[static_cast<int64_t>(row) * a.heads + head] =
+        total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  }
+}
+
+template <class T>
+static void launch_rows(const RowsArgs& a, uint64_t units, bool scheduled, hipStream_t s) {
+  const auto grid = static_cast<unsigned>(units * a.heads);
+  if (scheduled && a.key_dim == 192 && a.value_dim == 128) rows_attend_kernel<T, 192, 128><<<grid, 256, 0, s>>>(a);
+  else if (scheduled && a.key_dim == 96 && a.value_dim == 64) rows_attend_kernel<T, 96, 64><<<grid, 256, 0, s>>>(a);
+  else if (scheduled && a.key_dim == 128 && a.value_dim == 128) rows_attend_kernel<T, 128, 128><<<grid, 256, 0, s>>>(a);
+  else rows_any_kernel<T><<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads)), 256, 0, s>>>(a);
+}
+
+}  // namespace kv
+}  // namespace grm
+
+using namespace grm::kv;
+
+extern "C" int grm_hip_latent_expand(const grm_latent_desc* c, const void* weight, int heads,
+                                     int key_dim, int value_dim, const int32_t* block_table,
+                                     int table_width, int requests, const int32_t* starts,
+                                     const int32_t* cu_rows, uint64_t rows, void* k_out, void* v_out,
+                                     void* stream) {
+  GRM_CHECK_RC(check_latent(c));
+  GRM_CHECK_RC(check_ranges(block_table, table_width, requests, starts, cu_rows, rows));
+  if (heads <= 0 || heads > 65535) return grm::fail(-1, "bad heads");
+  if (key_dim <= 0 || key_dim > 512 || key_dim % 8 != 0 || value_dim <= 0 || value_dim > 512 ||
+      value_dim % 8 != 0) {
+    return grm::fail(-1, "key_dim and value_dim must be multiples of 8, at most 512");
+  }
+  if (rows == 0) {
+    grm::clear_error();
+    return 0;
+  }
+  if (!weight || !k_out || !v_out) return grm::fail(-1, "null weight or output");
+  if (!aligned16(weight) || !aligned16(k_out) || !aligned16(v_out)) {
+    return grm::fail(-1, "weight and outputs must be 16-byte aligned");
+  }
+  ExpandArgs a{};
+  a.rows = static_cast<const uint16_t*>(c->rows);
+  a.weight = static_cast<const uint16_t*>(weight);
+  a.k = static_cast<uint16_t*>(k_out);
+  a.v = static_cast<uint16_t*>(v_out);
+  a.of = {block_table, starts, cu_rows, table_width, requests, block_log2(c->block_tokens), rows,
+          c->blocks};
+  a.rank = c->rank;
+  a.rope = c->rope;
+  a.heads = heads;
+  a.key_dim = key_dim;
+  a.value_dim = value_dim;
+  const auto s = static_cast<hipStream_t>(stream);
+  const bool bf = c->dtype == grm::kBF16;
+  const uint64_t columns = static_cast<uint64_t>(heads) * (key_dim + value_dim);
+  const uint64_t blocks = (rows + kExpandRows - 1) / kExpandRows * ((columns + kExpandCols - 1) / kExpandCols);
+  if (blocks >= 1ull << 31) return grm::fail(-1, "too many rows for so many heads");
+  if (c->rank % kExpandStep == 0) {
+    const auto grid = static_cast<unsigned>(blocks);
+    if (bf) latent_expand_kernel<BF16><<<grid, 256, 0, s>>>(a);
+    else latent_expand_kernel<F16><<<grid, 256, 0, s>>>(a);
+  } else {
+    const auto grid = static_cast<unsigned>(rows);
+    if (bf) latent_expand_any_kernel<BF16><<<grid, 256, 0, s>>>(a);
+    else latent_expand_any_kernel<F16><<<grid, 256, 0, s>>>(a);
+  }
+  GRM_HIP_CHECK(hipGetLastError());
+  grm::clear_error();
+  return 0;
+}
+
+extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work, uint64_t work_bytes,
+                                   int dtype, int key_dim, int value_dim, const void* q,
+                                   int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                   int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                                   int64_t v_row_stride, int64_t v_head_stride, uint64_t rows,
+                                   const int32_t* cu_rows, const int32_t* starts, void* out,
+                                   int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                                   float softmax_scale, void* stream) {
+  GRM_CHECK_RC(check_batch(b, true));
+  if (b->kv_heads != 1) return grm::fail(-1, "a latent cache's batch has one kv head");
+  if (dtype != grm::kBF16 && dtype != grm::kF16) return grm::fail(-1, "dense rows are BF16 or F16");
+  if (key_dim <= 0 || key_dim > 512 || key_dim % 8 != 0 || value_dim <= 0 || value_dim > 512 ||
+      value_dim % 8 != 0) {
+    return grm::fail(-1, "key_dim and value_dim must be multiples of 8, at most 512");
+  }
+  if (rows > static_cast<uint64_t>(kMaxLen)) return grm::fail(-1, "too many rows");
+  if (!(softmax_scale - softmax_scale == 0.0f)) return grm::fail(-1, "softmax_scale must be finite");
+  if (b->requests == 0 || b->tokens == 0) {
+    grm::clear_error();
+    return 0;
+  }
+  if (!q || !out || !cu_rows || (rows && (!k || !v))) return grm::fail(-1, "null array");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(k) || !aligned16(v) ||
+      (q_token_stride | q_head_stride | out_token_stride | out_head_stride | k_row_stride |
+       k_head_stride | v_row_stride | v_head_stride) % 8 != 0) {
+    return grm::fail(-1, "queries, rows and output: 16-byte aligned rows");
+  }
+  if (!work || !aligned16(work)) return grm::fail(-1, "latent work must be 16-byte aligned");
+  LatentLayout l;
+  GRM_CHECK_RC(latent_layout_of(b, &l));
+  if (work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_latent_work_bytes");
+  RowsArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.cu_new = b->cu_new;
+  a.ctx_lens = b->ctx_lens;
+  a.cu_rows = cu_rows;
+  a.starts = starts;
+  a.work = static_cast<const char*>(work);
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.k_row = k_row_stride;
+  a.k_head = k_head_stride;
+  a.v_row = v_row_stride;
+  a.v_head = v_head_stride;
+  a.out_token = out_token_stride;
+  a.out_head = out_head_stride;
+  a.at_rows = l.at_rows;
+  a.scale = softmax_scale;
+  a.requests = b->requests;
+  a.tokens = b->tokens;
+  a.window = b->window;
+  a.heads = b->heads;
+  a.key_dim = key_dim;
+  a.value_dim = value_dim;
+  a.rows = static_cast<int32_t>(rows);
+  const bool scheduled = l.cap_rows * static_cast<uint64_t>(b->heads) < (1ull << 31);
+  const auto s = static_cast<hipStream_t>(stream);
+  if (dtype == grm::kBF16) launch_rows<BF16>(a, l.cap_rows, scheduled, s);
+  else launch_rows<F16>(a, l.cap_rows, scheduled, s);
+  GRM_HIP_CHECK(hipGetLastError());
+  grm::clear_error();
+  return 0;
+}

@@ -11,7 +11,11 @@ A row holds a token's latent and its turned key part, shared by all heads::
 
 In the absorbed form a head's query is taken to the latent's space before (its
 own part times the weights that make a head's keys), and its output, a mean of
-latents, goes through the weights that make its values after.
+latents, goes through the weights that make its values after.  Prompts take less
+in the expanded form::
+
+    k, v = cache.expand(weight, key_dim, table, starts, cu_rows, rows)
+    out = attend_rows(batch, q, k, v, cu_rows)
 
 Batches, memory, streams and errors are those of ``kv_cache``; laws and layouts
 those of ``include/grm_hip_router.h``.
@@ -20,6 +24,7 @@ those of ``include/grm_hip_router.h``.
 from __future__ import annotations
 
 import ctypes
+import math
 import sys
 
 from . import _lib
@@ -220,5 +225,73 @@ class LatentCache:
             _lib.check(rc, "latent read")
         return out
 
+    def expand(self, weight, key_dim: int, block_table, starts, cu_rows, rows: int, *,
+               stream=None):
+        """A head's own keys and values, dense: (k [rows, heads, key_dim + rope],
+        v [rows, heads, dim - key_dim]) of the positions that ``read`` would give,
+        for ``weight`` [heads, dim, rank] of the cache's type, contiguous: its
+        first ``key_dim`` rows make a head's keys (before the turned part), the
+        others its values.  What prompts attend over with ``attend_rows``."""
+        if len(weight.shape) != 3:
+            raise ValueError("weight must be [heads, key_dim + value_dim, rank]")
+        heads, dim = int(weight.shape[0]), int(weight.shape[1])
+        key_dim = int(key_dim)
+        if not 0 < key_dim < dim:
+            raise ValueError(f"key_dim {key_dim} of {dim} rows a head")
+        if getattr(weight, "requires_grad", False):
+            _rows(weight, "weight", tuple(weight.shape))  # refused where gradients are recorded
+        wp = _dense(weight, "weight", self.dtype, (heads, dim, self.rank))
+        _same_device(weight, "weight", self.device)
+        at = self._ranges(block_table, starts, cu_rows, rows)
+        k = _empty(starts, (at[5], heads, key_dim + self.rope), self.dtype, stream)
+        v = _empty(starts, (at[5], heads, dim - key_dim), self.dtype, stream)
+        rc = _call(self._lib.grm_hip_latent_expand, starts, self.device, self._ref, wp, heads,
+                   key_dim, dim - key_dim, *at, k.data_ptr(), v.data_ptr(), _stream(starts, stream))
+        if rc:
+            _lib.check(rc, "latent expand")
+        return k, v
 
-__all__ = ["LatentCache"]
+
+def attend_rows(batch: KvBatch, q, k, v, cu_rows, *, starts=None,
+                softmax_scale: float | None = None, out=None, lse=None, return_lse: bool = False,
+                stream=None):
+    """Causal attention of a latent batch's queries ``q`` [tokens, heads, dk]
+    over dense rows ``k`` [rows, heads, dk] and ``v`` [rows, heads, dv] (bf16 or
+    f16, of one type), as ``LatentCache.expand`` makes them: request r's are
+    ``cu_rows[r]`` to ``cu_rows[r + 1] - 1``, the first of them its position
+    ``starts[r]`` (0 unless told).  Returns ``out`` [tokens, heads, dv] (also taken
+    as an argument), with ``return_lse`` also the fp32 [tokens, heads]
+    log-sum-exp, by which results over parts of the rows can be joined."""
+    _latent_batch(batch)
+    if not batch._planned:
+        raise ValueError("the batch has no plan yet: call plan() first")
+    d = batch._desc
+    if len(k.shape) != 3 or len(v.shape) != 3:
+        raise ValueError("k and v must be [rows, heads, dim]")
+    rows, dk, dv = int(k.shape[0]), int(k.shape[2]), int(v.shape[2])
+    name = _type(q, "q")
+    if name not in ("bf16", "f16"):
+        raise ValueError(f"q must be bf16 or f16, got {q.dtype}")
+    q, at_q = _aligned(q, "q", (d.tokens, d.heads, dk), name, stream)
+    k, at_k = _aligned(k, "k", (rows, d.heads, dk), name, stream)
+    v, at_v = _aligned(v, "v", (rows, d.heads, dv), name, stream)
+    cu = _dense(cu_rows, "cu_rows", "i32", (d.requests + 1,))
+    sp = None if starts is None else _dense(starts, "starts", "i32", (d.requests,))
+    for a, what in ((q, "q"), (k, "k"), (v, "v"), (cu_rows, "cu_rows"), (starts, "starts")):
+        if a is not None:
+            _same_device(a, what, batch.device)
+    out, to, result = _output(q, out, (d.tokens, d.heads, dv), name, batch.device, stream)
+    lse, lp = _statistics(q, lse, return_lse, (d.tokens, d.heads), batch.device, stream)
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(dk)
+    on = batch._on(q, stream)
+    rc = _call(batch._lib.grm_hip_rows_attend, q, batch.device, batch._ref, batch._latent_at,
+               batch._latent_bytes, _lib.DTYPE_CODES[name], dk, dv, *at_q, *at_k, *at_v, rows, cu,
+               sp, *to, lp, softmax_scale, on)
+    if rc:
+        _lib.check(rc, "rows attend")
+    _written(out, result, on)
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["LatentCache", "attend_rows"]

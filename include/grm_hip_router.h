@@ -711,6 +711,40 @@ int grm_hip_latent_attend(const grm_latent_desc* cache, const grm_kv_batch_desc*
                           float softmax_scale, void* scratch, uint64_t scratch_bytes,
                           void* stream);
 
+/* The expanded form.  A head's own keys and values of positions [starts[r],
+ * starts[r] + cu_rows[r + 1] - cu_rows[r]) of each request:
+ *   k_out[row][head] = [weight[head][0 .. key_dim) latent | key part],
+ *   v_out[row][head] = weight[head][key_dim .. key_dim + value_dim) latent
+ * for the cached row's latent; weight [heads][key_dim + value_dim][rank],
+ * k_out [rows][heads][key_dim + rope], v_out [rows][heads][value_dim], all
+ * contiguous, of the cache's dtype, 16-byte aligned; fp32 sums, rounded once.
+ * key_dim and value_dim are multiples of 8, at most 512.  Positions without a
+ * block give rows of 0. */
+int grm_hip_latent_expand(const grm_latent_desc* cache, const void* weight, int heads, int key_dim,
+                          int value_dim, const int32_t* block_table, int table_width, int requests,
+                          const int32_t* starts, const int32_t* cu_rows, uint64_t rows, void* k_out,
+                          void* v_out, void* stream);
+
+/* Causal attention of the step's tokens over dense rows: q [tokens][heads]
+ * [key_dim], k [rows][heads][key_dim], v [rows][heads][value_dim], out [tokens]
+ * [heads][value_dim] of dtype (BF16, F16); strides in elements, multiples of 16
+ * bytes.  Request r's rows are cu_rows[r] .. cu_rows[r + 1] - 1 (`rows` in all),
+ * the first of them position starts[r] (NULL: 0); its new token i, of position
+ * ctx_lens[r] + i, sees those up to its own and within the window.  With the
+ * lse of parts of a request's rows, parts can be joined.  key_dim and value_dim
+ * are multiples of 8, at most 512.  A value that is not finite leaves no finite
+ * result in its channel of the tokens that see its row (other channels of theirs
+ * may be NaN too), and changes no other token's.  For prompts: 128 tokens of a
+ * head go through its rows alone. */
+int grm_hip_rows_attend(const grm_kv_batch_desc* batch, const void* work, uint64_t work_bytes,
+                        int dtype, int key_dim, int value_dim, const void* q,
+                        int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                        int64_t v_row_stride, int64_t v_head_stride, uint64_t rows,
+                        const int32_t* cu_rows, const int32_t* starts, void* out,
+                        int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                        float softmax_scale, void* stream);
+
 /* ---- Synthetic workload keys (host only) --------------------------------
  * Rows [row0, row0 + rows) of the synthetic INT8 key stream: each row's dim
  * values are normal quantiles (normal_table[65536], the caller's table of

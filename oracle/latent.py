@@ -95,3 +95,42 @@ def attend(q, rows, rank, ctx, new, table, scale, window=0, out_type="bf16", hea
                     q[row, h], k, k[:, :rank], scale, UNIT[out_type], out_type, d)
             row += 1
     return out, lse, ob, lb
+
+
+def expand(rows, weight, key_dim, rank, ctx_rows, table, out_type):
+    """(k, v, bounds) of ranges [(request, first position, count)]: k [rows,
+    heads, key_dim + rope], v [rows, heads, value_dim]."""
+    w = np.asarray(weight, np.float64)
+    heads = w.shape[0]
+    got = np.concatenate([gather(rows, table[r], range(p, p + n))[0] for r, p, n in ctx_rows]
+                         + [np.zeros((0, rows.shape[2]))])
+    made = np.einsum("rc,hnc->rhn", got[:, :rank], w)
+    mass = np.einsum("rc,hnc->rhn", np.abs(got[:, :rank]), np.abs(w))
+    turned = np.repeat(got[:, None, rank:], heads, 1)
+    # products of 16-bit values are exact; `rank` fp32 additions, one rounding
+    off = mass * (rank + 2) * 2 * U32
+    bound = off + UNIT[out_type] * (np.abs(made) + off) + TINY[out_type]
+    k = np.concatenate([made[..., :key_dim], turned], -1)
+    kb = np.concatenate([bound[..., :key_dim], np.zeros_like(turned)], -1)
+    return k, made[..., key_dim:], kb, bound[..., key_dim:]
+
+
+def attend_rows(q, k, v, ctx, new, cu_rows, starts, scale, window=0, out_type="bf16", heads_of=None):
+    """(out, lse, bounds) over dense rows."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    tokens, heads, d = q.shape
+    out, lse = np.zeros((tokens, heads, v.shape[2])), np.full((tokens, heads), -np.inf)
+    ob, lb = np.zeros_like(out), np.zeros_like(lse)
+    row = 0
+    for r, (c, n) in enumerate(zip(ctx, new)):
+        a, b = cu_rows[r], cu_rows[r + 1]
+        at = starts[r] + np.arange(b - a)
+        for i in range(n):
+            see = at <= c + i
+            if window:
+                see &= at > c + i - window
+            for h in (range(heads) if heads_of is None else heads_of):
+                out[row, h], lse[row, h], ob[row, h], lb[row, h] = attend_one(
+                    q[row, h], k[a:b][see, h], v[a:b][see, h], scale, UNIT[out_type], out_type, d)
+            row += 1
+    return out, lse, ob, lb

@@ -226,3 +226,42 @@ def test_python_checks_of_latent_batches():
     ints = [fake((3,), np.int32), fake((3,), np.int32), fake((3, 4), np.int32)]
     with pytest.raises(ValueError, match="kv_heads"):
         g.KvBatch(*ints, 16, tokens=3, max_new=1, heads=4, kv_heads=2, latent=True)
+
+
+def test_bad_expanded_calls_are_refused():
+    lib = g.load()
+    c = ctypes.byref(latent_desc())
+
+    def expand(cache=c, weight=0x1000, heads=4, key=64, value=64, table=0x1000, width=4, requests=3,
+               starts=0x1000, cu=0x1000, rows=5, k=0x1000, v=0x1000):
+        return lib.grm_hip_latent_expand(cache, weight, heads, key, value, table, width, requests,
+                                         starts, cu, rows, k, v, None)
+    for kw in (dict(cache=None), dict(weight=None), dict(weight=0x1008), dict(heads=0),
+               dict(heads=65536), dict(key=0), dict(key=12), dict(key=520), dict(value=0),
+               dict(value=12), dict(value=520), dict(table=None), dict(requests=0), dict(starts=None),
+               dict(cu=None), dict(k=None), dict(v=0x1004), dict(rows=1 << 31), dict(width=-1),
+               dict(rows=1 << 29, heads=65535)):
+        assert expand(**kw) == -1, kw
+    assert expand(rows=0) == 0
+
+    def rows(batch=None, work=0x1000, dtype=1, dk=64, dv=64, q=0x1000, k=0x1000, v=0x1000, stride=64,
+             n=5, cu=0x1000, out=0x1000, scale=1.0):
+        b = batch or one_head()
+        return lib.grm_hip_rows_attend(ctypes.byref(b), work, 1 << 40, dtype, dk, dv, q, 256, 64, k,
+                                       stride, 64, v, 256, 64, n, cu, None, out, 256, 64, None, scale,
+                                       None)
+    for kw in (dict(batch=one_head(kv_heads=2)), dict(work=None), dict(work=0x1008), dict(dtype=0),
+               dict(dk=0), dict(dk=12), dict(dk=520), dict(dv=4), dict(dv=1024), dict(q=None),
+               dict(k=None), dict(v=None), dict(cu=None), dict(out=None), dict(q=0x1002),
+               dict(k=0x1008), dict(stride=60), dict(n=1 << 31), dict(scale=float("nan"))):
+        assert rows(**kw) == -1, kw
+
+
+def test_python_checks_of_the_expanded_form():
+    c = g.LatentCache(fake((4, 16, 96), np.float16), 64)
+    at = (fake((3, 4), np.int32), fake((3,), np.int32), fake((4,), np.int32), 5)
+    for weight, key in ((fake((4, 64), np.float16), 32), (fake((4, 64, 64), np.float32), 32),
+                        (fake((4, 64, 32), np.float16), 32), (fake((4, 64, 64), np.float16), 64),
+                        (fake((4, 64, 64), np.float16), 0)):
+        with pytest.raises(ValueError):
+            c.expand(weight, key, *at)
