@@ -289,28 +289,34 @@ static bool latent_cores(const grm_latent_desc* c, const grm_kv_batch_desc* b) {
          ((c->rank == 512 && c->rope == 64) || (c->rank == 256 && c->rope == 32));
 }
 
-// Blocks to a CU: what the ring's LDS allows.
-static int latent_per_cu(int rank) { return rank == 512 ? 1 : 2; }
+// Wavefronts to a block of so many columns.
+static int latent_waves(int cols) { return cols == kLatentCols ? 8 : 4; }
 
-template <class T, int R, int P, int W, int G>
+static uint64_t latent_scratch(const LatentLayout& l, int rank) {
+  return static_cast<uint64_t>(l.runs / 2 * latent_per_cu(rank, latent_waves(l.cols))) * 2 *
+         latent_part_floats(l.cols, rank) * 4;
+}
+
+template <class T, int R, int P, int W, int G, int NW>
 static void launch_cols(LatentArgs a, hipStream_t stream) {
-  constexpr int kCols = LatentShape<T, R, P, W, G>::kCols;
-  latent_attend_kernel<T, R, P, W, G><<<static_cast<unsigned>(a.runs), 256, 0, stream>>>(a);
+  typedef LatentShape<T, R, P, W, G, NW> S;
+  constexpr int kCols = S::kCols;
+  latent_attend_kernel<T, R, P, W, G, NW><<<static_cast<unsigned>(a.runs), S::kThreads, 0, stream>>>(a);
   // real columns of a unit: whole tokens'
   const int cols = std::max(1, kCols / a.heads) * a.heads;
   constexpr int kEach = 256 / (R / 4);
   const dim3 grid(static_cast<unsigned>(a.runs - 1), static_cast<unsigned>((cols + kEach - 1) / kEach));
   if (a.runs > 1) {
-    latent_join_kernel<T, R, kCols><<<grid, 256, 0, stream>>>(a, LatentShape<T, R, P, W, G>::kBias);
+    latent_join_kernel<T, R, kCols><<<grid, 256, 0, stream>>>(a, S::kBias);
   }
 }
 
 template <class T, int R, int P>
 static void launch_latent(const LatentArgs& a, int cols, hipStream_t stream) {
-  if (cols == 16) launch_cols<T, R, P, 16, 4>(a, stream);
-  else if (cols == 32) launch_cols<T, R, P, 32, 4>(a, stream);
-  else if (cols == 64) launch_cols<T, R, P, 32, 2>(a, stream);
-  else launch_cols<T, R, P, 32, 1>(a, stream);
+  if (cols == 16) launch_cols<T, R, P, 16, 4, 4>(a, stream);
+  else if (cols == 32) launch_cols<T, R, P, 16, 2, 4>(a, stream);
+  else if (cols == 64) launch_cols<T, R, P, 16, 1, 4>(a, stream);
+  else launch_cols<T, R, P, 16, 1, 8>(a, stream);
 }
 
 template <class T>
@@ -377,9 +383,7 @@ extern "C" int grm_hip_latent_attend_bytes(const grm_latent_desc* c, const grm_k
   GRM_CHECK_RC(check_latent_pair(c, b, false));
   LatentLayout l;
   GRM_CHECK_RC(latent_layout_of(b, &l));
-  *out_bytes = latent_cores(c, b) ? static_cast<uint64_t>(l.runs / 2 * latent_per_cu(c->rank)) * 2 *
-                                        latent_part_floats(l.cols, c->rank) * 4
-                                  : 0;
+  *out_bytes = latent_cores(c, b) ? latent_scratch(l, c->rank) : 0;
   grm::clear_error();
   return 0;
 }
@@ -402,16 +406,15 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
     return grm::fail(-1, "queries and output: 16-byte aligned rows");
   }
   const bool cores = latent_cores(c, b);
-  const int per = latent_per_cu(c->rank);
   if (cores && (!work || !aligned16(work))) {
     return grm::fail(-1, "latent work must be 16-byte aligned");
   }
   LatentLayout l;
   GRM_CHECK_RC(latent_layout_of(b, &l));
+  const int per = latent_per_cu(c->rank, latent_waves(l.cols));
   if (cores) {
     if (work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_latent_work_bytes");
-    const uint64_t need = static_cast<uint64_t>(l.runs / 2 * per) * 2 * latent_part_floats(l.cols, c->rank) * 4;
-    if (!scratch || !aligned16(scratch) || scratch_bytes < need) {
+    if (!scratch || !aligned16(scratch) || scratch_bytes < latent_scratch(l, c->rank)) {
       return grm::fail(-1, "scratch is smaller than grm_hip_latent_attend_bytes, or not 16-byte aligned");
     }
   }

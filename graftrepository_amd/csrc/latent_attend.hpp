@@ -18,9 +18,7 @@
 // Rows go to LDS by direct loads (no registers), a ring of four tiles, and are
 // read from there twice: as the first product's operand 16 bytes to a lane, and
 // transposed (ds_read_b64_tr_b16) as the second's.  Chunks of 16 bytes are stored
-// at c ^ f(row) of their 128, where f sends the eight rows that a quarter of a
-// wavefront reads to eight places, and the four that a transposed read takes to
-// four pairs of places: neither has a bank conflict.
+// at c ^ turn(row) of their 256, which keeps both reads free of bank conflicts.
 //
 // Layout of the products (W columns to a wavefront, lane = c + W h):
 //   S^T = K Q^T.  W = 32 (32x32x16): row 8 m + 4 h' + j is key 16 h' + 4 m + j, so
@@ -143,6 +141,11 @@ __device__ __forceinline__ u32x2 read_transposed(const char* p) {
       (__attribute__((address_space(3))) s16x4*)p));
 }
 
+// Blocks to a CU and tiles in a block's ring: what LDS and, for eight wavefronts,
+// registers allow.
+__host__ __device__ constexpr int latent_per_cu(int rank, int waves) { return rank == 256 && waves == 4 ? 2 : 1; }
+__host__ __device__ constexpr int latent_ring(int rank, int waves) { return rank == 256 && waves == 8 ? 8 : 4; }
+
 // A product's reads from LDS and what is done with each, in this order: reads run
 // AHEAD before their use, and no further (left to itself the compiler reads all
 // of them first, and spills).
@@ -159,15 +162,16 @@ __device__ __forceinline__ void in_order(Read read, Use use) {
   }
 }
 
-template <class T, int R, int P, int W, int G>
+template <class T, int R, int P, int W, int G, int NW>
 struct LatentShape {
-  static constexpr int kGroups = G;              // tiles at once
-  static constexpr int kColGroups = 4 / G;       // wavefronts that share a tile
+  static constexpr int kThreads = NW * kWave;
+  static constexpr int kColGroups = NW / G;      // wavefronts that share a tile
   static constexpr int kCols = W * kColGroups;
   static constexpr int kRowBytes = 2 * (R + P);
   static constexpr int kTileBytes = kLatentTile * kRowBytes;
-  static constexpr int kStages = 4 / G;          // of the ring, G tiles each
-  static constexpr int kLds = 4 * kTileBytes;
+  static constexpr int kRing = latent_ring(R, NW);
+  static constexpr int kStages = kRing / G;      // of the ring, G tiles each
+  static constexpr int kLds = kRing * kTileBytes;
   static constexpr int kH = kWave / W;           // lanes of a column
   static constexpr int kStep = 8 * kH;           // values to an instruction
   static constexpr int kLatSteps = R / kStep, kKeySteps = P / kStep;
@@ -199,14 +203,17 @@ struct LatentShape {
     }
   }
 
-  // where a row's chunks are turned to
-  static __device__ __forceinline__ int turn8(int row) {
-    return 2 * (row & 3) + ((W == 32 ? row >> 4 : row >> 3) & 1);
+  // Where a row's chunks of 16 bytes go: chunk c of 256 bytes to c ^ turn(row).  A
+  // 16-byte read is served 16 lanes at a time (0-3, 12-15, 20-23, 24-27; 4-11, 16-19,
+  // 28-31; and so on), a transposed one 32: either finds all 64 banks.
+  static __device__ __forceinline__ int turn_low(int row) {
+    return W == 32 ? row >> 2 & 3 : -(row >> 3) & 3;
   }
-  static __device__ __forceinline__ int turn4(int row) {  // key parts of 64 bytes
-    return ((row >> 1) & 1) + 2 * ((W == 32 ? row >> 4 : row >> 3) & 1);
+  // rows of Bytes (64, 128 or whole 256)
+  template <int Bytes>
+  static __device__ __forceinline__ int turn(int row) {
+    return turn_low(row) + (Bytes % 256 == 0 ? 4 * (row & 3) : Bytes % 128 == 0 ? 4 * (row >> 1 & 1) : 0);
   }
-  static __device__ __forceinline__ int turn_key(int row) { return P == 32 ? turn4(row) : turn8(row); }
 };
 
 template <class T>
@@ -235,12 +242,12 @@ __host__ __device__ constexpr size_t latent_part_floats(int cols, int rank) {
   return static_cast<size_t>(cols) * (rank + 2);
 }
 
-template <class T, int R, int P, int W, int G>
-__global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(LatentArgs a) {
-  typedef LatentShape<T, R, P, W, G> S;
+template <class T, int R, int P, int W, int G, int NW>
+__global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void latent_attend_kernel(LatentArgs a) {
+  typedef LatentShape<T, R, P, W, G, NW> S;
   typedef typename S::Acc Acc;
   __shared__ __align__(1024) char ring[S::kLds];
-  __shared__ float s_m[4][W], s_l[4][W];
+  __shared__ float s_m[NW][W], s_l[NW][W];
   __shared__ int s_odd;
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % W, h = lane / W;
@@ -265,13 +272,13 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
   // ---- lane offsets into a tile
   // first product: row of this lane's key
   const int key_row = W == 32 ? 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3) : 8 * (c >> 2) + (c & 3);
-  const int k_at = key_row * 2 * R + 16 * (h ^ S::turn8(key_row));
-  const int p_at = kLatentTile * 2 * R + key_row * 2 * P + 16 * (h ^ S::turn_key(key_row));
+  const int k_lane = key_row * 2 * R + 16 * (h ^ S::template turn<2 * R>(key_row));
+  const int p_lane = kLatentTile * 2 * R + key_row * 2 * P + 16 * (h ^ S::template turn<2 * P>(key_row));
   // second product: a lane of 16 names four columns of a row
   const int i16 = lane % 16;
   const int v_row = W == 32 ? 16 * h + i16 / 4 : 8 * h + i16 / 4;
-  const int v_at = v_row * 2 * R + 8 * (i16 & 1) +
-                   16 * (((W == 32 ? 2 * (lane >> 4 & 1) : 0) + (i16 % 4 >> 1)) ^ S::turn8(v_row));
+  const int v_lane = v_row * 2 * R + 8 * (i16 & 1) +
+                   16 * (((W == 32 ? 2 * (lane >> 4 & 1) : 0) + (i16 % 4 >> 1)) ^ S::template turn<2 * R>(v_row));
 
   for (int64_t at = begin; at < end; ++u) {
     const int64_t first = firsts[u], last = firsts[u + 1];
@@ -336,7 +343,7 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
       for (int i = 0; i < S::kLatLoads; ++i) {
         const int row = row0 + i * S::kLatRows;                      // of the load
         const int r = row + lane / (64 / S::kLatRows), chunk = lane % (64 / S::kLatRows);
-        const uint32_t off = (r & 15) * S::kRowBytes + 16 * (chunk ^ S::turn8(r));
+        const uint32_t off = (r & 15) * S::kRowBytes + 16 * (chunk ^ S::template turn<2 * R>(r));
         __builtin_amdgcn_global_load_lds(
             reinterpret_cast<const u32x4*>(base[S::kRowsEach == 32 ? i * S::kLatRows / 16 : row / 16] + off),
             (__attribute__((address_space(3))) void*)(to + row * 2 * R), 16, 0, 0);
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
         const int row = (row0 / S::kKeyRows + i) * S::kKeyRows;
         constexpr int kChunks = 2 * P / 16;
         const int r = row + lane / kChunks, chunk = lane % kChunks;
-        const uint32_t off = (r & 15) * S::kRowBytes + 2 * R + 16 * (chunk ^ S::turn_key(r));
+        const uint32_t off = (r & 15) * S::kRowBytes + 2 * R + 16 * (chunk ^ S::template turn<2 * P>(r));
         __builtin_amdgcn_global_load_lds(
             reinterpret_cast<const u32x4*>(base[S::kRowsEach == 32 ? i * S::kKeyRows / 16 : row / 16] + off),
             (__attribute__((address_space(3))) void*)(to + kLatentTile * 2 * R + row * 2 * P), 16, 0, 0);
@@ -366,12 +373,12 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
       }
     }
     // In registers before the rows' loads begin, so that a stage waits for rows only.
-    // At rank 512 they live in AGPRs, where the matrix instructions read them, and
+    // At rank 512, with four wavefronts, they live in AGPRs, where the matrix instructions read them, and
     // leave the VGPRs to the sums (this file is built with the MFMA
     // VGPR-accumulator form).
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s) {
-      if constexpr (R == 512) asm volatile("" : "+a"(q[s]));
+      if constexpr (R == 512 && NW == 4) asm volatile("" : "+a"(q[s]));
       else asm volatile("" : "+v"(q[s]));
     }
     asm volatile("" ::: "memory");
@@ -422,7 +429,7 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
       return tile * kLatentTile < all_from || (tile + G) * kLatentTile - 1 > first_pos;
     };
     auto keep_finite = [&](int i, bool odd) {
-      if constexpr (G < 4) {
+      if constexpr (S::kColGroups > 1) {
         if (odd && lane == 0) s_odd = 1;
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
         block_barrier();
@@ -448,7 +455,7 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
         *reinterpret_cast<u32x4*>(rows + at) = v;
       }
       __builtin_amdgcn_s_waitcnt(0xc07f);
-      if constexpr (G < 4) block_barrier();
+      if constexpr (S::kColGroups > 1) block_barrier();
       else asm volatile("" ::: "memory");
     };
     if (!busy) {  // brings its rows
@@ -464,6 +471,9 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
       there &= ~(3u << (2 * slot));
       const int tile = tile_lo + group + G * i;
       const char* from = ring + (slot * G + group) * S::kTileBytes;
+      // (what follows from these is made for each tile, not kept beside the sums)
+      int k_at = k_lane, p_at = p_lane, v_at = v_lane;
+      asm volatile("" : "+v"(k_at), "+v"(p_at));
 
       // scores
       Acc s[S::kRowTiles];
@@ -473,14 +483,15 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
         for (int e = 0; e < S::kAcc; ++e) s[r][e] = 0.0f;
       }
       auto key_chunk = [&](int step, int r) {
-        // a step is 16 kH bytes of a row; steps of 128 bytes on have a constant
-        // distance
-        constexpr int kIn = 8 / S::kH;  // steps to 128 bytes
+        // a step is 16 kH bytes of a row; steps of 256 bytes (128 of short rows) on
+        // have a constant distance
         if (step < S::kLatSteps) {
+          constexpr int kIn = 16 / S::kH;
           return *reinterpret_cast<const u32x4*>(
-              from + ((k_at ^ (16 * S::kH * (step % kIn))) + 128 * (step / kIn) + r * 4 * 2 * R));
+              from + ((k_at ^ (16 * S::kH * (step % kIn))) + 256 * (step / kIn) + r * 4 * 2 * R));
         }
         const int k = step - S::kLatSteps;
+        constexpr int kIn = 8 / S::kH;
         return *reinterpret_cast<const u32x4*>(
             from + ((p_at ^ (16 * S::kH * (k % kIn))) + 128 * (k / kIn) + r * 4 * 2 * P));
       };
@@ -543,12 +554,15 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
         w[e / 8][e % 8 / 2] = S::weights(x, y);
       }
       // values
+      asm volatile("" : "+v"(v_at));
       auto value_chunk = [&](int d, int k) {
-        // W = 32: two value tiles to 128 bytes, 8 keys on from 16 h + 8 k; W = 16:
-        // four tiles to 128 bytes
-        constexpr int kIn = 64 / W;
-        const char* p = from + ((v_at ^ (2 * W * (d % kIn))) + 128 * (d / kIn) + k * 8 * 2 * R);
-        const u32x2 lo = read_transposed(p), hi = read_transposed(p + 4 * 2 * R);
+        // 128 / W value tiles to 256 bytes; W = 32: 8 keys on from 16 h + 8 k
+        constexpr int kIn = 128 / W;
+        auto four = [&](int t) {  // keys 4 t on of the eight
+          return read_transposed(from + ((v_at ^ (2 * W * (d % kIn) + (W == 32 ? 16 * (2 * k + t) : 0))) +
+                                         256 * (d / kIn) + (8 * k + 4 * t) * 2 * R));
+        };
+        const u32x2 lo = four(0), hi = four(1);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
       in_order<S::kTilesD * (S::kPer / 8), 4>(
@@ -583,7 +597,7 @@ __global__ __launch_bounds__(256, R == 256 ? 2 : 1) void latent_attend_kernel(La
       m = top;
       l = total;
       constexpr int kVecs = S::kAcc / 4;
-      constexpr int kAt = S::kLds / (4 * kWave * 16 * kVecs);          // value tiles at once
+      constexpr int kAt = S::kLds / (NW * kWave * 16 * kVecs);         // value tiles at once
       constexpr int kTiles = kAt / G * G < S::kTilesD ? kAt / G * G : S::kTilesD;
       static_assert(kTiles > 0 && S::kTilesD % kTiles == 0, "whole rounds");
       f32x4* box = reinterpret_cast<f32x4*>(ring);

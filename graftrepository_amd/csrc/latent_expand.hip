@@ -24,9 +24,9 @@ struct ExpandArgs {
 
 // 128 rows x 256 columns to a block, 64 x 128 to a wavefront, 32 of the rank a
 // stage; three stages of direct loads in LDS, two blocks to a CU, so that one's
-// stores run beside the other's products.  Chunks of 16 bytes are stored at c ^ (row >> 1
-// & 3) of their 64: eight rows' chunk c lie in eight places.  Results leave
-// through LDS, 16 bytes to a lane.
+// stores run beside the other's products.  Chunks of 16 bytes are stored at c ^ (row >> 3
+// & 3) of their 64: the 16 rows that are read at once lie in all banks.  Results
+// leave through LDS, 16 bytes to a lane.
 constexpr int kExpandRows = 128, kExpandCols = 256, kExpandStep = 32, kExpandStages = 3;
 constexpr int kExpandStage = (kExpandRows + kExpandCols) * kExpandStep * 2;  // bytes
 constexpr int kExpandOut = kExpandCols * 2 + 16;                             // of a row on its way out
@@ -50,17 +50,17 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(ExpandArgs a) {
   }
   __syncthreads();
   // loads of 16 rows by four chunks: two of cache rows, four of weights
-  const int r16 = lane / 4, chunk = (lane % 4) ^ (r16 >> 1 & 3);
+  const int r16 = lane / 4, chunk = (lane % 4) ^ (r16 >> 3);  // of an even load
   const uint16_t* from[6];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t row = s_row[(2 * wave + i) * 16 + r16];
-    from[i] = (row >= 0 ? a.rows + row * values : reinterpret_cast<const uint16_t*>(latent_zeros)) + 8 * chunk;
+    from[i] = (row >= 0 ? a.rows + row * values : reinterpret_cast<const uint16_t*>(latent_zeros)) + 8 * (chunk ^ 2 * i);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int n = min(col0 + (4 * wave + i) * 16 + r16, columns - 1);
-    from[2 + i] = a.weight + static_cast<int64_t>(n) * a.rank + 8 * chunk;
+    from[2 + i] = a.weight + static_cast<int64_t>(n) * a.rank + 8 * (chunk ^ 2 * (i & 1));
   }
   auto issue = [&](int step) {
     char* to = lds + (step % kExpandStages) * kExpandStage;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(ExpandArgs a) {
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     }
   }
-  const int at = c * 64 + 16 * (h ^ (c >> 1 & 3));
+  const int at = c * 64 + 16 * (h ^ (c >> 3 & 3));
   for (int s = 0; s < steps; ++s) {
     if (s + 1 < steps) wait_loads<6>();
     else wait_loads<0>();
@@ -238,7 +238,7 @@ struct RowsShape {
 template <class T, int DK, int DV>
 __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   typedef RowsShape<T, DK, DV> S;
-  typedef LatentShape<T, 256, 32, 32, 1> L;  // chunks' places and weights' rounding
+  typedef LatentShape<T, 256, 32, 32, 1, 4> L;  // chunks' places and weights' rounding
   static_assert(S::kKeyLoads * 4096 == kLatentTile * S::kKeyBytes &&
                     S::kValueLoads * 4096 == kLatentTile * S::kValueBytes,
                 "whole loads to a wavefront");
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     for (int j = 0; j < S::kKeyLoads; ++j) {
       constexpr int kChunks = S::kKeyBytes / 16;
       const int load = wave * S::kKeyLoads + j, at = load * kWave + lane, r = at / kChunks;
-      const int chunk = (at - r * kChunks) ^ L::turn8(r);
+      const int chunk = (at - r * kChunks) ^ L::template turn<S::kKeyBytes>(r);
       // (a row's last places in LDS may be nobody's)
       const int64_t key = keys.first + min(key0 + r, keys.count - 1);
       __builtin_amdgcn_global_load_lds(
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     for (int j = 0; j < S::kValueLoads; ++j) {
       constexpr int kChunks = S::kValueBytes / 16;
       const int load = wave * S::kValueLoads + j, at = load * kWave + lane, r = at / kChunks;
-      const int chunk = (at - r * kChunks) ^ L::turn8(r);
+      const int chunk = (at - r * kChunks) ^ L::template turn<S::kValueBytes>(r);
       const int64_t key = keys.first + min(key0 + r, keys.count - 1);
       __builtin_amdgcn_global_load_lds(
           reinterpret_cast<const u32x4*>(a.v + key * a.v_row + head * a.v_head + 8 * chunk),
@@ -320,10 +320,10 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     if (i < n) issue(i);
   }
   const int key_row = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
-  const int k_at = key_row * S::kKeyBytes + 16 * (h ^ L::turn8(key_row));
+  const int k_at = key_row * S::kKeyBytes + 16 * (h ^ L::template turn<S::kKeyBytes>(key_row));
   const int i16 = lane % 16, v_row = 16 * h + i16 / 4;
   const int v_at = kLatentTile * S::kKeyBytes + v_row * S::kValueBytes + 8 * (i16 & 1) +
-                   16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ L::turn8(v_row));
+                   16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ L::template turn<S::kValueBytes>(v_row));
   f32x16 o[S::kTilesD];
 #pragma unroll
   for (int d = 0; d < S::kTilesD; ++d) {
@@ -379,7 +379,10 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.0f;
     in_order<S::kSteps, 4>(
-        [&](int k) { return *reinterpret_cast<const u32x4*>(stage + ((k_at ^ 32 * (k % 4)) + 128 * (k / 4))); },
+        [&](int k) {
+          constexpr int kIn = S::kKeyBytes % 256 == 0 ? 8 : 4;  // steps to whole turns
+          return *reinterpret_cast<const u32x4*>(stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
+        },
         [&](int k, u32x4 f) { s = mfma<S::kBf>(f, q[k], s); });
     float score[16], top = -INFINITY, odd = 0.0f;
 #pragma unroll
@@ -429,8 +432,13 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     in_order<2 * S::kTilesD, 4>(
         [&](int k) {
           const int d = k / 2;
-          const char* p = stage + ((v_at ^ 64 * (d % 2)) + 128 * (d / 2) + (k % 2) * 8 * S::kValueBytes);
-          const u32x2 lo = read_transposed(p), hi = read_transposed(p + 4 * S::kValueBytes);
+          constexpr int kIn = S::kValueBytes % 256 == 0 ? 4 : 2;
+          auto four = [&](int t) {  // keys 4 t on of the eight
+            const int x = 2 * (k % 2) + t;
+            return read_transposed(stage + ((v_at ^ (64 * (d % kIn) + 16 * x)) + 64 * (d / kIn * kIn) +
+                                            4 * x * S::kValueBytes));
+          };
+          const u32x2 lo = four(0), hi = four(1);
           return u32x4{lo[0], lo[1], hi[0], hi[1]};
         },
         [&](int k, u32x4 f) { o[k / 2] = mfma<S::kBf>(f, w[k % 2], o[k / 2]); });
