@@ -14,8 +14,18 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
   const uint64_t busy = std::min(rows, reqs);
   const int64_t most = static_cast<int64_t>(std::max(1, b->max_new)) * b->heads;
   l.cols = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : kLatentCols;
-  l.unit_tokens = std::max(1, l.cols / b->heads);
-  l.runs = 2 * cus;  // at most
+  l.slices = 1;
+  // One token of many heads: two blocks with half of them each leave half the parts
+  // (and read the rows twice, the second time from L2).
+  if (l.cols == kLatentCols && b->max_new <= 0) {
+    l.cols /= 2;
+    l.slices = 2;
+  }
+  l.unit_tokens = std::max(1, l.cols * l.slices / b->heads);
+  for (int k = 0; k < 2; ++k) {
+    l.runs[k] = std::max(1, (k + 1) * cus / l.slices);
+    l.starts[k] = (l.runs[k] + 7) / 8 * 8;
+  }
   l.cap_units = rows / l.unit_tokens + busy;
   l.cap_rows = rows / kRowUnit + busy;
   l.reach = static_cast<int32_t>(std::min<int64_t>(
@@ -28,7 +38,9 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
   place(sizeof(LatentHead));
   l.at_units = place(l.cap_units * sizeof(LatentUnit));
   l.at_first = place((l.cap_units + 1) * 8);
-  l.at_runs = place(2 * static_cast<uint64_t>(l.runs) * 4);
+  for (int k = 0; k < 2; ++k) {
+    l.at_starts[k] = place(static_cast<uint64_t>(l.starts[k]) * sizeof(LatentStart));
+  }
   l.at_unit_scan = place((reqs + 1) * 4);
   l.at_row_scan = place((reqs + 1) * 4);
   l.at_rows = place(l.cap_rows * sizeof(RowUnit));
@@ -47,8 +59,8 @@ struct LatentPlanArgs {
   const int32_t* cu_new;
   char* work;
   int32_t requests, tokens, window, reach, unit_tokens, cap_units, cap_rows;
-  int32_t runs[2];
-  uint64_t at_units, at_first, at_runs, at_unit_scan, at_row_scan, at_rows;
+  int32_t runs[2], starts[2];
+  uint64_t at_units, at_first, at_starts[2], at_unit_scan, at_row_scan, at_rows;
 };
 
 // Exclusive sum over the block; the total in *sum.  Two barriers.
@@ -158,17 +170,38 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
   }
   if (tid == 0) {
     firsts[n_units] = tiles;
-    head->tiles = tiles;
     head->units = n_units;
     head->row_units = n_rows;
   }
   __syncthreads();  // the lists are read back by other threads of this block
-  // The unit that each run begins in.
   for (int k = 0; k < 2; ++k) {
-    const LongDeal deal(tiles, a.runs[k]);
-    int* to = reinterpret_cast<int*>(a.work + a.at_runs) + k * a.runs[1];
-    for (int r = tid; r < a.runs[k]; r += kPlanThreads) {
-      to[r] = r < deal.used ? last_of(firsts, n_units, deal.begin(r)) : 0;
+    LatentDeal deal;
+    const int64_t most = (tiles + kLatentLeast - 1) / kLatentLeast;
+    deal.used = static_cast<int>(min(most, static_cast<int64_t>(a.runs[k])));
+    deal.each = deal.used ? tiles / deal.used : 0;
+    deal.rem = deal.used ? static_cast<int>(tiles - deal.each * deal.used) : 0;
+    if (tid == 0) head->deal[k] = deal;
+    auto* to = reinterpret_cast<LatentStart*>(a.work + a.at_starts[k]);
+    for (int i = tid; i < a.starts[k]; i += kPlanThreads) {
+      // neighbouring runs to one XCD, to which every eighth entry goes
+      const int xcd = i % 8, nth = i / 8;
+      LatentStart s{};
+      s.run = -1;
+      if (nth < deal.used / 8 + (xcd < deal.used % 8)) {
+        s.run = xcd * (deal.used / 8) + min(xcd, deal.used % 8) + nth;
+        s.begin = deal.begin(s.run);
+        s.end = deal.begin(s.run + 1);
+        s.unit = last_of(firsts, n_units, s.begin);
+        s.first = firsts[s.unit];
+        s.last = firsts[s.unit + 1];
+        const LatentUnit u = units[s.unit];
+        s.request = u.request;
+        s.row = u.row;
+        s.tokens = u.tokens;
+        s.pos = u.pos;
+        s.tile_lo = u.tile_lo;
+      }
+      to[i] = s;
     }
   }
 }
@@ -289,34 +322,34 @@ static bool latent_cores(const grm_latent_desc* c, const grm_kv_batch_desc* b) {
          ((c->rank == 512 && c->rope == 64) || (c->rank == 256 && c->rope == 32));
 }
 
-// Wavefronts to a block of so many columns.
-static int latent_waves(int cols) { return cols == kLatentCols ? 8 : 4; }
+// Wavefronts to a block of so many columns, and blocks to a CU.
+static int latent_waves(int rank, int cols) { return cols == kLatentCols || (rank == 512 && cols == 64) ? 8 : 4; }
+static int latent_per(const LatentLayout& l, int rank) { return latent_per_cu(rank, latent_waves(rank, l.cols)); }
 
 static uint64_t latent_scratch(const LatentLayout& l, int rank) {
-  return static_cast<uint64_t>(l.runs / 2 * latent_per_cu(rank, latent_waves(l.cols))) * 2 *
+  return static_cast<uint64_t>(l.runs[latent_per(l, rank) - 1]) * 2 * l.slices *
          latent_part_floats(l.cols, rank) * 4;
 }
 
 template <class T, int R, int P, int W, int G, int NW>
-static void launch_cols(LatentArgs a, hipStream_t stream) {
+static void launch_cols(const LatentArgs& a, uint64_t units, hipStream_t stream) {
   typedef LatentShape<T, R, P, W, G, NW> S;
-  constexpr int kCols = S::kCols;
-  latent_attend_kernel<T, R, P, W, G, NW><<<static_cast<unsigned>(a.runs), S::kThreads, 0, stream>>>(a);
+  const auto blocks = static_cast<unsigned>((a.runs + 7) / 8 * 8 * a.slices);
+  latent_attend_kernel<T, R, P, W, G, NW><<<blocks, S::kThreads, 0, stream>>>(a);
   // real columns of a unit: whole tokens'
-  const int cols = std::max(1, kCols / a.heads) * a.heads;
-  constexpr int kEach = 256 / (R / 4);
-  const dim3 grid(static_cast<unsigned>(a.runs - 1), static_cast<unsigned>((cols + kEach - 1) / kEach));
-  if (a.runs > 1) {
-    latent_join_kernel<T, R, kCols><<<grid, 256, 0, stream>>>(a, S::kBias);
-  }
+  const int cols = std::max(1, S::kCols * a.slices / a.heads) * a.heads;
+  const bool by_unit = units < static_cast<uint64_t>(a.runs - 1);
+  const dim3 grid(by_unit ? static_cast<unsigned>(units) : static_cast<unsigned>(a.runs - 1),
+                  static_cast<unsigned>((cols + 15) / 16), R / 64);
+  if (a.runs > 1) latent_join_kernel<T, R, S::kCols><<<grid, 256, 0, stream>>>(a, S::kBias, by_unit);
 }
 
 template <class T, int R, int P>
-static void launch_latent(const LatentArgs& a, int cols, hipStream_t stream) {
-  if (cols == 16) launch_cols<T, R, P, 16, 4, 4>(a, stream);
-  else if (cols == 32) launch_cols<T, R, P, 16, 2, 4>(a, stream);
-  else if (cols == 64) launch_cols<T, R, P, 16, 1, 4>(a, stream);
-  else launch_cols<T, R, P, 16, 1, 8>(a, stream);
+static void launch_latent(const LatentArgs& a, int cols, uint64_t units, hipStream_t stream) {
+  if (cols == 16) launch_cols<T, R, P, 16, 4, 4>(a, units, stream);
+  else if (cols == 32) launch_cols<T, R, P, 16, 2, 4>(a, units, stream);
+  else if (cols == 64) launch_cols<T, R, P, 16, R == 512 ? 2 : 1, R == 512 ? 8 : 4>(a, units, stream);
+  else launch_cols<T, R, P, 16, 1, 8>(a, units, stream);
 }
 
 template <class T>
@@ -363,11 +396,13 @@ extern "C" int grm_hip_latent_plan(const grm_kv_batch_desc* b, void* work, uint6
   a.unit_tokens = l.unit_tokens;
   a.cap_units = static_cast<int32_t>(l.cap_units);
   a.cap_rows = static_cast<int32_t>(l.cap_rows);
-  a.runs[0] = l.runs / 2;
-  a.runs[1] = l.runs;
+  for (int k = 0; k < 2; ++k) {
+    a.runs[k] = l.runs[k];
+    a.starts[k] = l.starts[k];
+    a.at_starts[k] = l.at_starts[k];
+  }
   a.at_units = l.at_units;
   a.at_first = l.at_first;
-  a.at_runs = l.at_runs;
   a.at_unit_scan = l.at_unit_scan;
   a.at_row_scan = l.at_row_scan;
   a.at_rows = l.at_rows;
@@ -411,7 +446,7 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
   }
   LatentLayout l;
   GRM_CHECK_RC(latent_layout_of(b, &l));
-  const int per = latent_per_cu(c->rank, latent_waves(l.cols));
+  const int per = latent_per(l, c->rank);
   if (cores) {
     if (work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_latent_work_bytes");
     if (!scratch || !aligned16(scratch) || scratch_bytes < latent_scratch(l, c->rank)) {
@@ -435,7 +470,7 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
   a.blocks = c->blocks;
   a.at_units = l.at_units;
   a.at_first = l.at_first;
-  a.at_runs = l.at_runs + (per == 2 ? static_cast<uint64_t>(l.runs) * 4 : 0);
+  a.at_starts = l.at_starts[per - 1];
   a.scale = softmax_scale;
   a.requests = b->requests;
   a.width = b->table_width;
@@ -445,18 +480,20 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
   a.rank = c->rank;
   a.rope = c->rope;
   a.block_log2 = block_log2(c->block_tokens);
-  a.runs = l.runs / 2 * per;
+  a.runs = l.runs[per - 1];
+  a.slices = l.slices;
+  a.per = per;
   const auto s = static_cast<hipStream_t>(stream);
   const bool bf = c->dtype == grm::kBF16;
   if (!cores) {
     if (bf) launch_latent_any<BF16>(a, s);
     else launch_latent_any<F16>(a, s);
   } else if (c->rank == 512) {
-    if (bf) launch_latent<BF16, 512, 64>(a, l.cols, s);
-    else launch_latent<F16, 512, 64>(a, l.cols, s);
+    if (bf) launch_latent<BF16, 512, 64>(a, l.cols, l.cap_units, s);
+    else launch_latent<F16, 512, 64>(a, l.cols, l.cap_units, s);
   } else {
-    if (bf) launch_latent<BF16, 256, 32>(a, l.cols, s);
-    else launch_latent<F16, 256, 32>(a, l.cols, s);
+    if (bf) launch_latent<BF16, 256, 32>(a, l.cols, l.cap_units, s);
+    else launch_latent<F16, 256, 32>(a, l.cols, l.cap_units, s);
   }
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();

@@ -45,11 +45,23 @@ constexpr int kLatentCols = 128;    // columns to a unit, at most
 constexpr int kLatentLeast = 4;     // tiles to a run, at least
 constexpr int kRowUnit = 128;       // tokens to a unit of attention over dense rows
 
+// Tiles dealt to runs, equal to within one, kLatentLeast at least: `used` runs, of
+// which the first `rem` have one more than `each`.
+struct LatentDeal {
+  int64_t each;
+  int32_t used, rem;
+  __device__ int64_t begin(int r) const { return r * each + (r < rem ? r : rem); }
+  __device__ int run(int64_t t) const {
+    const int64_t more = rem * (each + 1);
+    return static_cast<int>(t < more ? t / (each + 1) : rem + (t - more) / each);
+  }
+};
+
 struct LatentHead {
-  int64_t tiles;      // of all units
+  LatentDeal deal[2];  // with one and two blocks to a CU
   int32_t units;
   int32_t row_units;
-  int32_t pad[12];
+  int32_t pad[6];
 };
 static_assert(sizeof(LatentHead) == 64, "the lists behind it stay aligned");
 
@@ -62,38 +74,31 @@ struct RowUnit {
   int32_t request, row, tokens, pos;
 };
 
+// What a block begins with, in the order of the blocks: its run's tiles, and the
+// first unit's.
+struct LatentStart {
+  int32_t run, unit;  // run -1: nothing to do
+  int32_t request, row, tokens, pos, tile_lo, pad;
+  int64_t begin, end, first, last;
+};
+static_assert(sizeof(LatentStart) == 64, "one line");
+
 typedef const __attribute__((address_space(4))) LatentHead* ConstLatentHead;
 typedef const __attribute__((address_space(4))) LatentUnit* ConstLatentUnit;
+typedef const __attribute__((address_space(4))) LatentStart* ConstLatentStart;
 typedef const __attribute__((address_space(4))) RowUnit* ConstRowUnit;
 typedef const __attribute__((address_space(4))) int64_t* ConstLong;
-
-// Tiles dealt to runs, equal to within one, kLatentLeast at least.
-struct LongDeal {
-  int64_t tiles, each;
-  int used, rem;
-  __host__ __device__ LongDeal(int64_t tiles_, int runs) : tiles(tiles_) {
-    const int64_t most = (tiles + kLatentLeast - 1) / kLatentLeast;
-    used = static_cast<int>(most < runs ? most : runs);
-    each = used ? tiles / used : 0;
-    rem = used ? static_cast<int>(tiles - each * used) : 0;
-  }
-  __host__ __device__ int64_t begin(int r) const {
-    return r >= used ? tiles : r * each + (r < rem ? r : rem);
-  }
-  __host__ __device__ int run(int64_t t) const {
-    const int64_t more = rem * (each + 1);
-    return static_cast<int>(t < more ? t / (each + 1) : rem + (t - more) / each);
-  }
-};
 
 // Sizes and places of the latent schedule, from host-known fields alone.
 struct LatentLayout {
   int cols;          // columns to a block: 16, 32, 64 or 128
+  int slices;        // blocks that share a unit's columns
   int unit_tokens;   // tokens to a unit
-  int runs;
+  int runs[2];       // with one and two blocks to a CU
+  int starts[2];     // entries of the list that blocks begin with
   uint64_t cap_units, cap_rows;
   int32_t reach;
-  uint64_t at_units, at_first, at_runs, at_unit_scan, at_row_scan, at_rows, bytes;
+  uint64_t at_units, at_first, at_starts[2], at_unit_scan, at_row_scan, at_rows, bytes;
 };
 
 int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out);
@@ -109,9 +114,10 @@ struct LatentArgs {
   const char* work;
   float* parts;
   int64_t q_token, q_head, out_token, out_head;  // strides
-  uint64_t blocks, at_units, at_first, at_runs;
+  uint64_t blocks, at_units, at_first, at_starts;
   float scale;
-  int32_t requests, width, tokens, window, heads, rank, rope, block_log2, runs;
+  int32_t requests, width, tokens, window, heads, rank, rope, block_log2;
+  int32_t runs, slices, per;  // per: blocks to a CU
 };
 
 // Rows of nobody: what a tile has where there is no block.  Written by no one.
@@ -130,6 +136,24 @@ __device__ __forceinline__ void block_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+
+// Sixteen bytes a lane from `base` + off straight to LDS, lane after lane from `to`
+// on.  Spelt out: before any read of LDS that follows one, the compiler waits for all
+// direct loads that it knows of, also those of a later stage, and a ring of stages
+// is then worth one (its own counts of loads are only too cautious for these).  What
+// reads the stage waits by wait_loads and a barrier.
+typedef __attribute__((address_space(3))) char* LdsPointer;
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsPointer)p));
+}
+__device__ __forceinline__ void load_direct(const char* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               : : "s"(to), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void load_direct(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               : : "s"(to), "v"(from) : "memory", "m0");
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -187,6 +211,7 @@ struct LatentShape {
   static constexpr int kLatLoads = kRowsEach / kLatRows;
   static constexpr int kKeyLoads = kRowsEach > kKeyRows ? kRowsEach / kKeyRows : 1;
   static constexpr int kLoads = kLatLoads + kKeyLoads;
+  static constexpr int kAhead = R == 512 && NW == 8 ? 4 : 8;  // reads from LDS before their use
   static constexpr bool kBf = T::code == kBF16;
   // Columns may pass their reference by 2^kSlack before the sums are scaled.
   static constexpr float kSlack = kBf ? 8.0f : 2.0f;
@@ -216,12 +241,9 @@ struct LatentShape {
   }
 };
 
+// Four values of a finished row.
 template <class T>
-__device__ inline void latent_finish(const LatentArgs& a, int row, int h, int d, f32x4 o, float inv,
-                                     bool empty) {
-  typename T::store* out = static_cast<typename T::store*>(a.out) +
-                           static_cast<int64_t>(row) * a.out_token +
-                           static_cast<int64_t>(h) * a.out_head + d;
+__device__ inline void latent_put(uint16_t* to, f32x4 o, float inv, bool empty) {
   u32x2 v;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -229,7 +251,7 @@ __device__ inline void latent_finish(const LatentArgs& a, int row, int h, int d,
     const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv);
     v[e] = lo | (hi << 16);
   }
-  *reinterpret_cast<u32x2*>(out) = v;
+  *reinterpret_cast<u32x2*>(to) = v;
 }
 
 template <class T>
@@ -237,9 +259,29 @@ __device__ inline float latent_lse(float m, float l, float bias) {
   return m == -INFINITY && l == 0.0f ? -INFINITY : (m - bias + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Floats of a part: its columns' sums, maxima and sums of weights.
+// Floats of a part: its columns' sums, maxima and sums of weights.  The sums lie as
+// a wavefront has them, [16 columns][16 values][4 lanes' four values][column], so that
+// it stores whole lines.
+__device__ inline int latent_part_at(int rank, int col, int d) {
+  return (col / 16 * (rank / 16) + d / 16) * 256 + (d % 16 / 4 * 16 + col % 16) * 4;
+}
 __host__ __device__ constexpr size_t latent_part_floats(int cols, int rank) {
   return static_cast<size_t>(cols) * (rank + 2);
+}
+
+// The unit that tile t lies in.
+__device__ inline int last_of_units(ConstLong firsts, int n, int64_t t) {
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int half = len >> 1;
+    if (firsts[lo + half] <= t) lo += half;
+    len -= half;
+  }
+  return lo;
+}
+
+__device__ inline size_t latent_part(int run, int which, int slices, int slice) {
+  return (static_cast<size_t>(run) * 2 + which) * slices + slice;
 }
 
 template <class T, int R, int P, int W, int G, int NW>
@@ -252,20 +294,19 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % W, h = lane / W;
   const int group = wave / S::kColGroups, col_group = wave % S::kColGroups;
-  const auto* head = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
-  const LongDeal deal(head->tiles, a.runs);
-  // Neighbouring runs on one XCD (blocks go to the eight in turn): a unit's
-  // neighbours read the same rows.
-  const int xcd = static_cast<int>(blockIdx.x % 8), nth = static_cast<int>(blockIdx.x / 8);
-  if (nth >= deal.used / 8 + (xcd < deal.used % 8)) return;
-  const int run = xcd * (deal.used / 8) + min(xcd, deal.used % 8) + nth;
-  const int64_t begin = deal.begin(run), end = deal.begin(run + 1);
+  // Blocks go to the eight XCDs in turn: a unit's slices are on one, as neighbouring
+  // runs are, since they read the same rows.
+  const int nth = static_cast<int>(blockIdx.x / 8), slice = nth % a.slices;
+  const auto* start = reinterpret_cast<ConstLatentStart>(reinterpret_cast<uintptr_t>(a.work) + a.at_starts) +
+                      (nth / a.slices * 8 + blockIdx.x % 8);
+  const int run = start->run;
+  if (run < 0) return;
+  const int64_t begin = start->begin, end = start->end;
   const auto* units = reinterpret_cast<ConstLatentUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_units);
   const auto* firsts = reinterpret_cast<ConstLong>(reinterpret_cast<uintptr_t>(a.work) + a.at_first);
   const auto* table = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.table));
-  int u = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) + a.at_runs)[run];
+  int u = start->unit;
   const int bs = 1 << a.block_log2;
-
   if (threadIdx.x == 0) s_odd = 0;
   __syncthreads();
 
@@ -281,27 +322,50 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
                    16 * (((W == 32 ? 2 * (lane >> 4 & 1) : 0) + (i16 % 4 >> 1)) ^ S::template turn<2 * R>(v_row));
 
   for (int64_t at = begin; at < end; ++u) {
-    const int64_t first = firsts[u], last = firsts[u + 1];
+    int64_t first = start->first, last = start->last;
+    int unit_lo = start->tile_lo, request = start->request, unit_row = start->row;
+    int tokens = start->tokens, first_pos = start->pos;
+    if (at != begin) {
+      first = firsts[u];
+      last = firsts[u + 1];
+      unit_lo = units[u].tile_lo;
+      request = units[u].request;
+      unit_row = units[u].row;
+      tokens = units[u].tokens;
+      first_pos = units[u].pos;
+    }
     const int64_t stop = last < end ? last : end;
-    const int tile_lo = units[u].tile_lo + static_cast<int>(at - first);
-    const int tile_hi = units[u].tile_lo + static_cast<int>(stop - first);
-    const int request = units[u].request, unit_row = units[u].row, tokens = units[u].tokens;
-    const int first_pos = units[u].pos, last_pos = first_pos + tokens - 1;
+    const int tile_lo = unit_lo + static_cast<int>(at - first);
+    const int tile_hi = unit_lo + static_cast<int>(stop - first);
+    const int last_pos = first_pos + tokens - 1;
     const bool is_whole = first >= begin && last <= end;
     const int which = first >= begin ? 1 : 0;
     at = stop;
-    if (tokens <= 0) continue;
+    const int col0 = slice * S::kCols, cols = min(S::kCols, tokens * a.heads - col0);
+    if (cols <= 0) continue;
     wait_loads<0>();  // the last unit's stores: loads are counted from here
-    const int cols = tokens * a.heads;
     const int first_seen = a.window > 0 ? max(0, first_pos + 1 - a.window) : 0;
     const int64_t table_row = static_cast<int64_t>(request) * a.width;
 
-    const int col = W * col_group + c;
-    const bool mine = col < cols;
-    const int token = mine ? col / a.heads : tokens - 1;
-    const int q_head = mine ? col - token * a.heads : 0;
-    const int pos = first_pos + token;
-    const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+    // A lane's column, made where it is used: kept, it would push sums out of the
+    // registers.
+    struct Column {
+      int c, h, col, token, head, pos;
+      bool mine;
+    };
+    auto column = [&]() {
+      int lane = __lane_id();
+      asm volatile("" : "+v"(lane));
+      Column x;
+      x.c = lane % W;
+      x.h = lane / W;
+      x.col = W * col_group + x.c;
+      x.mine = x.col < cols;
+      x.token = x.mine ? (col0 + x.col) / a.heads : tokens - 1;
+      x.head = x.mine ? col0 + x.col - x.token * a.heads : 0;
+      x.pos = first_pos + x.token;
+      return x;
+    };
     const int all_from = a.window > 0 ? max(0, last_pos + 1 - a.window) : 0;
     const bool busy = W * col_group < cols;  // this wavefront has a column
 
@@ -310,16 +374,20 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
     const int row0 = col_group * S::kRowsEach;
     uint32_t there = 0;  // two bits to a stage: its halves have a block
     // A half's block is looked up a stage before its loads.
-    int id[2];
+    struct Ids {
+      int id[2];
+    };
     auto look_up = [&](int stage) {
       const int key = (tile_lo + group + G * stage) * kLatentTile;
+      Ids f;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int j = (key + 16 * k) >> a.block_log2;
-        id[k] = table[table_row + max(0, min(j, a.width - 1))];
+        f.id[k] = table[table_row + max(0, min(j, a.width - 1))];
       }
+      return f;
     };
-    auto issue = [&](int stage) {
+    auto issue = [&](int stage, const Ids& f) {
       const int tile = tile_lo + group + G * stage;
       const int slot = (stage % S::kStages) * G + group;
       const char* base[2];
@@ -329,68 +397,65 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         const int key = tile * kLatentTile + 16 * k;
         const bool ok = tile < tile_hi && key <= last_pos && key + 15 >= first_seen &&
                         (key >> a.block_log2) < a.width &&
-                        static_cast<uint32_t>(id[k]) < a.blocks;
-        base[k] = ok ? a.rows + ((static_cast<uint64_t>(static_cast<uint32_t>(id[k])) << a.block_log2) +
+                        static_cast<uint32_t>(f.id[k]) < a.blocks;
+        base[k] = ok ? a.rows + ((static_cast<uint64_t>(static_cast<uint32_t>(f.id[k])) << a.block_log2) +
                                  (key & (bs - 1))) * S::kRowBytes
                      : reinterpret_cast<const char*>(latent_zeros);
         bits |= ok ? 1u << k : 0u;
       }
       there |= bits << (2 * (stage % S::kStages));
-      char* to = ring + slot * S::kTileBytes;
+      const uint32_t to = lds_address(ring) + slot * S::kTileBytes;
       int lane = __lane_id();
       asm volatile("" : "+v"(lane));  // offsets made here, not kept over the products
 #pragma unroll
       for (int i = 0; i < S::kLatLoads; ++i) {
         const int row = row0 + i * S::kLatRows;                      // of the load
         const int r = row + lane / (64 / S::kLatRows), chunk = lane % (64 / S::kLatRows);
-        const uint32_t off = (r & 15) * S::kRowBytes + 16 * (chunk ^ S::template turn<2 * R>(r));
-        __builtin_amdgcn_global_load_lds(
-            reinterpret_cast<const u32x4*>(base[S::kRowsEach == 32 ? i * S::kLatRows / 16 : row / 16] + off),
-            (__attribute__((address_space(3))) void*)(to + row * 2 * R), 16, 0, 0);
+        load_direct(base[S::kRowsEach == 32 ? i * S::kLatRows / 16 : row / 16],
+                    (r & 15) * S::kRowBytes + 16 * (chunk ^ S::template turn<2 * R>(r)), to + row * 2 * R);
       }
 #pragma unroll
       for (int i = 0; i < S::kKeyLoads; ++i) {
-        // (two wavefronts bring the same 16 rows where eight are a half load)
+        // (wavefronts bring the same rows where their own are no whole load)
         const int row = (row0 / S::kKeyRows + i) * S::kKeyRows;
         constexpr int kChunks = 2 * P / 16;
         const int r = row + lane / kChunks, chunk = lane % kChunks;
-        const uint32_t off = (r & 15) * S::kRowBytes + 2 * R + 16 * (chunk ^ S::template turn<2 * P>(r));
-        __builtin_amdgcn_global_load_lds(
-            reinterpret_cast<const u32x4*>(base[S::kRowsEach == 32 ? i * S::kKeyRows / 16 : row / 16] + off),
-            (__attribute__((address_space(3))) void*)(to + kLatentTile * 2 * R + row * 2 * P), 16, 0, 0);
+        load_direct(base[S::kRowsEach == 32 ? i * S::kKeyRows / 16 : row / 16],
+                    (r & 15) * S::kRowBytes + 2 * R + 16 * (chunk ^ S::template turn<2 * P>(r)),
+                    to + kLatentTile * 2 * R + row * 2 * P);
       }
     };
 
-    // ---- queries
+    // ---- the first stages' rows and the queries
+    constexpr int kFirst = S::kStages > 1 ? S::kStages - 1 : 1;
+    Ids ids[kFirst];
+#pragma unroll
+    for (int s = 0; s < kFirst; ++s) ids[s] = look_up(s);
     u32x4 q[S::kSteps];
     {
+      const Column x = column();
       const uint16_t* from = static_cast<const uint16_t*>(a.q) +
-                             static_cast<int64_t>(min(unit_row + token, a.tokens - 1)) * a.q_token +
-                             static_cast<int64_t>(q_head) * a.q_head + 8 * h;
+                             static_cast<int64_t>(min(unit_row + x.token, a.tokens - 1)) * a.q_token +
+                             static_cast<int64_t>(x.head) * a.q_head + 8 * x.h;
 #pragma unroll
       for (int s = 0; s < S::kSteps; ++s) {
         q[s] = *reinterpret_cast<const u32x4*>(from + S::kStep * s);
       }
     }
-    // In registers before the rows' loads begin, so that a stage waits for rows only.
-    // At rank 512, with four wavefronts, they live in AGPRs, where the matrix instructions read them, and
-    // leave the VGPRs to the sums (this file is built with the MFMA
-    // VGPR-accumulator form).
+    asm volatile("" ::: "memory");  // queries first: what waits for them counts on it
+    // (stages past the last bring zeros, so that there is one count)
+#pragma unroll
+    for (int s = 0; s < kFirst; ++s) issue(s, ids[s]);
+    Ids next = look_up(kFirst);
+    asm volatile("" ::: "memory");
+    // Queries are in registers before the loop, so that a stage waits for rows only.
+    // At rank 512, with four wavefronts, they live in AGPRs, where the matrix
+    // instructions read them, and leave the VGPRs to the sums (this file is built
+    // with the MFMA VGPR-accumulator form).
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s) {
       if constexpr (R == 512 && NW == 4) asm volatile("" : "+a"(q[s]));
       else asm volatile("" : "+v"(q[s]));
-    }
-    asm volatile("" ::: "memory");
-    look_up(0);
-    if constexpr (S::kStages > 1) {
-#pragma unroll
-      for (int s = 0; s < S::kStages - 1; ++s) {
-        if (s < n) {
-          issue(s);
-          look_up(s + 1);
-        }
-      }
     }
 
     Acc o[S::kTilesD];
@@ -404,20 +469,18 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
 
     // The stage's rows are in LDS, and all are done with the one before, whose place
     // the next loads take.
+    auto go_on = [&](int stage) {
+      if (stage < n) {
+        issue(stage, next);
+        next = look_up(stage + 1);
+      }
+    };
     auto enter = [&](int i) {
-      if constexpr (S::kStages == 1) {
-        asm volatile("" ::: "memory");
-        issue(i);
-        look_up(i + 1);
-        wait_loads<0>();
-      } else {
-        if (i + S::kStages - 2 < n) wait_loads<(S::kStages - 2) * S::kLoads>();
-        else wait_loads<0>();
+      if (i + S::kStages - 2 < n && S::kStages > 1) wait_loads<(S::kStages > 1 ? S::kStages - 2 : 0) * S::kLoads>();
+      else wait_loads<0>();
+      if constexpr (S::kStages > 1) {
         block_barrier();
-        if (i + S::kStages - 1 < n) {
-          issue(i + S::kStages - 1);
-          look_up(i + S::kStages);
-        }
+        go_on(i + S::kStages - 1);
       }
     };
     // A row that is not finite has no finite score with any column.  Where some
@@ -433,7 +496,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         if (odd && lane == 0) s_odd = 1;
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
         block_barrier();
-        odd = *static_cast<volatile int*>(&s_odd) != 0;
+        odd = s_odd != 0;
         __builtin_amdgcn_s_waitcnt(0xc07f);
         block_barrier();
         if (!odd) return;
@@ -464,6 +527,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         if (partly_seen(i)) keep_finite(i, false);
       }
     }
+    static_assert(S::kStages > 1 || S::kColGroups == 1, "one stage: a wavefront's own tiles");
     for (int i = 0; i < n && busy; ++i) {
       enter(i);
       const int slot = i % S::kStages;
@@ -495,7 +559,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         return *reinterpret_cast<const u32x4*>(
             from + ((p_at ^ (16 * S::kH * (k % kIn))) + 128 * (k / kIn) + r * 4 * 2 * P));
       };
-      in_order<S::kSteps * S::kRowTiles, 4>(
+      in_order<S::kSteps * S::kRowTiles, S::kAhead>(
           [&](int i) { return key_chunk(i / S::kRowTiles, i % S::kRowTiles); },
           [&](int i, u32x4 f) {
             s[i % S::kRowTiles] = mfma<S::kBf>(f, q[i / S::kRowTiles], s[i % S::kRowTiles]);
@@ -503,28 +567,37 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       float score[S::kPer];
 #pragma unroll
       for (int e = 0; e < S::kPer; ++e) score[e] = s[e / S::kAcc][e % S::kAcc];
-      float odd_sum = 0.0f;
+      if (partly_seen(i)) {
+        float odd = 0.0f;
 #pragma unroll
-      for (int e = 0; e < S::kPer; ++e) odd_sum = fmaf(score[e], 0.0f, odd_sum);
-      const bool odd = __any(odd_sum != 0.0f);
-      if (partly_seen(i)) keep_finite(i, odd);
-      const int key0 = tile * kLatentTile + S::kPer * h;  // a lane's first
+        for (int e = 0; e < S::kPer; ++e) odd = fmaf(score[e], 0.0f, odd);
+        keep_finite(i, __any(odd != 0.0f));
+      }
+      // NaN and +inf make their column's sums so by themselves; a weight of 0 would
+      // hide -inf.
+      float top = score[0], low = score[0];
+#pragma unroll
+      for (int e = 1; e < S::kPer; ++e) {
+        top = fmaxf(top, score[e]);
+        low = fminf(low, score[e]);
+      }
       const bool whole = tile * kLatentTile >= all_from && tile < tile_hi &&
-                         tile * kLatentTile + kLatentTile - 1 <= first_pos && have == 3u;
-      float top = -INFINITY;
-      if (whole && !odd) {
-#pragma unroll
-        for (int e = 0; e < S::kPer; ++e) {
-          score[e] *= mul;
-          top = fmaxf(top, score[e]);
-        }
+                         tile * kLatentTile + kLatentTile - 1 <= first_pos && have == 3u && mul >= 0.0f;
+      float scale_by = mul;  // of a score in the exponent
+      if (whole && !__any(low < -3.4028235e38f)) {
+        top *= mul;
       } else {
         // a lane's keys lie in one half
-        const bool some = tile < tile_hi && (have >> (S::kPer * h >> 4) & 1u);
+        const Column x = column();
+        const int key0 = tile * kLatentTile + S::kPer * x.h;  // a lane's first
+        const int seen_from = a.window > 0 ? max(0, x.pos + 1 - a.window) : 0;
+        const bool some = tile < tile_hi && (have >> (S::kPer * x.h >> 4) & 1u);
+        top = -INFINITY;
+        scale_by = 1.0f;
 #pragma unroll
         for (int e = 0; e < S::kPer; ++e) {
           const int key = key0 + e;
-          const bool see = some && key <= pos && key >= seen_from;
+          const bool see = some && key <= x.pos && key >= seen_from;
           const bool fine = fabsf(score[e]) <= 3.4028235e38f;
           poison += see && !fine ? NAN : 0.0f;
           score[e] = see && fine ? score[e] * mul : -INFINITY;
@@ -547,8 +620,8 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       u32x4 w[S::kPer / 8];
 #pragma unroll
       for (int e = 0; e < S::kPer; e += 2) {
-        const float x = __builtin_amdgcn_exp2f(score[e] + shift);
-        const float y = __builtin_amdgcn_exp2f(score[e + 1] + shift);
+        const float x = __builtin_amdgcn_exp2f(fmaf(score[e], scale_by, shift));
+        const float y = __builtin_amdgcn_exp2f(fmaf(score[e + 1], scale_by, shift));
         l += x;
         l += y;
         w[e / 8][e % 8 / 2] = S::weights(x, y);
@@ -565,11 +638,16 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         const u32x2 lo = four(0), hi = four(1);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
-      in_order<S::kTilesD * (S::kPer / 8), 4>(
+      in_order<S::kTilesD * (S::kPer / 8), S::kAhead>(
           [&](int i) { return value_chunk(i / (S::kPer / 8), i % (S::kPer / 8)); },
           [&](int i, u32x4 f) {
             o[i / (S::kPer / 8)] = mfma<S::kBf>(f, w[i % (S::kPer / 8)], o[i / (S::kPer / 8)]);
           });
+      if constexpr (S::kStages == 1) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the rows are read
+        asm volatile("" ::: "memory");
+        go_on(i + 1);
+      }
     }
 
 #pragma unroll
@@ -578,29 +656,55 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       poison += __shfl_xor(poison, by);
     }
     l += poison;
-    // ---- the groups' results together
+    // ---- the groups' results together, and out
+    const Column x = column();
+    float* part = a.parts + latent_part(run, which, a.slices, slice) * latent_part_floats(S::kCols, R);
+    constexpr int kVecs = S::kAcc / 4;
+    auto write = [&](auto value, int d_first, int d_last, int d_step) {
+      if (!x.mine) return;
+      if (is_whole) {
+        const float inv = 1.0f / l;
+        const bool empty = m == -INFINITY && l == 0.0f;
+        uint16_t* to = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(unit_row + x.token) * a.out_token +
+                       static_cast<int64_t>(x.head) * a.out_head + 4 * x.h;
+        for (int d = d_first; d < d_last; d += d_step) {
+#pragma unroll
+          for (int k = 0; k < kVecs; ++k) {
+            latent_put<T>(to + W * d + 4 * S::kH * k, value(d, k), inv, empty);
+          }
+        }
+      } else {
+        for (int d = d_first; d < d_last; d += d_step) {
+#pragma unroll
+          for (int k = 0; k < kVecs; ++k) {
+            *reinterpret_cast<f32x4*>(part + latent_part_at(R, x.col, W * d + 4 * S::kH * k + 4 * x.h)) = value(d, k);
+          }
+        }
+      }
+    };
     if constexpr (G > 1) {
-      if (h == 0) {
-        s_m[wave][c] = m;
-        s_l[wave][c] = l;
+      if (x.h == 0) {
+        s_m[wave][x.c] = m;
+        s_l[wave][x.c] = l;
       }
       __syncthreads();  // also: the ring is read
       float top = -INFINITY, total = 0.0f;
 #pragma unroll
-      for (int g = 0; g < G; ++g) top = fmaxf(top, s_m[g * S::kColGroups + col_group][c]);
+      for (int g = 0; g < G; ++g) top = fmaxf(top, s_m[g * S::kColGroups + col_group][x.c]);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float mg = s_m[g * S::kColGroups + col_group][c], lg = s_l[g * S::kColGroups + col_group][c];
+        const float mg = s_m[g * S::kColGroups + col_group][x.c];
+        const float lg = s_l[g * S::kColGroups + col_group][x.c];
         total += lg * (mg == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mg - top));
       }
       const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
       m = top;
       l = total;
-      constexpr int kVecs = S::kAcc / 4;
       constexpr int kAt = S::kLds / (NW * kWave * 16 * kVecs);         // value tiles at once
-      constexpr int kTiles = kAt / G * G < S::kTilesD ? kAt / G * G : S::kTilesD;
-      static_assert(kTiles > 0 && S::kTilesD % kTiles == 0, "whole rounds");
+      constexpr int kTiles = kAt >= S::kTilesD ? S::kTilesD : kAt >= 16 ? 16 : kAt >= 8 ? 8 : 4;
+      static_assert(kTiles <= kAt && S::kTilesD % kTiles == 0 && kTiles % G == 0, "whole rounds");
       f32x4* box = reinterpret_cast<f32x4*>(ring);
+      const int at_lane = x.c + W * x.h;
 #pragma unroll
       for (int d0 = 0; d0 < S::kTilesD; d0 += kTiles) {
         if (d0) __syncthreads();
@@ -611,85 +715,92 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
             f32x4 v;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = o[d0 + d][4 * k + e] * f;
-            box[((wave * kTiles + d) * kVecs + k) * kWave + lane] = v;
+            box[((wave * kTiles + d) * kVecs + k) * kWave + at_lane] = v;
           }
         }
         __syncthreads();
-        if (mine) {
-          const float inv = 1.0f / l;
-          const bool empty = m == -INFINITY && l == 0.0f;
-          float* part = a.parts + (static_cast<size_t>(run) * 2 + which) * latent_part_floats(S::kCols, R);
-          for (int d = group; d < kTiles; d += G) {
+        write([&](int d, int k) {
+          f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < kVecs; ++k) {
-              f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int g = 0; g < G; ++g) {
+            v += box[(((g * S::kColGroups + col_group) * kTiles + d - d0) * kVecs + k) * kWave + at_lane];
+          }
+          return v;
+        }, d0 + group, d0 + kTiles, G);
+      }
+      __syncthreads();  // the ring takes the next unit's rows
+    } else {
+      auto value = [&](int d, int k) {
+        f32x4 v;
 #pragma unroll
-              for (int g = 0; g < G; ++g) {
-                v += box[(((g * S::kColGroups + col_group) * kTiles + d) * kVecs + k) * kWave + lane];
-              }
-              const int x = W * (d0 + d) + 4 * S::kH * k + 4 * h;
-              if (is_whole) latent_finish<T>(a, unit_row + token, q_head, x, v, inv, empty);
-              else *reinterpret_cast<f32x4*>(part + col * R + x) = v;
-            }
+        for (int e = 0; e < 4; ++e) v[e] = o[d][4 * k + e];
+        return v;
+      };
+      if (x.mine && is_whole) {
+        const float inv = 1.0f / l;
+        const bool empty = m == -INFINITY && l == 0.0f;
+        uint16_t* to = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(unit_row + x.token) * a.out_token +
+                       static_cast<int64_t>(x.head) * a.out_head + 4 * x.h;
+#pragma unroll
+        for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+          for (int k = 0; k < kVecs; ++k) latent_put<T>(to + W * d + 4 * S::kH * k, value(d, k), inv, empty);
+        }
+      } else if (x.mine) {
+#pragma unroll
+        for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+          for (int k = 0; k < kVecs; ++k) {
+            *reinterpret_cast<f32x4*>(part + latent_part_at(R, x.col, W * d + 4 * S::kH * k + 4 * x.h)) = value(d, k);
           }
         }
       }
       __syncthreads();  // the ring takes the next unit's rows
-    } else if (mine) {
-      const float inv = 1.0f / l;
-      const bool empty = m == -INFINITY && l == 0.0f;
-      float* part = a.parts + (static_cast<size_t>(run) * 2 + which) * latent_part_floats(S::kCols, R);
-#pragma unroll
-      for (int d = 0; d < S::kTilesD; ++d) {
-#pragma unroll
-        for (int k = 0; k < S::kAcc / 4; ++k) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = o[d][4 * k + e];
-          const int x = W * d + 4 * S::kH * k + 4 * h;
-          if (is_whole) latent_finish<T>(a, unit_row + token, q_head, x, v, inv, empty);
-          else *reinterpret_cast<f32x4*>(part + col * R + x) = v;
-        }
-      }
     }
-    if constexpr (G == 1) __syncthreads();
-    if (mine && h == 0 && group == 0) {
+    if (x.mine && x.h == 0 && group == 0) {
       if (is_whole) {
         if (a.lse) {
-          a.lse[static_cast<size_t>(unit_row + token) * a.heads + q_head] = latent_lse<T>(m, l, S::kBias);
+          a.lse[static_cast<size_t>(unit_row + x.token) * a.heads + x.head] = latent_lse<T>(m, l, S::kBias);
         }
       } else {
-        float* part = a.parts + (static_cast<size_t>(run) * 2 + which) * latent_part_floats(S::kCols, R);
-        part[S::kCols * R + col] = m;
-        part[S::kCols * (R + 1) + col] = l;
+        part[S::kCols * R + x.col] = m;
+        part[S::kCols * (R + 1) + x.col] = l;
       }
     }
   }
 }
 
-// Joins the parts of the unit that a run's end cuts first: block x is the end of
-// run x, and a block of it takes 1024 / R columns, four values to a thread.
+// Joins the parts of cut units: block x is unit x's or, where there are fewer ends of
+// runs than units, those of the unit that the end of run x cuts first; it takes 16
+// columns and 64 values of each, a wavefront 16 of them, as they lie in a part.
 template <class T, int R, int COLS>
-__global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bias) {
-  constexpr int kVecs = R / 4, kEach = 256 / kVecs;
+__global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bias, int by_unit) {
   const auto* head = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
-  const LongDeal deal(head->tiles, a.runs);
-  const int run = static_cast<int>(blockIdx.x) + 1;
-  if (run >= deal.used) return;
+  const LatentDeal deal = {head->deal[a.per - 1].each, head->deal[a.per - 1].used, head->deal[a.per - 1].rem};
   const auto* units = reinterpret_cast<ConstLatentUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_units);
   const auto* firsts = reinterpret_cast<ConstLong>(reinterpret_cast<uintptr_t>(a.work) + a.at_first);
-  const int u = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.work) + a.at_runs)[run];
+  int u = static_cast<int>(blockIdx.x);
+  if (by_unit) {
+    if (u >= head->units) return;
+  } else {
+    if (u + 1 >= deal.used) return;
+    u = last_of_units(firsts, head->units, deal.begin(u + 1));
+  }
   const int64_t first = firsts[u], last = firsts[u + 1];
-  if (first >= deal.begin(run)) return;             // begins with this run
-  if (first < deal.begin(run - 1)) return;          // an end before this one cuts it too
-  const int from = run - 1, to = deal.run(last - 1);
+  const int from = by_unit ? deal.run(first) : static_cast<int>(blockIdx.x), to = deal.run(last - 1);
+  if (to == from) return;
+  // an end before this one cuts it too, or it begins with the run after
+  if (!by_unit && (first < deal.begin(from) || first >= deal.begin(from + 1))) return;
   const int from_which = first >= deal.begin(from) ? 1 : 0;
-  const int cols = units[u].tokens * a.heads;
-  const int c = static_cast<int>(blockIdx.y) * kEach + static_cast<int>(threadIdx.x) / kVecs;
-  const int d = static_cast<int>(threadIdx.x) % kVecs * 4;
-  if (c >= cols) return;
-  constexpr size_t kPart = latent_part_floats(COLS, R);
-  auto part = [&](int r) { return a.parts + (static_cast<size_t>(r) * 2 + (r == from ? from_which : 0)) * kPart; };
+  const int lane = __lane_id(), wave = static_cast<int>(threadIdx.x) / kWave;
+  const int col = 16 * static_cast<int>(blockIdx.y) + lane % 16;
+  const int d = 64 * static_cast<int>(blockIdx.z) + 16 * wave + lane / 16 * 4;
+  if (col >= units[u].tokens * a.heads) return;
+  const int slice = col / COLS, c = col - slice * COLS;
+  const int at = latent_part_at(R, c, d);
+  auto part = [&](int r) {
+    return a.parts + latent_part(r, r == from ? from_which : 0, a.slices, slice) * latent_part_floats(COLS, R);
+  };
   float m = -INFINITY, l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kBatch = 8;  // parts whose loads go out together
@@ -701,7 +812,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bi
       const float* p = part(min(r0 + k, to));
       pm[k] = p[COLS * R + c];
       pl[k] = p[COLS * (R + 1) + c];
-      po[k] = *reinterpret_cast<const f32x4*>(p + c * R + d);
+      po[k] = *reinterpret_cast<const f32x4*>(p + at);
     }
     float m2 = m;
 #pragma unroll
@@ -721,8 +832,10 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bi
     m = m2;
   }
   const bool empty = m == -INFINITY && l == 0.0f;
-  const int token = c / a.heads, h = c - token * a.heads;
-  latent_finish<T>(a, units[u].row + token, h, d, o, 1.0f / l, empty);
+  const int token = col / a.heads, h = col - token * a.heads;
+  latent_put<T>(static_cast<uint16_t*>(a.out) + static_cast<int64_t>(units[u].row + token) * a.out_token +
+                    static_cast<int64_t>(h) * a.out_head + d,
+                o, 1.0f / l, empty);
   if (a.lse && d == 0) {
     a.lse[static_cast<size_t>(units[u].row + token) * a.heads + h] = latent_lse<T>(m, l, bias);
   }

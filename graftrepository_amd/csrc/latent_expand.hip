@@ -63,13 +63,12 @@ __global__ __launch_bounds__(256, 2) void latent_expand_kernel(ExpandArgs a) {
     from[2 + i] = a.weight + static_cast<int64_t>(n) * a.rank + 8 * (chunk ^ 2 * (i & 1));
   }
   auto issue = [&](int step) {
-    char* to = lds + (step % kExpandStages) * kExpandStage;
+    const uint32_t to = lds_address(lds) + (step % kExpandStages) * kExpandStage;
 #pragma unroll
     for (int i = 0; i < 6; ++i) {
-      char* at = i < 2 ? to + (2 * wave + i) * 1024
-                       : to + kExpandRows * kExpandStep * 2 + (4 * wave + i - 2) * 1024;
-      __builtin_amdgcn_global_load_lds(reinterpret_cast<const u32x4*>(from[i] + step * kExpandStep),
-                                       (__attribute__((address_space(3))) void*)at, 16, 0, 0);
+      load_direct(from[i] + step * kExpandStep,
+                  i < 2 ? to + (2 * wave + i) * 1024
+                        : to + kExpandRows * kExpandStep * 2 + (4 * wave + i - 2) * 1024);
     }
   };
   const int steps = a.rank / kExpandStep;
@@ -276,32 +275,34 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   const int tile_hi = (min(last_pos - keys.start + 1, keys.count) + kLatentTile - 1) / kLatentTile;
   const int n = max(0, tile_hi - tile_lo);
 
+  // Offsets of this lane's rows in a tile, which stay; a tile past the rows' end has
+  // its last row again.
+  uint32_t offsets[S::kLoads];
+  auto offset_of = [&](int j, int last) {
+    const bool key = j < S::kKeyLoads;
+    constexpr int kKeyChunks = S::kKeyBytes / 16, kValueChunks = S::kValueBytes / 16;
+    const int at = (key ? wave * S::kKeyLoads + j : wave * S::kValueLoads + j - S::kKeyLoads) * kWave + lane;
+    const int r = at / (key ? kKeyChunks : kValueChunks), place = at - r * (key ? kKeyChunks : kValueChunks);
+    const int chunk = place ^ (key ? L::template turn<S::kKeyBytes>(r) : L::template turn<S::kValueBytes>(r));
+    // (a row's last places in LDS may be nobody's)
+    const int64_t row = static_cast<int64_t>(min(r, last)) * (key ? a.k_row : a.v_row);
+    return static_cast<uint32_t>(2 * (row + 8 * (!key || chunk < DK / 8 ? chunk : 0)));
+  };
+#pragma unroll
+  for (int j = 0; j < S::kLoads; ++j) offsets[j] = offset_of(j, kLatentTile);
   auto issue = [&](int i) {
-    char* to = ring + (i % S::kStages) * S::kStage;
+    const uint32_t to = lds_address(ring) + (i % S::kStages) * S::kStage;
     const int key0 = (tile_lo + i) * kLatentTile;
-    int lane = __lane_id();
-    asm volatile("" : "+v"(lane));  // offsets made here, not kept over the products
+    const int64_t first = keys.first + key0;
+    const char* k = reinterpret_cast<const char*>(a.k + first * a.k_row + head * a.k_head);
+    const char* v = reinterpret_cast<const char*>(a.v + first * a.v_row + head * a.v_head);
+    const bool cut = key0 + kLatentTile > keys.count;
 #pragma unroll
-    for (int j = 0; j < S::kKeyLoads; ++j) {
-      constexpr int kChunks = S::kKeyBytes / 16;
-      const int load = wave * S::kKeyLoads + j, at = load * kWave + lane, r = at / kChunks;
-      const int chunk = (at - r * kChunks) ^ L::template turn<S::kKeyBytes>(r);
-      // (a row's last places in LDS may be nobody's)
-      const int64_t key = keys.first + min(key0 + r, keys.count - 1);
-      __builtin_amdgcn_global_load_lds(
-          reinterpret_cast<const u32x4*>(a.k + key * a.k_row + head * a.k_head +
-                                         8 * (chunk < DK / 8 ? chunk : 0)),
-          (__attribute__((address_space(3))) void*)(to + load * 1024), 16, 0, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < S::kValueLoads; ++j) {
-      constexpr int kChunks = S::kValueBytes / 16;
-      const int load = wave * S::kValueLoads + j, at = load * kWave + lane, r = at / kChunks;
-      const int chunk = (at - r * kChunks) ^ L::template turn<S::kValueBytes>(r);
-      const int64_t key = keys.first + min(key0 + r, keys.count - 1);
-      __builtin_amdgcn_global_load_lds(
-          reinterpret_cast<const u32x4*>(a.v + key * a.v_row + head * a.v_head + 8 * chunk),
-          (__attribute__((address_space(3))) void*)(to + kLatentTile * S::kKeyBytes + load * 1024), 16, 0, 0);
+    for (int j = 0; j < S::kLoads; ++j) {
+      const bool key = j < S::kKeyLoads;
+      const uint32_t at = key ? (wave * S::kKeyLoads + j) * 1024
+                              : kLatentTile * S::kKeyBytes + (wave * S::kValueLoads + j - S::kKeyLoads) * 1024;
+      load_direct(key ? k : v, cut ? offset_of(j, keys.count - 1 - key0) : offsets[j], to + at);
     }
   };
 
@@ -311,14 +312,14 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s) q[s] = *reinterpret_cast<const u32x4*>(from + 16 * s);
   }
-  // In registers before the rows' loads begin, so that a stage waits for rows only.
-#pragma unroll
-  for (int s = 0; s < S::kSteps; ++s) asm volatile("" : "+v"(q[s]));
-  asm volatile("" ::: "memory");
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) {
     if (i < n) issue(i);
   }
+  // In registers before the loop, so that a stage waits for rows only.
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) asm volatile("" : "+v"(q[s]));
+  asm volatile("" ::: "memory");
   const int key_row = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
   const int k_at = key_row * S::kKeyBytes + 16 * (h ^ L::template turn<S::kKeyBytes>(key_row));
   const int i16 = lane % 16, v_row = 16 * h + i16 / 4;
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
       }
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
       block_barrier();
-      bad = *static_cast<volatile uint32_t*>(&s_bad[i & 1]);
+      bad = s_bad[i & 1];
     }
     if (!busy || key0 > wave_last || key0 + kLatentTile <= wave_from) continue;
 
@@ -384,20 +385,23 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
           return *reinterpret_cast<const u32x4*>(stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
         },
         [&](int k, u32x4 f) { s = mfma<S::kBf>(f, q[k], s); });
-    float score[16], top = -INFINITY, odd = 0.0f;
+    float score[16], top = s[0], low = s[0];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       score[e] = s[e];
-      odd = fmaf(s[e], 0.0f, odd);
+      top = fmaxf(top, s[e]);
+      low = fminf(low, s[e]);
     }
-    const bool whole = key0 >= wave_all_from && key0 + kLatentTile - 1 <= min(wave_first, keys.count - 1);
-    if (whole && bad == 0 && !__any(odd != 0.0f)) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        score[e] *= mul;
-        top = fmaxf(top, score[e]);
-      }
+    const bool whole = key0 >= wave_all_from && mul >= 0.0f &&
+                       key0 + kLatentTile - 1 <= min(wave_first, keys.count - 1);
+    float scale_by = mul;  // of a score in the exponent
+    // NaN and +inf make their column's sums so by themselves; a weight of 0 would hide
+    // -inf.
+    if (whole && bad == 0 && !__any(low < -3.4028235e38f)) {
+      top *= mul;
     } else {
+      top = -INFINITY;
+      scale_by = 1.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int key = key0 + 16 * h + e;
@@ -423,8 +427,8 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     u32x4 w[2];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-      const float x = __builtin_amdgcn_exp2f(score[e] + shift);
-      const float y = __builtin_amdgcn_exp2f(score[e + 1] + shift);
+      const float x = __builtin_amdgcn_exp2f(fmaf(score[e], scale_by, shift));
+      const float y = __builtin_amdgcn_exp2f(fmaf(score[e + 1], scale_by, shift));
       l += x;
       l += y;
       w[e / 8][e % 8 / 2] = L::weights(x, y);
@@ -684,7 +688,9 @@ extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work,
   a.key_dim = key_dim;
   a.value_dim = value_dim;
   a.rows = static_cast<int32_t>(rows);
-  const bool scheduled = l.cap_rows * static_cast<uint64_t>(b->heads) < (1ull << 31);
+  // the matrix cores' kernel takes a tile's rows by 32-bit offsets
+  const auto near = [](int64_t stride) { return stride >= 0 && stride < (1ll << 25); };
+  const bool scheduled = l.cap_rows * static_cast<uint64_t>(b->heads) < (1ull << 31) && near(k_row_stride) && near(v_row_stride);
   const auto s = static_cast<hipStream_t>(stream);
   if (dtype == grm::kBF16) launch_rows<BF16>(a, l.cap_rows, scheduled, s);
   else launch_rows<F16>(a, l.cap_rows, scheduled, s);
