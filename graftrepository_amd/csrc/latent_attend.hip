@@ -14,20 +14,13 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
   const uint64_t busy = std::min(rows, reqs);
   const int64_t most = static_cast<int64_t>(std::max(1, b->max_new)) * b->heads;
   l.cols = most <= 16 ? 16 : most <= 32 ? 32 : most <= 64 ? 64 : kLatentCols;
-  l.slices = 1;
-  // One token of many heads: two blocks with half of them each leave half the parts
-  // (and read the rows twice, the second time from L2).
-  if (l.cols == kLatentCols && b->max_new <= 0) {
-    l.cols /= 2;
-    l.slices = 2;
-  }
-  l.unit_tokens = std::max(1, l.cols * l.slices / b->heads);
+  l.unit_tokens = std::max(1, l.cols / b->heads);
   for (int k = 0; k < 2; ++k) {
-    l.runs[k] = std::max(1, (k + 1) * cus / l.slices);
+    l.runs[k] = (k + 1) * cus;
     l.starts[k] = (l.runs[k] + 7) / 8 * 8;
   }
-  l.cap_units = rows / l.unit_tokens + busy;
-  l.cap_rows = rows / kRowUnit + busy;
+  l.cap_units = std::min(rows, rows / l.unit_tokens + busy);
+  l.cap_rows = std::min(rows, rows / kRowUnit + busy);
   l.reach = static_cast<int32_t>(std::min<int64_t>(
       static_cast<int64_t>(b->table_width) * b->block_tokens, 2 * static_cast<int64_t>(kMaxLen)));
   auto place = [&l](uint64_t bytes) {
@@ -39,7 +32,10 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
   l.at_units = place(l.cap_units * sizeof(LatentUnit));
   l.at_first = place((l.cap_units + 1) * 8);
   for (int k = 0; k < 2; ++k) {
+    // a join is of a unit of its own and has an end of a run
+    l.joins[k] = static_cast<int>(std::min<uint64_t>(l.runs[k] - 1, l.cap_units));
     l.at_starts[k] = place(static_cast<uint64_t>(l.starts[k]) * sizeof(LatentStart));
+    l.at_joins[k] = place(static_cast<uint64_t>(l.joins[k]) * sizeof(LatentJoin));
   }
   l.at_unit_scan = place((reqs + 1) * 4);
   l.at_row_scan = place((reqs + 1) * 4);
@@ -59,8 +55,8 @@ struct LatentPlanArgs {
   const int32_t* cu_new;
   char* work;
   int32_t requests, tokens, window, reach, unit_tokens, cap_units, cap_rows;
-  int32_t runs[2], starts[2];
-  uint64_t at_units, at_first, at_starts[2], at_unit_scan, at_row_scan, at_rows;
+  int32_t runs[2], starts[2], joins[2];
+  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_rows;
 };
 
 // Exclusive sum over the block; the total in *sum.  Two barriers.
@@ -170,7 +166,6 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
   }
   if (tid == 0) {
     firsts[n_units] = tiles;
-    head->units = n_units;
     head->row_units = n_rows;
   }
   __syncthreads();  // the lists are read back by other threads of this block
@@ -180,7 +175,6 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
     deal.used = static_cast<int>(min(most, static_cast<int64_t>(a.runs[k])));
     deal.each = deal.used ? tiles / deal.used : 0;
     deal.rem = deal.used ? static_cast<int>(tiles - deal.each * deal.used) : 0;
-    if (tid == 0) head->deal[k] = deal;
     auto* to = reinterpret_cast<LatentStart*>(a.work + a.at_starts[k]);
     for (int i = tid; i < a.starts[k]; i += kPlanThreads) {
       // neighbouring runs to one XCD, to which every eighth entry goes
@@ -203,6 +197,30 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
       }
       to[i] = s;
     }
+    // Ends of runs that are the first in a unit.
+    auto* joins = reinterpret_cast<LatentJoin*>(a.work + a.at_joins[k]);
+    int done = 0;
+    for (int base = 0; base < deal.used - 1; base += kPlanThreads) {
+      const int e = base + tid;
+      LatentJoin j{};
+      bool cuts = false;
+      if (e < deal.used - 1) {
+        const int64_t at = deal.begin(e + 1);
+        const int u = last_of(firsts, n_units, at);
+        if (firsts[u] < at && firsts[u] >= deal.begin(e)) {
+          cuts = units[u].tokens > 0;
+          j.from = e;
+          j.to = deal.run(firsts[u + 1] - 1);
+          j.row = units[u].row;
+          j.tokens = units[u].tokens;
+        }
+      }
+      int64_t sum;
+      const int64_t v = block_sum<int64_t>(cuts, &sum, scratch);
+      if (cuts) joins[done + v] = j;
+      done += static_cast<int>(sum);
+    }
+    for (int i = done + tid; i < a.joins[k]; i += kPlanThreads) joins[i] = LatentJoin{};
   }
 }
 
@@ -327,29 +345,33 @@ static int latent_waves(int rank, int cols) { return cols == kLatentCols || (ran
 static int latent_per(const LatentLayout& l, int rank) { return latent_per_cu(rank, latent_waves(rank, l.cols)); }
 
 static uint64_t latent_scratch(const LatentLayout& l, int rank) {
-  return static_cast<uint64_t>(l.runs[latent_per(l, rank) - 1]) * 2 * l.slices *
+  return static_cast<uint64_t>(l.runs[latent_per(l, rank) - 1]) * 2 *
          latent_part_floats(l.cols, rank) * 4;
 }
 
 template <class T, int R, int P, int W, int G, int NW>
-static void launch_cols(const LatentArgs& a, uint64_t units, hipStream_t stream) {
+static void launch_cols(const LatentArgs& a, hipStream_t stream) {
   typedef LatentShape<T, R, P, W, G, NW> S;
-  const auto blocks = static_cast<unsigned>((a.runs + 7) / 8 * 8 * a.slices);
+  const auto blocks = static_cast<unsigned>((a.runs + 7) / 8 * 8);
   latent_attend_kernel<T, R, P, W, G, NW><<<blocks, S::kThreads, 0, stream>>>(a);
   // real columns of a unit: whole tokens'
-  const int cols = std::max(1, S::kCols * a.slices / a.heads) * a.heads;
-  const bool by_unit = units < static_cast<uint64_t>(a.runs - 1);
-  const dim3 grid(by_unit ? static_cast<unsigned>(units) : static_cast<unsigned>(a.runs - 1),
-                  static_cast<unsigned>((cols + 15) / 16), R / 64);
-  if (a.runs > 1) latent_join_kernel<T, R, S::kCols><<<grid, 256, 0, stream>>>(a, S::kBias, by_unit);
+  const int cols = std::max(1, S::kCols / a.heads) * a.heads;
+  if (a.joins == 0) return;
+  // Many parts to a unit: four wavefronts share them (32 sessions of 40 columns, 16
+  // parts on the average and 46 at most: 15 us without).
+  const bool split = a.runs > 12 * a.joins;
+  const dim3 grid(static_cast<unsigned>(a.joins), static_cast<unsigned>((cols + 15) / 16),
+                  split ? R / 16 : R / 64);
+  if (split) latent_join_kernel<T, R, S::kCols, true><<<grid, 256, 0, stream>>>(a, S::kBias);
+  else latent_join_kernel<T, R, S::kCols, false><<<grid, 256, 0, stream>>>(a, S::kBias);
 }
 
 template <class T, int R, int P>
-static void launch_latent(const LatentArgs& a, int cols, uint64_t units, hipStream_t stream) {
-  if (cols == 16) launch_cols<T, R, P, 16, 4, 4>(a, units, stream);
-  else if (cols == 32) launch_cols<T, R, P, 16, 2, 4>(a, units, stream);
-  else if (cols == 64) launch_cols<T, R, P, 16, R == 512 ? 2 : 1, R == 512 ? 8 : 4>(a, units, stream);
-  else launch_cols<T, R, P, 16, 1, 8>(a, units, stream);
+static void launch_latent(const LatentArgs& a, int cols, hipStream_t stream) {
+  if (cols == 16) launch_cols<T, R, P, 16, 4, 4>(a, stream);
+  else if (cols == 32) launch_cols<T, R, P, 16, 2, 4>(a, stream);
+  else if (cols == 64) launch_cols<T, R, P, 16, R == 512 ? 2 : 1, R == 512 ? 8 : 4>(a, stream);
+  else launch_cols<T, R, P, 16, 1, 8>(a, stream);
 }
 
 template <class T>
@@ -399,7 +421,9 @@ extern "C" int grm_hip_latent_plan(const grm_kv_batch_desc* b, void* work, uint6
   for (int k = 0; k < 2; ++k) {
     a.runs[k] = l.runs[k];
     a.starts[k] = l.starts[k];
+    a.joins[k] = l.joins[k];
     a.at_starts[k] = l.at_starts[k];
+    a.at_joins[k] = l.at_joins[k];
   }
   a.at_units = l.at_units;
   a.at_first = l.at_first;
@@ -471,6 +495,7 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
   a.at_units = l.at_units;
   a.at_first = l.at_first;
   a.at_starts = l.at_starts[per - 1];
+  a.at_joins = l.at_joins[per - 1];
   a.scale = softmax_scale;
   a.requests = b->requests;
   a.width = b->table_width;
@@ -481,19 +506,18 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
   a.rope = c->rope;
   a.block_log2 = block_log2(c->block_tokens);
   a.runs = l.runs[per - 1];
-  a.slices = l.slices;
-  a.per = per;
+  a.joins = l.joins[per - 1];
   const auto s = static_cast<hipStream_t>(stream);
   const bool bf = c->dtype == grm::kBF16;
   if (!cores) {
     if (bf) launch_latent_any<BF16>(a, s);
     else launch_latent_any<F16>(a, s);
   } else if (c->rank == 512) {
-    if (bf) launch_latent<BF16, 512, 64>(a, l.cols, l.cap_units, s);
-    else launch_latent<F16, 512, 64>(a, l.cols, l.cap_units, s);
+    if (bf) launch_latent<BF16, 512, 64>(a, l.cols, s);
+    else launch_latent<F16, 512, 64>(a, l.cols, s);
   } else {
-    if (bf) launch_latent<BF16, 256, 32>(a, l.cols, l.cap_units, s);
-    else launch_latent<F16, 256, 32>(a, l.cols, l.cap_units, s);
+    if (bf) launch_latent<BF16, 256, 32>(a, l.cols, s);
+    else launch_latent<F16, 256, 32>(a, l.cols, s);
   }
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();

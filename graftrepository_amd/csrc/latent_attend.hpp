@@ -58,10 +58,8 @@ struct LatentDeal {
 };
 
 struct LatentHead {
-  LatentDeal deal[2];  // with one and two blocks to a CU
-  int32_t units;
   int32_t row_units;
-  int32_t pad[6];
+  int32_t pad[15];
 };
 static_assert(sizeof(LatentHead) == 64, "the lists behind it stay aligned");
 
@@ -83,22 +81,29 @@ struct LatentStart {
 };
 static_assert(sizeof(LatentStart) == 64, "one line");
 
+// A unit that ends of runs cut: its parts are run `from`'s second and the first of
+// those up to `to`.  tokens 0: none.
+struct LatentJoin {
+  int32_t from, to, row, tokens;
+};
+
 typedef const __attribute__((address_space(4))) LatentHead* ConstLatentHead;
 typedef const __attribute__((address_space(4))) LatentUnit* ConstLatentUnit;
 typedef const __attribute__((address_space(4))) LatentStart* ConstLatentStart;
+typedef const __attribute__((address_space(4))) LatentJoin* ConstLatentJoin;
 typedef const __attribute__((address_space(4))) RowUnit* ConstRowUnit;
 typedef const __attribute__((address_space(4))) int64_t* ConstLong;
 
 // Sizes and places of the latent schedule, from host-known fields alone.
 struct LatentLayout {
   int cols;          // columns to a block: 16, 32, 64 or 128
-  int slices;        // blocks that share a unit's columns
   int unit_tokens;   // tokens to a unit
   int runs[2];       // with one and two blocks to a CU
   int starts[2];     // entries of the list that blocks begin with
+  int joins[2];      // and of the list of joins
   uint64_t cap_units, cap_rows;
   int32_t reach;
-  uint64_t at_units, at_first, at_starts[2], at_unit_scan, at_row_scan, at_rows, bytes;
+  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_rows, bytes;
 };
 
 int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out);
@@ -114,10 +119,10 @@ struct LatentArgs {
   const char* work;
   float* parts;
   int64_t q_token, q_head, out_token, out_head;  // strides
-  uint64_t blocks, at_units, at_first, at_starts;
+  uint64_t blocks, at_units, at_first, at_starts, at_joins;
   float scale;
   int32_t requests, width, tokens, window, heads, rank, rope, block_log2;
-  int32_t runs, slices, per;  // per: blocks to a CU
+  int32_t runs, joins;
 };
 
 // Rows of nobody: what a tile has where there is no block.  Written by no one.
@@ -269,20 +274,7 @@ __host__ __device__ constexpr size_t latent_part_floats(int cols, int rank) {
   return static_cast<size_t>(cols) * (rank + 2);
 }
 
-// The unit that tile t lies in.
-__device__ inline int last_of_units(ConstLong firsts, int n, int64_t t) {
-  int lo = 0, len = n;
-  while (len > 1) {
-    const int half = len >> 1;
-    if (firsts[lo + half] <= t) lo += half;
-    len -= half;
-  }
-  return lo;
-}
-
-__device__ inline size_t latent_part(int run, int which, int slices, int slice) {
-  return (static_cast<size_t>(run) * 2 + which) * slices + slice;
-}
+__device__ inline size_t latent_part(int run, int which) { return static_cast<size_t>(run) * 2 + which; }
 
 template <class T, int R, int P, int W, int G, int NW>
 __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void latent_attend_kernel(LatentArgs a) {
@@ -294,11 +286,8 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % W, h = lane / W;
   const int group = wave / S::kColGroups, col_group = wave % S::kColGroups;
-  // Blocks go to the eight XCDs in turn: a unit's slices are on one, as neighbouring
-  // runs are, since they read the same rows.
-  const int nth = static_cast<int>(blockIdx.x / 8), slice = nth % a.slices;
   const auto* start = reinterpret_cast<ConstLatentStart>(reinterpret_cast<uintptr_t>(a.work) + a.at_starts) +
-                      (nth / a.slices * 8 + blockIdx.x % 8);
+                      blockIdx.x;
   const int run = start->run;
   if (run < 0) return;
   const int64_t begin = start->begin, end = start->end;
@@ -341,7 +330,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
     const bool is_whole = first >= begin && last <= end;
     const int which = first >= begin ? 1 : 0;
     at = stop;
-    const int col0 = slice * S::kCols, cols = min(S::kCols, tokens * a.heads - col0);
+    const int cols = tokens * a.heads;
     if (cols <= 0) continue;
     wait_loads<0>();  // the last unit's stores: loads are counted from here
     const int first_seen = a.window > 0 ? max(0, first_pos + 1 - a.window) : 0;
@@ -361,8 +350,8 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       x.h = lane / W;
       x.col = W * col_group + x.c;
       x.mine = x.col < cols;
-      x.token = x.mine ? (col0 + x.col) / a.heads : tokens - 1;
-      x.head = x.mine ? col0 + x.col - x.token * a.heads : 0;
+      x.token = x.mine ? x.col / a.heads : tokens - 1;
+      x.head = x.mine ? x.col - x.token * a.heads : 0;
       x.pos = first_pos + x.token;
       return x;
     };
@@ -658,7 +647,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
     l += poison;
     // ---- the groups' results together, and out
     const Column x = column();
-    float* part = a.parts + latent_part(run, which, a.slices, slice) * latent_part_floats(S::kCols, R);
+    float* part = a.parts + latent_part(run, which) * latent_part_floats(S::kCols, R);
     constexpr int kVecs = S::kAcc / 4;
     auto write = [&](auto value, int d_first, int d_last, int d_step) {
       if (!x.mine) return;
@@ -770,59 +759,44 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
   }
 }
 
-// Joins the parts of cut units: block x is unit x's or, where there are fewer ends of
-// runs than units, those of the unit that the end of run x cuts first; it takes 16
-// columns and 64 values of each, a wavefront 16 of them, as they lie in a part.
-template <class T, int R, int COLS>
-__global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bias, int by_unit) {
-  const auto* head = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
-  const LatentDeal deal = {head->deal[a.per - 1].each, head->deal[a.per - 1].used, head->deal[a.per - 1].rem};
-  const auto* units = reinterpret_cast<ConstLatentUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_units);
-  const auto* firsts = reinterpret_cast<ConstLong>(reinterpret_cast<uintptr_t>(a.work) + a.at_first);
-  int u = static_cast<int>(blockIdx.x);
-  if (by_unit) {
-    if (u >= head->units) return;
-  } else {
-    if (u + 1 >= deal.used) return;
-    u = last_of_units(firsts, head->units, deal.begin(u + 1));
-  }
-  const int64_t first = firsts[u], last = firsts[u + 1];
-  const int from = by_unit ? deal.run(first) : static_cast<int>(blockIdx.x), to = deal.run(last - 1);
-  if (to == from) return;
-  // an end before this one cuts it too, or it begins with the run after
-  if (!by_unit && (first < deal.begin(from) || first >= deal.begin(from + 1))) return;
-  const int from_which = first >= deal.begin(from) ? 1 : 0;
+// Joins the parts of a cut unit.  A wavefront takes 16 columns and 16 values of each,
+// as they lie in a part, and all parts, or (SPLIT) a fourth of them.  (What it needs is
+// one line of the plan's: with the unit and its runs looked up here, 24 units of 128
+// columns and 11 parts took 32 us, now 23.)
+template <class T, int R, int COLS, bool SPLIT>
+__global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bias) {
+  const auto* j = reinterpret_cast<ConstLatentJoin>(reinterpret_cast<uintptr_t>(a.work) + a.at_joins) + blockIdx.x;
+  const int from = j->from, to = j->to, row = j->row, cols = j->tokens * a.heads;
+  if (16 * static_cast<int>(blockIdx.y) >= cols) return;
   const int lane = __lane_id(), wave = static_cast<int>(threadIdx.x) / kWave;
   const int col = 16 * static_cast<int>(blockIdx.y) + lane % 16;
-  const int d = 64 * static_cast<int>(blockIdx.z) + 16 * wave + lane / 16 * 4;
-  if (col >= units[u].tokens * a.heads) return;
-  const int slice = col / COLS, c = col - slice * COLS;
-  const int at = latent_part_at(R, c, d);
-  auto part = [&](int r) {
-    return a.parts + latent_part(r, r == from ? from_which : 0, a.slices, slice) * latent_part_floats(COLS, R);
-  };
+  const int d = 16 * (SPLIT ? static_cast<int>(blockIdx.z) : 4 * static_cast<int>(blockIdx.z) + wave) + lane / 16 * 4;
+  const bool mine = col < cols;
+  const int at = latent_part_at(R, col, d);
+  auto part = [&](int r) { return a.parts + latent_part(r, r == from) * latent_part_floats(COLS, R); };
   float m = -INFINITY, l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int kBatch = 8;  // parts whose loads go out together
-  for (int r0 = from; r0 <= to; r0 += kBatch) {
+  constexpr int kBatch = SPLIT ? 8 : 12;  // parts whose loads go out together
+  constexpr int kEvery = SPLIT ? 4 : 1;
+  for (int r0 = from + (SPLIT ? wave : 0); r0 <= to && mine; r0 += kBatch * kEvery) {
     float pm[kBatch], pl[kBatch];
     f32x4 po[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const float* p = part(min(r0 + k, to));
-      pm[k] = p[COLS * R + c];
-      pl[k] = p[COLS * (R + 1) + c];
+      const float* p = part(min(r0 + k * kEvery, to));
+      pm[k] = p[COLS * R + col];
+      pl[k] = p[COLS * (R + 1) + col];
       po[k] = *reinterpret_cast<const f32x4*>(p + at);
     }
     float m2 = m;
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) m2 = r0 + k <= to ? fmaxf(m2, pm[k]) : m2;
+    for (int k = 0; k < kBatch; ++k) m2 = r0 + k * kEvery <= to ? fmaxf(m2, pm[k]) : m2;
     const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
     o *= keep;
     l = l == l ? l * keep : l;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (r0 + k <= to) {
+      if (r0 + k * kEvery <= to) {
         // nothing seen: sums of 0 (or NaN, which stays)
         const float f = pm[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[k] - m2);
         o += po[k] * f;
@@ -831,13 +805,32 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bi
     }
     m = m2;
   }
+  if constexpr (SPLIT) {
+    __shared__ f32x4 s_o[4][kWave];
+    __shared__ float s_m[4][kWave], s_l[4][kWave];
+    s_o[wave][lane] = o;
+    s_m[wave][lane] = m;
+    s_l[wave][lane] = l;
+    __syncthreads();
+    if (wave) return;
+    m = fmaxf(fmaxf(s_m[0][lane], s_m[1][lane]), fmaxf(s_m[2][lane], s_m[3][lane]));
+    l = 0.0f;
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = s_m[w][lane] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][lane] - m);
+      o += s_o[w][lane] * f;
+      l += s_l[w][lane] == s_l[w][lane] ? s_l[w][lane] * f : NAN;
+    }
+  }
+  if (!mine) return;
   const bool empty = m == -INFINITY && l == 0.0f;
   const int token = col / a.heads, h = col - token * a.heads;
-  latent_put<T>(static_cast<uint16_t*>(a.out) + static_cast<int64_t>(units[u].row + token) * a.out_token +
+  latent_put<T>(static_cast<uint16_t*>(a.out) + static_cast<int64_t>(row + token) * a.out_token +
                     static_cast<int64_t>(h) * a.out_head + d,
                 o, 1.0f / l, empty);
   if (a.lse && d == 0) {
-    a.lse[static_cast<size_t>(units[u].row + token) * a.heads + h] = latent_lse<T>(m, l, bias);
+    a.lse[static_cast<size_t>(row + token) * a.heads + h] = latent_lse<T>(m, l, bias);
   }
 }
 
