@@ -137,8 +137,9 @@ SIGNATURES = {
     "grm_hip_latent_attend": (i32, [vp, vp, vp, u64, vp, i64, i64, vp, i64, i64, vp,
                                     ctypes.c_float, vp, u64, vp]),
     "grm_hip_latent_expand": (i32, [vp, vp, i32, i32, i32, vp, i32, i32, vp, vp, u64, vp, vp, vp]),
+    "grm_hip_rows_attend_bytes": (i32, [vp, i32, i32, vp]),
     "grm_hip_rows_attend": (i32, [vp, vp, u64, i32, i32, i32, vp, i64, i64, vp, i64, i64, vp, i64,
-                                  i64, u64, vp, vp, vp, i64, i64, vp, ctypes.c_float, vp]),
+                                  i64, u64, vp, vp, vp, i64, i64, vp, ctypes.c_float, vp, u64, vp]),
     "grm_hip_synth_int8_rows": (i32, [u64, u64, u64, i32, vp, i32, vp, vp]),
 }
 

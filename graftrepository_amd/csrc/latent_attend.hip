@@ -21,6 +21,12 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
   }
   l.cap_units = std::min(rows, rows / l.unit_tokens + busy);
   l.cap_rows = std::min(rows, rows / kRowUnit + busy);
+  // Pieces of dense rows are no shorter than a fourth of the even share (all tiles x
+  // heads / 2 blocks to a CU), and only longer units are cut.
+  const uint64_t even = 2 * static_cast<uint64_t>(cus) / b->heads + 1;
+  l.cap_items = l.cap_rows + 4 * even;
+  l.cap_parts = std::min(l.cap_items, 8 * even);
+  l.cap_row_joins = std::min(l.cap_rows, l.cap_parts / 2);
   l.reach = static_cast<int32_t>(std::min<int64_t>(
       static_cast<int64_t>(b->table_width) * b->block_tokens, 2 * static_cast<int64_t>(kMaxLen)));
   auto place = [&l](uint64_t bytes) {
@@ -39,7 +45,10 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
   }
   l.at_unit_scan = place((reqs + 1) * 4);
   l.at_row_scan = place((reqs + 1) * 4);
-  l.at_rows = place(l.cap_rows * sizeof(RowUnit));
+  l.at_lengths = place(l.cap_rows * 4);
+  l.at_cuts = place(l.cap_items * sizeof(RowItem));
+  l.at_items = place(l.cap_items * sizeof(RowItem));
+  l.at_row_joins = place(l.cap_row_joins * sizeof(RowJoin));
   *out = l;
   return 0;
 }
@@ -55,8 +64,10 @@ struct LatentPlanArgs {
   const int32_t* cu_new;
   char* work;
   int32_t requests, tokens, window, reach, unit_tokens, cap_units, cap_rows;
+  int32_t heads, slots, cap_items, cap_parts, cap_row_joins;
   int32_t runs[2], starts[2], joins[2];
-  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_rows;
+  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_lengths, at_cuts,
+      at_items, at_row_joins;
 };
 
 // Exclusive sum over the block; the total in *sum.  Two barriers.
@@ -109,7 +120,6 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
   auto* head = reinterpret_cast<LatentHead*>(a.work);
   auto* units = reinterpret_cast<LatentUnit*>(a.work + a.at_units);
   auto* firsts = reinterpret_cast<int64_t*>(a.work + a.at_first);
-  auto* row_units = reinterpret_cast<RowUnit*>(a.work + a.at_rows);
 
   // units and row units before each request; sums past an int end at the lists'
   // ends, which are never that long
@@ -159,14 +169,8 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
     }
     tiles += sum;
   }
-  for (int i = tid; i < n_rows; i += kPlanThreads) {
-    RowUnit u;
-    unit_of(row_at, i, kRowUnit, &u);
-    row_units[i] = u;
-  }
   if (tid == 0) {
     firsts[n_units] = tiles;
-    head->row_units = n_rows;
   }
   __syncthreads();  // the lists are read back by other threads of this block
   for (int k = 0; k < 2; ++k) {
@@ -221,6 +225,128 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
       done += static_cast<int>(sum);
     }
     for (int i = done + tid; i < a.joins[k]; i += kPlanThreads) joins[i] = LatentJoin{};
+  }
+
+  // ---- attention over dense rows
+  int* lengths = reinterpret_cast<int*>(a.work + a.at_lengths);
+  auto* cuts = reinterpret_cast<RowItem*>(a.work + a.at_cuts);
+  auto* items = reinterpret_cast<RowItem*>(a.work + a.at_items);
+  auto* row_joins = reinterpret_cast<RowJoin*>(a.work + a.at_row_joins);
+  auto row_unit = [&](int i, RowItem* u) {
+    unit_of(row_at, i, kRowUnit, u);
+    const int first = a.window > 0 ? max(0, u->pos + 1 - a.window) : 0;
+    return u->tokens > 0 ? max(1, (u->pos + u->tokens - first / kLatentTile * kLatentTile + kLatentTile - 1) / kLatentTile) : 0;
+  };
+  int64_t all = 0, sum;
+  int longest = 0;
+  for (int i = tid; i < n_rows; i += kPlanThreads) {
+    RowItem u;
+    lengths[i] = row_unit(i, &u);
+    all += lengths[i];
+    longest = max(longest, lengths[i]);
+  }
+  __shared__ int s_count[8], s_high[8], s_low[8], s_longest;
+  if (tid < 8) {
+    s_count[tid] = 0;
+    s_high[tid] = 0;
+    s_low[tid] = kMaxLen;
+  }
+  if (tid == 0) s_longest = 0;
+  block_sum<int64_t>(all, &all, scratch);
+  atomicMax(&s_longest, longest);
+  __syncthreads();
+  longest = s_longest;
+  // The longest share of a piece: of eight parts of the even share the one by which
+  // blocks, that take pieces longest first, are through first (as the wide units of
+  // the 8-bit cache are cut).  Four tiles are added to a piece for its start and
+  // end, which a piece of several has more of.
+  const float even = static_cast<float>(all) * a.heads / a.slots;
+  const float kOf[8] = {1.25f, 1.0f, 0.75f, 0.625f, 0.5f, 0.4f, 1.0f / 3.0f, 0.25f};
+  auto share_of = [&](int k) {
+    return max(kRowLeast, static_cast<int>(ceilf(fmaxf(even * kOf[k], 1.0f))));
+  };
+  int share = longest;
+  if (even < static_cast<float>(longest)) {
+    const int k = tid / 128;
+    const float part = 1.0f / static_cast<float>(share_of(k));
+    int count = 0, high = 0, low = kMaxLen;
+    for (int i = tid % 128; i < n_rows; i += 128) {
+      if (lengths[i] == 0) continue;
+      const float cut = fmaxf(1.0f, ceilf(static_cast<float>(lengths[i]) * part));
+      const int each = static_cast<int>(ceilf(static_cast<float>(lengths[i]) / cut));
+      count += static_cast<int>(cut);
+      high = max(high, each);
+      low = min(low, each);
+    }
+    atomicAdd(&s_count[k], count);
+    atomicMax(&s_high[k], high);
+    atomicMin(&s_low[k], low);
+    __syncthreads();
+    float best = INFINITY;
+    for (int c = -1; c < 8; ++c) {  // (-1: none is cut)
+      constexpr float kEnds = 4.0f, kJoin = 4.0f;
+      const float n = c < 0 ? static_cast<float>(n_rows) * a.heads : static_cast<float>(s_count[c]) * a.heads;
+      const float extra = c < 0 ? 0.0f : static_cast<float>(s_count[c] - n_rows) * a.heads;
+      const float rounds = n / a.slots, open = ceilf(rounds) - rounds;
+      const float low_of = c < 0 ? 1.0f : static_cast<float>(s_low[c]);
+      const float est = fmaxf((static_cast<float>(all) * a.heads + kEnds * n + 2.0f * kJoin * extra) / a.slots +
+                                  open * (low_of + kEnds),
+                              static_cast<float>(c < 0 ? longest : s_high[c]) + kEnds);
+      if (est < best) {
+        best = est;
+        share = c < 0 ? longest : share_of(c);
+      }
+    }
+  }
+  share = max(share, 1);
+  int done_items = 0, done_parts = 0, done_joins = 0;
+  for (int base = 0; base < n_rows; base += kPlanThreads) {
+    const int i = base + tid;
+    RowItem u{};
+    int cut = 0, n = 0;
+    if (i < n_rows) {
+      n = row_unit(i, &u);
+      cut = n > 0 ? (n + share - 1) / share : 0;
+    }
+    const int at = done_items + static_cast<int>(block_sum<int64_t>(cut, &sum, scratch));
+    done_items += static_cast<int>(sum);
+    const int part = done_parts + static_cast<int>(block_sum<int64_t>(cut > 1 ? cut : 0, &sum, scratch));
+    done_parts += static_cast<int>(sum);
+    const int join = done_joins + static_cast<int>(block_sum<int64_t>(cut > 1, &sum, scratch));
+    done_joins += static_cast<int>(sum);
+    // The even share bounds all three lists; a unit past them would be one piece.
+    const bool whole = cut <= 1 || part + cut > a.cap_parts || join >= a.cap_row_joins;
+    for (int p = 0; p < cut && at + p < a.cap_items; ++p) {
+      RowItem v = u;
+      v.piece = whole ? 0 : p;
+      v.pieces = whole ? 1 : cut;
+      v.part = whole ? -1 : part + p;
+      v.tiles = whole ? n : (n + cut - 1) / cut;
+      if (whole && p) v.tokens = 0;
+      cuts[at + p] = v;
+    }
+    if (cut > 1 && join < a.cap_row_joins) row_joins[join] = RowJoin{u.row, whole ? 0 : u.tokens, part, whole ? 0 : cut};
+  }
+  __syncthreads();
+  // Longest first, where a block can sort them.
+  const int n_items = min(done_items, a.cap_items);
+  int* keys = s_units;
+  if (n_items <= kPlanThreads) {
+    const int mine = tid < n_items ? cuts[tid].tiles : 0;
+    __syncthreads();
+    keys[tid] = mine;
+    __syncthreads();
+    if (tid < n_items) {
+      int rank = 0;
+      for (int i = 0; i < n_items; ++i) rank += keys[i] > mine || (keys[i] == mine && i < tid);
+      items[rank] = cuts[tid];
+    }
+  } else {
+    for (int i = tid; i < n_items; i += kPlanThreads) items[i] = cuts[n_items - 1 - i];
+  }
+  if (tid == 0) {
+    head->row_items = n_items;
+    head->row_joins = min(done_joins, a.cap_row_joins);
   }
 }
 
@@ -418,6 +544,11 @@ extern "C" int grm_hip_latent_plan(const grm_kv_batch_desc* b, void* work, uint6
   a.unit_tokens = l.unit_tokens;
   a.cap_units = static_cast<int32_t>(l.cap_units);
   a.cap_rows = static_cast<int32_t>(l.cap_rows);
+  a.heads = b->heads;
+  a.slots = l.runs[1];
+  a.cap_items = static_cast<int32_t>(l.cap_items);
+  a.cap_parts = static_cast<int32_t>(l.cap_parts);
+  a.cap_row_joins = static_cast<int32_t>(l.cap_row_joins);
   for (int k = 0; k < 2; ++k) {
     a.runs[k] = l.runs[k];
     a.starts[k] = l.starts[k];
@@ -429,7 +560,10 @@ extern "C" int grm_hip_latent_plan(const grm_kv_batch_desc* b, void* work, uint6
   a.at_first = l.at_first;
   a.at_unit_scan = l.at_unit_scan;
   a.at_row_scan = l.at_row_scan;
-  a.at_rows = l.at_rows;
+  a.at_lengths = l.at_lengths;
+  a.at_cuts = l.at_cuts;
+  a.at_items = l.at_items;
+  a.at_row_joins = l.at_row_joins;
   latent_plan_kernel<<<1, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();

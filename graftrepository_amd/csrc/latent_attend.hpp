@@ -44,6 +44,7 @@ constexpr int kLatentTile = 32;     // rows to a tile
 constexpr int kLatentCols = 128;    // columns to a unit, at most
 constexpr int kLatentLeast = 4;     // tiles to a run, at least
 constexpr int kRowUnit = 128;       // tokens to a unit of attention over dense rows
+constexpr int kRowLeast = 16;       // tiles to a piece of such a unit, at least
 
 // Tiles dealt to runs, equal to within one, kLatentLeast at least: `used` runs, of
 // which the first `rem` have one more than `each`.
@@ -58,8 +59,9 @@ struct LatentDeal {
 };
 
 struct LatentHead {
-  int32_t row_units;
-  int32_t pad[15];
+  int32_t row_items;
+  int32_t row_joins;
+  int32_t pad[14];
 };
 static_assert(sizeof(LatentHead) == 64, "the lists behind it stay aligned");
 
@@ -68,8 +70,16 @@ struct LatentUnit {
   int32_t request, row, tokens, pos;
   int32_t tile_lo, pad[3];
 };
-struct RowUnit {
+// Attention over dense rows: tokens of a request from `row` on against piece
+// `piece` of `pieces` of the rows they see.  part: where the result goes (of each
+// head), -1 where the piece is all.
+struct RowItem {
   int32_t request, row, tokens, pos;
+  int32_t piece, pieces, part, tiles;
+};
+// A unit in pieces: its parts are consecutive.
+struct RowJoin {
+  int32_t row, tokens, part, parts;
 };
 
 // What a block begins with, in the order of the blocks: its run's tiles, and the
@@ -91,7 +101,8 @@ typedef const __attribute__((address_space(4))) LatentHead* ConstLatentHead;
 typedef const __attribute__((address_space(4))) LatentUnit* ConstLatentUnit;
 typedef const __attribute__((address_space(4))) LatentStart* ConstLatentStart;
 typedef const __attribute__((address_space(4))) LatentJoin* ConstLatentJoin;
-typedef const __attribute__((address_space(4))) RowUnit* ConstRowUnit;
+typedef const __attribute__((address_space(4))) RowItem* ConstRowItem;
+typedef const __attribute__((address_space(4))) RowJoin* ConstRowJoin;
 typedef const __attribute__((address_space(4))) int64_t* ConstLong;
 
 // Sizes and places of the latent schedule, from host-known fields alone.
@@ -102,8 +113,10 @@ struct LatentLayout {
   int starts[2];     // entries of the list that blocks begin with
   int joins[2];      // and of the list of joins
   uint64_t cap_units, cap_rows;
+  uint64_t cap_items, cap_parts, cap_row_joins;  // of attention over dense rows
   int32_t reach;
-  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_rows, bytes;
+  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_lengths, at_cuts,
+      at_items, at_row_joins, bytes;
 };
 
 int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out);

@@ -197,7 +197,8 @@ struct RowsArgs {
   const int32_t* starts;  // NULL: 0
   const char* work;
   int64_t q_token, q_head, k_row, k_head, v_row, v_head, out_token, out_head;
-  uint64_t at_rows;
+  float* parts;
+  uint64_t at_items, at_row_joins;
   float scale;
   int32_t requests, tokens, window, heads, key_dim, value_dim, rows;
 };
@@ -220,38 +221,48 @@ __device__ inline KeyRows key_rows(const RowsArgs& a, int request) {
 // 128 tokens of a head to a block, 32 to a wavefront, against tiles of 32 rows that
 // all four read from LDS: the layout and the softmax of latent_attend.hpp, with a
 // head's own keys and values.
+//
+// In a wavefront, vector work stands beside matrix work: a tile's weights are made
+// between the instructions of the next tile's first product (each of which takes the
+// matrix cores eight times as long as its issue).  So a tile's keys are read one tile before its
+// values: three tiles of keys in LDS and four of values, two blocks to a CU.
 template <class T, int DK, int DV>
 struct RowsShape {
   static constexpr int kKeyBytes = (2 * DK + 127) / 128 * 128;  // of a row in LDS
   static constexpr int kValueBytes = 2 * DV;
-  static constexpr int kStage = kLatentTile * (kKeyBytes + kValueBytes);
-  static constexpr int kStages = 3;
+  static constexpr int kKeyTile = kLatentTile * kKeyBytes, kValueTile = kLatentTile * kValueBytes;
+  static constexpr int kKeyStages = 3, kValueStages = 4;
+  static constexpr int kValuesAt = kKeyStages * kKeyTile;
+  static constexpr int kLds = kValuesAt + kValueStages * kValueTile;
   // direct loads of a wavefront
-  static constexpr int kKeyLoads = kLatentTile * kKeyBytes / 4096, kValueLoads = kLatentTile * kValueBytes / 4096;
+  static constexpr int kKeyLoads = kKeyTile / 4096, kValueLoads = kValueTile / 4096;
   static constexpr int kLoads = kKeyLoads + kValueLoads;
   static constexpr int kSteps = DK / 16, kTilesD = DV / 32;
   static constexpr bool kBf = T::code == kBF16;
   static constexpr float kSlack = kBf ? 8.0f : 2.0f, kBias = kBf ? 0.0f : 13.0f;
 };
 
+// Floats of a part: its sums as the wavefronts have them, maxima, sums of weights.
+__host__ __device__ constexpr size_t rows_part_floats(int value_dim) {
+  return static_cast<size_t>(kRowUnit) * (value_dim + 2);
+}
+
 template <class T, int DK, int DV>
 __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   typedef RowsShape<T, DK, DV> S;
   typedef LatentShape<T, 256, 32, 32, 1, 4> L;  // chunks' places and weights' rounding
-  static_assert(S::kKeyLoads * 4096 == kLatentTile * S::kKeyBytes &&
-                    S::kValueLoads * 4096 == kLatentTile * S::kValueBytes,
+  static_assert(S::kKeyLoads * 4096 == S::kKeyTile && S::kValueLoads * 4096 == S::kValueTile,
                 "whole loads to a wavefront");
-  __shared__ __align__(1024) char ring[S::kStages * S::kStage];
+  __shared__ __align__(1024) char ring[S::kLds];
   __shared__ uint32_t s_bad[2];
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % 32, h = lane / 32;
   const auto* plan = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
-  // the last units of a request see most: they go first
-  const int head = static_cast<int>(blockIdx.x % a.heads);
-  const int unit = plan->row_units - 1 - static_cast<int>(blockIdx.x / a.heads);
-  if (unit < 0) return;
-  const auto* u = reinterpret_cast<ConstRowUnit>(reinterpret_cast<uintptr_t>(a.work) + a.at_rows) + unit;
-  const int tokens = u->tokens, first_pos = u->pos, unit_row = u->row;
+  // (heads go to the XCDs in turn with their blocks)
+  const int head = static_cast<int>(blockIdx.x % a.heads), nth = static_cast<int>(blockIdx.x / a.heads);
+  if (nth >= plan->row_items) return;
+  const auto* u = reinterpret_cast<ConstRowItem>(reinterpret_cast<uintptr_t>(a.work) + a.at_items) + nth;
+  const int tokens = u->tokens, first_pos = u->pos, unit_row = u->row, part = u->part;
   if (tokens <= 0) return;
   const KeyRows keys = key_rows(a, u->request);
   const int last_pos = first_pos + tokens - 1;
@@ -260,9 +271,6 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   // columns: tokens; positions are counted from the rows' first
   const bool mine = 32 * wave + c < tokens;
   const int token = min(32 * wave + c, tokens - 1);
-  const int pos = first_pos + token - keys.start;
-  const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-  const int seen_to = min(pos, keys.count - 1);
   const int wave_last = first_pos + min(32 * wave + 31, tokens - 1) - keys.start;
   const int wave_first = first_pos + min(32 * wave, tokens - 1) - keys.start;
   const int wave_from = a.window > 0 ? max(0, wave_first + 1 - a.window) : 0;
@@ -271,9 +279,11 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   const int block_first = first_pos - keys.start;
   const int all_from = a.window > 0 ? max(0, last_pos - keys.start + 1 - a.window) : 0;
   const int block_from = a.window > 0 ? max(0, block_first + 1 - a.window) : 0;
-  const int tile_lo = block_from / kLatentTile;
-  const int tile_hi = (min(last_pos - keys.start + 1, keys.count) + kLatentTile - 1) / kLatentTile;
-  const int n = max(0, tile_hi - tile_lo);
+  const int seen_lo = block_from / kLatentTile;
+  const int seen_hi = max(seen_lo, (min(last_pos - keys.start + 1, keys.count) + kLatentTile - 1) / kLatentTile);
+  const int tile_lo = seen_lo + static_cast<int>(static_cast<int64_t>(seen_hi - seen_lo) * u->piece / u->pieces);
+  const int tile_hi = seen_lo + static_cast<int>(static_cast<int64_t>(seen_hi - seen_lo) * (u->piece + 1) / u->pieces);
+  const int n = tile_hi - tile_lo;
 
   // Offsets of this lane's rows in a tile, which stay; a tile past the rows' end has
   // its last row again.
@@ -290,20 +300,37 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   };
 #pragma unroll
   for (int j = 0; j < S::kLoads; ++j) offsets[j] = offset_of(j, kLatentTile);
-  auto issue = [&](int i) {
-    const uint32_t to = lds_address(ring) + (i % S::kStages) * S::kStage;
-    const int key0 = (tile_lo + i) * kLatentTile;
-    const int64_t first = keys.first + key0;
-    const char* k = reinterpret_cast<const char*>(a.k + first * a.k_row + head * a.k_head);
-    const char* v = reinterpret_cast<const char*>(a.v + first * a.v_row + head * a.v_head);
-    const bool cut = key0 + kLatentTile > keys.count;
+  // Loads are issued tile after tile: where the next one's rows are, and its places.
+  const int64_t row0 = keys.first + static_cast<int64_t>(tile_lo) * kLatentTile;
+  const char* next_k = reinterpret_cast<const char*>(a.k + row0 * a.k_row + head * a.k_head);
+  const char* next_v = reinterpret_cast<const char*>(a.v + row0 * a.v_row + head * a.v_head);
+  const int64_t k_step = 2 * kLatentTile * a.k_row, v_step = 2 * kLatentTile * a.v_row;
+  uint32_t to_k = lds_address(ring) + wave * S::kKeyLoads * 1024;
+  uint32_t to_v = lds_address(ring) + S::kValuesAt + wave * S::kValueLoads * 1024;
+  const uint32_t end_k = to_k + S::kKeyStages * S::kKeyTile, end_v = to_v + S::kValueStages * S::kValueTile;
+  int rows_left = keys.count - tile_lo * kLatentTile;
+  auto issue = [&]() {
+    if (rows_left >= kLatentTile) {
 #pragma unroll
-    for (int j = 0; j < S::kLoads; ++j) {
-      const bool key = j < S::kKeyLoads;
-      const uint32_t at = key ? (wave * S::kKeyLoads + j) * 1024
-                              : kLatentTile * S::kKeyBytes + (wave * S::kValueLoads + j - S::kKeyLoads) * 1024;
-      load_direct(key ? k : v, cut ? offset_of(j, keys.count - 1 - key0) : offsets[j], to + at);
+      for (int j = 0; j < S::kLoads; ++j) {
+        const bool key = j < S::kKeyLoads;
+        load_direct(key ? next_k : next_v, offsets[j], key ? to_k + j * 1024 : to_v + (j - S::kKeyLoads) * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < S::kLoads; ++j) {
+        const bool key = j < S::kKeyLoads;
+        load_direct(key ? next_k : next_v, offset_of(j, rows_left - 1),
+                    key ? to_k + j * 1024 : to_v + (j - S::kKeyLoads) * 1024);
+      }
     }
+    next_k += k_step;
+    next_v += v_step;
+    rows_left -= kLatentTile;
+    to_k += S::kKeyTile;
+    if (to_k == end_k) to_k -= S::kKeyStages * S::kKeyTile;
+    to_v += S::kValueTile;
+    if (to_v == end_v) to_v -= S::kValueStages * S::kValueTile;
   };
 
   u32x4 q[S::kSteps];
@@ -312,10 +339,8 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s) q[s] = *reinterpret_cast<const u32x4*>(from + 16 * s);
   }
-#pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) {
-    if (i < n) issue(i);
-  }
+  if (n > 0) issue();
+  if (n > 1) issue();
   // In registers before the loop, so that a stage waits for rows only.
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s) asm volatile("" : "+v"(q[s]));
@@ -323,7 +348,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   const int key_row = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
   const int k_at = key_row * S::kKeyBytes + 16 * (h ^ L::template turn<S::kKeyBytes>(key_row));
   const int i16 = lane % 16, v_row = 16 * h + i16 / 4;
-  const int v_at = kLatentTile * S::kKeyBytes + v_row * S::kValueBytes + 8 * (i16 & 1) +
+  const int v_at = S::kValuesAt + v_row * S::kValueBytes + 8 * (i16 & 1) +
                    16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ L::template turn<S::kValueBytes>(v_row));
   f32x16 o[S::kTilesD];
 #pragma unroll
@@ -333,59 +358,114 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   }
   float m = -INFINITY, l = 0.0f, poison = 0.0f;
   const float mul = a.scale * kLog2e;
-
-  for (int i = 0; i < n; ++i) {
-    if (i + S::kStages - 2 < n) wait_loads<(S::kStages - 2) * S::kLoads>();
-    else wait_loads<0>();
-    block_barrier();
-    if (i + S::kStages - 1 < n) issue(i + S::kStages - 1);
+  // Exponents' arguments of the tile whose scores were made last: score * scale_by +
+  // shift.
+  float score[16], scale_by = 1.0f, shift = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) score[e] = -INFINITY;
+  auto active = [&](int i) {  // some column of this wavefront's sees a row of tile i
     const int key0 = (tile_lo + i) * kLatentTile;
-    char* stage = ring + (i % S::kStages) * S::kStage;
-    // Where some column does not see all rows, values that are no finite numbers
-    // (which a weight of 0 would not keep out) are taken from LDS, and the rows
-    // that had them noted.
-    const bool partly = key0 < all_from || key0 + kLatentTile - 1 > min(block_first, keys.count - 1);
-    uint32_t bad = 0;
-    if (threadIdx.x == 0) s_bad[(i + 1) & 1] = 0;  // all have read it before this stage
-    if (partly) {
-      constexpr uint32_t kLo = S::kBf ? 0x7f80u : 0x7c00u, kHi = kLo << 16;
-#pragma unroll
-      for (int at = 16 * static_cast<int>(threadIdx.x); at < kLatentTile * S::kValueBytes; at += 4096) {
-        u32x4* p = reinterpret_cast<u32x4*>(stage + kLatentTile * S::kKeyBytes + at);
-        u32x4 v = *p;
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if ((v[e] & kLo) == kLo) {
-            v[e] &= 0xffff0000u;
-            odd = true;
-          }
-          if ((v[e] & kHi) == kHi) {
-            v[e] &= 0xffffu;
-            odd = true;
-          }
-        }
-        if (odd) {
-          *p = v;
-          atomicOr(&s_bad[i & 1], 1u << (at / S::kValueBytes));
-        }
-      }
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-      block_barrier();
-      bad = s_bad[i & 1];
-    }
-    if (!busy || key0 > wave_last || key0 + kLatentTile <= wave_from) continue;
+    return busy && i >= 0 && i < n && key0 <= wave_last && key0 + kLatentTile > wave_from;
+  };
 
+  int k_slot = 0, v_slot = 0;  // of tile i + 1
+  // Step i: scores of tile i + 1 beside the weights of tile i, then tile i's values.
+  for (int i = -1; i < n; ++i) {
+    uint32_t bad = 0;
+    if (i + 1 < n) {
+      if (i + 2 < n) wait_loads<S::kLoads>();
+      else wait_loads<0>();
+      block_barrier();
+      if (i + 3 < n) issue();
+      // Where some column does not see all rows, values that are no finite numbers
+      // (which a weight of 0 would not keep out) are taken from LDS, and the rows
+      // that had them noted.
+      const int key0 = (tile_lo + i + 1) * kLatentTile;
+      const bool partly = key0 < all_from || key0 + kLatentTile - 1 > min(block_first, keys.count - 1);
+      if (threadIdx.x == 0) s_bad[i & 1] = 0;  // all have read it before this step
+      if (partly) {
+        constexpr uint32_t kLo = S::kBf ? 0x7f80u : 0x7c00u, kHi = kLo << 16;
+        char* values = ring + S::kValuesAt + v_slot;
+#pragma unroll
+        for (int at = 16 * static_cast<int>(threadIdx.x); at < S::kValueTile; at += 4096) {
+          u32x4* p = reinterpret_cast<u32x4*>(values + at);
+          u32x4 v = *p;
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if ((v[e] & kLo) == kLo) {
+              v[e] &= 0xffff0000u;
+              odd = true;
+            }
+            if ((v[e] & kHi) == kHi) {
+              v[e] &= 0xffffu;
+              odd = true;
+            }
+          }
+          if (odd) {
+            *p = v;
+            atomicOr(&s_bad[(i + 1) & 1], 1u << (at / S::kValueBytes));
+          }
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        block_barrier();
+        bad = s_bad[(i + 1) & 1];
+      }
+    }
+    const bool weigh = active(i), next = active(i + 1);
+    const char* k_stage = ring + k_slot;
+    const char* v_stage = ring + (v_slot ? v_slot : S::kValueStages * S::kValueTile) - S::kValueTile;  // of tile i
+    k_slot = k_slot == (S::kKeyStages - 1) * S::kKeyTile ? 0 : k_slot + S::kKeyTile;
+    v_slot = v_slot == (S::kValueStages - 1) * S::kValueTile ? 0 : v_slot + S::kValueTile;
+    if (!weigh && !next) continue;
+
+    // (scores of a tile that is not active are of whatever is in LDS, and not used)
     f32x16 s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+    u32x4 w[2];
+    auto weights = [&](int pair) {
+      const int e = 2 * pair;
+      const float x = __builtin_amdgcn_exp2f(fmaf(score[e], scale_by, shift));
+      const float y = __builtin_amdgcn_exp2f(fmaf(score[e + 1], scale_by, shift));
+      l += x;
+      l += y;
+      w[e / 8][e % 8 / 2] = L::weights(x, y);
+    };
     in_order<S::kSteps, 4>(
         [&](int k) {
           constexpr int kIn = S::kKeyBytes % 256 == 0 ? 8 : 4;  // steps to whole turns
-          return *reinterpret_cast<const u32x4*>(stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
+          return *reinterpret_cast<const u32x4*>(k_stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
         },
-        [&](int k, u32x4 f) { s = mfma<S::kBf>(f, q[k], s); });
-    float score[16], top = s[0], low = s[0];
+        [&](int k, u32x4 f) {
+          s = mfma<S::kBf>(f, q[k], s);
+#pragma unroll
+          for (int pair = 8 * k / S::kSteps; pair < 8 * (k + 1) / S::kSteps; ++pair) weights(pair);
+        });
+    if (weigh) {
+      in_order<2 * S::kTilesD, 4>(
+          [&](int k) {
+            const int d = k % S::kTilesD, x0 = 2 * (k / S::kTilesD);
+            constexpr int kIn = S::kValueBytes % 256 == 0 ? 4 : 2;
+            auto four = [&](int x) {  // keys 4 x on of the lane's sixteen
+              return read_transposed(v_stage + ((v_at ^ (64 * (d % kIn) + 16 * x)) + 64 * (d / kIn * kIn) +
+                                              4 * x * S::kValueBytes));
+            };
+            const u32x2 lo = four(x0), hi = four(x0 + 1);
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+          },
+          [&](int k, u32x4 f) {
+            o[k % S::kTilesD] = mfma<S::kBf>(f, w[k / S::kTilesD], o[k % S::kTilesD]);
+          });
+    }
+    if (!next) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) score[e] = -INFINITY;
+      scale_by = 1.0f;
+      continue;
+    }
+    const int key0 = (tile_lo + i + 1) * kLatentTile;
+    float top = s[0], low = s[0];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       score[e] = s[e];
@@ -394,12 +474,15 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     }
     const bool whole = key0 >= wave_all_from && mul >= 0.0f &&
                        key0 + kLatentTile - 1 <= min(wave_first, keys.count - 1);
-    float scale_by = mul;  // of a score in the exponent
+    scale_by = mul;
     // NaN and +inf make their column's sums so by themselves; a weight of 0 would hide
     // -inf.
     if (whole && bad == 0 && !__any(low < -3.4028235e38f)) {
       top *= mul;
     } else {
+      const int pos = first_pos + token - keys.start;
+      const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+      const int seen_to = min(pos, keys.count - 1);
       top = -INFINITY;
       scale_by = 1.0f;
 #pragma unroll
@@ -423,33 +506,29 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
       l *= keep;
       m = m2;
     }
-    const float shift = S::kBias - (m == -INFINITY ? 0.0f : m);
-    u32x4 w[2];
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const float x = __builtin_amdgcn_exp2f(fmaf(score[e], scale_by, shift));
-      const float y = __builtin_amdgcn_exp2f(fmaf(score[e + 1], scale_by, shift));
-      l += x;
-      l += y;
-      w[e / 8][e % 8 / 2] = L::weights(x, y);
-    }
-    in_order<2 * S::kTilesD, 4>(
-        [&](int k) {
-          const int d = k / 2;
-          constexpr int kIn = S::kValueBytes % 256 == 0 ? 4 : 2;
-          auto four = [&](int t) {  // keys 4 t on of the eight
-            const int x = 2 * (k % 2) + t;
-            return read_transposed(stage + ((v_at ^ (64 * (d % kIn) + 16 * x)) + 64 * (d / kIn * kIn) +
-                                            4 * x * S::kValueBytes));
-          };
-          const u32x2 lo = four(0), hi = four(1);
-          return u32x4{lo[0], lo[1], hi[0], hi[1]};
-        },
-        [&](int k, u32x4 f) { o[k / 2] = mfma<S::kBf>(f, w[k % 2], o[k / 2]); });
+    shift = S::kBias - (m == -INFINITY ? 0.0f : m);
   }
   l += __shfl_xor(l, 32);
   poison += __shfl_xor(poison, 32);
   l += poison;
+  if (part >= 0) {
+    float* to = a.parts + (static_cast<int64_t>(part) * a.heads + head) * rows_part_floats(DV);
+#pragma unroll
+    for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[d][4 * k + e];
+        *reinterpret_cast<f32x4*>(to + (((wave * S::kTilesD + d) * 4 + k) * kWave + lane) * 4) = v;
+      }
+    }
+    if (h == 0) {
+      to[kRowUnit * DV + 32 * wave + c] = m;
+      to[kRowUnit * (DV + 1) + 32 * wave + c] = l;
+    }
+    return;
+  }
   if (!mine) return;
   const float inv = 1.0f / l;
   const bool empty = m == -INFINITY && l == 0.0f;
@@ -458,18 +537,70 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   for (int d = 0; d < S::kTilesD; ++d) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      u32x2 v;
+      f32x4 v;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t lo = T::put(empty ? 0.0f : o[d][4 * k + 2 * e] * inv);
-        const uint32_t hi = T::put(empty ? 0.0f : o[d][4 * k + 2 * e + 1] * inv);
-        v[e] = lo | (hi << 16);
-      }
-      *reinterpret_cast<u32x2*>(to + 32 * d + 8 * k) = v;
+      for (int e = 0; e < 4; ++e) v[e] = o[d][4 * k + e];
+      latent_put<T>(to + 32 * d + 8 * k, v, inv, empty);
     }
   }
   if (a.lse && h == 0) {
     a.lse[static_cast<int64_t>(unit_row + token) * a.heads + head] = latent_lse<T>(m, l, S::kBias);
+  }
+}
+
+// Joins the parts of units in pieces: 1024 values to a step of a block, as they lie.
+template <class T, int DV>
+__global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a, float bias) {
+  const auto* plan = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
+  const auto* joins = reinterpret_cast<ConstRowJoin>(reinterpret_cast<uintptr_t>(a.work) + a.at_row_joins);
+  constexpr int kSteps = kRowUnit * DV / 1024;
+  const int64_t all = static_cast<int64_t>(plan->row_joins) * a.heads * kSteps;
+  for (int64_t step = blockIdx.x; step < all; step += gridDim.x) {
+    const int piece = static_cast<int>(step % kSteps), head = static_cast<int>(step / kSteps % a.heads);
+    const auto* j = joins + step / kSteps / a.heads;
+    const int at = 256 * piece + static_cast<int>(threadIdx.x);  // of four values
+    const int lane = at % kWave, k = at / kWave % 4, d = at / (4 * kWave) % (DV / 32), wave = at / (DV * 8);
+    const int token = 32 * wave + lane % 32, x = 32 * d + 8 * k + 4 * (lane / 32);
+    if (token >= j->tokens) continue;
+    auto part = [&](int p) {
+      return a.parts + (static_cast<int64_t>(j->part + p) * a.heads + head) * rows_part_floats(DV);
+    };
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kBatch = 4;  // parts whose loads go out together
+    for (int p0 = 0; p0 < j->parts; p0 += kBatch) {
+      float pm[kBatch], pl[kBatch];
+      f32x4 po[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        const float* p = part(min(p0 + e, j->parts - 1));
+        pm[e] = p[kRowUnit * DV + token];
+        pl[e] = p[kRowUnit * (DV + 1) + token];
+        po[e] = *reinterpret_cast<const f32x4*>(p + 4 * at);
+      }
+      float m2 = m;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) m2 = p0 + e < j->parts ? fmaxf(m2, pm[e]) : m2;
+      const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
+      o *= keep;
+      l = l == l ? l * keep : l;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        if (p0 + e < j->parts) {
+          // nothing seen: sums of 0 (or NaN, which stays)
+          const float f = pm[e] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm[e] - m2);
+          o += po[e] * f;
+          l += pl[e] == pl[e] ? pl[e] * f : NAN;
+        }
+      }
+      m = m2;
+    }
+    const bool empty = m == -INFINITY && l == 0.0f;
+    latent_put<T>(a.out + static_cast<int64_t>(j->row + token) * a.out_token + head * a.out_head + x, o,
+                  1.0f / l, empty);
+    if (a.lse && x == 0) {
+      a.lse[static_cast<int64_t>(j->row + token) * a.heads + head] = latent_lse<T>(m, l, bias);
+    }
   }
 }
 
@@ -564,13 +695,32 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowsArgs a) {
   }
 }
 
+// The matrix cores' dims of keys and values.
+static bool rows_cores(int key_dim, int value_dim) {
+  return (key_dim == 192 && value_dim == 128) || (key_dim == 96 && value_dim == 64) ||
+         (key_dim == 128 && value_dim == 128);
+}
+
+template <class T, int DK, int DV>
+static void launch_rows_cores(const RowsArgs& a, const LatentLayout& l, hipStream_t s) {
+  rows_attend_kernel<T, DK, DV><<<static_cast<unsigned>(l.cap_items * a.heads), 256, 0, s>>>(a);
+  if (l.cap_row_joins == 0) return;
+  const uint64_t steps = l.cap_row_joins * a.heads * (kRowUnit * DV / 1024);
+  rows_join_kernel<T, DV><<<static_cast<unsigned>(std::min<uint64_t>(steps, 4 * l.runs[1])), 256, 0, s>>>(
+      a, RowsShape<T, DK, DV>::kBias);
+}
+
 template <class T>
-static void launch_rows(const RowsArgs& a, uint64_t units, bool scheduled, hipStream_t s) {
-  const auto grid = static_cast<unsigned>(units * a.heads);
-  if (scheduled && a.key_dim == 192 && a.value_dim == 128) rows_attend_kernel<T, 192, 128><<<grid, 256, 0, s>>>(a);
-  else if (scheduled && a.key_dim == 96 && a.value_dim == 64) rows_attend_kernel<T, 96, 64><<<grid, 256, 0, s>>>(a);
-  else if (scheduled && a.key_dim == 128 && a.value_dim == 128) rows_attend_kernel<T, 128, 128><<<grid, 256, 0, s>>>(a);
-  else rows_any_kernel<T><<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads)), 256, 0, s>>>(a);
+static void launch_rows(const RowsArgs& a, const LatentLayout& l, bool cores, hipStream_t s) {
+  if (!cores) {
+    rows_any_kernel<T><<<dim3(static_cast<unsigned>(a.tokens), static_cast<unsigned>(a.heads)), 256, 0, s>>>(a);
+  } else if (a.key_dim == 192) {
+    launch_rows_cores<T, 192, 128>(a, l, s);
+  } else if (a.key_dim == 96) {
+    launch_rows_cores<T, 96, 64>(a, l, s);
+  } else {
+    launch_rows_cores<T, 128, 128>(a, l, s);
+  }
 }
 
 }  // namespace kv
@@ -629,6 +779,19 @@ extern "C" int grm_hip_latent_expand(const grm_latent_desc* c, const void* weigh
   return 0;
 }
 
+extern "C" int grm_hip_rows_attend_bytes(const grm_kv_batch_desc* b, int key_dim, int value_dim,
+                                         uint64_t* out_bytes) {
+  if (!out_bytes) return grm::fail(-1, "null output pointer");
+  GRM_CHECK_RC(check_batch(b, false));
+  LatentLayout l;
+  GRM_CHECK_RC(latent_layout_of(b, &l));
+  *out_bytes = rows_cores(key_dim, value_dim) && l.cap_row_joins
+                   ? l.cap_parts * b->heads * rows_part_floats(value_dim) * 4
+                   : 0;
+  grm::clear_error();
+  return 0;
+}
+
 extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work, uint64_t work_bytes,
                                    int dtype, int key_dim, int value_dim, const void* q,
                                    int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -636,7 +799,8 @@ extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work,
                                    int64_t v_row_stride, int64_t v_head_stride, uint64_t rows,
                                    const int32_t* cu_rows, const int32_t* starts, void* out,
                                    int64_t out_token_stride, int64_t out_head_stride, float* lse,
-                                   float softmax_scale, void* stream) {
+                                   float softmax_scale, void* scratch, uint64_t scratch_bytes,
+                                   void* stream) {
   GRM_CHECK_RC(check_batch(b, true));
   if (b->kv_heads != 1) return grm::fail(-1, "a latent cache's batch has one kv head");
   if (dtype != grm::kBF16 && dtype != grm::kF16) return grm::fail(-1, "dense rows are BF16 or F16");
@@ -679,7 +843,9 @@ extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work,
   a.v_head = v_head_stride;
   a.out_token = out_token_stride;
   a.out_head = out_head_stride;
-  a.at_rows = l.at_rows;
+  a.parts = static_cast<float*>(scratch);
+  a.at_items = l.at_items;
+  a.at_row_joins = l.at_row_joins;
   a.scale = softmax_scale;
   a.requests = b->requests;
   a.tokens = b->tokens;
@@ -690,10 +856,17 @@ extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work,
   a.rows = static_cast<int32_t>(rows);
   // the matrix cores' kernel takes a tile's rows by 32-bit offsets
   const auto near = [](int64_t stride) { return stride >= 0 && stride < (1ll << 25); };
-  const bool scheduled = l.cap_rows * static_cast<uint64_t>(b->heads) < (1ull << 31) && near(k_row_stride) && near(v_row_stride);
+  const bool cores = rows_cores(key_dim, value_dim) && near(k_row_stride) && near(v_row_stride) &&
+                     l.cap_items * static_cast<uint64_t>(b->heads) < (1ull << 31);
+  if (cores && l.cap_row_joins) {
+    const uint64_t need = l.cap_parts * b->heads * rows_part_floats(value_dim) * 4;
+    if (!scratch || !aligned16(scratch) || scratch_bytes < need) {
+      return grm::fail(-1, "scratch is smaller than grm_hip_rows_attend_bytes, or not 16-byte aligned");
+    }
+  }
   const auto s = static_cast<hipStream_t>(stream);
-  if (dtype == grm::kBF16) launch_rows<BF16>(a, l.cap_rows, scheduled, s);
-  else launch_rows<F16>(a, l.cap_rows, scheduled, s);
+  if (dtype == grm::kBF16) launch_rows<BF16>(a, l, cores, s);
+  else launch_rows<F16>(a, l, cores, s);
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();
   return 0;

@@ -284,10 +284,18 @@ def attend_rows(batch: KvBatch, q, k, v, cu_rows, *, starts=None,
     lse, lp = _statistics(q, lse, return_lse, (d.tokens, d.heads), batch.device, stream)
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(dk)
+    key = ("rows", dk, dv)
+    need = batch._scratch.get(key)
+    if need is None:
+        got = u64()
+        _lib.check(_call(batch._lib.grm_hip_rows_attend_bytes, q, batch.device, batch._ref, dk, dv,
+                         ctypes.byref(got)), "rows scratch size")
+        need = batch._scratch[key] = got.value
     on = batch._on(q, stream)
     rc = _call(batch._lib.grm_hip_rows_attend, q, batch.device, batch._ref, batch._latent_at,
                batch._latent_bytes, _lib.DTYPE_CODES[name], dk, dv, *at_q, *at_k, *at_v, rows, cu,
-               sp, *to, lp, softmax_scale, on)
+               sp, *to, lp, softmax_scale,
+               batch._scratch_on(q, need, on, stream) if need else None, need, on)
     if rc:
         _lib.check(rc, "rows attend")
     _written(out, result, on)

@@ -725,6 +725,10 @@ int grm_hip_latent_expand(const grm_latent_desc* cache, const void* weight, int 
                           const int32_t* starts, const int32_t* cu_rows, uint64_t rows, void* k_out,
                           void* v_out, void* stream);
 
+/* Bytes of scratch one grm_hip_rows_attend call of these dims needs (may be 0). */
+int grm_hip_rows_attend_bytes(const grm_kv_batch_desc* batch, int key_dim, int value_dim,
+                              uint64_t* out_bytes);
+
 /* Causal attention of the step's tokens over dense rows: q [tokens][heads]
  * [key_dim], k [rows][heads][key_dim], v [rows][heads][value_dim], out [tokens]
  * [heads][value_dim] of dtype (BF16, F16); strides in elements, multiples of 16
@@ -735,7 +739,7 @@ int grm_hip_latent_expand(const grm_latent_desc* cache, const void* weight, int 
  * are multiples of 8, at most 512.  A value that is not finite leaves no finite
  * result in its channel of the tokens that see its row (other channels of theirs
  * may be NaN too), and changes no other token's.  For prompts: 128 tokens of a
- * head go through its rows alone. */
+ * head are a unit of work, whose rows are cut where there are few. */
 int grm_hip_rows_attend(const grm_kv_batch_desc* batch, const void* work, uint64_t work_bytes,
                         int dtype, int key_dim, int value_dim, const void* q,
                         int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -743,7 +747,7 @@ int grm_hip_rows_attend(const grm_kv_batch_desc* batch, const void* work, uint64
                         int64_t v_row_stride, int64_t v_head_stride, uint64_t rows,
                         const int32_t* cu_rows, const int32_t* starts, void* out,
                         int64_t out_token_stride, int64_t out_head_stride, float* lse,
-                        float softmax_scale, void* stream);
+                        float softmax_scale, void* scratch, uint64_t scratch_bytes, void* stream);
 
 /* ---- Synthetic workload keys (host only) --------------------------------
  * Rows [row0, row0 + rows) of the synthetic INT8 key stream: each row's dim

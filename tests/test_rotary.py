@@ -249,7 +249,7 @@ def test_bad_expanded_calls_are_refused():
         b = batch or one_head()
         return lib.grm_hip_rows_attend(ctypes.byref(b), work, 1 << 40, dtype, dk, dv, q, 256, 64, k,
                                        stride, 64, v, 256, 64, n, cu, None, out, 256, 64, None, scale,
-                                       None)
+                                       None, 0, None)
     for kw in (dict(batch=one_head(kv_heads=2)), dict(work=None), dict(work=0x1008), dict(dtype=0),
                dict(dk=0), dict(dk=12), dict(dk=520), dict(dv=4), dict(dv=1024), dict(q=None),
                dict(k=None), dict(v=None), dict(cu=None), dict(out=None), dict(q=0x1002),
