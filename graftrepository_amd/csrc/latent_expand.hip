@@ -360,18 +360,106 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   const float mul = a.scale * kLog2e;
   // Exponents' arguments of the tile whose scores were made last: score * scale_by +
   // shift.
-  float score[16], scale_by = 1.0f, shift = 0.0f;
+  f32x16 scores;
+  float scale_by = 1.0f, shift = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) score[e] = -INFINITY;
-  auto active = [&](int i) {  // some column of this wavefront's sees a row of tile i
-    const int key0 = (tile_lo + i) * kLatentTile;
-    return busy && i >= 0 && i < n && key0 <= wave_last && key0 + kLatentTile > wave_from;
+  for (int e = 0; e < 16; ++e) scores[e] = -INFINITY;
+  int k_slot = 0, v_slot = 0;  // of tile i + 1
+
+  // The weights of `now` beside the scores of the tile in k_stage, which are left in
+  // `then` (not `now`).
+  auto weigh_and_score = [&](const char* k_stage, const f32x16& now, f32x16& then, u32x4 (&w)[2]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) then[e] = 0.0f;
+    in_order<S::kSteps, 4>(
+        [&](int k) {
+          constexpr int kIn = S::kKeyBytes % 256 == 0 ? 8 : 4;  // steps to whole turns
+          return *reinterpret_cast<const u32x4*>(k_stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
+        },
+        [&](int k, u32x4 f) {
+          then = mfma<S::kBf>(f, q[k], then);
+#pragma unroll
+          for (int e = 16 * k / S::kSteps / 2 * 2; e < 16 * (k + 1) / S::kSteps / 2 * 2; e += 2) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(now[e], scale_by, shift));
+            const float y = __builtin_amdgcn_exp2f(fmaf(now[e + 1], scale_by, shift));
+            l += x;
+            l += y;
+            w[e / 8][e % 8 / 2] = L::weights(x, y);
+          }
+        });
+  };
+  auto add_values = [&](const char* v_stage, const u32x4 (&w)[2]) {
+    in_order<2 * S::kTilesD, 4>(
+        [&](int k) {
+          const int d = k % S::kTilesD, x0 = 2 * (k / S::kTilesD);
+          constexpr int kIn = S::kValueBytes % 256 == 0 ? 4 : 2;
+          auto four = [&](int x) {  // keys 4 x on of the lane's sixteen
+            return read_transposed(v_stage + ((v_at ^ (64 * (d % kIn) + 16 * x)) + 64 * (d / kIn * kIn) +
+                                              4 * x * S::kValueBytes));
+          };
+          const u32x2 lo = four(x0), hi = four(x0 + 1);
+          return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        },
+        [&](int k, u32x4 f) {
+          o[k % S::kTilesD] = mfma<S::kBf>(f, w[k / S::kTilesD], o[k % S::kTilesD]);
+        });
+  };
+  // Scores of a tile from key0 on as arguments: what no column sees out of them, and
+  // the reference moved where one passes it.  `whole`: all columns see all rows.
+  auto settle = [&](f32x16& s, int key0, bool whole, uint32_t bad) {
+    float top = s[0], low = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) {
+      top = fmaxf(top, s[e]);
+      low = fminf(low, s[e]);
+    }
+    scale_by = mul;
+    // NaN and +inf make their column's sums so by themselves; a weight of 0 would hide
+    // -inf.
+    if (whole && !__any(low < -3.4028235e38f)) {
+      top *= mul;
+    } else {
+      const int pos = first_pos + token - keys.start;
+      const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+      const int seen_to = min(pos, keys.count - 1);
+      top = -INFINITY;
+      scale_by = 1.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = key0 + 16 * h + e;
+        const bool see = key <= seen_to && key >= seen_from;
+        const bool fine = fabsf(s[e]) <= 3.4028235e38f;
+        poison += see && (!fine || (bad >> (16 * h + e) & 1u)) ? NAN : 0.0f;
+        s[e] = see && fine ? s[e] * mul : -INFINITY;
+        top = fmaxf(top, s[e]);
+      }
+    }
+    if (__any(top > m + S::kSlack)) {
+      float m2 = fmaxf(m, top);
+      m2 = fmaxf(m2, __shfl_xor(m2, 32));
+      const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
+      if (__any(m != -INFINITY)) {
+#pragma unroll
+        for (int d = 0; d < S::kTilesD; ++d) o[d] *= keep;
+      }
+      l *= keep;
+      m = m2;
+      shift = S::kBias - (m == -INFINITY ? 0.0f : m);
+    }
+  };
+  shift = S::kBias;
+  auto turn_slots = [&]() {
+    k_slot = k_slot == (S::kKeyStages - 1) * S::kKeyTile ? 0 : k_slot + S::kKeyTile;
+    v_slot = v_slot == (S::kValueStages - 1) * S::kValueTile ? 0 : v_slot + S::kValueTile;
+  };
+  auto values_before = [&]() {  // of tile i
+    return ring + (v_slot ? v_slot : S::kValueStages * S::kValueTile) - S::kValueTile;
   };
 
-  int k_slot = 0, v_slot = 0;  // of tile i + 1
   // Step i: scores of tile i + 1 beside the weights of tile i, then tile i's values.
-  for (int i = -1; i < n; ++i) {
+  auto step = [&](int i) {
     uint32_t bad = 0;
+    const int key0 = (tile_lo + i + 1) * kLatentTile;
     if (i + 1 < n) {
       if (i + 2 < n) wait_loads<S::kLoads>();
       else wait_loads<0>();
@@ -380,7 +468,6 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
       // Where some column does not see all rows, values that are no finite numbers
       // (which a weight of 0 would not keep out) are taken from LDS, and the rows
       // that had them noted.
-      const int key0 = (tile_lo + i + 1) * kLatentTile;
       const bool partly = key0 < all_from || key0 + kLatentTile - 1 > min(block_first, keys.count - 1);
       if (threadIdx.x == 0) s_bad[i & 1] = 0;  // all have read it before this step
       if (partly) {
@@ -412,102 +499,55 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
         bad = s_bad[(i + 1) & 1];
       }
     }
-    const bool weigh = active(i), next = active(i + 1);
-    const char* k_stage = ring + k_slot;
-    const char* v_stage = ring + (v_slot ? v_slot : S::kValueStages * S::kValueTile) - S::kValueTile;  // of tile i
-    k_slot = k_slot == (S::kKeyStages - 1) * S::kKeyTile ? 0 : k_slot + S::kKeyTile;
-    v_slot = v_slot == (S::kValueStages - 1) * S::kValueTile ? 0 : v_slot + S::kValueTile;
-    if (!weigh && !next) continue;
-
-    // (scores of a tile that is not active are of whatever is in LDS, and not used)
-    f32x16 s;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+    // some column of this wavefront's sees a row of the tile
+    const bool weigh = busy && i >= 0 && key0 - kLatentTile <= wave_last && key0 > wave_from;
+    const bool next = busy && i + 1 < n && key0 <= wave_last && key0 + kLatentTile > wave_from;
+    const char *k_stage = ring + k_slot, *v_stage = values_before();
+    turn_slots();
+    if (!weigh && !next) return;
+    // (scores of a tile that is not looked at are of whatever is in LDS, and not used)
+    f32x16 then;
     u32x4 w[2];
-    auto weights = [&](int pair) {
-      const int e = 2 * pair;
-      const float x = __builtin_amdgcn_exp2f(fmaf(score[e], scale_by, shift));
-      const float y = __builtin_amdgcn_exp2f(fmaf(score[e + 1], scale_by, shift));
-      l += x;
-      l += y;
-      w[e / 8][e % 8 / 2] = L::weights(x, y);
-    };
-    in_order<S::kSteps, 4>(
-        [&](int k) {
-          constexpr int kIn = S::kKeyBytes % 256 == 0 ? 8 : 4;  // steps to whole turns
-          return *reinterpret_cast<const u32x4*>(k_stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
-        },
-        [&](int k, u32x4 f) {
-          s = mfma<S::kBf>(f, q[k], s);
-#pragma unroll
-          for (int pair = 8 * k / S::kSteps; pair < 8 * (k + 1) / S::kSteps; ++pair) weights(pair);
-        });
-    if (weigh) {
-      in_order<2 * S::kTilesD, 4>(
-          [&](int k) {
-            const int d = k % S::kTilesD, x0 = 2 * (k / S::kTilesD);
-            constexpr int kIn = S::kValueBytes % 256 == 0 ? 4 : 2;
-            auto four = [&](int x) {  // keys 4 x on of the lane's sixteen
-              return read_transposed(v_stage + ((v_at ^ (64 * (d % kIn) + 16 * x)) + 64 * (d / kIn * kIn) +
-                                              4 * x * S::kValueBytes));
-            };
-            const u32x2 lo = four(x0), hi = four(x0 + 1);
-            return u32x4{lo[0], lo[1], hi[0], hi[1]};
-          },
-          [&](int k, u32x4 f) {
-            o[k % S::kTilesD] = mfma<S::kBf>(f, w[k / S::kTilesD], o[k % S::kTilesD]);
-          });
-    }
-    if (!next) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) score[e] = -INFINITY;
-      scale_by = 1.0f;
-      continue;
-    }
-    const int key0 = (tile_lo + i + 1) * kLatentTile;
-    float top = s[0], low = s[0];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      score[e] = s[e];
-      top = fmaxf(top, s[e]);
-      low = fminf(low, s[e]);
-    }
-    const bool whole = key0 >= wave_all_from && mul >= 0.0f &&
-                       key0 + kLatentTile - 1 <= min(wave_first, keys.count - 1);
-    scale_by = mul;
-    // NaN and +inf make their column's sums so by themselves; a weight of 0 would hide
-    // -inf.
-    if (whole && bad == 0 && !__any(low < -3.4028235e38f)) {
-      top *= mul;
+    weigh_and_score(k_stage, scores, then, w);
+    if (weigh) add_values(v_stage, w);
+    scores = then;
+    if (next) {
+      settle(scores, key0, key0 >= wave_all_from && mul >= 0.0f && bad == 0 &&
+                               key0 + kLatentTile - 1 <= min(wave_first, keys.count - 1), bad);
     } else {
-      const int pos = first_pos + token - keys.start;
-      const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-      const int seen_to = min(pos, keys.count - 1);
-      top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) scores[e] = -INFINITY;
       scale_by = 1.0f;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = key0 + 16 * h + e;
-        const bool see = key <= seen_to && key >= seen_from;
-        const bool fine = fabsf(score[e]) <= 3.4028235e38f;
-        poison += see && (!fine || (bad >> (16 * h + e) & 1u)) ? NAN : 0.0f;
-        score[e] = see && fine ? score[e] * mul : -INFINITY;
-        top = fmaxf(top, score[e]);
-      }
     }
-    if (__any(top > m + S::kSlack)) {
-      float m2 = fmaxf(m, top);
-      m2 = fmaxf(m2, __shfl_xor(m2, 32));
-      const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
-      if (__any(m != -INFINITY)) {
-#pragma unroll
-        for (int d = 0; d < S::kTilesD; ++d) o[d] *= keep;
-      }
-      l *= keep;
-      m = m2;
+  };
+  // The same where all columns of the block see all rows of both tiles, and the tile
+  // that is loaded is whole: without the questions, which took as long as the products.
+  auto inner_step = [&](int i, f32x16& now, f32x16& then) {
+    wait_loads<S::kLoads>();
+    block_barrier();
+    issue();
+    const char *k_stage = ring + k_slot, *v_stage = values_before();
+    turn_slots();
+    u32x4 w[2];
+    weigh_and_score(k_stage, now, then, w);
+    add_values(v_stage, w);
+    settle(then, (tile_lo + i + 1) * kLatentTile, true, 0);
+  };
+  const int whole_lo = max(0, (all_from + kLatentTile - 1) / kLatentTile - tile_lo);
+  const int whole_hi = (min(block_first, keys.count - 1) + 1) / kLatentTile - tile_lo;  // tiles [lo, hi)
+  const int inner_lo = whole_lo, inner_hi = busy && mul >= 0.0f ? min(whole_hi - 1, n - 4) : 0;
+  int i = -1;
+  for (; i < min(inner_lo, n); ++i) step(i);
+  if (i + 2 <= inner_hi) {
+    f32x16 other;
+    for (; i + 2 <= inner_hi; i += 2) {
+      inner_step(i, scores, other);
+      inner_step(i + 1, other, scores);
     }
-    shift = S::kBias - (m == -INFINITY ? 0.0f : m);
+    // (the flags that steps clear for each other)
+    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
   }
+  for (; i < n; ++i) step(i);
   l += __shfl_xor(l, 32);
   poison += __shfl_xor(poison, 32);
   l += poison;
