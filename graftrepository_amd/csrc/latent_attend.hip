@@ -35,16 +35,15 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
     return at;
   };
   place(sizeof(LatentHead));
-  l.at_units = place(l.cap_units * sizeof(LatentUnit));
-  l.at_first = place((l.cap_units + 1) * 8);
   for (int k = 0; k < 2; ++k) {
+    l.at_units[k] = place(l.cap_units * sizeof(LatentUnit));
+    l.at_first[k] = place((l.cap_units + 1) * 8);
     // a join is of a unit of its own and has an end of a run
     l.joins[k] = static_cast<int>(std::min<uint64_t>(l.runs[k] - 1, l.cap_units));
     l.at_starts[k] = place(static_cast<uint64_t>(l.starts[k]) * sizeof(LatentStart));
     l.at_joins[k] = place(static_cast<uint64_t>(l.joins[k]) * sizeof(LatentJoin));
   }
-  l.at_unit_scan = place((reqs + 1) * 4);
-  l.at_row_scan = place((reqs + 1) * 4);
+  for (int k = 0; k < 3; ++k) l.at_scan[k] = place((reqs + 1) * 4);
   l.at_lengths = place(l.cap_rows * 4);
   l.at_cuts = place(l.cap_items * sizeof(RowItem));
   l.at_items = place(l.cap_items * sizeof(RowItem));
@@ -66,8 +65,8 @@ struct LatentPlanArgs {
   int32_t requests, tokens, window, reach, unit_tokens, cap_units, cap_rows;
   int32_t heads, slots, cap_items, cap_parts, cap_row_joins;
   int32_t runs[2], starts[2], joins[2];
-  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_lengths, at_cuts,
-      at_items, at_row_joins;
+  uint64_t at_units[2], at_first[2], at_starts[2], at_joins[2], at_scan[3], at_lengths, at_cuts, at_items,
+      at_row_joins;
 };
 
 // Exclusive sum over the block; the total in *sum.  Two barriers.
@@ -106,57 +105,49 @@ __device__ inline int last_of(const N* pre, int n, N x) {
   return lo;
 }
 
-// One block, beside nothing: latency (a scan over the requests, one over the
-// units, a search for each run).
-__global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArgs a) {
-  __shared__ int64_t scratch[kPlanWaves];
-  constexpr int kHeld = 4096;  // requests whose sums stay in LDS
-  __shared__ int s_units[kHeld + 1];
-  __shared__ int s_rows[kHeld + 1];
-  const int tid = threadIdx.x;
-  const bool held = a.requests <= kHeld;
-  int* unit_at = held ? s_units : reinterpret_cast<int*>(a.work + a.at_unit_scan);
-  int* row_at = held ? s_rows : reinterpret_cast<int*>(a.work + a.at_row_scan);
-  auto* head = reinterpret_cast<LatentHead*>(a.work);
-  auto* units = reinterpret_cast<LatentUnit*>(a.work + a.at_units);
-  auto* firsts = reinterpret_cast<int64_t*>(a.work + a.at_first);
-
-  // units and row units before each request; sums past an int end at the lists'
-  // ends, which are never that long
-  int64_t units_all = 0, rows_all = 0;
+// Sums over the requests of their units of `each` tokens, exclusive, in `at`; the
+// total (sums past an int end at the lists' ends, which are never that long).
+__device__ inline int64_t scan_units(const LatentPlanArgs& a, int each, int* at, int64_t* scratch) {
+  int64_t all = 0;
   for (int base = 0; base < a.requests; base += kPlanThreads) {
-    const int r = base + tid;
+    const int r = base + threadIdx.x;
     const int fresh = r < a.requests ? clamp_len(a.new_lens[r]) : 0;
     int64_t sum;
-    int64_t v = block_sum<int64_t>((fresh + a.unit_tokens - 1) / a.unit_tokens, &sum, scratch);
-    if (r < a.requests) unit_at[r] = static_cast<int>(min(units_all + v, static_cast<int64_t>(0x7fffffff)));
-    units_all += sum;
-    v = block_sum<int64_t>((fresh + kRowUnit - 1) / kRowUnit, &sum, scratch);
-    if (r < a.requests) row_at[r] = static_cast<int>(min(rows_all + v, static_cast<int64_t>(0x7fffffff)));
-    rows_all += sum;
+    const int64_t v = block_sum<int64_t>((fresh + each - 1) / each, &sum, scratch);
+    if (r < a.requests) at[r] = static_cast<int>(min(all + v, static_cast<int64_t>(0x7fffffff)));
+    all += sum;
   }
-  const int n_units = static_cast<int>(min(units_all, static_cast<int64_t>(a.cap_units)));
-  const int n_rows = static_cast<int>(min(rows_all, static_cast<int64_t>(a.cap_rows)));
-  __syncthreads();
+  return all;
+}
 
-  // Unit i's first token within its request, its rows and how many: those past
-  // the batch's rows are none.
-  auto unit_of = [&](const int* at, int i, int each, auto* u) {
-    u->request = last_of(at, a.requests, i);
-    const int t0 = (i - at[u->request]) * each;
-    const int fresh = clamp_len(a.new_lens[u->request]);
-    u->pos = clamp_len(a.ctx_lens[u->request]) + t0;
-    const int64_t row = static_cast<int64_t>(a.cu_new[u->request]) + t0;
-    u->row = static_cast<int>(min(row, static_cast<int64_t>(a.tokens)));
-    u->tokens = max(0, min(min(each, fresh - t0), a.tokens - u->row));
-  };
+// Unit i's first token within its request, its rows and how many: those past the
+// batch's rows are none.
+template <class U>
+__device__ inline void unit_of(const LatentPlanArgs& a, const int* at, int i, int each, U* u) {
+  u->request = last_of(at, a.requests, i);
+  const int t0 = (i - at[u->request]) * each;
+  const int fresh = clamp_len(a.new_lens[u->request]);
+  u->pos = clamp_len(a.ctx_lens[u->request]) + t0;
+  const int64_t row = static_cast<int64_t>(a.cu_new[u->request]) + t0;
+  u->row = static_cast<int>(min(row, static_cast<int64_t>(a.tokens)));
+  u->tokens = max(0, min(min(each, fresh - t0), a.tokens - u->row));
+}
+
+// Attention over the cache with k + 1 blocks to a CU.
+__device__ inline void plan_cache(const LatentPlanArgs& a, int k, int* at, int64_t* scratch) {
+  const int tid = threadIdx.x;
+  auto* units = reinterpret_cast<LatentUnit*>(a.work + a.at_units[k]);
+  auto* firsts = reinterpret_cast<int64_t*>(a.work + a.at_first[k]);
+  const int n_units = static_cast<int>(
+      min(scan_units(a, a.unit_tokens, at, scratch), static_cast<int64_t>(a.cap_units)));
+  __syncthreads();
   int64_t tiles = 0;
   for (int base = 0; base < n_units; base += kPlanThreads) {
     const int i = base + tid;
     int64_t mine = 0, sum;
     LatentUnit u{};
     if (i < n_units) {
-      unit_of(unit_at, i, a.unit_tokens, &u);
+      unit_of(a, at, i, a.unit_tokens, &u);
       const int first = a.window > 0 ? max(0, u.pos + 1 - a.window) : 0;
       u.tile_lo = first / kLatentTile;
       const int hi = (min(u.pos + u.tokens, a.reach) + kLatentTile - 1) / kLatentTile;
@@ -169,74 +160,77 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
     }
     tiles += sum;
   }
-  if (tid == 0) {
-    firsts[n_units] = tiles;
-  }
+  if (tid == 0) firsts[n_units] = tiles;
   __syncthreads();  // the lists are read back by other threads of this block
-  for (int k = 0; k < 2; ++k) {
-    LatentDeal deal;
-    const int64_t most = (tiles + kLatentLeast - 1) / kLatentLeast;
-    deal.used = static_cast<int>(min(most, static_cast<int64_t>(a.runs[k])));
-    deal.each = deal.used ? tiles / deal.used : 0;
-    deal.rem = deal.used ? static_cast<int>(tiles - deal.each * deal.used) : 0;
-    auto* to = reinterpret_cast<LatentStart*>(a.work + a.at_starts[k]);
-    for (int i = tid; i < a.starts[k]; i += kPlanThreads) {
-      // neighbouring runs to one XCD, to which every eighth entry goes
-      const int xcd = i % 8, nth = i / 8;
-      LatentStart s{};
-      s.run = -1;
-      if (nth < deal.used / 8 + (xcd < deal.used % 8)) {
-        s.run = xcd * (deal.used / 8) + min(xcd, deal.used % 8) + nth;
-        s.begin = deal.begin(s.run);
-        s.end = deal.begin(s.run + 1);
-        s.unit = last_of(firsts, n_units, s.begin);
-        s.first = firsts[s.unit];
-        s.last = firsts[s.unit + 1];
-        const LatentUnit u = units[s.unit];
-        s.request = u.request;
-        s.row = u.row;
-        s.tokens = u.tokens;
-        s.pos = u.pos;
-        s.tile_lo = u.tile_lo;
-      }
-      to[i] = s;
+  LatentDeal deal;
+  const int64_t most = (tiles + kLatentLeast - 1) / kLatentLeast;
+  deal.used = static_cast<int>(min(most, static_cast<int64_t>(a.runs[k])));
+  deal.each = deal.used ? tiles / deal.used : 0;
+  deal.rem = deal.used ? static_cast<int>(tiles - deal.each * deal.used) : 0;
+  auto* to = reinterpret_cast<LatentStart*>(a.work + a.at_starts[k]);
+  for (int i = tid; i < a.starts[k]; i += kPlanThreads) {
+    // neighbouring runs to one XCD, to which every eighth entry goes
+    const int xcd = i % 8, nth = i / 8;
+    LatentStart s{};
+    s.run = -1;
+    if (nth < deal.used / 8 + (xcd < deal.used % 8)) {
+      s.run = xcd * (deal.used / 8) + min(xcd, deal.used % 8) + nth;
+      s.begin = deal.begin(s.run);
+      s.end = deal.begin(s.run + 1);
+      s.unit = last_of(firsts, n_units, s.begin);
+      s.first = firsts[s.unit];
+      s.last = firsts[s.unit + 1];
+      const LatentUnit u = units[s.unit];
+      s.request = u.request;
+      s.row = u.row;
+      s.tokens = u.tokens;
+      s.pos = u.pos;
+      s.tile_lo = u.tile_lo;
     }
-    // Ends of runs that are the first in a unit.
-    auto* joins = reinterpret_cast<LatentJoin*>(a.work + a.at_joins[k]);
-    int done = 0;
-    for (int base = 0; base < deal.used - 1; base += kPlanThreads) {
-      const int e = base + tid;
-      LatentJoin j{};
-      bool cuts = false;
-      if (e < deal.used - 1) {
-        const int64_t at = deal.begin(e + 1);
-        const int u = last_of(firsts, n_units, at);
-        if (firsts[u] < at && firsts[u] >= deal.begin(e)) {
-          cuts = units[u].tokens > 0;
-          j.from = e;
-          j.to = deal.run(firsts[u + 1] - 1);
-          j.row = units[u].row;
-          j.tokens = units[u].tokens;
-        }
-      }
-      int64_t sum;
-      const int64_t v = block_sum<int64_t>(cuts, &sum, scratch);
-      if (cuts) joins[done + v] = j;
-      done += static_cast<int>(sum);
-    }
-    for (int i = done + tid; i < a.joins[k]; i += kPlanThreads) joins[i] = LatentJoin{};
+    to[i] = s;
   }
+  // Ends of runs that are the first in a unit.
+  auto* joins = reinterpret_cast<LatentJoin*>(a.work + a.at_joins[k]);
+  int done = 0;
+  for (int base = 0; base < deal.used - 1; base += kPlanThreads) {
+    const int e = base + tid;
+    LatentJoin j{};
+    bool cuts = false;
+    if (e < deal.used - 1) {
+      const int64_t end = deal.begin(e + 1);
+      const int u = last_of(firsts, n_units, end);
+      if (firsts[u] < end && firsts[u] >= deal.begin(e)) {
+        cuts = units[u].tokens > 0;
+        j.from = e;
+        j.to = deal.run(firsts[u + 1] - 1);
+        j.row = units[u].row;
+        j.tokens = units[u].tokens;
+      }
+    }
+    int64_t sum;
+    const int64_t v = block_sum<int64_t>(cuts, &sum, scratch);
+    if (cuts) joins[done + v] = j;
+    done += static_cast<int>(sum);
+  }
+  for (int i = done + tid; i < a.joins[k]; i += kPlanThreads) joins[i] = LatentJoin{};
+}
 
-  // ---- attention over dense rows
+// Attention over dense rows.
+__device__ inline void plan_rows(const LatentPlanArgs& a, int* at, int64_t* scratch) {
+  const int tid = threadIdx.x;
+  auto* head = reinterpret_cast<LatentHead*>(a.work);
   int* lengths = reinterpret_cast<int*>(a.work + a.at_lengths);
   auto* cuts = reinterpret_cast<RowItem*>(a.work + a.at_cuts);
   auto* items = reinterpret_cast<RowItem*>(a.work + a.at_items);
   auto* row_joins = reinterpret_cast<RowJoin*>(a.work + a.at_row_joins);
   auto row_unit = [&](int i, RowItem* u) {
-    unit_of(row_at, i, kRowUnit, u);
+    unit_of(a, at, i, kRowUnit, u);
     const int first = a.window > 0 ? max(0, u->pos + 1 - a.window) : 0;
     return u->tokens > 0 ? max(1, (u->pos + u->tokens - first / kLatentTile * kLatentTile + kLatentTile - 1) / kLatentTile) : 0;
   };
+  const int n_rows = static_cast<int>(
+      min(scan_units(a, kRowUnit, at, scratch), static_cast<int64_t>(a.cap_rows)));
+  __syncthreads();
   int64_t all = 0, sum;
   int longest = 0;
   for (int i = tid; i < n_rows; i += kPlanThreads) {
@@ -308,7 +302,7 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
       n = row_unit(i, &u);
       cut = n > 0 ? (n + share - 1) / share : 0;
     }
-    const int at = done_items + static_cast<int>(block_sum<int64_t>(cut, &sum, scratch));
+    const int from = done_items + static_cast<int>(block_sum<int64_t>(cut, &sum, scratch));
     done_items += static_cast<int>(sum);
     const int part = done_parts + static_cast<int>(block_sum<int64_t>(cut > 1 ? cut : 0, &sum, scratch));
     done_parts += static_cast<int>(sum);
@@ -316,29 +310,33 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
     done_joins += static_cast<int>(sum);
     // The even share bounds all three lists; a unit past them would be one piece.
     const bool whole = cut <= 1 || part + cut > a.cap_parts || join >= a.cap_row_joins;
-    for (int p = 0; p < cut && at + p < a.cap_items; ++p) {
+    for (int p = 0; p < cut && from + p < a.cap_items; ++p) {
       RowItem v = u;
       v.piece = whole ? 0 : p;
       v.pieces = whole ? 1 : cut;
       v.part = whole ? -1 : part + p;
       v.tiles = whole ? n : (n + cut - 1) / cut;
       if (whole && p) v.tokens = 0;
-      cuts[at + p] = v;
+      cuts[from + p] = v;
     }
     if (cut > 1 && join < a.cap_row_joins) row_joins[join] = RowJoin{u.row, whole ? 0 : u.tokens, part, whole ? 0 : cut};
   }
   __syncthreads();
   // Longest first, where a block can sort them.
   const int n_items = min(done_items, a.cap_items);
-  int* keys = s_units;
+  __shared__ __align__(16) int keys[kPlanThreads];
   if (n_items <= kPlanThreads) {
-    const int mine = tid < n_items ? cuts[tid].tiles : 0;
-    __syncthreads();
+    // all different; no list is so long that pieces reach the bound
+    const int mine = tid < n_items ? min(cuts[tid].tiles, (1 << 21) - 1) * kPlanThreads + kPlanThreads - 1 - tid : -1;
     keys[tid] = mine;
     __syncthreads();
     if (tid < n_items) {
       int rank = 0;
-      for (int i = 0; i < n_items; ++i) rank += keys[i] > mine || (keys[i] == mine && i < tid);
+      for (int i = 0; i < n_items; i += 4) {
+        const auto k = *reinterpret_cast<const u32x4*>(keys + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += static_cast<int>(k[e]) > mine;
+      }
       items[rank] = cuts[tid];
     }
   } else {
@@ -348,6 +346,18 @@ __global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArg
     head->row_items = n_items;
     head->row_joins = min(done_joins, a.cap_row_joins);
   }
+}
+
+// Three blocks, a plan to each: latency (a scan over the requests, one over the units,
+// a search for each run; the cuts of dense rows and their order).
+__global__ __launch_bounds__(kPlanThreads) void latent_plan_kernel(LatentPlanArgs a) {
+  __shared__ int64_t scratch[kPlanWaves];
+  constexpr int kHeld = 4096;  // requests whose sums stay in LDS
+  __shared__ int s_at[kHeld + 1];
+  const int k = blockIdx.x;
+  int* at = a.requests <= kHeld ? s_at : reinterpret_cast<int*>(a.work + a.at_scan[k]);
+  if (k < 2) plan_cache(a, k, at, scratch);
+  else plan_rows(a, at, scratch);
 }
 
 // ------------------------------------------------------- any shape of row
@@ -553,18 +563,17 @@ extern "C" int grm_hip_latent_plan(const grm_kv_batch_desc* b, void* work, uint6
     a.runs[k] = l.runs[k];
     a.starts[k] = l.starts[k];
     a.joins[k] = l.joins[k];
+    a.at_units[k] = l.at_units[k];
+    a.at_first[k] = l.at_first[k];
     a.at_starts[k] = l.at_starts[k];
     a.at_joins[k] = l.at_joins[k];
   }
-  a.at_units = l.at_units;
-  a.at_first = l.at_first;
-  a.at_unit_scan = l.at_unit_scan;
-  a.at_row_scan = l.at_row_scan;
+  for (int k = 0; k < 3; ++k) a.at_scan[k] = l.at_scan[k];
   a.at_lengths = l.at_lengths;
   a.at_cuts = l.at_cuts;
   a.at_items = l.at_items;
   a.at_row_joins = l.at_row_joins;
-  latent_plan_kernel<<<1, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  latent_plan_kernel<<<3, kPlanThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();
   return 0;
@@ -626,8 +635,8 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
   a.out_token = out_token_stride;
   a.out_head = out_head_stride;
   a.blocks = c->blocks;
-  a.at_units = l.at_units;
-  a.at_first = l.at_first;
+  a.at_units = l.at_units[per - 1];
+  a.at_first = l.at_first[per - 1];
   a.at_starts = l.at_starts[per - 1];
   a.at_joins = l.at_joins[per - 1];
   a.scale = softmax_scale;

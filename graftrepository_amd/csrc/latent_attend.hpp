@@ -115,8 +115,8 @@ struct LatentLayout {
   uint64_t cap_units, cap_rows;
   uint64_t cap_items, cap_parts, cap_row_joins;  // of attention over dense rows
   int32_t reach;
-  uint64_t at_units, at_first, at_starts[2], at_joins[2], at_unit_scan, at_row_scan, at_lengths, at_cuts,
-      at_items, at_row_joins, bytes;
+  uint64_t at_units[2], at_first[2], at_starts[2], at_joins[2], at_scan[3], at_lengths, at_cuts, at_items,
+      at_row_joins, bytes;
 };
 
 int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out);

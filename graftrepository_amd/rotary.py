@@ -103,7 +103,9 @@ class Rotary:
             d.magnitude, d.dim, d.layout = magnitude, dim, int(layout == "interleaved")
             d.inverse = int(inverse)
             self._desc[inverse] = d
-        self._ref = ctypes.byref(self._desc[False])
+        self._refs = tuple(ctypes.byref(d) for d in self._desc.values())
+        self._ref = self._refs[0]
+        self._rotate = None  # the library's entry, from the first call on
 
     def apply(self, x, positions, *, start: int = 0, out=None, inverse: bool = False, stream=None):
         """``x`` [tokens, heads, head_dim] (f32, bf16 or f16; any row and head
@@ -111,7 +113,7 @@ class Rotary:
         ``positions`` int32 [tokens]; the others are copied.  ``out`` (x's type
         and shape) may be ``x``.  ``inverse`` undoes it.  Rows whose position is
         below 0 (a batch's rows past its last token) are not written."""
-        shape = tuple(int(n) for n in x.shape)
+        shape = tuple(x.shape)
         if len(shape) != 3:
             raise ValueError(f"x must be [tokens, heads, head_dim], got {shape}")
         start = _size(start, "start")
@@ -123,15 +125,22 @@ class Rotary:
         _same_device(positions, "positions", device)
         if out is None:
             out = _empty(x, shape, name, stream)
-        op, oname, ot, oh = (xp, name, xt, xh) if out is x else _rows(out, "out", shape, "rotation")
-        if oname != name:
-            raise ValueError("out must have x's type")
-        _one_device(x=x, out=out)
+            op, ot, oh = out.data_ptr(), shape[1] * shape[2], shape[2]
+        elif out is x:
+            op, ot, oh = xp, xt, xh
+        else:
+            op, oname, ot, oh = _rows(out, "out", shape, "rotation")
+            if oname != name:
+                raise ValueError("out must have x's type")
+            _one_device(x=x, out=out)
         if shape[0] and shape[1]:
-            _lib.check(_call(_lib.load().grm_hip_rotate, x, device,
-                             ctypes.byref(self._desc[bool(inverse)]), xp, _lib.DTYPE_CODES[name],
-                             xt, xh, op, ot, oh, pos, shape[0], shape[1], shape[2], start,
-                             _stream(x, stream)), "rotate")
+            if self._rotate is None:
+                self._rotate = _lib.load().grm_hip_rotate
+            rc = _call(self._rotate, x, device, self._refs[bool(inverse)], xp,
+                       _lib.DTYPE_CODES[name], xt, xh, op, ot, oh, pos, shape[0], shape[1],
+                       shape[2], start, _stream(x, stream))
+            if rc:
+                _lib.check(rc, "rotate")
         return out
 
 
