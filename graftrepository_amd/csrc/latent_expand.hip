@@ -240,6 +240,12 @@ struct RowsShape {
   static constexpr int kSteps = DK / 16, kTilesD = DV / 32;
   static constexpr bool kBf = T::code == kBF16;
   static constexpr float kSlack = kBf ? 8.0f : 2.0f, kBias = kBf ? 0.0f : 13.0f;
+  // Where a value row's chunks of 16 bytes go (chunk c to c ^ value_turn): a transposed
+  // read takes 64 bytes of each of four rows, which then lie in all 64 banks.  The
+  // same for every fourth row, so that these are a constant apart.
+  static __device__ __forceinline__ int value_turn(int row) {
+    return kValueBytes % 256 == 0 ? 4 * (row & 3) : 4 * (row >> 1 & 1);
+  }
 };
 
 // Floats of a part: its sums as the wavefronts have them, maxima, sums of weights.
@@ -293,7 +299,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     constexpr int kKeyChunks = S::kKeyBytes / 16, kValueChunks = S::kValueBytes / 16;
     const int at = (key ? wave * S::kKeyLoads + j : wave * S::kValueLoads + j - S::kKeyLoads) * kWave + lane;
     const int r = at / (key ? kKeyChunks : kValueChunks), place = at - r * (key ? kKeyChunks : kValueChunks);
-    const int chunk = place ^ (key ? L::template turn<S::kKeyBytes>(r) : L::template turn<S::kValueBytes>(r));
+    const int chunk = place ^ (key ? L::template turn<S::kKeyBytes>(r) : S::value_turn(r));
     // (a row's last places in LDS may be nobody's)
     const int64_t row = static_cast<int64_t>(min(r, last)) * (key ? a.k_row : a.v_row);
     return static_cast<uint32_t>(2 * (row + 8 * (!key || chunk < DK / 8 ? chunk : 0)));
@@ -349,7 +355,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   const int k_at = key_row * S::kKeyBytes + 16 * (h ^ L::template turn<S::kKeyBytes>(key_row));
   const int i16 = lane % 16, v_row = 16 * h + i16 / 4;
   const int v_at = S::kValuesAt + v_row * S::kValueBytes + 8 * (i16 & 1) +
-                   16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ L::template turn<S::kValueBytes>(v_row));
+                   16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ S::value_turn(v_row));
   f32x16 o[S::kTilesD];
 #pragma unroll
   for (int d = 0; d < S::kTilesD; ++d) {
@@ -366,53 +372,72 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   for (int e = 0; e < 16; ++e) scores[e] = -INFINITY;
   int k_slot = 0, v_slot = 0;  // of tile i + 1
 
-  // The weights of `now` beside the scores of the tile in k_stage, which are left in
-  // `then` (not `now`).
-  auto weigh_and_score = [&](const char* k_stage, const f32x16& now, f32x16& then, u32x4 (&w)[2]) {
+  // Both products: the scores of the tile in k_stage, left in `then` (not `now`) with
+  // their extremes, and where `weigh` says so the values in v_stage by the weights of
+  // `now`.  A value's first half needs eight weights, its second the others, so that
+  // weights are made beside all instructions but the last half's, and the extremes
+  // beside those.
+  auto products = [&](auto weigh, const char* k_stage, const char* v_stage, const f32x16& now, f32x16& then,
+                      float& top, float& low) {
+    constexpr int kScores = S::kSteps, kEarly = kScores + S::kTilesD, kAll = kEarly + S::kTilesD;
+    u32x4 w[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) then[e] = 0.0f;
-    in_order<S::kSteps, 4>(
+    in_order<decltype(weigh)::value ? kAll : kScores, 4>(
         [&](int k) {
-          constexpr int kIn = S::kKeyBytes % 256 == 0 ? 8 : 4;  // steps to whole turns
-          return *reinterpret_cast<const u32x4*>(k_stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
-        },
-        [&](int k, u32x4 f) {
-          then = mfma<S::kBf>(f, q[k], then);
-#pragma unroll
-          for (int e = 16 * k / S::kSteps / 2 * 2; e < 16 * (k + 1) / S::kSteps / 2 * 2; e += 2) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(now[e], scale_by, shift));
-            const float y = __builtin_amdgcn_exp2f(fmaf(now[e + 1], scale_by, shift));
-            l += x;
-            l += y;
-            w[e / 8][e % 8 / 2] = L::weights(x, y);
+          if (k < kScores) {
+            constexpr int kIn = S::kKeyBytes % 256 == 0 ? 8 : 4;  // steps to whole turns
+            return *reinterpret_cast<const u32x4*>(k_stage + ((k_at ^ 32 * (k % kIn)) + 32 * (k / kIn * kIn)));
           }
-        });
-  };
-  auto add_values = [&](const char* v_stage, const u32x4 (&w)[2]) {
-    in_order<2 * S::kTilesD, 4>(
-        [&](int k) {
-          const int d = k % S::kTilesD, x0 = 2 * (k / S::kTilesD);
+          const int d = (k - kScores) % S::kTilesD, x0 = 2 * ((k - kScores) / S::kTilesD);
           constexpr int kIn = S::kValueBytes % 256 == 0 ? 4 : 2;
           auto four = [&](int x) {  // keys 4 x on of the lane's sixteen
-            return read_transposed(v_stage + ((v_at ^ (64 * (d % kIn) + 16 * x)) + 64 * (d / kIn * kIn) +
+            return read_transposed(v_stage + ((v_at ^ 64 * (d % kIn)) + 64 * (d / kIn * kIn) +
                                               4 * x * S::kValueBytes));
           };
           const u32x2 lo = four(x0), hi = four(x0 + 1);
           return u32x4{lo[0], lo[1], hi[0], hi[1]};
         },
         [&](int k, u32x4 f) {
-          o[k % S::kTilesD] = mfma<S::kBf>(f, w[k / S::kTilesD], o[k % S::kTilesD]);
+          if (k < kScores) {
+            then = mfma<S::kBf>(f, q[k], then);
+          } else {
+            const int d = (k - kScores) % S::kTilesD;
+            o[d] = mfma<S::kBf>(f, w[k < kEarly ? 0 : 1], o[d]);
+          }
+          if constexpr (decltype(weigh)::value) {
+            if (k < kEarly) {
+#pragma unroll
+              for (int e = 16 * k / kEarly / 2 * 2; e < 16 * (k + 1) / kEarly / 2 * 2; e += 2) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(now[e], scale_by, shift));
+                const float y = __builtin_amdgcn_exp2f(fmaf(now[e + 1], scale_by, shift));
+                l += x;
+                l += y;
+                w[e / 8][e % 8 / 2] = L::weights(x, y);
+              }
+            } else {
+              const int d = k - kEarly;
+              if (d == 0) top = low = then[0];
+#pragma unroll
+              for (int e = 16 * d / S::kTilesD; e < 16 * (d + 1) / S::kTilesD; ++e) {
+                top = fmaxf(top, then[e]);
+                low = fminf(low, then[e]);
+              }
+            }
+          }
         });
+    if constexpr (!decltype(weigh)::value) {
+      top = low = then[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) {
+        top = fmaxf(top, then[e]);
+        low = fminf(low, then[e]);
+      }
+    }
   };
   // Scores of a tile from key0 on as arguments: what no column sees out of them, and
   // the reference moved where one passes it.  `whole`: all columns see all rows.
-  auto settle = [&](f32x16& s, int key0, bool whole, uint32_t bad) {
-    float top = s[0], low = s[0];
-#pragma unroll
-    for (int e = 1; e < 16; ++e) {
-      top = fmaxf(top, s[e]);
-      low = fminf(low, s[e]);
-    }
+  auto settle = [&](f32x16& s, float top, float low, int key0, bool whole, uint32_t bad) {
     scale_by = mul;
     // NaN and +inf make their column's sums so by themselves; a weight of 0 would hide
     // -inf.
@@ -507,12 +532,12 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     if (!weigh && !next) return;
     // (scores of a tile that is not looked at are of whatever is in LDS, and not used)
     f32x16 then;
-    u32x4 w[2];
-    weigh_and_score(k_stage, scores, then, w);
-    if (weigh) add_values(v_stage, w);
+    float top, low;
+    if (weigh) products(std::true_type{}, k_stage, v_stage, scores, then, top, low);
+    else products(std::false_type{}, k_stage, v_stage, scores, then, top, low);
     scores = then;
     if (next) {
-      settle(scores, key0, key0 >= wave_all_from && mul >= 0.0f && bad == 0 &&
+      settle(scores, top, low, key0, key0 >= wave_all_from && mul >= 0.0f && bad == 0 &&
                                key0 + kLatentTile - 1 <= min(wave_first, keys.count - 1), bad);
     } else {
 #pragma unroll
@@ -528,10 +553,9 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
     issue();
     const char *k_stage = ring + k_slot, *v_stage = values_before();
     turn_slots();
-    u32x4 w[2];
-    weigh_and_score(k_stage, now, then, w);
-    add_values(v_stage, w);
-    settle(then, (tile_lo + i + 1) * kLatentTile, true, 0);
+    float top, low;
+    products(std::true_type{}, k_stage, v_stage, now, then, top, low);
+    settle(then, top, low, (tile_lo + i + 1) * kLatentTile, true, 0);
   };
   const int whole_lo = max(0, (all_from + kLatentTile - 1) / kLatentTile - tile_lo);
   const int whole_hi = (min(block_first, keys.count - 1) + 1) / kLatentTile - tile_lo;  // tiles [lo, hi)
