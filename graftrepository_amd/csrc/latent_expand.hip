@@ -253,27 +253,20 @@ __host__ __device__ constexpr size_t rows_part_floats(int value_dim) {
   return static_cast<size_t>(kRowUnit) * (value_dim + 2);
 }
 
-template <class T, int DK, int DV>
-__global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
+// A unit's piece.  Values that are no finite numbers (in a row that no column sees, with
+// a weight of 0; a score of -inf, which would hide its row) take questions at every tile.
+// Without CAREFUL there are none: at its end such a thing shows in the sums or in the
+// least score, nothing is written then, and the answer is false.
+template <class T, int DK, int DV, bool CAREFUL>
+__device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const RowItem& u, char* ring,
+                                             uint32_t* s_bad) {
   typedef RowsShape<T, DK, DV> S;
   typedef LatentShape<T, 256, 32, 32, 1, 4> L;  // chunks' places and weights' rounding
-  static_assert(S::kKeyLoads * 4096 == S::kKeyTile && S::kValueLoads * 4096 == S::kValueTile,
-                "whole loads to a wavefront");
-  __shared__ __align__(1024) char ring[S::kLds];
-  __shared__ uint32_t s_bad[2];
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % 32, h = lane / 32;
-  const auto* plan = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
-  // (heads go to the XCDs in turn with their blocks)
-  const int head = static_cast<int>(blockIdx.x % a.heads), nth = static_cast<int>(blockIdx.x / a.heads);
-  if (nth >= plan->row_items) return;
-  const auto* u = reinterpret_cast<ConstRowItem>(reinterpret_cast<uintptr_t>(a.work) + a.at_items) + nth;
-  const int tokens = u->tokens, first_pos = u->pos, unit_row = u->row, part = u->part;
-  if (tokens <= 0) return;
-  const KeyRows keys = key_rows(a, u->request);
+  const int tokens = u.tokens, first_pos = u.pos, unit_row = u.row, part = u.part;
+  const KeyRows keys = key_rows(a, u.request);
   const int last_pos = first_pos + tokens - 1;
-  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;  // (the first stage's barrier is after)
-
   // columns: tokens; positions are counted from the rows' first
   const bool mine = 32 * wave + c < tokens;
   const int token = min(32 * wave + c, tokens - 1);
@@ -287,8 +280,8 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   const int block_from = a.window > 0 ? max(0, block_first + 1 - a.window) : 0;
   const int seen_lo = block_from / kLatentTile;
   const int seen_hi = max(seen_lo, (min(last_pos - keys.start + 1, keys.count) + kLatentTile - 1) / kLatentTile);
-  const int tile_lo = seen_lo + static_cast<int>(static_cast<int64_t>(seen_hi - seen_lo) * u->piece / u->pieces);
-  const int tile_hi = seen_lo + static_cast<int>(static_cast<int64_t>(seen_hi - seen_lo) * (u->piece + 1) / u->pieces);
+  const int tile_lo = seen_lo + static_cast<int>(static_cast<int64_t>(seen_hi - seen_lo) * u.piece / u.pieces);
+  const int tile_hi = seen_lo + static_cast<int>(static_cast<int64_t>(seen_hi - seen_lo) * (u.piece + 1) / u.pieces);
   const int n = tile_hi - tile_lo;
 
   // Offsets of this lane's rows in a tile, which stay; a tile past the rows' end has
@@ -362,7 +355,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   }
-  float m = -INFINITY, l = 0.0f, poison = 0.0f;
+  float m = -INFINITY, l = 0.0f, poison = 0.0f, lowest = 0.0f;
   const float mul = a.scale * kLog2e;
   // Exponents' arguments of the tile whose scores were made last: score * scale_by +
   // shift.
@@ -439,25 +432,37 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   // the reference moved where one passes it.  `whole`: all columns see all rows.
   auto settle = [&](f32x16& s, float top, float low, int key0, bool whole, uint32_t bad) {
     scale_by = mul;
+    if (!CAREFUL) lowest = fminf(lowest, low);
     // NaN and +inf make their column's sums so by themselves; a weight of 0 would hide
     // -inf.
-    if (whole && !__any(low < -3.4028235e38f)) {
+    if (whole && !(CAREFUL && __any(low < -3.4028235e38f))) {
       top *= mul;
     } else {
       const int pos = first_pos + token - keys.start;
-      const int seen_from = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-      const int seen_to = min(pos, keys.count - 1);
-      top = -INFINITY;
+      // of the lane's sixteen keys it sees from `from` to `to`
+      const int at = key0 + 16 * h;
+      const int from = a.window > 0 ? max(0, pos + 1 - a.window) - at : 0;
+      const int to = min(pos, keys.count - 1) - at;
       scale_by = 1.0f;
+      if constexpr (CAREFUL) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = key0 + 16 * h + e;
-        const bool see = key <= seen_to && key >= seen_from;
-        const bool fine = fabsf(s[e]) <= 3.4028235e38f;
-        poison += see && (!fine || (bad >> (16 * h + e) & 1u)) ? NAN : 0.0f;
-        s[e] = see && fine ? s[e] * mul : -INFINITY;
-        top = fmaxf(top, s[e]);
+        for (int e = 0; e < 16; ++e) {
+          const bool see = e <= to && e >= from;
+          const bool fine = fabsf(s[e]) <= 3.4028235e38f;
+          poison += see && (!fine || (bad >> (16 * h + e) & 1u)) ? NAN : 0.0f;
+          s[e] = see && fine ? s[e] * mul : -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = e <= to ? s[e] * mul : -INFINITY;
+        if (__any(from > 0)) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = e >= from ? s[e] : -INFINITY;
+        }
       }
+      top = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
     }
     if (__any(top > m + S::kSlack)) {
       float m2 = fmaxf(m, top);
@@ -493,8 +498,9 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
       // Where some column does not see all rows, values that are no finite numbers
       // (which a weight of 0 would not keep out) are taken from LDS, and the rows
       // that had them noted.
-      const bool partly = key0 < all_from || key0 + kLatentTile - 1 > min(block_first, keys.count - 1);
-      if (threadIdx.x == 0) s_bad[i & 1] = 0;  // all have read it before this step
+      const bool partly =
+          CAREFUL && (key0 < all_from || key0 + kLatentTile - 1 > min(block_first, keys.count - 1));
+      if (CAREFUL && threadIdx.x == 0) s_bad[i & 1] = 0;  // all have read it before this step
       if (partly) {
         constexpr uint32_t kLo = S::kBf ? 0x7f80u : 0x7c00u, kHi = kLo << 16;
         char* values = ring + S::kValuesAt + v_slot;
@@ -559,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   };
   const int whole_lo = max(0, (all_from + kLatentTile - 1) / kLatentTile - tile_lo);
   const int whole_hi = (min(block_first, keys.count - 1) + 1) / kLatentTile - tile_lo;  // tiles [lo, hi)
-  const int inner_lo = whole_lo, inner_hi = busy && mul >= 0.0f ? min(whole_hi - 1, n - 4) : 0;
+  const int inner_lo = whole_lo, inner_hi = !CAREFUL && busy && mul >= 0.0f ? min(whole_hi - 1, n - 4) : 0;
   int i = -1;
   for (; i < min(inner_lo, n); ++i) step(i);
   if (i + 2 <= inner_hi) {
@@ -568,10 +574,21 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
       inner_step(i, scores, other);
       inner_step(i + 1, other, scores);
     }
-    // (the flags that steps clear for each other)
-    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
   }
   for (; i < n; ++i) step(i);
+  if constexpr (!CAREFUL) {
+    // (columns past the tokens have the last one's sums; a wavefront without columns
+    // has seen nothing)
+    float odd = l * 0.0f;
+#pragma unroll
+    for (int d = 0; d < S::kTilesD; ++d) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) odd = fmaf(o[d][e], 0.0f, odd);
+    }
+    if (__any(odd != 0.0f || lowest < -3.4028235e38f) && lane == 0) s_bad[0] = 1;
+    __syncthreads();
+    if (s_bad[0]) return false;
+  }
   l += __shfl_xor(l, 32);
   poison += __shfl_xor(poison, 32);
   l += poison;
@@ -591,9 +608,9 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
       to[kRowUnit * DV + 32 * wave + c] = m;
       to[kRowUnit * (DV + 1) + 32 * wave + c] = l;
     }
-    return;
+    return true;
   }
-  if (!mine) return;
+  if (!mine) return true;
   const float inv = 1.0f / l;
   const bool empty = m == -INFINITY && l == 0.0f;
   uint16_t* to = a.out + static_cast<int64_t>(unit_row + token) * a.out_token + head * a.out_head + 4 * h;
@@ -610,6 +627,27 @@ __global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
   if (a.lse && h == 0) {
     a.lse[static_cast<int64_t>(unit_row + token) * a.heads + head] = latent_lse<T>(m, l, S::kBias);
   }
+  return true;
+}
+
+template <class T, int DK, int DV>
+__global__ __launch_bounds__(256, 2) void rows_attend_kernel(RowsArgs a) {
+  typedef RowsShape<T, DK, DV> S;
+  static_assert(S::kKeyLoads * 4096 == S::kKeyTile && S::kValueLoads * 4096 == S::kValueTile,
+                "whole loads to a wavefront");
+  __shared__ __align__(1024) char ring[S::kLds];
+  __shared__ uint32_t s_bad[2];
+  const auto* plan = reinterpret_cast<ConstLatentHead>(reinterpret_cast<uintptr_t>(a.work));
+  // (heads go to the XCDs in turn with their blocks)
+  const int head = static_cast<int>(blockIdx.x % a.heads), nth = static_cast<int>(blockIdx.x / a.heads);
+  const auto* at = reinterpret_cast<ConstRowItem>(reinterpret_cast<uintptr_t>(a.work) + a.at_items) + nth;
+  const RowItem u{at->request, at->row, at->tokens, at->pos, at->piece, at->pieces, at->part, at->tiles};
+  if (nth >= plan->row_items || u.tokens <= 0) return;
+  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;  // (the first stage's barrier is after)
+  if (attend_piece<T, DK, DV, false>(a, head, u, ring, s_bad)) return;
+  __syncthreads();
+  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+  attend_piece<T, DK, DV, true>(a, head, u, ring, s_bad);
 }
 
 // Joins the parts of units in pieces: 1024 values to a step of a block, as they lie.
