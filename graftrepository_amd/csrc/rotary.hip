@@ -27,7 +27,7 @@ int rotary_of(const grm_rotary_desc* d, int channels, Rotary* out) {
   }
   *out = Rotary{};
   const double sign = d->inverse ? -1.0 : 1.0;
-  for (int i = 0; i < d->dim / 2; ++i) out->turns[i] = sign * d->turns[i];
+  for (int i = 0; i < d->dim / 2; ++i) out->quarters[i] = 4.0 * sign * d->turns[i];
   out->magnitude = d->inverse ? 1.0f / d->magnitude : d->magnitude;
   out->dim = d->dim;
   out->layout = d->layout;
