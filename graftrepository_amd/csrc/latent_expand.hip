@@ -24,7 +24,10 @@ struct ExpandArgs {
 
 // 128 rows x 256 columns to a block, 64 x 128 to a wavefront, 32 of the rank a
 // stage; three stages of direct loads in LDS, two blocks to a CU, so that one's
-// stores run beside the other's products.  Chunks of 16 bytes are stored at c ^ (row >> 3
+// stores run beside the other's products.  Bound by the rounds of so few steps (16 at
+// rank 512) and their ends: 4096 rows of 32 heads x 256 columns take 50 us (681
+// TFLOP/s), 4137 rows 57; torch's product of the same sizes without the gather, in
+// one plane, 44 and 74.  Chunks of 16 bytes are stored at c ^ (row >> 3
 // & 3) of their 64: the 16 rows that are read at once lie in all banks.  Results
 // leave through LDS, 16 bytes to a lane.
 constexpr int kExpandRows = 128, kExpandCols = 256, kExpandStep = 32, kExpandStages = 3;
@@ -224,8 +227,18 @@ __device__ inline KeyRows key_rows(const RowsArgs& a, int request) {
 //
 // In a wavefront, vector work stands beside matrix work: a tile's weights are made
 // between the instructions of the next tile's first product (each of which takes the
-// matrix cores eight times as long as its issue).  So a tile's keys are read one tile before its
-// values: three tiles of keys in LDS and four of values, two blocks to a CU.
+// matrix cores eight times as long as its issue).  So a tile's keys are read one tile
+// before its values: three tiles of keys in LDS and four of values, two blocks to a
+// CU.  The rest is one stream of tiles: those that all columns see are asked nothing.
+//
+// Bound by the matrix cores on long rows: a prompt of 16384 tokens, 32 heads of 192 and
+// 128, 1040 TFLOP/s in bf16 (a large matrix product here has 1221); 40 heads of 96
+// and 64 in fp16 820, where a tile's vector instructions take as long as its
+// products.  Short ones by a unit's ends, about ten tiles' time each, and the
+// slots that stay empty at the end: 4096 tokens 840, 1024 tokens 320.
+//
+// A unit of 128 tokens is cut where there are fewer than the blocks that fit: by the
+// plan, at the share of eight for which the longest-first order ends first.
 template <class T, int DK, int DV>
 struct RowsShape {
   static constexpr int kKeyBytes = (2 * DK + 127) / 128 * 128;  // of a row in LDS
@@ -240,9 +253,14 @@ struct RowsShape {
   static constexpr int kSteps = DK / 16, kTilesD = DV / 32;
   static constexpr bool kBf = T::code == kBF16;
   static constexpr float kSlack = kBf ? 8.0f : 2.0f, kBias = kBf ? 0.0f : 13.0f;
-  // Where a value row's chunks of 16 bytes go (chunk c to c ^ value_turn): a transposed
-  // read takes 64 bytes of each of four rows, which then lie in all 64 banks.  The
-  // same for every fourth row, so that these are a constant apart.
+  // Where a row's chunks of 16 bytes go: chunk c to c ^ turn.  A 16-byte read is served
+  // 16 lanes at a time (0-3, 12-15, 20-23, 24-27; 4-11, 16-19, 28-31; and so on), whose
+  // rows are then in all 64 banks.
+  static __device__ __forceinline__ int key_turn(int row) {
+    return (row >> 2 & 3) + (kKeyBytes % 256 == 0 ? 4 * (row & 3) : 4 * (row >> 1 & 1));
+  }
+  // A transposed read takes 64 bytes of each of four rows, which then lie in all
+  // banks.  The same for every fourth row, so that these are a constant apart.
   static __device__ __forceinline__ int value_turn(int row) {
     return kValueBytes % 256 == 0 ? 4 * (row & 3) : 4 * (row >> 1 & 1);
   }
@@ -254,14 +272,15 @@ __host__ __device__ constexpr size_t rows_part_floats(int value_dim) {
 }
 
 // A unit's piece.  Values that are no finite numbers (in a row that no column sees, with
-// a weight of 0; a score of -inf, which would hide its row) take questions at every tile.
-// Without CAREFUL there are none: at its end such a thing shows in the sums or in the
-// least score, nothing is written then, and the answer is false.
+// a weight of 0; a score of -inf, which would hide its row) take questions at every tile
+// that is seen in part.  Without CAREFUL there are none: at its end such a thing shows
+// in the sums or in the least score, nothing is written then, and the answer is
+// false.  (With the questions three prompts took 117 us in place of 112, a chunk of 1021
+// tokens 119 in place of 110.)
 template <class T, int DK, int DV, bool CAREFUL>
 __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const RowItem& u, char* ring,
                                              uint32_t* s_bad) {
   typedef RowsShape<T, DK, DV> S;
-  typedef LatentShape<T, 256, 32, 32, 1, 4> L;  // chunks' places and weights' rounding
   const int lane = __lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane % 32, h = lane / 32;
   const int tokens = u.tokens, first_pos = u.pos, unit_row = u.row, part = u.part;
@@ -292,7 +311,7 @@ __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const 
     constexpr int kKeyChunks = S::kKeyBytes / 16, kValueChunks = S::kValueBytes / 16;
     const int at = (key ? wave * S::kKeyLoads + j : wave * S::kValueLoads + j - S::kKeyLoads) * kWave + lane;
     const int r = at / (key ? kKeyChunks : kValueChunks), place = at - r * (key ? kKeyChunks : kValueChunks);
-    const int chunk = place ^ (key ? L::template turn<S::kKeyBytes>(r) : S::value_turn(r));
+    const int chunk = place ^ (key ? S::key_turn(r) : S::value_turn(r));
     // (a row's last places in LDS may be nobody's)
     const int64_t row = static_cast<int64_t>(min(r, last)) * (key ? a.k_row : a.v_row);
     return static_cast<uint32_t>(2 * (row + 8 * (!key || chunk < DK / 8 ? chunk : 0)));
@@ -345,7 +364,7 @@ __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const 
   for (int s = 0; s < S::kSteps; ++s) asm volatile("" : "+v"(q[s]));
   asm volatile("" ::: "memory");
   const int key_row = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
-  const int k_at = key_row * S::kKeyBytes + 16 * (h ^ L::template turn<S::kKeyBytes>(key_row));
+  const int k_at = key_row * S::kKeyBytes + 16 * (h ^ S::key_turn(key_row));
   const int i16 = lane % 16, v_row = 16 * h + i16 / 4;
   const int v_at = S::kValuesAt + v_row * S::kValueBytes + 8 * (i16 & 1) +
                    16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ S::value_turn(v_row));
@@ -406,7 +425,7 @@ __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const 
                 const float y = __builtin_amdgcn_exp2f(fmaf(now[e + 1], scale_by, shift));
                 l += x;
                 l += y;
-                w[e / 8][e % 8 / 2] = L::weights(x, y);
+                w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y);
               }
             } else {
               const int d = k - kEarly;

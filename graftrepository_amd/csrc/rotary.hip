@@ -3,7 +3,8 @@
 // A block takes some tokens and heads.  It makes the angles of its tokens once,
 // in LDS, for all of its heads; then a thread turns eight pairs (two 16-byte
 // loads and stores) or copies eight channels that are not turned.  Bound by
-// bytes; few rows are one chain: position, angle, values.
+// bytes; few rows are one chain: position, angle, values.  8011 rows of 40 heads x 96
+// in fp16 take 27 us (123 MB, 4.5 TB/s), 32 rows of 32 heads x 128 3.7.
 #include "rotary.hpp"
 
 namespace grm {
