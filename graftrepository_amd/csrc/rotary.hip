@@ -163,6 +163,7 @@ extern "C" int grm_hip_rotate(const grm_rotary_desc* rotary, const void* x, int 
       start > head_dim) {
     return grm::fail(-1, "bad heads, head_dim or start");
   }
+  if (static_cast<int64_t>(heads) * head_dim > 0x7fffffff) return grm::fail(-1, "a row is too long");
   if (tokens > static_cast<uint64_t>(kMaxLen)) return grm::fail(-1, "too many tokens");
   Rotary r;
   GRM_CHECK_RC(rotary_of(rotary, head_dim - start, &r));
@@ -171,6 +172,9 @@ extern "C" int grm_hip_rotate(const grm_rotary_desc* rotary, const void* x, int 
     return 0;
   }
   if (!x || !out || !positions) return grm::fail(-1, "null array");
+  if ((out_token_stride == 0 && tokens > 1) || (out_head_stride == 0 && heads > 1)) {
+    return grm::fail(-1, "rows or heads of the output are one another's memory");
+  }
   RotateArgs a{};
   a.x = x;
   a.out = out;

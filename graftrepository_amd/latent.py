@@ -182,7 +182,7 @@ class LatentCache:
         out, to, result = _output(q, out, (d.tokens, d.heads, self.rank), self.dtype, self.device,
                                   stream)
         lse, lp = _statistics(q, lse, return_lse, (d.tokens, d.heads), self.device, stream)
-        key = ("latent", self.rank)
+        key = ("latent", self.rank, self.rope)
         need = batch._scratch.get(key)
         if need is None:
             got = u64()

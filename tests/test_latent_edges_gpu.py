@@ -218,3 +218,104 @@ def test_values_that_require_gradients_are_refused(hip_lib):
             attend_rows(s.batch(), x["q"], x["k"], x["v"], ints(s.cu))
     with pytest.raises(ValueError, match="bf16 or f16"):
         attend_rows(s.batch(), s.q.float(), s.k.float(), s.v.float(), ints(s.cu))
+
+
+def test_one_batch_serves_rows_of_unlike_key_parts(hip_lib):
+    # of one rank, but with and without the matrix cores' kernel and its scratch
+    a = Setup([600, 3], [2, 1], 512, 64, 16, 16)
+    b = Setup([600, 3], [2, 1], 512, 0, 16, 16)
+    b.table = a.table
+    batch = a.batch()
+    rows = b.rows.nan_to_num(0.5)[:a.rows.shape[0]].contiguous()
+    plain = LatentCache(rows, 512).attend(batch, b.q, b.scale)
+    out = LatentCache(a.rows, 512).attend(batch, a.q, a.scale)
+    a.check(out, None, heads_of=[3])
+    assert torch.equal(LatentCache(rows, 512).attend(batch, b.q, b.scale), plain)
+
+
+def test_more_requests_than_the_plan_holds_in_lds(hip_lib):
+    n, heads = 5000, 4
+    rng = np.random.default_rng(9)
+    ctx = rng.integers(0, 15, n)
+    table = dev(rng.permutation(n).astype(np.int32)[:, None])
+    rows = dev(rng.standard_normal((n, 16, 288)), torch.bfloat16)
+    q = dev(rng.standard_normal((n, heads, 288)), torch.bfloat16)
+    k = dev(rng.standard_normal((n, heads, 96)), torch.bfloat16)
+    v = dev(rng.standard_normal((n, heads, 64)), torch.bfloat16)
+    cache = LatentCache(rows, 256)
+
+    def run(a, b):
+        batch = KvBatch(ints(ctx[a:b]), ints([1] * (b - a)), table[a:b], 16, tokens=b - a, max_new=1,
+                        heads=heads, kv_heads=1, latent=True).plan()
+        cu = ints(np.arange(b - a + 1))
+        return (cache.attend(batch, q[a:b], 0.1),
+                attend_rows(batch, k[a:b], k[a:b], v[a:b], cu, starts=ints(ctx[a:b])))
+
+    # a tile to a request: nothing is cut, and every request's result its own
+    whole, halves = run(0, n), [run(0, 2500), run(2500, n)]
+    for i in range(2):
+        assert torch.equal(whole[i], torch.cat([h[i] for h in halves]))
+    assert torch.equal(whole[1], v)           # of one row that a token sees
+
+
+def test_rows_past_4_gib_of_a_cache(hip_lib):
+    blocks, bs, rank, rope, heads = 59000, 64, 512, 64, 16
+    big = torch.empty((blocks, bs, rank + rope), device="cuda", dtype=torch.bfloat16)
+    small = torch.zeros((4, bs, rank + rope), device="cuda", dtype=torch.bfloat16)
+    assert big.numel() * 2 > 1 << 32
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    x = torch.randn(200, rank + rope, generator=gen, device="cuda")
+    q = torch.randn(1, heads, rank + rope, generator=gen, device="cuda").bfloat16()
+    w = (torch.randn(heads, 256, rank, generator=gen, device="cuda") / rank ** 0.5).bfloat16()
+    rotary, got = Rotary(rope), []
+    for rows, ids in ((big, [blocks - 1, 3, blocks - 2, blocks - 3]), (small, [0, 1, 2, 3])):
+        table = ints([ids])
+        cache = LatentCache(rows, rank)
+        b = KvBatch(ints([0]), ints([200]), table, bs, tokens=200, max_new=200, heads=heads, kv_heads=1,
+                    latent=True).plan()
+        cache.append(b, x[:, :rank], x[:, rank:], rotary=rotary)
+        one = KvBatch(ints([199]), ints([1]), table, bs, tokens=1, max_new=1, heads=heads, kv_heads=1,
+                      latent=True).plan()
+        cu = ints([0, 200])
+        got.append([cache.attend(one, q, 0.05), cache.read(table, ints([0]), cu, 200),
+                    *cache.expand(w, 128, table, ints([0]), cu, 200)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+def test_dense_rows_past_4_gib(hip_lib):
+    s = Rows([100], [40], 192, 128, 2, "bf16")
+    want, lse = s.run()
+    n, stride = 140, 1 << 24                 # 32 MiB from row to row
+    base = torch.empty(n * stride, device="cuda", dtype=torch.bfloat16)
+    for name, d in (("k", 192), ("v", 128)):
+        far = base.as_strided((n, 2, d), (stride, d, 1), 0 if name == "k" else 1024)
+        far.copy_(getattr(s, name))
+        setattr(s, name, far)
+    out, lse2 = s.run()
+    assert torch.equal(out, want) and torch.equal(lse, lse2)
+
+
+def test_two_streams_over_rows_with_a_batch_each(hip_lib):
+    s = Rows([3000, 40], [60, 200], 96, 64, 4, "f16")
+    want, _ = s.run()
+    torch.cuda.synchronize()
+    got = []
+    for st in [torch.cuda.Stream() for _ in range(2)]:
+        with torch.cuda.stream(st):
+            b = s.batch()
+            got += [attend_rows(b, s.q, s.k, s.v, ints(s.cu), starts=ints(s.starts)) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_heads_that_share_rows(hip_lib):
+    # strides of 0: every head has the same keys and values
+    s = Rows([50, 0], [30, 80], 128, 128, 3, "bf16")
+    k, v = s.k[:, :1].clone(), s.v[:, :1].clone()
+    s.k, s.v = k.expand(-1, 3, -1).contiguous(), v.expand(-1, 3, -1).contiguous()
+    want, _ = s.run()
+    s.k, s.v = k.expand(-1, 3, -1), v.expand(-1, 3, -1)
+    got, _ = s.run()
+    assert torch.equal(got, want)

@@ -265,3 +265,15 @@ def test_python_checks_of_the_expanded_form():
                         (fake((4, 64, 64), np.float16), 0)):
         with pytest.raises(ValueError):
             c.expand(weight, key, *at)
+
+
+def test_rows_that_are_one_another_are_not_turned_in_place():
+    lib = g.load()
+    d = ctypes.byref(rotary_desc())
+    for strides in ((0, 64), (128, 0)):     # a row given to all tokens, a head to all heads
+        assert lib.grm_hip_rotate(d, 0x1000, 0, *strides, 0x1000, *strides, 0x1000, 4, 2, 64, 0,
+                                  None) == -1
+        assert b"memory" in lib.grm_hip_last_error()
+    # a row of more values than an index holds
+    assert lib.grm_hip_rotate(d, 0x1000, 0, 64, 64, 0x2000, 64, 64, 0x1000, 4, 65535, 65536, 0,
+                              None) == -1
