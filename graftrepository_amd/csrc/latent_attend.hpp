@@ -14,8 +14,10 @@
 // memory once for all heads.  With few columns wavefronts take several tiles at
 // once, G of them, and are joined through LDS at the unit's end: 16 columns, four
 // wavefronts and G = 4; 32, four and 2; 64, eight and 2 (at rank 256 four and 1, two
-// blocks to a CU); 128, eight and 1.  (With 32 columns to a wavefront and rows turned
-// over 128 bytes a step of 32 sessions with 40 heads took 33 us, with these 23.)
+// blocks to a CU); 128, eight and 1.  (32 columns to a wavefront, four wavefronts, read
+// half as much from LDS but leave one wavefront to a SIMD: 24 sessions of 128 heads 59
+// us in place of 55, a chunk 116 in place of 102, long ones the same.  Weights made
+// beside the next tile's scores cost registers and gained nothing here.)
 //
 // Rows go to LDS by direct loads (no registers), a ring of four or eight tiles, and
 // are read from there twice: as the first product's operand 16 bytes to a lane, and

@@ -364,10 +364,13 @@ __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const 
   for (int s = 0; s < S::kSteps; ++s) asm volatile("" : "+v"(q[s]));
   asm volatile("" ::: "memory");
   const int key_row = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);
-  const int k_at = key_row * S::kKeyBytes + 16 * (h ^ S::key_turn(key_row));
+  int k_at = key_row * S::kKeyBytes + 16 * (h ^ S::key_turn(key_row));
   const int i16 = lane % 16, v_row = 16 * h + i16 / 4;
-  const int v_at = S::kValuesAt + v_row * S::kValueBytes + 8 * (i16 & 1) +
+  int v_at = S::kValuesAt + v_row * S::kValueBytes + 8 * (i16 & 1) +
                    16 * ((2 * (lane >> 4 & 1) + (i16 % 4 >> 1)) ^ S::value_turn(v_row));
+  // (a register each; parts of them, spilled, were read back before every loop, and
+  // waited for every direct load)
+  asm volatile("" : "+v"(k_at), "+v"(v_at));
   f32x16 o[S::kTilesD];
 #pragma unroll
   for (int d = 0; d < S::kTilesD; ++d) {
