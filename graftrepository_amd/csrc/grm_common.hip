@@ -64,6 +64,9 @@ int reserve_mapped(MappedCands* m, size_t count) {
     (void)hipHostFree(h);
     return fail_hip(rc, "hipHostGetDevicePointer");
   }
+  // Pinned memory that another bank freed comes back as it was, and numbers of routes
+  // begin anew in each: an entry of that bank's route could carry this one's tag.
+  memset(h, 0, count * sizeof(Cand));
   m->host = static_cast<Cand*>(h);
   m->dev = static_cast<Cand*>(d);
   m->count = count;
@@ -93,8 +96,8 @@ int wait_event(hipEvent_t ev) {
 int begin_flags(MappedBuf* buf, size_t max, unsigned* seq) {
   if (buf->bytes < max * sizeof(unsigned)) {
     GRM_CHECK_RC(reserve_mapped_bytes(buf, max * sizeof(unsigned)));
+    // (the number goes on: the lists may hold entries with a lower one's tag)
     memset(buf->host, 0, max * sizeof(unsigned));
-    *seq = 0;
   }
   if (++*seq == 0) *seq = 1;  // 0 is what a fresh buffer holds
   return 0;

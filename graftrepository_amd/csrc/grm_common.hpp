@@ -381,7 +381,8 @@ bool event_timing();
 
 // Pinned host buffer the device writes directly (mapped, coherent): the
 // route kernels leave their per-block results there so the final merge
-// needs neither a merge launch nor a device-to-host copy call.
+// needs neither a merge launch nor a device-to-host copy call.  Cleared when
+// new, so that no entry carries a route's tag.
 struct MappedCands {
   Cand* host = nullptr;
   Cand* dev = nullptr;
