@@ -167,6 +167,41 @@ __device__ inline void plan_cache(const LatentPlanArgs& a, int k, int* at, int64
   deal.used = static_cast<int>(min(most, static_cast<int64_t>(a.runs[k])));
   deal.each = deal.used ? tiles / deal.used : 0;
   deal.rem = deal.used ? static_cast<int>(tiles - deal.each * deal.used) : 0;
+  // Few units: each gets runs of its own, where the longest of those is at most
+  // kLatentChange tiles longer than an even run (which changes from unit to unit
+  // somewhere, with queries to fetch and one part more).  The length is the least of 16
+  // candidates with which all fit: the last one does, since tiles / length + units of them
+  // do.
+  __shared__ int s_runs[kPlanWaves], s_piece[kPlanThreads];
+  const int own = a.runs[k] - n_units;
+  bool whole_runs = false;
+  if (n_units > 0 && n_units <= kPlanThreads && own > 0) {
+    const int wave = tid / kWave, lane = tid % kWave;
+    const int64_t least = max(static_cast<int64_t>(kLatentLeast), (tiles + a.runs[k] - 1) / a.runs[k]);
+    const int64_t most_len = max(least, (tiles + own - 1) / own);
+    auto length = [&](int c) { return least + (most_len - least) * c / (kPlanWaves - 1); };
+    int64_t count = 0;
+    for (int i = lane; i < n_units; i += kWave) {
+      count += (firsts[i + 1] - firsts[i] + length(wave) - 1) / length(wave);
+    }
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) count += __shfl_xor(count, d);
+    if (lane == 0) s_runs[wave] = static_cast<int>(min(count, static_cast<int64_t>(0x7fffffff)));
+    __syncthreads();
+    int c = 0;
+    while (c < kPlanWaves - 1 && s_runs[c] > a.runs[k]) ++c;
+    const int64_t even = deal.each + (deal.rem > 0);
+    whole_runs = length(c) <= even + kLatentChange;
+    if (whole_runs) {
+      const int64_t mine = tid < n_units ? firsts[tid + 1] - firsts[tid] : 0;
+      int64_t sum;
+      const int64_t v = block_sum<int64_t>((mine + length(c) - 1) / length(c), &sum, scratch);
+      s_piece[tid] = static_cast<int>(v);
+      deal.used = static_cast<int>(sum);
+      __syncthreads();
+    }
+  }
+  auto pieces_of = [&](int u) { return (u + 1 < n_units ? s_piece[u + 1] : deal.used) - s_piece[u]; };
   auto* to = reinterpret_cast<LatentStart*>(a.work + a.at_starts[k]);
   for (int i = tid; i < a.starts[k]; i += kPlanThreads) {
     // neighbouring runs to one XCD, to which every eighth entry goes
@@ -175,11 +210,20 @@ __device__ inline void plan_cache(const LatentPlanArgs& a, int k, int* at, int64
     s.run = -1;
     if (nth < deal.used / 8 + (xcd < deal.used % 8)) {
       s.run = xcd * (deal.used / 8) + min(xcd, deal.used % 8) + nth;
-      s.begin = deal.begin(s.run);
-      s.end = deal.begin(s.run + 1);
-      s.unit = last_of(firsts, n_units, s.begin);
-      s.first = firsts[s.unit];
-      s.last = firsts[s.unit + 1];
+      if (whole_runs) {
+        s.unit = last_of(s_piece, n_units, s.run);
+        s.first = firsts[s.unit];
+        s.last = firsts[s.unit + 1];
+        const int pieces = pieces_of(s.unit), piece = s.run - s_piece[s.unit];
+        s.begin = s.first + (s.last - s.first) * piece / pieces;
+        s.end = s.first + (s.last - s.first) * (piece + 1) / pieces;
+      } else {
+        s.begin = deal.begin(s.run);
+        s.end = deal.begin(s.run + 1);
+        s.unit = last_of(firsts, n_units, s.begin);
+        s.first = firsts[s.unit];
+        s.last = firsts[s.unit + 1];
+      }
       const LatentUnit u = units[s.unit];
       s.request = u.request;
       s.row = u.row;
@@ -189,14 +233,20 @@ __device__ inline void plan_cache(const LatentPlanArgs& a, int k, int* at, int64
     }
     to[i] = s;
   }
-  // Ends of runs that are the first in a unit.
+  // Units that are cut: those of more than one run, or ends of runs that are the first
+  // in a unit.
   auto* joins = reinterpret_cast<LatentJoin*>(a.work + a.at_joins[k]);
   int done = 0;
-  for (int base = 0; base < deal.used - 1; base += kPlanThreads) {
+  const int ends = whole_runs ? n_units : deal.used - 1;
+  for (int base = 0; base < ends; base += kPlanThreads) {
     const int e = base + tid;
     LatentJoin j{};
     bool cuts = false;
-    if (e < deal.used - 1) {
+    if (e < ends && whole_runs) {
+      const int pieces = pieces_of(e);
+      cuts = pieces > 1 && units[e].tokens > 0;
+      j = LatentJoin{s_piece[e], s_piece[e] + pieces - 1, units[e].row, units[e].tokens};
+    } else if (e < ends) {
       const int64_t end = deal.begin(e + 1);
       const int u = last_of(firsts, n_units, end);
       if (firsts[u] < end && firsts[u] >= deal.begin(e)) {

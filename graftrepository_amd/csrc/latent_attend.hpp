@@ -58,6 +58,7 @@ constexpr int kLatentTile = 32;     // rows to a tile
 constexpr int kLatentCols = 128;    // columns to a unit, at most
 constexpr int kWaveCols = 16;      // columns to a wavefront
 constexpr int kLatentLeast = 4;     // tiles to a run, at least
+constexpr int kLatentChange = 2;    // tiles' time that a change of unit within a run takes
 constexpr int kRowUnit = 128;       // tokens to a unit of attention over dense rows
 constexpr int kRowLeast = 16;       // tiles to a piece of such a unit, at least
 
