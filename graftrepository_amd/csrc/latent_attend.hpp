@@ -6,9 +6,9 @@
 //
 // A unit is the columns (token, head) of some neighbouring tokens of a request,
 // at most 128; all of a step's (unit, tile of 32 rows) pairs are dealt to blocks
-// in equal runs (`latent_plan_kernel`).  A unit that a run's end cuts leaves parts
-// in scratch, which a second launch joins in order: results do not depend on
-// timing.
+// in runs (`latent_plan_kernel`): of one unit each where units are few, else equal
+// ones.  A unit that a run's end cuts leaves parts in scratch, which a second launch
+// joins in order: results do not depend on timing.
 //
 // A wavefront holds 16 columns' queries and sums in registers: a row is read from
 // memory once for all heads.  With few columns wavefronts take several tiles at
@@ -43,9 +43,9 @@
 // rank 256): 32 sessions of 65535 tokens, 16 heads 5.9 TB/s, 40 heads at rank 256
 // 5.2; 256 sessions of 4095, 128 heads 828 TFLOP/s; a chunk of 256 tokens of 16 heads
 // on 32767 916.  Short steps are start, change of session and parts: 24 sessions of
-// 98 thousand rows in all and 128 heads take 55 us, and 20 for the join of 67 MB of
-// parts, which is near a copy's rate.  (64 columns to a block, half the parts and
-// twice the loads, took as long.)
+// 98 thousand rows in all and 128 heads take 47 us (55 in equal runs, 24 of which have
+// two units), and 19.5 for the join of 67 MB of parts, which is near a copy's rate.
+// (64 columns to a block, half the parts and twice the loads, took as long.)
 #pragma once
 
 #include "kv_attend.hpp"
@@ -56,9 +56,12 @@ namespace kv {
 
 constexpr int kLatentTile = 32;     // rows to a tile
 constexpr int kLatentCols = 128;    // columns to a unit, at most
-constexpr int kWaveCols = 16;      // columns to a wavefront
+constexpr int kWaveCols = 16;       // columns to a wavefront
 constexpr int kLatentLeast = 4;     // tiles to a run, at least
-constexpr int kLatentChange = 2;    // tiles' time that a change of unit within a run takes
+// Tiles that runs of a unit's own may be longer than even ones (with 2 a chunk beside
+// decoding sessions took 104 us in place of 97, with 4 24 sessions of 16383 tokens and
+// 128 heads 182 in place of 174).
+constexpr int kLatentChange = 3;
 constexpr int kRowUnit = 128;       // tokens to a unit of attention over dense rows
 constexpr int kRowLeast = 16;       // tiles to a piece of such a unit, at least
 
