@@ -319,3 +319,15 @@ def test_heads_that_share_rows(hip_lib):
     s.k, s.v = k.expand(-1, 3, -1), v.expand(-1, 3, -1)
     got, _ = s.run()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n", [130, 250, 300, 1100])
+@pytest.mark.parametrize("rank,rope,heads", [(512, 64, 128), (256, 32, 40)])
+def test_fewer_and_more_sessions_than_runs(hip_lib, n, rank, rope, heads):
+    # runs of a session's own, runs that go on from one to the next, and lists longer than
+    # a block plans at once
+    rng = np.random.default_rng(n)
+    ctx = rng.integers(0, 300 if n < 1000 else 90, n).tolist()
+    s = Setup(ctx, [1] * n, rank, rope, 32, heads, "f16")
+    out, lse = LatentCache(s.rows, rank).attend(s.batch(), s.q, s.scale, return_lse=True)
+    s.check(out, lse, heads_of=[heads - 1])
