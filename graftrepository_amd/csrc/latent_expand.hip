@@ -454,9 +454,9 @@ __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const 
   // the reference moved where one passes it.  `whole`: all columns see all rows.
   auto settle = [&](f32x16& s, float top, float low, int key0, bool whole, uint32_t bad) {
     scale_by = mul;
-    if (!CAREFUL) lowest = fminf(lowest, low);
     // NaN and +inf make their column's sums so by themselves; a weight of 0 would hide
-    // -inf.
+    // -inf (with a negative scale +inf).
+    if (!CAREFUL) lowest = fminf(lowest, mul < 0.0f ? -top : low);
     if (whole && !(CAREFUL && __any(low < -3.4028235e38f))) {
       top *= mul;
     } else {
