@@ -223,12 +223,23 @@ __device__ __forceinline__ void in_order(Read read, Use use) {
   }
 }
 
-// Two weights, rounded.
+// Sums of bf16 values are kept at 2^-kDown of themselves: weights up to 2^8 of up to
+// 2^30 rows would take those of large values out of fp32's range, though their mean is
+// in it.
+constexpr int kDown = 40;
+template <class T>
+__host__ __device__ constexpr float latent_up() { return T::code == kBF16 ? 0x1p40f : 1.0f; }
+static_assert(kDown == 40, "the power in latent_up");
+
+// Two weights, rounded; bf16 ones then taken down by their exponents (those below
+// 2^-86 of the largest lose digits or go, which no sum of fp32 would show).
 template <bool BF>
 __device__ __forceinline__ uint32_t two_weights(float x, float y) {
   if constexpr (BF) {
     typedef __bf16 pair __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, pair{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+    typedef unsigned short bits __attribute__((ext_vector_type(2)));
+    const auto w = __builtin_bit_cast(bits, pair{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(w, bits{kDown << 7, kDown << 7}));
   } else {
     return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
   }
@@ -281,8 +292,8 @@ __device__ inline void latent_put(uint16_t* to, f32x4 o, float inv, bool empty) 
   u32x2 v;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv);
-    const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv);
+    const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv * latent_up<T>());
+    const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv * latent_up<T>());
     v[e] = lo | (hi << 16);
   }
   *reinterpret_cast<u32x2*>(to) = v;

@@ -776,7 +776,7 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowsArgs a) {
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
     l = l * keep + sum;
-    s_p[wave][lane] = p;
+    s_p[wave][lane] = p / latent_up<T>();
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] *= keep;
@@ -811,7 +811,7 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowsArgs a) {
   uint16_t* out = a.out + static_cast<int64_t>(row) * a.out_token + head * a.out_head;
   for (int d = threadIdx.x; d < a.value_dim; d += 256) {
     const float x = f[0] * s_o[0][d] + f[1] * s_o[1][d] + f[2] * s_o[2][d] + f[3] * s_o[3][d];
-    out[d] = T::put(total == 0.0f ? 0.0f : x / total);
+    out[d] = T::put(total == 0.0f ? 0.0f : x / total * latent_up<T>());
   }
   if (a.lse && threadIdx.x == 0) {
     a.lse[static_cast<int64_t>(row) * a.heads + head] =
