@@ -115,6 +115,12 @@ int check_batch(const grm_kv_batch_desc* b, bool with_arrays);
 int check_cache(const grm_kv_cache_desc* c);
 int check_pair(const grm_kv_cache_desc* c, const grm_kv_batch_desc* b, bool with_arrays);
 
+// A launch's first dimension holds fewer than 2^32 threads: so many blocks of 256.
+constexpr uint64_t kMaxBlocks = 0xffffffffull / 256;
+inline int check_blocks(uint64_t blocks) {
+  return blocks > kMaxBlocks ? fail(-1, "too many rows for one call") : 0;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------- storage types

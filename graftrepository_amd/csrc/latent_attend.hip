@@ -658,6 +658,7 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
     return grm::fail(-1, "queries and output: 16-byte aligned rows");
   }
   const bool cores = latent_cores(c, b);
+  if (!cores) GRM_CHECK_RC(check_blocks(static_cast<uint64_t>(b->tokens)));
   if (cores && (!work || !aligned16(work))) {
     return grm::fail(-1, "latent work must be 16-byte aligned");
   }

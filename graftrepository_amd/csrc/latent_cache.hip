@@ -195,6 +195,8 @@ extern "C" int grm_hip_latent_append(const grm_latent_desc* c, const grm_kv_batc
   a.rank = c->rank;
   a.rope = c->rope;
   a.turned = r.dim / 16;
+  const int64_t items = static_cast<int64_t>(a.tokens) * ((a.rank + a.rope) / 16);
+  GRM_CHECK_RC(check_blocks((items + kRowThreads - 1) / kRowThreads));
   const int64_t unit = dtype == grm::kF32 ? 4 : 8;
   const bool aligned = aligned16(latents) && aligned16(keys) &&
                        (latent_token_stride | (c->rope ? key_token_stride : 0)) % unit == 0;
@@ -219,6 +221,7 @@ extern "C" int grm_hip_latent_read(const grm_latent_desc* c, const int32_t* bloc
     return 0;
   }
   if (!out || !aligned16(out)) return grm::fail(-1, "output must be 16-byte aligned");
+  GRM_CHECK_RC(check_blocks((rows + kReadRowsEach - 1) / kReadRowsEach));
   LatentReadArgs a{};
   a.rows = static_cast<const uint16_t*>(c->rows);
   a.out = out;

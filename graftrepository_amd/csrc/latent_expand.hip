@@ -888,7 +888,7 @@ extern "C" int grm_hip_latent_expand(const grm_latent_desc* c, const void* weigh
   const bool bf = c->dtype == grm::kBF16;
   const uint64_t columns = static_cast<uint64_t>(heads) * (key_dim + value_dim);
   const uint64_t blocks = (rows + kExpandRows - 1) / kExpandRows * ((columns + kExpandCols - 1) / kExpandCols);
-  if (blocks >= 1ull << 31) return grm::fail(-1, "too many rows for so many heads");
+  GRM_CHECK_RC(check_blocks(c->rank % kExpandStep == 0 ? blocks : rows));
   if (c->rank % kExpandStep == 0) {
     const auto grid = static_cast<unsigned>(blocks);
     if (bf) latent_expand_kernel<BF16><<<grid, 256, 0, s>>>(a);
@@ -945,6 +945,10 @@ extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work,
     return grm::fail(-1, "queries, rows and output: 16-byte aligned rows");
   }
   if (!work || !aligned16(work)) return grm::fail(-1, "latent work must be 16-byte aligned");
+  // the matrix cores' kernel takes a tile's rows by 32-bit offsets
+  const auto near = [](int64_t stride) { return stride >= 0 && stride < (1ll << 25); };
+  const bool shape = rows_cores(key_dim, value_dim) && near(k_row_stride) && near(v_row_stride);
+  if (!shape) GRM_CHECK_RC(check_blocks(static_cast<uint64_t>(b->tokens)));
   LatentLayout l;
   GRM_CHECK_RC(latent_layout_of(b, &l));
   if (work_bytes < l.bytes) return grm::fail(-1, "work is smaller than grm_hip_latent_work_bytes");
@@ -978,10 +982,8 @@ extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work,
   a.key_dim = key_dim;
   a.value_dim = value_dim;
   a.rows = static_cast<int32_t>(rows);
-  // the matrix cores' kernel takes a tile's rows by 32-bit offsets
-  const auto near = [](int64_t stride) { return stride >= 0 && stride < (1ll << 25); };
-  const bool cores = rows_cores(key_dim, value_dim) && near(k_row_stride) && near(v_row_stride) &&
-                     l.cap_items * static_cast<uint64_t>(b->heads) < (1ull << 31);
+  const bool cores = shape && l.cap_items * static_cast<uint64_t>(b->heads) <= kMaxBlocks;
+  if (!cores) GRM_CHECK_RC(check_blocks(static_cast<uint64_t>(b->tokens)));
   if (cores && l.cap_row_joins) {
     const uint64_t need = l.cap_parts * b->heads * rows_part_floats(value_dim) * 4;
     if (!scratch || !aligned16(scratch) || scratch_bytes < need) {

@@ -121,6 +121,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_any_kernel(RotateArgs a
   }
 }
 
+// As many tokens as a grid has room for.
 template <class T>
 static void launch_rotate(RotateArgs a, const Rotary& r, bool in_place, hipStream_t stream) {
   const int rest = in_place ? 0 : a.head_dim - r.dim;
@@ -176,14 +177,10 @@ extern "C" int grm_hip_rotate(const grm_rotary_desc* rotary, const void* x, int 
     return grm::fail(-1, "rows or heads of the output are one another's memory");
   }
   RotateArgs a{};
-  a.x = x;
-  a.out = out;
-  a.positions = positions;
   a.x_token = x_token_stride;
   a.x_head = x_head_stride;
   a.out_token = out_token_stride;
   a.out_head = out_head_stride;
-  a.tokens = tokens;
   a.heads = heads;
   a.head_dim = head_dim;
   a.start = start;
@@ -192,9 +189,17 @@ extern "C" int grm_hip_rotate(const grm_rotary_desc* rotary, const void* x, int 
     return grm::fail(-1, "in place, but with other strides");
   }
   const auto s = static_cast<hipStream_t>(stream);
-  if (dtype == grm::kF32) launch_rotate<F32>(a, r, in_place, s);
-  else if (dtype == grm::kBF16) launch_rotate<BF16>(a, r, in_place, s);
-  else launch_rotate<F16>(a, r, in_place, s);
+  const int64_t size = dtype == grm::kF32 ? 4 : 2;
+  for (uint64_t from = 0; from < tokens; from += kMaxBlocks) {
+    const auto row = static_cast<int64_t>(from);
+    a.x = static_cast<const char*>(x) + row * x_token_stride * size;
+    a.out = static_cast<char*>(out) + row * out_token_stride * size;
+    a.positions = positions + row;
+    a.tokens = std::min(tokens - from, kMaxBlocks);
+    if (dtype == grm::kF32) launch_rotate<F32>(a, r, in_place, s);
+    else if (dtype == grm::kBF16) launch_rotate<BF16>(a, r, in_place, s);
+    else launch_rotate<F16>(a, r, in_place, s);
+  }
   GRM_HIP_CHECK(hipGetLastError());
   grm::clear_error();
   return 0;

@@ -656,7 +656,11 @@ int grm_hip_kv_append_turned(const grm_kv_cache_desc* cache, const grm_kv_batch_
  * leaves attention to its engine; no counterpart.
  *
  * A row with a value that is not finite makes the outputs of every token that
- * sees it NaN, and no other's.  Rows that no token sees may hold anything. */
+ * sees it NaN, and no other's.  Rows that no token sees may hold anything.
+ *
+ * A call whose rows are more than one launch has room for (2^24 blocks: tokens of
+ * the plain kernels, 128 x 256 pieces of an expansion, 16 rows of a read) is
+ * refused. */
 typedef struct grm_latent_desc {
   void* rows;
   uint64_t blocks;
