@@ -22,10 +22,13 @@ int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out) {
   l.cap_units = std::min(rows, rows / l.unit_tokens + busy);
   l.cap_rows = std::min(rows, rows / kRowUnit + busy);
   // Pieces of dense rows are no shorter than a fourth of the even share (all tiles x
-  // heads / 2 blocks to a CU), and only longer units are cut.
-  const uint64_t even = 2 * static_cast<uint64_t>(cus) / b->heads + 1;
-  l.cap_items = l.cap_rows + 4 * even;
-  l.cap_parts = std::min(l.cap_items, 8 * even);
+  // heads / 2 blocks to a CU), and only longer units are cut: into two pieces or more, so
+  // that pieces are at most twice the units' tiles over that fourth.  (Items have a few
+  // more, for a share that is rounded down; parts past the end would be whole units.)
+  // With as many heads as blocks no unit is longer than the even share.
+  const uint64_t slots = 2 * static_cast<uint64_t>(cus), heads = static_cast<uint64_t>(b->heads);
+  l.cap_items = l.cap_rows + 4 * (slots / heads + 1);
+  l.cap_parts = heads < slots ? std::min(l.cap_items, 8 * slots / heads) : 0;
   l.cap_row_joins = std::min(l.cap_rows, l.cap_parts / 2);
   l.reach = static_cast<int32_t>(std::min<int64_t>(
       static_cast<int64_t>(b->table_width) * b->block_tokens, 2 * static_cast<int64_t>(kMaxLen)));
