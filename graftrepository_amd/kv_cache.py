@@ -137,12 +137,32 @@ def _strides(a) -> tuple[int, ...]:
     return tuple(reversed(out))
 
 
-def _rows(a, what: str, shape, of: str = "cache") -> tuple[int, str, int, int]:
-    """(address, type, row stride, head stride) of [rows, heads, dim] values
-    whose last axis is contiguous."""
+_forward = None  # torch's forward-mode differentiation, once torch is there
+
+
+def _no_tangent(a, what: str, of: str) -> None:
+    global _forward
+    if _forward is None:
+        _forward = sys.modules.get("torch.autograd.forward_ad")
+    if _forward is not None and _is_torch(a) and _forward.unpack_dual(a).tangent is not None:
+        raise ValueError(f"{what} has a forward-mode tangent, and the {of} has no derivative: "
+                         "pass its primal part")
+
+
+def _no_gradient(a, what: str, of: str = "cache") -> None:
+    """Values whose derivative, in either mode, a result would be without."""
     if getattr(a, "requires_grad", False) and sys.modules["torch"].is_grad_enabled():
         raise ValueError(f"{what} requires a gradient, and the {of} has no backward pass: "
                          "detach it, or call under torch.no_grad()")
+    # (outside of its levels, which are numbered from 0, no tensor has a tangent)
+    if getattr(_forward, "_current_level", 0) >= 0:
+        _no_tangent(a, what, of)
+
+
+def _rows(a, what: str, shape, of: str = "cache") -> tuple[int, str, int, int]:
+    """(address, type, row stride, head stride) of [rows, heads, dim] values
+    whose last axis is contiguous."""
+    _no_gradient(a, what, of)
     if _FLOATS and _FLOATS.get(getattr(a, "dtype", None)) and a.is_cuda and a.shape == shape:
         st = a.stride()
         if st[2] == 1:  # the usual call, on its short way

@@ -28,9 +28,9 @@ import math
 import sys
 
 from . import _lib
-from .kv_cache import (KvBatch, _call, _copied, _dense, _empty, _is_torch, _name_of, _off,
-                       _one_device, _rows, _same_device, _stream, _torch_stream, _type, i32, u64,
-                       vp)
+from .kv_cache import (KvBatch, _call, _copied, _dense, _empty, _is_torch, _name_of,
+                       _no_gradient, _off, _one_device, _rows, _same_device, _stream,
+                       _torch_stream, _type, i32, u64, vp)
 from .payload import DeviceArray
 
 
@@ -238,8 +238,7 @@ class LatentCache:
         key_dim = int(key_dim)
         if not 0 < key_dim < dim:
             raise ValueError(f"key_dim {key_dim} of {dim} rows a head")
-        if getattr(weight, "requires_grad", False):
-            _rows(weight, "weight", tuple(weight.shape))  # refused where gradients are recorded
+        _no_gradient(weight, "weight")
         wp = _dense(weight, "weight", self.dtype, (heads, dim, self.rank))
         _same_device(weight, "weight", self.device)
         at = self._ranges(block_table, starts, cu_rows, rows)
