@@ -31,12 +31,15 @@
 //   O^T = V^T P^T: those are the lane's part of the B operand; the A operand's
 //     lane has the same keys of a value column.
 //
-// Scores, statistics and sums are fp32.  Weights go to the cache's type (one
-// term: off by 2^-8 of each weight in bf16, 2^-11 in fp16, as the output's own
-// rounding; a second term would cost half of a product, and the outputs' error
-// against 64 bits is 1.2 times the plain form's without it); their sum is taken
-// before that.  fp16 weights are scaled by 2^13, so that those below 2^-27 of the
-// largest still count.
+// Scores, statistics and sums are fp32.  Weights go to the cache's type, and their sum
+// is taken before that.  With 16 columns they go in two terms, which is free there:
+// matrix cores wait for rows (32 sessions of 16000 tokens 118 us with one term, 119 with
+// two, at rank 256 54 and 54).  More columns have one term, off by 2^-8 of each weight in
+// bf16 and 2^-11 in fp16, as the output's own rounding: their outputs are up to 1.2 times
+// as far from 64 bits as the plain form's, and a second term took 124 to 128 us at 32
+// columns (410 to 450 for 65535 tokens), 136 to 155 at 64, 65 to 76 at 64 of rank 256;
+// 128 are bound by the matrix cores, of whose work it would be half as much again.  fp16
+// weights are scaled by 2^13, so that those below 2^-27 of the largest still count.
 //
 // Bound by bytes where a step has one token to a session and few heads, by the matrix
 // cores beyond about 100 columns.  Measured (a CU has one block but for 64 columns at
@@ -245,6 +248,22 @@ __device__ __forceinline__ uint32_t two_weights(float x, float y) {
   }
 }
 
+// Two weights in two terms, each as in two_weights.  A bf16 one is cut, not rounded, so that
+// what is left has no sign, which the exponents are taken down by.
+template <bool BF>
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t* first, uint32_t* rest) {
+  if constexpr (BF) {
+    const float x1 = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    const float y1 = __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+    *first = two_weights<BF>(x1, y1);
+    *rest = two_weights<BF>(x - x1, y - y1);
+  } else {
+    const f16x2 w = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    *first = __builtin_bit_cast(uint32_t, w);
+    *rest = two_weights<BF>(x - static_cast<float>(w[0]), y - static_cast<float>(w[1]));
+  }
+}
+
 template <class T, int R, int P, int G, int NW>
 struct LatentShape {
   static constexpr int kThreads = NW * kWave;
@@ -272,6 +291,7 @@ struct LatentShape {
   static constexpr int kLoads = kLatLoads + kKeyLoads;
   static constexpr int kAhead = R == 512 && NW == 8 ? 4 : 8;  // reads from LDS before their use
   static constexpr bool kBf = T::code == kBF16;
+  static constexpr bool kTwo = kCols == 16;  // weights in two terms
   // Columns may pass their reference by 2^kSlack before the sums are scaled.
   static constexpr float kSlack = kBf ? 8.0f : 2.0f;
   static constexpr float kBias = kBf ? 0.0f : 13.0f;
@@ -645,14 +665,21 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         m = m2;
       }
       const float shift = S::kBias - (m == -INFINITY ? 0.0f : m);
-      u32x4 w[S::kPer / 8];
+      u32x4 w[S::kPer / 8], rest[S::kPer / 8];
 #pragma unroll
       for (int e = 0; e < S::kPer; e += 2) {
         const float x = __builtin_amdgcn_exp2f(fmaf(score[e], scale_by, shift));
         const float y = __builtin_amdgcn_exp2f(fmaf(score[e + 1], scale_by, shift));
         l += x;
         l += y;
-        w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y);
+        if constexpr (S::kTwo) {
+          uint32_t first, other;
+          split_weights<S::kBf>(x, y, &first, &other);
+          w[e / 8][e % 8 / 2] = first;
+          rest[e / 8][e % 8 / 2] = other;
+        } else {
+          w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y);
+        }
       }
       // values
       asm volatile("" : "+v"(v_at));
@@ -668,7 +695,9 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
       in_order<S::kTilesD * (S::kPer / 8), S::kAhead>(
           [&](int i) { return value_chunk(i / (S::kPer / 8), i % (S::kPer / 8)); },
           [&](int i, u32x4 f) {
-            o[i / (S::kPer / 8)] = mfma<S::kBf>(f, w[i % (S::kPer / 8)], o[i / (S::kPer / 8)]);
+            f32x4& to = o[i / (S::kPer / 8)];
+            to = mfma<S::kBf>(f, w[i % (S::kPer / 8)], to);
+            if constexpr (S::kTwo) to = mfma<S::kBf>(f, rest[i % (S::kPer / 8)], to);
           });
       if constexpr (S::kStages == 1) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the rows are read
