@@ -32,10 +32,12 @@ def turned(x, positions, frequencies, magnitude, layout, start=0, inverse=False)
 
 
 def turned_bound(out, mass, out_type):
-    """The angle's part of a turn in fp32 is off by 2^-26 (a half step below
-    1/2), 2 pi 2^-26 = 1.6 units; its sine and cosine by 2 more; two products
-    with the magnitude (itself rounded) 2; two products and a sum 3: 9 units of
-    the sum of magnitudes.  Then one rounding to the type."""
+    """A sine or cosine is off by 2.2 units of 2^-24 at most (its quarter turn's
+    rounding, its series; tests/test_rotary_angles.py derives it and holds them to
+    it alone).  Times the magnitude, itself rounded and with `inverse` divided by:
+    3 more; two products and their sum: 2 (each value is in one product).  7.2
+    units of the sum of magnitudes; 9 leave room for far positions, whose angle
+    is rounded in fp64.  Then one rounding to the type."""
     return 9 * U32 * mass + UNIT[out_type] * (np.abs(out) + 9 * U32 * mass) + TINY[out_type]
 
 
