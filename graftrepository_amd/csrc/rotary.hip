@@ -30,6 +30,7 @@ int rotary_of(const grm_rotary_desc* d, int channels, Rotary* out) {
   const double sign = d->inverse ? -1.0 : 1.0;
   for (int i = 0; i < d->dim / 2; ++i) out->quarters[i] = 4.0 * sign * d->turns[i];
   out->magnitude = d->inverse ? 1.0f / d->magnitude : d->magnitude;
+  if (out->magnitude - out->magnitude != 0.0f) return fail(-1, "rotary: magnitude too small to divide by");
   out->dim = d->dim;
   out->layout = d->layout;
   return 0;

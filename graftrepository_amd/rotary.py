@@ -85,15 +85,18 @@ class Rotary:
             raise ValueError(f"base must be finite and above 1, got {base}")
         if not (factor > 0 and math.isfinite(factor)):
             raise ValueError(f"factor must be positive and finite, got {factor}")
-        if not (trained > 0 and 0 < slow < fast):
-            raise ValueError("trained must be positive, and 0 < slow < fast")
+        if not (0 < trained < math.inf and 0 < slow < fast < math.inf):
+            raise ValueError("trained must be positive, 0 < slow < fast, and all finite")
         if magnitude is None:
             magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "yarn" and factor > 1 else 1.0
         if not 1e-30 < magnitude < 1e30:
             raise ValueError(f"magnitude must be positive and finite, got {magnitude}")
         self.dim, self.layout, self.magnitude = dim, layout, magnitude
-        self.frequencies = _frequencies(dim, float(base), scaling, float(factor), trained, fast,
-                                        slow, factors)
+        try:
+            self.frequencies = _frequencies(dim, float(base), scaling, float(factor), trained,
+                                            fast, slow, factors)
+        except ArithmeticError as e:  # a factor of 0, a base past fp64's range
+            raise ValueError(f"no frequencies of these arguments: {e}") from None
         if not all(math.isfinite(f) and abs(f) <= 2 * math.pi for f in self.frequencies):
             raise ValueError("a frequency past one turn a position")
         self._desc = {}
