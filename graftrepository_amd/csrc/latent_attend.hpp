@@ -44,8 +44,8 @@
 // Bound by bytes where a step has one token to a session and few heads, by the matrix
 // cores beyond about 100 columns.  Measured (a CU has one block but for 64 columns at
 // rank 256): 32 sessions of 65535 tokens, 16 heads 5.9 TB/s, 40 heads at rank 256
-// 5.2; 256 sessions of 4095, 128 heads 828 TFLOP/s; a chunk of 256 tokens of 16 heads
-// on 32767 916.  Short steps are start, change of session and parts: 24 sessions of
+// 5.1; 256 sessions of 4095, 128 heads 836 TFLOP/s; a chunk of 256 tokens of 16 heads
+// on 32767 935.  Short steps are start, change of session and parts: 24 sessions of
 // 98 thousand rows in all and 128 heads take 47 us (55 in equal runs, 24 of which have
 // two units), and 19.5 for the join of 67 MB of parts, which is near a copy's rate.
 // (64 columns to a block, half the parts and twice the loads, took as long.)

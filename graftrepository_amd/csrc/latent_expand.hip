@@ -25,9 +25,9 @@ struct ExpandArgs {
 // 128 rows x 256 columns to a block, 64 x 128 to a wavefront, 32 of the rank a
 // stage; three stages of direct loads in LDS, two blocks to a CU, so that one's
 // stores run beside the other's products.  Bound by the rounds of so few steps (16 at
-// rank 512) and their ends: 4096 rows of 32 heads x 256 columns take 50 us (681
+// rank 512) and their ends: 4096 rows of 32 heads x 256 columns take 50 us (688
 // TFLOP/s), 4137 rows 57; torch's product of the same sizes without the gather, in
-// one plane, 44 and 74.  Chunks of 16 bytes are stored at c ^ (row >> 3
+// one plane, 47 and 73.  Chunks of 16 bytes are stored at c ^ (row >> 3
 // & 3) of their 64: the 16 rows that are read at once lie in all banks.  Results
 // leave through LDS, 16 bytes to a lane.
 constexpr int kExpandRows = 128, kExpandCols = 256, kExpandStep = 32, kExpandStages = 3;
@@ -232,10 +232,10 @@ __device__ inline KeyRows key_rows(const RowsArgs& a, int request) {
 // CU.  The rest is one stream of tiles: those that all columns see are asked nothing.
 //
 // Bound by the matrix cores on long rows: a prompt of 16384 tokens, 32 heads of 192 and
-// 128, 1040 TFLOP/s in bf16 (a large matrix product here has 1221); 40 heads of 96
-// and 64 in fp16 820, where a tile's vector instructions take as long as its
+// 128, 1083 TFLOP/s in bf16 (a large matrix product here has 1221); 40 heads of 96
+// and 64 in fp16 845, where a tile's vector instructions take as long as its
 // products.  Short ones by a unit's ends, about ten tiles' time each, and the
-// slots that stay empty at the end: 4096 tokens 840, 1024 tokens 320.
+// slots that stay empty at the end: 4096 tokens 899, 1024 tokens 346.
 //
 // A unit of 128 tokens is cut where there are fewer than the blocks that fit: by the
 // plan, at the share of eight for which the longest-first order ends first.
