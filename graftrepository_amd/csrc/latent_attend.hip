@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256) void latent_any_kernel(LatentArgs a) {
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
     l = l * keep + sum;
-    s_p[wave][lane] = p / latent_up<T>();
+    s_p[wave][lane] = p * a.unit.down;
     s_row[wave][lane] = s == s ? at : -1;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(256) void latent_any_kernel(LatentArgs a) {
               static_cast<int64_t>(h) * a.out_head;
   for (int d = threadIdx.x; d < a.rank; d += 256) {
     const float v = f[0] * s_o[0][d] + f[1] * s_o[1][d] + f[2] * s_o[2][d] + f[3] * s_o[3][d];
-    out[d] = T::put(total == 0.0f ? 0.0f : v / total * latent_up<T>());
+    out[d] = T::put(total == 0.0f ? 0.0f : v / total * a.unit.up);
   }
   if (a.lse && threadIdx.x == 0) {
     a.lse[static_cast<size_t>(row) * a.heads + h] =
@@ -693,6 +693,7 @@ extern "C" int grm_hip_latent_attend(const grm_latent_desc* c, const grm_kv_batc
   a.at_first = l.at_first[per - 1];
   a.at_starts = l.at_starts[per - 1];
   a.at_joins = l.at_joins[per - 1];
+  a.unit = sum_unit(c->dtype, l.reach);
   a.scale = softmax_scale;
   a.requests = b->requests;
   a.width = b->table_width;

@@ -143,6 +143,31 @@ struct LatentLayout {
 
 int latent_layout_of(const grm_kv_batch_desc* b, LatentLayout* out);
 
+// Columns may pass their reference by 2^slack before the sums are scaled (bf16 with 2 as
+// fp16 has: 24 sessions of 128 heads 69 us in place of 66.5, three prompts 175 for 170).
+__host__ __device__ constexpr int slack_of(int dtype) { return dtype == kBF16 ? 8 : 2; }
+
+// Sums of bf16 values are kept at 2^-bits of themselves: weights up to 2^slack of n rows
+// would take those of large values out of fp32's range, though their mean is in it.  No
+// more bits than that, since values below 2^(bits - 140) lose theirs at the other end.
+struct SumUnit {
+  uint32_t bits;     // of two bf16 exponents
+  float up, down;    // 2^bits, 2^-bits
+};
+inline SumUnit sum_unit(int dtype, int64_t n) {
+  SumUnit u{0u, 1.0f, 1.0f};
+  if (dtype != kBF16) return u;
+  int rows = 0;
+  while ((int64_t{1} << rows) < n) ++rows;
+  const int bits = rows + slack_of(dtype) + 1;  // (one for what the sums round up)
+  u.bits = static_cast<uint32_t>(bits) << 7 | static_cast<uint32_t>(bits) << 23;
+  for (int i = 0; i < bits; ++i) {
+    u.up *= 2.0f;
+    u.down *= 0.5f;
+  }
+  return u;
+}
+
 struct LatentArgs {
   const char* rows;
   const void* q;
@@ -155,6 +180,7 @@ struct LatentArgs {
   float* parts;
   int64_t q_token, q_head, out_token, out_head;  // strides
   uint64_t blocks, at_units, at_first, at_starts, at_joins;
+  SumUnit unit;
   float scale;
   int32_t requests, width, tokens, window, heads, rank, rope, block_log2;
   int32_t runs, joins;
@@ -226,23 +252,15 @@ __device__ __forceinline__ void in_order(Read read, Use use) {
   }
 }
 
-// Sums of bf16 values are kept at 2^-kDown of themselves: weights up to 2^8 of up to
-// 2^30 rows would take those of large values out of fp32's range, though their mean is
-// in it.
-constexpr int kDown = 40;
-template <class T>
-__host__ __device__ constexpr float latent_up() { return T::code == kBF16 ? 0x1p40f : 1.0f; }
-static_assert(kDown == 40, "the power in latent_up");
-
-// Two weights, rounded; bf16 ones then taken down by their exponents (those below
-// 2^-86 of the largest lose digits or go, which no sum of fp32 would show).
+// Two weights, rounded; bf16 ones then taken down by their exponents (those below 2^-80 of
+// the largest lose digits or go, which no sum of fp32 would show).
 template <bool BF>
-__device__ __forceinline__ uint32_t two_weights(float x, float y) {
+__device__ __forceinline__ uint32_t two_weights(float x, float y, const SumUnit& unit) {
   if constexpr (BF) {
     typedef __bf16 pair __attribute__((ext_vector_type(2)));
-    typedef unsigned short bits __attribute__((ext_vector_type(2)));
-    const auto w = __builtin_bit_cast(bits, pair{static_cast<__bf16>(x), static_cast<__bf16>(y)});
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(w, bits{kDown << 7, kDown << 7}));
+    typedef unsigned short halves __attribute__((ext_vector_type(2)));
+    const auto w = __builtin_bit_cast(halves, pair{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(w, __builtin_bit_cast(halves, unit.bits)));
   } else {
     return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
   }
@@ -251,16 +269,17 @@ __device__ __forceinline__ uint32_t two_weights(float x, float y) {
 // Two weights in two terms, each as in two_weights.  A bf16 one is cut, not rounded, so that
 // what is left has no sign, which the exponents are taken down by.
 template <bool BF>
-__device__ __forceinline__ void split_weights(float x, float y, uint32_t* first, uint32_t* rest) {
+__device__ __forceinline__ void split_weights(float x, float y, const SumUnit& unit, uint32_t* first,
+                                              uint32_t* rest) {
   if constexpr (BF) {
     const float x1 = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
     const float y1 = __uint_as_float(__float_as_uint(y) & 0xffff0000u);
-    *first = two_weights<BF>(x1, y1);
-    *rest = two_weights<BF>(x - x1, y - y1);
+    *first = two_weights<BF>(x1, y1, unit);
+    *rest = two_weights<BF>(x - x1, y - y1, unit);
   } else {
     const f16x2 w = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
     *first = __builtin_bit_cast(uint32_t, w);
-    *rest = two_weights<BF>(x - static_cast<float>(w[0]), y - static_cast<float>(w[1]));
+    *rest = two_weights<BF>(x - static_cast<float>(w[0]), y - static_cast<float>(w[1]), unit);
   }
 }
 
@@ -292,8 +311,7 @@ struct LatentShape {
   static constexpr int kAhead = R == 512 && NW == 8 ? 4 : 8;  // reads from LDS before their use
   static constexpr bool kBf = T::code == kBF16;
   static constexpr bool kTwo = kCols == 16;  // weights in two terms
-  // Columns may pass their reference by 2^kSlack before the sums are scaled.
-  static constexpr float kSlack = kBf ? 8.0f : 2.0f;
+  static constexpr float kSlack = slack_of(T::code);
   static constexpr float kBias = kBf ? 0.0f : 13.0f;
 
   // Where a row's chunks of 16 bytes go: chunk c of 256 bytes to c ^ turn(row).  A
@@ -308,12 +326,12 @@ struct LatentShape {
 
 // Four values of a finished row.
 template <class T>
-__device__ inline void latent_put(uint16_t* to, f32x4 o, float inv, bool empty) {
+__device__ inline void latent_put(uint16_t* to, f32x4 o, float inv, bool empty, float up) {
   u32x2 v;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv * latent_up<T>());
-    const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv * latent_up<T>());
+    const uint32_t lo = T::put(empty ? 0.0f : o[2 * e] * inv * up);
+    const uint32_t hi = T::put(empty ? 0.0f : o[2 * e + 1] * inv * up);
     v[e] = lo | (hi << 16);
   }
   *reinterpret_cast<u32x2*>(to) = v;
@@ -674,11 +692,11 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         l += y;
         if constexpr (S::kTwo) {
           uint32_t first, other;
-          split_weights<S::kBf>(x, y, &first, &other);
+          split_weights<S::kBf>(x, y, a.unit, &first, &other);
           w[e / 8][e % 8 / 2] = first;
           rest[e / 8][e % 8 / 2] = other;
         } else {
-          w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y);
+          w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y, a.unit);
         }
       }
       // values
@@ -726,7 +744,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
         for (int d = d_first; d < d_last; d += d_step) {
 #pragma unroll
           for (int k = 0; k < kVecs; ++k) {
-            latent_put<T>(to + kWaveCols * d + 4 * S::kH * k, value(d, k), inv, empty);
+            latent_put<T>(to + kWaveCols * d + 4 * S::kH * k, value(d, k), inv, empty, a.unit.up);
           }
         }
       } else {
@@ -800,7 +818,7 @@ __global__ __launch_bounds__(NW * kWave, latent_per_cu(R, NW) * NW / 4) void lat
 #pragma unroll
         for (int d = 0; d < S::kTilesD; ++d) {
 #pragma unroll
-          for (int k = 0; k < kVecs; ++k) latent_put<T>(to + kWaveCols * d + 4 * S::kH * k, value(d, k), inv, empty);
+          for (int k = 0; k < kVecs; ++k) latent_put<T>(to + kWaveCols * d + 4 * S::kH * k, value(d, k), inv, empty, a.unit.up);
         }
       } else if (x.mine) {
 #pragma unroll
@@ -895,7 +913,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a, float bi
   const int token = col / a.heads, h = col - token * a.heads;
   latent_put<T>(static_cast<uint16_t*>(a.out) + static_cast<int64_t>(row + token) * a.out_token +
                     static_cast<int64_t>(h) * a.out_head + d,
-                o, 1.0f / l, empty);
+                o, 1.0f / l, empty, a.unit.up);
   if (a.lse && d == 0) {
     a.lse[static_cast<size_t>(row + token) * a.heads + h] = latent_lse<T>(m, l, bias);
   }

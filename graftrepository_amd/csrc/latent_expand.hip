@@ -202,6 +202,7 @@ struct RowsArgs {
   int64_t q_token, q_head, k_row, k_head, v_row, v_head, out_token, out_head;
   float* parts;
   uint64_t at_items, at_row_joins;
+  SumUnit unit;
   float scale;
   int32_t requests, tokens, window, heads, key_dim, value_dim, rows;
 };
@@ -252,7 +253,7 @@ struct RowsShape {
   static constexpr int kLoads = kKeyLoads + kValueLoads;
   static constexpr int kSteps = DK / 16, kTilesD = DV / 32;
   static constexpr bool kBf = T::code == kBF16;
-  static constexpr float kSlack = kBf ? 8.0f : 2.0f, kBias = kBf ? 0.0f : 13.0f;
+  static constexpr float kSlack = slack_of(T::code), kBias = kBf ? 0.0f : 13.0f;
   // Where a row's chunks of 16 bytes go: chunk c to c ^ turn.  A 16-byte read is served
   // 16 lanes at a time (0-3, 12-15, 20-23, 24-27; 4-11, 16-19, 28-31; and so on), whose
   // rows are then in all 64 banks.
@@ -428,7 +429,7 @@ __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const 
                 const float y = __builtin_amdgcn_exp2f(fmaf(now[e + 1], scale_by, shift));
                 l += x;
                 l += y;
-                w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y);
+                w[e / 8][e % 8 / 2] = two_weights<S::kBf>(x, y, a.unit);
               }
             } else {
               const int d = k - kEarly;
@@ -643,7 +644,7 @@ __device__ __forceinline__ bool attend_piece(const RowsArgs& a, int head, const 
       f32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = o[d][4 * k + e];
-      latent_put<T>(to + 32 * d + 8 * k, v, inv, empty);
+      latent_put<T>(to + 32 * d + 8 * k, v, inv, empty, a.unit.up);
     }
   }
   if (a.lse && h == 0) {
@@ -721,7 +722,7 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a, float bias) 
     }
     const bool empty = m == -INFINITY && l == 0.0f;
     latent_put<T>(a.out + static_cast<int64_t>(j->row + token) * a.out_token + head * a.out_head + x, o,
-                  1.0f / l, empty);
+                  1.0f / l, empty, a.unit.up);
     if (a.lse && x == 0) {
       a.lse[static_cast<int64_t>(j->row + token) * a.heads + head] = latent_lse<T>(m, l, bias);
     }
@@ -776,7 +777,7 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowsArgs a) {
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
     l = l * keep + sum;
-    s_p[wave][lane] = p / latent_up<T>();
+    s_p[wave][lane] = p * a.unit.down;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] *= keep;
@@ -811,7 +812,7 @@ __global__ __launch_bounds__(256) void rows_any_kernel(RowsArgs a) {
   uint16_t* out = a.out + static_cast<int64_t>(row) * a.out_token + head * a.out_head;
   for (int d = threadIdx.x; d < a.value_dim; d += 256) {
     const float x = f[0] * s_o[0][d] + f[1] * s_o[1][d] + f[2] * s_o[2][d] + f[3] * s_o[3][d];
-    out[d] = T::put(total == 0.0f ? 0.0f : x / total * latent_up<T>());
+    out[d] = T::put(total == 0.0f ? 0.0f : x / total * a.unit.up);
   }
   if (a.lse && threadIdx.x == 0) {
     a.lse[static_cast<int64_t>(row) * a.heads + head] =
@@ -974,6 +975,7 @@ extern "C" int grm_hip_rows_attend(const grm_kv_batch_desc* b, const void* work,
   a.parts = static_cast<float*>(scratch);
   a.at_items = l.at_items;
   a.at_row_joins = l.at_row_joins;
+  a.unit = sum_unit(dtype, static_cast<int64_t>(rows));
   a.scale = softmax_scale;
   a.requests = b->requests;
   a.tokens = b->tokens;

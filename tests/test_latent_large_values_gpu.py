@@ -57,3 +57,54 @@ def test_a_maximum_that_lags_behind(hip_lib, dk, dv):
     s.v = large(np.random.default_rng(2), tuple(s.v.shape))
     s.scale = 1.6 * np.log(2.0)
     s.check(*s.run(softmax_scale=s.scale))
+
+
+def sized(rng, shape):
+    """Values of both signs in [1/8, 15/8], bf16."""
+    return dev(rng.choice([-1.0, 1.0], shape) * rng.integers(16, 240, shape) / 128, torch.bfloat16)
+
+
+def same_multiple(got, power, rows):
+    """The second results are 2^power times the first.  Sums stand at 2^-bits of
+    themselves, bits = ceil(log2 rows) + 9 (rows that the call could see).  Where terms
+    of theirs are below 2^-126, each of 2 rows products and additions is off by half of
+    fp32's least step, 2^-150: by rows 2^(bits - 149) in an output, whose sum of weights
+    is 1 or more, before it is rounded.  Two numbers so far from one another round to
+    such as are a step of bf16 further apart at most (2^-7 of them)."""
+    (out, lse), (out2, lse2) = got
+    assert torch.equal(lse, lse2)
+    want, off = out.double() * 2.0 ** power, (out2.double() - out.double() * 2.0 ** power).abs()
+    if power < -60:
+        bits = int(np.ceil(np.log2(rows))) + 9
+        assert (off <= 2.0 ** -7 * want.abs() + 2 * rows * 2.0 ** (bits - 149)).all()
+        assert (off > 0).double().mean() < 1e-3
+    else:
+        assert (off == 0).all()
+
+
+@pytest.mark.parametrize("power", [-100, -60, 60, 126])
+@pytest.mark.parametrize("ctx,new", [([300, 0], [1, 1]), ([4000], [3]), ([70], [200])])
+@pytest.mark.parametrize("rank,rope,heads", [(512, 64, 16), (512, 64, 128), (256, 32, 40), (64, 16, 4)])
+def test_latents_times_a_power_of_two(hip_lib, rank, rope, heads, ctx, new, power):
+    # (the scores are the key parts')
+    s = Setup(ctx, new, rank, rope, 16, heads)
+    s.rows.nan_to_num_(0.0)
+    s.q[..., :rank] = 0
+    s.rows[..., :rank] = sized(s.rng, tuple(s.rows.shape[:2]) + (rank,))
+    batch, got = s.batch(), []
+    for p in (0, power):
+        s.rows[..., :rank] *= 2.0 ** p
+        got.append(LatentCache(s.rows, rank).attend(batch, s.q, s.scale, return_lse=True))
+    same_multiple(got, power, s.table.shape[1] * 16)
+
+
+@pytest.mark.parametrize("power", [-100, -60, 60, 126])
+@pytest.mark.parametrize("ctx,new", [([300, 0], [1, 1]), ([4000], [3]), ([100], [200])])
+@pytest.mark.parametrize("dk,dv", [(192, 128), (96, 64), (128, 128), (24, 40)])
+def test_values_times_a_power_of_two(hip_lib, dk, dv, ctx, new, power):
+    s, got = Rows(ctx, new, dk, dv, 2), []
+    s.v = sized(np.random.default_rng(1), tuple(s.v.shape))
+    for p in (0, power):
+        s.v = s.v * 2.0 ** p
+        got.append(s.run())
+    same_multiple(got, power, s.k.shape[0])
